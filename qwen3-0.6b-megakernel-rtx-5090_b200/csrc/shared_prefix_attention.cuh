@@ -1,0 +1,311 @@
+// Attention of one new token per sequence over cache rows that all sequences share (a prefix) and rows of their own.
+//
+// out = softmax(scale * q . k) v over the prefix rows and the sequence's own ones.  The prefix is the same for all sequences, so
+// its scores are matrix products: the queries of all sequences that read a kv head are the rows of one operand, the
+// prefix rows cross HBM once for all of them instead of once for each.  A softmax over a split range is joined from partial
+// states - the maximum M, the sum L of 2^(s - M) and the unnormalised output A of each part, all fp32 - as sum(2^(M_i - M) A_i) /
+// sum(2^(M_i - M) L_i), so the prefix may be split over many CTAs and the own rows handled by others.  A part without visible rows
+// has M = -inf and L = 0 and weighs nothing.
+//
+// An item is a block of query rows against a range of cache rows of one kv head: (row tile, kv head, prefix range) or (sequence, kv
+// head, range of own rows).
+#ifndef QMK_SHARED_PREFIX_ATTENTION_CUH_
+#define QMK_SHARED_PREFIX_ATTENTION_CUH_
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace qmk_spa {
+
+constexpr int MAX_SEQS = 128;
+constexpr int MAX_GROUP = 16;                    // query heads per kv head: one m16 tile of a sequence's own rows
+constexpr int THREADS = 128, WARPS = 4;
+constexpr int KEYS = 64;                         // cache rows per tile
+constexpr int STAGES = 3;
+constexpr int OWN_RANGE = 256;                   // own rows per item
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+struct Params {
+  const void *q;
+  long long q_seq, q_head;                       // strides, in elements
+  int seqs, group, q_heads, kv_heads;
+  const void *k_prefix, *v_prefix;
+  long long prefix_row, prefix_head;
+  int prefix_len, prefix_parts, prefix_range, row_tiles;   // range: prefix rows per item, a multiple of KEYS
+  long long own_row, own_head;
+  int own_rows, own_parts;
+  const int *own_lens;
+  int own_bias;                                  // added to own_lens
+  float scale_log2;                              // scale * log2 e
+  float *part_out;                               // [part][seq][q_head][dim]
+  float2 *part_ml;                               // [part][seq][q_head]
+  void *out;
+  float *lse;
+  const void *k_own[MAX_SEQS], *v_own[MAX_SEQS];
+};
+
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ uint32_t s32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// 16 bytes to shared memory; zeros where there is no row
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+template <typename T> struct Half;
+template <> struct Half<__half> {
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  }
+  static __device__ __forceinline__ __half from(float a) { return __float2half_rn(a); }
+  // Weights are at most 2^P_SHIFT: rounding 2^-11 of the value down to 2^-14, and so for weights of 2^-26 of the row's largest on.
+  static constexpr float P_SHIFT = 12.0f;
+};
+template <> struct Half<__nv_bfloat16> {
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  }
+  static __device__ __forceinline__ __nv_bfloat16 from(float a) { return __float2bfloat16_rn(a); }
+  static constexpr float P_SHIFT = 0.0f;
+};
+
+// mma.sync tiles: MT warps side by side own 16 query rows each, the 4 / MT groups of warps take the tile's cache rows in turn; every
+// warp has a running maximum, sum and output of its own.
+template <typename T, int D, int MT>
+__device__ __forceinline__ void item_mma(const Params &p, unsigned char *smem, int part, int kv_head, int row0, int live_rows,
+                                         const T *kp, const T *vp, long long row_stride, int nrows) {
+  constexpr int KG = WARPS / MT, WK = KEYS / KG;           // groups of warps over the cache rows, rows a group takes of a tile
+  constexpr int CHUNKS = D / 8, ROW_BYTES = D * 2, TILE = KEYS * ROW_BYTES;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, mt = warp % MT, kg = warp / MT;
+  const int quad = lane & 3, rq = lane >> 2;
+  const uint32_t base = s32(smem);
+  // query fragments straight from global memory: row r of the tile is head r % group of sequence r / group (own rows: one sequence)
+  uint32_t qa[D / 16][4];
+  {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int r = row0 + mt * 16 + rq + 8 * half;
+      const bool live = mt * 16 + rq + 8 * half < live_rows;
+      const int b = r / p.group, h = kv_head * p.group + r % p.group;
+      const T *src = static_cast<const T *>(p.q) + (live ? b * p.q_seq + h * p.q_head : 0);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        qa[ks][half] = live ? *reinterpret_cast<const uint32_t *>(src + ks * 16 + quad * 2) : 0u;
+        qa[ks][2 + half] = live ? *reinterpret_cast<const uint32_t *>(src + ks * 16 + 8 + quad * 2) : 0u;
+      }
+    }
+  }
+  float acc[D / 8][4];
+#pragma unroll
+  for (int t = 0; t < D / 8; ++t) { acc[t][0] = 0.f; acc[t][1] = 0.f; acc[t][2] = 0.f; acc[t][3] = 0.f; }
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  const int tiles = (nrows + KEYS - 1) / KEYS;
+  auto load = [&](int t) {
+    if (t < tiles) {
+      const uint32_t dst = base + (t % STAGES) * 2 * TILE;
+#pragma unroll
+      for (int i = tid; i < KEYS * CHUNKS; i += THREADS) {
+        const int r = i / CHUNKS, c = i % CHUNKS, row = t * KEYS + r;
+        const bool there = row < nrows;
+        const long long off = (there ? row : 0) * row_stride + c * 8;
+        const uint32_t at = r * ROW_BYTES + ((c ^ (r & 7)) << 4);
+        copy16(dst + at, kp + off, there);
+        copy16(dst + TILE + at, vp + off, there);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int t = 0; t < STAGES - 1; ++t) load(t);
+  for (int t = 0; t < tiles; ++t) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    __syncthreads();                                       // tile t is there, tile t - 1 has been read
+    load(t + STAGES - 1);
+    const uint32_t kt = base + (t % STAGES) * 2 * TILE, vt = kt + TILE;
+    float sc[WK / 8][4];
+#pragma unroll
+    for (int n = 0; n < WK / 8; ++n) { sc[n][0] = 0.f; sc[n][1] = 0.f; sc[n][2] = 0.f; sc[n][3] = 0.f; }
+#pragma unroll
+    for (int n = 0; n < WK / 16; ++n) {
+      const int r = kg * WK + n * 16 + (lane & 7) + (lane >> 4) * 8;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        uint32_t b[4];
+        ldsm4(kt + r * ROW_BYTES + (((2 * ks + ((lane >> 3) & 1)) ^ (r & 7)) << 4), b);
+        Half<T>::mma(sc[2 * n], qa[ks], b[0], b[1]);
+        Half<T>::mma(sc[2 * n + 1], qa[ks], b[2], b[3]);
+      }
+    }
+    const int key0 = t * KEYS + kg * WK;
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < WK / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float v = key0 + n * 8 + quad * 2 + (i & 1) < nrows ? sc[n][i] * p.scale_log2 : -INFINITY;
+        sc[n][i] = v;
+        mx[i >> 1] = fmaxf(mx[i >> 1], v);
+      }
+    float sub[2], corr[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+      const float mn = fmaxf(m[h], mx[h]);
+      sub[h] = mn == -INFINITY ? 0.f : mn;                 // nothing seen yet: 2^(-inf - 0) = 0, not NaN
+      corr[h] = exp2f(m[h] - sub[h]);
+      m[h] = mn;
+      sub[h] -= Half<T>::P_SHIFT;
+      l[h] *= corr[h];
+    }
+#pragma unroll
+    for (int n = 0; n < WK / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sc[n][i] = exp2f(sc[n][i] - sub[i >> 1]);
+        l[i >> 1] += sc[n][i];
+      }
+#pragma unroll
+    for (int t2 = 0; t2 < D / 8; ++t2) { acc[t2][0] *= corr[0]; acc[t2][1] *= corr[0]; acc[t2][2] *= corr[1]; acc[t2][3] *= corr[1]; }
+#pragma unroll
+    for (int n = 0; n < WK / 16; ++n) {
+      const uint32_t pa[4] = {Half<T>::pack(sc[2 * n][0], sc[2 * n][1]), Half<T>::pack(sc[2 * n][2], sc[2 * n][3]),
+                              Half<T>::pack(sc[2 * n + 1][0], sc[2 * n + 1][1]), Half<T>::pack(sc[2 * n + 1][2], sc[2 * n + 1][3])};
+      const int r = kg * WK + n * 16 + (lane & 15);
+#pragma unroll
+      for (int dp = 0; dp < D / 16; ++dp) {
+        uint32_t b[4];
+        ldsm4_trans(vt + r * ROW_BYTES + (((2 * dp + (lane >> 4)) ^ (r & 7)) << 4), b);
+        Half<T>::mma(acc[2 * dp], pa, b[0], b[1]);
+        Half<T>::mma(acc[2 * dp + 1], pa, b[2], b[3]);
+      }
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+  }
+  __syncthreads();                                         // the ring is free: the groups' states are joined in it
+  constexpr int PITCH = D + 4;                             // floats between rows
+  float *const so = reinterpret_cast<float *>(smem);       // [KG][MT * 16][PITCH]
+  float2 *const sml = reinterpret_cast<float2 *>(so + KG * MT * 16 * PITCH);
+  {
+    float *const mine = so + (kg * MT + mt) * 16 * PITCH;
+#pragma unroll
+    for (int t = 0; t < D / 8; ++t) {
+      *reinterpret_cast<float2 *>(mine + rq * PITCH + t * 8 + quad * 2) = make_float2(acc[t][0], acc[t][1]);
+      *reinterpret_cast<float2 *>(mine + (rq + 8) * PITCH + t * 8 + quad * 2) = make_float2(acc[t][2], acc[t][3]);
+    }
+    if (quad == 0) {
+      sml[(kg * MT + mt) * 16 + rq] = make_float2(m[0], l[0]);
+      sml[(kg * MT + mt) * 16 + rq + 8] = make_float2(m[1], l[1]);
+    }
+  }
+  __syncthreads();
+  const size_t rows_all = static_cast<size_t>(p.seqs) * p.q_heads;
+  for (int i = tid; i < MT * 16 * (D / 4); i += THREADS) {
+    const int r = i / (D / 4), c = i % (D / 4) * 4;
+    if (r >= live_rows) continue;
+    float M = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < KG; ++g) M = fmaxf(M, sml[g * MT * 16 + r].x);
+    float L = 0.f;
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int g = 0; g < KG; ++g) {
+      const float2 ml = sml[g * MT * 16 + r];
+      const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
+      const float4 a = *reinterpret_cast<const float4 *>(so + (g * MT * 16 + r) * PITCH + c);
+      L += ml.y * f;
+      A.x += a.x * f; A.y += a.y * f; A.z += a.z * f; A.w += a.w * f;
+    }
+    const int b = (row0 + r) / p.group, h = kv_head * p.group + (row0 + r) % p.group;
+    const size_t at = part * rows_all + static_cast<size_t>(b) * p.q_heads + h;
+    *reinterpret_cast<float4 *>(p.part_out + at * D + c) = A;
+    if (c == 0) p.part_ml[at] = make_float2(M, L);
+  }
+}
+
+// Prefix items first: they are the longest.
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(THREADS) attend_parts(const __grid_constant__ Params p) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  pdl_wait();
+  pdl_trigger();
+  const int prefix_items = p.prefix_parts * p.row_tiles * p.kv_heads;
+  int id = static_cast<int>(blockIdx.x);
+  if (id < prefix_items) {
+    const int kv = id % p.kv_heads, tile = id / p.kv_heads % p.row_tiles, part = id / (p.kv_heads * p.row_tiles);
+    const int first = part * p.prefix_range, n = min(p.prefix_range, p.prefix_len - first);
+    const int row0 = tile * MT * 16, live = min(MT * 16, p.seqs * p.group - row0);
+    const size_t off = static_cast<size_t>(kv) * p.prefix_head + static_cast<size_t>(first) * p.prefix_row;
+    item_mma<T, D, MT>(p, smem, part, kv, row0, live, static_cast<const T *>(p.k_prefix) + off, static_cast<const T *>(p.v_prefix) + off,
+                       p.prefix_row, n);
+    return;
+  }
+  id -= prefix_items;
+  const int kv = id % p.kv_heads, b = id / p.kv_heads % p.seqs, own = id / (p.kv_heads * p.seqs);
+  const int len = min(max(p.own_lens[b] + p.own_bias, 0), p.own_rows), first = own * OWN_RANGE, n = min(OWN_RANGE, len - first);
+  const int part = p.prefix_parts + own;
+  if (n <= 0) {                                            // no rows: a state that weighs nothing
+    if (threadIdx.x < p.group)
+      p.part_ml[(static_cast<size_t>(part) * p.seqs + b) * p.q_heads + kv * p.group + threadIdx.x] = make_float2(-INFINITY, 0.f);
+    return;
+  }
+  const size_t off = static_cast<size_t>(kv) * p.own_head + static_cast<size_t>(first) * p.own_row;
+  item_mma<T, D, 1>(p, smem, part, kv, b * p.group, p.group, static_cast<const T *>(p.k_own[b]) + off, static_cast<const T *>(p.v_own[b]) + off,
+                    p.own_row, n);
+}
+
+// A warp joins the parts of a (sequence, query head).
+template <typename T, int D>
+__global__ void __launch_bounds__(128) join_parts(const __grid_constant__ Params p) {
+  pdl_wait();
+  pdl_trigger();
+  const int rows = p.seqs * p.q_heads, row = static_cast<int>(blockIdx.x) * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const int parts = p.prefix_parts + p.own_parts;
+  float M = -INFINITY;
+  for (int i = lane; i < parts; i += 32) M = fmaxf(M, p.part_ml[static_cast<size_t>(i) * rows + row].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  float L = 0.f, A[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) A[i] = 0.f;
+  for (int i = 0; i < parts; ++i) {
+    const float2 ml = p.part_ml[static_cast<size_t>(i) * rows + row];
+    if (ml.x == -INFINITY && ml.y == 0.f) continue;        // (nothing may have been written to its output)
+    const float f = exp2f(ml.x - M);
+    L += ml.y * f;
+    const float *src = p.part_out + (static_cast<size_t>(i) * rows + row) * D + lane * (D / 32);
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) A[k] += src[k] * f;
+  }
+  const float inv = L == 0.f ? 0.f : 1.0f / L;
+  T *dst = static_cast<T *>(p.out) + static_cast<size_t>(row) * D + lane * (D / 32);
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) dst[k] = Half<T>::from(A[k] * inv);
+  if (p.lse && lane == 0) p.lse[row] = L == 0.f ? -INFINITY : (M - Half<T>::P_SHIFT) * LN2 + logf(L);
+}
+
+}  // namespace qmk_spa
+#endif  // QMK_SHARED_PREFIX_ATTENTION_CUH_

@@ -1,0 +1,127 @@
+// C entry of the attention over a shared prefix (shared_prefix_attention.cuh).
+#include "../../include/qwen_megakernel.h"
+
+#include <algorithm>
+#include <mutex>
+#include <string>
+
+#include "engine_internal.h"
+#include "prefill_sm100.h"
+#include "shared_prefix_attention.cuh"
+
+namespace {
+
+using namespace qmk_spa;
+
+int refuse(const std::string &why) {
+  qmk_internal::note_error("qmk_attention_shared_prefix: " + why);
+  return QMK_ERR_BAD_ARGUMENT;
+}
+
+struct Split {
+  int row_warps, row_tiles, prefix_parts, prefix_range, own_parts;
+};
+Split split_of(int seqs, int q_heads, int kv_heads, int prefix_len, int own_rows) {
+  Split s;
+  const int rows = seqs * (q_heads / kv_heads);
+  s.row_warps = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  s.row_tiles = (rows + 16 * s.row_warps - 1) / (16 * s.row_warps);
+  const int items = s.row_tiles * kv_heads, tiles = (prefix_len + KEYS - 1) / KEYS;
+  int parts = std::max(1, 2 * 148 / items);
+  s.prefix_range = std::max(2, (tiles + parts - 1) / parts) * KEYS;
+  s.prefix_parts = (prefix_len + s.prefix_range - 1) / s.prefix_range;
+  s.own_parts = (own_rows + OWN_RANGE - 1) / OWN_RANGE;
+  return s;
+}
+long long workspace_bytes(const Split &s, int seqs, int q_heads, int head_dim) {
+  return static_cast<long long>(s.prefix_parts + s.own_parts) * seqs * q_heads * (head_dim * 4ll + 8);
+}
+
+template <typename T, int D>
+cudaError_t launch(const Params &p, const Split &s, cudaStream_t stream) {
+  constexpr int smem = STAGES * 2 * KEYS * D * 2;
+  static_assert(smem >= WARPS * 16 * (D + 4) * 4 + WARPS * 16 * 8, "the groups' states fit the ring");
+  void (*kernel)(Params) = s.row_warps == 1 ? attend_parts<T, D, 1> : s.row_warps == 2 ? attend_parts<T, D, 2> : attend_parts<T, D, 4>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  const int items = s.prefix_parts * s.row_tiles * p.kv_heads + s.own_parts * p.kv_heads * p.seqs;
+  if (items > 0) {
+    e = qmk_tc::launch_kernel(kernel, dim3(items), dim3(THREADS), smem, stream, p);
+    if (e != cudaSuccess) return e;
+  }
+  return qmk_tc::launch_kernel(join_parts<T, D>, dim3((p.seqs * p.q_heads + 3) / 4), dim3(128), 0, stream, p);
+}
+
+}  // namespace
+
+extern "C" long long qmk_attention_shared_prefix_workspace(int num_sequences, int q_heads, int kv_heads, int head_dim, int prefix_len,
+                                                           int own_rows) {
+  if (num_sequences < 1 || num_sequences > MAX_SEQS || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || prefix_len < 0 || own_rows < 0)
+    return 0;
+  return workspace_bytes(split_of(num_sequences, q_heads, kv_heads, prefix_len, own_rows), num_sequences, q_heads, head_dim);
+}
+
+extern "C" int qmk_attention_shared_prefix(const qmk_shared_prefix_args *a, cudaStream_t stream) {
+  qmk_internal::begin_call();
+  if (!a) return refuse("null pointer argument");
+  if (a->num_sequences < 1 || a->num_sequences > MAX_SEQS) return refuse("num_sequences must be in [1, 128]");
+  if (a->type < 0 || a->type > 1) return refuse("the type is fp16 (0) or bf16 (1)");
+  if (a->head_dim != 64 && a->head_dim != 128) return refuse("head_dim must be 64 or 128");
+  if (a->kv_heads < 1 || a->q_heads < 1 || a->q_heads % a->kv_heads || a->q_heads / a->kv_heads > MAX_GROUP || a->q_heads > 1024)
+    return refuse("q_heads must be 1 to 16 times kv_heads, and at most 1024");
+  if (a->prefix_len < 0 || a->own_rows < 0) return refuse("negative length");
+  if (!a->q || !a->out || (a->prefix_len > 0 && (!a->k_prefix || !a->v_prefix)) || (a->own_rows > 0 && (!a->k_own || !a->v_own || !a->own_lens)))
+    return refuse("null pointer argument");
+  if (!(a->scale > -3.0e38f && a->scale < 3.0e38f)) return refuse("the scale must be finite");
+  auto aligned = [](const void *ptr) { return (reinterpret_cast<unsigned long long>(ptr) & 15u) == 0; };
+  bool ok = aligned(a->q) && aligned(a->k_prefix) && aligned(a->v_prefix) && aligned(a->out) && aligned(a->workspace);
+  for (int b = 0; a->own_rows > 0 && b < a->num_sequences; ++b) {
+    if (!a->k_own[b] || !a->v_own[b]) return refuse("null pointer argument");
+    ok = ok && aligned(a->k_own[b]) && aligned(a->v_own[b]);
+  }
+  if (!ok) return refuse("pointers must be 16-byte aligned");
+  if (a->q_seq_stride % 8 || a->q_head_stride % 8 || a->prefix_row_stride % 8 || a->prefix_head_stride % 8 || a->own_row_stride % 8 || a->own_head_stride % 8)
+    return refuse("strides must be multiples of 8 elements");
+  const Split s = split_of(a->num_sequences, a->q_heads, a->kv_heads, a->prefix_len, a->own_rows);
+  if (!a->workspace || a->workspace_bytes < workspace_bytes(s, a->num_sequences, a->q_heads, a->head_dim)) return refuse("workspace too small");
+  Params p;
+  p.q = a->q;
+  p.q_seq = a->q_seq_stride;
+  p.q_head = a->q_head_stride;
+  p.seqs = a->num_sequences;
+  p.group = a->q_heads / a->kv_heads;
+  p.q_heads = a->q_heads;
+  p.kv_heads = a->kv_heads;
+  p.k_prefix = a->k_prefix;
+  p.v_prefix = a->v_prefix;
+  p.prefix_row = a->prefix_row_stride;
+  p.prefix_head = a->prefix_head_stride;
+  p.prefix_len = a->prefix_len;
+  p.prefix_parts = s.prefix_parts;
+  p.prefix_range = s.prefix_range;
+  p.row_tiles = s.row_tiles;
+  p.own_row = a->own_row_stride;
+  p.own_head = a->own_head_stride;
+  p.own_rows = a->own_rows;
+  p.own_parts = s.own_parts;
+  p.own_lens = a->own_lens;
+  p.own_bias = a->own_lens_add;
+  p.scale_log2 = a->scale * LOG2E;
+  const long long states = static_cast<long long>(s.prefix_parts + s.own_parts) * p.seqs * p.q_heads;
+  p.part_out = static_cast<float *>(a->workspace);
+  p.part_ml = reinterpret_cast<float2 *>(p.part_out + states * a->head_dim);
+  p.out = a->out;
+  p.lse = a->lse;
+  for (int b = 0; a->own_rows > 0 && b < p.seqs; ++b) {
+    p.k_own[b] = a->k_own[b];
+    p.v_own[b] = a->v_own[b];
+  }
+  const cudaError_t e = a->type == 0 ? (a->head_dim == 64 ? launch<__half, 64>(p, s, stream) : launch<__half, 128>(p, s, stream))
+                                     : (a->head_dim == 64 ? launch<__nv_bfloat16, 64>(p, s, stream) : launch<__nv_bfloat16, 128>(p, s, stream));
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    qmk_internal::note_error(std::string("qmk_attention_shared_prefix: ") + cudaGetErrorString(e));
+    return QMK_ERR_CUDA;
+  }
+  return QMK_OK;
+}

@@ -90,6 +90,24 @@ _lib.qmk_gemm_f16_tn.argtypes = [_P, _P, _P, _I, _I, _I, _P]
 _lib.qmk_gemm_f16_tn.restype = _I
 _lib.qmk_gemm_packed_tn.argtypes = [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]
 _lib.qmk_gemm_packed_tn.restype = _I
+_LL = ctypes.c_longlong
+_lib.qmk_sample_tokens.argtypes = [_P, _I, _LL, _I, _I, _P, _P, _F, _P, _I, _P, _F, _P, _F, _P, _P, _P]
+_lib.qmk_sample_tokens.restype = _I
+
+
+class _SharedPrefixArgs(ctypes.Structure):
+    _fields_ = [("type", _I), ("num_sequences", _I), ("q_heads", _I), ("kv_heads", _I), ("head_dim", _I),
+                ("q", _P), ("q_seq_stride", _LL), ("q_head_stride", _LL),
+                ("k_prefix", _P), ("v_prefix", _P), ("prefix_len", _I), ("prefix_row_stride", _LL), ("prefix_head_stride", _LL),
+                ("k_own", _P), ("v_own", _P), ("own_rows", _I), ("own_row_stride", _LL), ("own_head_stride", _LL),
+                ("own_lens", _P), ("own_lens_add", _I), ("scale", _F), ("out", _P), ("lse", _P), ("workspace", _P),
+                ("workspace_bytes", _LL)]
+
+
+_lib.qmk_attention_shared_prefix.argtypes = [ctypes.POINTER(_SharedPrefixArgs), _P]
+_lib.qmk_attention_shared_prefix.restype = _I
+_lib.qmk_attention_shared_prefix_workspace.argtypes = [_I] * 6
+_lib.qmk_attention_shared_prefix_workspace.restype = _LL
 
 
 class _EngineConfig(ctypes.Structure):
@@ -129,7 +147,7 @@ _lib.qmk_selftest_gemm_pair_wait_timeout.restype = _I
 EXPORTED_SYMBOLS = (
     "launch_ldg_decode_direct", "launch_ldg_decode_persistent", "launch_ldg_generate_nosync",
     "launch_ldg_prefill", "qmk_abi_version", "qmk_configure", "qmk_set_inv_freq", "qmk_set_logits_dump",
-    "qmk_set_weight_format", "qmk_set_tuning", "qmk_set_tuning2", "qmk_set_profile_buffer", "qmk_set_fused", "qmk_set_step_overlap", "qmk_set_prefill_attention", "qmk_set_decode_attention", "qmk_invalidate_weights", "qmk_release_weights", "qmk_decode", "qmk_generate", "qmk_generate_static", "qmk_generate_batch", "qmk_gemm_f16_tn", "qmk_gemm_packed_tn", "qmk_decode_batched", "qmk_prefill_chunked", "qmk_prefill_packed", "qmk_prefill_packed_passes", "qmk_prefill", "qmk_engine_create", "qmk_engine_destroy", "qmk_engine_apply", "qmk_engine_decode", "qmk_engine_generate", "qmk_engine_prefill", "qmk_sync_status", "qmk_last_error", "qmk_num_ctas",
+    "qmk_set_weight_format", "qmk_set_tuning", "qmk_set_tuning2", "qmk_set_profile_buffer", "qmk_set_fused", "qmk_set_step_overlap", "qmk_set_prefill_attention", "qmk_set_decode_attention", "qmk_invalidate_weights", "qmk_release_weights", "qmk_decode", "qmk_generate", "qmk_generate_static", "qmk_generate_batch", "qmk_gemm_f16_tn", "qmk_gemm_packed_tn", "qmk_sample_tokens", "qmk_attention_shared_prefix", "qmk_attention_shared_prefix_workspace", "qmk_decode_batched", "qmk_prefill_chunked", "qmk_prefill_packed", "qmk_prefill_packed_passes", "qmk_prefill", "qmk_engine_create", "qmk_engine_destroy", "qmk_engine_apply", "qmk_engine_decode", "qmk_engine_generate", "qmk_engine_prefill", "qmk_sync_status", "qmk_last_error", "qmk_num_ctas",
     "qmk_scratch_bytes", "qmk_selftest_decode_ring", "qmk_selftest_wait_timeout", "qmk_selftest_gemm_wait_timeout", "qmk_selftest_attention_wait_timeout", "qmk_selftest_gemm_pair_wait_timeout", "qmk_selftest_decode_attention_wait_timeout",
 )
 
@@ -607,6 +625,105 @@ def gemm_packed_tn(a: torch.Tensor, b: torch.Tensor, weight_format, b2: torch.Te
     if rc != 0:
         raise RuntimeError(f"gemm_packed_tn failed with status {rc}")
     return out
+
+
+_LOGIT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _per_row(value, dtype, rows, device, name):
+    """(device pointer or 0, scalar) of an option that is a number or a CUDA tensor with a value per row."""
+    if isinstance(value, torch.Tensor):
+        _check(value.dtype == dtype and value.device == device and value.dim() == 1 and value.shape[0] == rows and value.is_contiguous(),
+               f"sample_tokens: {name} must be a number or a contiguous {dtype} tensor with one value per row on the logits' device")
+        return value.data_ptr(), 0
+    return 0, value
+
+
+def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One token per row of ``logits [rows, vocab]`` (CUDA, fp32 / fp16 / bf16, contiguous along the vocabulary), picked with the number
+    of [0, 1) that ``uniforms [rows]`` (fp32) gives for the row: ``(tokens int32 [rows], logprobs fp32 [rows])``.  ``temperature`` (0: the
+    largest value), ``top_k`` (0: off), ``top_p`` (1: off) and ``min_p`` (0: off) are numbers, or tensors with a value per row (fp32,
+    ``top_k`` int32).  The definition, ties and empty rows included: ``qmk_sample_tokens`` in include/qwen_megakernel.h.  Runs on the
+    current stream of the logits' device, does not synchronise, may be captured in a graph."""
+    _require_cuda()
+    code = _LOGIT_TYPES.get(logits.dtype)
+    _check(code is not None and logits.is_cuda and logits.dim() == 2 and (logits.shape[1] < 2 or logits.stride(1) == 1),
+           "sample_tokens: logits must be a CUDA matrix [rows, vocab] of fp32, fp16 or bf16, contiguous along the vocabulary")
+    rows, vocab = logits.shape
+    device = logits.device
+    _check(uniforms.dtype == torch.float32 and uniforms.device == device and uniforms.dim() == 1 and uniforms.shape[0] == rows
+           and uniforms.is_contiguous(), "sample_tokens: uniforms must be a contiguous fp32 tensor with one value per row on the logits' device")
+    t_ptr, t = _per_row(temperature, torch.float32, rows, device, "temperature")
+    k_ptr, k = _per_row(top_k, torch.int32, rows, device, "top_k")
+    p_ptr, p = _per_row(top_p, torch.float32, rows, device, "top_p")
+    m_ptr, m = _per_row(min_p, torch.float32, rows, device, "min_p")
+    with torch.cuda.device(device):
+        tokens = torch.empty(rows, dtype=torch.int32, device=device)
+        logprobs = torch.empty(rows, dtype=torch.float32, device=device)
+        rc = _lib.qmk_sample_tokens(logits.data_ptr(), code, logits.stride(0), rows, vocab, uniforms.data_ptr(), t_ptr, float(t), k_ptr, int(k),
+                                    p_ptr, float(p), m_ptr, float(m), tokens.data_ptr(), logprobs.data_ptr(), _stream())
+    if rc != 0:
+        raise RuntimeError(f"sample_tokens: {_lib.qmk_last_error().decode()} (status {rc})")
+    return tokens, logprobs
+
+
+MAX_SHARED_PREFIX_SEQUENCES = 128
+
+
+def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k_own, v_own, own_lens: torch.Tensor,
+                            scale: float = None):
+    """Attention of one new token per sequence over rows that all share and rows of their own: ``(out, lse)``.
+
+    ``q [n, q_heads, dim]``; ``k_prefix`` / ``v_prefix [kv_heads, prefix, dim]``, the first rows of every sequence; ``k_own`` / ``v_own``
+    ``[n, kv_heads, rows, dim]``, or lists of ``n`` tensors ``[kv_heads, rows, dim]`` with the same strides (views of cache tensors), of which
+    sequence ``b`` sees the first ``own_lens[b]`` (int32 on the device, taken into ``[0, rows]``).  fp16 or bf16; at most 128 sequences,
+    16 query heads per kv head, ``dim`` 64 or 128.  ``scale`` defaults to ``dim ** -0.5``.  ``out`` is like ``q`` (contiguous), ``lse``
+    the fp32 ``[n, q_heads]`` logarithms of the softmax sums; a sequence that sees no row gets zeros and -inf.  Runs on the current
+    stream of the tensors' device, does not synchronise, may be captured in a graph."""
+    _require_cuda()
+    who = "attention_shared_prefix"
+    _check(q.is_cuda and q.dim() == 3 and q.dtype in (torch.float16, torch.bfloat16) and q.stride(2) == 1,
+           f"{who}: q must be a CUDA tensor [n, q_heads, dim] of fp16 or bf16, contiguous along dim")
+    n, q_heads, dim = q.shape
+    device, dtype = q.device, q.dtype
+    _check(1 <= n <= MAX_SHARED_PREFIX_SEQUENCES, f"{who}: 1 to {MAX_SHARED_PREFIX_SEQUENCES} sequences per call")
+    _check(k_prefix.dim() == 3 and k_prefix.shape == v_prefix.shape and k_prefix.shape[2] == dim and k_prefix.dtype == v_prefix.dtype == dtype
+           and k_prefix.device == v_prefix.device == device and k_prefix.stride() == v_prefix.stride() and k_prefix.stride(2) == 1,
+           f"{who}: k_prefix and v_prefix must be [kv_heads, prefix, dim], of q's type and device and with the same strides")
+    kv_heads, prefix = k_prefix.shape[:2]
+    ints = ctypes.c_void_p * n
+    if isinstance(k_own, torch.Tensor) and isinstance(v_own, torch.Tensor):
+        _check(k_own.dim() == 4 and k_own.shape == v_own.shape and k_own.shape[0] == n and k_own.stride() == v_own.stride(),
+               f"{who}: k_own and v_own must be [n, kv_heads, rows, dim] with the same strides")
+        shape, strides = k_own.shape[1:], k_own.stride()[1:]
+        step = k_own.stride(0) * 2
+        kp, vp = k_own.data_ptr(), v_own.data_ptr()
+        k_ptrs, v_ptrs = ints(*[kp + i * step for i in range(n)]), ints(*[vp + i * step for i in range(n)])
+        like = k_own.dtype == v_own.dtype == dtype and k_own.device == v_own.device == device
+    else:
+        k_own, v_own = list(k_own), list(v_own)
+        _check(len(k_own) == n and len(v_own) == n, f"{who}: one own cache pair per sequence")
+        shape, strides = k_own[0].shape, k_own[0].stride()
+        like = all(t.shape == shape and t.stride() == strides and t.dtype == dtype and t.device == device for t in (*k_own, *v_own))
+        k_ptrs, v_ptrs = ints(*[t.data_ptr() for t in k_own]), ints(*[t.data_ptr() for t in v_own])
+    _check(like and len(shape) == 3 and shape[0] == kv_heads and shape[2] == dim and strides[2] == 1,
+           f"{who}: own caches must be [kv_heads, rows, dim] each, of q's type and device and with the same strides")
+    rows = shape[1]
+    _check(own_lens.dtype == torch.int32 and own_lens.device == device and own_lens.dim() == 1 and own_lens.shape[0] == n and own_lens.is_contiguous(),
+           f"{who}: own_lens must be a contiguous int32 tensor with one value per sequence on q's device")
+    with torch.cuda.device(device):
+        out = torch.empty((n, q_heads, dim), dtype=dtype, device=device)
+        lse = torch.empty((n, q_heads), dtype=torch.float32, device=device)
+        need = _lib.qmk_attention_shared_prefix_workspace(n, q_heads, kv_heads, dim, prefix, rows)
+        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+        args = _SharedPrefixArgs(0 if dtype == torch.float16 else 1, n, q_heads, kv_heads, dim, q.data_ptr(), q.stride(0), q.stride(1),
+                                 k_prefix.data_ptr(), v_prefix.data_ptr(), prefix, k_prefix.stride(1), k_prefix.stride(0),
+                                 ctypes.addressof(k_ptrs), ctypes.addressof(v_ptrs), rows, strides[1], strides[0], own_lens.data_ptr(), 0,
+                                 dim ** -0.5 if scale is None else float(scale), out.data_ptr(), lse.data_ptr(), workspace.data_ptr(), workspace.numel())
+        rc = _lib.qmk_attention_shared_prefix(ctypes.byref(args), _stream())
+    if rc != 0:
+        raise RuntimeError(f"{who}: {_lib.qmk_last_error().decode()} (status {rc})")
+    return out, lse
 
 
 def sync_status() -> int:

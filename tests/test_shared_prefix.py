@@ -1,0 +1,229 @@
+"""``attention_shared_prefix`` against softmax(scale q k^T) v in 64 bits on the same rounded inputs.
+
+Tolerance of an output element, with A = sum of weight * |v| for it: its own rounding, eps / 2 of it; the weights' rounding to the operand type before they
+multiply v, eps / 2 of A; the scores' fp32 sums over dim products, dim 2^-24 of the largest sum of |q k| times scale as an absolute
+error of the exponent, so the same relative error of a weight, twice (numerator and denominator); the fp32 sums of the output, whose accumulator may
+truncate: 2^-23 for each of the n / 16 steps, and as much for the sum of weights.  exp2 in hardware adds 2^-22.  Weights below 2^-26 of the
+largest lose bits in fp16: 2^-37 |v| each at most.  The logarithm has the scores' error, 2^-22 of itself, and that of the sum."""
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def C(built_library):
+    import qwen_megakernel_C
+    return qwen_megakernel_C
+
+
+@pytest.fixture(scope="module")
+def gpu(C):
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return C
+
+
+def inputs(seqs, q_heads, kv_heads, dim, prefix, own, lens, dtype, seed=0, gain=1.0):
+    g = torch.Generator().manual_seed(seed)
+    q, kp, vp, ko, vo = (torch.randn(*s, generator=g).mul_(gain if i == 0 else 1.0).to(DTYPES[dtype]).cuda() for i, s in enumerate(
+        ((seqs, q_heads, dim), (kv_heads, prefix, dim), (kv_heads, prefix, dim), (seqs, kv_heads, own, dim), (seqs, kv_heads, own, dim))))
+    return q, kp, vp, ko, vo, torch.tensor(lens, dtype=torch.int32).cuda()
+
+
+def check(got, q, kp, vp, ko, vo, lens, scale=None):
+    out, lse = got
+    seqs, q_heads, dim = q.shape
+    kv_heads, prefix = kp.shape[:2]
+    group = q_heads // kv_heads
+    scale = dim ** -0.5 if scale is None else scale
+    assert out.dtype == q.dtype and out.shape == q.shape and out.is_contiguous() and lse.dtype == torch.float32 and lse.shape == (seqs, q_heads)
+    eps = torch.finfo(q.dtype).eps
+    for b in range(seqs):
+        n = min(max(int(lens[b]), 0), ko[b].shape[1])
+        k = torch.cat((kp, ko[b][:, :n]), 1).double().repeat_interleave(group, 0)
+        v = torch.cat((vp, vo[b][:, :n]), 1).double().repeat_interleave(group, 0)
+        total = prefix + n
+        if total == 0:
+            assert bool((out[b] == 0).all()) and bool((lse[b] == -math.inf).all())
+            continue
+        s = torch.einsum("hd,hnd->hn", q[b].double(), k) * scale
+        w = torch.softmax(s, 1)
+        want, a = torch.einsum("hn,hnd->hd", w, v), torch.einsum("hn,hnd->hd", w, v.abs())
+        ds = dim * 2.0 ** -24 * (torch.einsum("hd,hnd->hn", q[b].double().abs(), k.abs()).amax(1, keepdim=True) * abs(scale)) + s.abs().amax(1, keepdim=True) * 2.0 ** -23
+        steps = (total / 16 + 2) * 2.0 ** -23
+        tol = eps / 2 * (want.abs() + a * 1.001) + a * (2 * ds + 2 * steps + 2.0 ** -21) + total * 2.0 ** -37 * v.abs().amax()
+        err = (out[b].double() - want).abs()
+        assert bool((err <= tol).all()), (b, float((err / tol).max()))
+        want_lse = torch.logsumexp(s, 1)
+        err = (lse[b].double() - want_lse).abs()
+        assert bool((err <= ds[:, 0] + 2.0 ** -22 * (1 + want_lse.abs()) + steps).all()), (b, float(err.max()))
+
+
+# ------------------------------------------------------------------------------------------------------------- refusals (no device)
+def args(C, **change):
+    n = change.get("num_sequences", 2)
+    own = (ctypes.c_void_p * max(n, 1))(*[4096] * max(n, 1))
+    a = dict(type=0, num_sequences=2, q_heads=16, kv_heads=8, head_dim=128, q=4096, q_seq_stride=2048, q_head_stride=128, k_prefix=4096, v_prefix=4096,
+             prefix_len=10, prefix_row_stride=128, prefix_head_stride=1280, k_own=ctypes.addressof(own), v_own=ctypes.addressof(own), own_rows=4,
+             own_row_stride=128, own_head_stride=512, own_lens=4096, own_lens_add=0, scale=1.0, out=4096, lse=None, workspace=4096, workspace_bytes=1 << 30)
+    a.update(change)
+    made = C._SharedPrefixArgs(**a)
+    made.keep = own
+    return made
+
+
+@pytest.mark.parametrize("change,text", [(dict(num_sequences=0), b"num_sequences"), (dict(num_sequences=129), b"num_sequences"), (dict(type=2), b"type"),
+                                         (dict(head_dim=96), b"head_dim"), (dict(kv_heads=0), b"kv_heads"), (dict(q_heads=12), b"kv_heads"),
+                                         (dict(q_heads=136), b"kv_heads"), (dict(prefix_len=-1), b"length"), (dict(own_rows=-1), b"length"),
+                                         (dict(q=None), b"null"), (dict(out=None), b"null"), (dict(k_prefix=None), b"null"), (dict(own_lens=None), b"null"),
+                                         (dict(k_own=None), b"null"), (dict(scale=float("inf")), b"scale"), (dict(scale=float("nan")), b"scale"),
+                                         (dict(q=4098), b"aligned"), (dict(v_prefix=4104), b"aligned"), (dict(q_seq_stride=2049), b"strides"),
+                                         (dict(prefix_row_stride=132), b"strides"), (dict(own_head_stride=4), b"strides"),
+                                         (dict(workspace=None), b"workspace"), (dict(workspace_bytes=100), b"workspace")])
+def test_refused_before_anything_runs(C, change, text):
+    assert C._lib.qmk_attention_shared_prefix(ctypes.byref(args(C, **change)), None) == 2 and text in C._lib.qmk_last_error()
+
+
+def test_null_arguments_and_null_caches_are_refused(C):
+    assert C._lib.qmk_attention_shared_prefix(None, None) == 2
+    holes = (ctypes.c_void_p * 2)(4096, None)
+    assert C._lib.qmk_attention_shared_prefix(ctypes.byref(args(C, v_own=ctypes.addressof(holes))), None) == 2 and b"null" in C._lib.qmk_last_error()
+
+
+@pytest.mark.gpu
+def test_wrong_tensors_are_refused(gpu):
+    good = inputs(2, 4, 2, 64, 8, 8, [1, 2], "fp16")
+    q, kp, vp, ko, vo, lens = good
+    bad = [(q.float(), *good[1:]), (q[0], *good[1:]), (q.cpu(), *good[1:]), (q, kp.bfloat16(), vp, ko, vo, lens), (q, kp[:1], vp[:1], ko, vo, lens),
+           (q, kp, vp[:, :4], ko, vo, lens), (q, kp, vp, ko[:1], vo[:1], lens), (q, kp, vp, ko, vo[:, :, :4], lens), (q, kp, vp, ko, vo, lens.long()),
+           (q, kp, vp, ko, vo, lens[:1]), (q, kp, vp, ko, vo, lens.cpu()), (q, kp, vp, list(ko)[:1], list(vo), lens), (q, kp, vp, ko.float(), vo.float(), lens),
+           (q[:, :3], *good[1:]), (q, kp, vp, [ko[0], ko[1].transpose(0, 1)], list(vo), lens)]
+    for case in bad:
+        with pytest.raises(RuntimeError):
+            gpu.attention_shared_prefix(*case)
+
+
+# ------------------------------------------------------------------------------------------------------------- results
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("q_heads,kv_heads,dim", [(16, 8, 128), (4, 4, 64), (6, 2, 128), (8, 1, 64), (16, 1, 128), (32, 4, 64)])
+@pytest.mark.parametrize("seqs,prefix,own", [(1, 1, 1), (1, 0, 5), (2, 63, 16), (3, 64, 64), (5, 65, 300), (17, 1000, 33), (40, 129, 65), (128, 200, 20)])
+def test_matches_the_definition(gpu, dtype, q_heads, kv_heads, dim, seqs, prefix, own):
+    lens = [(own * (i + 1) // seqs) if i % 5 else (0 if i else own) for i in range(seqs)]
+    case = inputs(seqs, q_heads, kv_heads, dim, prefix, own, lens, dtype, seed=seqs + prefix)
+    check(gpu.attention_shared_prefix(*case), *case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs,q_heads,kv_heads,prefix,own", [(8, 16, 8, 32768, 64), (64, 16, 8, 4097, 513), (128, 16, 8, 2049, 100), (33, 32, 4, 5000, 1), (100, 8, 8, 777, 1025)])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_long_prefixes_and_full_batches(gpu, dtype, seqs, q_heads, kv_heads, prefix, own):
+    case = inputs(seqs, q_heads, kv_heads, 128, prefix, own, [(7919 * i) % (own + 1) for i in range(seqs)], dtype, seed=prefix, gain=1.5)
+    check(gpu.attention_shared_prefix(*case), *case)
+
+
+@pytest.mark.gpu
+def test_no_rows_at_all_and_lengths_outside_the_cache(gpu):
+    q, kp, vp, ko, vo, _ = inputs(6, 16, 8, 128, 0, 40, [0] * 6, "fp16")
+    lens = torch.tensor([0, -3, 40, 41, 10 ** 6, 1], dtype=torch.int32).cuda()     # taken into [0, 40]
+    check(gpu.attention_shared_prefix(q, kp, vp, ko, vo, lens), q, kp, vp, ko, vo, lens)
+    none = ko[:, :, :0]
+    out, lse = gpu.attention_shared_prefix(q, kp, vp, none, none, lens)
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+    q, kp, vp, ko, vo, _ = inputs(6, 16, 8, 128, 100, 0, [0] * 6, "fp16")
+    check(gpu.attention_shared_prefix(q, kp, vp, ko, vo, lens), q, kp, vp, ko, vo, lens)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs", [3, 20, 70])
+@pytest.mark.parametrize("garbage", [float("nan"), float("inf"), -65504.0])
+def test_rows_behind_the_last_are_not_looked_at(gpu, garbage, seqs):
+    """Views of larger buffers: what lies behind the prefix, behind a sequence's last row and between heads is garbage."""
+    q, kp, vp, ko, vo, lens = inputs(seqs, 16, 8, 128, 301, 77, [(13 * i) % 78 for i in range(seqs)], "fp16", seed=4)
+    def bury(t, dim):
+        shape = list(t.shape)
+        shape[dim] += 51
+        wide = torch.full(shape, garbage, dtype=t.dtype, device="cuda")
+        wide.narrow(dim, 0, t.shape[dim]).copy_(t)
+        return wide.narrow(dim, 0, t.shape[dim])
+    kp, vp, ko, vo = bury(kp, 1), bury(vp, 1), bury(ko, 2), bury(vo, 2)
+    for b, n in enumerate(lens.tolist()):
+        ko[b, :, n:] = garbage
+        vo[b, :, n:] = garbage
+    got = gpu.attention_shared_prefix(q, kp, vp, ko, vo, lens)
+    assert not bool(got[0].isnan().any())
+    check(got, q, kp, vp, ko, vo, lens)
+
+
+@pytest.mark.gpu
+def test_other_strides_and_lists_of_caches(gpu):
+    """Heads between rows ([rows, heads, dim] caches), queries in a wider buffer, caches of separate allocations: views of one layer of
+    the engine's [layer][head][position] caches."""
+    seqs, prefix, own = 9, 150, 60
+    lens = torch.tensor([(11 * i) % 61 for i in range(seqs)], dtype=torch.int32).cuda()
+    g = torch.Generator().manual_seed(8)
+    caches = [[torch.randn(3, 8, prefix + own, 128, generator=g).half().cuda() for _ in range(seqs)] for _ in range(2)]
+    q = torch.randn(seqs, 40, 128, generator=g).half().cuda()[:, 8:24]
+    kp, vp = caches[0][0][1][:, :prefix], caches[1][0][1][:, :prefix]
+    ko, vo = ([c[1][:, prefix:] for c in side] for side in caches)
+    check(gpu.attention_shared_prefix(q, kp, vp, ko, vo, lens), q, kp, vp, ko, vo, lens)
+    turned = [torch.randn(*s, generator=g).half().cuda() for s in ((prefix, 8, 128), (prefix, 8, 128), (seqs, own, 8, 128), (seqs, own, 8, 128))]
+    case = (q, turned[0].transpose(0, 1), turned[1].transpose(0, 1), turned[2].transpose(1, 2), turned[3].transpose(1, 2), lens)
+    check(gpu.attention_shared_prefix(*case), *case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [0.0, -0.05, 1.0, 3.0])
+def test_scales(gpu, scale):
+    case = inputs(20, 16, 8, 128, 333, 50, [(17 * i) % 51 for i in range(20)], "fp16", seed=2, gain=0.5)
+    check(gpu.attention_shared_prefix(*case, scale=scale), *case, scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs", [4, 66])
+def test_a_maximum_that_rises_late(gpu, seqs):
+    """Scores that grow along the rows: the running maximum is raised again and again, by more than any threshold."""
+    q, kp, vp, ko, vo, lens = inputs(seqs, 16, 8, 128, 2000, 40, [40] * seqs, "fp16", seed=6)
+    q[:] = q[:1, :1]
+    kp += (torch.linspace(-2, 2, 2000).cuda()[None, :, None] * q[0, 0]).half()
+    case = (q, kp, vp, ko, vo, lens)
+    check(gpu.attention_shared_prefix(*case), *case)
+
+
+@pytest.mark.gpu
+def test_same_bits_again_on_other_streams_and_in_graphs(gpu):
+    case = inputs(30, 16, 8, 128, 999, 99, [(31 * i) % 100 for i in range(30)], "fp16", seed=5)
+    want = gpu.attention_shared_prefix(*case)
+    for _ in range(3):
+        again = gpu.attention_shared_prefix(*case)
+        assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+    q2 = case[0].flip(0).contiguous()
+    lens2 = case[5].flip(0).contiguous()
+    want2 = gpu.attention_shared_prefix(q2, *case[1:5], lens2)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for i in range(8):                               # two at a time
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(gpu.attention_shared_prefix(*(case if i % 2 == 0 else (q2, *case[1:5], lens2))))
+    torch.cuda.synchronize()
+    for i, (o, l) in enumerate(got):
+        w = want if i % 2 == 0 else want2
+        assert torch.equal(o, w[0]) and torch.equal(l, w[1])
+    q, lens = case[0].clone(), case[5].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(streams[0]):
+        gpu.attention_shared_prefix(q, *case[1:5], lens)
+        with torch.cuda.graph(graph, stream=streams[0]):
+            out, lse = gpu.attention_shared_prefix(q, *case[1:5], lens)
+        for new_q, new_lens, w in ((case[0], case[5], want), (q2, lens2, want2), (case[0], case[5], want)):
+            q.copy_(new_q)
+            lens.copy_(new_lens)
+            graph.replay()
+            assert torch.equal(out, w[0]) and torch.equal(lse, w[1])
