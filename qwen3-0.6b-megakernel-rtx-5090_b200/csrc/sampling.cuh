@@ -11,6 +11,10 @@
 // more than a token in the tail of a large vocabulary has.
 //
 // A cluster of CTAs takes a row and keeps it in shared memory as fp32: the row crosses HBM once, however often it is looked at.
+// A threshold (of top-k, of top-p) is found by narrowing down: a histogram of counts over the distance to the maximum, then, where
+// the tokens up to the border's bin are few, a list of them that one CTA sorts and finishes; else the border's bins alone are looked
+// at again (see sample_rows).  Rows whose border lies among more equal values than a list holds go through eight-bit
+// histograms of the keys (search).
 #ifndef QMK_SAMPLING_CUH_
 #define QMK_SAMPLING_CUH_
 
@@ -18,6 +22,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <stddef.h>
 #include <stdint.h>
 
 namespace qmk_sample {
@@ -27,9 +32,15 @@ namespace cg = cooperative_groups;
 constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int MAX_VOCAB = 1 << 18;               // masses of at most 2^45 in 63 bits
 constexpr int MAX_CLUSTER = 8;
-constexpr int BINS = 256;                        // of a histogram: eight bits of the key
+constexpr int MAX_SLICE = MAX_VOCAB / MAX_CLUSTER;
+constexpr int BINS = 2048;                       // of the distance to the maximum: 4 per thread
+constexpr float SPAN = 32.5f;                    // times the temperature: masses further below the maximum round to nothing (e^-32.5 < 2^-46)
+constexpr int KEY_BINS = 256;                    // of a histogram of keys: eight bits
+constexpr int LIST = 1024;                       // tokens that one CTA sorts
 constexpr int NO_TOKEN = 0x7fffffff;             // pick of a row without a largest value, as in the greedy steps
 constexpr float LARGEST_UNIFORM = 0x1.fffffep-1f;
+static_assert(BINS == 4 * THREADS && LIST == 2 * THREADS, "bins and list entries per thread");
+static_assert(MAX_SLICE <= WARPS * 16 * 128, "a warp's range of the slice is at most 16 groups of 128 tokens");
 
 struct Params {
   const void *logits;
@@ -44,14 +55,22 @@ struct Params {
   float *logprobs;                               // may be null
 };
 
-struct Shared {
-  unsigned long long mass[2][BINS];              // histograms, in turn: one is read by the cluster while the next is filled
-  unsigned long long sum[BINS];                  // the cluster's
-  unsigned long long warp[WARPS];
-  unsigned long long cta[8];                     // one slot per exchange of the cluster, see Row
-  unsigned long long found[3];
-  int cut;
+struct __align__(16) Shared {                   // (the row lies behind it)
+  unsigned int counts[BINS];                     // this CTA's histogram, read by the cluster
+  union {
+    unsigned long long masses[BINS];             // the border's bins once more, by exact mass
+    unsigned long long keys[2][KEY_BINS];    // search: histograms in turn, one is read while the next is filled
+    unsigned long long sorted[LIST];
+  };
+  unsigned long long list[LIST];                 // this CTA's candidates
+  unsigned long long warp[WARPS], group[WARPS];
+  unsigned long long cta[16];                    // one slot per exchange of the cluster, see gather
+  unsigned long long found[4];
+  unsigned long long threshold;                  // written by the CTA that finds it
+  int listed, bin_lo, bin_hi;
 };
+
+static_assert(sizeof(Shared) % 16 == 0 && offsetof(Shared, masses) % 16 == 0, "vector accesses");
 
 // Order of the values as whole numbers: larger value, larger key.  (x is not NaN, zeros are +0.)
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -70,15 +89,91 @@ __device__ __forceinline__ V warp_sum(V v) {
   return v;
 }
 
-// What is kept: values above a threshold, and of those equal to it the ones up to an index.
-struct Kept {
-  uint32_t key;
-  int cut;
-  __device__ __forceinline__ bool operator()(uint32_t k, int i) const { return k > key || (k == key && i <= cut); }
+// A token's place in the order, larger is earlier: the key, then the lower index.
+__device__ __forceinline__ unsigned long long place_of(float x, int index) {
+  return (static_cast<unsigned long long>(key_of(x)) << 32) | static_cast<uint32_t>(~index);
+}
+__device__ __forceinline__ float value_of(unsigned long long place) {
+  const uint32_t k = static_cast<uint32_t>(place >> 32);
+  return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+__device__ __forceinline__ int index_of(unsigned long long place) { return static_cast<int>(~static_cast<uint32_t>(place)); }
+
+// 2^t for t <= 0, relative error below 2^-42 (Taylor's series of e^(r ln 2) to the tenth power, |r| <= 1/2): a third of the
+// instructions of exp().  t < -47 gives 0.
+__device__ __forceinline__ double power_of_two(double t) {
+  if (!(t >= -47.0)) return 0.0;
+  const double magic = 6755399441055744.0;       // 1.5 * 2^52: the sum's low word is the nearest whole number
+  const double y = t + magic, r = t - (y - magic);
+  double q = 7.05491162080112e-09;               // (ln 2)^k / k!
+  q = fma(q, r, 1.0178086009239699e-07);
+  q = fma(q, r, 1.3215486790144307e-06);
+  q = fma(q, r, 1.5252733804059841e-05);
+  q = fma(q, r, 1.5403530393381608e-04);
+  q = fma(q, r, 1.3333558146428443e-03);
+  q = fma(q, r, 9.618129107628477e-03);
+  q = fma(q, r, 5.550410866482158e-02);
+  q = fma(q, r, 2.402265069591007e-01);
+  q = fma(q, r, 6.931471805599453e-01);
+  q = fma(q, r, 1.0);
+  return __hiloint2double(__double2hiint(q) + (__double2loint(y) << 20), __double2loint(q));
+}
+// round(w * 2^45) for w in [0, 1]: the last bit of w + 2^7 is 2^-45
+__device__ __forceinline__ unsigned long long mass_of(double w) {
+  return static_cast<unsigned long long>(__double_as_longlong(w + 128.0)) - 0x4060000000000000ull;
+}
+
+// Bitonic sort of `size` entries (a power of two, 32 to 2 THREADS), largest first, by the whole CTA; a short one by its first warp.
+__device__ __forceinline__ void sort_descending(unsigned long long *v, int size, int tid) {
+  __syncthreads();
+  const bool short_one = size <= 64;
+  if (!short_one || tid < 32) {
+    for (int block = 2; block <= size; block <<= 1)
+      for (int step = block >> 1; step > 0; step >>= 1) {
+        const int i = 2 * tid - (tid & (step - 1)), j = i + step;
+        if (j < size) {
+          const unsigned long long a = v[i], b = v[j];
+          if ((a < b) == ((i & block) == 0)) { v[i] = b; v[j] = a; }
+        }
+        if (short_one) __syncwarp(); else __syncthreads();
+      }
+  }
+  __syncthreads();
+}
+
+// 16 bytes of logits as values
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void load(const float *p, float (&v)[4]) {
+    const float4 a = __ldg(reinterpret_cast<const float4 *>(p));
+    v[0] = clean(a.x); v[1] = clean(a.y); v[2] = clean(a.z); v[3] = clean(a.w);
+  }
+};
+template <> struct Vec<__half> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void load(const __half *p, float (&v)[8]) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p));
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+      v[2 * i] = clean(f.x); v[2 * i + 1] = clean(f.y);
+    }
+  }
+};
+template <> struct Vec<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void load(const __nv_bfloat16 *p, float (&v)[8]) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p));
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[2 * i] = clean(__uint_as_float(w[i] << 16)); v[2 * i + 1] = clean(__uint_as_float(w[i] & 0xffff0000u)); }
+  }
 };
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS) sample_rows(const Params p) {
+__global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   Shared &s = *reinterpret_cast<Shared *>(smem_raw);
   float *const x = reinterpret_cast<float *>(smem_raw + sizeof(Shared));
@@ -86,20 +181,23 @@ __global__ void __launch_bounds__(THREADS) sample_rows(const Params p) {
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int row = static_cast<int>(blockIdx.x) / ranks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int first = rank * p.slice, n = max(0, min(p.slice, p.vocab - first));     // this CTA's tokens [first, first + n)
+  const int n4 = (n + 3) >> 2;                   // in fours, the last one filled up with -inf
+  const float4 *const x4 = reinterpret_cast<const float4 *>(x);
   const float temperature = p.temperatures ? p.temperatures[row] : p.temperature;
   const float top_p = p.top_ps ? p.top_ps[row] : p.top_p, min_p = p.min_ps ? p.min_ps[row] : p.min_p;
   const int top_k = p.top_ks ? p.top_ks[row] : p.top_k;
   const float u_raw = p.uniforms[row];
-  const float u = u_raw >= 0.0f ? fminf(u_raw, LARGEST_UNIFORM) : 0.0f;
+  const double u = u_raw >= 0.0f ? fminf(u_raw, LARGEST_UNIFORM) : 0.0f;
   int exchange = 0;                              // slots of Shared::cta are used in turn
 
-  // one value of every CTA to every CTA, in the order of the ranks
+  // one value of every CTA to every CTA, in the order of the ranks; what the CTA wrote before is there for the others behind it
   auto gather = [&](unsigned long long mine, auto &&take) {
-    const int slot = exchange++ & 7;
+    const int slot = exchange++ & 15;
     if (tid == 0) s.cta[slot] = mine;
     cluster.sync();
     for (int r = 0; r < ranks; ++r) take(r, *cluster.map_shared_rank(&s.cta[slot], r));
   };
+  // sum over the CTA, to all threads; `before`: of the threads in front of this one
   auto block_sum = [&](unsigned long long v) {
     v = warp_sum(v);
     __syncthreads();
@@ -110,17 +208,61 @@ __global__ void __launch_bounds__(THREADS) sample_rows(const Params p) {
     for (int w = 0; w < WARPS; ++w) total += s.warp[w];
     return total;
   };
+  auto block_scan = [&](unsigned long long v, unsigned long long &before) {
+    unsigned long long run = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long up = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += up;
+    }
+    __syncthreads();
+    if (lane == 31) s.warp[warp] = run;
+    __syncthreads();
+    unsigned long long total = 0, ahead = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      ahead += w < warp ? s.warp[w] : 0;
+      total += s.warp[w];
+    }
+    before = ahead + run - v;
+    return total;
+  };
 
   // ---- the row, once; its largest value and where that is first
-  unsigned long long best = 0;                   // key, then the index from above
+  for (int b = tid; b < BINS / 4; b += THREADS) reinterpret_cast<uint4 *>(s.counts)[b] = make_uint4(0, 0, 0, 0);
+  if (tid == 0) s.listed = 0;
+  unsigned long long best = 0;
   {
+    constexpr int N = Vec<T>::N;
     const T *const src = static_cast<const T *>(p.logits) + row * p.row_stride + first;
-    for (int i = tid; i < n; i += THREADS) {
+    float high = -INFINITY;
+    int at = first;
+    bool any = false;                            // (a row of -inf: its first token)
+    auto keep = [&](float v, int i) {
+      if (v > high || !any) { high = v; at = first + i; any = true; }
+    };
+    int i0 = 0;
+    if ((reinterpret_cast<unsigned long long>(src) & 15) == 0) {
+      const int nv = n / N;
+#pragma unroll 4
+      for (int i = tid; i < nv; i += THREADS) {
+        float v[N];
+        Vec<T>::load(src + i * N, v);
+#pragma unroll
+        for (int j = 0; j < N; j += 4) *reinterpret_cast<float4 *>(x + i * N + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+#pragma unroll
+        for (int j = 0; j < N; ++j) keep(v[j], i * N + j);
+      }
+      i0 = nv * N;
+    }
+#pragma unroll 8
+    for (int i = i0 + tid; i < n; i += THREADS) {
       const float v = load_logit(src + i);
       x[i] = v;
-      const unsigned long long c = (static_cast<unsigned long long>(key_of(v)) << 32) | static_cast<uint32_t>(~(first + i));
-      best = c > best ? c : best;
+      keep(v, i);
     }
+    if (tid < 4 * n4 - n) x[n + tid] = -INFINITY;
+    if (any) best = place_of(high, at);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
@@ -133,140 +275,374 @@ __global__ void __launch_bounds__(THREADS) sample_rows(const Params p) {
     const unsigned long long mine = best;
     gather(mine, [&](int, unsigned long long v) { best = v > best ? v : best; });
   }
-  const uint32_t top_key = static_cast<uint32_t>(best >> 32);
-  const int top_index = static_cast<int>(~static_cast<uint32_t>(best));
-  const float top = __uint_as_float(top_key & 0x80000000u ? top_key ^ 0x80000000u : ~top_key);
-  const bool empty = top == -INFINITY, greedy = !(temperature > 0.0f) || top_k == 1;
-  if (empty || greedy) {
+  const float top = value_of(best);
+  const bool empty = top == -INFINITY;
+  if (empty || !(temperature > 0.0f) || top_k == 1) {
     if (rank == 0 && tid == 0) {
-      p.tokens[row] = empty ? NO_TOKEN : top_index;
+      p.tokens[row] = empty ? NO_TOKEN : index_of(best);
       if (p.logprobs) p.logprobs[row] = empty ? NAN : 0.0f;
     }
     cluster.sync();                              // (nobody leaves while its shared memory is read)
     return;
   }
 
-  // (a row with infinite logits: they share the mass alone)
-  auto exponent = [&](float v) { return v == top ? 0.0 : top == INFINITY ? -INFINITY : (static_cast<double>(v) - static_cast<double>(top)) / static_cast<double>(temperature); };
-  auto weight = [&](float v) { return v == -INFINITY ? 0.0 : exp(exponent(v)); };
-  auto mass_of = [&](float v) { return static_cast<unsigned long long>(__double2ull_rn(weight(v) * 0x1p45)); };
+  const double slope = 1.4426950408889634 / static_cast<double>(temperature);
+  // log2 of the mass (differences with infinite values end as 0 mass; infinite maxima share it)
+  auto exponent = [&](float v) { return v == top ? 0.0 : (static_cast<double>(v) - static_cast<double>(top)) * slope; };
+  auto mass = [&](float v) { return mass_of(power_of_two(exponent(v))); };
+  const double least = min_p > 0.0f ? static_cast<double>(min_p) : 0.0, least_exponent = least > 0.0 ? log2(least) - 1e-6 : -1e300;
+  auto above_least = [&](float v) {              // the mass where min_p lets the token stay
+    const double t = exponent(v);
+    if (!(t >= least_exponent)) return 0ull;
+    const double w = power_of_two(t);
+    return w >= least || v == top ? mass_of(w) : 0ull;
+  };
+  const double share = top_p > 0.0f ? static_cast<double>(top_p) : 0.0;
+  auto share_of = [&](unsigned long long total) {        // of the ranks, those in front of which the mass is below this stay
+    const unsigned long long t = __double2ull_ru(share * __ull2double_rn(total));
+    return t < 1 ? 1ull : t < total ? t : total;
+  };
+  auto draw_from = [&](unsigned long long total) { return __double2ull_rd(u * __ull2double_rn(total)); };
+  auto write = [&](int index, float v, unsigned long long total) {
+    p.tokens[row] = index;
+    const double z = v == top ? 0.0 : (static_cast<double>(v) - static_cast<double>(top)) / static_cast<double>(temperature);
+    if (p.logprobs) p.logprobs[row] = static_cast<float>(z - log(__ull2double_rn(total) * 0x1p-45));
+  };
+  // every token of the slice: f(value, index)
+  auto each = [&](auto &&f) {
+    for (int i = tid; i < n4; i += THREADS) {
+      const float4 v = x4[i];
+      const int at = first + 4 * i;
+      f(v.x, at); f(v.y, at + 1); f(v.z, at + 2); f(v.w, at + 3);
+    }
+  };
 
-  // The lowest index of the row at which the running sum of `value` exceeds `target(total)`; the CTA that holds it calls found(index, value, total).
+  // The lowest index of the row at which the running sum of `value` exceeds `target(total)`; one thread calls found(index, x, total).  A
+  // warp has a range of the slice, in groups of 128 tokens.
   auto pick = [&](auto &&value, auto &&target, auto &&found) {
-    const int seg = (n + WARPS - 1) / WARPS, lo = min(n, warp * seg), hi = min(n, lo + seg);   // a warp, a range of the indices
-    unsigned long long sum = 0;
-    for (int i = lo + lane; i < hi; i += 32) sum += value(i);
+    const int seg = (n4 + WARPS * 32 - 1) / (WARPS * 32) * 32, lo = min(n4, warp * seg), hi = min(n4, lo + seg);
+    auto four = [&](int i, unsigned long long (&v)[4]) {
+      const float4 f = x4[i];
+      const int at = first + 4 * i;
+      v[0] = value(f.x, at); v[1] = value(f.y, at + 1); v[2] = value(f.z, at + 2); v[3] = value(f.w, at + 3);
+    };
+    unsigned long long sum = 0, v[4];
+    for (int i = lo + lane; i < hi; i += 32) { four(i, v); sum += (v[0] + v[1]) + (v[2] + v[3]); }
     const unsigned long long mine = block_sum(sum);
     unsigned long long before = 0, total = 0;
-    gather(mine, [&](int r, unsigned long long v) { before += r < rank ? v : 0; total += v; });
+    gather(mine, [&](int r, unsigned long long c) { before += r < rank ? c : 0; total += c; });
     const unsigned long long want = target(total);
-    if (before <= want && want < before + mine) {          // (the same for every thread of the CTA)
-      unsigned long long at = before;
-      int w = 0;
-      for (; w < WARPS - 1 && at + s.warp[w] <= want; ++w) at += s.warp[w];
-      if (warp == w) {
-        bool done = false;
-        for (int i0 = lo; i0 < hi && !done; i0 += 32) {
-          const int i = i0 + lane;
-          const unsigned long long v = i < hi ? value(i) : 0;
-          unsigned long long run = v;
+    if (!(before <= want && want < before + mine)) return;     // (the same for every thread of the CTA)
+    int w = 0;
+    for (; w < WARPS - 1 && before + s.warp[w] <= want; ++w) before += s.warp[w];
+    const int at = min(n4, w * seg) + warp * 32 + lane;        // warp g: group g of that range
+    v[0] = v[1] = v[2] = v[3] = 0;
+    if (warp * 32 < seg && at < n4) four(at, v);
+    const unsigned long long own = (v[0] + v[1]) + (v[2] + v[3]);
+    unsigned long long run = own;
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const unsigned long long up = __shfl_up_sync(0xffffffffu, run, o);
-            if (lane >= o) run += up;
-          }
-          const unsigned int over = __ballot_sync(0xffffffffu, at + run > want);
-          if (over) {
-            if (lane == __ffs(over) - 1) found(i, total);
-            done = true;
-          }
-          at += __shfl_sync(0xffffffffu, run, 31);
-        }
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long up = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += up;
+    }
+    if (lane == 31) s.group[warp] = run;
+    __syncthreads();
+    for (int g = 0; g < warp; ++g) before += s.group[g];
+    before += run - own;
+    if (before <= want && want < before + own) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (before <= want && want < before + v[j]) found(first + 4 * at + j, x[4 * at + j], total);
+        before += v[j];
       }
     }
   };
 
-  // The threshold behind which the running sum of `value`, in the order of the values, reaches target(total): eight bits of the
-  // key at a time, then the ties.  `value(i)` is 0 for tokens that are out already.
-  int turn = 0;
-  auto search = [&](auto &&value, auto &&target) -> Kept {
+  // The candidates of all CTAs to rank 0, sorted there, largest first; their number.  More than LIST: nothing is sorted.
+  auto collect = [&](auto &&candidate) {
+    each([&](float v, int i) {
+      if (candidate(v, i)) {
+        const int at = atomicAdd(&s.listed, 1);
+        if (at < LIST) s.list[at] = place_of(v, i);
+      }
+    });
+    __syncthreads();
+    int total = 0, ahead[MAX_CLUSTER + 1];
+#pragma unroll
+    for (int r = 0; r <= MAX_CLUSTER; ++r) ahead[r] = 0;
+    const int slot = exchange++ & 15;
+    if (tid == 0) s.cta[slot] = static_cast<unsigned long long>(s.listed);
+    cluster.sync();
+#pragma unroll
+    for (int r = 0; r < MAX_CLUSTER; ++r) {
+      ahead[r] = total;
+      if (r < ranks) total += static_cast<int>(min(*cluster.map_shared_rank(&s.cta[slot], r), static_cast<unsigned long long>(MAX_VOCAB)));
+    }
+    ahead[MAX_CLUSTER] = total;
+    if (rank == 0 && total <= LIST) {
+      int size = 32;
+      while (size < total) size <<= 1;
+#pragma unroll
+      for (int r = 0; r < MAX_CLUSTER; ++r) {
+        if (r >= ranks) continue;
+        const unsigned long long *const theirs = cluster.map_shared_rank(s.list, r);
+        for (int i = tid; i < ahead[r + 1] - ahead[r]; i += THREADS) s.sorted[ahead[r] + i] = theirs[i];
+      }
+      for (int i = total + tid; i < size; i += THREADS) s.sorted[i] = 0;
+      sort_descending(s.sorted, size, tid);
+    }
+    return total;
+  };
+  // rank 0: the threshold behind the sorted candidate number `count` (from 1 on), to every CTA
+  auto announce = [&](int count) {
+    const unsigned long long at = s.sorted[count - 1];
+    if (tid < ranks) *cluster.map_shared_rank(&s.threshold, tid) = at;
+  };
+  // Rank 0, where the list holds every token that may stay: the first k of it, of those the ones that top-p (`want`: their mass, 0 where it is
+  // a share of the list's) and min_p leave, then these by index and the pick among them.
+  auto finish_list = [&](int total, unsigned long long k, unsigned long long want) {
+    const int limit = static_cast<int>(min(static_cast<unsigned long long>(total), k));
+    unsigned long long c[2], m[2], before;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      c[j] = 2 * tid + j < limit ? s.sorted[2 * tid + j] : 0;
+      m[j] = 2 * tid + j < limit ? mass(value_of(c[j])) : 0;
+    }
+    const unsigned long long all = block_scan(m[0] + m[1], before);
+    if (top_p < 1.0f) want = want ? want : share_of(all); else want = ~0ull;
+    const bool keep0 = 2 * tid < limit && before < want && (tid == 0 || above_least(value_of(c[0])) || least == 0.0);
+    const bool keep1 = 2 * tid + 1 < limit && before + m[0] < want && (above_least(value_of(c[1])) || least == 0.0);
+    const int stay = __syncthreads_count(keep0) + __syncthreads_count(keep1);
+    int size = 32;
+    while (size < stay) size <<= 1;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)                   // the halves change places: by index, the lowest (its complement the largest) first
+      if (2 * tid + j < size) s.sorted[2 * tid + j] = 2 * tid + j < stay ? (c[j] << 32) | (c[j] >> 32) : 0;
+    sort_descending(s.sorted, size, tid);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      c[j] = 2 * tid + j < stay ? s.sorted[2 * tid + j] : 0;
+      c[j] = (c[j] << 32) | (c[j] >> 32);
+      m[j] = 2 * tid + j < stay ? mass(value_of(c[j])) : 0;
+    }
+    const unsigned long long kept = block_scan(m[0] + m[1], before), at = draw_from(kept);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (before <= at && at < before + m[j]) write(index_of(c[j]), value_of(c[j]), kept);
+      before += m[j];
+    }
+  };
+
+  // The place behind which the running sum of `value`, in the order, reaches target(total): eight bits of the key at a time, then the
+  // ties by index.  `value` is 0 for tokens that are out already, and the same for equal values.
+  auto search = [&](auto &&value, auto &&target) -> unsigned long long {
     uint32_t prefix = 0;
     unsigned long long want = 0, before = 0;
-    bool everything = false;
-    for (int shift = 24; shift >= 0 && !everything; shift -= 8) {
-      unsigned long long *const hist = s.mass[turn & 1];
-      for (int b = tid; b < BINS; b += THREADS) hist[b] = 0;
+    cluster.sync();                              // (the space of the histograms was another's)
+    for (int shift = 24, turn = 0; shift >= 0; shift -= 8, ++turn) {
+      unsigned long long *const hist = s.keys[turn & 1];
+      if (tid < KEY_BINS) hist[tid] = 0;
       __syncthreads();
-      for (int i = tid; i < n; i += THREADS) {
-        const uint32_t k = key_of(x[i]);
-        if (shift < 24 && (k >> (shift + 8)) != prefix) continue;
-        const unsigned long long v = value(i);
-        if (v) atomicAdd(&hist[(k >> shift) & (BINS - 1)], v);
-      }
+      each([&](float v, int i) {
+        const uint32_t k = key_of(v);
+        if (shift < 24 && (k >> (shift + 8)) != prefix) return;
+        if (i >= p.vocab) return;
+        const unsigned long long c = value(v, i);
+        if (c) atomicAdd(&hist[(k >> shift) & (KEY_BINS - 1)], c);
+      });
       cluster.sync();
-      for (int b = tid; b < BINS; b += THREADS) {
-        unsigned long long v = 0;
-        for (int r = 0; r < ranks; ++r) v += cluster.map_shared_rank(hist, r)[b];
-        s.sum[b] = v;
-      }
+      unsigned long long c = 0, ahead;
+      const int bin = KEY_BINS - 1 - tid;
+      if (tid < KEY_BINS)
+        for (int r = 0; r < ranks; ++r) c += cluster.map_shared_rank(hist, r)[bin];
+      const unsigned long long total = block_scan(c, ahead);
+      if (shift == 24) want = target(total);
+      if (tid == 0) s.found[0] = s.found[1] = 0;
       __syncthreads();
-      if (tid == 0) {
-        unsigned long long total = 0, at = before;
-        for (int b = 0; b < BINS; ++b) total += s.sum[b];
-        if (shift == 24) want = target(total);
-        int b = BINS - 1;
-        while (b > 0 && at + s.sum[b] < want) at += s.sum[b--];
-        s.found[0] = at + s.sum[b] < want ? ~0ull : b;     // fewer in all: everything stays
-        s.found[1] = at;
-        s.found[2] = want;
-      }
+      if (before + ahead < want && want <= before + ahead + c) { s.found[0] = bin; s.found[1] = before + ahead; }
       __syncthreads();
-      everything = s.found[0] == ~0ull;
       prefix = (prefix << 8) | static_cast<uint32_t>(s.found[0]);
       before = s.found[1];
-      want = s.found[2];
-      ++turn;
     }
-    if (everything) return Kept{0u, 0x7fffffff};
-    // tokens of the threshold's value, as many as the sum before them leaves room for
-    if (tid == 0) s.cut = 0x7fffffff;
+    // tokens of the border's value: as many as the sum in front of them leaves room for
+    if (tid == 0) s.threshold = 0;
     const uint32_t key = prefix;
-    unsigned long long each = 0;
-    for (int i = tid; i < n; i += THREADS)
-      if (key_of(x[i]) == key) { const unsigned long long v = value(i); each = v > each ? v : each; }
+    unsigned long long one = 0;
+    each([&](float v, int i) { if (i < p.vocab && key_of(v) == key) { const unsigned long long c = value(v, i); one = c > one ? c : one; } });
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) { const unsigned long long other = __shfl_xor_sync(0xffffffffu, each, o); each = other > each ? other : each; }
+    for (int o = 16; o > 0; o >>= 1) { const unsigned long long other = __shfl_xor_sync(0xffffffffu, one, o); one = other > one ? other : one; }
     __syncthreads();
-    if (lane == 0) s.warp[warp] = each;
+    if (lane == 0) s.warp[warp] = one;
     __syncthreads();
-    for (int w = 0; w < WARPS; ++w) each = s.warp[w] > each ? s.warp[w] : each;
-    gather(each, [&](int, unsigned long long v) { each = v > each ? v : each; });
-    const unsigned long long room = each ? (want - before + each - 1) / each : 1;
-    pick([&](int i) -> unsigned long long { return key_of(x[i]) == key && value(i) != 0; }, [&](unsigned long long) { return room - 1; },
-         [&](int i, unsigned long long) { for (int r = 0; r < ranks; ++r) *cluster.map_shared_rank(&s.cut, r) = first + i; });
+    for (int w = 0; w < WARPS; ++w) one = s.warp[w] > one ? s.warp[w] : one;
+    const unsigned long long mine = one;
+    gather(mine, [&](int, unsigned long long v) { one = v > one ? v : one; });
+    const unsigned long long room = one ? (want - before + one - 1) / one : 1;
+    pick([&](float v, int i) -> unsigned long long { return i < p.vocab && key_of(v) == key && value(v, i) != 0; },
+         [&](unsigned long long) { return room - 1; },
+         [&](int i, float v, unsigned long long) { for (int r = 0; r < ranks; ++r) *cluster.map_shared_rank(&s.threshold, r) = place_of(v, i); });
     cluster.sync();
-    return Kept{key, s.cut};
+    return s.threshold;
   };
 
-  Kept kept{0u, 0x7fffffff};
-  if (top_k > 0 && top_k < p.vocab)
-    kept = search([&](int) { return 1ull; }, [&](unsigned long long) { return static_cast<unsigned long long>(top_k); });
-  if (top_p < 1.0f) {
-    const Kept by_k = kept;
-    const double share = top_p > 0.0f ? static_cast<double>(top_p) : 0.0;
-    kept = search([&](int i) { return by_k(key_of(x[i]), first + i) ? mass_of(x[i]) : 0ull; },
-                  [&](unsigned long long total) { const unsigned long long t = __double2ull_ru(share * __ull2double_rn(total)); return t < 1 ? 1ull : t < total ? t : total; });
+  // Bins of the distance to the maximum.  Subtraction, product and rounding are monotonous, so a bin is a range of the order.  (Halves: a
+  // difference of the largest values stays finite.)
+  const float per_bin = 2.0f * static_cast<float>(BINS) / (SPAN * temperature);
+  auto bin_of = [&](float v) {
+    const float b = (0.5f * top - 0.5f * v) * per_bin;
+    if (v == top) return 0;
+    return b < static_cast<float>(BINS) - 0.5f ? static_cast<int>(__float_as_uint(b + 8388608.0f) & 0xffffu) : BINS;     // (no number, from 0 * inf: out)
+  };
+  auto clear_counts = [&]() { reinterpret_cast<uint4 *>(s.counts)[tid] = make_uint4(0, 0, 0, 0); };
+  // counts of the cluster in the bins 4 tid .. 4 tid + 3, and of all bins in front
+  auto cluster_counts = [&](unsigned int (&c)[4], unsigned long long &before) {
+    c[0] = c[1] = c[2] = c[3] = 0;
+    for (int r = 0; r < ranks; ++r) {
+      const uint4 o = cluster.map_shared_rank(reinterpret_cast<uint4 *>(s.counts), r)[tid];
+      c[0] += o.x; c[1] += o.y; c[2] += o.z; c[3] += o.w;
+    }
+    return block_scan(static_cast<unsigned long long>(c[0]) + c[1] + c[2] + c[3], before);
+  };
+
+  unsigned long long threshold = 0;              // tokens whose place is not below it stay
+  if (top_k > 0 && top_k < p.vocab) {
+    const unsigned long long k = static_cast<unsigned long long>(top_k);
+    each([&](float v, int) { const int b = bin_of(v); if (b < BINS) atomicAdd(&s.counts[b], 1u); });
+    cluster.sync();
+    unsigned int c[4];
+    unsigned long long before;
+    if (cluster_counts(c, before) > k) {         // (otherwise every token that has a mass stays)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (before < k && k <= before + c[j]) { s.bin_hi = 4 * tid + j; s.found[0] = before; s.found[1] = before + c[j]; }
+        before += c[j];
+      }
+      __syncthreads();
+      const int border = s.bin_hi;
+      const unsigned long long above = s.found[0], up_to = s.found[1];
+      if (up_to <= LIST) {
+        const int total = collect([&](float v, int) { return bin_of(v) <= border; });
+        if (rank == 0) finish_list(total, k, 0);
+        cluster.sync();
+        return;
+      }
+      if (up_to - above <= LIST) {
+        collect([&](float v, int) { return bin_of(v) == border; });
+        if (rank == 0) announce(static_cast<int>(k - above));
+        cluster.sync();
+        threshold = s.threshold;
+      } else {
+        threshold = search([&](float, int) { return 1ull; }, [&](unsigned long long) { return k; });
+      }
+    } else {
+      cluster.sync();
+    }
+    clear_counts();
+    if (tid == 0) s.listed = 0;
+    __syncthreads();
   }
-  const double least = min_p > 0.0f ? static_cast<double>(min_p) : 0.0;
-  pick([&](int i) -> unsigned long long {
-         const float v = x[i];
-         return kept(key_of(v), first + i) && (weight(v) >= least || v == top) ? mass_of(v) : 0ull;
-       },
-       [&](unsigned long long total) { return __double2ull_rd(static_cast<double>(u) * __ull2double_rn(total)); },
-       [&](int i, unsigned long long total) {
-         p.tokens[row] = first + i;
-         if (p.logprobs) p.logprobs[row] = static_cast<float>(exponent(x[i]) - log(__ull2double_rn(total) * 0x1p-45));
-       });
+  if (top_p < 1.0f) {
+    unsigned long long sum = 0;
+    each([&](float v, int i) {
+      const int b = bin_of(v);
+      if (b < BINS && place_of(v, i) >= threshold) {
+        atomicAdd(&s.counts[b], 1u);
+        sum += mass(v);
+      }
+    });
+    if (tid == 0) { s.bin_lo = 0; s.bin_hi = BINS - 1; }
+    const unsigned long long own = block_sum(sum);
+    unsigned long long total = 0;
+    gather(own, [&](int, unsigned long long v) { total += v; });
+    const unsigned long long want = share_of(total);
+    // The border's bin from counts alone: a mass in bin j lies between e^-((j + 1/2) d) and e^-((j - 1/2) d), d = SPAN / BINS, up to the rounding of
+    // the bin (2e-5 covers it: 2^-22 of at most 2048 bins) and of the mass.
+    unsigned int c[4];
+    unsigned long long count, low[4], high[4], below, ahead;
+    cluster_counts(c, count);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const double d = static_cast<double>(SPAN) / BINS, at = 4 * tid + j;
+      low[j] = __double2ull_rd(fmax(c[j] * (power_of_two(-1.4426950408889634 * d * (at + 0.5)) * (1.0 - 2e-5) - 0x1p-46), 0.0) * 0x1p45);
+      high[j] = __double2ull_ru(c[j] * (power_of_two(-1.4426950408889634 * d * fmax(at - 0.5, 0.0)) * (1.0 + 2e-5) + 0x1p-46) * 0x1p45);
+    }
+    block_scan((low[0] + low[1]) + (low[2] + low[3]), below);
+    block_scan((high[0] + high[1]) + (high[2] + high[3]), ahead);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (ahead < want) atomicMax(&s.bin_lo, 4 * tid + j);
+      if (below + low[j] >= want) atomicMin(&s.bin_hi, 4 * tid + j);
+      ahead += high[j];
+      below += low[j];
+    }
+    __syncthreads();
+    const int lo = s.bin_lo, hi = s.bin_hi;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      count += c[j];
+      if (4 * tid + j == hi) s.found[0] = count;
+    }
+    __syncthreads();
+    if (s.found[0] <= LIST) {
+      const int listed = collect([&](float v, int i) { return bin_of(v) <= hi && place_of(v, i) >= threshold; });
+      if (rank == 0) finish_list(listed, ~0ull, want);
+      cluster.sync();
+      return;
+    }
+    // The border's bins once more: exact masses in finer bins of their range, and the exact mass in front of them.
+    const float from = lo > 0 ? (static_cast<float>(lo) - 0.5f) / per_bin : 0.0f, finer = per_bin * static_cast<float>(BINS) / static_cast<float>(hi - lo + 1);
+    auto finer_bin = [&](float v) { return min(static_cast<int>(fmaxf(((0.5f * top - 0.5f * v) - from) * finer, 0.0f)), BINS - 1); };
+    for (int b = tid; b < BINS; b += THREADS) s.masses[b] = 0;
+    if (tid == 0) s.bin_lo = -1;
+    __syncthreads();
+    sum = 0;
+    each([&](float v, int i) {
+      const int b = bin_of(v);
+      if (b > hi || place_of(v, i) < threshold) return;
+      if (b < lo) sum += mass(v);
+      else atomicAdd(&s.masses[finer_bin(v)], mass(v));
+    });
+    unsigned long long front = 0, m[4] = {0, 0, 0, 0};
+    gather(block_sum(sum), [&](int, unsigned long long v) { front += v; });
+    for (int r = 0; r < ranks; ++r) {
+      const ulonglong2 *const theirs = cluster.map_shared_rank(reinterpret_cast<ulonglong2 *>(s.masses), r) + 2 * tid;
+      const ulonglong2 a = theirs[0], b = theirs[1];
+      m[0] += a.x; m[1] += a.y; m[2] += b.x; m[3] += b.y;
+    }
+    block_scan((m[0] + m[1]) + (m[2] + m[3]), below);
+    below += front;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (below < want && want <= below + m[j]) { s.bin_lo = 4 * tid + j; s.found[1] = below; }
+      below += m[j];
+    }
+    __syncthreads();
+    const int border = s.bin_lo;
+    int listed = LIST + 1;
+    if (border >= 0) {
+      front = s.found[1];
+      listed = collect([&](float v, int i) {
+        const int b = bin_of(v);
+        return b >= lo && b <= hi && finer_bin(v) == border && place_of(v, i) >= threshold;
+      });
+    }
+    if (listed <= LIST) {
+      if (rank == 0) {
+        unsigned long long w[2], ahead2;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) w[j] = 2 * tid + j < listed ? mass(value_of(s.sorted[2 * tid + j])) : 0;
+        block_scan(w[0] + w[1], ahead2);
+        ahead2 += front;
+        const int stay = __syncthreads_count(2 * tid < listed && ahead2 < want) + __syncthreads_count(2 * tid + 1 < listed && ahead2 + w[0] < want);
+        announce(max(stay, 1));
+      }
+      cluster.sync();
+      threshold = s.threshold;
+    } else {
+      threshold = search([&](float v, int i) { return place_of(v, i) >= threshold ? mass(v) : 0ull; }, [&](unsigned long long) { return want; });
+    }
+  }
+  pick([&](float v, int i) -> unsigned long long { return place_of(v, i) >= threshold ? above_least(v) : 0ull; }, draw_from, write);
   cluster.sync();
 }
 
