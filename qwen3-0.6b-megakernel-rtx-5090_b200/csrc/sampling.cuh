@@ -12,9 +12,8 @@
 //
 // A cluster of CTAs takes a row and keeps it in shared memory as fp32: the row crosses HBM once, however often it is looked at.
 // A threshold (of top-k, of top-p) is found by narrowing down: a histogram of counts over the distance to the maximum, then, where
-// the tokens up to the border's bin are few, a list of them that one CTA sorts and finishes; else the border's bins alone are looked
-// at again (see sample_rows).  Rows whose border lies among more equal values than a list holds go through eight-bit
-// histograms of the keys (search).
+// the tokens up to the border's bin are few, a list of them that one CTA sorts and finishes; else a list of the border's bins alone.  Rows
+// whose border lies among more (nearly) equal values than a list holds go through eight-bit histograms of the keys (search).
 #ifndef QMK_SAMPLING_CUH_
 #define QMK_SAMPLING_CUH_
 
@@ -35,10 +34,12 @@ constexpr int MAX_CLUSTER = 8;
 constexpr int MAX_SLICE = MAX_VOCAB / MAX_CLUSTER;
 constexpr int BINS = 2048;                       // of the distance to the maximum: 4 per thread
 constexpr float SPAN = 32.5f;                    // times the temperature: masses further below the maximum round to nothing (e^-32.5 < 2^-46)
+constexpr float ONE = 8192.0f;                   // a mass of its bin's middle in a histogram of masses: 2^18 of them fit 32 bits
 constexpr int KEY_BINS = 256;                    // of a histogram of keys: eight bits
 constexpr int LIST = 1024;                       // tokens that one CTA sorts
 constexpr int NO_TOKEN = 0x7fffffff;             // pick of a row without a largest value, as in the greedy steps
 constexpr float LARGEST_UNIFORM = 0x1.fffffep-1f;
+constexpr float LARGEST_TEMPERATURE = 0x1p100f;  // (SPAN temperatures and the products with it stay finite)
 static_assert(BINS == 4 * THREADS && LIST == 2 * THREADS, "bins and list entries per thread");
 static_assert(MAX_SLICE <= WARPS * 16 * 128, "a warp's range of the slice is at most 16 groups of 128 tokens");
 
@@ -56,28 +57,27 @@ struct Params {
 };
 
 struct __align__(16) Shared {                   // (the row lies behind it)
-  unsigned int counts[BINS];                     // this CTA's histogram, read by the cluster
+  unsigned int counts[BINS];                     // this CTA's histogram, read by the cluster: tokens, or their masses (see share)
   union {
-    unsigned long long masses[BINS];             // the border's bins once more, by exact mass
     unsigned long long keys[2][KEY_BINS];    // search: histograms in turn, one is read while the next is filled
     unsigned long long sorted[LIST];
   };
   unsigned long long list[LIST];                 // this CTA's candidates
   unsigned long long warp[WARPS], group[WARPS];
-  unsigned long long cta[16];                    // one slot per exchange of the cluster, see gather
+  unsigned long long inbox[16][MAX_CLUSTER];     // one row per exchange of the cluster, see gather
   unsigned long long found[4];
   unsigned long long threshold;                  // written by the CTA that finds it
-  int listed, bin_lo, bin_hi;
+  int listed, collected, bin_lo, bin_hi;
 };
 
-static_assert(sizeof(Shared) % 16 == 0 && offsetof(Shared, masses) % 16 == 0, "vector accesses");
+static_assert(sizeof(Shared) % 16 == 0 && offsetof(Shared, keys) % 16 == 0, "vector accesses");
 
 // Order of the values as whole numbers: larger value, larger key.  (x is not NaN, zeros are +0.)
 __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t u = __float_as_uint(x);
   return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ float clean(float x) { return x == x ? x + 0.0f : -INFINITY; }
+__device__ __forceinline__ float clean(float x) { return fmaxf(x + 0.0f, -INFINITY); }      // (the larger of a NaN and a number is the number)
 __device__ __forceinline__ float load_logit(const float *p) { return clean(*p); }
 __device__ __forceinline__ float load_logit(const __half *p) { return clean(__half2float(*p)); }
 __device__ __forceinline__ float load_logit(const __nv_bfloat16 *p) { return clean(__bfloat162float(*p)); }
@@ -99,22 +99,20 @@ __device__ __forceinline__ float value_of(unsigned long long place) {
 }
 __device__ __forceinline__ int index_of(unsigned long long place) { return static_cast<int>(~static_cast<uint32_t>(place)); }
 
-// 2^t for t <= 0, relative error below 2^-42 (Taylor's series of e^(r ln 2) to the tenth power, |r| <= 1/2): a third of the
-// instructions of exp().  t < -47 gives 0.
+// 2^t for -1000 < t <= 0, relative error below 2^-44: 2^r for |r| <= 1/2 as 1 + r times the polynomial that agrees with (2^r - 1) / r in nine
+// Chebyshev nodes (3.7e-14), a third of the instructions of exp2().
 __device__ __forceinline__ double power_of_two(double t) {
-  if (!(t >= -47.0)) return 0.0;
   const double magic = 6755399441055744.0;       // 1.5 * 2^52: the sum's low word is the nearest whole number
   const double y = t + magic, r = t - (y - magic);
-  double q = 7.05491162080112e-09;               // (ln 2)^k / k!
-  q = fma(q, r, 1.0178086009239699e-07);
-  q = fma(q, r, 1.3215486790144307e-06);
-  q = fma(q, r, 1.5252733804059841e-05);
-  q = fma(q, r, 1.5403530393381608e-04);
-  q = fma(q, r, 1.3333558146428443e-03);
-  q = fma(q, r, 9.618129107628477e-03);
-  q = fma(q, r, 5.550410866482158e-02);
-  q = fma(q, r, 2.402265069591007e-01);
-  q = fma(q, r, 6.931471805599453e-01);
+  double q = 1.0203121063391729e-07;
+  q = fma(q, r, 1.3255224878668817e-06);
+  q = fma(q, r, 1.525268684626772e-05);
+  q = fma(q, r, 0.00015403455852453838);
+  q = fma(q, r, 0.0013333558179043112);
+  q = fma(q, r, 0.009618129159402558);
+  q = fma(q, r, 0.055504108664760424);
+  q = fma(q, r, 0.2402265069581299);
+  q = fma(q, r, 0.6931471805599453);
   q = fma(q, r, 1.0);
   return __hiloint2double(__double2hiint(q) + (__double2loint(y) << 20), __double2loint(q));
 }
@@ -183,19 +181,23 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
   const int first = rank * p.slice, n = max(0, min(p.slice, p.vocab - first));     // this CTA's tokens [first, first + n)
   const int n4 = (n + 3) >> 2;                   // in fours, the last one filled up with -inf
   const float4 *const x4 = reinterpret_cast<const float4 *>(x);
-  const float temperature = p.temperatures ? p.temperatures[row] : p.temperature;
+  const float asked = p.temperatures ? p.temperatures[row] : p.temperature, temperature = fminf(asked, LARGEST_TEMPERATURE);
   const float top_p = p.top_ps ? p.top_ps[row] : p.top_p, min_p = p.min_ps ? p.min_ps[row] : p.min_p;
   const int top_k = p.top_ks ? p.top_ks[row] : p.top_k;
   const float u_raw = p.uniforms[row];
   const double u = u_raw >= 0.0f ? fminf(u_raw, LARGEST_UNIFORM) : 0.0f;
-  int exchange = 0;                              // slots of Shared::cta are used in turn
+  const double slope = 1.4426950408889634 / static_cast<double>(temperature);
+  const double least = min_p > 0.0f ? static_cast<double>(min_p) : 0.0, log_least = least > 0.0 ? log(least) : 0.0;
+  int exchange = 0;                              // rows of Shared::inbox are used in turn
+  cluster.barrier_arrive();                      // (waited for in front of the first store to another CTA)
 
-  // one value of every CTA to every CTA, in the order of the ranks; what the CTA wrote before is there for the others behind it
+  // One value of every CTA to every CTA, in the order of the ranks; what the CTA wrote before is there for the others behind it.  (Written
+  // to the others, whose threads read their own shared memory: eight loads from other SMs one behind the other took 2 us.)
   auto gather = [&](unsigned long long mine, auto &&take) {
     const int slot = exchange++ & 15;
-    if (tid == 0) s.cta[slot] = mine;
+    if (tid < ranks) *cluster.map_shared_rank(&s.inbox[slot][rank], tid) = mine;
     cluster.sync();
-    for (int r = 0; r < ranks; ++r) take(r, *cluster.map_shared_rank(&s.cta[slot], r));
+    for (int r = 0; r < ranks; ++r) take(r, s.inbox[slot][r]);
   };
   // sum over the CTA, to all threads; `before`: of the threads in front of this one
   auto block_sum = [&](unsigned long long v) {
@@ -230,17 +232,11 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
 
   // ---- the row, once; its largest value and where that is first
   for (int b = tid; b < BINS / 4; b += THREADS) reinterpret_cast<uint4 *>(s.counts)[b] = make_uint4(0, 0, 0, 0);
-  if (tid == 0) s.listed = 0;
-  unsigned long long best = 0;
+  if (tid == 0) { s.listed = 0; s.collected = 0; }
+  float high = -INFINITY;                        // the largest this thread has seen
   {
     constexpr int N = Vec<T>::N;
     const T *const src = static_cast<const T *>(p.logits) + row * p.row_stride + first;
-    float high = -INFINITY;
-    int at = first;
-    bool any = false;                            // (a row of -inf: its first token)
-    auto keep = [&](float v, int i) {
-      if (v > high || !any) { high = v; at = first + i; any = true; }
-    };
     int i0 = 0;
     if ((reinterpret_cast<unsigned long long>(src) & 15) == 0) {
       const int nv = n / N;
@@ -249,9 +245,10 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
         float v[N];
         Vec<T>::load(src + i * N, v);
 #pragma unroll
-        for (int j = 0; j < N; j += 4) *reinterpret_cast<float4 *>(x + i * N + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-#pragma unroll
-        for (int j = 0; j < N; ++j) keep(v[j], i * N + j);
+        for (int j = 0; j < N; j += 4) {
+          *reinterpret_cast<float4 *>(x + i * N + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+          high = fmaxf(fmaxf(fmaxf(v[j], v[j + 1]), fmaxf(v[j + 2], v[j + 3])), high);
+        }
       }
       i0 = nv * N;
     }
@@ -259,43 +256,78 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
     for (int i = i0 + tid; i < n; i += THREADS) {
       const float v = load_logit(src + i);
       x[i] = v;
-      keep(v, i);
+      high = fmaxf(high, v);
     }
     if (tid < 4 * n4 - n) x[n + tid] = -INFINITY;
-    if (any) best = place_of(high, at);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-      best = other > best ? other : best;
-    }
+  }
+  float top;
+  {
+    uint32_t best = __reduce_max_sync(0xffffffffu, key_of(high));
     if (lane == 0) s.warp[warp] = best;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) best = s.warp[w] > best ? s.warp[w] : best;
-    const unsigned long long mine = best;
-    gather(mine, [&](int, unsigned long long v) { best = v > best ? v : best; });
+    for (int w = 0; w < WARPS; ++w) best = max(best, static_cast<uint32_t>(s.warp[w]));
+    const uint32_t mine = best;
+    cluster.barrier_wait();
+    gather(mine, [&](int, unsigned long long v) { best = max(best, static_cast<uint32_t>(v)); });
+    top = value_of(static_cast<unsigned long long>(best) << 32);
   }
-  const float top = value_of(best);
+  // A warp has a range of the slice, in groups of 128 tokens; of every group a thread has four.
+  const int seg = (n4 + WARPS * 32 - 1) / (WARPS * 32) * 32, seg_lo = min(n4, warp * seg), seg_hi = min(n4, seg_lo + seg);
+  // every token of the slice: f(value, index)
+  auto each = [&](auto &&f) {
+    for (int i = seg_lo + lane; i < seg_hi; i += 32) {
+      const float4 v = x4[i];
+      const int at = first + 4 * i;
+      f(v.x, at); f(v.y, at + 1); f(v.z, at + 2); f(v.w, at + 3);
+    }
+  };
+  // the same where f has nothing to do for values below `bound`, which most are
+  auto each_from = [&](float bound, auto &&f) {
+    for (int i = seg_lo + lane; i < seg_hi; i += 32) {
+      const float4 v = x4[i];
+      if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= bound)) continue;
+      const int at = first + 4 * i;
+      f(v.x, at); f(v.y, at + 1); f(v.z, at + 2); f(v.w, at + 3);
+    }
+  };
   const bool empty = top == -INFINITY;
-  if (empty || !(temperature > 0.0f) || top_k == 1) {
+  if (empty || !(asked > 0.0f) || top_k == 1) {
+    uint32_t at = 0xffffffffu;
+    if (!empty) each_from(top, [&](float v, int i) { if (v == top) at = min(at, static_cast<uint32_t>(i)); });
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (lane == 0) s.warp[warp] = at;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) at = min(at, static_cast<uint32_t>(s.warp[w]));
+    const uint32_t mine = at;
+    gather(mine, [&](int, unsigned long long v) { at = min(at, static_cast<uint32_t>(v)); });
     if (rank == 0 && tid == 0) {
-      p.tokens[row] = empty ? NO_TOKEN : index_of(best);
+      p.tokens[row] = empty ? NO_TOKEN : static_cast<int>(at);
       if (p.logprobs) p.logprobs[row] = empty ? NAN : 0.0f;
     }
     cluster.sync();                              // (nobody leaves while its shared memory is read)
     return;
   }
+  if (top == INFINITY) {                         // infinite logits share the mass, whatever the others are
+    for (int i = tid; i < 4 * n4; i += THREADS) x[i] = x[i] == INFINITY ? 0.0f : -INFINITY;
+    high = high == INFINITY ? 0.0f : -INFINITY;
+    top = 0.0f;
+    __syncthreads();
+  }
 
-  const double slope = 1.4426950408889634 / static_cast<double>(temperature);
-  // log2 of the mass (differences with infinite values end as 0 mass; infinite maxima share it)
-  auto exponent = [&](float v) { return v == top ? 0.0 : (static_cast<double>(v) - static_cast<double>(top)) * slope; };
-  auto mass = [&](float v) { return mass_of(power_of_two(exponent(v))); };
-  const double least = min_p > 0.0f ? static_cast<double>(min_p) : 0.0, least_exponent = least > 0.0 ? log2(least) - 1e-6 : -1e300;
-  auto above_least = [&](float v) {              // the mass where min_p lets the token stay
-    const double t = exponent(v);
-    if (!(t >= least_exponent)) return 0ull;
-    const double w = power_of_two(t);
-    return w >= least || v == top ? mass_of(w) : 0ull;
+  const double top64 = top;
+  const float nothing = top - 1.01f * SPAN * temperature;      // below it masses round to 0 (and the exponent of 2 may be any)
+  auto weight = [&](float v) { return power_of_two((static_cast<double>(v) - top64) * slope); };
+  auto mass = [&](float v) {                     // (chosen behind the arithmetic: four tokens' run side by side)
+    const unsigned long long m = mass_of(weight(v));
+    return v >= nothing ? m : 0ull;
+  };
+  // min_p: a bound for the values that stay, a little low, and the mass of those that do
+  const float least_value = least > 0.0 ? static_cast<float>(top64 + log_least * static_cast<double>(temperature) * (1.0 + 1e-6) - 1e-6 * fabs(top64)) : -INFINITY;
+  auto above_least = [&](float v) {
+    const double w = weight(v);
+    return v >= nothing && (w >= least || v == top) ? mass_of(w) : 0ull;
   };
   const double share = top_p > 0.0f ? static_cast<double>(top_p) : 0.0;
   auto share_of = [&](unsigned long long total) {        // of the ranks, those in front of which the mass is below this stay
@@ -308,28 +340,17 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
     const double z = v == top ? 0.0 : (static_cast<double>(v) - static_cast<double>(top)) / static_cast<double>(temperature);
     if (p.logprobs) p.logprobs[row] = static_cast<float>(z - log(__ull2double_rn(total) * 0x1p-45));
   };
-  // every token of the slice: f(value, index)
-  auto each = [&](auto &&f) {
-    for (int i = tid; i < n4; i += THREADS) {
-      const float4 v = x4[i];
-      const int at = first + 4 * i;
-      f(v.x, at); f(v.y, at + 1); f(v.z, at + 2); f(v.w, at + 3);
-    }
+  // The lowest index of the row at which the running sum of `value` exceeds `target(total)`; one thread calls found(index, x, total).
+  // Values below `bound` have none.  find: the same where the sums of the warps' ranges are in Shared::warp and `mine` is the CTA's.
+  auto four = [&](float bound, auto &&value, int i, unsigned long long (&v)[4]) {
+    const float4 f = x4[i];
+    const int at = first + 4 * i;
+    v[0] = v[1] = v[2] = v[3] = 0;
+    if (!(fmaxf(fmaxf(f.x, f.y), fmaxf(f.z, f.w)) >= bound)) return;
+    v[0] = value(f.x, at); v[1] = value(f.y, at + 1); v[2] = value(f.z, at + 2); v[3] = value(f.w, at + 3);
   };
-
-  // The lowest index of the row at which the running sum of `value` exceeds `target(total)`; one thread calls found(index, x, total).  A
-  // warp has a range of the slice, in groups of 128 tokens.
-  auto pick = [&](auto &&value, auto &&target, auto &&found) {
-    const int seg = (n4 + WARPS * 32 - 1) / (WARPS * 32) * 32, lo = min(n4, warp * seg), hi = min(n4, lo + seg);
-    auto four = [&](int i, unsigned long long (&v)[4]) {
-      const float4 f = x4[i];
-      const int at = first + 4 * i;
-      v[0] = value(f.x, at); v[1] = value(f.y, at + 1); v[2] = value(f.z, at + 2); v[3] = value(f.w, at + 3);
-    };
-    unsigned long long sum = 0, v[4];
-    for (int i = lo + lane; i < hi; i += 32) { four(i, v); sum += (v[0] + v[1]) + (v[2] + v[3]); }
-    const unsigned long long mine = block_sum(sum);
-    unsigned long long before = 0, total = 0;
+  auto find = [&](unsigned long long mine, float bound, auto &&value, auto &&target, auto &&found) {
+    unsigned long long before = 0, total = 0, v[4];
     gather(mine, [&](int r, unsigned long long c) { before += r < rank ? c : 0; total += c; });
     const unsigned long long want = target(total);
     if (!(before <= want && want < before + mine)) return;     // (the same for every thread of the CTA)
@@ -337,7 +358,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
     for (; w < WARPS - 1 && before + s.warp[w] <= want; ++w) before += s.warp[w];
     const int at = min(n4, w * seg) + warp * 32 + lane;        // warp g: group g of that range
     v[0] = v[1] = v[2] = v[3] = 0;
-    if (warp * 32 < seg && at < n4) four(at, v);
+    if (warp * 32 < seg && at < n4) four(bound, value, at, v);
     const unsigned long long own = (v[0] + v[1]) + (v[2] + v[3]);
     unsigned long long run = own;
 #pragma unroll
@@ -357,37 +378,33 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
       }
     }
   };
+  auto pick = [&](float bound, auto &&value, auto &&target, auto &&found) {
+    unsigned long long sum = 0, v[4];
+    for (int i = seg_lo + lane; i < seg_hi; i += 32) { four(bound, value, i, v); sum += (v[0] + v[1]) + (v[2] + v[3]); }
+    find(block_sum(sum), bound, value, target, found);
+  };
 
-  // The candidates of all CTAs to rank 0, sorted there, largest first; their number.  More than LIST: nothing is sorted.
-  auto collect = [&](auto &&candidate) {
-    each([&](float v, int i) {
-      if (candidate(v, i)) {
-        const int at = atomicAdd(&s.listed, 1);
-        if (at < LIST) s.list[at] = place_of(v, i);
-      }
-    });
+  // Candidates: to the CTA's own list, then (collect) to rank 0's, in any order, where they are sorted, largest first.  Their number in all;
+  // more than LIST: nothing is sorted.  The others have nothing more to give rank 0 then and may leave.
+  auto list = [&](float v, int i) {
+    const int at = atomicAdd(&s.listed, 1);
+    if (at < LIST) s.list[at] = place_of(v, i);
+  };
+  auto collect = [&]() {
     __syncthreads();
-    int total = 0, ahead[MAX_CLUSTER + 1];
-#pragma unroll
-    for (int r = 0; r <= MAX_CLUSTER; ++r) ahead[r] = 0;
-    const int slot = exchange++ & 15;
-    if (tid == 0) s.cta[slot] = static_cast<unsigned long long>(s.listed);
-    cluster.sync();
-#pragma unroll
-    for (int r = 0; r < MAX_CLUSTER; ++r) {
-      ahead[r] = total;
-      if (r < ranks) total += static_cast<int>(min(*cluster.map_shared_rank(&s.cta[slot], r), static_cast<unsigned long long>(MAX_VOCAB)));
+    const int mine = s.listed;
+    if (tid == 0) s.found[3] = mine > 0 ? atomicAdd(cluster.map_shared_rank(&s.collected, 0), mine) : 0;
+    __syncthreads();
+    const unsigned long long base = s.found[3];
+    if (mine > 0 && base + mine <= LIST) {
+      unsigned long long *const to = cluster.map_shared_rank(s.sorted, 0) + base;
+      for (int i = tid; i < mine; i += THREADS) to[i] = s.list[i];
     }
-    ahead[MAX_CLUSTER] = total;
+    int total = 0;
+    gather(mine, [&](int, unsigned long long c) { total += static_cast<int>(c); });
     if (rank == 0 && total <= LIST) {
       int size = 32;
       while (size < total) size <<= 1;
-#pragma unroll
-      for (int r = 0; r < MAX_CLUSTER; ++r) {
-        if (r >= ranks) continue;
-        const unsigned long long *const theirs = cluster.map_shared_rank(s.list, r);
-        for (int i = tid; i < ahead[r + 1] - ahead[r]; i += THREADS) s.sorted[ahead[r] + i] = theirs[i];
-      }
       for (int i = total + tid; i < size; i += THREADS) s.sorted[i] = 0;
       sort_descending(s.sorted, size, tid);
     }
@@ -453,8 +470,10 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
       cluster.sync();
       unsigned long long c = 0, ahead;
       const int bin = KEY_BINS - 1 - tid;
-      if (tid < KEY_BINS)
-        for (int r = 0; r < ranks; ++r) c += cluster.map_shared_rank(hist, r)[bin];
+      if (tid < KEY_BINS) {
+#pragma unroll
+        for (int r = 0; r < MAX_CLUSTER; ++r) c += r < ranks ? cluster.map_shared_rank(hist, r)[bin] : 0;
+      }
       const unsigned long long total = block_scan(c, ahead);
       if (shift == 24) want = target(total);
       if (tid == 0) s.found[0] = s.found[1] = 0;
@@ -478,40 +497,80 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
     const unsigned long long mine = one;
     gather(mine, [&](int, unsigned long long v) { one = v > one ? v : one; });
     const unsigned long long room = one ? (want - before + one - 1) / one : 1;
-    pick([&](float v, int i) -> unsigned long long { return i < p.vocab && key_of(v) == key && value(v, i) != 0; },
+    pick(-INFINITY, [&](float v, int i) -> unsigned long long { return i < p.vocab && key_of(v) == key && value(v, i) != 0; },
          [&](unsigned long long) { return room - 1; },
          [&](int i, float v, unsigned long long) { for (int r = 0; r < ranks; ++r) *cluster.map_shared_rank(&s.threshold, r) = place_of(v, i); });
     cluster.sync();
     return s.threshold;
   };
 
-  // Bins of the distance to the maximum.  Subtraction, product and rounding are monotonous, so a bin is a range of the order.  (Halves: a
-  // difference of the largest values stays finite.)
-  const float per_bin = 2.0f * static_cast<float>(BINS) / (SPAN * temperature);
-  auto bin_of = [&](float v) {
-    const float b = (0.5f * top - 0.5f * v) * per_bin;
-    if (v == top) return 0;
-    return b < static_cast<float>(BINS) - 0.5f ? static_cast<int>(__float_as_uint(b + 8388608.0f) & 0xffffu) : BINS;     // (no number, from 0 * inf: out)
+  // Bins of the distance to the maximum, bin j around j / per_bin.  Differences, products and rounding are monotonous, so a bin is a
+  // range of the order.
+  const float per_bin = fminf(static_cast<float>(BINS) / (SPAN * temperature), 3e38f);
+  auto bin_of = [&](float v) {                   // BINS or more: out
+    const float b = fmaf(top - v, per_bin, 8388608.0f);        // (the last bit is 1: rounded to the nearest whole number)
+    return b < 8388608.0f + BINS ? static_cast<int>(__float_as_uint(b) & 0xffffu) : BINS;
   };
+  // ... and the mass over that of the bin's middle, e^-(d f) with f in [-1/2, 1/2] and d = SPAN / BINS, as 1 - d f (off by 3.2e-5), times ONE and
+  // rounded (6.2e-5)
+  auto bin_and_mass = [&](float v, unsigned int &m) {
+    const float b = fmaf(top - v, per_bin, 8388608.0f), f = fmaf(top - v, per_bin, 8388608.0f - b);
+    m = __float_as_uint(fmaf(f, -SPAN / BINS * ONE, 8388608.0f + ONE)) & 0xffffu;
+    return b < 8388608.0f + BINS ? static_cast<int>(__float_as_uint(b) & 0xffffu) : BINS;
+  };
+  // no value of the bins 0 .. j is below this
+  auto bound_of = [&](int j) { return top - (static_cast<float>(j) + 0.51f) / per_bin * (1.0f + 1e-5f) - 1e-6f * fabsf(top); };
   auto clear_counts = [&]() { reinterpret_cast<uint4 *>(s.counts)[tid] = make_uint4(0, 0, 0, 0); };
   // counts of the cluster in the bins 4 tid .. 4 tid + 3, and of all bins in front
   auto cluster_counts = [&](unsigned int (&c)[4], unsigned long long &before) {
     c[0] = c[1] = c[2] = c[3] = 0;
-    for (int r = 0; r < ranks; ++r) {
-      const uint4 o = cluster.map_shared_rank(reinterpret_cast<uint4 *>(s.counts), r)[tid];
+#pragma unroll
+    for (int r = 0; r < MAX_CLUSTER; ++r) {
+      const uint4 o = r < ranks ? cluster.map_shared_rank(reinterpret_cast<uint4 *>(s.counts), r)[tid] : make_uint4(0, 0, 0, 0);
       c[0] += o.x; c[1] += o.y; c[2] += o.z; c[3] += o.w;
     }
     return block_scan(static_cast<unsigned long long>(c[0]) + c[1] + c[2] + c[3], before);
   };
 
-  unsigned long long threshold = 0;              // tokens whose place is not below it stay
+  // Kept: tokens whose place is not below the threshold.
+  float kept_value = -INFINITY;
+  int kept_index = 0x7fffffff;
+  bool cut = false;
+  auto cut_at = [&](unsigned long long place) { kept_value = value_of(place); kept_index = index_of(place); cut = true; };
+  auto kept = [&](float v, int i) { return v > kept_value || (v == kept_value && i <= kept_index); };
   if (top_k > 0 && top_k < p.vocab) {
     const unsigned long long k = static_cast<unsigned long long>(top_k);
+    unsigned int c[4];
+    unsigned long long before, counted;
+    // Few: the largest values of the threads are k tokens at least down to some bin, which leaves out most others without a look at them.
+    if (top_k <= LIST * 3 / 4 && top_k * 5 <= ranks * THREADS) {
+      const int b = bin_of(high);
+      if (b < BINS) atomicAdd(&s.counts[b], 1u);
+      cluster.sync();
+      counted = cluster_counts(c, before);
+      if (tid == 0) s.bin_hi = BINS - 1;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (before < k && k <= before + c[j]) s.bin_hi = 4 * tid + j;
+        before += c[j];
+      }
+      __syncthreads();
+      const int border = s.bin_hi;
+      each_from(bound_of(border), [&](float v, int i) { if (bin_of(v) <= border) list(v, i); });
+      const int total = collect();
+      if (total <= LIST) {
+        if (rank == 0) finish_list(total, k, 0);
+        return;
+      }
+      clear_counts();
+      if (tid == 0) { s.listed = 0; s.collected = 0; }
+      cluster.sync();
+    }
     each([&](float v, int) { const int b = bin_of(v); if (b < BINS) atomicAdd(&s.counts[b], 1u); });
     cluster.sync();
-    unsigned int c[4];
-    unsigned long long before;
-    if (cluster_counts(c, before) > k) {         // (otherwise every token that has a mass stays)
+    counted = cluster_counts(c, before);
+    if (counted > k) {                           // (otherwise every token that has a mass stays)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (before < k && k <= before + c[j]) { s.bin_hi = 4 * tid + j; s.found[0] = before; s.found[1] = before + c[j]; }
@@ -521,128 +580,141 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
       const int border = s.bin_hi;
       const unsigned long long above = s.found[0], up_to = s.found[1];
       if (up_to <= LIST) {
-        const int total = collect([&](float v, int) { return bin_of(v) <= border; });
+        each_from(bound_of(border), [&](float v, int i) { if (bin_of(v) <= border) list(v, i); });
+        const int total = collect();
         if (rank == 0) finish_list(total, k, 0);
-        cluster.sync();
         return;
       }
       if (up_to - above <= LIST) {
-        collect([&](float v, int) { return bin_of(v) == border; });
+        each_from(bound_of(border), [&](float v, int i) { if (bin_of(v) == border) list(v, i); });
+        collect();
         if (rank == 0) announce(static_cast<int>(k - above));
         cluster.sync();
-        threshold = s.threshold;
+        cut_at(s.threshold);
       } else {
-        threshold = search([&](float, int) { return 1ull; }, [&](unsigned long long) { return k; });
+        cut_at(search([&](float, int) { return 1ull; }, [&](unsigned long long) { return k; }));
       }
     } else {
       cluster.sync();
     }
     clear_counts();
-    if (tid == 0) s.listed = 0;
-    __syncthreads();
+    if (tid == 0) { s.listed = 0; s.collected = 0; }
+    cluster.sync();                              // (rank 0's counter is the others')
   }
   if (top_p < 1.0f) {
     unsigned long long sum = 0;
     each([&](float v, int i) {
-      const int b = bin_of(v);
-      if (b < BINS && place_of(v, i) >= threshold) {
-        atomicAdd(&s.counts[b], 1u);
-        sum += mass(v);
-      }
+      unsigned int q;
+      const int b = bin_and_mass(v, q);
+      const unsigned long long m = mass(v);
+      const bool in = b < BINS && (!cut || kept(v, i));
+      if (in) atomicAdd(&s.counts[b], q);
+      sum += in ? m : 0;
     });
     if (tid == 0) { s.bin_lo = 0; s.bin_hi = BINS - 1; }
     const unsigned long long own = block_sum(sum);
     unsigned long long total = 0;
     gather(own, [&](int, unsigned long long v) { total += v; });
     const unsigned long long want = share_of(total);
-    // The border's bin from counts alone: a mass in bin j lies between e^-((j + 1/2) d) and e^-((j - 1/2) d), d = SPAN / BINS, up to the rounding of
-    // the bin (2e-5 covers it: 2^-22 of at most 2048 bins) and of the mass.
+    // The border's bin, or a few that it may be in: the histogram's sums are off by 1.2e-4 (above, and the rounding of the bin's number), and
+    // masses by 2^-46 each.
     unsigned int c[4];
-    unsigned long long count, low[4], high[4], below, ahead;
-    cluster_counts(c, count);
+    unsigned long long unused, low[4], high[4], below, ahead;
+    cluster_counts(c, unused);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const double d = static_cast<double>(SPAN) / BINS, at = 4 * tid + j;
-      low[j] = __double2ull_rd(fmax(c[j] * (power_of_two(-1.4426950408889634 * d * (at + 0.5)) * (1.0 - 2e-5) - 0x1p-46), 0.0) * 0x1p45);
-      high[j] = __double2ull_ru(c[j] * (power_of_two(-1.4426950408889634 * d * fmax(at - 0.5, 0.0)) * (1.0 + 2e-5) + 0x1p-46) * 0x1p45);
+      const double middle = power_of_two(-1.4426950408889634 * SPAN / BINS * (4 * tid + j)), n_ = c[j] * (1.0 / ONE);
+      low[j] = __double2ull_rd(n_ * fmax(middle * (1.0 - 1.3e-4) - 0x1.1p-46, 0.0) * 0x1p45);
+      high[j] = __double2ull_ru(n_ * (middle * (1.0 + 1.3e-4) + 0x1.1p-46) * 0x1p45);
     }
     block_scan((low[0] + low[1]) + (low[2] + low[3]), below);
     block_scan((high[0] + high[1]) + (high[2] + high[3]), ahead);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (ahead < want) atomicMax(&s.bin_lo, 4 * tid + j);
-      if (below + low[j] >= want) atomicMin(&s.bin_hi, 4 * tid + j);
+      if (ahead < want && want <= ahead + high[j]) s.bin_lo = 4 * tid + j;
+      if (below < want && want <= below + low[j]) s.bin_hi = 4 * tid + j;
       ahead += high[j];
       below += low[j];
     }
     __syncthreads();
     const int lo = s.bin_lo, hi = s.bin_hi;
+    unsigned long long tokens = 0, border_tokens = 0;          // at most: a token is 0.992 ONE at least
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      count += c[j];
-      if (4 * tid + j == hi) s.found[0] = count;
+      if (4 * tid + j <= hi) tokens += c[j];
+      if (4 * tid + j >= lo && 4 * tid + j <= hi) border_tokens += c[j];
     }
-    __syncthreads();
-    if (s.found[0] <= LIST) {
-      const int listed = collect([&](float v, int i) { return bin_of(v) <= hi && place_of(v, i) >= threshold; });
+    const unsigned long long most = static_cast<unsigned long long>(0.99f * ONE) * LIST;
+    const bool few = block_sum(tokens) <= most, few_at_border = block_sum(border_tokens) <= most;
+    if (few) {
+      each_from(bound_of(hi), [&](float v, int i) { if (bin_of(v) <= hi && kept(v, i)) list(v, i); });
+      const int listed = collect();
       if (rank == 0) finish_list(listed, ~0ull, want);
-      cluster.sync();
       return;
     }
-    // The border's bins once more: exact masses in finer bins of their range, and the exact mass in front of them.
-    const float from = lo > 0 ? (static_cast<float>(lo) - 0.5f) / per_bin : 0.0f, finer = per_bin * static_cast<float>(BINS) / static_cast<float>(hi - lo + 1);
-    auto finer_bin = [&](float v) { return min(static_cast<int>(fmaxf(((0.5f * top - 0.5f * v) - from) * finer, 0.0f)), BINS - 1); };
-    for (int b = tid; b < BINS; b += THREADS) s.masses[b] = 0;
-    if (tid == 0) s.bin_lo = -1;
-    __syncthreads();
-    sum = 0;
-    each([&](float v, int i) {
-      const int b = bin_of(v);
-      if (b > hi || place_of(v, i) < threshold) return;
-      if (b < lo) sum += mass(v);
-      else atomicAdd(&s.masses[finer_bin(v)], mass(v));
-    });
-    unsigned long long front = 0, m[4] = {0, 0, 0, 0};
-    gather(block_sum(sum), [&](int, unsigned long long v) { front += v; });
-    for (int r = 0; r < ranks; ++r) {
-      const ulonglong2 *const theirs = cluster.map_shared_rank(reinterpret_cast<ulonglong2 *>(s.masses), r) + 2 * tid;
-      const ulonglong2 a = theirs[0], b = theirs[1];
-      m[0] += a.x; m[1] += a.y; m[2] += b.x; m[3] += b.y;
-    }
-    block_scan((m[0] + m[1]) + (m[2] + m[3]), below);
-    below += front;
+    // rank 0: how many of the sorted candidates stay behind the mass `front`
+    auto announce_share = [&](int listed, unsigned long long front) {
+      unsigned long long w[2], before;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (below < want && want <= below + m[j]) { s.bin_lo = 4 * tid + j; s.found[1] = below; }
-      below += m[j];
-    }
-    __syncthreads();
-    const int border = s.bin_lo;
-    int listed = LIST + 1;
-    if (border >= 0) {
-      front = s.found[1];
-      listed = collect([&](float v, int i) {
-        const int b = bin_of(v);
-        return b >= lo && b <= hi && finer_bin(v) == border && place_of(v, i) >= threshold;
-      });
-    }
-    if (listed <= LIST) {
-      if (rank == 0) {
-        unsigned long long w[2], ahead2;
+      for (int j = 0; j < 2; ++j) w[j] = 2 * tid + j < listed ? mass(value_of(s.sorted[2 * tid + j])) : 0;
+      block_scan(w[0] + w[1], before);
+      before += front;
+      const int stay = __syncthreads_count(2 * tid < listed && before < want) + __syncthreads_count(2 * tid + 1 < listed && before + w[0] < want);
+      announce(max(stay, 1));
+    };
+    // The mass in front of the border's bins, exactly, and their tokens.
+    unsigned long long front = 0;
+    sum = 0;
+    each_from(bound_of(hi), [&](float v, int i) {
+      const int b = bin_of(v);
+      const bool in = b <= hi && kept(v, i);
+      if (in && b >= lo && few_at_border) list(v, i);
+      const unsigned long long m = mass(v);
+      sum += in && b < lo ? m : 0;
+    });
+    const unsigned long long mine = block_sum(sum), ranges = warp_sum(sum);
+    gather(mine, [&](int, unsigned long long v) { front += v; });
+    if (few_at_border) {
+      const int listed = collect();
+      if (rank == 0) {                           // how many of them stay
+        unsigned long long w[2], before;
 #pragma unroll
         for (int j = 0; j < 2; ++j) w[j] = 2 * tid + j < listed ? mass(value_of(s.sorted[2 * tid + j])) : 0;
-        block_scan(w[0] + w[1], ahead2);
-        ahead2 += front;
-        const int stay = __syncthreads_count(2 * tid < listed && ahead2 < want) + __syncthreads_count(2 * tid + 1 < listed && ahead2 + w[0] < want);
+        block_scan(w[0] + w[1], before);
+        before += front;
+        const int stay = __syncthreads_count(2 * tid < listed && before < want) + __syncthreads_count(2 * tid + 1 < listed && before + w[0] < want);
         announce(max(stay, 1));
       }
       cluster.sync();
-      threshold = s.threshold;
-    } else {
-      threshold = search([&](float v, int i) { return place_of(v, i) >= threshold ? mass(v) : 0ull; }, [&](unsigned long long) { return want; });
+      cut_at(s.threshold);
+      if (least == 0.0 || weight(kept_value) >= least) {       // (min_p takes nothing away) the ranges' sums are there but for the listed tokens that stay
+        if (lane == 0) s.group[warp] = ranges;
+        __syncthreads();
+        sum = 0;
+        for (int i = tid; i < s.listed; i += THREADS) {
+          const float v = value_of(s.list[i]);
+          const int at = index_of(s.list[i]);
+          const unsigned long long m = kept(v, at) ? mass(v) : 0;
+          sum += m;
+          if (m) atomicAdd(&s.group[((at - first) >> 2) / seg], m);
+        }
+        const unsigned long long own_mass = mine + block_sum(sum);
+        __syncthreads();
+        if (tid < WARPS) s.warp[tid] = s.group[tid];
+        __syncthreads();
+        find(own_mass, kept_value, [&](float v, int i) -> unsigned long long { const unsigned long long m = mass(v); return kept(v, i) ? m : 0ull; }, draw_from, write);
+        cluster.sync();
+        return;
+      }
+    } else {                                     // (many equal values, or a very flat row)
+      cut_at(search([&](float v, int i) { const int b = bin_of(v); return b >= lo && b <= hi && kept(v, i) ? mass(v) : 0ull; },
+                    [&](unsigned long long) { return want - front; }));
     }
   }
-  pick([&](float v, int i) -> unsigned long long { return place_of(v, i) >= threshold ? above_least(v) : 0ull; }, draw_from, write);
+  if (cut || least > 0.0)
+    pick(fmaxf(kept_value, least_value), [&](float v, int i) -> unsigned long long { const unsigned long long m = above_least(v); return kept(v, i) ? m : 0ull; }, draw_from, write);
+  else
+    pick(-INFINITY, [&](float v, int) { return mass(v); }, draw_from, write);
   cluster.sync();
 }
 
