@@ -10,7 +10,9 @@
 // moves a border of the cumulative distribution by 2^-46 a token, where 32-bit floating sums would move it by up to 2^-24 of the total,
 // more than a token in the tail of a large vocabulary has.
 //
-// A cluster of CTAs takes a row and keeps it in shared memory as fp32: the row crosses HBM once, however often it is looked at.
+// A cluster of CTAs takes a row, as many as leave every row's CTAs resident together.  A row is read from one to three times; it crosses
+// HBM the first time, and is in L1 or L2 then.  (Rows kept in shared memory as fp32 needed clusters of eight for 151,936 tokens, so 128
+// rows four waves of CTAs in lockstep: 76 us for the plain draw and 88 with top-k, where two CTAs a row without it take XXX and YYY.)
 // A threshold (of top-k, of top-p) is found by narrowing down: a histogram of counts over the distance to the maximum, then, where
 // the tokens up to the border's bin are few, a list of them that one CTA sorts and finishes; else a list of the border's bins alone.  Rows
 // whose border lies among more (nearly) equal values than a list holds go through eight-bit histograms of the keys (search).
@@ -31,22 +33,24 @@ namespace cg = cooperative_groups;
 constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int MAX_VOCAB = 1 << 18;               // masses of at most 2^45 in 63 bits
 constexpr int MAX_CLUSTER = 8;
-constexpr int MAX_SLICE = MAX_VOCAB / MAX_CLUSTER;
+constexpr int GROUPS = (MAX_VOCAB / 4 + 1 + WARPS * 32 - 1) / (WARPS * 32);   // of 128 tokens, in a warp's range of a row: at most
 constexpr int BINS = 2048;                       // of the distance to the maximum: 4 per thread
 constexpr float SPAN = 32.5f;                    // times the temperature: masses further below the maximum round to nothing (e^-32.5 < 2^-46)
 constexpr float ONE = 8192.0f;                   // a mass of its bin's middle in a histogram of masses: 2^18 of them fit 32 bits
 constexpr int KEY_BINS = 256;                    // of a histogram of keys: eight bits
-constexpr int LIST = 1024;                       // tokens that one CTA sorts
+constexpr int LIST = 2048;                       // tokens that one CTA sorts: EACH per thread
+constexpr int STEPS = 64, COLUMNS = 16;            // of the table of powers, see power_polynomial
+constexpr int TURN = 3;                           // fours that a thread has in each of two turns of its ring
 constexpr int NO_TOKEN = 0x7fffffff;             // pick of a row without a largest value, as in the greedy steps
 constexpr float LARGEST_UNIFORM = 0x1.fffffep-1f;
 constexpr float LARGEST_TEMPERATURE = 0x1p100f;  // (SPAN temperatures and the products with it stay finite)
-static_assert(BINS == 4 * THREADS && LIST == 2 * THREADS, "bins and list entries per thread");
-static_assert(MAX_SLICE <= WARPS * 16 * 128, "a warp's range of the slice is at most 16 groups of 128 tokens");
+constexpr int EACH = LIST / THREADS;
+static_assert(BINS == 4 * THREADS && LIST == 4 * THREADS, "bins and list entries per thread");
 
 struct Params {
   const void *logits;
   long long row_stride;                          // elements
-  int vocab, slice;                              // slice: tokens a CTA of the cluster keeps
+  int vocab;
   const float *uniforms;
   const float *temperatures, *top_ps, *min_ps;   // per row, or null: the scalar for all
   const int *top_ks;
@@ -56,14 +60,15 @@ struct Params {
   float *logprobs;                               // may be null
 };
 
-struct __align__(16) Shared {                   // (the row lies behind it)
+struct __align__(16) Shared {
   unsigned int counts[BINS];                     // this CTA's histogram, read by the cluster: tokens, or their masses (see share)
   union {
     unsigned long long keys[2][KEY_BINS];    // search: histograms in turn, one is read while the next is filled
     unsigned long long sorted[LIST];
   };
   unsigned long long list[LIST];                 // this CTA's candidates
-  unsigned long long warp[WARPS], group[WARPS];
+  double powers[STEPS * COLUMNS];                // 2^(j / 64), a column for each lane of half a warp
+  unsigned long long warp[WARPS], warp_kept[WARPS], group[GROUPS];
   unsigned long long inbox[16][MAX_CLUSTER];     // one row per exchange of the cluster, see gather
   unsigned long long found[4];
   unsigned long long threshold;                  // written by the CTA that finds it
@@ -72,15 +77,15 @@ struct __align__(16) Shared {                   // (the row lies behind it)
 
 static_assert(sizeof(Shared) % 16 == 0 && offsetof(Shared, keys) % 16 == 0, "vector accesses");
 
-// Order of the values as whole numbers: larger value, larger key.  (x is not NaN, zeros are +0.)
+// Order of the values as whole numbers: larger value, larger key, zeros of both signs the same.  (x is not NaN.)
 __device__ __forceinline__ uint32_t key_of(float x) {
-  const uint32_t u = __float_as_uint(x);
+  const uint32_t u = __float_as_uint(x + 0.0f);
   return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ float clean(float x) { return fmaxf(x + 0.0f, -INFINITY); }      // (the larger of a NaN and a number is the number)
-__device__ __forceinline__ float load_logit(const float *p) { return clean(*p); }
-__device__ __forceinline__ float load_logit(const __half *p) { return clean(__half2float(*p)); }
-__device__ __forceinline__ float load_logit(const __nv_bfloat16 *p) { return clean(__bfloat162float(*p)); }
+// A logit that is no number is left as it is by the loads: maxima pass over it and no comparison holds for it.
+__device__ __forceinline__ float as_float(float x) { return x; }
+__device__ __forceinline__ float as_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
 template <typename V>
 __device__ __forceinline__ V warp_sum(V v) {
@@ -99,37 +104,30 @@ __device__ __forceinline__ float value_of(unsigned long long place) {
 }
 __device__ __forceinline__ int index_of(unsigned long long place) { return static_cast<int>(~static_cast<uint32_t>(place)); }
 
-// 2^t for -1000 < t <= 0, relative error below 2^-44: 2^r for |r| <= 1/2 as 1 + r times the polynomial that agrees with (2^r - 1) / r in nine
-// Chebyshev nodes (3.7e-14), a third of the instructions of exp2().
-__device__ __forceinline__ double power_of_two(double t) {
-  const double magic = 6755399441055744.0;       // 1.5 * 2^52: the sum's low word is the nearest whole number
-  const double y = t + magic, r = t - (y - magic);
-  double q = 1.0203121063391729e-07;
-  q = fma(q, r, 1.3255224878668817e-06);
-  q = fma(q, r, 1.525268684626772e-05);
-  q = fma(q, r, 0.00015403455852453838);
-  q = fma(q, r, 0.0013333558179043112);
-  q = fma(q, r, 0.009618129159402558);
-  q = fma(q, r, 0.055504108664760424);
-  q = fma(q, r, 0.2402265069581299);
-  q = fma(q, r, 0.6931471805599453);
-  q = fma(q, r, 1.0);
-  return __hiloint2double(__double2hiint(q) + (__double2loint(y) << 20), __double2loint(q));
+// 2^(y / 64) for whole-number and fractional parts y = 64 n + j + r, |r| <= 1/2: 2^n times a table's 2^(j / 64) times 1 + r times the polynomial that agrees with
+// (2^(r / 64) - 1) / r in four Chebyshev nodes (relative error 5e-15, the table's 2^-53).  A table halves the fp64 instructions, which the sums of
+// masses are bound by: 15 a token without it, 9 with it.  Every half of a warp has columns of its own, so that lookups never collide.
+__device__ __forceinline__ double power_polynomial(double r) {
+  double q = 5.732857292414682e-10;
+  q = fma(q, r, 2.1173168200092995e-07);
+  q = fma(q, r, 5.864904955054418e-05);
+  q = fma(q, r, 0.010830424696239445);
+  return fma(q, r, 1.0);
 }
-// round(w * 2^45) for w in [0, 1]: the last bit of w + 2^7 is 2^-45
-__device__ __forceinline__ unsigned long long mass_of(double w) {
-  return static_cast<unsigned long long>(__double_as_longlong(w + 128.0)) - 0x4060000000000000ull;
+// round(w * 2^45) for w in [0, 1] from w + 2^7, whose last bit is 2^-45
+__device__ __forceinline__ unsigned long long mass_of(double w_and_128) {
+  return static_cast<unsigned long long>(__double_as_longlong(w_and_128)) - 0x4060000000000000ull;
 }
 
-// Bitonic sort of `size` entries (a power of two, 32 to 2 THREADS), largest first, by the whole CTA; a short one by its first warp.
+// Bitonic sort of `size` entries (a power of two, 32 to LIST), largest first, by the whole CTA; a short one by its first warp.
 __device__ __forceinline__ void sort_descending(unsigned long long *v, int size, int tid) {
   __syncthreads();
   const bool short_one = size <= 64;
   if (!short_one || tid < 32) {
     for (int block = 2; block <= size; block <<= 1)
       for (int step = block >> 1; step > 0; step >>= 1) {
-        const int i = 2 * tid - (tid & (step - 1)), j = i + step;
-        if (j < size) {
+        for (int pair = tid; pair < size >> 1; pair += THREADS) {
+          const int i = 2 * pair - (pair & (step - 1)), j = i + step;
           const unsigned long long a = v[i], b = v[j];
           if ((a < b) == ((i & block) == 0)) { v[i] = b; v[j] = a; }
         }
@@ -139,54 +137,96 @@ __device__ __forceinline__ void sort_descending(unsigned long long *v, int size,
   __syncthreads();
 }
 
-// 16 bytes of logits as values
-template <typename T> struct Vec;
-template <> struct Vec<float> {
-  static constexpr int N = 4;
-  static __device__ __forceinline__ void load(const float *p, float (&v)[4]) {
-    const float4 a = __ldg(reinterpret_cast<const float4 *>(p));
-    v[0] = clean(a.x); v[1] = clean(a.y); v[2] = clean(a.z); v[3] = clean(a.w);
-  }
-};
-template <> struct Vec<__half> {
-  static constexpr int N = 8;
-  static __device__ __forceinline__ void load(const __half *p, float (&v)[8]) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-      v[2 * i] = clean(f.x); v[2 * i + 1] = clean(f.y);
-    }
-  }
-};
-template <> struct Vec<__nv_bfloat16> {
-  static constexpr int N = 8;
-  static __device__ __forceinline__ void load(const __nv_bfloat16 *p, float (&v)[8]) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { v[2 * i] = clean(__uint_as_float(w[i] << 16)); v[2 * i + 1] = clean(__uint_as_float(w[i] & 0xffff0000u)); }
-  }
-};
+// Four logits from an address that is a multiple of their size
+__device__ __forceinline__ float4 load_four(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+__device__ __forceinline__ float4 load_four(const __half *p) {
+  const uint2 a = *reinterpret_cast<const uint2 *>(p);
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&a.x)), g = __half22float2(*reinterpret_cast<const __half2 *>(&a.y));
+  return make_float4(f.x, f.y, g.x, g.y);
+}
+__device__ __forceinline__ float4 load_four(const __nv_bfloat16 *p) {
+  const uint2 a = *reinterpret_cast<const uint2 *>(p);
+  return make_float4(__uint_as_float(a.x << 16), __uint_as_float(a.x & 0xffff0000u), __uint_as_float(a.y << 16), __uint_as_float(a.y & 0xffff0000u));
+}
+// ... to shared memory, on their way until the thread waits for them
+template <typename T>
+__device__ __forceinline__ void copy_four(unsigned char *to, const T *from) {
+  const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+  if (sizeof(T) == 4) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(from) : "memory");
+}
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
-  extern __shared__ __align__(16) unsigned char smem_raw[];
-  Shared &s = *reinterpret_cast<Shared *>(smem_raw);
-  float *const x = reinterpret_cast<float *>(smem_raw + sizeof(Shared));
+  extern __shared__ __align__(16) unsigned char smem[];
+  Shared &s = *reinterpret_cast<Shared *>(smem);
+  unsigned char *const ring = smem + sizeof(Shared);
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int row = static_cast<int>(blockIdx.x) / ranks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int first = rank * p.slice, n = max(0, min(p.slice, p.vocab - first));     // this CTA's tokens [first, first + n)
-  const int n4 = (n + 3) >> 2;                   // in fours, the last one filled up with -inf
-  const float4 *const x4 = reinterpret_cast<const float4 *>(x);
+  // Tokens go in fours, each four within one aligned piece of memory: the first and the last of a row may be in part outside (-inf).  This CTA's
+  // fours are [0, n4), four i begins with token first + 4 i; a warp has a range of them, in groups of 32 (128 tokens), of a group a thread has one.
+  const T *const src = static_cast<const T *>(p.logits) + row * p.row_stride;
+  const int off = static_cast<int>(reinterpret_cast<unsigned long long>(src) / sizeof(T) & 3), fours = (p.vocab + off + 3) >> 2;
+  const int per_rank = (fours + ranks - 1) / ranks, first = 4 * rank * per_rank - off, n4 = max(0, min(per_rank, fours - rank * per_rank));
+  const int seg = (n4 + WARPS * 32 - 1) / (WARPS * 32) * 32, seg_lo = min(n4, warp * seg), seg_hi = min(n4, seg_lo + seg);
+  const int whole_lo = first < 0 ? 1 : 0, whole_hi = first + 4 * n4 > p.vocab ? n4 - 1 : n4;        // fours [whole_lo, whole_hi) are all inside
+  bool infinite = false;                         // the largest value is: it counts as 0 and everything else as -inf
+  auto counted = [&](float4 v) {
+    if (infinite) v = make_float4(v.x == INFINITY ? 0.0f : -INFINITY, v.y == INFINITY ? 0.0f : -INFINITY, v.z == INFINITY ? 0.0f : -INFINITY, v.w == INFINITY ? 0.0f : -INFINITY);
+    return v;
+  };
+  auto fetch = [&](int i) {
+    const int at = first + 4 * i;
+    if (i >= whole_lo && i < whole_hi) return counted(load_four(src + at));
+    return counted(make_float4(at >= 0 ? as_float(src[at]) : -INFINITY, at + 1 >= 0 && at + 1 < p.vocab ? as_float(src[at + 1]) : -INFINITY,
+                               at + 2 >= 0 && at + 2 < p.vocab ? as_float(src[at + 2]) : -INFINITY, at + 3 < p.vocab ? as_float(src[at + 3]) : -INFINITY));
+  };
+  // f(values, four, which of 0 .. TURN - 1 in turn) for this thread's fours.  A thread copies them to slots of its own in shared memory, TURN at a time, the
+  // next ones under way while these are worked on.
+  auto walk = [&](auto &&f) {
+    constexpr int SLOT = THREADS * 4 * sizeof(T);
+    int i = seg_lo + lane;
+    if (seg_lo < whole_lo && seg_lo < seg_hi) {  // (the row's first four, not all of it inside: its group by itself)
+      if (i < seg_hi) f(fetch(i), i, 0);
+      i += 32;
+    }
+    const int whole = min(seg_hi, whole_hi), steps = whole > i ? (whole - i + 31) >> 5 : 0;      // (of this thread)
+    const T *from = src + (first + 4 * i);
+    unsigned char *slots = ring + tid * (4 * sizeof(T));
+    auto copy = [&](int k, unsigned char *to) {
+#pragma unroll
+      for (int j = 0; j < TURN; ++j)
+        if (k + j < steps) copy_four(to + j * SLOT, from + 128 * (k + j));
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    copy(0, slots);
+    copy(TURN, slots + TURN * SLOT);
+    int k = 0;
+    unsigned char *here = slots, *there = slots + TURN * SLOT;
+    for (; k + TURN <= steps; k += TURN) {
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+#pragma unroll
+      for (int j = 0; j < TURN; ++j) f(counted(load_four(reinterpret_cast<const T *>(here + j * SLOT))), i + 32 * (k + j), j);
+      copy(k + 2 * TURN, here);
+      unsigned char *const next = there;
+      there = here;
+      here = next;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < TURN - 1; ++j)
+      if (k + j < steps) f(counted(load_four(reinterpret_cast<const T *>(here + j * SLOT))), i + 32 * (k + j), j);
+    i += 32 * steps;
+    if (i < seg_hi) f(fetch(i), i, 0);           // (the row's last four)
+    __syncwarp();
+  };
   const float asked = p.temperatures ? p.temperatures[row] : p.temperature, temperature = fminf(asked, LARGEST_TEMPERATURE);
   const float top_p = p.top_ps ? p.top_ps[row] : p.top_p, min_p = p.min_ps ? p.min_ps[row] : p.min_p;
   const int top_k = p.top_ks ? p.top_ks[row] : p.top_k;
   const float u_raw = p.uniforms[row];
   const double u = u_raw >= 0.0f ? fminf(u_raw, LARGEST_UNIFORM) : 0.0f;
-  const double slope = 1.4426950408889634 / static_cast<double>(temperature);
+  const double slope = STEPS * 1.4426950408889634 / static_cast<double>(temperature);       // 64ths of powers of two per unit of a logit
   const double least = min_p > 0.0f ? static_cast<double>(min_p) : 0.0, log_least = least > 0.0 ? log(least) : 0.0;
   int exchange = 0;                              // rows of Shared::inbox are used in turn
   cluster.barrier_arrive();                      // (waited for in front of the first store to another CTA)
@@ -233,36 +273,12 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
   // ---- the row, once; its largest value and where that is first
   for (int b = tid; b < BINS / 4; b += THREADS) reinterpret_cast<uint4 *>(s.counts)[b] = make_uint4(0, 0, 0, 0);
   if (tid == 0) { s.listed = 0; s.collected = 0; }
-  float high = -INFINITY;                        // the largest this thread has seen
-  {
-    constexpr int N = Vec<T>::N;
-    const T *const src = static_cast<const T *>(p.logits) + row * p.row_stride + first;
-    int i0 = 0;
-    if ((reinterpret_cast<unsigned long long>(src) & 15) == 0) {
-      const int nv = n / N;
-#pragma unroll 4
-      for (int i = tid; i < nv; i += THREADS) {
-        float v[N];
-        Vec<T>::load(src + i * N, v);
-#pragma unroll
-        for (int j = 0; j < N; j += 4) {
-          *reinterpret_cast<float4 *>(x + i * N + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-          high = fmaxf(fmaxf(fmaxf(v[j], v[j + 1]), fmaxf(v[j + 2], v[j + 3])), high);
-        }
-      }
-      i0 = nv * N;
-    }
-#pragma unroll 8
-    for (int i = i0 + tid; i < n; i += THREADS) {
-      const float v = load_logit(src + i);
-      x[i] = v;
-      high = fmaxf(high, v);
-    }
-    if (tid < 4 * n4 - n) x[n + tid] = -INFINITY;
-  }
+  for (int i = tid; i < STEPS * COLUMNS; i += THREADS) s.powers[i] = exp2(static_cast<double>(i / COLUMNS) / STEPS);      // (read behind the first barrier)
+  float high[TURN] = {-INFINITY, -INFINITY, -INFINITY};          // the largest values of three parts of what this thread has seen
+  walk([&](float4 v, int, int j) { high[j] = fmaxf(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), high[j]); });
   float top;
   {
-    uint32_t best = __reduce_max_sync(0xffffffffu, key_of(high));
+    uint32_t best = __reduce_max_sync(0xffffffffu, key_of(fmaxf(fmaxf(high[0], high[1]), high[2])));
     if (lane == 0) s.warp[warp] = best;
     __syncthreads();
 #pragma unroll
@@ -272,24 +288,20 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
     gather(mine, [&](int, unsigned long long v) { best = max(best, static_cast<uint32_t>(v)); });
     top = value_of(static_cast<unsigned long long>(best) << 32);
   }
-  // A warp has a range of the slice, in groups of 128 tokens; of every group a thread has four.
-  const int seg = (n4 + WARPS * 32 - 1) / (WARPS * 32) * 32, seg_lo = min(n4, warp * seg), seg_hi = min(n4, seg_lo + seg);
-  // every token of the slice: f(value, index)
+  // every token of this CTA: f(value, index)
   auto each = [&](auto &&f) {
-    for (int i = seg_lo + lane; i < seg_hi; i += 32) {
-      const float4 v = x4[i];
+    walk([&](float4 v, int i, int) {
       const int at = first + 4 * i;
       f(v.x, at); f(v.y, at + 1); f(v.z, at + 2); f(v.w, at + 3);
-    }
+    });
   };
   // the same where f has nothing to do for values below `bound`, which most are
   auto each_from = [&](float bound, auto &&f) {
-    for (int i = seg_lo + lane; i < seg_hi; i += 32) {
-      const float4 v = x4[i];
-      if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= bound)) continue;
+    walk([&](float4 v, int i, int) {
+      if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= bound)) return;
       const int at = first + 4 * i;
       f(v.x, at); f(v.y, at + 1); f(v.z, at + 2); f(v.w, at + 3);
-    }
+    });
   };
   const bool empty = top == -INFINITY;
   if (empty || !(asked > 0.0f) || top_k == 1) {
@@ -310,24 +322,36 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
     return;
   }
   if (top == INFINITY) {                         // infinite logits share the mass, whatever the others are
-    for (int i = tid; i < 4 * n4; i += THREADS) x[i] = x[i] == INFINITY ? 0.0f : -INFINITY;
-    high = high == INFINITY ? 0.0f : -INFINITY;
+    infinite = true;
     top = 0.0f;
-    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < TURN; ++j) high[j] = high[j] == INFINITY ? 0.0f : -INFINITY;
   }
 
   const double top64 = top;
   const float nothing = top - 1.01f * SPAN * temperature;      // below it masses round to 0 (and the exponent of 2 may be any)
-  auto weight = [&](float v) { return power_of_two((static_cast<double>(v) - top64) * slope); };
+  const double *const powers = s.powers + (lane & (COLUMNS - 1));
+  // 2^n 2^(j / 64) and the polynomial whose product is the mass of v
+  auto factors = [&](float v, double &power) {
+    constexpr double magic = 6755399441055744.0;             // 1.5 * 2^52: the sum's low word is the nearest whole number
+    const double d = static_cast<double>(v) - top64, y = fma(d, slope, magic);
+    const int k = __double2loint(y);
+    const double p = powers[(k & (STEPS - 1)) * COLUMNS];
+    power = __hiloint2double(__double2hiint(p) + ((k >> 6) << 20), __double2loint(p));
+    return power_polynomial(fma(d, slope, -(y - magic)));
+  };
+  auto weight = [&](float v) { double power; const double q = factors(v, power); return power * q; };
   auto mass = [&](float v) {                     // (chosen behind the arithmetic: four tokens' run side by side)
-    const unsigned long long m = mass_of(weight(v));
+    double power;
+    const double q = factors(v, power);
+    const unsigned long long m = mass_of(fma(power, q, 128.0));
     return v >= nothing ? m : 0ull;
   };
   // min_p: a bound for the values that stay, a little low, and the mass of those that do
   const float least_value = least > 0.0 ? static_cast<float>(top64 + log_least * static_cast<double>(temperature) * (1.0 + 1e-6) - 1e-6 * fabs(top64)) : -INFINITY;
   auto above_least = [&](float v) {
-    const double w = weight(v);
-    return v >= nothing && (w >= least || v == top) ? mass_of(w) : 0ull;
+    const unsigned long long m = mass(v);
+    return weight(v) >= least || v == top ? m : 0ull;
   };
   const double share = top_p > 0.0f ? static_cast<double>(top_p) : 0.0;
   auto share_of = [&](unsigned long long total) {        // of the ranks, those in front of which the mass is below this stay
@@ -341,47 +365,69 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
     if (p.logprobs) p.logprobs[row] = static_cast<float>(z - log(__ull2double_rn(total) * 0x1p-45));
   };
   // The lowest index of the row at which the running sum of `value` exceeds `target(total)`; one thread calls found(index, x, total).
-  // Values below `bound` have none.  find: the same where the sums of the warps' ranges are in Shared::warp and `mine` is the CTA's.
-  auto four = [&](float bound, auto &&value, int i, unsigned long long (&v)[4]) {
-    const float4 f = x4[i];
+  // Values below `bound` have none.  find: the same where the sums of the warps' ranges are in `sums` and `mine` is the CTA's.
+  auto four = [&](float bound, auto &&value, int i, unsigned long long (&v)[4], const float4 f) {
     const int at = first + 4 * i;
     v[0] = v[1] = v[2] = v[3] = 0;
     if (!(fmaxf(fmaxf(f.x, f.y), fmaxf(f.z, f.w)) >= bound)) return;
     v[0] = value(f.x, at); v[1] = value(f.y, at + 1); v[2] = value(f.z, at + 2); v[3] = value(f.w, at + 3);
   };
-  auto find = [&](unsigned long long mine, float bound, auto &&value, auto &&target, auto &&found) {
+  auto warp_scan = [&](unsigned long long v) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long up = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += up;
+    }
+    return v;
+  };
+  auto find = [&](unsigned long long mine, const unsigned long long *sums, float bound, auto &&value, auto &&target, auto &&found) {
     unsigned long long before = 0, total = 0, v[4];
+    float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     gather(mine, [&](int r, unsigned long long c) { before += r < rank ? c : 0; total += c; });
     const unsigned long long want = target(total);
     if (!(before <= want && want < before + mine)) return;     // (the same for every thread of the CTA)
     int w = 0;
-    for (; w < WARPS - 1 && before + s.warp[w] <= want; ++w) before += s.warp[w];
-    const int at = min(n4, w * seg) + warp * 32 + lane;        // warp g: group g of that range
-    v[0] = v[1] = v[2] = v[3] = 0;
-    if (warp * 32 < seg && at < n4) four(bound, value, at, v);
-    const unsigned long long own = (v[0] + v[1]) + (v[2] + v[3]);
-    unsigned long long run = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long up = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += up;
+    for (; w < WARPS - 1 && before + sums[w] <= want; ++w) before += sums[w];
+    const int lo = min(n4, w * seg), hi = min(n4, lo + seg), groups = (hi - lo + 31) >> 5;
+    for (int g = warp; g < groups; g += WARPS) {
+      v[0] = v[1] = v[2] = v[3] = 0;
+      if (lo + 32 * g + lane < hi) four(bound, value, lo + 32 * g + lane, v, fetch(lo + 32 * g + lane));
+      const unsigned long long sum = warp_sum((v[0] + v[1]) + (v[2] + v[3]));
+      if (lane == 0) s.group[g] = sum;
     }
-    if (lane == 31) s.group[warp] = run;
     __syncthreads();
-    for (int g = 0; g < warp; ++g) before += s.group[g];
-    before += run - own;
-    if (before <= want && want < before + own) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (before <= want && want < before + v[j]) found(first + 4 * at + j, x[4 * at + j], total);
-        before += v[j];
+    if (warp != 0) return;
+    int g = 0;
+    for (int g0 = 0; g0 < groups; g0 += 32) {                  // the group
+      const unsigned long long sum = g0 + lane < groups ? s.group[g0 + lane] : 0, run = warp_scan(sum);
+      const unsigned int over = __ballot_sync(0xffffffffu, want < before + run);
+      if (over) {
+        g = g0 + __ffs(over) - 1;
+        before += __shfl_sync(0xffffffffu, run - sum, __ffs(over) - 1);
+        break;
       }
+      before += __shfl_sync(0xffffffffu, run, 31);
+    }
+    v[0] = v[1] = v[2] = v[3] = 0;
+    const int i = lo + 32 * g + lane;
+    if (i < hi) { f = fetch(i); four(bound, value, i, v, f); }
+    const unsigned long long own = (v[0] + v[1]) + (v[2] + v[3]);
+    before += warp_scan(own) - own;
+    const float x[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (before <= want && want < before + v[j]) found(first + 4 * i + j, x[j], total);
+      before += v[j];
     }
   };
   auto pick = [&](float bound, auto &&value, auto &&target, auto &&found) {
-    unsigned long long sum = 0, v[4];
-    for (int i = seg_lo + lane; i < seg_hi; i += 32) { four(bound, value, i, v); sum += (v[0] + v[1]) + (v[2] + v[3]); }
-    find(block_sum(sum), bound, value, target, found);
+    unsigned long long sum = 0;
+    walk([&](float4 f, int i, int) {
+      unsigned long long v[4];
+      four(bound, value, i, v, f);
+      sum += (v[0] + v[1]) + (v[2] + v[3]);
+    });
+    find(block_sum(sum), s.warp, bound, value, target, found);
   };
 
   // Candidates: to the CTA's own list, then (collect) to rank 0's, in any order, where they are sorted, largest first.  Their number in all;
@@ -419,32 +465,39 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
   // a share of the list's) and min_p leave, then these by index and the pick among them.
   auto finish_list = [&](int total, unsigned long long k, unsigned long long want) {
     const int limit = static_cast<int>(min(static_cast<unsigned long long>(total), k));
-    unsigned long long c[2], m[2], before;
+    unsigned long long c[EACH], m[EACH], before, sum = 0;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      c[j] = 2 * tid + j < limit ? s.sorted[2 * tid + j] : 0;
-      m[j] = 2 * tid + j < limit ? mass(value_of(c[j])) : 0;
+    for (int j = 0; j < EACH; ++j) {
+      c[j] = EACH * tid + j < limit ? s.sorted[EACH * tid + j] : 0;
+      m[j] = EACH * tid + j < limit ? mass(value_of(c[j])) : 0;
+      sum += m[j];
     }
-    const unsigned long long all = block_scan(m[0] + m[1], before);
+    const unsigned long long all = block_scan(sum, before);
     if (top_p < 1.0f) want = want ? want : share_of(all); else want = ~0ull;
-    const bool keep0 = 2 * tid < limit && before < want && (tid == 0 || above_least(value_of(c[0])) || least == 0.0);
-    const bool keep1 = 2 * tid + 1 < limit && before + m[0] < want && (above_least(value_of(c[1])) || least == 0.0);
-    const int stay = __syncthreads_count(keep0) + __syncthreads_count(keep1);
+    int stay = 0;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const bool keep = EACH * tid + j < limit && before < want && (EACH * tid + j == 0 || least == 0.0 || above_least(value_of(c[j])));
+      stay += __syncthreads_count(keep);
+      before += m[j];
+    }
     int size = 32;
     while (size < stay) size <<= 1;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)                   // the halves change places: by index, the lowest (its complement the largest) first
-      if (2 * tid + j < size) s.sorted[2 * tid + j] = 2 * tid + j < stay ? (c[j] << 32) | (c[j] >> 32) : 0;
+    for (int j = 0; j < EACH; ++j)                // the halves change places: by index, the lowest (its complement the largest) first
+      if (EACH * tid + j < size) s.sorted[EACH * tid + j] = EACH * tid + j < stay ? (c[j] << 32) | (c[j] >> 32) : 0;
     sort_descending(s.sorted, size, tid);
+    sum = 0;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      c[j] = 2 * tid + j < stay ? s.sorted[2 * tid + j] : 0;
+    for (int j = 0; j < EACH; ++j) {
+      c[j] = EACH * tid + j < stay ? s.sorted[EACH * tid + j] : 0;
       c[j] = (c[j] << 32) | (c[j] >> 32);
-      m[j] = 2 * tid + j < stay ? mass(value_of(c[j])) : 0;
+      m[j] = EACH * tid + j < stay ? mass(value_of(c[j])) : 0;
+      sum += m[j];
     }
-    const unsigned long long kept = block_scan(m[0] + m[1], before), at = draw_from(kept);
+    const unsigned long long kept = block_scan(sum, before), at = draw_from(kept);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < EACH; ++j) {
       if (before <= at && at < before + m[j]) write(index_of(c[j]), value_of(c[j]), kept);
       before += m[j];
     }
@@ -461,9 +514,10 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
       if (tid < KEY_BINS) hist[tid] = 0;
       __syncthreads();
       each([&](float v, int i) {
+        if (!(v == v)) return;
         const uint32_t k = key_of(v);
         if (shift < 24 && (k >> (shift + 8)) != prefix) return;
-        if (i >= p.vocab) return;
+        if (i < 0 || i >= p.vocab) return;
         const unsigned long long c = value(v, i);
         if (c) atomicAdd(&hist[(k >> shift) & (KEY_BINS - 1)], c);
       });
@@ -487,7 +541,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
     if (tid == 0) s.threshold = 0;
     const uint32_t key = prefix;
     unsigned long long one = 0;
-    each([&](float v, int i) { if (i < p.vocab && key_of(v) == key) { const unsigned long long c = value(v, i); one = c > one ? c : one; } });
+    each([&](float v, int i) { if (i >= 0 && i < p.vocab && v == v && key_of(v) == key) { const unsigned long long c = value(v, i); one = c > one ? c : one; } });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) { const unsigned long long other = __shfl_xor_sync(0xffffffffu, one, o); one = other > one ? other : one; }
     __syncthreads();
@@ -497,7 +551,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
     const unsigned long long mine = one;
     gather(mine, [&](int, unsigned long long v) { one = v > one ? v : one; });
     const unsigned long long room = one ? (want - before + one - 1) / one : 1;
-    pick(-INFINITY, [&](float v, int i) -> unsigned long long { return i < p.vocab && key_of(v) == key && value(v, i) != 0; },
+    pick(-INFINITY, [&](float v, int i) -> unsigned long long { return i >= 0 && i < p.vocab && v == v && key_of(v) == key && value(v, i) != 0; },
          [&](unsigned long long) { return room - 1; },
          [&](int i, float v, unsigned long long) { for (int r = 0; r < ranks; ++r) *cluster.map_shared_rank(&s.threshold, r) = place_of(v, i); });
     cluster.sync();
@@ -542,10 +596,13 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
     const unsigned long long k = static_cast<unsigned long long>(top_k);
     unsigned int c[4];
     unsigned long long before, counted;
-    // Few: the largest values of the threads are k tokens at least down to some bin, which leaves out most others without a look at them.
-    if (top_k <= LIST * 3 / 4 && top_k * 5 <= ranks * THREADS) {
-      const int b = bin_of(high);
-      if (b < BINS) atomicAdd(&s.counts[b], 1u);
+    // Few: the largest values of the threads' parts are k tokens at least down to some bin, which leaves out most others without a look at them.
+    if (top_k <= LIST * 5 / 8 && top_k * 2 <= min(TURN * ranks * THREADS, fours)) {
+#pragma unroll
+      for (int j = 0; j < TURN; ++j) {
+        const int b = bin_of(high[j]);
+        if (b < BINS) atomicAdd(&s.counts[b], 1u);
+      }
       cluster.sync();
       counted = cluster_counts(c, before);
       if (tid == 0) s.bin_hi = BINS - 1;
@@ -603,27 +660,34 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
   }
   if (top_p < 1.0f) {
     unsigned long long sum = 0;
-    each([&](float v, int i) {
-      unsigned int q;
-      const int b = bin_and_mass(v, q);
-      const unsigned long long m = mass(v);
-      const bool in = b < BINS && (!cut || kept(v, i));
-      if (in) atomicAdd(&s.counts[b], q);
-      sum += in ? m : 0;
+    walk([&](float4 v4, int i, int) {              // (four tokens' arithmetic side by side, then the atomics)
+      const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+      unsigned int q[4];
+      int b[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        b[j] = bin_and_mass(v[j], q[j]);
+        const unsigned long long m = mass(v[j]);
+        if (cut && !kept(v[j], first + 4 * i + j)) b[j] = BINS;
+        sum += b[j] < BINS ? m : 0;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (b[j] < BINS) atomicAdd(&s.counts[b[j]], q[j]);
     });
     if (tid == 0) { s.bin_lo = 0; s.bin_hi = BINS - 1; }
     const unsigned long long own = block_sum(sum);
     unsigned long long total = 0;
     gather(own, [&](int, unsigned long long v) { total += v; });
     const unsigned long long want = share_of(total);
-    // The border's bin, or a few that it may be in: the histogram's sums are off by 1.2e-4 (above, and the rounding of the bin's number), and
+    // The border's bin, or a few that it may be in: the histogram's sums are off by 1.2e-4 (above, and the roundings of the bin's number and middle), and
     // masses by 2^-46 each.
     unsigned int c[4];
     unsigned long long unused, low[4], high[4], below, ahead;
     cluster_counts(c, unused);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const double middle = power_of_two(-1.4426950408889634 * SPAN / BINS * (4 * tid + j)), n_ = c[j] * (1.0 / ONE);
+      const double middle = exp2f(-1.4426950408889634f * SPAN / BINS * (4 * tid + j)), n_ = c[j] * (1.0 / ONE);
       low[j] = __double2ull_rd(n_ * fmax(middle * (1.0 - 1.3e-4) - 0x1.1p-46, 0.0) * 0x1p45);
       high[j] = __double2ull_ru(n_ * (middle * (1.0 + 1.3e-4) + 0x1.1p-46) * 0x1p45);
     }
@@ -665,30 +729,51 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
     // The mass in front of the border's bins, exactly, and their tokens.
     unsigned long long front = 0;
     sum = 0;
-    each_from(bound_of(hi), [&](float v, int i) {
-      const int b = bin_of(v);
-      const bool in = b <= hi && kept(v, i);
-      if (in && b >= lo && few_at_border) list(v, i);
-      const unsigned long long m = mass(v);
-      sum += in && b < lo ? m : 0;
+    const float from = bound_of(hi);
+    walk([&](float4 v4, int i, int) {
+      if (!(fmaxf(fmaxf(v4.x, v4.y), fmaxf(v4.z, v4.w)) >= from)) return;
+      const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+      bool at_border = false;
+      int b[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        b[j] = bin_of(v[j]);
+        const unsigned long long m = mass(v[j]);
+        if (b[j] > hi || !kept(v[j], first + 4 * i + j)) b[j] = BINS;
+        sum += b[j] < lo ? m : 0;
+        at_border = at_border || (b[j] >= lo && b[j] < BINS);
+      }
+      if (at_border && few_at_border) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (b[j] >= lo && b[j] < BINS) list(v[j], first + 4 * i + j);
+      }
     });
     const unsigned long long mine = block_sum(sum), ranges = warp_sum(sum);
     gather(mine, [&](int, unsigned long long v) { front += v; });
     if (few_at_border) {
       const int listed = collect();
       if (rank == 0) {                           // how many of them stay
-        unsigned long long w[2], before;
+        unsigned long long w[EACH], before, all = 0;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) w[j] = 2 * tid + j < listed ? mass(value_of(s.sorted[2 * tid + j])) : 0;
-        block_scan(w[0] + w[1], before);
+        for (int j = 0; j < EACH; ++j) {
+          w[j] = EACH * tid + j < listed ? mass(value_of(s.sorted[EACH * tid + j])) : 0;
+          all += w[j];
+        }
+        block_scan(all, before);
         before += front;
-        const int stay = __syncthreads_count(2 * tid < listed && before < want) + __syncthreads_count(2 * tid + 1 < listed && before + w[0] < want);
+        int stay = 0;
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+          stay += __syncthreads_count(EACH * tid + j < listed && before < want);
+          before += w[j];
+        }
         announce(max(stay, 1));
       }
       cluster.sync();
       cut_at(s.threshold);
       if (least == 0.0 || weight(kept_value) >= least) {       // (min_p takes nothing away) the ranges' sums are there but for the listed tokens that stay
-        if (lane == 0) s.group[warp] = ranges;
+        if (lane == 0) s.warp_kept[warp] = ranges;
         __syncthreads();
         sum = 0;
         for (int i = tid; i < s.listed; i += THREADS) {
@@ -696,13 +781,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
           const int at = index_of(s.list[i]);
           const unsigned long long m = kept(v, at) ? mass(v) : 0;
           sum += m;
-          if (m) atomicAdd(&s.group[((at - first) >> 2) / seg], m);
+          if (m) atomicAdd(&s.warp_kept[((at - first) >> 2) / seg], m);
         }
-        const unsigned long long own_mass = mine + block_sum(sum);
-        __syncthreads();
-        if (tid < WARPS) s.warp[tid] = s.group[tid];
-        __syncthreads();
-        find(own_mass, kept_value, [&](float v, int i) -> unsigned long long { const unsigned long long m = mass(v); return kept(v, i) ? m : 0ull; }, draw_from, write);
+        find(mine + block_sum(sum), s.warp_kept, kept_value, [&](float v, int i) -> unsigned long long { const unsigned long long m = mass(v); return kept(v, i) ? m : 0ull; }, draw_from, write);
         cluster.sync();
         return;
       }

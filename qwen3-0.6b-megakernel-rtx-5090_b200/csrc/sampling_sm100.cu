@@ -16,22 +16,22 @@ int refuse(const std::string &why) {
   return QMK_ERR_BAD_ARGUMENT;
 }
 
-// Row slices of up to 12,288 tokens (48 KB) while there are CTAs to take them: the smallest cluster that keeps them that short.
-int cluster_size(int vocab) {
+// CTAs per row: as many as still are all resident at once (two an SM), each with 2048 tokens at least.
+int cluster_size(int rows, int vocab, int sms) {
   int c = 1;
-  while (c < MAX_CLUSTER && vocab > c * 12288) c *= 2;
+  while (c < MAX_CLUSTER && 2 * c * rows <= 2 * sms && vocab > c * 2048) c *= 2;
   return c;
 }
 
 template <typename T>
 cudaError_t launch(const Params &p, int rows, int ranks, cudaStream_t stream) {
-  const size_t smem = sizeof(Shared) + static_cast<size_t>(p.slice) * sizeof(float);
-  cudaError_t e = cudaFuncSetAttribute(sample_rows<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  constexpr int smem = sizeof(Shared) + 2 * TURN * THREADS * 4 * sizeof(T);
+  cudaError_t e = cudaFuncSetAttribute(sample_rows<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
+  cfg.dynamicSmemBytes = smem;
   cfg.gridDim = dim3(static_cast<unsigned int>(rows) * ranks);
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -58,12 +58,19 @@ extern "C" int qmk_sample_tokens(const void *logits, int logits_type, long long 
   if (!temperatures && !(temperature >= 0.0f)) return refuse("the temperature must not be negative");
   if (!top_ps && !(top_p > 0.0f)) return refuse("top_p must be above 0");
   if (!min_ps && !(min_p >= 0.0f && min_p <= 1.0f)) return refuse("min_p must be in [0, 1]");
+  int device = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    qmk_internal::note_error(std::string("qmk_sample_tokens: ") + cudaGetErrorString(e));
+    return QMK_ERR_CUDA;
+  }
   Params p;
-  const int ranks = cluster_size(vocab);
+  const int ranks = cluster_size(rows, vocab, sms);
   p.logits = logits;
   p.row_stride = row_stride;
   p.vocab = vocab;
-  p.slice = ((vocab + ranks - 1) / ranks + 3) / 4 * 4;
   p.uniforms = uniforms;
   p.temperatures = temperatures;
   p.top_ps = top_ps;
@@ -75,9 +82,9 @@ extern "C" int qmk_sample_tokens(const void *logits, int logits_type, long long 
   p.top_k = top_k;
   p.tokens = tokens;
   p.logprobs = logprobs;
-  const cudaError_t e = logits_type == 0 ? launch<float>(p, rows, ranks, stream)
-                        : logits_type == 1 ? launch<__half>(p, rows, ranks, stream)
-                                           : launch<__nv_bfloat16>(p, rows, ranks, stream);
+  e = logits_type == 0 ? launch<float>(p, rows, ranks, stream)
+      : logits_type == 1 ? launch<__half>(p, rows, ranks, stream)
+                         : launch<__nv_bfloat16>(p, rows, ranks, stream);
   if (e != cudaSuccess) {
     cudaGetLastError();
     qmk_internal::note_error(std::string("qmk_sample_tokens: ") + cudaGetErrorString(e));
