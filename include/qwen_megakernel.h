@@ -439,6 +439,8 @@ typedef struct qmk_shared_prefix_args {
   long long prefix_row_stride, prefix_head_stride;
   const void *const *k_own;          /* HOST arrays of DEVICE pointers, one per sequence: [kv_heads][own_rows][head_dim], the same strides for all */
   const void *const *v_own;
+  const void *k_own_base, *v_own_base;   /* used where k_own is null: the caches of sequence 0, own_seq_stride elements between sequences */
+  long long own_seq_stride;
   int own_rows;                      /* rows that an own cache holds; 0: none */
   long long own_row_stride, own_head_stride;
   const int *own_lens;               /* DEVICE, one per sequence; own_lens + own_lens_add is taken into [0, own_rows] */

@@ -70,21 +70,24 @@ extern "C" int qmk_attention_shared_prefix(const qmk_shared_prefix_args *a, cuda
   if (a->kv_heads < 1 || a->q_heads < 1 || a->q_heads % a->kv_heads || a->q_heads / a->kv_heads > MAX_GROUP || a->q_heads > 1024)
     return refuse("q_heads must be 1 to 16 times kv_heads, and at most 1024");
   if (a->prefix_len < 0 || a->own_rows < 0) return refuse("negative length");
-  if (!a->q || !a->out || (a->prefix_len > 0 && (!a->k_prefix || !a->v_prefix)) || (a->own_rows > 0 && (!a->k_own || !a->v_own || !a->own_lens)))
+  if (!a->q || !a->out || (a->prefix_len > 0 && (!a->k_prefix || !a->v_prefix)) || (a->own_rows > 0 && (a->k_own ? !a->v_own : !a->k_own_base || !a->v_own_base)) || (a->own_rows > 0 && !a->own_lens))
     return refuse("null pointer argument");
   if (!(a->scale > -3.0e38f && a->scale < 3.0e38f)) return refuse("the scale must be finite");
   auto aligned = [](const void *ptr) { return (reinterpret_cast<unsigned long long>(ptr) & 15u) == 0; };
   bool ok = aligned(a->q) && aligned(a->k_prefix) && aligned(a->v_prefix) && aligned(a->out) && aligned(a->workspace);
+  Params p;
   for (int b = 0; a->own_rows > 0 && b < a->num_sequences; ++b) {
-    if (!a->k_own[b] || !a->v_own[b]) return refuse("null pointer argument");
-    ok = ok && aligned(a->k_own[b]) && aligned(a->v_own[b]);
+    const long long at = 2 * b * a->own_seq_stride;
+    p.k_own[b] = a->k_own ? a->k_own[b] : static_cast<const char *>(a->k_own_base) + at;
+    p.v_own[b] = a->k_own ? a->v_own[b] : static_cast<const char *>(a->v_own_base) + at;
+    if (!p.k_own[b] || !p.v_own[b]) return refuse("null pointer argument");
+    ok = ok && aligned(p.k_own[b]) && aligned(p.v_own[b]);
   }
   if (!ok) return refuse("pointers must be 16-byte aligned");
   if (a->q_seq_stride % 8 || a->q_head_stride % 8 || a->prefix_row_stride % 8 || a->prefix_head_stride % 8 || a->own_row_stride % 8 || a->own_head_stride % 8)
     return refuse("strides must be multiples of 8 elements");
   const Split s = split_of(a->num_sequences, a->q_heads, a->kv_heads, a->prefix_len, a->own_rows);
   if (!a->workspace || a->workspace_bytes < workspace_bytes(s, a->num_sequences, a->q_heads, a->head_dim)) return refuse("workspace too small");
-  Params p;
   p.q = a->q;
   p.q_seq = a->q_seq_stride;
   p.q_head = a->q_head_stride;
@@ -112,10 +115,6 @@ extern "C" int qmk_attention_shared_prefix(const qmk_shared_prefix_args *a, cuda
   p.part_ml = reinterpret_cast<float2 *>(p.part_out + states * a->head_dim);
   p.out = a->out;
   p.lse = a->lse;
-  for (int b = 0; a->own_rows > 0 && b < p.seqs; ++b) {
-    p.k_own[b] = a->k_own[b];
-    p.v_own[b] = a->v_own[b];
-  }
   const cudaError_t e = a->type == 0 ? (a->head_dim == 64 ? launch<__half, 64>(p, s, stream) : launch<__half, 128>(p, s, stream))
                                      : (a->head_dim == 64 ? launch<__nv_bfloat16, 64>(p, s, stream) : launch<__nv_bfloat16, 128>(p, s, stream));
   if (e != cudaSuccess) {

@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import array
 import ctypes
+import functools
 import os
 
 import torch
@@ -99,7 +100,7 @@ class _SharedPrefixArgs(ctypes.Structure):
     _fields_ = [("type", _I), ("num_sequences", _I), ("q_heads", _I), ("kv_heads", _I), ("head_dim", _I),
                 ("q", _P), ("q_seq_stride", _LL), ("q_head_stride", _LL),
                 ("k_prefix", _P), ("v_prefix", _P), ("prefix_len", _I), ("prefix_row_stride", _LL), ("prefix_head_stride", _LL),
-                ("k_own", _P), ("v_own", _P), ("own_rows", _I), ("own_row_stride", _LL), ("own_head_stride", _LL),
+                ("k_own", _P), ("v_own", _P), ("k_own_base", _P), ("v_own_base", _P), ("own_seq_stride", _LL), ("own_rows", _I), ("own_row_stride", _LL), ("own_head_stride", _LL),
                 ("own_lens", _P), ("own_lens_add", _I), ("scale", _F), ("out", _P), ("lse", _P), ("workspace", _P),
                 ("workspace_bytes", _LL)]
 
@@ -627,16 +628,28 @@ def gemm_packed_tn(a: torch.Tensor, b: torch.Tensor, weight_format, b2: torch.Te
     return out
 
 
+# The two operators below are called once per layer or step: their checks are plain expressions, and the stream is asked for without an
+# object around it (a call's host time 25 -> 12 us for a row of logits, of which the launch is 5).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 _LOGIT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_FP32, _INT32 = torch.float32, torch.int32
 
 
-def _per_row(value, dtype, rows, device, name):
+def _on_device(index: int, call, *args):
+    """``call(*args, stream)`` with the device current and its current stream."""
+    if torch.cuda.current_device() == index:
+        return call(*args, _raw_stream(index))
+    with torch.cuda.device(index):
+        return call(*args, _raw_stream(index))
+
+
+def _per_row(value, dtype, rows, index, name):
     """(device pointer or 0, scalar) of an option that is a number or a CUDA tensor with a value per row."""
-    if isinstance(value, torch.Tensor):
-        _check(value.dtype == dtype and value.device == device and value.dim() == 1 and value.shape[0] == rows and value.is_contiguous(),
-               f"sample_tokens: {name} must be a number or a contiguous {dtype} tensor with one value per row on the logits' device")
-        return value.data_ptr(), 0
-    return 0, value
+    if not isinstance(value, torch.Tensor):
+        return 0, value
+    if not (value.dtype is dtype and value.is_cuda and value.get_device() == index and value.dim() == 1 and value.shape[0] == rows and value.is_contiguous()):
+        raise RuntimeError(f"sample_tokens: {name} must be a number or a contiguous {dtype} tensor with one value per row on the logits' device")
+    return value.data_ptr(), 0
 
 
 def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -645,23 +658,23 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
     largest value), ``top_k`` (0: off), ``top_p`` (1: off) and ``min_p`` (0: off) are numbers, or tensors with a value per row (fp32,
     ``top_k`` int32).  The definition, ties and empty rows included: ``qmk_sample_tokens`` in include/qwen_megakernel.h.  Runs on the
     current stream of the logits' device, does not synchronise, may be captured in a graph."""
-    _require_cuda()
     code = _LOGIT_TYPES.get(logits.dtype)
-    _check(code is not None and logits.is_cuda and logits.dim() == 2 and (logits.shape[1] < 2 or logits.stride(1) == 1),
-           "sample_tokens: logits must be a CUDA matrix [rows, vocab] of fp32, fp16 or bf16, contiguous along the vocabulary")
+    if code is None or not logits.is_cuda or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        _require_cuda()
+        raise RuntimeError("sample_tokens: logits must be a CUDA matrix [rows, vocab] of fp32, fp16 or bf16, contiguous along the vocabulary")
     rows, vocab = logits.shape
-    device = logits.device
-    _check(uniforms.dtype == torch.float32 and uniforms.device == device and uniforms.dim() == 1 and uniforms.shape[0] == rows
-           and uniforms.is_contiguous(), "sample_tokens: uniforms must be a contiguous fp32 tensor with one value per row on the logits' device")
-    t_ptr, t = _per_row(temperature, torch.float32, rows, device, "temperature")
-    k_ptr, k = _per_row(top_k, torch.int32, rows, device, "top_k")
-    p_ptr, p = _per_row(top_p, torch.float32, rows, device, "top_p")
-    m_ptr, m = _per_row(min_p, torch.float32, rows, device, "min_p")
-    with torch.cuda.device(device):
-        tokens = torch.empty(rows, dtype=torch.int32, device=device)
-        logprobs = torch.empty(rows, dtype=torch.float32, device=device)
-        rc = _lib.qmk_sample_tokens(logits.data_ptr(), code, logits.stride(0), rows, vocab, uniforms.data_ptr(), t_ptr, float(t), k_ptr, int(k),
-                                    p_ptr, float(p), m_ptr, float(m), tokens.data_ptr(), logprobs.data_ptr(), _stream())
+    index = logits.get_device()
+    if not (uniforms.dtype is _FP32 and uniforms.is_cuda and uniforms.get_device() == index and uniforms.dim() == 1 and uniforms.shape[0] == rows
+            and uniforms.is_contiguous()):
+        raise RuntimeError("sample_tokens: uniforms must be a contiguous fp32 tensor with one value per row on the logits' device")
+    t_ptr, t = _per_row(temperature, _FP32, rows, index, "temperature")
+    k_ptr, k = _per_row(top_k, _INT32, rows, index, "top_k")
+    p_ptr, p = _per_row(top_p, _FP32, rows, index, "top_p")
+    m_ptr, m = _per_row(min_p, _FP32, rows, index, "min_p")
+    logprobs = torch.empty_like(uniforms)
+    tokens = torch.empty_like(uniforms, dtype=_INT32)
+    rc = _on_device(index, _lib.qmk_sample_tokens, logits.data_ptr(), code, logits.stride(0), rows, vocab, uniforms.data_ptr(), t_ptr, t, k_ptr, k,
+                    p_ptr, p, m_ptr, m, tokens.data_ptr(), logprobs.data_ptr())
     if rc != 0:
         raise RuntimeError(f"sample_tokens: {_lib.qmk_last_error().decode()} (status {rc})")
     return tokens, logprobs
@@ -680,50 +693,69 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     16 query heads per kv head, ``dim`` 64 or 128.  ``scale`` defaults to ``dim ** -0.5``.  ``out`` is like ``q`` (contiguous), ``lse``
     the fp32 ``[n, q_heads]`` logarithms of the softmax sums; a sequence that sees no row gets zeros and -inf.  Runs on the current
     stream of the tensors' device, does not synchronise, may be captured in a graph."""
-    _require_cuda()
     who = "attention_shared_prefix"
-    _check(q.is_cuda and q.dim() == 3 and q.dtype in (torch.float16, torch.bfloat16) and q.stride(2) == 1,
-           f"{who}: q must be a CUDA tensor [n, q_heads, dim] of fp16 or bf16, contiguous along dim")
+    dtype = q.dtype
+    if dtype is torch.float16:
+        code = 0
+    elif dtype is torch.bfloat16:
+        code = 1
+    else:
+        code = -1
+    if code < 0 or not q.is_cuda or q.dim() != 3 or q.stride(2) != 1:
+        _require_cuda()
+        raise RuntimeError(f"{who}: q must be a CUDA tensor [n, q_heads, dim] of fp16 or bf16, contiguous along dim")
     n, q_heads, dim = q.shape
-    device, dtype = q.device, q.dtype
-    _check(1 <= n <= MAX_SHARED_PREFIX_SEQUENCES, f"{who}: 1 to {MAX_SHARED_PREFIX_SEQUENCES} sequences per call")
-    _check(k_prefix.dim() == 3 and k_prefix.shape == v_prefix.shape and k_prefix.shape[2] == dim and k_prefix.dtype == v_prefix.dtype == dtype
-           and k_prefix.device == v_prefix.device == device and k_prefix.stride() == v_prefix.stride() and k_prefix.stride(2) == 1,
-           f"{who}: k_prefix and v_prefix must be [kv_heads, prefix, dim], of q's type and device and with the same strides")
-    kv_heads, prefix = k_prefix.shape[:2]
-    ints = ctypes.c_void_p * n
+    index = q.get_device()
+    if not 1 <= n <= MAX_SHARED_PREFIX_SEQUENCES:
+        raise RuntimeError(f"{who}: 1 to {MAX_SHARED_PREFIX_SEQUENCES} sequences per call")
+    prefix_strides = k_prefix.stride()
+    if not (k_prefix.dim() == 3 and k_prefix.shape == v_prefix.shape and k_prefix.shape[2] == dim and k_prefix.dtype is dtype and v_prefix.dtype is dtype
+            and k_prefix.get_device() == index and v_prefix.get_device() == index and prefix_strides == v_prefix.stride() and prefix_strides[2] == 1):
+        raise RuntimeError(f"{who}: k_prefix and v_prefix must be [kv_heads, prefix, dim], of q's type and device and with the same strides")
+    kv_heads, prefix, _ = k_prefix.shape
     if isinstance(k_own, torch.Tensor) and isinstance(v_own, torch.Tensor):
-        _check(k_own.dim() == 4 and k_own.shape == v_own.shape and k_own.shape[0] == n and k_own.stride() == v_own.stride(),
-               f"{who}: k_own and v_own must be [n, kv_heads, rows, dim] with the same strides")
-        shape, strides = k_own.shape[1:], k_own.stride()[1:]
-        step = k_own.stride(0) * 2
-        kp, vp = k_own.data_ptr(), v_own.data_ptr()
-        k_ptrs, v_ptrs = ints(*[kp + i * step for i in range(n)]), ints(*[vp + i * step for i in range(n)])
-        like = k_own.dtype == v_own.dtype == dtype and k_own.device == v_own.device == device
+        shape, strides = k_own.shape, k_own.stride()
+        if not (len(shape) == 4 and shape == v_own.shape and shape[0] == n and strides == v_own.stride()):
+            raise RuntimeError(f"{who}: k_own and v_own must be [n, kv_heads, rows, dim] with the same strides")
+        _, heads, rows, own_dim = shape
+        own_seq, own_head, own_row, own_last = strides
+        like = k_own.dtype is dtype and v_own.dtype is dtype and k_own.get_device() == index and v_own.get_device() == index
+        k_ptrs, v_ptrs, k_base, v_base, keep = 0, 0, k_own.data_ptr(), v_own.data_ptr(), None
     else:
         k_own, v_own = list(k_own), list(v_own)
-        _check(len(k_own) == n and len(v_own) == n, f"{who}: one own cache pair per sequence")
+        if not (len(k_own) == n and len(v_own) == n and all(t.dim() == 3 for t in (*k_own, *v_own))):
+            raise RuntimeError(f"{who}: one own cache pair [kv_heads, rows, dim] per sequence")
         shape, strides = k_own[0].shape, k_own[0].stride()
-        like = all(t.shape == shape and t.stride() == strides and t.dtype == dtype and t.device == device for t in (*k_own, *v_own))
-        k_ptrs, v_ptrs = ints(*[t.data_ptr() for t in k_own]), ints(*[t.data_ptr() for t in v_own])
-    _check(like and len(shape) == 3 and shape[0] == kv_heads and shape[2] == dim and strides[2] == 1,
-           f"{who}: own caches must be [kv_heads, rows, dim] each, of q's type and device and with the same strides")
-    rows = shape[1]
-    _check(own_lens.dtype == torch.int32 and own_lens.device == device and own_lens.dim() == 1 and own_lens.shape[0] == n and own_lens.is_contiguous(),
-           f"{who}: own_lens must be a contiguous int32 tensor with one value per sequence on q's device")
-    with torch.cuda.device(device):
-        out = torch.empty((n, q_heads, dim), dtype=dtype, device=device)
-        lse = torch.empty((n, q_heads), dtype=torch.float32, device=device)
-        need = _lib.qmk_attention_shared_prefix_workspace(n, q_heads, kv_heads, dim, prefix, rows)
-        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
-        args = _SharedPrefixArgs(0 if dtype == torch.float16 else 1, n, q_heads, kv_heads, dim, q.data_ptr(), q.stride(0), q.stride(1),
-                                 k_prefix.data_ptr(), v_prefix.data_ptr(), prefix, k_prefix.stride(1), k_prefix.stride(0),
-                                 ctypes.addressof(k_ptrs), ctypes.addressof(v_ptrs), rows, strides[1], strides[0], own_lens.data_ptr(), 0,
-                                 dim ** -0.5 if scale is None else float(scale), out.data_ptr(), lse.data_ptr(), workspace.data_ptr(), workspace.numel())
-        rc = _lib.qmk_attention_shared_prefix(ctypes.byref(args), _stream())
+        heads, rows, own_dim = shape
+        own_seq, (own_head, own_row, own_last) = 0, strides
+        like = all(t.shape == shape and t.stride() == strides and t.dtype is dtype and t.get_device() == index for t in (*k_own, *v_own))
+        pointers = ctypes.c_void_p * n
+        keep = pointers(*[t.data_ptr() for t in k_own]), pointers(*[t.data_ptr() for t in v_own])
+        k_ptrs, v_ptrs, k_base, v_base = ctypes.addressof(keep[0]), ctypes.addressof(keep[1]), 0, 0
+    if not (like and heads == kv_heads and own_dim == dim and own_last == 1):
+        raise RuntimeError(f"{who}: own caches must be [kv_heads, rows, dim] each, of q's type and device and with the same strides")
+    if not (own_lens.dtype is _INT32 and own_lens.is_cuda and own_lens.get_device() == index and own_lens.dim() == 1 and own_lens.shape[0] == n
+            and own_lens.is_contiguous()):
+        raise RuntimeError(f"{who}: own_lens must be a contiguous int32 tensor with one value per sequence on q's device")
+    device = q.device
+    out = torch.empty((n, q_heads, dim), dtype=dtype, device=device)
+    lse = torch.empty((n, q_heads), dtype=_FP32, device=device)
+    need = _shared_prefix_workspace(n, q_heads, kv_heads, dim, prefix, rows)
+    workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    q_seq, q_head, _ = q.stride()
+    args = _SharedPrefixArgs(code, n, q_heads, kv_heads, dim, q.data_ptr(), q_seq, q_head, k_prefix.data_ptr(), v_prefix.data_ptr(), prefix,
+                             prefix_strides[1], prefix_strides[0], k_ptrs, v_ptrs, k_base, v_base, own_seq, rows, own_row, own_head, own_lens.data_ptr(), 0,
+                             dim ** -0.5 if scale is None else scale, out.data_ptr(), lse.data_ptr(), workspace.data_ptr(), need)
+    rc = _on_device(index, _lib.qmk_attention_shared_prefix, args)
     if rc != 0:
         raise RuntimeError(f"{who}: {_lib.qmk_last_error().decode()} (status {rc})")
     return out, lse
+
+
+@functools.lru_cache(maxsize=256)
+def _shared_prefix_workspace(*sizes):
+    """Bytes of workspace for these sizes (``qmk_attention_shared_prefix_workspace``, at least a few)."""
+    return max(int(_lib.qmk_attention_shared_prefix_workspace(*sizes)), 256)
 
 
 def sync_status() -> int:
