@@ -26,7 +26,8 @@ HEADERS = [os.path.join(os.path.dirname(HERE), "include", "qwen_megakernel.h"),
            os.path.join(HERE, "csrc", "gemm_tcgen05.cuh"), os.path.join(HERE, "csrc", "gemm_pair_tcgen05.cuh"), os.path.join(HERE, "csrc", "prefill_sm100.h"),
            os.path.join(HERE, "csrc", "prefill_kernels.cuh"), os.path.join(HERE, "csrc", "engine_internal.h"), os.path.join(HERE, "csrc", "buffer_group.h"),
            os.path.join(HERE, "csrc", "attention_tcgen05.cuh"), os.path.join(HERE, "csrc", "decode_attention_mma.cuh"),
-           os.path.join(HERE, "csrc", "sampling.cuh"), os.path.join(HERE, "csrc", "shared_prefix_attention.cuh")]
+           os.path.join(HERE, "csrc", "sampling.cuh"), os.path.join(HERE, "csrc", "shared_prefix_attention.cuh"),
+           os.path.join(HERE, "csrc", "shared_prefix_tcgen05.cuh")]
 LIB_PATH = os.path.join(HERE, "libqwen_megakernel.so")
 
 NVCC_FLAGS = [

@@ -104,7 +104,7 @@ __device__ __forceinline__ float fast_exp2(float x) {
 
 // An issuing thread's way out after a time-out: the products it has issued end, and so do the copies of the tiles [next, next + STAGES)
 // below `end`, which its loader may have asked for before it left.
-__device__ __noinline__ void issuer_drain(uint32_t stopped, uint32_t full0, int next, int end, unsigned long long budget_ns) {
+static __device__ __noinline__ void issuer_drain(uint32_t stopped, uint32_t full0, int next, int end, unsigned long long budget_ns) {
   qmk_gemm::mma_commit(stopped);
   qmk_gemm::bar_drain(stopped, 0, budget_ns);
   for (int j = next; j < end && j < next + STAGES; ++j)

@@ -154,7 +154,7 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 }
 // The same with the waiting out of line: what surrounds the products in the issuing thread's loop costs more than the try itself
 // (16 K blocks in place, 64 rows x 32 columns: 3600 cycles with the loop above inlined, 3200 so, 1600 with no wait between them).
-__device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int *abort_flag, unsigned int *status,
+static __device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int *abort_flag, unsigned int *status,
                                            unsigned long long budget_ns) {
   return bar_wait(bar, parity, abort_flag, status, budget_ns);
 }
@@ -219,7 +219,7 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
 }
 
 // Behind a time-out: waits for a phase that copies or MMAs under way complete (microseconds; 2 ms at most, or the budget).
-__device__ __noinline__ void bar_drain(uint32_t bar, uint32_t parity, unsigned long long budget_ns) {
+static __device__ __noinline__ void bar_drain(uint32_t bar, uint32_t parity, unsigned long long budget_ns) {
   const unsigned long long t0 = gtime(), limit = budget_ns > 2000000ull ? budget_ns : 2000000ull;
   while (!bar_try(bar, parity))
     if (gtime() - t0 > limit) break;

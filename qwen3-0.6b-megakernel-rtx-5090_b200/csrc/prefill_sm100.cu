@@ -67,6 +67,18 @@ int make_map_f16(CUtensorMap *map, const void *ptr, uint64_t rows, uint64_t cols
   return QMK_OK;
 }
 
+// Tensor map of fp16 or bf16 values with any strides (bytes, of the dimensions behind the first), 128-byte swizzle, zeros outside.
+bool make_map_tiled(CUtensorMap *map, bool bf16, unsigned int rank, const void *ptr, const unsigned long long *dims, const unsigned long long *strides,
+                    const unsigned int *box) {
+  EncodeTiledFn enc = encoder();
+  cuuint64_t d[5], st[4];
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  for (unsigned int i = 0; i < rank; ++i) d[i] = dims[i];
+  for (unsigned int i = 0; i + 1 < rank; ++i) st[i] = strides[i];
+  return enc && enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void *>(ptr), d, st, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Packed weight rows (weight formats 1 and 2): bytes of values, where the NVFP4 block scales and the 16-byte trailer
 // with the fp32 scale sit inside a row, and the bytes between rows.
 PackedRow packed_row(int wq, int K) {

@@ -34,6 +34,7 @@ struct Params {
   const void *k_prefix, *v_prefix;
   long long prefix_row, prefix_head;
   int prefix_len, prefix_parts, prefix_range, row_tiles;   // range: prefix rows per item, a multiple of KEYS
+  int prefix_items;                              // of attend_parts: 0 where prefix_parts_tc takes them, which runs beside it then
   long long own_row, own_head;
   int own_rows, own_parts;
   const int *own_lens;
@@ -72,6 +73,7 @@ template <> struct Half<__half> {
   static __device__ __forceinline__ __half from(float a) { return __float2half_rn(a); }
   // Weights are at most 2^P_SHIFT: rounding 2^-11 of the value down to 2^-14, and so for weights of 2^-26 of the row's largest on.
   static constexpr float P_SHIFT = 12.0f;
+  static constexpr bool BF16 = false;
 };
 template <> struct Half<__nv_bfloat16> {
   static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -84,6 +86,7 @@ template <> struct Half<__nv_bfloat16> {
   }
   static __device__ __forceinline__ __nv_bfloat16 from(float a) { return __float2bfloat16_rn(a); }
   static constexpr float P_SHIFT = 0.0f;
+  static constexpr bool BF16 = true;
 };
 
 // mma.sync tiles: MT warps side by side own 16 query rows each, the 4 / MT groups of warps take the tile's cache rows in turn; every
@@ -249,11 +252,12 @@ __device__ __forceinline__ void item_mma(const Params &p, unsigned char *smem, i
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(THREADS) attend_parts(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) unsigned char smem[];
-  pdl_wait();
+  // (behind prefix_parts_tc, which has waited for what is read here: this kernel runs beside it and ends behind it)
+  const bool beside = p.prefix_items == 0 && p.prefix_parts > 0;
+  if (!beside) pdl_wait();
   pdl_trigger();
-  const int prefix_items = p.prefix_parts * p.row_tiles * p.kv_heads;
   int id = static_cast<int>(blockIdx.x);
-  if (id < prefix_items) {
+  if (id < p.prefix_items) {
     const int kv = id % p.kv_heads, tile = id / p.kv_heads % p.row_tiles, part = id / (p.kv_heads * p.row_tiles);
     const int first = part * p.prefix_range, n = min(p.prefix_range, p.prefix_len - first);
     const int row0 = tile * MT * 16, live = min(MT * 16, p.seqs * p.group - row0);
@@ -262,49 +266,89 @@ __global__ void __launch_bounds__(THREADS) attend_parts(const __grid_constant__ 
                        p.prefix_row, n);
     return;
   }
-  id -= prefix_items;
+  id -= p.prefix_items;
   const int kv = id % p.kv_heads, b = id / p.kv_heads % p.seqs, own = id / (p.kv_heads * p.seqs);
   const int len = min(max(p.own_lens[b] + p.own_bias, 0), p.own_rows), first = own * OWN_RANGE, n = min(OWN_RANGE, len - first);
   const int part = p.prefix_parts + own;
   if (n <= 0) {                                            // no rows: a state that weighs nothing
     if (threadIdx.x < p.group)
       p.part_ml[(static_cast<size_t>(part) * p.seqs + b) * p.q_heads + kv * p.group + threadIdx.x] = make_float2(-INFINITY, 0.f);
-    return;
+  } else {
+    const size_t off = static_cast<size_t>(kv) * p.own_head + static_cast<size_t>(first) * p.own_row;
+    item_mma<T, D, 1>(p, smem, part, kv, b * p.group, p.group, static_cast<const T *>(p.k_own[b]) + off, static_cast<const T *>(p.v_own[b]) + off,
+                      p.own_row, n);
   }
-  const size_t off = static_cast<size_t>(kv) * p.own_head + static_cast<size_t>(first) * p.own_row;
-  item_mma<T, D, 1>(p, smem, part, kv, b * p.group, p.group, static_cast<const T *>(p.k_own[b]) + off, static_cast<const T *>(p.v_own[b]) + off,
-                    p.own_row, n);
+  if (beside) pdl_wait();
 }
 
-// A warp joins the parts of a (sequence, query head).
+// A CTA joins the parts of a (sequence, query head): a warp takes every fourth part, eight parts' outputs on their way at a time.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) join_parts(const __grid_constant__ Params p) {
+  constexpr int E = D / 32, AHEAD = 8;
+  __shared__ float sm[4], sl[4];
+  __shared__ __align__(16) float sa[4][D];
   pdl_wait();
   pdl_trigger();
-  const int rows = p.seqs * p.q_heads, row = static_cast<int>(blockIdx.x) * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= rows) return;
+  const int rows = p.seqs * p.q_heads, row = static_cast<int>(blockIdx.x), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int parts = p.prefix_parts + p.own_parts;
-  float M = -INFINITY;
-  for (int i = lane; i < parts; i += 32) M = fmaxf(M, p.part_ml[static_cast<size_t>(i) * rows + row].x);
+  float M = -INFINITY, L = 0.f, A[E];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  float L = 0.f, A[D / 32];
+  for (int i = 0; i < E; ++i) A[i] = 0.f;
+  for (int i0 = warp; i0 < parts; i0 += 4 * 32) {          // this lane's part: its maximum and sum
+    const int mine = i0 + 4 * lane;
+    const float2 ml = mine < parts ? p.part_ml[static_cast<size_t>(mine) * rows + row] : make_float2(-INFINITY, 0.f);
+    float top = ml.x;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) A[i] = 0.f;
-  for (int i = 0; i < parts; ++i) {
-    const float2 ml = p.part_ml[static_cast<size_t>(i) * rows + row];
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;        // (nothing may have been written to its output)
-    const float f = exp2f(ml.x - M);
-    L += ml.y * f;
-    const float *src = p.part_out + (static_cast<size_t>(i) * rows + row) * D + lane * (D / 32);
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top = fmaxf(top, M);
+    const float f0 = M == -INFINITY ? 0.f : exp2f(M - top);
+    M = top;
+    // a part without rows has written no output and weighs nothing (one whose scores are not numbers is not among these)
+    const bool there = !(ml.x == -INFINITY && ml.y == 0.f);
+    const float f = there ? exp2f(ml.x == -INFINITY && top == -INFINITY ? 0.f : ml.x - top) : 0.f;
+    L = L * f0 + ml.y * f;
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) A[k] += src[k] * f;
+    for (int k = 0; k < E; ++k) A[k] *= f0;
+    const int count = min(32, (parts - i0 + 3) >> 2);
+    for (int j0 = 0; j0 < count; j0 += AHEAD) {
+      float v[AHEAD][E], w[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        w[j] = __shfl_sync(0xffffffffu, f, j0 + j);
+        const bool need = j0 + j < count && __shfl_sync(0xffffffffu, static_cast<int>(there), j0 + j);
+        const float *src = p.part_out + (static_cast<size_t>(i0 + 4 * (j0 + j)) * rows + row) * D + lane * E;
+        if (need) {
+          if (E == 4) { const float4 a = *reinterpret_cast<const float4 *>(src); v[j][0] = a.x; v[j][1] = a.y; v[j][E - 2] = a.z; v[j][E - 1] = a.w; }
+          else { const float2 a = *reinterpret_cast<const float2 *>(src); v[j][0] = a.x; v[j][1] = a.y; }
+        } else {
+#pragma unroll
+          for (int k = 0; k < E; ++k) v[j][k] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+        for (int k = 0; k < E; ++k) A[k] = fmaf(v[j][k], w[j], A[k]);
+    }
   }
-  const float inv = L == 0.f ? 0.f : 1.0f / L;
-  T *dst = static_cast<T *>(p.out) + static_cast<size_t>(row) * D + lane * (D / 32);
 #pragma unroll
-  for (int k = 0; k < D / 32; ++k) dst[k] = Half<T>::from(A[k] * inv);
-  if (p.lse && lane == 0) p.lse[row] = L == 0.f ? -INFINITY : (M - Half<T>::P_SHIFT) * LN2 + logf(L);
+  for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+  if (lane == 0) { sm[warp] = M; sl[warp] = L; }
+#pragma unroll
+  for (int k = 0; k < E; ++k) sa[warp][lane * E + k] = A[k];
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d >= D) return;
+  const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  float total = 0.f, out = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float f = sm[w] == -INFINITY ? (sl[w] == 0.f ? 0.f : 1.f) : exp2f(sm[w] - top);
+    total = fmaf(sl[w], f, total);
+    out = fmaf(sa[w][d], f, out);
+  }
+  static_cast<T *>(p.out)[static_cast<size_t>(row) * D + d] = Half<T>::from(total == 0.f ? 0.f : out / total);
+  if (p.lse && d == 0) p.lse[row] = total == 0.f ? -INFINITY : (top - Half<T>::P_SHIFT) * LN2 + logf(total);
 }
 
 }  // namespace qmk_spa

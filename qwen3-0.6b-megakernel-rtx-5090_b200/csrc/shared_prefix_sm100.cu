@@ -8,6 +8,7 @@
 #include "engine_internal.h"
 #include "prefill_sm100.h"
 #include "shared_prefix_attention.cuh"
+#include "shared_prefix_tcgen05.cuh"
 
 namespace {
 
@@ -18,38 +19,66 @@ int refuse(const std::string &why) {
   return QMK_ERR_BAD_ARGUMENT;
 }
 
+// How a call is cut into items.  More than 32 rows of queries against a kv head go through tcgen05, 128 at a time: XXX.
 struct Split {
-  int row_warps, row_tiles, prefix_parts, prefix_range, own_parts;
+  bool tc;
+  int row_warps, row_tiles, seqs_per_tile, prefix_parts, prefix_range, own_parts;
 };
-Split split_of(int seqs, int q_heads, int kv_heads, int prefix_len, int own_rows) {
+constexpr int SMS = 148;
+Split split_of(int seqs, int q_heads, int kv_heads, int prefix_len, int own_rows, bool tc) {
   Split s;
-  const int rows = seqs * (q_heads / kv_heads);
+  const int group = q_heads / kv_heads, rows = seqs * group, tiles = (prefix_len + KEYS - 1) / KEYS;
+  s.tc = tc && rows > 32 && prefix_len > 0;
   s.row_warps = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  s.row_tiles = (rows + 16 * s.row_warps - 1) / (16 * s.row_warps);
-  const int items = s.row_tiles * kv_heads, tiles = (prefix_len + KEYS - 1) / KEYS;
-  int parts = std::max(1, 2 * 148 / items);
+  s.seqs_per_tile = std::min(128 / group, seqs);
+  s.row_tiles = s.tc ? (seqs + s.seqs_per_tile - 1) / s.seqs_per_tile : (rows + 16 * s.row_warps - 1) / (16 * s.row_warps);
+  const int items = s.row_tiles * kv_heads, parts = std::max(1, (s.tc ? SMS : 2 * SMS) / items);
   s.prefix_range = std::max(2, (tiles + parts - 1) / parts) * KEYS;
   s.prefix_parts = (prefix_len + s.prefix_range - 1) / s.prefix_range;
   s.own_parts = (own_rows + OWN_RANGE - 1) / OWN_RANGE;
   return s;
 }
 long long workspace_bytes(const Split &s, int seqs, int q_heads, int head_dim) {
-  return static_cast<long long>(s.prefix_parts + s.own_parts) * seqs * q_heads * (head_dim * 4ll + 8);
+  return 16 + static_cast<long long>(s.prefix_parts + s.own_parts) * seqs * q_heads * (head_dim * 4ll + 8);
+}
+
+// Maps of the queries and of the prefix for prefix_parts_tc; false where the strides are none that a map can have.
+bool make_maps(CUtensorMap *maps, const Params &p, const Split &s, int head_dim, bool bf16) {
+  const unsigned long long dim = head_dim, q_dims[4] = {dim, static_cast<unsigned long long>(p.group), static_cast<unsigned long long>(p.kv_heads), static_cast<unsigned long long>(p.seqs)};
+  const unsigned long long q_strides[3] = {2ull * p.q_head, 2ull * p.q_head * p.group, 2ull * p.q_seq};
+  const unsigned int q_box[4] = {64, static_cast<unsigned int>(p.group), 1, static_cast<unsigned int>(s.seqs_per_tile)};
+  const unsigned long long kv_dims[3] = {dim, static_cast<unsigned long long>(p.prefix_len), static_cast<unsigned long long>(p.kv_heads)};
+  const unsigned long long kv_strides[2] = {2ull * p.prefix_row, 2ull * p.prefix_head};
+  const unsigned int kv_box[3] = {64, KEYS, 1};
+  return qmk_tc::make_map_tiled(maps, bf16, 4, p.q, q_dims, q_strides, q_box) && qmk_tc::make_map_tiled(maps + 1, bf16, 3, p.k_prefix, kv_dims, kv_strides, kv_box) &&
+         qmk_tc::make_map_tiled(maps + 2, bf16, 3, p.v_prefix, kv_dims, kv_strides, kv_box);
 }
 
 template <typename T, int D>
-cudaError_t launch(const Params &p, const Split &s, cudaStream_t stream) {
+cudaError_t launch(Params &p, const Split &s, const CUtensorMap *maps, unsigned int *status, cudaStream_t stream) {
   constexpr int smem = STAGES * 2 * KEYS * D * 2;
   static_assert(smem >= WARPS * 16 * (D + 4) * 4 + WARPS * 16 * 8, "the groups' states fit the ring");
-  void (*kernel)(Params) = s.row_warps == 1 ? attend_parts<T, D, 1> : s.row_warps == 2 ? attend_parts<T, D, 2> : attend_parts<T, D, 4>;
+  void (*kernel)(Params) = s.tc || s.row_warps == 1 ? attend_parts<T, D, 1> : s.row_warps == 2 ? attend_parts<T, D, 2> : attend_parts<T, D, 4>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess && s.tc) e = cudaFuncSetAttribute(prefix_parts_tc<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(tc_smem_bytes<D>()));
   if (e != cudaSuccess) return e;
-  const int items = s.prefix_parts * s.row_tiles * p.kv_heads + s.own_parts * p.kv_heads * p.seqs;
-  if (items > 0) {
-    e = qmk_tc::launch_kernel(kernel, dim3(items), dim3(THREADS), smem, stream, p);
+  const int prefix_items = s.prefix_parts * s.row_tiles * p.kv_heads, own_items = s.own_parts * p.kv_heads * p.seqs;
+  p.prefix_items = s.tc ? 0 : prefix_items;
+  bool dependent = qmk_tc::pdl_active();
+  if (s.tc) {
+    e = qmk_tc::launch_kernel(prefix_parts_tc<T, D>, dim3(prefix_items), dim3(TC_THREADS), tc_smem_bytes<D>(), stream, maps[0], maps[1], maps[2], p, s.seqs_per_tile,
+                              status);
     if (e != cudaSuccess) return e;
+    dependent = true;                            // (of the launch before, inside this call)
   }
-  return qmk_tc::launch_kernel(join_parts<T, D>, dim3((p.seqs * p.q_heads + 3) / 4), dim3(128), 0, stream, p);
+  if (p.prefix_items + own_items > 0) {
+    const qmk_tc::PdlScope scope(dependent);
+    e = qmk_tc::launch_kernel(kernel, dim3(p.prefix_items + own_items), dim3(THREADS), smem, stream, p);
+    if (e != cudaSuccess) return e;
+    dependent = true;
+  }
+  const qmk_tc::PdlScope scope(dependent);
+  return qmk_tc::launch_kernel(join_parts<T, D>, dim3(p.seqs * p.q_heads), dim3(128), 0, stream, p);
 }
 
 }  // namespace
@@ -58,7 +87,8 @@ extern "C" long long qmk_attention_shared_prefix_workspace(int num_sequences, in
                                                            int own_rows) {
   if (num_sequences < 1 || num_sequences > MAX_SEQS || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || prefix_len < 0 || own_rows < 0)
     return 0;
-  return workspace_bytes(split_of(num_sequences, q_heads, kv_heads, prefix_len, own_rows), num_sequences, q_heads, head_dim);
+  return std::max(workspace_bytes(split_of(num_sequences, q_heads, kv_heads, prefix_len, own_rows, true), num_sequences, q_heads, head_dim),
+                  workspace_bytes(split_of(num_sequences, q_heads, kv_heads, prefix_len, own_rows, false), num_sequences, q_heads, head_dim));
 }
 
 extern "C" int qmk_attention_shared_prefix(const qmk_shared_prefix_args *a, cudaStream_t stream) {
@@ -86,8 +116,8 @@ extern "C" int qmk_attention_shared_prefix(const qmk_shared_prefix_args *a, cuda
   if (!ok) return refuse("pointers must be 16-byte aligned");
   if (a->q_seq_stride % 8 || a->q_head_stride % 8 || a->prefix_row_stride % 8 || a->prefix_head_stride % 8 || a->own_row_stride % 8 || a->own_head_stride % 8)
     return refuse("strides must be multiples of 8 elements");
-  const Split s = split_of(a->num_sequences, a->q_heads, a->kv_heads, a->prefix_len, a->own_rows);
-  if (!a->workspace || a->workspace_bytes < workspace_bytes(s, a->num_sequences, a->q_heads, a->head_dim)) return refuse("workspace too small");
+  if (!a->workspace || a->workspace_bytes < qmk_attention_shared_prefix_workspace(a->num_sequences, a->q_heads, a->kv_heads, a->head_dim, a->prefix_len, a->own_rows))
+    return refuse("workspace too small");
   p.q = a->q;
   p.q_seq = a->q_seq_stride;
   p.q_head = a->q_head_stride;
@@ -100,23 +130,28 @@ extern "C" int qmk_attention_shared_prefix(const qmk_shared_prefix_args *a, cuda
   p.prefix_row = a->prefix_row_stride;
   p.prefix_head = a->prefix_head_stride;
   p.prefix_len = a->prefix_len;
-  p.prefix_parts = s.prefix_parts;
-  p.prefix_range = s.prefix_range;
-  p.row_tiles = s.row_tiles;
   p.own_row = a->own_row_stride;
   p.own_head = a->own_head_stride;
   p.own_rows = a->own_rows;
-  p.own_parts = s.own_parts;
   p.own_lens = a->own_lens;
   p.own_bias = a->own_lens_add;
   p.scale_log2 = a->scale * LOG2E;
+  // (a scale of 0 would turn the masked scores of a last tile, -inf, into NaN there)
+  Split s = split_of(p.seqs, p.q_heads, p.kv_heads, p.prefix_len, p.own_rows, p.scale_log2 != 0.0f);
+  CUtensorMap maps[3];
+  if (s.tc && !make_maps(maps, p, s, a->head_dim, a->type == 1)) s = split_of(p.seqs, p.q_heads, p.kv_heads, p.prefix_len, p.own_rows, false);
+  p.prefix_parts = s.prefix_parts;
+  p.prefix_range = s.prefix_range;
+  p.row_tiles = s.row_tiles;
+  p.own_parts = s.own_parts;
   const long long states = static_cast<long long>(s.prefix_parts + s.own_parts) * p.seqs * p.q_heads;
-  p.part_out = static_cast<float *>(a->workspace);
+  unsigned int *const status = static_cast<unsigned int *>(a->workspace);
+  p.part_out = static_cast<float *>(a->workspace) + 4;
   p.part_ml = reinterpret_cast<float2 *>(p.part_out + states * a->head_dim);
   p.out = a->out;
   p.lse = a->lse;
-  const cudaError_t e = a->type == 0 ? (a->head_dim == 64 ? launch<__half, 64>(p, s, stream) : launch<__half, 128>(p, s, stream))
-                                     : (a->head_dim == 64 ? launch<__nv_bfloat16, 64>(p, s, stream) : launch<__nv_bfloat16, 128>(p, s, stream));
+  const cudaError_t e = a->type == 0 ? (a->head_dim == 64 ? launch<__half, 64>(p, s, maps, status, stream) : launch<__half, 128>(p, s, maps, status, stream))
+                                     : (a->head_dim == 64 ? launch<__nv_bfloat16, 64>(p, s, maps, status, stream) : launch<__nv_bfloat16, 128>(p, s, maps, status, stream));
   if (e != cudaSuccess) {
     cudaGetLastError();
     qmk_internal::note_error(std::string("qmk_attention_shared_prefix: ") + cudaGetErrorString(e));

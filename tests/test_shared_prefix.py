@@ -112,7 +112,7 @@ def test_wrong_tensors_are_refused(gpu):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 @pytest.mark.parametrize("q_heads,kv_heads,dim", [(16, 8, 128), (4, 4, 64), (6, 2, 128), (8, 1, 64), (16, 1, 128), (32, 4, 64)])
-@pytest.mark.parametrize("seqs,prefix,own", [(1, 1, 1), (1, 0, 5), (2, 63, 16), (3, 64, 64), (5, 65, 300), (17, 1000, 33), (40, 129, 65), (128, 200, 20)])
+@pytest.mark.parametrize("seqs,prefix,own", [(1, 1, 1), (1, 0, 5), (2, 63, 16), (3, 64, 64), (5, 65, 300), (17, 1000, 33), (40, 129, 65), (128, 200, 20), (37, 64, 1), (100, 448, 7)])
 def test_matches_the_definition(gpu, dtype, q_heads, kv_heads, dim, seqs, prefix, own):
     lens = [(own * (i + 1) // seqs) if i % 5 else (0 if i else own) for i in range(seqs)]
     case = inputs(seqs, q_heads, kv_heads, dim, prefix, own, lens, dtype, seed=seqs + prefix)
@@ -161,10 +161,11 @@ def test_rows_behind_the_last_are_not_looked_at(gpu, garbage, seqs):
 
 
 @pytest.mark.gpu
-def test_other_strides_and_lists_of_caches(gpu):
+@pytest.mark.parametrize("seqs", [9, 70])
+def test_other_strides_and_lists_of_caches(gpu, seqs):
     """Heads between rows ([rows, heads, dim] caches), queries in a wider buffer, caches of separate allocations: views of one layer of
     the engine's [layer][head][position] caches."""
-    seqs, prefix, own = 9, 150, 60
+    prefix, own = 150, 60
     lens = torch.tensor([(11 * i) % 61 for i in range(seqs)], dtype=torch.int32).cuda()
     g = torch.Generator().manual_seed(8)
     caches = [[torch.randn(3, 8, prefix + own, 128, generator=g).half().cuda() for _ in range(seqs)] for _ in range(2)]
@@ -175,12 +176,15 @@ def test_other_strides_and_lists_of_caches(gpu):
     turned = [torch.randn(*s, generator=g).half().cuda() for s in ((prefix, 8, 128), (prefix, 8, 128), (seqs, own, 8, 128), (seqs, own, 8, 128))]
     case = (q, turned[0].transpose(0, 1), turned[1].transpose(0, 1), turned[2].transpose(1, 2), turned[3].transpose(1, 2), lens)
     check(gpu.attention_shared_prefix(*case), *case)
+    same = q[:1].expand(seqs, 16, 128)               # one query for all: stride 0
+    check(gpu.attention_shared_prefix(same, *case[1:]), same, *case[1:])
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("scale", [0.0, -0.05, 1.0, 3.0])
-def test_scales(gpu, scale):
-    case = inputs(20, 16, 8, 128, 333, 50, [(17 * i) % 51 for i in range(20)], "fp16", seed=2, gain=0.5)
+@pytest.mark.parametrize("seqs", [20, 80])
+def test_scales(gpu, scale, seqs):
+    case = inputs(seqs, 16, 8, 128, 333, 50, [(17 * i) % 51 for i in range(seqs)], "fp16", seed=2, gain=0.5)
     check(gpu.attention_shared_prefix(*case, scale=scale), *case, scale=scale)
 
 
