@@ -25,6 +25,7 @@ constexpr int THREADS = 128, WARPS = 4;
 constexpr int KEYS = 64;                         // cache rows per tile
 constexpr int STAGES = 3;
 constexpr int OWN_RANGE = 256;                   // own rows per item
+constexpr int OWN_STAGES = 2;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct Params {
@@ -34,7 +35,7 @@ struct Params {
   const void *k_prefix, *v_prefix;
   long long prefix_row, prefix_head;
   int prefix_len, prefix_parts, prefix_range, row_tiles;   // range: prefix rows per item, a multiple of KEYS
-  int prefix_items;                              // of attend_parts: 0 where prefix_parts_tc takes them, which runs beside it then
+  int prefix_items;                              // of attend_parts
   long long own_row, own_head;
   int own_rows, own_parts;
   const int *own_lens;
@@ -236,7 +237,7 @@ __device__ __forceinline__ void item_mma(const Params &p, unsigned char *smem, i
 #pragma unroll
     for (int g = 0; g < KG; ++g) {
       const float2 ml = sml[g * MT * 16 + r];
-      const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
+      const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2f(ml.x - M);
       const float4 a = *reinterpret_cast<const float4 *>(so + (g * MT * 16 + r) * PITCH + c);
       L += ml.y * f;
       A.x += a.x * f; A.y += a.y * f; A.z += a.z * f; A.w += a.w * f;
@@ -248,37 +249,184 @@ __device__ __forceinline__ void item_mma(const Params &p, unsigned char *smem, i
   }
 }
 
-// Prefix items first: they are the longest.
-template <typename T, int D, int MT>
-__global__ void __launch_bounds__(THREADS) attend_parts(const __grid_constant__ Params p) {
-  extern __shared__ __align__(128) unsigned char smem[];
-  // (behind prefix_parts_tc, which has waited for what is read here: this kernel runs beside it and ends behind it)
-  const bool beside = p.prefix_items == 0 && p.prefix_parts > 0;
-  if (!beside) pdl_wait();
-  pdl_trigger();
-  int id = static_cast<int>(blockIdx.x);
-  if (id < p.prefix_items) {
-    const int kv = id % p.kv_heads, tile = id / p.kv_heads % p.row_tiles, part = id / (p.kv_heads * p.row_tiles);
-    const int first = part * p.prefix_range, n = min(p.prefix_range, p.prefix_len - first);
-    const int row0 = tile * MT * 16, live = min(MT * 16, p.seqs * p.group - row0);
-    const size_t off = static_cast<size_t>(kv) * p.prefix_head + static_cast<size_t>(first) * p.prefix_row;
-    item_mma<T, D, MT>(p, smem, part, kv, row0, live, static_cast<const T *>(p.k_prefix) + off, static_cast<const T *>(p.v_prefix) + off,
-                       p.prefix_row, n);
-    return;
+// A sequence's own rows against its query heads of a kv head (NT blocks of eight).  Turned round: cache rows are the 16 rows of an mma.sync tile
+// and heads its eight columns, scores = K q^T and out^T = V^T p^T, so two heads cost half the products and a third of the registers that 16 query rows
+// would.  A warp takes 16 of a tile's 64 rows; p^T becomes an operand by transposing 8 x 8 blocks in registers.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+template <typename T, int D, int NT>
+__device__ __forceinline__ void item_own(const Params &p, unsigned char *smem, int part, int kv_head, int b, const T *kp, const T *vp, int nrows) {
+  constexpr int CHUNKS = D / 8, ROW_BYTES = D * 2, TILE = KEYS * ROW_BYTES;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane & 3, rq = lane >> 2;
+  const uint32_t base = s32(smem);
+  const int tiles = (nrows + KEYS - 1) / KEYS;
+  auto load = [&](int t) {
+    if (t < tiles) {
+      const uint32_t dst = base + (t % OWN_STAGES) * 2 * TILE;
+#pragma unroll
+      for (int i = tid; i < KEYS * CHUNKS; i += THREADS) {
+        const int r = i / CHUNKS, c = i % CHUNKS, row = t * KEYS + r;
+        const bool there = row < nrows;
+        const long long off = (there ? row : 0) * p.own_row + c * 8;
+        const uint32_t at = r * ROW_BYTES + ((c ^ (r & 7)) << 4);
+        copy16(dst + at, kp + off, there);
+        copy16(dst + TILE + at, vp + off, there);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int t = 0; t < OWN_STAGES; ++t) load(t);
+  uint32_t qb[NT][D / 16][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const bool live = nt * 8 + rq < p.group;
+    const T *src = static_cast<const T *>(p.q) + b * p.q_seq + (kv_head * p.group + (live ? nt * 8 + rq : 0)) * p.q_head + quad * 2;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      qb[nt][ks][0] = live ? *reinterpret_cast<const uint32_t *>(src + ks * 16) : 0u;
+      qb[nt][ks][1] = live ? *reinterpret_cast<const uint32_t *>(src + ks * 16 + 8) : 0u;
+    }
   }
-  id -= p.prefix_items;
+  float acc[NT][D / 16][4], m[NT][2], l[NT][2];            // heads 2 quad and 2 quad + 1 of each block
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    m[nt][0] = m[nt][1] = -INFINITY;
+    l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) { acc[nt][t][0] = 0.f; acc[nt][t][1] = 0.f; acc[nt][t][2] = 0.f; acc[nt][t][3] = 0.f; }
+  }
+  for (int t = 0; t < tiles; ++t) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(OWN_STAGES - 1) : "memory");
+    __syncthreads();
+    const uint32_t kt = base + (t % OWN_STAGES) * 2 * TILE, vt = kt + TILE;
+    const int key0 = t * KEYS + warp * 16;
+    if (key0 < nrows) {                                    // (the same for the warp)
+      float sc[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) { sc[nt][0] = 0.f; sc[nt][1] = 0.f; sc[nt][2] = 0.f; sc[nt][3] = 0.f; }
+      const int kr = warp * 16 + (lane & 15);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        uint32_t a[4];
+        ldsm4(kt + kr * ROW_BYTES + (((2 * ks + (lane >> 4)) ^ (kr & 7)) << 4), a);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) Half<T>::mma(sc[nt], a, qb[nt][ks][0], qb[nt][ks][1]);
+      }
+      uint32_t pb[NT][2];
+      const bool top_row = key0 + rq < nrows, low_row = key0 + rq + 8 < nrows;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[nt][i] = (i < 2 ? top_row : low_row) ? sc[nt][i] * p.scale_log2 : -INFINITY;
+        float corr[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float mx = fmaxf(sc[nt][h], sc[nt][2 + h]);
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          const float mn = fmaxf(m[nt][h], mx);
+          float sub = mn == -INFINITY ? 0.f : mn;          // scores of -inf only: 2^(-inf - 0) = 0, not NaN
+          corr[h] = exp2f(m[nt][h] - sub);
+          m[nt][h] = mn;
+          sub -= Half<T>::P_SHIFT;
+          sc[nt][h] = exp2f(sc[nt][h] - sub);
+          sc[nt][2 + h] = exp2f(sc[nt][2 + h] - sub);
+          l[nt][h] = l[nt][h] * corr[h] + (sc[nt][h] + sc[nt][2 + h]);
+        }
+        pb[nt][0] = transposed(Half<T>::pack(sc[nt][0], sc[nt][1]));
+        pb[nt][1] = transposed(Half<T>::pack(sc[nt][2], sc[nt][3]));
+#pragma unroll
+        for (int t2 = 0; t2 < D / 16; ++t2) { acc[nt][t2][0] *= corr[0]; acc[nt][t2][1] *= corr[1]; acc[nt][t2][2] *= corr[0]; acc[nt][t2][3] *= corr[1]; }
+      }
+      const int vr = warp * 16 + (lane & 7) + 8 * (lane >> 4);
+#pragma unroll
+      for (int dp = 0; dp < D / 16; ++dp) {
+        uint32_t a[4];
+        ldsm4_trans(vt + vr * ROW_BYTES + (((2 * dp + ((lane >> 3) & 1)) ^ (vr & 7)) << 4), a);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) Half<T>::mma(acc[nt][dp], a, pb[nt][0], pb[nt][1]);
+      }
+    }
+    __syncthreads();                                       // the tile has been read
+    load(t + OWN_STAGES);
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  constexpr int PITCH = D + 4, HEADS = NT * 8;             // floats between heads
+  float *const so = reinterpret_cast<float *>(smem);       // [warp][head][PITCH]
+  float2 *const sml = reinterpret_cast<float2 *>(so + WARPS * HEADS * PITCH);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], o);
+      float *const mine = so + (warp * HEADS + nt * 8 + quad * 2 + h) * PITCH + rq;
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) { mine[t * 16] = acc[nt][t][h]; mine[t * 16 + 8] = acc[nt][t][2 + h]; }
+      if (rq == 0) sml[warp * HEADS + nt * 8 + quad * 2 + h] = make_float2(m[nt][h], l[nt][h]);
+    }
+  }
+  __syncthreads();
+  const size_t at0 = (static_cast<size_t>(part) * p.seqs + b) * p.q_heads + kv_head * p.group;
+  for (int i = tid; i < p.group * (D / 4); i += THREADS) {
+    const int h = i / (D / 4), c = i % (D / 4) * 4;
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) M = fmaxf(M, sml[w * HEADS + h].x);
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float2 ml = sml[w * HEADS + h];
+      const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2f(ml.x - M);
+      const float4 a = *reinterpret_cast<const float4 *>(so + (w * HEADS + h) * PITCH + c);
+      L += ml.y * f;
+      A.x += a.x * f; A.y += a.y * f; A.z += a.z * f; A.w += a.w * f;
+    }
+    *reinterpret_cast<float4 *>(p.part_out + (at0 + h) * D + c) = A;
+    if (c == 0) p.part_ml[at0 + h] = make_float2(M, L);
+  }
+}
+// Own item `id`: (kv head, sequence, range)
+template <typename T, int D, int NT>
+__device__ __forceinline__ void own_item(const Params &p, unsigned char *smem, int id) {
   const int kv = id % p.kv_heads, b = id / p.kv_heads % p.seqs, own = id / (p.kv_heads * p.seqs);
   const int len = min(max(p.own_lens[b] + p.own_bias, 0), p.own_rows), first = own * OWN_RANGE, n = min(OWN_RANGE, len - first);
   const int part = p.prefix_parts + own;
   if (n <= 0) {                                            // no rows: a state that weighs nothing
     if (threadIdx.x < p.group)
       p.part_ml[(static_cast<size_t>(part) * p.seqs + b) * p.q_heads + kv * p.group + threadIdx.x] = make_float2(-INFINITY, 0.f);
-  } else {
-    const size_t off = static_cast<size_t>(kv) * p.own_head + static_cast<size_t>(first) * p.own_row;
-    item_mma<T, D, 1>(p, smem, part, kv, b * p.group, p.group, static_cast<const T *>(p.k_own[b]) + off, static_cast<const T *>(p.v_own[b]) + off,
-                      p.own_row, n);
+    return;
   }
-  if (beside) pdl_wait();
+  const size_t off = static_cast<size_t>(kv) * p.own_head + static_cast<size_t>(first) * p.own_row;
+  item_own<T, D, NT>(p, smem, part, kv, b, static_cast<const T *>(p.k_own[b]) + off, static_cast<const T *>(p.v_own[b]) + off, n);
+}
+
+// Prefix items first: they are the longest.
+template <typename T, int D, int MT, int NT>
+__global__ void __launch_bounds__(THREADS) attend_parts(const __grid_constant__ Params p) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  pdl_wait();
+  pdl_trigger();
+  const int id = static_cast<int>(blockIdx.x);
+  if (id >= p.prefix_items) { own_item<T, D, NT>(p, smem, id - p.prefix_items); return; }
+  const int kv = id % p.kv_heads, tile = id / p.kv_heads % p.row_tiles, part = id / (p.kv_heads * p.row_tiles);
+  const int first = part * p.prefix_range, n = min(p.prefix_range, p.prefix_len - first);
+  const int row0 = tile * MT * 16, live = min(MT * 16, p.seqs * p.group - row0);
+  const size_t off = static_cast<size_t>(kv) * p.prefix_head + static_cast<size_t>(first) * p.prefix_row;
+  item_mma<T, D, MT>(p, smem, part, kv, row0, live, static_cast<const T *>(p.k_prefix) + off, static_cast<const T *>(p.v_prefix) + off, p.prefix_row, n);
+}
+// The own rows alone, launched behind prefix_parts_tc, which has waited for what is read here: they run beside it and end behind it.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(THREADS, 3) own_parts(const __grid_constant__ Params p) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  pdl_trigger();
+  own_item<T, D, NT>(p, smem, static_cast<int>(blockIdx.x));
+  pdl_wait();
 }
 
 // A CTA joins the parts of a (sequence, query head): a warp takes every fourth part, eight parts' outputs on their way at a time.

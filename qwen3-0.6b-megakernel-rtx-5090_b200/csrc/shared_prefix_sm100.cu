@@ -29,11 +29,11 @@ Split split_of(int seqs, int q_heads, int kv_heads, int prefix_len, int own_rows
   Split s;
   const int group = q_heads / kv_heads, rows = seqs * group, tiles = (prefix_len + KEYS - 1) / KEYS;
   s.tc = tc && rows > 32 && prefix_len > 0;
-  s.row_warps = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  s.row_warps = rows <= 16 ? 1 : 2;
   s.seqs_per_tile = std::min(128 / group, seqs);
   s.row_tiles = s.tc ? (seqs + s.seqs_per_tile - 1) / s.seqs_per_tile : (rows + 16 * s.row_warps - 1) / (16 * s.row_warps);
   const int items = s.row_tiles * kv_heads, parts = std::max(1, (s.tc ? SMS : 2 * SMS) / items);
-  s.prefix_range = std::max(2, (tiles + parts - 1) / parts) * KEYS;
+  s.prefix_range = std::max(2, ((tiles + parts - 1) / parts + 1) / 2 * 2) * KEYS;      // (whole tiles of prefix_parts_tc)
   s.prefix_parts = (prefix_len + s.prefix_range - 1) / s.prefix_range;
   s.own_parts = (own_rows + OWN_RANGE - 1) / OWN_RANGE;
   return s;
@@ -54,31 +54,40 @@ bool make_maps(CUtensorMap *maps, const Params &p, const Split &s, int head_dim,
          qmk_tc::make_map_tiled(maps + 2, bf16, 3, p.v_prefix, kv_dims, kv_strides, kv_box);
 }
 
-template <typename T, int D>
+template <typename T, int D, int NT>
 cudaError_t launch(Params &p, const Split &s, const CUtensorMap *maps, unsigned int *status, cudaStream_t stream) {
-  constexpr int smem = STAGES * 2 * KEYS * D * 2;
-  static_assert(smem >= WARPS * 16 * (D + 4) * 4 + WARPS * 16 * 8, "the groups' states fit the ring");
-  void (*kernel)(Params) = s.tc || s.row_warps == 1 ? attend_parts<T, D, 1> : s.row_warps == 2 ? attend_parts<T, D, 2> : attend_parts<T, D, 4>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess && s.tc) e = cudaFuncSetAttribute(prefix_parts_tc<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(tc_smem_bytes<D>()));
-  if (e != cudaSuccess) return e;
+  constexpr int own_smem = OWN_STAGES * 2 * KEYS * D * 2, smem = STAGES * 2 * KEYS * D * 2;
+  static_assert(own_smem >= WARPS * NT * 8 * (D + 4) * 4 + WARPS * NT * 8 * 8 && smem >= WARPS * 16 * (D + 4) * 4 + WARPS * 16 * 8 && smem >= own_smem,
+                "the warps' states fit the ring");
+  void (*const kernel)(Params) = s.row_warps == 1 ? attend_parts<T, D, 1, NT> : attend_parts<T, D, 2, NT>;
+  cudaError_t e;
   const int prefix_items = s.prefix_parts * s.row_tiles * p.kv_heads, own_items = s.own_parts * p.kv_heads * p.seqs;
-  p.prefix_items = s.tc ? 0 : prefix_items;
   bool dependent = qmk_tc::pdl_active();
   if (s.tc) {
-    e = qmk_tc::launch_kernel(prefix_parts_tc<T, D>, dim3(prefix_items), dim3(TC_THREADS), tc_smem_bytes<D>(), stream, maps[0], maps[1], maps[2], p, s.seqs_per_tile,
-                              status);
-    if (e != cudaSuccess) return e;
+    p.prefix_items = 0;
+    e = cudaFuncSetAttribute(prefix_parts_tc<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(tc_smem_bytes<D>()));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(own_parts<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, own_smem);
+    if (e == cudaSuccess)
+      e = qmk_tc::launch_kernel(prefix_parts_tc<T, D>, dim3(prefix_items), dim3(TC_THREADS), tc_smem_bytes<D>(), stream, maps[0], maps[1], maps[2], p,
+                                s.seqs_per_tile, status);
     dependent = true;                            // (of the launch before, inside this call)
-  }
-  if (p.prefix_items + own_items > 0) {
-    const qmk_tc::PdlScope scope(dependent);
-    e = qmk_tc::launch_kernel(kernel, dim3(p.prefix_items + own_items), dim3(THREADS), smem, stream, p);
+    const qmk_tc::PdlScope scope(true);
+    if (e == cudaSuccess && own_items > 0) e = qmk_tc::launch_kernel(own_parts<T, D, NT>, dim3(own_items), dim3(THREADS), own_smem, stream, p);
+    if (e != cudaSuccess) return e;
+  } else if (prefix_items + own_items > 0) {
+    p.prefix_items = prefix_items;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) e = qmk_tc::launch_kernel(kernel, dim3(prefix_items + own_items), dim3(THREADS), prefix_items > 0 ? smem : own_smem, stream, p);
     if (e != cudaSuccess) return e;
     dependent = true;
   }
   const qmk_tc::PdlScope scope(dependent);
   return qmk_tc::launch_kernel(join_parts<T, D>, dim3(p.seqs * p.q_heads), dim3(128), 0, stream, p);
+}
+template <typename T>
+cudaError_t launch(Params &p, const Split &s, int head_dim, const CUtensorMap *maps, unsigned int *status, cudaStream_t stream) {
+  if (p.group > 8) return head_dim == 64 ? launch<T, 64, 2>(p, s, maps, status, stream) : launch<T, 128, 2>(p, s, maps, status, stream);
+  return head_dim == 64 ? launch<T, 64, 1>(p, s, maps, status, stream) : launch<T, 128, 1>(p, s, maps, status, stream);
 }
 
 }  // namespace
@@ -150,8 +159,7 @@ extern "C" int qmk_attention_shared_prefix(const qmk_shared_prefix_args *a, cuda
   p.part_ml = reinterpret_cast<float2 *>(p.part_out + states * a->head_dim);
   p.out = a->out;
   p.lse = a->lse;
-  const cudaError_t e = a->type == 0 ? (a->head_dim == 64 ? launch<__half, 64>(p, s, maps, status, stream) : launch<__half, 128>(p, s, maps, status, stream))
-                                     : (a->head_dim == 64 ? launch<__nv_bfloat16, 64>(p, s, maps, status, stream) : launch<__nv_bfloat16, 128>(p, s, maps, status, stream));
+  const cudaError_t e = a->type == 0 ? launch<__half>(p, s, a->head_dim, maps, status, stream) : launch<__nv_bfloat16>(p, s, a->head_dim, maps, status, stream);
   if (e != cudaSuccess) {
     cudaGetLastError();
     qmk_internal::note_error(std::string("qmk_attention_shared_prefix: ") + cudaGetErrorString(e));
