@@ -454,6 +454,24 @@ typedef struct qmk_shared_prefix_args {
 int qmk_attention_shared_prefix(const qmk_shared_prefix_args *args, cudaStream_t stream);
 long long qmk_attention_shared_prefix_workspace(int num_sequences, int q_heads, int kv_heads, int head_dim, int prefix_len, int own_rows);
 
+/* qmk_decode_batched with sampled picks and a shared prefix: many answers to one prompt, or many prompts behind one system prompt.  Every
+ * step picks with qmk_sample_tokens, sequence b with uniforms[step * num_sequences + b] (DEVICE) and its own temperatures[b], top_ks[b], top_ps[b],
+ * min_ps[b] (HOST arrays), and writes tokens and logarithms to output_logs[b] and logprob_logs[b] (HOST arrays of DEVICE pointers, num_steps entries
+ * each).  The attention is qmk_attention_shared_prefix: cache rows [0, prefix_len) of every sequence are those of k_prefix / v_prefix (caches of the
+ * usual shape, which may be one of k_caches; not read where prefix_len is 0) and are read once for all; a sequence's own cache is read from row prefix_len
+ * on, rows in front of that need not hold anything.  start_positions[b] >= prefix_len.  Queries are rounded to fp16 as in qmk_prefill_chunked.
+ * The remaining arguments, limits and errors are qmk_decode_batched's; blocks until done. */
+int qmk_sample_batched(
+    int num_sequences, const int *first_token_ids, const int *start_positions,
+    int num_steps, const void *embed_weight,
+    const struct LDGLayerWeight *layer_weights, const void *final_norm_weight,
+    const void *lm_head_weight, const void *cos_table, const void *sin_table,
+    const void *k_prefix, const void *v_prefix, int prefix_len,
+    void *const *k_caches, void *const *v_caches, const float *uniforms,
+    const float *temperatures, const int *top_ks, const float *top_ps, const float *min_ps,
+    int *const *output_logs, float *const *logprob_logs,
+    int num_layers, int max_seq_len, float attn_scale, cudaStream_t stream);
+
 /* Synchronises the device and returns the status word of the last launch
  * (QMK_OK, or the first error a CTA recorded). */
 int qmk_sync_status(void);

@@ -593,6 +593,67 @@ class BatchDecoder:
         return outs
 
 
+    def sample_ids(self, prompts: Sequence[Sequence[int]], max_tokens: int, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                   uniforms: Optional[torch.Tensor] = None, generator: Optional[torch.Generator] = None):
+        """Sampled answers, one per prompt: ``(token lists, logprob lists)``, cut at EOS (which is not returned).  The same prompt n times gives n
+        answers to it.  What all prompts begin with is read once per step for all of them (``sample_batched``), whatever engine decodes
+        greedily here; prompts that are all the same (but for the last token) are prefilled once, others each in their slot.
+
+        ``temperature`` (0: greedy), ``top_k`` (0: off), ``top_p`` (1: off), ``min_p`` (0: off): numbers, or a list with one per prompt;
+        ``uniforms``: fp32 CUDA tensor ``[max_tokens, len(prompts)]`` of numbers in [0, 1), drawn with ``generator`` where it is not given.
+        Behind the call slot 0 holds its prompt and answer, as does every slot of prompts that differ; the other slots of a prompt that was
+        prefilled once hold the answer alone and start from position 0."""
+        n = len(prompts)
+        if not 1 <= n <= self.num_sequences:
+            raise ValueError(f"between 1 and {self.num_sequences} prompts per call")
+        prompts = [list(ids) for ids in prompts]
+        max_tokens = int(max_tokens)
+        if any(not ids for ids in prompts):
+            raise ValueError("empty prompt")
+        if any(len(ids) - 1 + max_tokens > self.max_seq_len for ids in prompts):
+            raise ValueError("prompt + max_tokens exceeds max_seq_len")
+
+        def each(value, name):
+            values = list(value) if isinstance(value, (list, tuple)) else [value] * n
+            if len(values) != n:
+                raise ValueError(f"{name}: a number, or one per prompt")
+            return values
+        options = [each(v, name) for v, name in ((temperature, "temperature"), (top_k, "top_k"), (top_p, "top_p"), (min_p, "min_p"))]
+        heads = [ids[:-1] for ids in prompts]
+        shortest = min(heads, key=len)
+        shared = next((i for i, token in enumerate(shortest) if any(ids[i] != token for ids in heads)), len(shortest))
+        once = all(len(ids) == shared for ids in heads)
+        base = self._base
+        dev = base._embed_weight.device
+        steps = max(max_tokens, 0)
+        if uniforms is None:
+            uniforms = torch.rand(steps, n, device=dev, generator=generator)
+        elif tuple(uniforms.shape) != (steps, n):
+            raise ValueError(f"uniforms must be [{steps}, {n}]")
+        self.prefill_many([0] if once else list(range(n)), heads[:1] if once else heads)
+        if once:
+            self.positions[1:n] = [0] * (n - 1)
+        if steps == 0:
+            return [[] for _ in range(n)], [[] for _ in range(n)]
+        self._all_logs[:n, :steps].fill_(-1)
+        logprobs = torch.zeros(n, steps, dtype=torch.float32, device=dev)
+        base.apply_options()
+        _require_megakernel_op("sample_batched")(
+            [ids[-1] for ids in prompts], [len(ids) for ids in heads], steps, base._embed_weight, base._layer_weights_packed, base._final_norm_weight,
+            base._lm_head_weight, base._cos_table, base._sin_table, self._k_caches[0], self._v_caches[0], shared, self._k_caches[:n], self._v_caches[:n],
+            uniforms.contiguous(), *options, [self._logs[b][:steps] for b in range(n)], list(logprobs.unbind(0)), base.num_layers, self.max_seq_len,
+            base._attn_scale)
+        eos = base._eos()
+        outs, scores = [], []
+        for b, (tokens, values) in enumerate(zip(self._all_logs[:n, :steps].cpu().tolist(), logprobs.cpu().tolist())):
+            end = next((i for i, token in enumerate(tokens) if token == -1 or token == eos), steps)
+            outs.append(tokens[:end])
+            scores.append(values[:end])
+            if b == 0 or not once:
+                self.positions[b] += end
+        return outs, scores
+
+
 def generate(prompt: str, max_tokens: int = 50, verbose: bool = True) -> str:
     """Load the model, generate once, return the text."""
     text, _, _ = Decoder(verbose=verbose).generate(prompt, max_tokens)

@@ -1092,5 +1092,37 @@ __global__ void __launch_bounds__(256) argmax_pairs(const float *val, const int 
   }
 }
 
+// What the steps of a qmk_sample_batched call read beside the weights: options and addresses of the call, and what next_sampled_step leaves
+// for the step at hand.
+struct SampleState {
+  unsigned long long kv_ptrs[2 * 128];           // K and V cache of every sequence
+  float *logprob_logs[128];
+  float temperature[128], top_p[128], min_p[128];
+  int top_k[128];
+  const float *uniforms;                         // [steps][sequences]
+  int steps;
+  // of the step
+  int2 rows[128];                                // sequence and position, as qk_norm_rope_cache takes them
+  float u[128], logprobs[128];
+};
+// Behind a step's picks (picked = 1): they go to the logs and the positions advance.  Then, and in front of the first step (picked = 0), the
+// next one's rows and uniform numbers.  One block, a thread a sequence.
+__global__ void __launch_bounds__(128) next_sampled_step(SampleState *st, int picked, int batch, const int *tokens, int *const *log_ptrs,
+                                                         const int *start_positions, int *positions) {
+  pdl_wait();
+  pdl_trigger();
+  const int b = threadIdx.x;
+  if (b >= batch) return;
+  int pos = positions[b];
+  const int start = start_positions[b];
+  if (picked) {
+    log_ptrs[b][pos - start] = tokens[b];
+    st->logprob_logs[b][pos - start] = st->logprobs[b];
+    positions[b] = ++pos;
+  }
+  st->rows[b] = make_int2(b, pos);
+  if (pos - start < st->steps) st->u[b] = st->uniforms[static_cast<size_t>(pos - start) * batch + b];
+}
+
 }  // namespace qmk_pf
 #endif  // QMK_PREFILL_KERNELS_CUH_

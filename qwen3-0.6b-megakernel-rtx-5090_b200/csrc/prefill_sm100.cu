@@ -542,6 +542,12 @@ struct Workspace {                  // per device, allocated on first use, never
   cudaGraphExec_t step_graph[129] = {};
   unsigned long long step_key[129][12] = {};
   unsigned long long graph_epoch = 1;    // bumped whenever tensor maps baked into the graphs are rebuilt
+  // steps of qmk_sample_batched: theirs by batch size likewise, and what changes from call to call or step to step
+  cudaGraphExec_t sample_graph[129] = {};
+  std::vector<unsigned long long> sample_key[129];
+  qmk_pf::SampleState *sample = nullptr;
+  unsigned char *shared_ws = nullptr;    // attention over a shared prefix
+  size_t shared_ws_bytes = 0;
   __half **k_ptrs = nullptr, **v_ptrs = nullptr;
   CUtensorMap *kv_maps = nullptr;        // [128][2]: tiled-copy descriptors of every sequence's K and V cache (decode_attention_mma)
   unsigned char *packed = nullptr;       // tables of a packed prefill (row info, attention items, per-sequence descriptors and cache pointers)
@@ -1274,28 +1280,52 @@ int ensure_decode_workspace(Workspace &w, const void *lm_head, int vocab, int wq
   }
   return QMK_OK;
 }
+int ensure_sampling(Workspace &w, size_t attention_bytes) {
+  if (!w.sample) {
+    void *at = nullptr;
+    PF_CUDA(cudaMalloc(&at, sizeof(qmk_pf::SampleState)));
+    w.sample = static_cast<qmk_pf::SampleState *>(at);
+  }
+  if (w.shared_ws_bytes < attention_bytes) {
+    if (w.shared_ws) cudaFree(w.shared_ws);
+    w.shared_ws = nullptr;
+    w.shared_ws_bytes = 0;
+    void *at = nullptr;
+    PF_CUDA(cudaMalloc(&at, attention_bytes));
+    w.shared_ws = static_cast<unsigned char *>(at);
+    w.shared_ws_bytes = attention_bytes;
+  }
+  return QMK_OK;
+}
 }  // namespace
 
-extern "C" int qmk_decode_batched(int num_sequences, const int *first_token_ids, const int *start_positions, int num_steps,
-                                  const void *embed_weight, const LDGLayerWeight *layer_weights,
-                                  const void *final_norm_weight, const void *lm_head_weight, const void *cos_table,
-                                  const void *sin_table, void *const *k_caches, void *const *v_caches,
-                                  int *const *output_logs, int num_layers, int max_seq_len, float attn_scale,
-                                  cudaStream_t stream) {
-  qmk_internal::begin_call();
+// What qmk_sample_batched has beyond qmk_decode_batched.
+struct Sampling {
+  const void *k_prefix, *v_prefix;
+  int prefix_len;
+  const float *uniforms;
+  const float *temperatures;
+  const int *top_ks;
+  const float *top_ps, *min_ps;
+  float *const *logprob_logs;
+};
+static int decode_batched(const char *who, const Sampling *sampling, int num_sequences, const int *first_token_ids, const int *start_positions, int num_steps,
+                          const void *embed_weight, const LDGLayerWeight *layer_weights, const void *final_norm_weight, const void *lm_head_weight,
+                          const void *cos_table, const void *sin_table, void *const *k_caches, void *const *v_caches, int *const *output_logs,
+                          int num_layers, int max_seq_len, float attn_scale, cudaStream_t stream) {
   using namespace qmk_pf;
   if (num_steps <= 0) return QMK_OK;
   qmk_internal::PrefillEnv env;
   int rc = qmk_internal::prefill_env(max_seq_len, stream, &env);
   if (rc != QMK_OK) return rc;
   if (num_sequences < 1 || num_sequences > MAX_BATCH)
-    return qmk_internal::report(QMK_ERR_BAD_ARGUMENT, "qmk_decode_batched: num_sequences must be in [1, 128]");
+    return qmk_internal::report(QMK_ERR_BAD_ARGUMENT, std::string(who) + ": num_sequences must be in [1, 128]");
   if (!first_token_ids || !start_positions || !k_caches || !v_caches || !output_logs || !embed_weight || !layer_weights ||
       !final_norm_weight || !lm_head_weight)
-    return qmk_internal::report(QMK_ERR_BAD_ARGUMENT, "qmk_decode_batched: null pointer argument");
+    return qmk_internal::report(QMK_ERR_BAD_ARGUMENT, std::string(who) + ": null pointer argument");
   const int wq = env.wfmt;   // packed FP8 / NVFP4 matrices stay packed in HBM and are expanded inside the GEMMs
   if (env.vocab % 128 != 0)
-    return qmk_internal::report(QMK_ERR_BAD_ARGUMENT, "qmk_decode_batched needs a vocabulary that is a multiple of 128");
+    return qmk_internal::report(QMK_ERR_BAD_ARGUMENT, std::string(who) + " needs a vocabulary that is a multiple of 128");
   if (num_layers < 1 || num_layers > MAX_LAYERS)
     return qmk_internal::report(QMK_ERR_BAD_ARGUMENT, "num_layers must be in [1, 48]");
   if (env.rope_from_table && (!cos_table || !sin_table))
@@ -1303,14 +1333,27 @@ extern "C" int qmk_decode_batched(int num_sequences, const int *first_token_ids,
   const int B = num_sequences;
   for (int b = 0; b < B; ++b) {
     if (!k_caches[b] || !v_caches[b] || !output_logs[b])
-      return qmk_internal::report(QMK_ERR_BAD_ARGUMENT, "qmk_decode_batched: null cache or log pointer");
+      return qmk_internal::report(QMK_ERR_BAD_ARGUMENT, std::string(who) + ": null cache or log pointer");
     if (start_positions[b] < 0 || start_positions[b] + num_steps > max_seq_len)
       return qmk_internal::report(QMK_ERR_POSITION, "start_position + steps exceeds max_seq_len");
     if (first_token_ids[b] < 0 || first_token_ids[b] >= env.vocab)
       return qmk_internal::report(QMK_ERR_BAD_TOKEN, "first token outside [0, vocab)");
     for (int a = 0; a < b; ++a)
       if (k_caches[a] == k_caches[b] || v_caches[a] == v_caches[b] || output_logs[a] == output_logs[b])
-        return qmk_internal::report(QMK_ERR_BAD_ARGUMENT, "qmk_decode_batched: two sequences share a cache or an output log");
+        return qmk_internal::report(QMK_ERR_BAD_ARGUMENT, std::string(who) + ": two sequences share a cache or an output log");
+  }
+  if (sampling) {
+    if (!sampling->uniforms || !sampling->temperatures || !sampling->top_ks || !sampling->top_ps || !sampling->min_ps || !sampling->logprob_logs)
+      return qmk_internal::report(QMK_ERR_BAD_ARGUMENT, std::string(who) + ": null pointer argument");
+    if (sampling->prefix_len < 0 || (sampling->prefix_len > 0 && (!sampling->k_prefix || !sampling->v_prefix)))
+      return qmk_internal::report(QMK_ERR_BAD_ARGUMENT, std::string(who) + ": prefix_len is negative, or the prefix's caches are null");
+    for (int b = 0; b < B; ++b) {
+      if (start_positions[b] < sampling->prefix_len)
+        return qmk_internal::report(QMK_ERR_POSITION, std::string(who) + ": a sequence starts inside the shared prefix");
+      if (!sampling->logprob_logs[b]) return qmk_internal::report(QMK_ERR_BAD_ARGUMENT, std::string(who) + ": null cache or log pointer");
+      if (!(sampling->temperatures[b] >= 0.f) || !(sampling->top_ps[b] > 0.f) || !(sampling->min_ps[b] >= 0.f && sampling->min_ps[b] <= 1.f))
+        return qmk_internal::report(QMK_ERR_BAD_ARGUMENT, std::string(who) + ": temperature below 0, top_p not above 0 or min_p outside [0, 1]");
+    }
   }
   int dev = 0;
   PF_CUDA(cudaGetDevice(&dev));
@@ -1320,6 +1363,13 @@ extern "C" int qmk_decode_batched(int num_sequences, const int *first_token_ids,
   rc = ensure_workspace(w, 512);   // room for the split-K partial matrices (4 x 128 rows)
   if (rc == QMK_OK) rc = ensure_weight_maps(w, layer_weights, num_layers, wq, stream);
   if (rc == QMK_OK) rc = ensure_decode_workspace(w, lm_head_weight, env.vocab, wq);
+  // Rows of its own that a sequence may have in this call, in whole ranges of the attention's items.
+  int own_rows = 0;
+  if (sampling) {
+    for (int b = 0; b < B; ++b) own_rows = std::max(own_rows, start_positions[b] + num_steps - sampling->prefix_len);
+    own_rows = std::min((own_rows + 255) / 256 * 256, max_seq_len - sampling->prefix_len);
+    if (rc == QMK_OK) rc = ensure_sampling(w, static_cast<size_t>(qmk_attention_shared_prefix_workspace(B, NQ, NKV, D, sampling->prefix_len, own_rows)));
+  }
   if (rc != QMK_OK) return rc;
   std::vector<unsigned long long> rec(w.table, w.table + static_cast<size_t>(num_layers) * 12);
   const float *rope = env.rope_from_table ? nullptr : env.rope;
@@ -1336,7 +1386,22 @@ extern "C" int qmk_decode_batched(int num_sequences, const int *first_token_ids,
   PF_CUDA(cudaMemcpyAsync(w.log_ptrs, output_logs, sizeof(void *) * B, cudaMemcpyHostToDevice, stream));
   std::string err;
   std::vector<CUtensorMap> host_maps;
-  if (env.attn_mma) {   // per-sequence descriptors of the whole [layer][kv head][position] caches, boxes of 16 rows x 64 dims
+  SampleState host_state;
+  if (sampling) {
+    for (int b = 0; b < B; ++b) {
+      host_state.kv_ptrs[2 * b] = reinterpret_cast<unsigned long long>(k_caches[b]);
+      host_state.kv_ptrs[2 * b + 1] = reinterpret_cast<unsigned long long>(v_caches[b]);
+      host_state.logprob_logs[b] = sampling->logprob_logs[b];
+      host_state.temperature[b] = sampling->temperatures[b];
+      host_state.top_p[b] = sampling->top_ps[b];
+      host_state.min_p[b] = sampling->min_ps[b];
+      host_state.top_k[b] = sampling->top_ks[b];
+    }
+    host_state.uniforms = sampling->uniforms;
+    host_state.steps = num_steps;
+    PF_CUDA(cudaMemcpyAsync(w.sample, &host_state, sizeof(host_state), cudaMemcpyHostToDevice, stream));
+    PF_CUDA(cudaStreamSynchronize(stream));   // (the copy's source is this call's)
+  } else if (env.attn_mma) {   // per-sequence descriptors of the whole [layer][kv head][position] caches, boxes of 16 rows x 64 dims
     host_maps.resize(2 * static_cast<size_t>(B));
     const uint64_t cache_rows = static_cast<uint64_t>(num_layers) * NKV * static_cast<uint64_t>(max_seq_len);
     for (int b = 0; b < B && rc == QMK_OK; ++b) {
@@ -1416,7 +1481,40 @@ extern "C" int qmk_decode_batched(int num_sequences, const int *first_token_ids,
                                               live, a_box, wq, raws)) != QMK_OK)
           return r2;
       }
-      if (env.attn_mma)
+      if (sampling) {
+        // heads: normalised, rotated, queries as fp16, the new cache rows; then the shared rows once for all sequences and each one's own
+        PF_CUDA(qmk_tc::launch_kernel(qk_norm_rope_cache, dim3(B), dim3(256), 0, s, w.q, w.k, w.v, 0, reinterpret_cast<const __half *>(r[4]),
+                                      reinterpret_cast<const __half *>(r[5]), rope, cosv, sinv, w.qr, nullptr, nullptr, 0, max_seq_len, w.sample->rows,
+                                      w.sample->kv_ptrs, layer_off, 1.0f));
+        const void *k_own[MAX_BATCH], *v_own[MAX_BATCH];
+        for (int b = 0; b < B; ++b) {
+          k_own[b] = static_cast<const __half *>(k_caches[b]) + layer_off + static_cast<size_t>(sampling->prefix_len) * D;
+          v_own[b] = static_cast<const __half *>(v_caches[b]) + layer_off + static_cast<size_t>(sampling->prefix_len) * D;
+        }
+        qmk_shared_prefix_args a = {};
+        a.num_sequences = B;
+        a.q_heads = NQ;
+        a.kv_heads = NKV;
+        a.head_dim = D;
+        a.q = w.qr;
+        a.q_seq_stride = QS;
+        a.q_head_stride = D;
+        a.k_prefix = sampling->prefix_len ? static_cast<const __half *>(sampling->k_prefix) + layer_off : nullptr;
+        a.v_prefix = sampling->prefix_len ? static_cast<const __half *>(sampling->v_prefix) + layer_off : nullptr;
+        a.prefix_len = sampling->prefix_len;
+        a.prefix_row_stride = a.own_row_stride = D;
+        a.prefix_head_stride = a.own_head_stride = static_cast<long long>(max_seq_len) * D;
+        a.k_own = k_own;
+        a.v_own = v_own;
+        a.own_rows = own_rows;
+        a.own_lens = w.positions;
+        a.own_lens_add = 1 - sampling->prefix_len;      // (the row at the position itself has just been written)
+        a.scale = attn_scale;
+        a.out = w.attn;
+        a.workspace = w.shared_ws;
+        a.workspace_bytes = static_cast<long long>(w.shared_ws_bytes);
+        if ((r2 = qmk_attention_shared_prefix(&a, s)) != QMK_OK) { err = qmk_last_error(); return r2; }
+      } else if (env.attn_mma)
         PF_CUDA(qmk_tc::launch_kernel(decode_attention_mma<>, dim3(attn_ctas), dim3((DAM_WARPS + 1) * 32), DAM_SMEM_BYTES, s,
                                       w.q, w.k, w.v, reinterpret_cast<const __half *>(r[4]), reinterpret_cast<const __half *>(r[5]),
                                       rope, cosv, sinv, w.k_ptrs, w.v_ptrs, layer_off, w.attn_plan, l, w.attn, max_seq_len, attn_scale,
@@ -1448,14 +1546,19 @@ extern "C" int qmk_decode_batched(int num_sequences, const int *first_token_ids,
                                   static_cast<const __half *>(final_norm_weight), w.xn, nullptr));
     // Without a logits dump the LM head's epilogue picks the largest logit of each 128-column tile itself and the
     // rows of logits (B x 608 KB per step) are never written
-    const bool fused_pick = env.logits_out == nullptr;
+    const bool fused_pick = env.logits_out == nullptr && !sampling;
     if (fused_pick) qmk_tc::set_argmax_target(w.amax_val, w.amax_idx);
     qmk_tc::RingBudgetScope lm_scope(PREFILL_RING_BYTES);   // 1187 tiles: two CTAs per SM, four waves instead of eight
     r2 = qmk_tc::launch_gemm(w.map_xn_b, w.map_lm, w.logits, M, env.vocab, H, 128, w.status, env.timeout_ms, s, &err, live, a_box,
                              wq, lm_head_weight);
     qmk_tc::set_argmax_target(nullptr, nullptr);
     if (r2 != QMK_OK) return r2;
-    if (fused_pick)
+    if (sampling) {
+      SampleState *const st = w.sample;
+      if ((r2 = qmk_sample_tokens(w.logits, 0, env.vocab, B, env.vocab, st->u, st->temperature, 0.f, st->top_k, 0, st->top_p, 0.f, st->min_p, 0.f, w.tokens,
+                                  st->logprobs, s)) != QMK_OK) { err = qmk_last_error(); return r2; }
+      PF_CUDA(qmk_tc::launch_kernel(next_sampled_step, dim3(1), dim3(MAX_BATCH), 0, s, st, 1, B, w.tokens, w.log_ptrs, w.start_positions, w.positions));
+    } else if (fused_pick)
       PF_CUDA(qmk_tc::launch_kernel(argmax_pairs, dim3(B), dim3(256), 0, s, w.amax_val, w.amax_idx, env.vocab / 128, w.tokens,
                                     w.log_ptrs, w.start_positions, w.positions));
     else
@@ -1464,6 +1567,7 @@ extern "C" int qmk_decode_batched(int num_sequences, const int *first_token_ids,
     return QMK_OK;
   };
 
+  if (sampling) next_sampled_step<<<1, MAX_BATCH, 0, stream>>>(w.sample, 0, B, w.tokens, w.log_ptrs, w.start_positions, w.positions);
   if (env.logits_out) {
     // debug dump [sequence][step][vocab]: plain launches with a copy after every step
     for (int step = 0; step < num_steps && rc == QMK_OK; ++step) {
@@ -1486,25 +1590,40 @@ extern "C" int qmk_decode_batched(int num_sequences, const int *first_token_ids,
         reinterpret_cast<unsigned long long>(rope), reinterpret_cast<unsigned long long>(cos_table),
         reinterpret_cast<unsigned long long>(sin_table) ^ (static_cast<unsigned long long>(env.timeout_ms) << 48) ^
             (static_cast<unsigned long long>(env.pdl != 0) << 63) ^ (static_cast<unsigned long long>(env.attn_mma != 0) << 62)};
-    if (memcmp(key, w.step_key[B], sizeof(key)) != 0) {
-      if (w.step_graph[B]) { cudaGraphExecDestroy(w.step_graph[B]); w.step_graph[B] = nullptr; }
-      w.step_key[B][0] = 0;
+    // (a sampled step's attention has the caches' addresses in its launches)
+    std::vector<unsigned long long> sample_key;
+    if (sampling) {
+      sample_key.assign(key, key + 12);
+      for (unsigned long long v : {static_cast<unsigned long long>(sampling->prefix_len), static_cast<unsigned long long>(own_rows),
+                                   reinterpret_cast<unsigned long long>(sampling->k_prefix), reinterpret_cast<unsigned long long>(sampling->v_prefix),
+                                   reinterpret_cast<unsigned long long>(w.shared_ws), reinterpret_cast<unsigned long long>(w.logits)})
+        sample_key.push_back(v);
+      for (int b = 0; b < B; ++b) {
+        sample_key.push_back(reinterpret_cast<unsigned long long>(k_caches[b]));
+        sample_key.push_back(reinterpret_cast<unsigned long long>(v_caches[b]));
+      }
+    }
+    cudaGraphExec_t &step_graph = sampling ? w.sample_graph[B] : w.step_graph[B];
+    if (sampling ? sample_key != w.sample_key[B] : memcmp(key, w.step_key[B], sizeof(key)) != 0) {
+      if (step_graph) { cudaGraphExecDestroy(step_graph); step_graph = nullptr; }
+      if (sampling) w.sample_key[B].clear(); else w.step_key[B][0] = 0;
       cudaGraph_t graph = nullptr;
       PF_CUDA(cudaStreamBeginCapture(w.gstream, cudaStreamCaptureModeThreadLocal));
       rc = enqueue_step(w.gstream);
       cudaError_t ce = cudaStreamEndCapture(w.gstream, &graph);   // always end the capture, also after an error
       if (rc == QMK_OK && ce != cudaSuccess) { rc = QMK_ERR_CUDA; err = std::string("graph capture: ") + cudaGetErrorString(ce); }
       if (rc == QMK_OK) {
-        ce = cudaGraphInstantiate(&w.step_graph[B], graph, 0);
+        ce = cudaGraphInstantiate(&step_graph, graph, 0);
         if (ce != cudaSuccess) { rc = QMK_ERR_CUDA; err = std::string("cudaGraphInstantiate: ") + cudaGetErrorString(ce); }
       }
       if (graph) cudaGraphDestroy(graph);
-      if (rc == QMK_OK) memcpy(w.step_key[B], key, sizeof(key));
+      if (rc == QMK_OK && sampling) w.sample_key[B] = sample_key;
+      else if (rc == QMK_OK) memcpy(w.step_key[B], key, sizeof(key));
     }
     if (rc == QMK_OK) {
       PF_CUDA(cudaEventRecord(w.ev_in, stream));          // the graph stream starts after the caller's stream
       PF_CUDA(cudaStreamWaitEvent(w.gstream, w.ev_in, 0));
-      for (int step = 0; step < num_steps; ++step) PF_CUDA(cudaGraphLaunch(w.step_graph[B], w.gstream));
+      for (int step = 0; step < num_steps; ++step) PF_CUDA(cudaGraphLaunch(step_graph, w.gstream));
       PF_CUDA(cudaEventRecord(w.ev_out, w.gstream));
       PF_CUDA(cudaStreamWaitEvent(stream, w.ev_out, 0));  // ... and the caller's stream continues after it
     }
@@ -1518,6 +1637,29 @@ extern "C" int qmk_decode_batched(int num_sequences, const int *first_token_ids,
                                 host_status[0] == QMK_ERR_BAD_TOKEN ? "decode_batched: a pick outside [0, vocab) (logits without a largest value)"
                                                                     : "decode_batched: a bounded device wait ran out");
   return QMK_OK;
+}
+
+extern "C" int qmk_decode_batched(int num_sequences, const int *first_token_ids, const int *start_positions, int num_steps,
+                                  const void *embed_weight, const LDGLayerWeight *layer_weights,
+                                  const void *final_norm_weight, const void *lm_head_weight, const void *cos_table,
+                                  const void *sin_table, void *const *k_caches, void *const *v_caches,
+                                  int *const *output_logs, int num_layers, int max_seq_len, float attn_scale,
+                                  cudaStream_t stream) {
+  qmk_internal::begin_call();
+  return decode_batched("qmk_decode_batched", nullptr, num_sequences, first_token_ids, start_positions, num_steps, embed_weight, layer_weights,
+                        final_norm_weight, lm_head_weight, cos_table, sin_table, k_caches, v_caches, output_logs, num_layers, max_seq_len, attn_scale, stream);
+}
+
+extern "C" int qmk_sample_batched(int num_sequences, const int *first_token_ids, const int *start_positions, int num_steps, const void *embed_weight,
+                                  const LDGLayerWeight *layer_weights, const void *final_norm_weight, const void *lm_head_weight,
+                                  const void *cos_table, const void *sin_table, const void *k_prefix, const void *v_prefix, int prefix_len,
+                                  void *const *k_caches, void *const *v_caches, const float *uniforms, const float *temperatures, const int *top_ks,
+                                  const float *top_ps, const float *min_ps, int *const *output_logs, float *const *logprob_logs, int num_layers,
+                                  int max_seq_len, float attn_scale, cudaStream_t stream) {
+  qmk_internal::begin_call();
+  const Sampling sampling = {k_prefix, v_prefix, prefix_len, uniforms, temperatures, top_ks, top_ps, min_ps, logprob_logs};
+  return decode_batched("qmk_sample_batched", &sampling, num_sequences, first_token_ids, start_positions, num_steps, embed_weight, layer_weights,
+                        final_norm_weight, lm_head_weight, cos_table, sin_table, k_caches, v_caches, output_logs, num_layers, max_seq_len, attn_scale, stream);
 }
 
 // Bounded-wait self test of the GEMM kernel: one 128 x 128 tile whose loads are never issued.  The MMA thread's

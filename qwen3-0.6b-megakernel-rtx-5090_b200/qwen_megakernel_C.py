@@ -109,6 +109,8 @@ _lib.qmk_attention_shared_prefix.argtypes = [ctypes.POINTER(_SharedPrefixArgs), 
 _lib.qmk_attention_shared_prefix.restype = _I
 _lib.qmk_attention_shared_prefix_workspace.argtypes = [_I] * 6
 _lib.qmk_attention_shared_prefix_workspace.restype = _LL
+_lib.qmk_sample_batched.argtypes = [_I, _P, _P, _I, *([_P] * 6), _P, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _F, _P]
+_lib.qmk_sample_batched.restype = _I
 
 
 class _EngineConfig(ctypes.Structure):
@@ -148,7 +150,7 @@ _lib.qmk_selftest_gemm_pair_wait_timeout.restype = _I
 EXPORTED_SYMBOLS = (
     "launch_ldg_decode_direct", "launch_ldg_decode_persistent", "launch_ldg_generate_nosync",
     "launch_ldg_prefill", "qmk_abi_version", "qmk_configure", "qmk_set_inv_freq", "qmk_set_logits_dump",
-    "qmk_set_weight_format", "qmk_set_tuning", "qmk_set_tuning2", "qmk_set_profile_buffer", "qmk_set_fused", "qmk_set_step_overlap", "qmk_set_prefill_attention", "qmk_set_decode_attention", "qmk_invalidate_weights", "qmk_release_weights", "qmk_decode", "qmk_generate", "qmk_generate_static", "qmk_generate_batch", "qmk_gemm_f16_tn", "qmk_gemm_packed_tn", "qmk_sample_tokens", "qmk_attention_shared_prefix", "qmk_attention_shared_prefix_workspace", "qmk_decode_batched", "qmk_prefill_chunked", "qmk_prefill_packed", "qmk_prefill_packed_passes", "qmk_prefill", "qmk_engine_create", "qmk_engine_destroy", "qmk_engine_apply", "qmk_engine_decode", "qmk_engine_generate", "qmk_engine_prefill", "qmk_sync_status", "qmk_last_error", "qmk_num_ctas",
+    "qmk_set_weight_format", "qmk_set_tuning", "qmk_set_tuning2", "qmk_set_profile_buffer", "qmk_set_fused", "qmk_set_step_overlap", "qmk_set_prefill_attention", "qmk_set_decode_attention", "qmk_invalidate_weights", "qmk_release_weights", "qmk_decode", "qmk_generate", "qmk_generate_static", "qmk_generate_batch", "qmk_gemm_f16_tn", "qmk_gemm_packed_tn", "qmk_sample_tokens", "qmk_attention_shared_prefix", "qmk_attention_shared_prefix_workspace", "qmk_sample_batched", "qmk_decode_batched", "qmk_prefill_chunked", "qmk_prefill_packed", "qmk_prefill_packed_passes", "qmk_prefill", "qmk_engine_create", "qmk_engine_destroy", "qmk_engine_apply", "qmk_engine_decode", "qmk_engine_generate", "qmk_engine_prefill", "qmk_sync_status", "qmk_last_error", "qmk_num_ctas",
     "qmk_scratch_bytes", "qmk_selftest_decode_ring", "qmk_selftest_wait_timeout", "qmk_selftest_gemm_wait_timeout", "qmk_selftest_attention_wait_timeout", "qmk_selftest_gemm_pair_wait_timeout", "qmk_selftest_decode_attention_wait_timeout",
 )
 
@@ -518,6 +520,38 @@ def decode_batched(first_token_ids, start_positions, num_steps, embed_weight, la
     if rc != 0:
         raise RuntimeError(f"decode_batched: {_lib.qmk_last_error().decode()} (status {rc})")
     return output_logs
+
+
+def sample_batched(first_token_ids, start_positions, num_steps, embed_weight, layer_weights_packed, final_norm_weight, lm_head_weight, cos_table,
+                   sin_table, k_prefix, v_prefix, prefix_len, k_caches, v_caches, uniforms, temperatures, top_ks, top_ps, min_ps, output_logs,
+                   logprob_logs, num_layers, max_seq_len, attn_scale):
+    """``decode_batched`` with sampled picks over a shared prefix (``qmk_sample_batched``): every sequence's first ``prefix_len`` cache rows are
+    those of ``k_prefix`` / ``v_prefix`` (cache tensors; None where ``prefix_len`` is 0), its own cache is read from there on.  ``uniforms``: fp32
+    CUDA tensor ``[num_steps, n]``; ``temperatures`` / ``top_ks`` / ``top_ps`` / ``min_ps``: a number per sequence; ``output_logs`` int32 and
+    ``logprob_logs`` fp32 CUDA tensors of >= ``num_steps`` entries per sequence.  Blocks; raises ``RuntimeError`` on any reported error."""
+    _require_cuda()
+    n, num_steps = len(first_token_ids), int(num_steps)
+    _check(1 <= n <= MAX_GEMM_BATCH_SEQUENCES, "sample_batched: 1 to 128 sequences per call")
+    _check(all(len(v) == n for v in (start_positions, k_caches, v_caches, temperatures, top_ks, top_ps, min_ps, output_logs, logprob_logs)),
+           "sample_batched: per-sequence lists differ in length")
+    for logs, dtype in ((output_logs, torch.int32), (logprob_logs, torch.float32)):
+        for log in logs:
+            _check(log.dtype == dtype and log.is_cuda and log.is_contiguous() and log.numel() >= num_steps,
+                   f"sample_batched: each log must be a contiguous {dtype} CUDA tensor of >= num_steps entries")
+    _check(uniforms.dtype == torch.float32 and uniforms.is_cuda and uniforms.is_contiguous() and tuple(uniforms.shape) == (num_steps, n),
+           f"sample_batched: uniforms must be a contiguous fp32 CUDA tensor [{num_steps}, {n}]")
+    _check_table(layer_weights_packed, "sample_batched")
+    ints, floats, ptrs = ctypes.c_int * n, ctypes.c_float * n, ctypes.c_void_p * n
+    rc = _lib.qmk_sample_batched(
+        n, ints(*[int(t) for t in first_token_ids]), ints(*[int(p) for p in start_positions]), num_steps,
+        _ptr(embed_weight), _ptr(layer_weights_packed), _ptr(final_norm_weight), _ptr(lm_head_weight), _ptr(cos_table), _ptr(sin_table),
+        _ptr(k_prefix), _ptr(v_prefix), int(prefix_len), ptrs(*[_ptr(t) for t in k_caches]), ptrs(*[_ptr(t) for t in v_caches]),
+        _ptr(uniforms), floats(*[float(v) for v in temperatures]), ints(*[int(v) for v in top_ks]), floats(*[float(v) for v in top_ps]),
+        floats(*[float(v) for v in min_ps]), ptrs(*[_ptr(t) for t in output_logs]), ptrs(*[_ptr(t) for t in logprob_logs]),
+        int(num_layers), int(max_seq_len), float(attn_scale), _stream())
+    if rc != 0:
+        raise RuntimeError(f"sample_batched: {_lib.qmk_last_error().decode()} (status {rc})")
+    return output_logs, logprob_logs
 
 
 def prefill_chunked(token_ids, embed_weight, layer_weights_packed, cos_table, sin_table, k_cache, v_cache,

@@ -1,0 +1,182 @@
+"""``BatchDecoder.sample_ids`` / ``sample_batched``: sampled decode steps over a shared prefix, against the CPU oracle and the definition of a pick.
+
+Logits are compared with the oracle's on the same tokens under the bar of the batched decode (GEMM operands and queries are fp16: 3e-2).  Picks are
+compared for equality with the definition applied to the step's own logits, rows on a border excepted (see test_sample_tokens.py)."""
+
+import ctypes
+
+import pytest
+import torch
+
+import synthetic as S
+from oracle.decoder_ref import Decoder as OracleDecoder
+from test_sample_tokens import definition
+
+LOGIT_TOL = 3e-2
+VOCAB = 2048
+
+
+@pytest.fixture(scope="module")
+def C(built_library):
+    import qwen_megakernel_C
+    return qwen_megakernel_C
+
+
+@pytest.fixture(scope="module")
+def gpu(C):
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return C
+
+
+def _engine(w, n, max_seq_len, eos=-1, **kw):
+    from Model.Qwen06B_architecture import BatchDecoder
+    return BatchDecoder(weights=S.weights_to(w, "cuda"), tokenizer=S.StubTokenizer(eos, VOCAB), num_sequences=n, max_seq_len=max_seq_len, **kw)
+
+
+def _oracle_logits(w, prompt, tokens, max_seq_len):
+    """The oracle's logits of every step that picks one of ``tokens`` behind ``prompt``."""
+    o = OracleDecoder(w, max_seq_len=max_seq_len)
+    if len(prompt) > 1:
+        o.prefill(prompt[:-1])
+    rows = []
+    for token in [prompt[-1], *tokens[:-1]]:
+        o.step(token)
+        rows.append(o.last_logits.clone())
+    return torch.stack(rows)
+
+
+def _run(gpu, eng, prompts, steps, **kw):
+    dump = torch.zeros(len(prompts), steps, VOCAB, device="cuda")
+    gpu.set_logits_dump(dump)
+    try:
+        return (*eng.sample_ids(prompts, steps, **kw), dump.cpu())
+    finally:
+        gpu.set_logits_dump(None)
+
+
+def _check(w, eng, prompts, steps, tokens, logprobs, dump, uniforms, options, max_seq_len, which=None):
+    borders = 0
+    for b in which if which is not None else range(len(prompts)):
+        assert len(tokens[b]) == steps == len(logprobs[b])
+        assert float((dump[b] - _oracle_logits(w, prompts[b], tokens[b], max_seq_len)).abs().max()) < LOGIT_TOL, f"sequence {b}"
+        for i in range(steps):
+            t, k, p, m = (o[b] for o in options)
+            want, lp, near = definition(dump[b, i].double().numpy(), float(uniforms[i, b]), t, k, p, m)
+            borders += near
+            if not near:
+                assert tokens[b][i] == want, (b, i)
+                assert abs(logprobs[b][i] - lp) <= abs(lp) * 2.0 ** -24 + 2.0 ** -28
+    assert borders <= 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,prompt_len", [(1, 1), (2, 2), (5, 300), (20, 65), (70, 129)])
+def test_many_answers_to_one_prompt(gpu, n, prompt_len):
+    steps, L = 4, 384
+    w = S.make_weights(seed=31, num_layers=3, vocab_size=VOCAB, norm_std=0.1, max_seq_len=16)
+    prompts = [S.make_prompt(prompt_len, seed=3, vocab_size=VOCAB)] * n
+    g = torch.Generator().manual_seed(n)
+    uniforms = torch.rand(steps, n, generator=g)
+    options = [[0.7 + 0.1 * (i % 5) for i in range(n)], [(0, 50, 7)[i % 3] for i in range(n)], [(1.0, 0.9)[i % 2] for i in range(n)],
+               [(0.0, 0.0, 0.02)[i % 3] for i in range(n)]]
+    eng = _engine(w, n, L, engine="gemm", prefill_mode="tensor")
+    kw = dict(uniforms=uniforms.cuda(), temperature=options[0], top_k=options[1], top_p=options[2], min_p=options[3])
+    tokens, logprobs, dump = _run(gpu, eng, prompts, steps, **kw)
+    _check(w, eng, prompts, steps, tokens, logprobs, dump, uniforms, options, L, which=sorted({0, 1, n // 2, n - 1} & set(range(n))))
+    assert n < 5 or len({tuple(t) for t in tokens}) > 1
+    assert eng.positions[:n] == [prompt_len - 1 + steps] + [0] * (n - 1)
+    for _ in range(2):                               # without the dump a captured step is replayed: the same picks
+        again, again_lp = eng.sample_ids(prompts, steps, **kw)
+        assert again == tokens and again_lp == logprobs
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["fp16", "fp8", "nvfp4"])
+def test_prompts_with_a_common_beginning(gpu, fmt):
+    """Prompts that share their first 90 tokens and go on differently, at different lengths; their slots go on greedily behind it."""
+    n, steps, L = 6, 3, 256
+    w = S.make_weights(seed=33, num_layers=2, vocab_size=VOCAB, norm_std=0.1, max_seq_len=16)
+    import quantize as Q
+    packed = {"fp16": lambda x: x, "fp8": lambda x: Q.quantize_weights_fp8(x)[0], "nvfp4": lambda x: Q.quantize_weights_nvfp4(x)[0]}[fmt](w)
+    w = {"fp16": lambda x: x, "fp8": lambda x: Q.expand_weights_fp8(x)[1], "nvfp4": lambda x: Q.expand_weights_nvfp4(x)[1]}[fmt](w)
+    system = S.make_prompt(90, seed=5, vocab_size=VOCAB)
+    prompts = [system + S.make_prompt(1 + 13 * i, seed=50 + i, vocab_size=VOCAB) for i in range(n)]
+    uniforms = torch.rand(steps, n, generator=torch.Generator().manual_seed(1))
+    options = [[0.9] * n, [0] * n, [0.95] * n, [0.0] * n]
+    eng = _engine(packed, n, L, engine="gemm", prefill_mode="tensor", weight_format=fmt)
+    tokens, logprobs, dump = _run(gpu, eng, prompts, steps, uniforms=uniforms.cuda(), temperature=0.9, top_p=0.95)
+    _check(w, eng, prompts, steps, tokens, logprobs, dump, uniforms, options, L)
+    assert eng.positions == [len(p) - 1 + steps for p in prompts]
+    more = eng.decode_slots(list(range(n)), [t[-1] for t in tokens], 2)
+    gpu.set_weight_format("fp16")
+    for b in range(n):
+        o = OracleDecoder(w, max_seq_len=L)
+        o.prefill(prompts[b] + tokens[b][:-1])
+        assert more[b] == [o.step(tokens[b][-1]), o.step(more[b][0])]
+
+
+@pytest.mark.gpu
+def test_temperature_zero_is_the_greedy_decode(gpu):
+    n, steps, L = 7, 6, 256
+    w = S.make_weights(seed=35, num_layers=3, vocab_size=VOCAB, norm_std=0.1, max_seq_len=16)
+    prompts = [S.make_prompt(5 + 20 * i, seed=70 + i, vocab_size=VOCAB) for i in range(n)]
+    eng = _engine(w, n, L, engine="gemm", prefill_mode="tensor")
+    greedy = eng.generate_ids(prompts, steps)
+    tokens, logprobs = eng.sample_ids(prompts, steps, temperature=0.0)
+    assert tokens == greedy and logprobs == [[0.0] * steps] * n
+    assert eng.generate_ids(prompts, steps) == greedy            # (graphs of both kinds of steps side by side)
+
+
+@pytest.mark.gpu
+def test_seeds_ends_and_other_engines(gpu):
+    steps, L = 12, 128
+    w = S.make_weights(seed=37, num_layers=2, vocab_size=VOCAB, norm_std=0.1, max_seq_len=16)
+    prompt = S.make_prompt(30, seed=8, vocab_size=VOCAB)
+
+    def draw(eng, seed, **kw):
+        return eng.sample_ids([prompt] * 3, steps, temperature=1.0, top_k=40, generator=torch.Generator("cuda").manual_seed(seed), **kw)[0]
+    eng = _engine(w, 3, L)                           # the engine that decodes greedily in one persistent launch
+    first = draw(eng, 1)
+    assert draw(eng, 1) == first and draw(eng, 2) != first and all(0 <= t < VOCAB for ids in first for t in ids)
+    eos = first[1][4]
+    cut = draw(_engine(w, 3, L, eos=eos), 1)
+    assert cut == [ids[:ids.index(eos)] if eos in ids else ids for ids in first]
+    assert eng.sample_ids([prompt], 0) == ([[]], [[]])
+    for bad in (dict(prompts=[]), dict(prompts=[prompt] * 4), dict(prompts=[[]]), dict(prompts=[prompt], max_tokens=200),
+                dict(prompts=[prompt], top_k=[1, 2]), dict(prompts=[prompt], uniforms=torch.zeros(3, 1, device="cuda"))):
+        with pytest.raises(ValueError):
+            eng.sample_ids(**{"max_tokens": steps, **bad})
+    for bad in (dict(temperature=-1.0), dict(top_p=0.0), dict(min_p=2.0)):
+        with pytest.raises(RuntimeError):
+            eng.sample_ids([prompt], steps, **bad)
+    assert draw(eng, 1) == first
+
+
+@pytest.mark.gpu
+def test_refusals_leave_a_text(gpu):
+    eng = _engine(S.make_weights(seed=37, num_layers=2, vocab_size=VOCAB, norm_std=0.1, max_seq_len=16), 2, 64)
+    base = eng._base
+    base.apply_options()
+    logs = [torch.zeros(4, dtype=torch.int32, device="cuda") for _ in range(2)]
+    scores = [torch.zeros(4, device="cuda") for _ in range(2)]
+    def call(**change):
+        a = dict(first=[1, 2], start=[8, 9], steps=4, prefix=(eng._k_caches[0], eng._v_caches[0], 8), k=eng._k_caches, v=eng._v_caches, t=[1.0, 1.0])
+        a.update(change)
+        gpu.sample_batched(a["first"], a["start"], a["steps"], base._embed_weight, base._layer_weights_packed, base._final_norm_weight, base._lm_head_weight,
+                           base._cos_table, base._sin_table, *a["prefix"], a["k"], a["v"], torch.rand(a["steps"], 2, device="cuda"), a["t"], [0, 0], [1.0, 1.0],
+                           [0.0, 0.0], logs, scores, base.num_layers, 64, base._attn_scale)
+    call()
+    for change, text in ((dict(start=[8, 7]), "inside the shared prefix"), (dict(prefix=(None, None, 8)), "prefix"), (dict(prefix=(eng._k_caches[0], eng._v_caches[0], -1)), "prefix"),
+                         (dict(start=[8, 61]), "max_seq_len"), (dict(first=[1, VOCAB]), "vocab"), (dict(k=[eng._k_caches[0]] * 2), "share"), (dict(t=[1.0, -1.0]), "temperature")):
+        with pytest.raises(RuntimeError, match=text):
+            call(**change)
+    call()
+
+
+def test_null_pointers_are_refused(C):
+    lib = C._lib
+    if torch.cuda.is_available():
+        assert lib.qmk_sample_batched(1, None, None, 1, *[None] * 8, 0, *[None] * 9, 1, 64, 1.0, None) != 0 and b"null" in lib.qmk_last_error()
+    else:
+        assert lib.qmk_sample_batched(1, None, None, 1, *[None] * 8, 0, *[None] * 9, 1, 64, 1.0, None) != 0 and lib.qmk_last_error() == b"no CUDA device"
