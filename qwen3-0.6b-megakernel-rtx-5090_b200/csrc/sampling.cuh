@@ -430,6 +430,73 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
     find(block_sum(sum), s.warp, bound, value, target, found);
   };
 
+  // s.sorted[0 .. count) to descending order, by `key`, a number that does not grow along it: entries go to 2048 buckets between the largest and the
+  // smallest key, and each finds its place among its bucket's few.  (A bitonic sort of 2048 took 13 us, this takes XXX.)  Crowded buckets, and short
+  // lists, are left to the bitonic sort.
+  auto sort_by = [&](int count, auto &&key) {
+    int size = 32;
+    while (size < count) size <<= 1;
+    if (size > 64) {
+      unsigned long long c[EACH];
+      float k[EACH], high = -INFINITY, low = INFINITY;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) {
+        const int i = tid + j * THREADS;
+        c[j] = i < count ? s.sorted[i] : 0;
+        k[j] = i < count ? key(c[j]) : 0.0f;
+        if (i < count) { high = fmaxf(high, k[j]); low = fminf(low, k[j]); }
+        s.counts[i] = 0;
+      }
+      const uint32_t up = __reduce_max_sync(0xffffffffu, key_of(high)), down = __reduce_min_sync(0xffffffffu, key_of(low));
+      if (lane == 0) s.warp[warp] = (static_cast<unsigned long long>(up) << 32) | down;
+      __syncthreads();
+      uint32_t top_key = 0, low_key = 0xffffffffu;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) { top_key = max(top_key, static_cast<uint32_t>(s.warp[w] >> 32)); low_key = min(low_key, static_cast<uint32_t>(s.warp[w])); }
+      high = value_of(static_cast<unsigned long long>(top_key) << 32);
+      low = value_of(static_cast<unsigned long long>(low_key) << 32);
+      const float scale = high > low ? (BINS - 1) / (high - low) : 0.0f;
+      int b[EACH], slot[EACH];
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) {
+        b[j] = min(max(static_cast<int>((high - k[j]) * scale), 0), BINS - 1);
+        slot[j] = tid + j * THREADS < count ? static_cast<int>(atomicAdd(&s.counts[b[j]], 1u)) : 0;
+      }
+      __syncthreads();
+      const uint4 n4_ = reinterpret_cast<const uint4 *>(s.counts)[tid];
+      unsigned long long before;
+      block_scan(static_cast<unsigned long long>(n4_.x) + n4_.y + n4_.z + n4_.w, before);
+      const uint32_t at = static_cast<uint32_t>(before);
+      reinterpret_cast<uint4 *>(s.counts)[tid] = make_uint4(at, at + n4_.x, at + n4_.x + n4_.y, at + n4_.x + n4_.y + n4_.z);
+      const bool crowded = __syncthreads_or(max(max(n4_.x, n4_.y), max(n4_.z, n4_.w)) > 32);
+      if (!crowded) {
+#pragma unroll
+        for (int j = 0; j < EACH; ++j)
+          if (tid + j * THREADS < count) s.sorted[s.counts[b[j]] + slot[j]] = c[j];
+        __syncthreads();
+        int place[EACH];
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+          place[j] = 0;
+          if (tid + j * THREADS < count) {
+            const int from = static_cast<int>(s.counts[b[j]]), to = b[j] + 1 < BINS ? static_cast<int>(s.counts[b[j] + 1]) : count;
+            place[j] = from;
+            for (int i = from; i < to; ++i) place[j] += s.sorted[i] > c[j];
+          }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < EACH; ++j)
+          if (tid + j * THREADS < count) s.sorted[place[j]] = c[j];
+        __syncthreads();
+        return;
+      }
+    }
+    for (int i = count + tid; i < size; i += THREADS) s.sorted[i] = 0;
+    sort_descending(s.sorted, size, tid);
+  };
+
   // Candidates: to the CTA's own list, then (collect) to rank 0's, in any order, where they are sorted, largest first.  Their number in all;
   // more than LIST: nothing is sorted.  The others have nothing more to give rank 0 then and may leave.
   auto list = [&](float v, int i) {
@@ -448,12 +515,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
     }
     int total = 0;
     gather(mine, [&](int, unsigned long long c) { total += static_cast<int>(c); });
-    if (rank == 0 && total <= LIST) {
-      int size = 32;
-      while (size < total) size <<= 1;
-      for (int i = total + tid; i < size; i += THREADS) s.sorted[i] = 0;
-      sort_descending(s.sorted, size, tid);
-    }
+    if (rank == 0 && total <= LIST) sort_by(total, [](unsigned long long place) { return value_of(place); });
     return total;
   };
   // rank 0: the threshold behind the sorted candidate number `count` (from 1 on), to every CTA
@@ -481,12 +543,10 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
       stay += __syncthreads_count(keep);
       before += m[j];
     }
-    int size = 32;
-    while (size < stay) size <<= 1;
 #pragma unroll
     for (int j = 0; j < EACH; ++j)                // the halves change places: by index, the lowest (its complement the largest) first
-      if (EACH * tid + j < size) s.sorted[EACH * tid + j] = EACH * tid + j < stay ? (c[j] << 32) | (c[j] >> 32) : 0;
-    sort_descending(s.sorted, size, tid);
+      if (EACH * tid + j < stay) s.sorted[EACH * tid + j] = (c[j] << 32) | (c[j] >> 32);
+    sort_by(stay, [](unsigned long long swapped) { return -static_cast<float>(~static_cast<uint32_t>(swapped >> 32)); });
     sum = 0;
 #pragma unroll
     for (int j = 0; j < EACH; ++j) {
