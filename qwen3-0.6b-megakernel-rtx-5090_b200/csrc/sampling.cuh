@@ -36,7 +36,8 @@ constexpr int MAX_CLUSTER = 8;
 constexpr int GROUPS = (MAX_VOCAB / 4 + 1 + WARPS * 32 - 1) / (WARPS * 32);   // of 128 tokens, in a warp's range of a row: at most
 constexpr int BINS = 2048;                       // of the distance to the maximum: 4 per thread
 constexpr float SPAN = 32.5f;                    // times the temperature: masses further below the maximum round to nothing (e^-32.5 < 2^-46)
-constexpr float ONE = 8192.0f;                   // a mass of its bin's middle in a histogram of masses: 2^18 of them fit 32 bits
+constexpr int MASS_BINS = 3072;                  // of masses, 2^(1/64) wide, down to 2^-48: 6 per thread
+constexpr double ONE = 8192.0;                   // a mass of its bin's middle in a histogram of masses: 2^18 of them fit 32 bits
 constexpr int KEY_BINS = 256;                    // of a histogram of keys: eight bits
 constexpr int LIST = 2048;                       // tokens that one CTA sorts: EACH per thread
 constexpr int STEPS = 64, COLUMNS = 16;            // of the table of powers, see power_polynomial
@@ -45,7 +46,7 @@ constexpr int NO_TOKEN = 0x7fffffff;             // pick of a row without a larg
 constexpr float LARGEST_UNIFORM = 0x1.fffffep-1f;
 constexpr float LARGEST_TEMPERATURE = 0x1p100f;  // (SPAN temperatures and the products with it stay finite)
 constexpr int EACH = LIST / THREADS;
-static_assert(BINS == 4 * THREADS && LIST == 4 * THREADS, "bins and list entries per thread");
+static_assert(BINS == 4 * THREADS && MASS_BINS == 6 * THREADS && LIST == 4 * THREADS, "bins and list entries per thread");
 
 struct Params {
   const void *logits;
@@ -61,7 +62,7 @@ struct Params {
 };
 
 struct __align__(16) Shared {
-  unsigned int counts[BINS];                     // this CTA's histogram, read by the cluster: tokens, or their masses (see share)
+  unsigned int counts[MASS_BINS];                // this CTA's histogram, read by the cluster: of tokens (BINS) or of masses
   union {
     unsigned long long keys[2][KEY_BINS];    // search: histograms in turn, one is read while the next is filled
     unsigned long long sorted[LIST];
@@ -70,9 +71,9 @@ struct __align__(16) Shared {
   double powers[STEPS * COLUMNS];                // 2^(j / 64), a column for each lane of half a warp
   unsigned long long warp[WARPS], warp_kept[WARPS], group[GROUPS];
   unsigned long long inbox[16][MAX_CLUSTER];     // one row per exchange of the cluster, see gather
-  unsigned long long found[4];
+  unsigned long long found[4], border[4];
   unsigned long long threshold;                  // written by the CTA that finds it
-  int listed, collected, bin_lo, bin_hi;
+  int listed, collected;
 };
 
 static_assert(sizeof(Shared) % 16 == 0 && offsetof(Shared, keys) % 16 == 0, "vector accesses");
@@ -271,7 +272,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
   };
 
   // ---- the row, once; its largest value and where that is first
-  for (int b = tid; b < BINS / 4; b += THREADS) reinterpret_cast<uint4 *>(s.counts)[b] = make_uint4(0, 0, 0, 0);
+  for (int b = tid; b < MASS_BINS / 4; b += THREADS) reinterpret_cast<uint4 *>(s.counts)[b] = make_uint4(0, 0, 0, 0);
   if (tid == 0) { s.listed = 0; s.collected = 0; }
   for (int i = tid; i < STEPS * COLUMNS; i += THREADS) s.powers[i] = exp2(static_cast<double>(i / COLUMNS) / STEPS);      // (read behind the first barrier)
   float high[TURN] = {-INFINITY, -INFINITY, -INFINITY};          // the largest values of three parts of what this thread has seen
@@ -332,21 +333,29 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
   const float nothing = top - 1.01f * SPAN * temperature;      // below it masses round to 0 (and the exponent of 2 may be any)
   const double *const powers = s.powers + (lane & (COLUMNS - 1));
   // 2^n 2^(j / 64) and the polynomial whose product is the mass of v
-  auto factors = [&](float v, double &power) {
+  auto factors = [&](float v, double &power, int &k) {
     constexpr double magic = 6755399441055744.0;             // 1.5 * 2^52: the sum's low word is the nearest whole number
     const double d = static_cast<double>(v) - top64, y = fma(d, slope, magic);
-    const int k = __double2loint(y);
+    k = __double2loint(y);
     const double p = powers[(k & (STEPS - 1)) * COLUMNS];
     power = __hiloint2double(__double2hiint(p) + ((k >> 6) << 20), __double2loint(p));
     return power_polynomial(fma(d, slope, -(y - magic)));
   };
-  auto weight = [&](float v) { double power; const double q = factors(v, power); return power * q; };
-  auto mass = [&](float v) {                     // (chosen behind the arithmetic: four tokens' run side by side)
+  auto weight = [&](float v) { double power; int k; const double q = factors(v, power, k); return power * q; };
+  // ... and the bin of masses, 64ths of a power of two below the maximum, with the mass in units of its bin's middle (ONE)
+  auto mass_and_bin = [&](float v, int &bin, unsigned int &units) {      // (chosen behind the arithmetic: four tokens' run side by side)
     double power;
-    const double q = factors(v, power);
+    int k;
+    const double q = factors(v, power, k);
     const unsigned long long m = mass_of(fma(power, q, 128.0));
+    units = static_cast<unsigned int>(__double2loint(fma(q, ONE, 4503599627370496.0)));
+    bin = v >= nothing ? -k : MASS_BINS;
     return v >= nothing ? m : 0ull;
   };
+  auto mass = [&](float v) { int bin; unsigned int units; return mass_and_bin(v, bin, units); };
+  auto mass_bin = [&](float v) { return v >= nothing ? -__double2loint(fma(static_cast<double>(v) - top64, slope, 6755399441055744.0)) : MASS_BINS; };
+  // no value of the bins 0 .. j of masses is below this
+  auto mass_bound = [&](int j) { return top - (static_cast<float>(j) + 0.51f) * temperature * (0.6931472f / STEPS) * (1.0f + 1e-5f) - 1e-6f * fabsf(top); };
   // min_p: a bound for the values that stay, a little low, and the mass of those that do
   const float least_value = least > 0.0 ? static_cast<float>(top64 + log_least * static_cast<double>(temperature) * (1.0 + 1e-6) - 1e-6 * fabs(top64)) : -INFINITY;
   auto above_least = [&](float v) {
@@ -436,7 +445,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
   auto sort_by = [&](int count, auto &&key) {
     int size = 32;
     while (size < count) size <<= 1;
-    if (size > 64) {
+    if (size > 32) {
       unsigned long long c[EACH];
       float k[EACH], high = -INFINITY, low = INFINITY;
       __syncthreads();
@@ -469,7 +478,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
       block_scan(static_cast<unsigned long long>(n4_.x) + n4_.y + n4_.z + n4_.w, before);
       const uint32_t at = static_cast<uint32_t>(before);
       reinterpret_cast<uint4 *>(s.counts)[tid] = make_uint4(at, at + n4_.x, at + n4_.x + n4_.y, at + n4_.x + n4_.y + n4_.z);
-      const bool crowded = __syncthreads_or(max(max(n4_.x, n4_.y), max(n4_.z, n4_.w)) > 32);
+      const bool crowded = __syncthreads_or(max(max(n4_.x, n4_.y), max(n4_.z, n4_.w)) > 256);
       if (!crowded) {
 #pragma unroll
         for (int j = 0; j < EACH; ++j)
@@ -625,25 +634,49 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
     const float b = fmaf(top - v, per_bin, 8388608.0f);        // (the last bit is 1: rounded to the nearest whole number)
     return b < 8388608.0f + BINS ? static_cast<int>(__float_as_uint(b) & 0xffffu) : BINS;
   };
-  // ... and the mass over that of the bin's middle, e^-(d f) with f in [-1/2, 1/2] and d = SPAN / BINS, as 1 - d f (off by 3.2e-5), times ONE and
-  // rounded (6.2e-5)
-  auto bin_and_mass = [&](float v, unsigned int &m) {
-    const float b = fmaf(top - v, per_bin, 8388608.0f), f = fmaf(top - v, per_bin, 8388608.0f - b);
-    m = __float_as_uint(fmaf(f, -SPAN / BINS * ONE, 8388608.0f + ONE)) & 0xffffu;
-    return b < 8388608.0f + BINS ? static_cast<int>(__float_as_uint(b) & 0xffffu) : BINS;
-  };
   // no value of the bins 0 .. j is below this
   auto bound_of = [&](int j) { return top - (static_cast<float>(j) + 0.51f) / per_bin * (1.0f + 1e-5f) - 1e-6f * fabsf(top); };
-  auto clear_counts = [&]() { reinterpret_cast<uint4 *>(s.counts)[tid] = make_uint4(0, 0, 0, 0); };
-  // counts of the cluster in the bins 4 tid .. 4 tid + 3, and of all bins in front
-  auto cluster_counts = [&](unsigned int (&c)[4], unsigned long long &before) {
-    c[0] = c[1] = c[2] = c[3] = 0;
+  auto clear_counts = [&]() { for (int b = tid; b < MASS_BINS / 4; b += THREADS) reinterpret_cast<uint4 *>(s.counts)[b] = make_uint4(0, 0, 0, 0); };
+  // The cluster's histogram: a CTA adds up its share of the bins, of which a thread has up to six, one behind the other.  (Every CTA reading
+  // all of the others' 3072 bins took 10 us.)
+  struct Share { unsigned int c[6]; int bin, mine; };
+  auto share_of_bins = [&](int bins) {
+    Share h;
+    const int all = bins / ranks, each_ = (all + THREADS - 1) / THREADS;
+    h.bin = rank * all + tid * each_;
+    h.mine = max(0, min(each_, all - tid * each_));
 #pragma unroll
-    for (int r = 0; r < MAX_CLUSTER; ++r) {
-      const uint4 o = r < ranks ? cluster.map_shared_rank(reinterpret_cast<uint4 *>(s.counts), r)[tid] : make_uint4(0, 0, 0, 0);
-      c[0] += o.x; c[1] += o.y; c[2] += o.z; c[3] += o.w;
+    for (int j = 0; j < 6; ++j) {
+      h.c[j] = 0;
+      if (j < h.mine) {
+#pragma unroll
+        for (int r = 0; r < MAX_CLUSTER; ++r) h.c[j] += r < ranks ? cluster.map_shared_rank(s.counts, r)[h.bin + j] : 0;
+      }
     }
-    return block_scan(static_cast<unsigned long long>(c[0]) + c[1] + c[2] + c[3], before);
+    return h;
+  };
+  // The bin in which the running count reaches k, the counts in front of it and up to it, to every CTA (Shared::border); returns the count of all.
+  auto count_border = [&](unsigned long long k) {
+    const Share h = share_of_bins(BINS);
+    unsigned long long before, front = 0, total = 0, sum = 0;
+#pragma unroll
+    for (int j = 0; j < 6; ++j) sum += h.c[j];
+    const unsigned long long mine = block_scan(sum, before);
+    gather(mine, [&](int r, unsigned long long v) { front += r < rank ? v : 0; total += v; });
+    before += front;
+#pragma unroll
+    for (int j = 0; j < 6; ++j) {
+      if (j < h.mine && before < k && k <= before + h.c[j])
+        for (int r = 0; r < ranks; ++r) {
+          unsigned long long *const to = cluster.map_shared_rank(s.border, r);
+          to[0] = h.bin + j;
+          to[1] = before;
+          to[2] = before + h.c[j];
+        }
+      before += h.c[j];
+    }
+    cluster.sync();
+    return total;
   };
 
   // Kept: tokens whose place is not below the threshold.
@@ -654,8 +687,6 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
   auto kept = [&](float v, int i) { return v > kept_value || (v == kept_value && i <= kept_index); };
   if (top_k > 0 && top_k < p.vocab) {
     const unsigned long long k = static_cast<unsigned long long>(top_k);
-    unsigned int c[4];
-    unsigned long long before, counted;
     // Few: the largest values of the threads' parts are k tokens at least down to some bin, which leaves out most others without a look at them.
     if (top_k <= LIST * 5 / 8 && top_k * 2 <= min(TURN * ranks * THREADS, fours)) {
 #pragma unroll
@@ -664,16 +695,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
         if (b < BINS) atomicAdd(&s.counts[b], 1u);
       }
       cluster.sync();
-      counted = cluster_counts(c, before);
-      if (tid == 0) s.bin_hi = BINS - 1;
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (before < k && k <= before + c[j]) s.bin_hi = 4 * tid + j;
-        before += c[j];
-      }
-      __syncthreads();
-      const int border = s.bin_hi;
+      const int border = count_border(k) < k ? BINS - 1 : static_cast<int>(s.border[0]);
       each_from(bound_of(border), [&](float v, int i) { if (bin_of(v) <= border) list(v, i); });
       const int total = collect();
       if (total <= LIST) {
@@ -686,16 +708,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
     }
     each([&](float v, int) { const int b = bin_of(v); if (b < BINS) atomicAdd(&s.counts[b], 1u); });
     cluster.sync();
-    counted = cluster_counts(c, before);
-    if (counted > k) {                           // (otherwise every token that has a mass stays)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (before < k && k <= before + c[j]) { s.bin_hi = 4 * tid + j; s.found[0] = before; s.found[1] = before + c[j]; }
-        before += c[j];
-      }
-      __syncthreads();
-      const int border = s.bin_hi;
-      const unsigned long long above = s.found[0], up_to = s.found[1];
+    if (count_border(k) > k) {                   // (otherwise every token that has a mass stays)
+      const int border = static_cast<int>(s.border[0]);
+      const unsigned long long above = s.border[1], up_to = s.border[2];
       if (up_to <= LIST) {
         each_from(bound_of(border), [&](float v, int i) { if (bin_of(v) <= border) list(v, i); });
         const int total = collect();
@@ -711,9 +726,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
       } else {
         cut_at(search([&](float, int) { return 1ull; }, [&](unsigned long long) { return k; }));
       }
-    } else {
-      cluster.sync();
     }
+    cluster.sync();
     clear_counts();
     if (tid == 0) { s.listed = 0; s.collected = 0; }
     cluster.sync();                              // (rank 0's counter is the others')
@@ -722,74 +736,75 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
     unsigned long long sum = 0;
     walk([&](float4 v4, int i, int) {              // (four tokens' arithmetic side by side, then the atomics)
       const float v[4] = {v4.x, v4.y, v4.z, v4.w};
-      unsigned int q[4];
+      unsigned int units[4];
       int b[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        b[j] = bin_and_mass(v[j], q[j]);
-        const unsigned long long m = mass(v[j]);
-        if (cut && !kept(v[j], first + 4 * i + j)) b[j] = BINS;
-        sum += b[j] < BINS ? m : 0;
+        unsigned long long m = mass_and_bin(v[j], b[j], units[j]);
+        if (cut && !kept(v[j], first + 4 * i + j)) { b[j] = MASS_BINS; m = 0; }
+        sum += m;
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (b[j] < BINS) atomicAdd(&s.counts[b[j]], q[j]);
+        if (b[j] < MASS_BINS) atomicAdd(&s.counts[b[j]], units[j]);
     });
-    if (tid == 0) { s.bin_lo = 0; s.bin_hi = BINS - 1; }
+    // (as long as nobody finds them: the first bin with nothing in front, the last with everything up to it)
+    if (tid == 0) { s.border[0] = 0; s.border[1] = 0; s.border[2] = MASS_BINS - 1; s.border[3] = ~0ull; }
     const unsigned long long own = block_sum(sum);
     unsigned long long total = 0;
     gather(own, [&](int, unsigned long long v) { total += v; });
     const unsigned long long want = share_of(total);
-    // The border's bin, or a few that it may be in: the histogram's sums are off by 1.2e-4 (above, and the roundings of the bin's number and middle), and
-    // masses by 2^-46 each.
-    unsigned int c[4];
-    unsigned long long unused, low[4], high[4], below, ahead;
-    cluster_counts(c, unused);
+    // The border's bin, or a few that it may be in: units are rounded (6.1e-5 of them; the middle's power adds 2^-21), masses by 2^-46 each.
+    const Share h = share_of_bins(MASS_BINS);
+    unsigned long long low[6], high_[6], below, ahead, units_before, lows = 0, highs = 0, units_sum = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const double middle = exp2f(-1.4426950408889634f * SPAN / BINS * (4 * tid + j)), n_ = c[j] * (1.0 / ONE);
-      low[j] = __double2ull_rd(n_ * fmax(middle * (1.0 - 1.3e-4) - 0x1.1p-46, 0.0) * 0x1p45);
-      high[j] = __double2ull_ru(n_ * (middle * (1.0 + 1.3e-4) + 0x1.1p-46) * 0x1p45);
+    for (int j = 0; j < 6; ++j) {
+      const double middle = exp2f(static_cast<float>(-(h.bin + j)) / STEPS), n_ = h.c[j] * (1.0 / ONE);
+      low[j] = __double2ull_rd(n_ * fmax(middle * (1.0 - 6.5e-5) - 0x1.1p-46, 0.0) * 0x1p45);
+      high_[j] = __double2ull_ru(n_ * (middle * (1.0 + 6.5e-5) + 0x1.1p-46) * 0x1p45);
+      lows += low[j];
+      highs += high_[j];
+      units_sum += h.c[j];
     }
-    block_scan((low[0] + low[1]) + (low[2] + low[3]), below);
-    block_scan((high[0] + high[1]) + (high[2] + high[3]), ahead);
+    const unsigned long long all_low = block_scan(lows, below), all_high = block_scan(highs, ahead), all_units = block_scan(units_sum, units_before);
+    {
+      const int slot = exchange;                 // three sums at once
+      exchange += 3;
+      if (tid < ranks) {
+        *cluster.map_shared_rank(&s.inbox[slot & 15][rank], tid) = all_low;
+        *cluster.map_shared_rank(&s.inbox[(slot + 1) & 15][rank], tid) = all_high;
+        *cluster.map_shared_rank(&s.inbox[(slot + 2) & 15][rank], tid) = all_units;
+      }
+      cluster.sync();
+      for (int r = 0; r < rank; ++r) { below += s.inbox[slot & 15][r]; ahead += s.inbox[(slot + 1) & 15][r]; units_before += s.inbox[(slot + 2) & 15][r]; }
+    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (ahead < want && want <= ahead + high[j]) s.bin_lo = 4 * tid + j;
-      if (below < want && want <= below + low[j]) s.bin_hi = 4 * tid + j;
-      ahead += high[j];
+    for (int j = 0; j < 6; ++j) {
+      if (j < h.mine) {
+        if (ahead < want && want <= ahead + high_[j])
+          for (int r = 0; r < ranks; ++r) { unsigned long long *const to = cluster.map_shared_rank(s.border, r); to[0] = h.bin + j; to[1] = units_before; }
+        if (below < want && want <= below + low[j])
+          for (int r = 0; r < ranks; ++r) { unsigned long long *const to = cluster.map_shared_rank(s.border, r); to[2] = h.bin + j; to[3] = units_before + h.c[j]; }
+      }
+      ahead += high_[j];
       below += low[j];
+      units_before += h.c[j];
     }
-    __syncthreads();
-    const int lo = s.bin_lo, hi = s.bin_hi;
-    unsigned long long tokens = 0, border_tokens = 0;          // at most: a token is 0.992 ONE at least
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (4 * tid + j <= hi) tokens += c[j];
-      if (4 * tid + j >= lo && 4 * tid + j <= hi) border_tokens += c[j];
-    }
-    const unsigned long long most = static_cast<unsigned long long>(0.99f * ONE) * LIST;
-    const bool few = block_sum(tokens) <= most, few_at_border = block_sum(border_tokens) <= most;
+    cluster.sync();
+    const int lo = static_cast<int>(s.border[0]), hi = static_cast<int>(s.border[2]);
+    // (a token is 0.994 ONE at least)
+    const unsigned long long most = static_cast<unsigned long long>(0.99 * ONE) * LIST, units_to = s.border[3];
+    const bool few = units_to <= most, few_at_border = units_to - s.border[1] <= most;
     if (few) {
-      each_from(bound_of(hi), [&](float v, int i) { if (bin_of(v) <= hi && kept(v, i)) list(v, i); });
+      each_from(mass_bound(hi), [&](float v, int i) { if (mass_bin(v) <= hi && kept(v, i)) list(v, i); });
       const int listed = collect();
       if (rank == 0) finish_list(listed, ~0ull, want);
       return;
     }
-    // rank 0: how many of the sorted candidates stay behind the mass `front`
-    auto announce_share = [&](int listed, unsigned long long front) {
-      unsigned long long w[2], before;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) w[j] = 2 * tid + j < listed ? mass(value_of(s.sorted[2 * tid + j])) : 0;
-      block_scan(w[0] + w[1], before);
-      before += front;
-      const int stay = __syncthreads_count(2 * tid < listed && before < want) + __syncthreads_count(2 * tid + 1 < listed && before + w[0] < want);
-      announce(max(stay, 1));
-    };
     // The mass in front of the border's bins, exactly, and their tokens.
     unsigned long long front = 0;
     sum = 0;
-    const float from = bound_of(hi);
+    const float from = mass_bound(hi);
     walk([&](float4 v4, int i, int) {
       if (!(fmaxf(fmaxf(v4.x, v4.y), fmaxf(v4.z, v4.w)) >= from)) return;
       const float v[4] = {v4.x, v4.y, v4.z, v4.w};
@@ -797,16 +812,16 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
       int b[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        b[j] = bin_of(v[j]);
-        const unsigned long long m = mass(v[j]);
-        if (b[j] > hi || !kept(v[j], first + 4 * i + j)) b[j] = BINS;
+        unsigned int units;
+        const unsigned long long m = mass_and_bin(v[j], b[j], units);
+        if (b[j] > hi || (cut && !kept(v[j], first + 4 * i + j))) b[j] = MASS_BINS;
         sum += b[j] < lo ? m : 0;
-        at_border = at_border || (b[j] >= lo && b[j] < BINS);
+        at_border = at_border || (b[j] >= lo && b[j] < MASS_BINS);
       }
       if (at_border && few_at_border) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (b[j] >= lo && b[j] < BINS) list(v[j], first + 4 * i + j);
+          if (b[j] >= lo && b[j] < MASS_BINS) list(v[j], first + 4 * i + j);
       }
     });
     const unsigned long long mine = block_sum(sum), ranges = warp_sum(sum);
@@ -848,7 +863,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
         return;
       }
     } else {                                     // (many equal values, or a very flat row)
-      cut_at(search([&](float v, int i) { const int b = bin_of(v); return b >= lo && b <= hi && kept(v, i) ? mass(v) : 0ull; },
+      cut_at(search([&](float v, int i) { const int b = mass_bin(v); return b >= lo && b <= hi && kept(v, i) ? mass(v) : 0ull; },
                     [&](unsigned long long) { return want - front; }));
     }
   }
