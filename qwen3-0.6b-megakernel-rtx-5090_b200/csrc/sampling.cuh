@@ -157,8 +157,9 @@ __device__ __forceinline__ void copy_four(unsigned char *to, const T *from) {
   else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(from) : "memory");
 }
 
-template <typename T>
-__global__ void __launch_bounds__(THREADS, 2) sample_rows(const Params p) {
+// AN_SM: CTAs of an SM.  One has twice the registers (few rows), two hide each other's waits.
+template <typename T, int AN_SM>
+__global__ void __launch_bounds__(THREADS, AN_SM) sample_rows(const Params p) {
   extern __shared__ __align__(16) unsigned char smem[];
   Shared &s = *reinterpret_cast<Shared *>(smem);
   unsigned char *const ring = smem + sizeof(Shared);

@@ -24,9 +24,10 @@ int cluster_size(int rows, int vocab, int sms) {
 }
 
 template <typename T>
-cudaError_t launch(const Params &p, int rows, int ranks, cudaStream_t stream) {
+cudaError_t launch(const Params &p, int rows, int ranks, int sms, cudaStream_t stream) {
+  void (*const kernel)(Params) = rows * ranks <= sms ? sample_rows<T, 1> : sample_rows<T, 2>;
   constexpr int smem = sizeof(Shared) + 2 * TURN * THREADS * 4 * sizeof(T);
-  cudaError_t e = cudaFuncSetAttribute(sample_rows<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.dynamicSmemBytes = smem;
@@ -40,7 +41,7 @@ cudaError_t launch(const Params &p, int rows, int ranks, cudaStream_t stream) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_rows<T>, p);
+  return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
 }  // namespace
@@ -82,9 +83,9 @@ extern "C" int qmk_sample_tokens(const void *logits, int logits_type, long long 
   p.top_k = top_k;
   p.tokens = tokens;
   p.logprobs = logprobs;
-  e = logits_type == 0 ? launch<float>(p, rows, ranks, stream)
-      : logits_type == 1 ? launch<__half>(p, rows, ranks, stream)
-                         : launch<__nv_bfloat16>(p, rows, ranks, stream);
+  e = logits_type == 0 ? launch<float>(p, rows, ranks, sms, stream)
+      : logits_type == 1 ? launch<__half>(p, rows, ranks, sms, stream)
+                         : launch<__nv_bfloat16>(p, rows, ranks, sms, stream);
   if (e != cudaSuccess) {
     cudaGetLastError();
     qmk_internal::note_error(std::string("qmk_sample_tokens: ") + cudaGetErrorString(e));
