@@ -113,7 +113,7 @@ extern "C" int qmk_attention_shared_prefix(const qmk_shared_prefix_args *a, cuda
     return refuse("null pointer argument");
   if (!(a->scale > -3.0e38f && a->scale < 3.0e38f)) return refuse("the scale must be finite");
   auto aligned = [](const void *ptr) { return (reinterpret_cast<unsigned long long>(ptr) & 15u) == 0; };
-  bool ok = aligned(a->q) && aligned(a->k_prefix) && aligned(a->v_prefix) && aligned(a->out) && aligned(a->workspace);
+  bool ok = aligned(a->q) && aligned(a->k_prefix) && aligned(a->v_prefix) && aligned(a->out) && (reinterpret_cast<unsigned long long>(a->workspace) & 31u) == 0;
   Params p;
   for (int b = 0; a->own_rows > 0 && b < a->num_sequences; ++b) {
     const long long at = 2 * b * a->own_seq_stride;
@@ -122,7 +122,7 @@ extern "C" int qmk_attention_shared_prefix(const qmk_shared_prefix_args *a, cuda
     if (!p.k_own[b] || !p.v_own[b]) return refuse("null pointer argument");
     ok = ok && aligned(p.k_own[b]) && aligned(p.v_own[b]);
   }
-  if (!ok) return refuse("pointers must be 16-byte aligned");
+  if (!ok) return refuse("pointers must be 16-byte aligned, the workspace 32");
   if (a->q_seq_stride % 8 || a->q_head_stride % 8 || a->prefix_row_stride % 8 || a->prefix_head_stride % 8 || a->own_row_stride % 8 || a->own_head_stride % 8)
     return refuse("strides must be multiples of 8 elements");
   if (!a->workspace || a->workspace_bytes < qmk_attention_shared_prefix_workspace(a->num_sequences, a->q_heads, a->kv_heads, a->head_dim, a->prefix_len, a->own_rows))
@@ -154,9 +154,9 @@ extern "C" int qmk_attention_shared_prefix(const qmk_shared_prefix_args *a, cuda
   p.row_tiles = s.row_tiles;
   p.own_parts = s.own_parts;
   const long long states = static_cast<long long>(s.prefix_parts + s.own_parts) * p.seqs * p.q_heads;
-  unsigned int *const status = static_cast<unsigned int *>(a->workspace);
-  p.part_out = static_cast<float *>(a->workspace) + 4;
+  p.part_out = static_cast<float *>(a->workspace);
   p.part_ml = reinterpret_cast<float2 *>(p.part_out + states * a->head_dim);
+  unsigned int *const status = reinterpret_cast<unsigned int *>(p.part_ml + states);
   p.out = a->out;
   p.lse = a->lse;
   const cudaError_t e = a->type == 0 ? launch<__half>(p, s, a->head_dim, maps, status, stream) : launch<__nv_bfloat16>(p, s, a->head_dim, maps, status, stream);

@@ -25,7 +25,6 @@ constexpr unsigned long long WAIT_NS = 2000000000ull;
 constexpr int TC_THREADS = qmk_attn::THREADS;
 constexpr int TC_ROWS = 128;                                       // prefix rows per tile
 constexpr uint32_t BOX_BYTES = 64 * 128, BLOCK_BYTES = 128 * 128;  // [64 rows x 64 dims], [128 rows x 64 dims or keys], swizzled
-constexpr int AHEAD = 4;                                            // tiles
 constexpr float RAISE = 3.0f;                                      // log2
 template <int D> constexpr uint32_t tc_tile_bytes() { return (D / 64) * BLOCK_BYTES; }          // of queries, keys, values
 template <int D> constexpr size_t tc_smem_bytes() { return 5 * tc_tile_bytes<D>() + 4 * BLOCK_BYTES + 256; }
@@ -34,10 +33,6 @@ static_assert(tc_smem_bytes<128>() <= 232448, "shared memory of a CTA");
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, int c3, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar) : "memory");
-}
-
-__device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap *map, int c0, int c1, int c2) {
-  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(map), "r"(c0), "r"(c1), "r"(c2) : "memory");
 }
 
 // map_q: {dims, heads of a kv head, kv heads, sequences}, boxes of {64, group, 1, seqs_per_tile}; map_k / map_v: {dims, prefix rows, kv heads}, boxes of
@@ -107,15 +102,6 @@ prefix_parts_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 #pragma unroll
       for (int r = 0; r < 2; ++r) tma_load_3d(to + h * BLOCK_BYTES + r * BOX_BYTES, map, 64 * h, first + j * TC_ROWS + 64 * r, kv, full);
   };
-  // A tile's slot is free again only when the chain's next product is due, so the loads' latency is on the chain's way: L2's, not HBM's,
-  // where tiles are asked for AHEAD of their loads.
-  auto prefetch_tile = [&](bool is_v, int j) {
-    if (j >= ntiles) return;
-#pragma unroll
-    for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) tma_prefetch_3d(is_v ? &map_v : &map_k, 64 * h, first + j * TC_ROWS + 64 * r, kv);
-  };
   const int k_prefilled = ntiles < 2 ? ntiles : 2;
   if (warp == 0 && elect_one()) {          // (rows of the tile that the box does not cover hold what was there: they stay in their own rows)
     bar_expect_tx(q_full, static_cast<uint32_t>(HALVES) * 128u * static_cast<uint32_t>(p.group * seqs_per_tile));
@@ -133,12 +119,10 @@ prefix_parts_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     if (elect_one()) {                     // ---- producers: the K ring (warp 0) and the V ring
       const bool is_v = warp != 0;
       int issued = is_v ? 0 : k_prefilled;
-      for (int j = issued; j < AHEAD; ++j) prefetch_tile(is_v, j);
       for (int j = issued; j < ntiles; ++j) {
         if (j >= 2 && !bar_wait(is_v ? v_empty(j & 1) : k_empty(j & 1), ((j >> 1) - 1) & 1, abort_flag, status, WAIT_NS)) break;
         if (*abort_flag) break;
         load_tile(is_v, j);
-        prefetch_tile(is_v, j + AHEAD);
         issued = j + 1;
       }
       if (*abort_flag)
@@ -311,14 +295,15 @@ prefix_parts_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         if (live) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            float v[4];
+          for (int i = 0; i < 32; i += 8) {      // (32 bytes at a time: whole sectors)
+            float v[8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < 8; ++k) {
               v[k] = __uint_as_float(oa[i + k]) * fa;
               if (two) v[k] = fmaf(__uint_as_float(ob[i + k]), fb, v[k]);
             }
-            *reinterpret_cast<float4 *>(dst + 32 * c + i) = make_float4(v[0], v[1], v[2], v[3]);
+            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 32 * c + i), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
+                         "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
           }
         }
       }

@@ -82,7 +82,7 @@ def args(C, **change):
                                          (dict(q_heads=136), b"kv_heads"), (dict(prefix_len=-1), b"length"), (dict(own_rows=-1), b"length"), (dict(k_own=None, k_own_base=4096, v_own_base=4096, own_seq_stride=12), b"aligned"),
                                          (dict(q=None), b"null"), (dict(out=None), b"null"), (dict(k_prefix=None), b"null"), (dict(own_lens=None), b"null"),
                                          (dict(k_own=None), b"null"), (dict(v_own=None), b"null"), (dict(k_own=None, k_own_base=4096), b"null"), (dict(scale=float("inf")), b"scale"), (dict(scale=float("nan")), b"scale"),
-                                         (dict(q=4098), b"aligned"), (dict(v_prefix=4104), b"aligned"), (dict(q_seq_stride=2049), b"strides"),
+                                         (dict(q=4098), b"aligned"), (dict(v_prefix=4104), b"aligned"), (dict(workspace=4112), b"aligned"), (dict(q_seq_stride=2049), b"strides"),
                                          (dict(prefix_row_stride=132), b"strides"), (dict(own_head_stride=4), b"strides"),
                                          (dict(workspace=None), b"workspace"), (dict(workspace_bytes=100), b"workspace")])
 def test_refused_before_anything_runs(C, change, text):
