@@ -65,8 +65,9 @@ prefix_parts_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   auto s_free = [&](int c) { return bars + 8u * (10 + c); };
   auto p_ready = [&](int c) { return bars + 8u * (12 + c); };
   auto pv_done = [&](int c) { return bars + 8u * (14 + c); };
+  auto turn = [&](int c) { return bars + 8u * (19 + c); };         // the other chain is through with its exponentials
   const uint32_t q_full = bars + 8u * 16, s_stopped = bars + 8u * 17, pv_stopped = bars + 8u * 18;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tc_smem + OFF_BARS + 8 * 19);
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tc_smem + OFF_BARS + 8 * 21);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
   if ((base & 1023u) != 0u) {              // the swizzled tiles need a 1024-byte aligned window: NaN instead of garbage
@@ -78,7 +79,7 @@ prefix_parts_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   if (threadIdx.x == 0) {
     for (int c = 0; c < CHAINS; ++c) {
       bar_init(k_full(c), 1); bar_init(k_empty(c), 1); bar_init(v_full(c), 1); bar_init(v_empty(c), 1);
-      bar_init(s_full(c), 1); bar_init(s_free(c), 4); bar_init(p_ready(c), 4); bar_init(pv_done(c), 1);
+      bar_init(s_full(c), 1); bar_init(s_free(c), 4); bar_init(p_ready(c), 4); bar_init(pv_done(c), 1); bar_init(turn(c), 4);
     }
     bar_init(q_full, 1);
     bar_init(s_stopped, 1);
@@ -243,6 +244,12 @@ prefix_parts_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       }
       l *= alpha;
       m_used = m_new;
+      // The chains take turns at the exponentials, so that one's products run under the other's: side by side in step, both wait for products
+      // and then share the units.
+      if (chain == 1 || n > 0) {
+        ok = __all_sync(0xffffffffu, bar_wait(turn(chain), (chain == 1 ? n : n - 1) & 1, abort_flag, status, WAIT_NS));
+        if (!ok) break;
+      }
       const float sub = Half<T>::P_SHIFT - (m_used == -INFINITY ? 0.f : m_used);
       const uint32_t prow = p_tile + static_cast<uint32_t>(row) * 128u, x = static_cast<uint32_t>(row & 7);
       float sum4[4] = {0.f, 0.f, 0.f, 0.f};
@@ -259,6 +266,7 @@ prefix_parts_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(prow + (seg >> 3) * BLOCK_BYTES + ((static_cast<uint32_t>(seg & 7) ^ x) << 4)), "r"(packed[0]),
                      "r"(packed[1]), "r"(packed[2]), "r"(packed[3]) : "memory");
       }
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(turn(chain ^ 1)) : "memory");
       l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
