@@ -26,6 +26,7 @@ constexpr int KEYS = 64;                         // cache rows per tile
 constexpr int STAGES = 3;
 constexpr int OWN_RANGE = 256;                   // own rows per item
 constexpr int OWN_STAGES = 2;
+constexpr int own_warps(int dim) { return dim == 64 ? 4 : 2; }               // of own_parts: tiles of 16 KB
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct Params {
@@ -251,181 +252,199 @@ __device__ __forceinline__ void item_mma(const Params &p, unsigned char *smem, i
 
 // A sequence's own rows against its query heads of a kv head (NT blocks of eight).  Turned round: cache rows are the 16 rows of an mma.sync tile
 // and heads its eight columns, scores = K q^T and out^T = V^T p^T, so two heads cost half the products and a third of the registers that 16 query rows
-// would.  A warp takes 16 of a tile's 64 rows; p^T becomes an operand by transposing 8 x 8 blocks in registers.
+// would.  A warp takes 16 of a tile's rows; p^T becomes an operand by transposing 8 x 8 blocks in registers.
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-template <typename T, int D, int NT>
-__device__ __forceinline__ void item_own(const Params &p, unsigned char *smem, int part, int kv_head, int b, const T *kp, const T *vp, int nrows) {
-  constexpr int CHUNKS = D / 8, ROW_BYTES = D * 2, TILE = KEYS * ROW_BYTES;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane & 3, rq = lane >> 2;
-  const uint32_t base = s32(smem);
-  const int tiles = (nrows + KEYS - 1) / KEYS;
-  auto load = [&](int t) {
-    if (t < tiles) {
-      const uint32_t dst = base + (t % OWN_STAGES) * 2 * TILE;
+template <typename T, int D, int NT, int W>
+struct OwnRows {
+  static constexpr int ROWS = 16 * W;                      // of a tile, 16 for each of W warps
+  static constexpr int CHUNKS = D / 8, ROW_BYTES = D * 2, TILE = ROWS * ROW_BYTES, PITCH = D + 4, HEADS = NT * 8;
+  static constexpr int STATE_BYTES = W * HEADS * (PITCH * 4 + 8);            // of the warps' states, where they are joined
+  uint32_t qb[NT][D / 16][2];
+  float acc[NT][D / 16][4], m[NT][2], l[NT][2];            // heads 2 quad and 2 quad + 1 of each block
+
+  static __device__ __forceinline__ void load(const Params &p, uint32_t dst, const T *kp, const T *vp, int t, int nrows) {
 #pragma unroll
-      for (int i = tid; i < KEYS * CHUNKS; i += THREADS) {
-        const int r = i / CHUNKS, c = i % CHUNKS, row = t * KEYS + r;
-        const bool there = row < nrows;
-        const long long off = (there ? row : 0) * p.own_row + c * 8;
-        const uint32_t at = r * ROW_BYTES + ((c ^ (r & 7)) << 4);
-        copy16(dst + at, kp + off, there);
-        copy16(dst + TILE + at, vp + off, there);
+    for (int i = threadIdx.x; i < ROWS * CHUNKS; i += 32 * W) {
+      const int r = i / CHUNKS, c = i % CHUNKS, row = t * ROWS + r;
+      const bool there = row < nrows;
+      const long long off = (there ? row : 0) * p.own_row + c * 8;
+      const uint32_t at = r * ROW_BYTES + ((c ^ (r & 7)) << 4);
+      copy16(dst + at, kp + off, there);
+      copy16(dst + TILE + at, vp + off, there);
+    }
+  }
+  __device__ __forceinline__ void begin(const Params &p, int kv_head, int b) {
+    const int lane = threadIdx.x & 31, quad = lane & 3, rq = lane >> 2;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const bool live = nt * 8 + rq < p.group;
+      const T *src = static_cast<const T *>(p.q) + b * p.q_seq + (kv_head * p.group + (live ? nt * 8 + rq : 0)) * p.q_head + quad * 2;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        qb[nt][ks][0] = live ? *reinterpret_cast<const uint32_t *>(src + ks * 16) : 0u;
+        qb[nt][ks][1] = live ? *reinterpret_cast<const uint32_t *>(src + ks * 16 + 8) : 0u;
+      }
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) { acc[nt][t][0] = 0.f; acc[nt][t][1] = 0.f; acc[nt][t][2] = 0.f; acc[nt][t][3] = 0.f; }
+    }
+  }
+  // this warp's 16 rows of tile t
+  __device__ __forceinline__ void tile(const Params &p, uint32_t kt, int t, int nrows) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rq = lane >> 2, key0 = t * ROWS + warp * 16;
+    const uint32_t vt = kt + TILE;
+    if (key0 >= nrows) return;                             // (the same for the warp)
+    float sc[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) { sc[nt][0] = 0.f; sc[nt][1] = 0.f; sc[nt][2] = 0.f; sc[nt][3] = 0.f; }
+    const int kr = warp * 16 + (lane & 15);
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      uint32_t a[4];
+      ldsm4(kt + kr * ROW_BYTES + (((2 * ks + (lane >> 4)) ^ (kr & 7)) << 4), a);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) Half<T>::mma(sc[nt], a, qb[nt][ks][0], qb[nt][ks][1]);
+    }
+    uint32_t pb[NT][2];
+    const bool top_row = key0 + rq < nrows, low_row = key0 + rq + 8 < nrows;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sc[nt][i] = (i < 2 ? top_row : low_row) ? sc[nt][i] * p.scale_log2 : -INFINITY;
+      float corr[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float mx = fmaxf(sc[nt][h], sc[nt][2 + h]);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float mn = fmaxf(m[nt][h], mx);
+        float sub = mn == -INFINITY ? 0.f : mn;            // scores of -inf only: 2^(-inf - 0) = 0, not NaN
+        corr[h] = exp2f(m[nt][h] - sub);
+        m[nt][h] = mn;
+        sub -= Half<T>::P_SHIFT;
+        sc[nt][h] = exp2f(sc[nt][h] - sub);
+        sc[nt][2 + h] = exp2f(sc[nt][2 + h] - sub);
+        l[nt][h] = l[nt][h] * corr[h] + (sc[nt][h] + sc[nt][2 + h]);
+      }
+      pb[nt][0] = transposed(Half<T>::pack(sc[nt][0], sc[nt][1]));
+      pb[nt][1] = transposed(Half<T>::pack(sc[nt][2], sc[nt][3]));
+#pragma unroll
+      for (int t2 = 0; t2 < D / 16; ++t2) { acc[nt][t2][0] *= corr[0]; acc[nt][t2][1] *= corr[1]; acc[nt][t2][2] *= corr[0]; acc[nt][t2][3] *= corr[1]; }
+    }
+    const int vr = warp * 16 + (lane & 7) + 8 * (lane >> 4);
+#pragma unroll
+    for (int dp = 0; dp < D / 16; ++dp) {
+      uint32_t a[4];
+      ldsm4_trans(vt + vr * ROW_BYTES + (((2 * dp + ((lane >> 3) & 1)) ^ (vr & 7)) << 4), a);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) Half<T>::mma(acc[nt][dp], a, pb[nt][0], pb[nt][1]);
+    }
+  }
+  // The warps' states, joined in `smem` (STATE_BYTES, free when this is called), to the workspace.
+  __device__ __forceinline__ void end(const Params &p, unsigned char *smem, int part, int kv_head, int b) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane & 3, rq = lane >> 2;
+    float *const so = reinterpret_cast<float *>(smem);     // [warp][head][PITCH]
+    float2 *const sml = reinterpret_cast<float2 *>(so + W * HEADS * PITCH);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], o);
+        float *const mine = so + (warp * HEADS + nt * 8 + quad * 2 + h) * PITCH + rq;
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) { mine[t * 16] = acc[nt][t][h]; mine[t * 16 + 8] = acc[nt][t][2 + h]; }
+        if (rq == 0) sml[warp * HEADS + nt * 8 + quad * 2 + h] = make_float2(m[nt][h], l[nt][h]);
       }
     }
+    __syncthreads();
+    const size_t at0 = (static_cast<size_t>(part) * p.seqs + b) * p.q_heads + kv_head * p.group;
+    for (int i = tid; i < p.group * (D / 4); i += 32 * W) {
+      const int h = i / (D / 4), c = i % (D / 4) * 4;
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) M = fmaxf(M, sml[w * HEADS + h].x);
+      float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float2 ml = sml[w * HEADS + h];
+        const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2f(ml.x - M);
+        const float4 a = *reinterpret_cast<const float4 *>(so + (w * HEADS + h) * PITCH + c);
+        L += ml.y * f;
+        A.x += a.x * f; A.y += a.y * f; A.z += a.z * f; A.w += a.w * f;
+      }
+      *reinterpret_cast<float4 *>(p.part_out + (at0 + h) * D + c) = A;
+      if (c == 0) p.part_ml[at0 + h] = make_float2(M, L);
+    }
+  }
+};
+// An own item: (kv head, sequence, range)
+struct OwnItem { int kv, b, own; };
+__device__ __forceinline__ OwnItem own_item(const Params &p, int id) { return OwnItem{id % p.kv_heads, id / p.kv_heads % p.seqs, id / (p.kv_heads * p.seqs)}; }
+__device__ __forceinline__ int own_len(const Params &p, int b) { return min(max(p.own_lens[b] + p.own_bias, 0), p.own_rows); }
+template <typename T>
+__device__ __forceinline__ const T *own_base(const Params &p, const void *const *caches, const OwnItem &it) {
+  return static_cast<const T *>(caches[it.b]) + static_cast<size_t>(it.kv) * p.own_head + static_cast<size_t>(it.own) * OWN_RANGE * p.own_row;
+}
+// no rows: a state that weighs nothing
+__device__ __forceinline__ void own_nothing(const Params &p, const OwnItem &it) {
+  if (threadIdx.x < p.group)
+    p.part_ml[(static_cast<size_t>(p.prefix_parts + it.own) * p.seqs + it.b) * p.q_heads + it.kv * p.group + threadIdx.x] = make_float2(-INFINITY, 0.f);
+}
+
+template <typename T, int D, int NT, int W>
+__device__ __forceinline__ void own_cta(const Params &p, unsigned char *smem, int id) {
+  using Own = OwnRows<T, D, NT, W>;
+  const OwnItem it = own_item(p, id);
+  const int n = min(OWN_RANGE, own_len(p, it.b) - it.own * OWN_RANGE), tiles = (n + Own::ROWS - 1) / Own::ROWS;
+  if (n <= 0) { own_nothing(p, it); return; }
+  const T *const kp = own_base<T>(p, p.k_own, it), *const vp = own_base<T>(p, p.v_own, it);
+  auto load = [&](int t) {
+    if (t < tiles) Own::load(p, s32(smem) + (t % OWN_STAGES) * 2 * Own::TILE, kp, vp, t, n);
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
   for (int t = 0; t < OWN_STAGES; ++t) load(t);
-  uint32_t qb[NT][D / 16][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const bool live = nt * 8 + rq < p.group;
-    const T *src = static_cast<const T *>(p.q) + b * p.q_seq + (kv_head * p.group + (live ? nt * 8 + rq : 0)) * p.q_head + quad * 2;
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-      qb[nt][ks][0] = live ? *reinterpret_cast<const uint32_t *>(src + ks * 16) : 0u;
-      qb[nt][ks][1] = live ? *reinterpret_cast<const uint32_t *>(src + ks * 16 + 8) : 0u;
-    }
-  }
-  float acc[NT][D / 16][4], m[NT][2], l[NT][2];            // heads 2 quad and 2 quad + 1 of each block
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    m[nt][0] = m[nt][1] = -INFINITY;
-    l[nt][0] = l[nt][1] = 0.f;
-#pragma unroll
-    for (int t = 0; t < D / 16; ++t) { acc[nt][t][0] = 0.f; acc[nt][t][1] = 0.f; acc[nt][t][2] = 0.f; acc[nt][t][3] = 0.f; }
-  }
+  Own own;
+  own.begin(p, it.kv, it.b);
   for (int t = 0; t < tiles; ++t) {
     asm volatile("cp.async.wait_group %0;" ::"n"(OWN_STAGES - 1) : "memory");
     __syncthreads();
-    const uint32_t kt = base + (t % OWN_STAGES) * 2 * TILE, vt = kt + TILE;
-    const int key0 = t * KEYS + warp * 16;
-    if (key0 < nrows) {                                    // (the same for the warp)
-      float sc[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) { sc[nt][0] = 0.f; sc[nt][1] = 0.f; sc[nt][2] = 0.f; sc[nt][3] = 0.f; }
-      const int kr = warp * 16 + (lane & 15);
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        uint32_t a[4];
-        ldsm4(kt + kr * ROW_BYTES + (((2 * ks + (lane >> 4)) ^ (kr & 7)) << 4), a);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) Half<T>::mma(sc[nt], a, qb[nt][ks][0], qb[nt][ks][1]);
-      }
-      uint32_t pb[NT][2];
-      const bool top_row = key0 + rq < nrows, low_row = key0 + rq + 8 < nrows;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sc[nt][i] = (i < 2 ? top_row : low_row) ? sc[nt][i] * p.scale_log2 : -INFINITY;
-        float corr[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float mx = fmaxf(sc[nt][h], sc[nt][2 + h]);
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          const float mn = fmaxf(m[nt][h], mx);
-          float sub = mn == -INFINITY ? 0.f : mn;          // scores of -inf only: 2^(-inf - 0) = 0, not NaN
-          corr[h] = exp2f(m[nt][h] - sub);
-          m[nt][h] = mn;
-          sub -= Half<T>::P_SHIFT;
-          sc[nt][h] = exp2f(sc[nt][h] - sub);
-          sc[nt][2 + h] = exp2f(sc[nt][2 + h] - sub);
-          l[nt][h] = l[nt][h] * corr[h] + (sc[nt][h] + sc[nt][2 + h]);
-        }
-        pb[nt][0] = transposed(Half<T>::pack(sc[nt][0], sc[nt][1]));
-        pb[nt][1] = transposed(Half<T>::pack(sc[nt][2], sc[nt][3]));
-#pragma unroll
-        for (int t2 = 0; t2 < D / 16; ++t2) { acc[nt][t2][0] *= corr[0]; acc[nt][t2][1] *= corr[1]; acc[nt][t2][2] *= corr[0]; acc[nt][t2][3] *= corr[1]; }
-      }
-      const int vr = warp * 16 + (lane & 7) + 8 * (lane >> 4);
-#pragma unroll
-      for (int dp = 0; dp < D / 16; ++dp) {
-        uint32_t a[4];
-        ldsm4_trans(vt + vr * ROW_BYTES + (((2 * dp + ((lane >> 3) & 1)) ^ (vr & 7)) << 4), a);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) Half<T>::mma(acc[nt][dp], a, pb[nt][0], pb[nt][1]);
-      }
-    }
+    own.tile(p, s32(smem) + (t % OWN_STAGES) * 2 * Own::TILE, t, n);
     __syncthreads();                                       // the tile has been read
     load(t + OWN_STAGES);
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
-  constexpr int PITCH = D + 4, HEADS = NT * 8;             // floats between heads
-  float *const so = reinterpret_cast<float *>(smem);       // [warp][head][PITCH]
-  float2 *const sml = reinterpret_cast<float2 *>(so + WARPS * HEADS * PITCH);
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], o);
-      float *const mine = so + (warp * HEADS + nt * 8 + quad * 2 + h) * PITCH + rq;
-#pragma unroll
-      for (int t = 0; t < D / 16; ++t) { mine[t * 16] = acc[nt][t][h]; mine[t * 16 + 8] = acc[nt][t][2 + h]; }
-      if (rq == 0) sml[warp * HEADS + nt * 8 + quad * 2 + h] = make_float2(m[nt][h], l[nt][h]);
-    }
-  }
-  __syncthreads();
-  const size_t at0 = (static_cast<size_t>(part) * p.seqs + b) * p.q_heads + kv_head * p.group;
-  for (int i = tid; i < p.group * (D / 4); i += THREADS) {
-    const int h = i / (D / 4), c = i % (D / 4) * 4;
-    float M = -INFINITY, L = 0.f;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) M = fmaxf(M, sml[w * HEADS + h].x);
-    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const float2 ml = sml[w * HEADS + h];
-      const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2f(ml.x - M);
-      const float4 a = *reinterpret_cast<const float4 *>(so + (w * HEADS + h) * PITCH + c);
-      L += ml.y * f;
-      A.x += a.x * f; A.y += a.y * f; A.z += a.z * f; A.w += a.w * f;
-    }
-    *reinterpret_cast<float4 *>(p.part_out + (at0 + h) * D + c) = A;
-    if (c == 0) p.part_ml[at0 + h] = make_float2(M, L);
-  }
-}
-// Own item `id`: (kv head, sequence, range)
-template <typename T, int D, int NT>
-__device__ __forceinline__ void own_item(const Params &p, unsigned char *smem, int id) {
-  const int kv = id % p.kv_heads, b = id / p.kv_heads % p.seqs, own = id / (p.kv_heads * p.seqs);
-  const int len = min(max(p.own_lens[b] + p.own_bias, 0), p.own_rows), first = own * OWN_RANGE, n = min(OWN_RANGE, len - first);
-  const int part = p.prefix_parts + own;
-  if (n <= 0) {                                            // no rows: a state that weighs nothing
-    if (threadIdx.x < p.group)
-      p.part_ml[(static_cast<size_t>(part) * p.seqs + b) * p.q_heads + kv * p.group + threadIdx.x] = make_float2(-INFINITY, 0.f);
-    return;
-  }
-  const size_t off = static_cast<size_t>(kv) * p.own_head + static_cast<size_t>(first) * p.own_row;
-  item_own<T, D, NT>(p, smem, part, kv, b, static_cast<const T *>(p.k_own[b]) + off, static_cast<const T *>(p.v_own[b]) + off, n);
+  own.end(p, smem, p.prefix_parts + it.own, it.kv, it.b);
 }
 
-// Prefix items first: they are the longest.
+// Few query rows: prefix items first, they are the longest, then the own ones.
 template <typename T, int D, int MT, int NT>
 __global__ void __launch_bounds__(THREADS) attend_parts(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) unsigned char smem[];
   pdl_wait();
   pdl_trigger();
   const int id = static_cast<int>(blockIdx.x);
-  if (id >= p.prefix_items) { own_item<T, D, NT>(p, smem, id - p.prefix_items); return; }
+  if (id >= p.prefix_items) { own_cta<T, D, NT, WARPS>(p, smem, id - p.prefix_items); return; }
   const int kv = id % p.kv_heads, tile = id / p.kv_heads % p.row_tiles, part = id / (p.kv_heads * p.row_tiles);
   const int first = part * p.prefix_range, n = min(p.prefix_range, p.prefix_len - first);
   const int row0 = tile * MT * 16, live = min(MT * 16, p.seqs * p.group - row0);
   const size_t off = static_cast<size_t>(kv) * p.prefix_head + static_cast<size_t>(first) * p.prefix_row;
   item_mma<T, D, MT>(p, smem, part, kv, row0, live, static_cast<const T *>(p.k_prefix) + off, static_cast<const T *>(p.v_prefix) + off, p.prefix_row, n);
 }
-// The own rows alone, launched behind prefix_parts_tc, which has waited for what is read here: they run beside it and end behind it.
+// Many: the own rows alone, launched behind prefix_parts_tc, which has waited for what is read here: they run beside it and end behind it.  Small CTAs, six
+// an SM: what one waits for (its length, the queries, the first rows, its warps at the end) passes under the others.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(THREADS, 3) own_parts(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(32 * own_warps(D), D == 64 ? 4 : 6) own_parts(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) unsigned char smem[];
   pdl_trigger();
-  own_item<T, D, NT>(p, smem, static_cast<int>(blockIdx.x));
+  own_cta<T, D, NT, own_warps(D)>(p, smem, static_cast<int>(blockIdx.x));
   pdl_wait();
 }
 
@@ -442,45 +461,38 @@ __global__ void __launch_bounds__(128) join_parts(const __grid_constant__ Params
   float M = -INFINITY, L = 0.f, A[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) A[i] = 0.f;
-  for (int i0 = warp; i0 < parts; i0 += 4 * 32) {          // this lane's part: its maximum and sum
-    const int mine = i0 + 4 * lane;
-    const float2 ml = mine < parts ? p.part_ml[static_cast<size_t>(mine) * rows + row] : make_float2(-INFINITY, 0.f);
-    float top = ml.x;
+  for (int i0 = warp; i0 < parts; i0 += 4 * AHEAD) {       // eight parts at a time, their outputs asked for with their maxima
+    float v[AHEAD][E];
+    float2 ml[AHEAD];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    top = fmaxf(top, M);
+    for (int j = 0; j < AHEAD; ++j) {
+      const size_t at = static_cast<size_t>(min(i0 + 4 * j, parts - 1)) * rows + row;
+      ml[j] = p.part_ml[at];
+      const float *src = p.part_out + at * D + lane * E;
+      if (E == 4) { const float4 a = *reinterpret_cast<const float4 *>(src); v[j][0] = a.x; v[j][1] = a.y; v[j][E - 2] = a.z; v[j][E - 1] = a.w; }
+      else { const float2 a = *reinterpret_cast<const float2 *>(src); v[j][0] = a.x; v[j][1] = a.y; }
+    }
+    float top = M;
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (i0 + 4 * j >= parts) ml[j] = make_float2(-INFINITY, 0.f);
+      top = fmaxf(top, ml[j].x);
+    }
     const float f0 = M == -INFINITY ? 0.f : exp2f(M - top);
     M = top;
-    // a part without rows has written no output and weighs nothing (one whose scores are not numbers is not among these)
-    const bool there = !(ml.x == -INFINITY && ml.y == 0.f);
-    const float f = there ? exp2f(ml.x == -INFINITY && top == -INFINITY ? 0.f : ml.x - top) : 0.f;
-    L = L * f0 + ml.y * f;
+    L *= f0;
 #pragma unroll
     for (int k = 0; k < E; ++k) A[k] *= f0;
-    const int count = min(32, (parts - i0 + 3) >> 2);
-    for (int j0 = 0; j0 < count; j0 += AHEAD) {
-      float v[AHEAD][E], w[AHEAD];
 #pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        w[j] = __shfl_sync(0xffffffffu, f, j0 + j);
-        const bool need = j0 + j < count && __shfl_sync(0xffffffffu, static_cast<int>(there), j0 + j);
-        const float *src = p.part_out + (static_cast<size_t>(i0 + 4 * (j0 + j)) * rows + row) * D + lane * E;
-        if (need) {
-          if (E == 4) { const float4 a = *reinterpret_cast<const float4 *>(src); v[j][0] = a.x; v[j][1] = a.y; v[j][E - 2] = a.z; v[j][E - 1] = a.w; }
-          else { const float2 a = *reinterpret_cast<const float2 *>(src); v[j][0] = a.x; v[j][1] = a.y; }
-        } else {
+    for (int j = 0; j < AHEAD; ++j) {
+      // a part without rows has written no output and weighs nothing (one whose scores are not numbers is not among these)
+      const bool there = !(ml[j].x == -INFINITY && ml[j].y == 0.f);
+      const float f = there ? (ml[j].x == -INFINITY ? 1.f : exp2f(ml[j].x - top)) : 0.f;
+      L = fmaf(ml[j].y, f, L);
 #pragma unroll
-          for (int k = 0; k < E; ++k) v[j][k] = 0.f;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j)
-#pragma unroll
-        for (int k = 0; k < E; ++k) A[k] = fmaf(v[j][k], w[j], A[k]);
+      for (int k = 0; k < E; ++k) A[k] = there ? fmaf(v[j][k], f, A[k]) : A[k];
     }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
   if (lane == 0) { sm[warp] = M; sl[warp] = L; }
 #pragma unroll
   for (int k = 0; k < E; ++k) sa[warp][lane * E + k] = A[k];

@@ -56,9 +56,11 @@ bool make_maps(CUtensorMap *maps, const Params &p, const Split &s, int head_dim,
 
 template <typename T, int D, int NT>
 cudaError_t launch(Params &p, const Split &s, const CUtensorMap *maps, unsigned int *status, cudaStream_t stream) {
-  constexpr int own_smem = OWN_STAGES * 2 * KEYS * D * 2, smem = STAGES * 2 * KEYS * D * 2;
-  static_assert(own_smem >= WARPS * NT * 8 * (D + 4) * 4 + WARPS * NT * 8 * 8 && smem >= WARPS * 16 * (D + 4) * 4 + WARPS * 16 * 8 && smem >= own_smem,
-                "the warps' states fit the ring");
+  using Own = OwnRows<T, D, NT, own_warps(D)>;
+  using Beside = OwnRows<T, D, NT, WARPS>;
+  constexpr int own_smem = OWN_STAGES * 2 * Own::TILE, beside_smem = OWN_STAGES * 2 * Beside::TILE, smem = STAGES * 2 * KEYS * D * 2;
+  static_assert(own_smem >= Own::STATE_BYTES && beside_smem >= Beside::STATE_BYTES && smem >= WARPS * 16 * (D + 4) * 4 + WARPS * 16 * 8 && smem >= beside_smem,
+                "the warps' states fit the rings");
   void (*const kernel)(Params) = s.row_warps == 1 ? attend_parts<T, D, 1, NT> : attend_parts<T, D, 2, NT>;
   cudaError_t e;
   const int prefix_items = s.prefix_parts * s.row_tiles * p.kv_heads, own_items = s.own_parts * p.kv_heads * p.seqs;
@@ -72,12 +74,12 @@ cudaError_t launch(Params &p, const Split &s, const CUtensorMap *maps, unsigned 
                                 s.seqs_per_tile, status);
     dependent = true;                            // (of the launch before, inside this call)
     const qmk_tc::PdlScope scope(true);
-    if (e == cudaSuccess && own_items > 0) e = qmk_tc::launch_kernel(own_parts<T, D, NT>, dim3(own_items), dim3(THREADS), own_smem, stream, p);
+    if (e == cudaSuccess && own_items > 0) e = qmk_tc::launch_kernel(own_parts<T, D, NT>, dim3(own_items), dim3(32 * own_warps(D)), own_smem, stream, p);
     if (e != cudaSuccess) return e;
   } else if (prefix_items + own_items > 0) {
     p.prefix_items = prefix_items;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess) e = qmk_tc::launch_kernel(kernel, dim3(prefix_items + own_items), dim3(THREADS), prefix_items > 0 ? smem : own_smem, stream, p);
+    if (e == cudaSuccess) e = qmk_tc::launch_kernel(kernel, dim3(prefix_items + own_items), dim3(THREADS), prefix_items > 0 ? smem : beside_smem, stream, p);
     if (e != cudaSuccess) return e;
     dependent = true;
   }
