@@ -706,7 +706,7 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
     p_ptr, p = _per_row(top_p, _FP32, rows, index, "top_p")
     m_ptr, m = _per_row(min_p, _FP32, rows, index, "min_p")
     logprobs = torch.empty_like(uniforms)
-    tokens = torch.empty_like(uniforms, dtype=_INT32)
+    tokens = torch.empty(rows, dtype=_INT32, device=logits.device)
     rc = _on_device(index, _lib.qmk_sample_tokens, logits.data_ptr(), code, logits.stride(0), rows, vocab, uniforms.data_ptr(), t_ptr, t, k_ptr, k,
                     p_ptr, p, m_ptr, m, tokens.data_ptr(), logprobs.data_ptr())
     if rc != 0:
@@ -772,10 +772,10 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
             and own_lens.is_contiguous()):
         raise RuntimeError(f"{who}: own_lens must be a contiguous int32 tensor with one value per sequence on q's device")
     device = q.device
-    out = torch.empty((n, q_heads, dim), dtype=dtype, device=device)
-    lse = torch.empty((n, q_heads), dtype=_FP32, device=device)
+    out = torch.empty_like(q) if q.is_contiguous() else torch.empty(n, q_heads, dim, dtype=dtype, device=device)
+    lse = torch.empty(n, q_heads, dtype=_FP32, device=device)
     need = _shared_prefix_workspace(n, q_heads, kv_heads, dim, prefix, rows)
-    workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    workspace = own_lens.new_empty(need >> 2)
     q_seq, q_head, _ = q.stride()
     args = _SharedPrefixArgs(code, n, q_heads, kv_heads, dim, q.data_ptr(), q_seq, q_head, k_prefix.data_ptr(), v_prefix.data_ptr(), prefix,
                              prefix_strides[1], prefix_strides[0], k_ptrs, v_ptrs, k_base, v_base, own_seq, rows, own_row, own_head, own_lens.data_ptr(), 0,
@@ -789,7 +789,7 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
 @functools.lru_cache(maxsize=256)
 def _shared_prefix_workspace(*sizes):
     """Bytes of workspace for these sizes (``qmk_attention_shared_prefix_workspace``, at least a few)."""
-    return max(int(_lib.qmk_attention_shared_prefix_workspace(*sizes)), 256)
+    return (max(int(_lib.qmk_attention_shared_prefix_workspace(*sizes)), 256) + 3) // 4 * 4
 
 
 def sync_status() -> int:
