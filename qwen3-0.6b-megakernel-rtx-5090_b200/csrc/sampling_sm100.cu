@@ -2,6 +2,7 @@
 #include "../../include/qwen_megakernel.h"
 
 #include <algorithm>
+#include <atomic>
 #include <string>
 
 #include "engine_internal.h"
@@ -16,32 +17,61 @@ int refuse(const std::string &why) {
   return QMK_ERR_BAD_ARGUMENT;
 }
 
-// CTAs per row: as many as still are all resident at once (two an SM), each with 2048 tokens at least.
-int cluster_size(int rows, int vocab, int sms) {
-  int c = 1;
-  while (c < MAX_CLUSTER && 2 * c * rows <= 2 * sms && vocab > c * 2048) c *= 2;
-  return c;
-}
+constexpr int DEVICES = 16;
 
+template <typename T, int AN_SM>
+struct Launch {
+  static constexpr int SMEM = sizeof(Shared) + 2 * TURN * THREADS * 4 * sizeof(T);
+  static void configure(cudaLaunchConfig_t *cfg, cudaLaunchAttribute *attr, int rows, int ranks, cudaStream_t stream) {
+    *cfg = {};
+    cfg->gridDim = dim3(static_cast<unsigned int>(rows) * ranks);
+    cfg->blockDim = dim3(THREADS);
+    cfg->dynamicSmemBytes = SMEM;
+    cfg->stream = stream;
+    attr->id = cudaLaunchAttributeClusterDimension;
+    attr->val.clusterDim.x = ranks;
+    attr->val.clusterDim.y = 1;
+    attr->val.clusterDim.z = 1;
+    cfg->attrs = attr;
+    cfg->numAttrs = 1;
+  }
+  // Rows whose clusters of `ranks` CTAs are resident together on this device; asked for once.  (Clusters lie inside a GPC, of which not all have as
+  // many SMs: 16 clusters of eight CTAs on 128 of 148 SMs took two waves, 24 us where four CTAs a row took 17.)
+  static cudaError_t resident(int device, int ranks, int *rows) {
+    static std::atomic<int> known[DEVICES][4];
+    std::atomic<int> &at = known[device][ranks == 8 ? 3 : ranks >> 1];
+    if ((*rows = at.load()) > 0) return cudaSuccess;
+    cudaError_t e = cudaFuncSetAttribute(sample_rows<T, AN_SM>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr;
+    configure(&cfg, &attr, 1, ranks, nullptr);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(rows, sample_rows<T, AN_SM>, &cfg);
+    if (e == cudaSuccess) at.store(*rows = std::max(*rows, 1));
+    return e;
+  }
+  static cudaError_t run(const Params &p, int rows, int ranks, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr;
+    configure(&cfg, &attr, rows, ranks, stream);
+    return cudaLaunchKernelEx(&cfg, sample_rows<T, AN_SM>, p);
+  }
+};
+
+// CTAs per row: as many as leave all rows resident at once, with at least 1024 tokens each; alone on their SMs where that is enough.
 template <typename T>
-cudaError_t launch(const Params &p, int rows, int ranks, int sms, cudaStream_t stream) {
-  void (*const kernel)(Params) = rows * ranks <= sms ? sample_rows<T, 1> : sample_rows<T, 2>;
-  constexpr int smem = sizeof(Shared) + 2 * TURN * THREADS * 4 * sizeof(T);
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.dynamicSmemBytes = smem;
-  cfg.gridDim = dim3(static_cast<unsigned int>(rows) * ranks);
-  cfg.blockDim = dim3(THREADS);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ranks;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+cudaError_t launch(const Params &p, int rows, cudaStream_t stream) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess && device >= DEVICES) e = cudaErrorInvalidDevice;
+  for (int ranks = MAX_CLUSTER; e == cudaSuccess; ranks /= 2) {
+    if (ranks > 1 && p.vocab <= ranks / 2 * 1024) continue;
+    int alone = 0, two = 0;
+    e = Launch<T, 1>::resident(device, ranks, &alone);
+    if (e == cudaSuccess && rows <= alone) return Launch<T, 1>::run(p, rows, ranks, stream);
+    if (e == cudaSuccess) e = Launch<T, 2>::resident(device, ranks, &two);
+    if (e == cudaSuccess && (rows <= two || ranks == 1)) return Launch<T, 2>::run(p, rows, ranks, stream);
+  }
+  return e;
 }
 
 }  // namespace
@@ -59,16 +89,7 @@ extern "C" int qmk_sample_tokens(const void *logits, int logits_type, long long 
   if (!temperatures && !(temperature >= 0.0f)) return refuse("the temperature must not be negative");
   if (!top_ps && !(top_p > 0.0f)) return refuse("top_p must be above 0");
   if (!min_ps && !(min_p >= 0.0f && min_p <= 1.0f)) return refuse("min_p must be in [0, 1]");
-  int device = 0, sms = 0;
-  cudaError_t e = cudaGetDevice(&device);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    qmk_internal::note_error(std::string("qmk_sample_tokens: ") + cudaGetErrorString(e));
-    return QMK_ERR_CUDA;
-  }
   Params p;
-  const int ranks = cluster_size(rows, vocab, sms);
   p.logits = logits;
   p.row_stride = row_stride;
   p.vocab = vocab;
@@ -83,9 +104,7 @@ extern "C" int qmk_sample_tokens(const void *logits, int logits_type, long long 
   p.top_k = top_k;
   p.tokens = tokens;
   p.logprobs = logprobs;
-  e = logits_type == 0 ? launch<float>(p, rows, ranks, sms, stream)
-      : logits_type == 1 ? launch<__half>(p, rows, ranks, sms, stream)
-                         : launch<__nv_bfloat16>(p, rows, ranks, sms, stream);
+  const cudaError_t e = logits_type == 0 ? launch<float>(p, rows, stream) : logits_type == 1 ? launch<__half>(p, rows, stream) : launch<__nv_bfloat16>(p, rows, stream);
   if (e != cudaSuccess) {
     cudaGetLastError();
     qmk_internal::note_error(std::string("qmk_sample_tokens: ") + cudaGetErrorString(e));
