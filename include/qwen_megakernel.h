@@ -427,7 +427,7 @@ int qmk_sample_tokens(const void *logits, int logits_type, long long row_stride,
  * out = softmax(scale * q . k) v over prefix rows [0, prefix_len) and own rows [0, own_lens[b] + own_lens_add), lse the natural
  * logarithm of the sum of exp(scale * q . k).  Nothing visible: zeros and -inf.  Rows behind the last are not read.  Strides in
  * elements, multiples of 8; the head dimension is contiguous; pointers 16-byte aligned (the workspace 32).  Limits: 1 to 128 sequences, 1 to 16 query heads
- * per kv head, head_dim 64 or 128.  Does not block, allocates nothing, may be captured; the workspace (DEVICE, size from
+ * per kv head, head_dim 64 or 128, 2^24 rows.  Does not block, allocates nothing, may be captured; the workspace (DEVICE, size from
  * qmk_attention_shared_prefix_workspace) belongs to the call until it is done. */
 typedef struct qmk_shared_prefix_args {
   int type;                          /* 0 fp16, 1 bf16: q, caches and out */

@@ -4,7 +4,7 @@
 // its scores are matrix products: the queries of all sequences that read a kv head are the rows of one operand, the
 // prefix rows cross HBM once for all of them instead of once for each.  A softmax over a split range is joined from partial
 // states - the maximum M, the sum L of 2^(s - M) and the unnormalised output A of each part, all fp32 - as sum(2^(M_i - M) A_i) /
-// sum(2^(M_i - M) L_i), so the prefix may be split over many CTAs and the own rows handled by others.  A part without visible rows
+// sum(2^(M_i - M) L_i), so the prefix may be split over many CTAs and the own rows handled by others.  A part whose scores are all -inf
 // has M = -inf and L = 0 and weighs nothing.
 //
 // An item is a block of query rows against a range of cache rows of one kv head: (row tile, kv head, prefix range) or (sequence, kv
@@ -24,7 +24,7 @@ constexpr int MAX_GROUP = 16;                    // query heads per kv head: one
 constexpr int THREADS = 128, WARPS = 4;
 constexpr int KEYS = 64;                         // cache rows per tile
 constexpr int STAGES = 3;
-constexpr int OWN_RANGE = 256;                   // own rows per item
+constexpr int OWN_RANGE = 256, OWN_PARTS = 16;   // own rows per item, more where a cache has more than OWN_PARTS such ranges
 constexpr int OWN_STAGES = 2;
 constexpr int own_warps(int dim) { return dim == 64 ? 4 : 2; }               // of own_parts: tiles of 16 KB
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -38,7 +38,7 @@ struct Params {
   int prefix_len, prefix_parts, prefix_range, row_tiles;   // range: prefix rows per item, a multiple of KEYS
   int prefix_items;                              // of attend_parts
   long long own_row, own_head;
-  int own_rows, own_parts;
+  int own_rows, own_parts, own_range;            // range: a multiple of 64
   const int *own_lens;
   int own_bias;                                  // added to own_lens
   float scale_log2;                              // scale * log2 e
@@ -389,20 +389,14 @@ __device__ __forceinline__ OwnItem own_item(const Params &p, int id) { return Ow
 __device__ __forceinline__ int own_len(const Params &p, int b) { return min(max(p.own_lens[b] + p.own_bias, 0), p.own_rows); }
 template <typename T>
 __device__ __forceinline__ const T *own_base(const Params &p, const void *const *caches, const OwnItem &it) {
-  return static_cast<const T *>(caches[it.b]) + static_cast<size_t>(it.kv) * p.own_head + static_cast<size_t>(it.own) * OWN_RANGE * p.own_row;
+  return static_cast<const T *>(caches[it.b]) + static_cast<size_t>(it.kv) * p.own_head + static_cast<size_t>(it.own) * p.own_range * p.own_row;
 }
-// no rows: a state that weighs nothing
-__device__ __forceinline__ void own_nothing(const Params &p, const OwnItem &it) {
-  if (threadIdx.x < p.group)
-    p.part_ml[(static_cast<size_t>(p.prefix_parts + it.own) * p.seqs + it.b) * p.q_heads + it.kv * p.group + threadIdx.x] = make_float2(-INFINITY, 0.f);
-}
-
 template <typename T, int D, int NT, int W>
 __device__ __forceinline__ void own_cta(const Params &p, unsigned char *smem, int id) {
   using Own = OwnRows<T, D, NT, W>;
   const OwnItem it = own_item(p, id);
-  const int n = min(OWN_RANGE, own_len(p, it.b) - it.own * OWN_RANGE), tiles = (n + Own::ROWS - 1) / Own::ROWS;
-  if (n <= 0) { own_nothing(p, it); return; }
+  const int n = min(p.own_range, own_len(p, it.b) - it.own * p.own_range), tiles = (n + Own::ROWS - 1) / Own::ROWS;
+  if (n <= 0) return;                                      // (join_parts goes by the length too)
   const T *const kp = own_base<T>(p, p.k_own, it), *const vp = own_base<T>(p, p.v_own, it);
   auto load = [&](int t) {
     if (t < tiles) Own::load(p, s32(smem) + (t % OWN_STAGES) * 2 * Own::TILE, kp, vp, t, n);
@@ -448,36 +442,40 @@ __global__ void __launch_bounds__(32 * own_warps(D), D == 64 ? 4 : 6) own_parts(
   pdl_wait();
 }
 
-// A CTA joins the parts of a (sequence, query head): a warp takes every fourth part, eight parts' outputs on their way at a time.
+// A CTA joins the parts of a (sequence, query head): a warp takes every fourth part.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) join_parts(const __grid_constant__ Params p) {
   constexpr int E = D / 32, AHEAD = 8;
   __shared__ float sm[4], sl[4];
   __shared__ __align__(16) float sa[4][D];
+  // Own ranges behind a sequence's length have no state.  (The lengths were there before the kernels were launched that this one follows; read while
+  // they run.)
+  const int parts = p.prefix_parts + (p.own_parts ? (own_len(p, static_cast<int>(blockIdx.x) / p.q_heads) + p.own_range - 1) / p.own_range : 0);
   pdl_wait();
   pdl_trigger();
   const int rows = p.seqs * p.q_heads, row = static_cast<int>(blockIdx.x), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int parts = p.prefix_parts + p.own_parts;
   float M = -INFINITY, L = 0.f, A[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) A[i] = 0.f;
-  for (int i0 = warp; i0 < parts; i0 += 4 * AHEAD) {       // eight parts at a time, their outputs asked for with their maxima
+  auto take = [&](int i0) {                                // up to eight parts, their outputs asked for with their maxima
     float v[AHEAD][E];
     float2 ml[AHEAD];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      const size_t at = static_cast<size_t>(min(i0 + 4 * j, parts - 1)) * rows + row;
-      ml[j] = p.part_ml[at];
-      const float *src = p.part_out + at * D + lane * E;
-      if (E == 4) { const float4 a = *reinterpret_cast<const float4 *>(src); v[j][0] = a.x; v[j][1] = a.y; v[j][E - 2] = a.z; v[j][E - 1] = a.w; }
-      else { const float2 a = *reinterpret_cast<const float2 *>(src); v[j][0] = a.x; v[j][1] = a.y; }
+      ml[j] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int k = 0; k < E; ++k) v[j][k] = 0.f;
+      if (i0 + 4 * j < parts) {
+        const size_t at = static_cast<size_t>(i0 + 4 * j) * rows + row;
+        ml[j] = p.part_ml[at];
+        const float *src = p.part_out + at * D + lane * E;
+        if (E == 4) { const float4 a = *reinterpret_cast<const float4 *>(src); v[j][0] = a.x; v[j][1] = a.y; v[j][E - 2] = a.z; v[j][E - 1] = a.w; }
+        else { const float2 a = *reinterpret_cast<const float2 *>(src); v[j][0] = a.x; v[j][1] = a.y; }
+      }
     }
     float top = M;
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      if (i0 + 4 * j >= parts) ml[j] = make_float2(-INFINITY, 0.f);
-      top = fmaxf(top, ml[j].x);
-    }
+    for (int j = 0; j < AHEAD; ++j) top = fmaxf(top, ml[j].x);
     const float f0 = M == -INFINITY ? 0.f : exp2f(M - top);
     M = top;
     L *= f0;
@@ -485,14 +483,14 @@ __global__ void __launch_bounds__(128) join_parts(const __grid_constant__ Params
     for (int k = 0; k < E; ++k) A[k] *= f0;
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      // a part without rows has written no output and weighs nothing (one whose scores are not numbers is not among these)
-      const bool there = !(ml[j].x == -INFINITY && ml[j].y == 0.f);
-      const float f = there ? (ml[j].x == -INFINITY ? 1.f : exp2f(ml[j].x - top)) : 0.f;
+      // (scores of -inf alone: nothing; a maximum of -inf with a sum that is no number: the result is none)
+      const float f = ml[j].x == -INFINITY ? (ml[j].y == 0.f ? 0.f : 1.f) : exp2f(ml[j].x - top);
       L = fmaf(ml[j].y, f, L);
 #pragma unroll
-      for (int k = 0; k < E; ++k) A[k] = there ? fmaf(v[j][k], f, A[k]) : A[k];
+      for (int k = 0; k < E; ++k) A[k] = fmaf(v[j][k], f, A[k]);
     }
-  }
+  };
+  for (int i0 = warp; i0 < parts; i0 += 4 * AHEAD) take(i0);
   if (lane == 0) { sm[warp] = M; sl[warp] = L; }
 #pragma unroll
   for (int k = 0; k < E; ++k) sa[warp][lane * E + k] = A[k];

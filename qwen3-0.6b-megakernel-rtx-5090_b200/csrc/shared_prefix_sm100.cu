@@ -22,9 +22,9 @@ int refuse(const std::string &why) {
 // How a call is cut into items.  More than 32 rows of queries against a kv head go through tcgen05, 128 at a time: XXX.
 struct Split {
   bool tc;
-  int row_warps, row_tiles, seqs_per_tile, prefix_parts, prefix_range, own_parts;
+  int row_warps, row_tiles, seqs_per_tile, prefix_parts, prefix_range, own_parts, own_range;
 };
-constexpr int SMS = 148;
+constexpr int SMS = 148, MAX_ROWS = 1 << 24;
 Split split_of(int seqs, int q_heads, int kv_heads, int prefix_len, int own_rows, bool tc) {
   Split s;
   const int group = q_heads / kv_heads, rows = seqs * group, tiles = (prefix_len + KEYS - 1) / KEYS;
@@ -35,7 +35,8 @@ Split split_of(int seqs, int q_heads, int kv_heads, int prefix_len, int own_rows
   const int items = s.row_tiles * kv_heads, parts = std::max(1, (s.tc ? SMS : 2 * SMS) / items);
   s.prefix_range = std::max(2, ((tiles + parts - 1) / parts + 1) / 2 * 2) * KEYS;      // (whole tiles of prefix_parts_tc)
   s.prefix_parts = (prefix_len + s.prefix_range - 1) / s.prefix_range;
-  s.own_parts = (own_rows + OWN_RANGE - 1) / OWN_RANGE;
+  s.own_range = std::max(OWN_RANGE, (own_rows / OWN_PARTS + 64) / 64 * 64);
+  s.own_parts = (own_rows + s.own_range - 1) / s.own_range;
   return s;
 }
 long long workspace_bytes(const Split &s, int seqs, int q_heads, int head_dim) {
@@ -110,7 +111,7 @@ extern "C" int qmk_attention_shared_prefix(const qmk_shared_prefix_args *a, cuda
   if (a->head_dim != 64 && a->head_dim != 128) return refuse("head_dim must be 64 or 128");
   if (a->kv_heads < 1 || a->q_heads < 1 || a->q_heads % a->kv_heads || a->q_heads / a->kv_heads > MAX_GROUP || a->q_heads > 1024)
     return refuse("q_heads must be 1 to 16 times kv_heads, and at most 1024");
-  if (a->prefix_len < 0 || a->own_rows < 0) return refuse("negative length");
+  if (a->prefix_len < 0 || a->own_rows < 0 || a->prefix_len > MAX_ROWS || a->own_rows > MAX_ROWS) return refuse("a length is negative or above 2^24");
   if (!a->q || !a->out || (a->prefix_len > 0 && (!a->k_prefix || !a->v_prefix)) || (a->own_rows > 0 && (a->k_own ? !a->v_own : !a->k_own_base || !a->v_own_base)) || (a->own_rows > 0 && !a->own_lens))
     return refuse("null pointer argument");
   if (!(a->scale > -3.0e38f && a->scale < 3.0e38f)) return refuse("the scale must be finite");
@@ -155,6 +156,7 @@ extern "C" int qmk_attention_shared_prefix(const qmk_shared_prefix_args *a, cuda
   p.prefix_range = s.prefix_range;
   p.row_tiles = s.row_tiles;
   p.own_parts = s.own_parts;
+  p.own_range = s.own_range;
   const long long states = static_cast<long long>(s.prefix_parts + s.own_parts) * p.seqs * p.q_heads;
   p.part_out = static_cast<float *>(a->workspace);
   p.part_ml = reinterpret_cast<float2 *>(p.part_out + states * a->head_dim);

@@ -206,6 +206,17 @@ def test_rows_apart_and_rows_that_are_not_aligned(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab", [(15, 151936), (33, 100001), (70, 30000), (150, 9001), (400, 2500), (3000, 40)])
+def test_every_number_of_ctas_a_row(gpu, rows, vocab):
+    """Few rows have eight CTAs each, many one: every row with its own options, fp16 and fp32."""
+    x, u, g = rows_of_logits(rows, vocab, rows)
+    pick = lambda *v: [v[i % len(v)] for i in range(rows)]
+    for dtype in ("fp32", "fp16"):
+        check(gpu, x.to(DTYPES[dtype]), u, temperature=torch.tensor(pick(0.8, 1.3, 0.0, 0.5, 1.0)), top_k=torch.tensor(pick(0, 50, 1000, 3, 0, 0, 1), dtype=torch.int32),
+              top_p=torch.tensor(pick(1.0, 0.9, 0.99)), min_p=torch.tensor(pick(0.0, 0.0, 0.03, 0.0)), skipped=0.03)
+
+
+@pytest.mark.gpu
 def test_a_pick_does_not_depend_on_its_batch(gpu):
     x, u, _ = rows_of_logits(64, 151936, 9)
     x, u = x.cuda(), u.cuda()

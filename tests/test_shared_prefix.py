@@ -79,7 +79,7 @@ def args(C, **change):
 
 @pytest.mark.parametrize("change,text", [(dict(num_sequences=0), b"num_sequences"), (dict(num_sequences=129), b"num_sequences"), (dict(type=2), b"type"),
                                          (dict(head_dim=96), b"head_dim"), (dict(kv_heads=0), b"kv_heads"), (dict(q_heads=12), b"kv_heads"),
-                                         (dict(q_heads=136), b"kv_heads"), (dict(prefix_len=-1), b"length"), (dict(own_rows=-1), b"length"), (dict(k_own=None, k_own_base=4096, v_own_base=4096, own_seq_stride=12), b"aligned"),
+                                         (dict(q_heads=136), b"kv_heads"), (dict(prefix_len=-1), b"length"), (dict(own_rows=-1), b"length"), (dict(prefix_len=(1 << 24) + 1), b"length"), (dict(k_own=None, k_own_base=4096, v_own_base=4096, own_seq_stride=12), b"aligned"),
                                          (dict(q=None), b"null"), (dict(out=None), b"null"), (dict(k_prefix=None), b"null"), (dict(own_lens=None), b"null"),
                                          (dict(k_own=None), b"null"), (dict(v_own=None), b"null"), (dict(k_own=None, k_own_base=4096), b"null"), (dict(scale=float("inf")), b"scale"), (dict(scale=float("nan")), b"scale"),
                                          (dict(q=4098), b"aligned"), (dict(v_prefix=4104), b"aligned"), (dict(workspace=4112), b"aligned"), (dict(q_seq_stride=2049), b"strides"),
@@ -124,6 +124,15 @@ def test_matches_the_definition(gpu, dtype, q_heads, kv_heads, dim, seqs, prefix
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 def test_long_prefixes_and_full_batches(gpu, dtype, seqs, q_heads, kv_heads, prefix, own):
     case = inputs(seqs, q_heads, kv_heads, 128, prefix, own, [(7919 * i) % (own + 1) for i in range(seqs)], dtype, seed=prefix, gain=1.5)
+    check(gpu.attention_shared_prefix(*case), *case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs,own,lens", [(1, 20000, [19999]), (3, 9001, [9001, 0, 300]), (40, 6000, [5999] + [0] * 20 + [64 * i for i in range(19)])])
+@pytest.mark.parametrize("prefix", [0, 77])
+def test_long_caches_of_their_own(gpu, seqs, own, lens, prefix):
+    """Caches of more rows than sixteen short ranges, most of them behind the sequence's last."""
+    case = inputs(seqs, 16, 8, 128, prefix, own, lens, "fp16", seed=own)
     check(gpu.attention_shared_prefix(*case), *case)
 
 
