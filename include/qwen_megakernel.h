@@ -412,12 +412,14 @@ int qmk_gemm_packed_tn(const void *a, const void *b, const void *b2, void *c, in
  * value, w = exp((x - m) / temperature).  Tokens in order of descending x, ties by ascending index; kept are the first of them, as many as
  * every filter allows: top_k (below 1 or from the vocabulary on: off) that number, top_p (from 1 on: off) the shortest prefix whose mass is top_p of the mass of what
  * top_k left, min_p (0: off) those with w >= min_p; always one.  tokens[row] (DEVICE int32) is the lowest index at which the
- * running sum of the kept w in the order of the indices exceeds uniforms[row] (DEVICE fp32, in [0, 1), drawn into it where it is not) times their total,
- * logprobs[row] (DEVICE fp32, may be null) the logarithm of w / total for it.  A temperature that is not above 0 takes the
- * largest value (the lowest index of ties).  A row without a largest value (all NaN or -inf) gives 2^31 - 1 and NaN, as a greedy step.
- * temperatures, top_ks, top_ps, min_ps: DEVICE arrays with a value per row, or null: the scalar behind it for all rows (a
- * scalar that is negative, or no number, is refused; in an array a top_p or min_p that is no number is off).  rows in [0, 65536], vocab in [1, 262144].  Picks do not depend on the
- * other rows or on the run: masses are summed as whole multiples of 2^-45.  Does not block, allocates nothing, may be captured. */
+ * running sum of the kept w in the order of the indices exceeds uniforms[row] (DEVICE fp32, in [0, 1), drawn into it where it is not) times
+ * their total, logprobs[row] (DEVICE fp32, may be null) the logarithm of w / total for it.  A temperature that is not above 0 takes the
+ * largest value (the lowest index of ties), one above 2^100 counts as 2^100.  A row without a largest value (all NaN or -inf) gives 2^31 - 1
+ * and NaN, as a greedy step.  temperatures, top_ks, top_ps, min_ps: DEVICE arrays with a value per row, or null: the scalar behind it for all
+ * rows (a scalar that is negative, or no number, and a top_p of 0 are refused; in an array a top_p that is not above 0 keeps the first token, and a top_p
+ * or min_p that is no number is off).  A row_stride of 0 draws from one row `rows` times.  rows in [0, 65536], vocab in [1, 262144].  Picks do
+ * not depend on the other rows or on the run: masses are summed as whole multiples of 2^-45.  Does not block, allocates nothing, may be
+ * captured behind a first call on the device. */
 int qmk_sample_tokens(const void *logits, int logits_type, long long row_stride, int rows, int vocab, const float *uniforms,
                       const float *temperatures, float temperature, const int *top_ks, int top_k, const float *top_ps, float top_p,
                       const float *min_ps, float min_p, int *tokens, float *logprobs, cudaStream_t stream);
@@ -425,10 +427,10 @@ int qmk_sample_tokens(const void *logits, int logits_type, long long row_stride,
 /* Attention of one new token per sequence, where all sequences share their first prefix_len cache rows (computed once for
  * all) and each goes on in rows of its own; no counterpart in the reference.  Per sequence b and query head h (kv head h / (q_heads / kv_heads)):
  * out = softmax(scale * q . k) v over prefix rows [0, prefix_len) and own rows [0, own_lens[b] + own_lens_add), lse the natural
- * logarithm of the sum of exp(scale * q . k).  Nothing visible: zeros and -inf.  Rows behind the last are not read.  Strides in
- * elements, multiples of 8; the head dimension is contiguous; pointers 16-byte aligned (the workspace 32).  Limits: 1 to 128 sequences, 1 to 16 query heads
- * per kv head, head_dim 64 or 128, 2^24 rows.  Does not block, allocates nothing, may be captured; the workspace (DEVICE, size from
- * qmk_attention_shared_prefix_workspace) belongs to the call until it is done. */
+ * logarithm of the sum of exp(scale * q . k).  Nothing visible: zeros and -inf.  Rows behind the last are not looked at.  Strides in
+ * elements, multiples of 8; the head dimension is contiguous; pointers 16-byte aligned (the workspace 32).  Limits: 1 to 128 sequences, 1 to
+ * 16 query heads per kv head, head_dim 64 or 128, 2^24 rows.  Does not block, allocates nothing, may be captured behind a first call with its types
+ * and sizes on the device; the workspace (DEVICE, size from qmk_attention_shared_prefix_workspace) belongs to the call until it is done. */
 typedef struct qmk_shared_prefix_args {
   int type;                          /* 0 fp16, 1 bf16: q, caches and out */
   int num_sequences, q_heads, kv_heads, head_dim;

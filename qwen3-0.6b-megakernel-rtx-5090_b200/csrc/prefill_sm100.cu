@@ -1334,7 +1334,7 @@ static int decode_batched(const char *who, const Sampling *sampling, int num_seq
   for (int b = 0; b < B; ++b) {
     if (!k_caches[b] || !v_caches[b] || !output_logs[b])
       return qmk_internal::report(QMK_ERR_BAD_ARGUMENT, std::string(who) + ": null cache or log pointer");
-    if (start_positions[b] < 0 || start_positions[b] + num_steps > max_seq_len)
+    if (start_positions[b] < 0 || num_steps > max_seq_len - start_positions[b])
       return qmk_internal::report(QMK_ERR_POSITION, "start_position + steps exceeds max_seq_len");
     if (first_token_ids[b] < 0 || first_token_ids[b] >= env.vocab)
       return qmk_internal::report(QMK_ERR_BAD_TOKEN, "first token outside [0, vocab)");

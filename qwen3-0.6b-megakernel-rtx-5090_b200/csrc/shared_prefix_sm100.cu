@@ -2,7 +2,6 @@
 #include "../../include/qwen_megakernel.h"
 
 #include <algorithm>
-#include <mutex>
 #include <string>
 
 #include "engine_internal.h"
@@ -19,16 +18,20 @@ int refuse(const std::string &why) {
   return QMK_ERR_BAD_ARGUMENT;
 }
 
-// How a call is cut into items.  More than 32 rows of queries against a kv head go through tcgen05, 128 at a time: XXX.
+// How a call is cut into items.  More than 32 rows of queries against a kv head and 96 M products (rows x prefix rows x kv heads x dims) go through
+// tcgen05, 128 rows at a time.  mma.sync against tcgen05, us a call in a graph, the prefix in L2, eight kv heads of 128 dims: 32 query rows each 9.0 and 9.9 with 1000
+// prefix rows, 20.4 and 20.2 with 16,384; 40 rows 30.3 and 20.8 with 16,384; 64 rows 9.2 and 10.0 with 200, 15.5 and 14.7 with 4096; 128 rows 16.8 and 16.2 with 1000,
+// 52.4 and 24.6 with 16,384.  Four kv heads of 64 dims: 64 rows 8.1 and 9.8 with 4096, 13.4 and 12.5 with 16,384.
 struct Split {
   bool tc;
   int row_warps, row_tiles, seqs_per_tile, prefix_parts, prefix_range, own_parts, own_range;
 };
 constexpr int SMS = 148, MAX_ROWS = 1 << 24;
-Split split_of(int seqs, int q_heads, int kv_heads, int prefix_len, int own_rows, bool tc) {
+constexpr long long TC_PRODUCTS = 96 << 20;
+Split split_of(int seqs, int q_heads, int kv_heads, int head_dim, int prefix_len, int own_rows, bool tc) {
   Split s;
   const int group = q_heads / kv_heads, rows = seqs * group, tiles = (prefix_len + KEYS - 1) / KEYS;
-  s.tc = tc && rows > 32 && prefix_len > 0;
+  s.tc = tc && rows > 32 && 1ll * rows * kv_heads * head_dim * prefix_len >= TC_PRODUCTS;
   s.row_warps = rows <= 16 ? 1 : 2;
   s.seqs_per_tile = std::min(128 / group, seqs);
   s.row_tiles = s.tc ? (seqs + s.seqs_per_tile - 1) / s.seqs_per_tile : (rows + 16 * s.row_warps - 1) / (16 * s.row_warps);
@@ -99,8 +102,8 @@ extern "C" long long qmk_attention_shared_prefix_workspace(int num_sequences, in
                                                            int own_rows) {
   if (num_sequences < 1 || num_sequences > MAX_SEQS || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || prefix_len < 0 || own_rows < 0)
     return 0;
-  return std::max(workspace_bytes(split_of(num_sequences, q_heads, kv_heads, prefix_len, own_rows, true), num_sequences, q_heads, head_dim),
-                  workspace_bytes(split_of(num_sequences, q_heads, kv_heads, prefix_len, own_rows, false), num_sequences, q_heads, head_dim));
+  return std::max(workspace_bytes(split_of(num_sequences, q_heads, kv_heads, head_dim, prefix_len, own_rows, true), num_sequences, q_heads, head_dim),
+                  workspace_bytes(split_of(num_sequences, q_heads, kv_heads, head_dim, prefix_len, own_rows, false), num_sequences, q_heads, head_dim));
 }
 
 extern "C" int qmk_attention_shared_prefix(const qmk_shared_prefix_args *a, cudaStream_t stream) {
@@ -114,7 +117,7 @@ extern "C" int qmk_attention_shared_prefix(const qmk_shared_prefix_args *a, cuda
   if (a->prefix_len < 0 || a->own_rows < 0 || a->prefix_len > MAX_ROWS || a->own_rows > MAX_ROWS) return refuse("a length is negative or above 2^24");
   if (!a->q || !a->out || (a->prefix_len > 0 && (!a->k_prefix || !a->v_prefix)) || (a->own_rows > 0 && (a->k_own ? !a->v_own : !a->k_own_base || !a->v_own_base)) || (a->own_rows > 0 && !a->own_lens))
     return refuse("null pointer argument");
-  if (!(a->scale > -3.0e38f && a->scale < 3.0e38f)) return refuse("the scale must be finite");
+  if (!(a->scale > -2.0e38f && a->scale < 2.0e38f)) return refuse("the scale must be finite, and below 2e38");   // (times log2 e too)
   auto aligned = [](const void *ptr) { return (reinterpret_cast<unsigned long long>(ptr) & 15u) == 0; };
   bool ok = aligned(a->q) && aligned(a->k_prefix) && aligned(a->v_prefix) && aligned(a->out) && (reinterpret_cast<unsigned long long>(a->workspace) & 31u) == 0;
   Params p;
@@ -126,7 +129,9 @@ extern "C" int qmk_attention_shared_prefix(const qmk_shared_prefix_args *a, cuda
     ok = ok && aligned(p.k_own[b]) && aligned(p.v_own[b]);
   }
   if (!ok) return refuse("pointers must be 16-byte aligned, the workspace 32");
-  if (a->q_seq_stride % 8 || a->q_head_stride % 8 || a->prefix_row_stride % 8 || a->prefix_head_stride % 8 || a->own_row_stride % 8 || a->own_head_stride % 8)
+  auto odd = [](long long stride, int size) { return size > 1 && stride % 8; };
+  if (odd(a->q_seq_stride, a->num_sequences) || odd(a->q_head_stride, a->q_heads) || odd(a->prefix_row_stride, a->prefix_len) || odd(a->prefix_head_stride, a->kv_heads) ||
+      odd(a->own_row_stride, a->own_rows) || odd(a->own_head_stride, a->kv_heads))
     return refuse("strides must be multiples of 8 elements");
   if (!a->workspace || a->workspace_bytes < qmk_attention_shared_prefix_workspace(a->num_sequences, a->q_heads, a->kv_heads, a->head_dim, a->prefix_len, a->own_rows))
     return refuse("workspace too small");
@@ -149,9 +154,9 @@ extern "C" int qmk_attention_shared_prefix(const qmk_shared_prefix_args *a, cuda
   p.own_bias = a->own_lens_add;
   p.scale_log2 = a->scale * LOG2E;
   // (a scale of 0 would turn the masked scores of a last tile, -inf, into NaN there)
-  Split s = split_of(p.seqs, p.q_heads, p.kv_heads, p.prefix_len, p.own_rows, p.scale_log2 != 0.0f);
+  Split s = split_of(p.seqs, p.q_heads, p.kv_heads, a->head_dim, p.prefix_len, p.own_rows, p.scale_log2 != 0.0f);
   CUtensorMap maps[3];
-  if (s.tc && !make_maps(maps, p, s, a->head_dim, a->type == 1)) s = split_of(p.seqs, p.q_heads, p.kv_heads, p.prefix_len, p.own_rows, false);
+  if (s.tc && !make_maps(maps, p, s, a->head_dim, a->type == 1)) s = split_of(p.seqs, p.q_heads, p.kv_heads, a->head_dim, p.prefix_len, p.own_rows, false);
   p.prefix_parts = s.prefix_parts;
   p.prefix_range = s.prefix_range;
   p.row_tiles = s.row_tiles;

@@ -5,8 +5,11 @@
 // (attention_tcgen05.cuh): even and odd tiles belong to two chains with four softmax warps (a query row per thread), a score buffer, a P tile and
 // an output accumulator each (all of TMEM), so that one chain's round trip - scores read, P stored, P . V - runs beside the other's
 // arithmetic; the loads of keys and values, the score products and P . V have an issuing thread each.  Here all queries see all rows, so there is no mask but for the
-// prefix's end, and a CTA leaves a partial state (unnormalised output, maximum, sum) instead of the result.  Tiles of 64 rows as there took
-// 1800 cycles each (16,384 rows, 256 query rows: 27.6 us), most of it the round trip's latency; a tile twice as long takes XXX.
+// prefix's end, and a CTA leaves a partial state (unnormalised output, maximum, sum) instead of the result.  A tile's time is
+// the round trip's latency (1800 cycles for a tile of 64 rows).  16,384 rows of 128 dims against 256 query rows of eight kv heads, caches cold: tiles
+// of 64 rows 27.6 us, of 128 rows 28.0, of 128 rows with the chains taking turns at the exponentials 26.3, 0.65 PFLOP/s.
+// (17 GFLOP at the rate of a large product are 10 us, and so are 67 MB from HBM.)  What bounds it: every product of 128 x 128 x 16 reads 8 KB of operands from shared
+// memory, and an SM has 16 exponentials a cycle, 1024 cycles a tile.  Two tiles of query rows a CTA, which read keys half as often, took 33.
 //
 // The running maximum is raised when it grew by more than 2^3; weights are stored times 2^P_SHIFT (fp16: 2^12, so at most 2^15), which keeps ten
 // more bits of the small ones than storing them as they are.

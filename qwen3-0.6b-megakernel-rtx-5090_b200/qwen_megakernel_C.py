@@ -92,6 +92,7 @@ _lib.qmk_gemm_f16_tn.restype = _I
 _lib.qmk_gemm_packed_tn.argtypes = [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]
 _lib.qmk_gemm_packed_tn.restype = _I
 _LL = ctypes.c_longlong
+_INT_MAX = 2 ** 31 - 1
 _lib.qmk_sample_tokens.argtypes = [_P, _I, _LL, _I, _I, _P, _P, _F, _P, _I, _P, _F, _P, _F, _P, _P, _P]
 _lib.qmk_sample_tokens.restype = _I
 
@@ -546,7 +547,7 @@ def sample_batched(first_token_ids, start_positions, num_steps, embed_weight, la
         n, ints(*[int(t) for t in first_token_ids]), ints(*[int(p) for p in start_positions]), num_steps,
         _ptr(embed_weight), _ptr(layer_weights_packed), _ptr(final_norm_weight), _ptr(lm_head_weight), _ptr(cos_table), _ptr(sin_table),
         _ptr(k_prefix), _ptr(v_prefix), int(prefix_len), ptrs(*[_ptr(t) for t in k_caches]), ptrs(*[_ptr(t) for t in v_caches]),
-        _ptr(uniforms), floats(*[float(v) for v in temperatures]), ints(*[int(v) for v in top_ks]), floats(*[float(v) for v in top_ps]),
+        _ptr(uniforms), floats(*[float(v) for v in temperatures]), ints(*[min(max(int(v), 0), _INT_MAX) for v in top_ks]), floats(*[float(v) for v in top_ps]),
         floats(*[float(v) for v in min_ps]), ptrs(*[_ptr(t) for t in output_logs]), ptrs(*[_ptr(t) for t in logprob_logs]),
         int(num_layers), int(max_seq_len), float(attn_scale), _stream())
     if rc != 0:
@@ -687,11 +688,11 @@ def _per_row(value, dtype, rows, index, name):
 
 
 def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
-    """One token per row of ``logits [rows, vocab]`` (CUDA, fp32 / fp16 / bf16, contiguous along the vocabulary), picked with the number
-    of [0, 1) that ``uniforms [rows]`` (fp32) gives for the row: ``(tokens int32 [rows], logprobs fp32 [rows])``.  ``temperature`` (0: the
-    largest value), ``top_k`` (0: off), ``top_p`` (1: off) and ``min_p`` (0: off) are numbers, or tensors with a value per row (fp32,
+    """One token per row of ``logits [rows, vocab]`` (CUDA, fp32 / fp16 / bf16, contiguous along the vocabulary; one
+    row expanded to many is many draws from it), picked with the number of [0, 1) that ``uniforms [rows]`` (fp32) gives for the row:
+    ``(tokens int32 [rows], logprobs fp32 [rows])``.  ``temperature`` (0: the largest value), ``top_k`` (0: off), ``top_p`` (1: off) and ``min_p`` (0: off) are numbers, or tensors with a value per row (fp32,
     ``top_k`` int32).  The definition, ties and empty rows included: ``qmk_sample_tokens`` in include/qwen_megakernel.h.  Runs on the
-    current stream of the logits' device, does not synchronise, may be captured in a graph."""
+    current stream of the logits' device, does not synchronise, may be captured in a graph (behind a call on the device)."""
     code = _LOGIT_TYPES.get(logits.dtype)
     if code is None or not logits.is_cuda or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         _require_cuda()
@@ -703,6 +704,8 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
         raise RuntimeError("sample_tokens: uniforms must be a contiguous fp32 tensor with one value per row on the logits' device")
     t_ptr, t = _per_row(temperature, _FP32, rows, index, "temperature")
     k_ptr, k = _per_row(top_k, _INT32, rows, index, "top_k")
+    if not 0 < k <= vocab:                       # (off; a number of more than 32 bits would lose its upper ones)
+        k = 0
     p_ptr, p = _per_row(top_p, _FP32, rows, index, "top_p")
     m_ptr, m = _per_row(min_p, _FP32, rows, index, "min_p")
     logprobs = torch.empty_like(uniforms)
@@ -726,7 +729,7 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     sequence ``b`` sees the first ``own_lens[b]`` (int32 on the device, taken into ``[0, rows]``).  fp16 or bf16; at most 128 sequences,
     16 query heads per kv head, ``dim`` 64 or 128.  ``scale`` defaults to ``dim ** -0.5``.  ``out`` is like ``q`` (contiguous), ``lse``
     the fp32 ``[n, q_heads]`` logarithms of the softmax sums; a sequence that sees no row gets zeros and -inf.  Runs on the current
-    stream of the tensors' device, does not synchronise, may be captured in a graph."""
+    stream of the tensors' device, does not synchronise, may be captured in a graph (behind a call with these types and sizes on the device)."""
     who = "attention_shared_prefix"
     dtype = q.dtype
     if dtype is torch.float16:

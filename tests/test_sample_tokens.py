@@ -247,3 +247,51 @@ def test_on_other_streams_and_in_graphs(gpu):
             buf.copy_(sign * x)
             graph.replay()
             assert tokens.tolist() == w
+
+
+@pytest.mark.gpu
+def test_many_draws_from_one_row(gpu):
+    x, _, g = rows_of_logits(1, 32003, 3)
+    u = torch.rand(200, generator=g)
+    for kw in ({}, dict(top_k=50, top_p=0.9), dict(top_p=0.9)):
+        got = gpu.sample_tokens(x.cuda().expand(200, 32003), u.cuda(), **kw)
+        want = gpu.sample_tokens(x.expand(200, 32003).contiguous().cuda(), u.cuda(), **kw)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+def test_offsets_of_more_than_32_bits(gpu):
+    """Rows 2^27 + 1 elements apart, the last from 2^32 on."""
+    x, u, _ = rows_of_logits(36, 5000, 7)
+    wide = torch.empty(36 * ((1 << 27) + 1), dtype=torch.float16, device="cuda").as_strided((36, 5000), ((1 << 27) + 1, 1))
+    wide.copy_(x)
+    for kw in ({}, dict(top_k=50), dict(top_p=0.9)):
+        got, want = gpu.sample_tokens(wide, u.cuda(), **kw), gpu.sample_tokens(x.half().cuda(), u.cuda(), **kw)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+def test_numbers_of_tokens_of_more_than_32_bits_are_all(gpu):
+    x, u, _ = rows_of_logits(4, 3000, 8)
+    x, u = x.cuda(), u.cuda()
+    want = gpu.sample_tokens(x, u)
+    for k in (3000, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 1, -1, 1 - 2 ** 32):
+        got = gpu.sample_tokens(x, u, top_k=k)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+def test_two_calls_at_once(gpu):
+    x, u, _ = rows_of_logits(20, 151936, 22)
+    x, u = x.cuda(), u.cuda()
+    want = [gpu.sample_tokens(x, u, top_p=0.9), gpu.sample_tokens(-x, u, top_k=40)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    minus = -x
+    torch.cuda.synchronize()
+    for i in range(10):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(gpu.sample_tokens(minus, u, top_k=40) if i % 2 else gpu.sample_tokens(x, u, top_p=0.9))
+    torch.cuda.synchronize()
+    for i, (tokens, logp) in enumerate(got):
+        assert torch.equal(tokens, want[i % 2][0]) and torch.equal(logp, want[i % 2][1])

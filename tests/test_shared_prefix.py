@@ -240,3 +240,108 @@ def test_same_bits_again_on_other_streams_and_in_graphs(gpu):
             lens.copy_(new_lens)
             graph.replay()
             assert torch.equal(out, w[0]) and torch.equal(lse, w[1])
+
+
+# ------------------------------------------------------------------- many queries against many rows (from 96 M products on)
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("q_heads,kv_heads,dim,seqs,prefix", [(16, 8, 128, 49, 1024), (16, 8, 128, 65, 1100), (16, 8, 128, 128, 513), (4, 4, 64, 128, 3333), (6, 2, 128, 128, 1153),
+                                                              (8, 1, 64, 111, 2000), (16, 1, 128, 127, 449), (32, 4, 64, 97, 640), (32, 4, 64, 5, 10000), (16, 16, 128, 33, 1500)])
+def test_many_queries_and_rows(gpu, dtype, q_heads, kv_heads, dim, seqs, prefix):
+    assert seqs * q_heads * dim * prefix >= 96 << 20
+    own = 90
+    case = inputs(seqs, q_heads, kv_heads, dim, prefix, own, [(19 * i) % (own + 1) for i in range(seqs)], dtype, seed=prefix)
+    check(gpu.attention_shared_prefix(*case), *case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("garbage", [float("nan"), float("inf"), -65504.0])
+def test_many_queries_do_not_look_behind_the_last_row(gpu, garbage):
+    q, kp, vp, ko, vo, lens = inputs(70, 16, 8, 128, 1001, 77, [(13 * i) % 78 for i in range(70)], "fp16", seed=14)
+    wide = [torch.full((8, 1301, 128), garbage, dtype=torch.float16, device="cuda") for _ in range(2)]
+    for w, t in zip(wide, (kp, vp)):
+        w[:, :1001] = t
+    for b, n in enumerate(lens.tolist()):
+        ko[b, :, n:] = garbage
+        vo[b, :, n:] = garbage
+    case = (q, wide[0][:, :1001], wide[1][:, :1001], ko, vo, lens)
+    got = gpu.attention_shared_prefix(*case)
+    assert not bool(got[0].isnan().any())
+    check(got, *case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [0.0, -0.05, 1.0, 3.0])
+def test_many_queries_and_scales(gpu, scale):
+    case = inputs(80, 16, 8, 128, 899, 50, [(17 * i) % 51 for i in range(80)], "fp16", seed=2, gain=0.5)
+    check(gpu.attention_shared_prefix(*case, scale=scale), *case, scale=scale)
+
+
+@pytest.mark.gpu
+def test_many_queries_whose_maximum_rises_late(gpu):
+    q, kp, vp, ko, vo, lens = inputs(66, 16, 8, 128, 4000, 40, [40] * 66, "fp16", seed=6)
+    q[:] = q[:1, :1]
+    kp += (torch.linspace(-2, 2, 4000).cuda()[None, :, None] * q[0, 0]).half()
+    case = (q, kp, vp, ko, vo, lens)
+    check(gpu.attention_shared_prefix(*case), *case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs", [9, 100])
+def test_broadcast_inputs_and_heads_between_rows(gpu, seqs):
+    """A kv head expanded to all, one query expanded to all, one own cache for all sequences, [rows, heads, dim] caches."""
+    q, kp, vp, ko, vo, lens = inputs(seqs, 16, 8, 128, 1001, 50, [(7 * i) % 51 for i in range(seqs)], "fp16", seed=31)
+    one = (q, kp[:1].expand(8, 1001, 128), vp[:1].expand(8, 1001, 128), ko[:1].expand(seqs, 8, 50, 128), vo[:1].expand(seqs, 8, 50, 128), lens)
+    check(gpu.attention_shared_prefix(*one), *one)
+    check(gpu.attention_shared_prefix(*one[:3], [ko[0]] * seqs, [vo[0]] * seqs, lens), *one)
+    same = (q[:1].expand(seqs, 16, 128), *one[1:])
+    check(gpu.attention_shared_prefix(*same), *same)
+    row = (q, kp[:, :1].expand(8, 1001, 128), vp[:, :1].expand(8, 1001, 128), ko, vo, lens)
+    check(gpu.attention_shared_prefix(*row), *row)
+    between = (q, kp.transpose(0, 1).contiguous().transpose(0, 1), vp.transpose(0, 1).contiguous().transpose(0, 1), ko, vo, lens)
+    check(gpu.attention_shared_prefix(*between), *between)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs", [9, 100])
+def test_offsets_of_more_than_32_bits(gpu, seqs):
+    """Rows 2^22 and heads 2^31 elements apart; own caches 2^25 apart, so the last from 2^31 on."""
+    q, kp, vp, ko, vo, lens = inputs(seqs, 4, 2, 128, 1100, 40, [(7 * i) % 41 for i in range(seqs)], "fp16", seed=41)
+    buf = torch.empty(1100 * (1 << 22) + (1 << 12), dtype=torch.float16, device="cuda")
+    rows = [buf.as_strided((2, 1100, 128), (256, 1 << 22, 1), at) for at in (0, 128)]
+    heads = [buf.as_strided((2, 1100, 128), (1 << 31, 256, 1), at) for at in (1024, 1152)]
+    own = [buf.as_strided((seqs, 2, 40, 128), (1 << 25, 128 * 128, 128, 1), at) for at in (1 << 20, (1 << 20) + 128 * 40)]
+    for k, v in (rows, heads):
+        k.copy_(kp)
+        v.copy_(vp)
+        check(gpu.attention_shared_prefix(q, k, v, ko, vo, lens), q, kp, vp, ko, vo, lens)
+    own[0].copy_(ko)
+    own[1].copy_(vo)
+    check(gpu.attention_shared_prefix(q, kp, vp, *own, lens), q, kp, vp, ko, vo, lens)
+
+
+@pytest.mark.gpu
+def test_many_queries_two_calls_at_once_and_in_graphs(gpu):
+    case = inputs(90, 16, 8, 128, 2000, 99, [(31 * i) % 100 for i in range(90)], "fp16", seed=5)
+    other = (case[0].flip(0).contiguous(), *case[1:5], case[5].flip(0).contiguous())
+    want = gpu.attention_shared_prefix(*case), gpu.attention_shared_prefix(*other)
+    check(want[0], *case)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    graphs, results = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for stream, graph, c in zip(streams, graphs, (case, other)):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.graph(graph, stream=stream):
+            results.append(gpu.attention_shared_prefix(*c))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for out, lse in results:
+            out.zero_()
+            lse.zero_()
+        torch.cuda.synchronize()
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        got = gpu.attention_shared_prefix(*case)
+        torch.cuda.synchronize()
+        for (o, l), w in zip((*results, got), (*want, want[0])):
+            assert torch.equal(o, w[0]) and torch.equal(l, w[1])
