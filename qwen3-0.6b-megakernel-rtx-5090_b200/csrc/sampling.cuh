@@ -12,15 +12,16 @@
 //
 // A cluster of CTAs takes a row, as many as leave every row's CTAs resident together.  A row is read from one to three times; it crosses
 // HBM the first time, and is in L1 or L2 then.  (Rows kept in shared memory as fp32 needed clusters of eight for 151,936 tokens, so 128
-// rows four waves of CTAs in lockstep: 76 us for the plain draw and 88 with top-k, where two CTAs a row without it take 50 and 38.)
+// rows four waves of CTAs in lockstep: 76 us for the plain draw and 88 with top-k, where two CTAs a row without it take 52 and 38.)
 // A threshold (of top-k, of top-p) is found by narrowing down: a histogram of counts over the distance to the maximum, then, where
 // the tokens up to the border's bin are few, a list of them that one CTA sorts and finishes; else a list of the border's bins alone.  Rows
-// whose border lies among more (nearly) equal values than a list holds go through eight-bit histograms of the keys (search).
+// whose border lies among more (nearly) equal values than a list holds go through eight-bit histograms of the keys (search).  Top-p alone, the
+// common case, has its histogram from the first pass, while the row crosses HBM: its bins lie on a ring and need no maximum.
 //
-// Measured, us a call in a graph with fp32 rows of 151,936 tokens, one / 32 / 128 of them (12 us of HBM): plain draw 12 / 18 / 50, min-p 10 / 13 / 29, top-k 50 with
-// top-p 17 / 22 / 38, top-p alone 32 / 54 / 133.  Few rows: the chain of reductions across the cluster, 1 to 2 us each.  Many: instruction issue, a
-// mass (a power of two in 64 bits, rounded to a whole number) of every token within SPAN of the maximum in each pass - the plain draw has one such pass and top-p
-// three; min-p and top-k compare in 32 bits and leave few tokens to weigh.
+// Measured, us a call in a graph with fp32 rows of 151,936 tokens, one / 32 / 128 of them (12 us of HBM): plain draw 13 / 20 / 52, min-p 10 / 13 / 29, top-k 50 with
+// top-p 17 / 22 / 38, top-p alone 30 / 44 / 91.  Few rows: the chain of reductions across the cluster, 1 to 2 us each.  Many: instruction issue, a
+// mass (a power of two in 64 bits, rounded to a whole number) of every token within SPAN of the maximum in each pass - the plain draw and top-p have one such
+// pass; min-p and top-k compare in 32 bits and leave few tokens to weigh.
 #ifndef QMK_SAMPLING_CUH_
 #define QMK_SAMPLING_CUH_
 
@@ -50,6 +51,10 @@ constexpr int TURN = 3;                           // fours that a thread has in 
 constexpr int NO_TOKEN = 0x7fffffff;             // pick of a row without a largest value, as in the greedy steps
 constexpr float LARGEST_UNIFORM = 0x1.fffffep-1f;
 constexpr float LARGEST_TEMPERATURE = 0x1p100f;  // (SPAN temperatures and the products with it stay finite)
+constexpr int RING = 4096;                       // bins of the first pass' counts
+constexpr float AROUND = 64.0f, SPAN_AROUND = 34.0f;     // logits, or temperatures where those are more, once round them: more than 1.01 SPAN and the rounding
+constexpr float COUNT = 8192.0f;                 // a token in the middle of its bin there: 2^18 of them fit 32 bits
+constexpr int WINDOW = 200;                      // tokens to either side of the border that these counts suggest
 constexpr int EACH = LIST / THREADS;
 static_assert(BINS == 4 * THREADS && MASS_BINS == 6 * THREADS && LIST == 4 * THREADS, "bins and list entries per thread");
 
@@ -67,7 +72,7 @@ struct Params {
 };
 
 struct __align__(16) Shared {
-  unsigned int counts[MASS_BINS];                // this CTA's histogram, read by the cluster: of tokens (BINS) or of masses
+  unsigned int counts[RING];                     // this CTA's histogram, read by the cluster: of tokens (BINS) or of masses (MASS_BINS, RING)
   union {
     unsigned long long keys[2][KEY_BINS];    // search: histograms in turn, one is read while the next is filled
     unsigned long long sorted[LIST];
@@ -76,7 +81,7 @@ struct __align__(16) Shared {
   double powers[STEPS * COLUMNS];                // 2^(j / 64), a column for each lane of half a warp
   unsigned long long warp[WARPS], warp_kept[WARPS], group[GROUPS];
   unsigned long long inbox[16][MAX_CLUSTER];     // one row per exchange of the cluster, see gather
-  unsigned long long found[4], border[4];
+  unsigned long long found[4], border[6];
   unsigned long long threshold;                  // written by the CTA that finds it
   int listed, collected;
 };
@@ -278,11 +283,32 @@ __global__ void __launch_bounds__(THREADS, AN_SM) sample_rows(const Params p) {
   };
 
   // ---- the row, once; its largest value and where that is first
-  for (int b = tid; b < MASS_BINS / 4; b += THREADS) reinterpret_cast<uint4 *>(s.counts)[b] = make_uint4(0, 0, 0, 0);
+  for (int b = tid; b < RING / 4; b += THREADS) reinterpret_cast<uint4 *>(s.counts)[b] = make_uint4(0, 0, 0, 0);
   if (tid == 0) { s.listed = 0; s.collected = 0; }
   for (int i = tid; i < STEPS * COLUMNS; i += THREADS) s.powers[i] = exp2(static_cast<double>(i / COLUMNS) / STEPS);      // (read behind the first barrier)
   float high[TURN] = {-INFINITY, -INFINITY, -INFINITY};          // the largest values of three parts of what this thread has seen
-  walk([&](float4 v, int, int j) { high[j] = fmaxf(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), high[j]); });
+  // Top-p alone: a histogram, too, over the value's place on a ring of bins, which needs no maximum (near_border), of masses in units of
+  // the bin's middle.  What is further below the thread's maximum so far than any mass reaches is left out.
+  const float grain = RING / fmaxf(AROUND, SPAN_AROUND * temperature), step = 1.0f / (grain * temperature);      // bins per logit, a bin's width in temperatures
+  const bool counting = top_p < 1.0f && !(top_k > 0 && top_k < p.vocab) && asked > 0.0f && step < 0.1f;
+  auto ring_bin = [&](float v) { return __float_as_int(fmaf(v, grain, 12582912.0f)); };      // (1.5 * 2^23: the nearest whole number in the low bits)
+  auto count = [&](float v) {
+    const float b = fmaf(v, grain, 12582912.0f), r = fmaf(v, grain, 12582912.0f - b) * step;
+    atomicAdd(&s.counts[__float_as_int(b) & (RING - 1)], static_cast<unsigned int>(__float_as_int(fmaf(fmaf(r, 0.5f, 1.0f) * r, COUNT, 8388608.0f + COUNT)) & 0x3fff));
+  };
+  if (counting) {
+    __syncthreads();                             // (the counts are 0)
+    walk([&](float4 v, int, int j) {
+      high[j] = fmaxf(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), high[j]);
+      const float low = fmaxf(fmaf(-1.01f * SPAN, temperature, high[j]), -3.4e38f);
+      if (v.x >= low) count(v.x);
+      if (v.y >= low) count(v.y);
+      if (v.z >= low) count(v.z);
+      if (v.w >= low) count(v.w);
+    });
+  } else {
+    walk([&](float4 v, int, int j) { high[j] = fmaxf(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), high[j]); });
+  }
   float top;
   {
     uint32_t best = __reduce_max_sync(0xffffffffu, key_of(fmaxf(fmaxf(high[0], high[1]), high[2])));
@@ -336,7 +362,7 @@ __global__ void __launch_bounds__(THREADS, AN_SM) sample_rows(const Params p) {
   }
 
   const double top64 = top;
-  const float nothing = top - 1.01f * SPAN * temperature;      // below it masses round to 0 (and the exponent of 2 may be any)
+  const float nothing = fmaf(-1.01f * SPAN, temperature, top);      // below it masses round to 0 (and the exponent of 2 may be any)
   const double *const powers = s.powers + (lane & (COLUMNS - 1));
   // 2^n 2^(j / 64) and the polynomial whose product is the mass of v
   auto factors = [&](float v, double &power, int &k) {
@@ -643,7 +669,7 @@ __global__ void __launch_bounds__(THREADS, AN_SM) sample_rows(const Params p) {
   };
   // no value of the bins 0 .. j is below this
   auto bound_of = [&](int j) { return top - (static_cast<float>(j) + 0.51f) / per_bin * (1.0f + 1e-5f) - 1e-6f * fabsf(top); };
-  auto clear_counts = [&]() { for (int b = tid; b < MASS_BINS / 4; b += THREADS) reinterpret_cast<uint4 *>(s.counts)[b] = make_uint4(0, 0, 0, 0); };
+  auto clear_counts = [&]() { for (int b = tid; b < RING / 4; b += THREADS) reinterpret_cast<uint4 *>(s.counts)[b] = make_uint4(0, 0, 0, 0); };
   // The cluster's histogram: a CTA adds up its share of the bins, of which a thread has up to six, one behind the other.  (Every CTA reading
   // all of the others' 3072 bins took 10 us.)
   struct Share { unsigned int c[6]; int bin, mine; };
@@ -739,7 +765,172 @@ __global__ void __launch_bounds__(THREADS, AN_SM) sample_rows(const Params p) {
     if (tid == 0) { s.listed = 0; s.collected = 0; }
     cluster.sync();                              // (rank 0's counter is the others')
   }
-  if (top_p < 1.0f) {
+  // Where the border of top-p lies in the sorted list, `front` being the mass in front of the list's tokens; then the pick, where min_p takes nothing
+  // away.  `mine`, `range`: the masses in front of them of this CTA and of this warp's range.
+  auto settle = [&](unsigned long long front, unsigned long long mine, unsigned long long range, unsigned long long want) {
+    const int listed = collect();
+    if (rank == 0) {                             // how many of them stay
+      unsigned long long w[EACH], before, all = 0;
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) {
+        w[j] = EACH * tid + j < listed ? mass(value_of(s.sorted[EACH * tid + j])) : 0;
+        all += w[j];
+      }
+      block_scan(all, before);
+      before += front;
+      int stay = 0;
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) {
+        stay += __syncthreads_count(EACH * tid + j < listed && before < want);
+        before += w[j];
+      }
+      announce(max(stay, 1));
+    }
+    cluster.sync();
+    cut_at(s.threshold);
+    if (least > 0.0 && weight(kept_value) < least) return false;
+    if (lane == 0) s.warp_kept[warp] = range;    // the ranges' sums are there but for the listed tokens that stay
+    __syncthreads();
+    unsigned long long sum = 0;
+    for (int i = tid; i < s.listed; i += THREADS) {
+      const float v = value_of(s.list[i]);
+      const int at = index_of(s.list[i]);
+      const unsigned long long m = kept(v, at) ? mass(v) : 0;
+      sum += m;
+      if (m) atomicAdd(&s.warp_kept[((at - first) >> 2) / seg], m);
+    }
+    find(mine + block_sum(sum), s.warp_kept, kept_value, [&](float v, int i) -> unsigned long long { const unsigned long long m = mass(v); return kept(v, i) ? m : 0ull; }, draw_from, write);
+    cluster.sync();
+    return true;
+  };
+  // Three sums over the CTA, and over the cluster with those of the ranks in front.
+  auto three_sums = [&](const unsigned long long (&v)[3], unsigned long long (&total)[3], unsigned long long (&front)[3]) {
+    const int slot = exchange;
+    exchange += 3;
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+      if (tid < ranks) *cluster.map_shared_rank(&s.inbox[(slot + j) & 15][rank], tid) = v[j];
+      total[j] = front[j] = 0;
+    }
+    cluster.sync();
+    for (int r = 0; r < ranks; ++r)
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        const unsigned long long c = s.inbox[(slot + j) & 15][r];
+        front[j] += r < rank ? c : 0;
+        total[j] += c;
+      }
+  };
+  // Top-p from the counts of the first pass: they say near which token the border is.  One pass adds up the
+  // masses, of all and of those in front of the WINDOW tokens to either side of it, which it lists; if the border is among them, the sums say
+  // so, and the rest is as exact as without the counts.  (128 rows of 151,936 tokens: 133 us by the bins of masses below, 91 so; with p = 0.999 384 and 94.)
+  enum { ELSEWHERE, LISTED, WRITTEN };
+  unsigned long long front_mass = 0, front_mine = 0, front_range = 0, want_mass = 0;         // for settle, where the border's tokens are listed
+  auto near_border = [&]() -> int {
+    const int top_bin = ring_bin(top);
+    const int all = RING / ranks, each_ = max(all / THREADS, 1), mine = tid * each_ < all ? each_ : 0, at0 = rank * all + tid * each_;
+    uint32_t *const units = reinterpret_cast<uint32_t *>(s.sorted) + tid * each_;        // the cluster's, of this thread's bins
+    static_assert(RING * sizeof(uint32_t) <= sizeof(s.sorted), "a CTA's share of the ring");
+    auto tokens = [&](int j) { return static_cast<unsigned long long>((units[j] + static_cast<uint32_t>(COUNT / 2)) / static_cast<uint32_t>(COUNT)); };
+    auto estimate = [&](int j) { return __float2ull_rn(static_cast<float>(units[j]) * exp2f(27.0f - static_cast<float>(at0 + j) * (step * 1.4426950f))); };
+    unsigned long long sums[3] = {0, 0, 0}, before[2], total[3], front[3];
+#pragma unroll 1
+    for (int j = 0; j < mine; ++j) {
+      uint32_t c = 0;
+#pragma unroll
+      for (int r = 0; r < MAX_CLUSTER; ++r) c += r < ranks ? cluster.map_shared_rank(s.counts, r)[(top_bin - at0 - j) & (RING - 1)] : 0;
+      units[j] = c;
+      sums[0] += tokens(j);
+      sums[1] += estimate(j);
+    }
+    if (tid == 0) { s.border[0] = 0; s.border[1] = 0; s.border[2] = RING - 1; s.border[3] = 0; s.border[4] = ~0ull; }
+    const unsigned long long own_tokens = sums[0], own_estimate = sums[1];
+    sums[0] = block_scan(own_tokens, before[0]);
+    sums[1] = block_scan(own_estimate, before[1]);
+    three_sums(sums, total, front);
+    const unsigned long long target = share_of(total[1]), n0 = front[0] + before[0];
+    {
+      unsigned long long run = front[1] + before[1], n = n0;
+      if (run < target && target <= run + own_estimate)
+#pragma unroll 1
+        for (int j = 0; j < mine; ++j) {
+          const unsigned long long e = estimate(j), c = tokens(j);
+          if (run < target && target <= run + e) {
+            const unsigned long long centre = n + static_cast<unsigned long long>(__ull2double_rn(c) * (__ull2double_rn(target - run) / __ull2double_rn(e)));
+            for (int r = 0; r < ranks; ++r) cluster.map_shared_rank(s.border, r)[1] = centre;
+          }
+          run += e;
+          n += c;
+        }
+    }
+    cluster.sync();
+    const unsigned long long centre = s.border[1], from_ = centre > 512 ? centre - WINDOW : 0, to_ = centre + WINDOW;   // (not many: all in front, too)
+    if ((n0 < from_ && from_ <= n0 + own_tokens) || (n0 < to_ && to_ <= n0 + own_tokens)) {
+      unsigned long long n = n0;
+#pragma unroll 1
+      for (int j = 0; j < mine; ++j) {
+        const unsigned long long c = tokens(j);
+        if (n < from_ && from_ <= n + c)
+          for (int r = 0; r < ranks; ++r) { unsigned long long *const to = cluster.map_shared_rank(s.border, r); to[0] = at0 + j; to[3] = n; }
+        if (n < to_ && to_ <= n + c)
+          for (int r = 0; r < ranks; ++r) { unsigned long long *const to = cluster.map_shared_rank(s.border, r); to[2] = at0 + j; to[4] = n + c; }
+        n += c;
+      }
+    }
+    cluster.sync();
+    const int lo = static_cast<int>(s.border[0]), hi = static_cast<int>(s.border[2]);
+    if (min(s.border[4], total[0]) - s.border[3] > LIST * 15 / 16) return ELSEWHERE;        // (bins of many tokens; the counts are rounded)
+    unsigned long long v_sum[3] = {0, 0, 0};     // of all, in front of the window, in it
+    walk([&](float4 v4, int i, int) {
+      const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+      unsigned long long m[4];
+      int b[4];
+      bool at_border = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        m[j] = mass(v[j]);
+        b[j] = v[j] >= nothing ? top_bin - ring_bin(v[j]) : RING;
+        v_sum[0] += m[j];
+        v_sum[1] += b[j] < lo ? m[j] : 0;
+        at_border = at_border || (b[j] >= lo && b[j] <= hi);
+      }
+      if (at_border) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (b[j] >= lo && b[j] <= hi) { v_sum[2] += m[j]; list(v[j], first + 4 * i + j); }
+      }
+    });
+    const unsigned long long range = warp_sum(v_sum[1]);
+    const unsigned long long own[3] = {block_sum(v_sum[0]), block_sum(v_sum[1]), block_sum(v_sum[2])};
+    three_sums(own, total, front);
+    const unsigned long long want = share_of(total[0]);
+    if (!(total[1] < want && want <= total[1] + total[2])) return ELSEWHERE;
+    if (lo == 0) {
+      const int listed = collect();
+      if (rank == 0) finish_list(listed, ~0ull, want);
+      return WRITTEN;
+    }
+    front_mass = total[1];
+    front_mine = own[1];
+    front_range = range;
+    want_mass = want;
+    return LISTED;
+  };
+  bool listed_border = false;
+  if (counting) {
+    int how = ELSEWHERE;
+    // (bins of whole numbers that floats hold: then those of the massive tokens are in the order of the values, and none of them round the ring)
+    if (!infinite && fabsf(top) * grain < 2097152.0f) how = near_border();
+    if (how == WRITTEN) return;
+    listed_border = how == LISTED;
+    if (!listed_border) {
+      cluster.sync();                            // (what the others read or write here has been)
+      clear_counts();
+      if (tid == 0) { s.listed = 0; s.collected = 0; }
+      cluster.sync();
+    }
+  }
+  if (top_p < 1.0f && !listed_border) {
     unsigned long long sum = 0;
     walk([&](float4 v4, int i, int) {              // (four tokens' arithmetic side by side, then the atomics)
       const float v[4] = {v4.x, v4.y, v4.z, v4.w};
@@ -831,49 +1022,20 @@ __global__ void __launch_bounds__(THREADS, AN_SM) sample_rows(const Params p) {
           if (b[j] >= lo && b[j] < MASS_BINS) list(v[j], first + 4 * i + j);
       }
     });
-    const unsigned long long mine = block_sum(sum), ranges = warp_sum(sum);
+    const unsigned long long mine = block_sum(sum), range = warp_sum(sum);
     gather(mine, [&](int, unsigned long long v) { front += v; });
     if (few_at_border) {
-      const int listed = collect();
-      if (rank == 0) {                           // how many of them stay
-        unsigned long long w[EACH], before, all = 0;
-#pragma unroll
-        for (int j = 0; j < EACH; ++j) {
-          w[j] = EACH * tid + j < listed ? mass(value_of(s.sorted[EACH * tid + j])) : 0;
-          all += w[j];
-        }
-        block_scan(all, before);
-        before += front;
-        int stay = 0;
-#pragma unroll
-        for (int j = 0; j < EACH; ++j) {
-          stay += __syncthreads_count(EACH * tid + j < listed && before < want);
-          before += w[j];
-        }
-        announce(max(stay, 1));
-      }
-      cluster.sync();
-      cut_at(s.threshold);
-      if (least == 0.0 || weight(kept_value) >= least) {       // (min_p takes nothing away) the ranges' sums are there but for the listed tokens that stay
-        if (lane == 0) s.warp_kept[warp] = ranges;
-        __syncthreads();
-        sum = 0;
-        for (int i = tid; i < s.listed; i += THREADS) {
-          const float v = value_of(s.list[i]);
-          const int at = index_of(s.list[i]);
-          const unsigned long long m = kept(v, at) ? mass(v) : 0;
-          sum += m;
-          if (m) atomicAdd(&s.warp_kept[((at - first) >> 2) / seg], m);
-        }
-        find(mine + block_sum(sum), s.warp_kept, kept_value, [&](float v, int i) -> unsigned long long { const unsigned long long m = mass(v); return kept(v, i) ? m : 0ull; }, draw_from, write);
-        cluster.sync();
-        return;
-      }
+      front_mass = front;
+      front_mine = mine;
+      front_range = range;
+      want_mass = want;
+      listed_border = true;
     } else {                                     // (many equal values, or a very flat row)
       cut_at(search([&](float v, int i) { const int b = mass_bin(v); return b >= lo && b <= hi && kept(v, i) ? mass(v) : 0ull; },
                     [&](unsigned long long) { return want - front; }));
     }
   }
+  if (listed_border && settle(front_mass, front_mine, front_range, want_mass)) return;
   if (cut || least > 0.0)
     pick(fmaxf(kept_value, least_value), [&](float v, int i) -> unsigned long long { const unsigned long long m = above_least(v); return kept(v, i) ? m : 0ull; }, draw_from, write);
   else

@@ -295,3 +295,34 @@ def test_two_calls_at_once(gpu):
     torch.cuda.synchronize()
     for i, (tokens, logp) in enumerate(got):
         assert torch.equal(tokens, want[i % 2][0]) and torch.equal(logp, want[i % 2][1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("vocab", [3001, 40000, 151936])
+def test_top_p_alone(gpu, dtype, vocab):
+    """From a few tokens that stay to nearly all, sharp and flat, a temperature per row; values of bf16 are equal in hundreds."""
+    ps, ts = (0.001, 0.3, 0.6, 0.9, 0.97, 0.999, 0.99999), (0.1, 0.17, 0.4, 0.8, 1.3, 2.5)
+    rows = len(ps) * len(ts)
+    x, u, _ = rows_of_logits(rows, vocab, 17)
+    # (equal values on both sides of a border of 64-bit sums: skipped as elsewhere)
+    check(gpu, x.to(DTYPES[dtype]), u, temperature=torch.tensor([t for t in ts for _ in ps]), top_p=torch.tensor(ps * len(ts)), skipped=0.05)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("masked", [-3.4028234663852886e38, -65504.0, -1e4, -100.0, -60.0, -40.0, float("-inf"), float("nan")])
+@pytest.mark.parametrize("stay", [1, 30, 5000])
+def test_top_p_of_rows_with_masked_tokens(gpu, masked, stay):
+    """Whole ranges of a row masked by low values, at its beginning, end or between; a few other outliers far below and above."""
+    x, u, g = rows_of_logits(12, 30000, 23)
+    for i in range(12):
+        at = (0, 30000 - stay, 12345)[i % 3]
+        keep = x[i, at:at + stay].clone()
+        x[i] = masked
+        x[i, at:at + stay] = keep
+        if i % 4 == 3:
+            x[i, at] = 90.0
+            x[i, 29999] = -70.0
+    for p in (0.5, 0.95):
+        check(gpu, x, u, temperature=0.8, top_p=p, skipped=0.1)
+    check(gpu, x, u, temperature=0.8, top_p=0.9, min_p=0.02, skipped=0.1)
