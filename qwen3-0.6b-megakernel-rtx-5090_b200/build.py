@@ -12,12 +12,15 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 SOURCES = [os.path.join(HERE, "csrc", "megakernel_sm100.cu"), os.path.join(HERE, "csrc", "megakernel_batch_sm100.cu"),
            os.path.join(HERE, "csrc", "megakernel_tc_sm100.cu"), os.path.join(HERE, "csrc", "megakernel_tc_fp8_sm100.cu"),
            *(os.path.join(HERE, "csrc", f"megakernel_tc_{fmt}seqs{n}_sm100.cu") for fmt in ("", "fp8_") for n in (2, 4)),
            os.path.join(HERE, "csrc", "prefill_sm100.cu"), os.path.join(HERE, "csrc", "sampling_sm100.cu"),
+           *(os.path.join(HERE, "csrc", f"sampling_{t}_sm100.cu") for t in ("fp32", "fp16", "bf16")),
            os.path.join(HERE, "csrc", "shared_prefix_sm100.cu")]
 HEADERS = [os.path.join(os.path.dirname(HERE), "include", "qwen_megakernel.h"),
            os.path.join(HERE, "csrc", "megakernel_device.cuh"), os.path.join(HERE, "csrc", "megakernel_params.h"),
@@ -26,7 +29,7 @@ HEADERS = [os.path.join(os.path.dirname(HERE), "include", "qwen_megakernel.h"),
            os.path.join(HERE, "csrc", "gemm_tcgen05.cuh"), os.path.join(HERE, "csrc", "gemm_pair_tcgen05.cuh"), os.path.join(HERE, "csrc", "prefill_sm100.h"),
            os.path.join(HERE, "csrc", "prefill_kernels.cuh"), os.path.join(HERE, "csrc", "engine_internal.h"), os.path.join(HERE, "csrc", "buffer_group.h"),
            os.path.join(HERE, "csrc", "attention_tcgen05.cuh"), os.path.join(HERE, "csrc", "decode_attention_mma.cuh"),
-           os.path.join(HERE, "csrc", "sampling.cuh"), os.path.join(HERE, "csrc", "shared_prefix_attention.cuh"),
+           os.path.join(HERE, "csrc", "sampling.cuh"), os.path.join(HERE, "csrc", "sampling_launch.cuh"), os.path.join(HERE, "csrc", "shared_prefix_attention.cuh"),
            os.path.join(HERE, "csrc", "shared_prefix_tcgen05.cuh")]
 LIB_PATH = os.path.join(HERE, "libqwen_megakernel.so")
 
@@ -82,14 +85,24 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not is_stale():
         return LIB_PATH
     tmp = LIB_PATH + ".tmp"
-    cmd = [_nvcc(), *NVCC_FLAGS, "-Xptxas", "-v", "-o", tmp, *SOURCES]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + proc.stdout + proc.stderr)
-    check_stack_frames(proc.stderr)
+
+    def run(cmd):
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        if proc.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + proc.stdout + proc.stderr)
+        return proc.stderr
+
+    # The sources side by side (216 s one behind the other), then the library of their objects
+    with tempfile.TemporaryDirectory() as objects, ThreadPoolExecutor(max(1, min(8, os.cpu_count() or 1))) as pool:
+        paths = [os.path.join(objects, os.path.basename(src)[:-len(".cu")] + ".o") for src in SOURCES]
+        compile_flags = [flag for flag in NVCC_FLAGS if flag != "-shared"]
+        logs = list(pool.map(lambda job: run([_nvcc(), *compile_flags, "-Xptxas", "-v", "-c", "-o", job[1], job[0]]), zip(SOURCES, paths)))
+        for log in logs:
+            check_stack_frames(log)
+        run([_nvcc(), *NVCC_FLAGS, "-o", tmp, *paths])
     os.replace(tmp, LIB_PATH)
     if verbose:
-        print(proc.stderr)
+        print("".join(logs))
     return LIB_PATH
 
 

@@ -42,7 +42,7 @@ constexpr int MAX_CLUSTER = 8;
 constexpr int GROUPS = (MAX_VOCAB / 4 + 1 + WARPS * 32 - 1) / (WARPS * 32);   // of 128 tokens, in a warp's range of a row: at most
 constexpr int BINS = 2048;                       // of the distance to the maximum: 4 per thread
 constexpr float SPAN = 32.5f;                    // times the temperature: masses further below the maximum round to nothing (e^-32.5 < 2^-46)
-constexpr int MASS_BINS = 3072;                  // of masses, 2^(1/64) wide, down to 2^-48: 6 per thread
+constexpr int MASS_BINS = 6 * THREADS;           // of masses, 2^(1/64) wide, down to 2^-48: 6 per thread
 constexpr double ONE = 8192.0;                   // a mass of its bin's middle in a histogram of masses: 2^18 of them fit 32 bits
 constexpr int KEY_BINS = 256;                    // of a histogram of keys: eight bits
 constexpr int LIST = 2048;                       // tokens that one CTA sorts: EACH per thread
@@ -56,7 +56,7 @@ constexpr float AROUND = 64.0f, SPAN_AROUND = 34.0f;     // logits, or temperatu
 constexpr float COUNT = 8192.0f;                 // a token in the middle of its bin there: 2^18 of them fit 32 bits
 constexpr int WINDOW = 200;                      // tokens to either side of the border that these counts suggest
 constexpr int EACH = LIST / THREADS;
-static_assert(BINS == 4 * THREADS && MASS_BINS == 6 * THREADS && LIST == 4 * THREADS, "bins and list entries per thread");
+static_assert(BINS == 4 * THREADS && LIST == 4 * THREADS, "bins and list entries per thread");
 
 struct Params {
   const void *logits;
@@ -70,6 +70,11 @@ struct Params {
   int *tokens;
   float *logprobs;                               // may be null
 };
+
+// (sampling_launch.cuh)
+cudaError_t launch_fp32(const Params &p, int rows, cudaStream_t stream);
+cudaError_t launch_fp16(const Params &p, int rows, cudaStream_t stream);
+cudaError_t launch_bf16(const Params &p, int rows, cudaStream_t stream);
 
 struct __align__(16) Shared {
   unsigned int counts[RING];                     // this CTA's histogram, read by the cluster: of tokens (BINS) or of masses (MASS_BINS, RING)
@@ -671,7 +676,7 @@ __global__ void __launch_bounds__(THREADS, AN_SM) sample_rows(const Params p) {
   auto bound_of = [&](int j) { return top - (static_cast<float>(j) + 0.51f) / per_bin * (1.0f + 1e-5f) - 1e-6f * fabsf(top); };
   auto clear_counts = [&]() { for (int b = tid; b < RING / 4; b += THREADS) reinterpret_cast<uint4 *>(s.counts)[b] = make_uint4(0, 0, 0, 0); };
   // The cluster's histogram: a CTA adds up its share of the bins, of which a thread has up to six, one behind the other.  (Every CTA reading
-  // all of the others' 3072 bins took 10 us.)
+  // all of the others' bins took 10 us.)
   struct Share { unsigned int c[6]; int bin, mine; };
   auto share_of_bins = [&](int bins) {
     Share h;

@@ -1,8 +1,6 @@
 // C entry of the sampling kernel (sampling.cuh).
 #include "../../include/qwen_megakernel.h"
 
-#include <algorithm>
-#include <atomic>
 #include <string>
 
 #include "engine_internal.h"
@@ -15,63 +13,6 @@ using namespace qmk_sample;
 int refuse(const std::string &why) {
   qmk_internal::note_error("qmk_sample_tokens: " + why);
   return QMK_ERR_BAD_ARGUMENT;
-}
-
-constexpr int DEVICES = 16;
-
-template <typename T, int AN_SM>
-struct Launch {
-  static constexpr int SMEM = sizeof(Shared) + 2 * TURN * THREADS * 4 * sizeof(T);
-  static void configure(cudaLaunchConfig_t *cfg, cudaLaunchAttribute *attr, int rows, int ranks, cudaStream_t stream) {
-    *cfg = {};
-    cfg->gridDim = dim3(static_cast<unsigned int>(rows) * ranks);
-    cfg->blockDim = dim3(THREADS);
-    cfg->dynamicSmemBytes = SMEM;
-    cfg->stream = stream;
-    attr->id = cudaLaunchAttributeClusterDimension;
-    attr->val.clusterDim.x = ranks;
-    attr->val.clusterDim.y = 1;
-    attr->val.clusterDim.z = 1;
-    cfg->attrs = attr;
-    cfg->numAttrs = 1;
-  }
-  // Rows whose clusters of `ranks` CTAs are resident together on this device; asked for once.  (Clusters lie inside a GPC, of which not all have as
-  // many SMs: 16 clusters of eight CTAs on 128 of 148 SMs took two waves, 24 us where four CTAs a row took 17.)
-  static cudaError_t resident(int device, int ranks, int *rows) {
-    static std::atomic<int> known[DEVICES][4];
-    std::atomic<int> &at = known[device][ranks == 8 ? 3 : ranks >> 1];
-    if ((*rows = at.load()) > 0) return cudaSuccess;
-    cudaError_t e = cudaFuncSetAttribute(sample_rows<T, AN_SM>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-    cudaLaunchConfig_t cfg;
-    cudaLaunchAttribute attr;
-    configure(&cfg, &attr, 1, ranks, nullptr);
-    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(rows, sample_rows<T, AN_SM>, &cfg);
-    if (e == cudaSuccess) at.store(*rows = std::max(*rows, 1));
-    return e;
-  }
-  static cudaError_t run(const Params &p, int rows, int ranks, cudaStream_t stream) {
-    cudaLaunchConfig_t cfg;
-    cudaLaunchAttribute attr;
-    configure(&cfg, &attr, rows, ranks, stream);
-    return cudaLaunchKernelEx(&cfg, sample_rows<T, AN_SM>, p);
-  }
-};
-
-// CTAs per row: as many as leave all rows resident at once, with at least 1024 tokens each; alone on their SMs where that is enough.
-template <typename T>
-cudaError_t launch(const Params &p, int rows, cudaStream_t stream) {
-  int device = 0;
-  cudaError_t e = cudaGetDevice(&device);
-  if (e == cudaSuccess && device >= DEVICES) e = cudaErrorInvalidDevice;
-  for (int ranks = MAX_CLUSTER; e == cudaSuccess; ranks /= 2) {
-    if (ranks > 1 && p.vocab <= ranks / 2 * 1024) continue;
-    int alone = 0, two = 0;
-    e = Launch<T, 1>::resident(device, ranks, &alone);
-    if (e == cudaSuccess && rows <= alone) return Launch<T, 1>::run(p, rows, ranks, stream);
-    if (e == cudaSuccess) e = Launch<T, 2>::resident(device, ranks, &two);
-    if (e == cudaSuccess && (rows <= two || ranks == 1)) return Launch<T, 2>::run(p, rows, ranks, stream);
-  }
-  return e;
 }
 
 }  // namespace
@@ -104,7 +45,7 @@ extern "C" int qmk_sample_tokens(const void *logits, int logits_type, long long 
   p.top_k = top_k;
   p.tokens = tokens;
   p.logprobs = logprobs;
-  const cudaError_t e = logits_type == 0 ? launch<float>(p, rows, stream) : logits_type == 1 ? launch<__half>(p, rows, stream) : launch<__nv_bfloat16>(p, rows, stream);
+  const cudaError_t e = logits_type == 0 ? launch_fp32(p, rows, stream) : logits_type == 1 ? launch_fp16(p, rows, stream) : launch_bf16(p, rows, stream);
   if (e != cudaSuccess) {
     cudaGetLastError();
     qmk_internal::note_error(std::string("qmk_sample_tokens: ") + cudaGetErrorString(e));
