@@ -884,7 +884,7 @@ __global__ void __launch_bounds__(THREADS, AN_SM) sample_rows(const Params p) {
     }
     cluster.sync();
     const int lo = static_cast<int>(s.border[0]), hi = static_cast<int>(s.border[2]);
-    if (min(s.border[4], total[0]) - s.border[3] > LIST * 15 / 16) return ELSEWHERE;        // (bins of many tokens; the counts are rounded)
+    if (min(s.border[4], total[0]) - s.border[3] > LIST * 7 / 8) return ELSEWHERE;        // (bins of many tokens; the counts are up to a tenth low)
     unsigned long long v_sum[3] = {0, 0, 0};     // of all, in front of the window, in it
     walk([&](float4 v4, int i, int) {
       const float v[4] = {v4.x, v4.y, v4.z, v4.w};
