@@ -19,6 +19,7 @@ import array
 import ctypes
 import functools
 import os
+import struct
 
 import torch
 
@@ -108,6 +109,11 @@ class _SharedPrefixArgs(ctypes.Structure):
 
 _lib.qmk_attention_shared_prefix.argtypes = [ctypes.POINTER(_SharedPrefixArgs), _P]
 _lib.qmk_attention_shared_prefix.restype = _I
+# The same as bytes, which take a fifth of the time to fill (1.3 us)
+_pack_shared_prefix_args = struct.Struct("@5i P2q 2Pi2q 4Pqi2q P if 3Pq")
+assert _pack_shared_prefix_args.size == ctypes.sizeof(_SharedPrefixArgs)
+_pack_shared_prefix_args = _pack_shared_prefix_args.pack
+_attention_shared_prefix = ctypes.CFUNCTYPE(_I, ctypes.c_char_p, _P)(("qmk_attention_shared_prefix", _lib))
 _lib.qmk_attention_shared_prefix_workspace.argtypes = [_I] * 6
 _lib.qmk_attention_shared_prefix_workspace.restype = _LL
 _lib.qmk_sample_batched.argtypes = [_I, _P, _P, _I, *([_P] * 6), _P, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _F, _P]
@@ -780,10 +786,11 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     need = _shared_prefix_workspace(n, q_heads, kv_heads, dim, prefix, rows)
     workspace = own_lens.new_empty(need >> 2)
     q_seq, q_head, _ = q.stride()
-    args = _SharedPrefixArgs(code, n, q_heads, kv_heads, dim, q.data_ptr(), q_seq, q_head, k_prefix.data_ptr(), v_prefix.data_ptr(), prefix,
-                             prefix_strides[1], prefix_strides[0], k_ptrs, v_ptrs, k_base, v_base, own_seq, rows, own_row, own_head, own_lens.data_ptr(), 0,
-                             dim ** -0.5 if scale is None else scale, out.data_ptr(), lse.data_ptr(), workspace.data_ptr(), need)
-    rc = _on_device(index, _lib.qmk_attention_shared_prefix, args)
+    args = _pack_shared_prefix_args(code, n, q_heads, kv_heads, dim, q.data_ptr(), q_seq, q_head, k_prefix.data_ptr(), v_prefix.data_ptr(), prefix,
+                                    prefix_strides[1], prefix_strides[0], k_ptrs, v_ptrs, k_base, v_base, own_seq, rows, own_row, own_head,
+                                    own_lens.data_ptr(), 0, dim ** -0.5 if scale is None else scale, out.data_ptr(), lse.data_ptr(), workspace.data_ptr(),
+                                    need)
+    rc = _on_device(index, _attention_shared_prefix, args)
     if rc != 0:
         raise RuntimeError(f"{who}: {_lib.qmk_last_error().decode()} (status {rc})")
     return out, lse
