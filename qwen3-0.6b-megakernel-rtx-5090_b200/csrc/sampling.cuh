@@ -19,7 +19,7 @@
 // common case, has its histogram from the first pass, while the row crosses HBM: its bins lie on a ring and need no maximum.
 //
 // Measured, us a call in a graph with fp32 rows of 151,936 tokens, one / 32 / 128 of them (12 us of HBM): plain draw 13 / 20 / 52, min-p 10 / 13 / 29, top-k 50 with
-// top-p 17 / 22 / 38, top-p alone 30 / 44 / 91.  Few rows: the chain of reductions across the cluster, 1 to 2 us each.  Many: instruction issue, a
+// top-p 17 / 22 / 38, top-p alone 29 / 43 / 86.  Few rows: the chain of reductions across the cluster, 1 to 2 us each.  Many: instruction issue, a
 // mass (a power of two in 64 bits, rounded to a whole number) of every token within SPAN of the maximum in each pass - the plain draw and top-p have one such
 // pass; min-p and top-k compare in 32 bits and leave few tokens to weigh.
 #ifndef QMK_SAMPLING_CUH_
@@ -306,6 +306,10 @@ __global__ void __launch_bounds__(THREADS, AN_SM) sample_rows(const Params p) {
     walk([&](float4 v, int, int j) {
       high[j] = fmaxf(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), high[j]);
       const float low = fmaxf(fmaf(-1.01f * SPAN, temperature, high[j]), -3.4e38f);
+      if (v.x >= low && v.y >= low && v.z >= low && v.w >= low) {      // (nearly always)
+        count(v.x); count(v.y); count(v.z); count(v.w);
+        return;
+      }
       if (v.x >= low) count(v.x);
       if (v.y >= low) count(v.y);
       if (v.z >= low) count(v.z);
@@ -828,7 +832,7 @@ __global__ void __launch_bounds__(THREADS, AN_SM) sample_rows(const Params p) {
   };
   // Top-p from the counts of the first pass: they say near which token the border is.  One pass adds up the
   // masses, of all and of those in front of the WINDOW tokens to either side of it, which it lists; if the border is among them, the sums say
-  // so, and the rest is as exact as without the counts.  (128 rows of 151,936 tokens: 133 us by the bins of masses below, 91 so; with p = 0.999 384 and 94.)
+  // so, and the rest is as exact as without the counts.  (128 rows of 151,936 tokens: 133 us by the bins of masses below, 86 so; with p = 0.999 384 and 89.)
   enum { ELSEWHERE, LISTED, WRITTEN };
   unsigned long long front_mass = 0, front_mine = 0, front_range = 0, want_mass = 0;         // for settle, where the border's tokens are listed
   auto near_border = [&]() -> int {
@@ -885,6 +889,8 @@ __global__ void __launch_bounds__(THREADS, AN_SM) sample_rows(const Params p) {
     cluster.sync();
     const int lo = static_cast<int>(s.border[0]), hi = static_cast<int>(s.border[2]);
     if (min(s.border[4], total[0]) - s.border[3] > LIST * 7 / 8) return ELSEWHERE;        // (bins of many tokens; the counts are up to a tenth low)
+    const int lo_bin = top_bin - lo, hi_bin = top_bin - hi;    // as ring_bin gives them: larger in front (tokens without a mass anywhere)
+    const unsigned int width = static_cast<unsigned int>(lo_bin - hi_bin);
     unsigned long long v_sum[3] = {0, 0, 0};     // of all, in front of the window, in it
     walk([&](float4 v4, int i, int) {
       const float v[4] = {v4.x, v4.y, v4.z, v4.w};
@@ -894,15 +900,15 @@ __global__ void __launch_bounds__(THREADS, AN_SM) sample_rows(const Params p) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         m[j] = mass(v[j]);
-        b[j] = v[j] >= nothing ? top_bin - ring_bin(v[j]) : RING;
+        b[j] = ring_bin(v[j]);
         v_sum[0] += m[j];
-        v_sum[1] += b[j] < lo ? m[j] : 0;
-        at_border = at_border || (b[j] >= lo && b[j] <= hi);
+        v_sum[1] += b[j] > lo_bin ? m[j] : 0;
+        at_border = at_border || static_cast<unsigned int>(b[j] - hi_bin) <= width;
       }
       if (at_border) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (b[j] >= lo && b[j] <= hi) { v_sum[2] += m[j]; list(v[j], first + 4 * i + j); }
+          if (static_cast<unsigned int>(b[j] - hi_bin) <= width && v[j] >= nothing) { v_sum[2] += m[j]; list(v[j], first + 4 * i + j); }
       }
     });
     const unsigned long long range = warp_sum(v_sum[1]);
