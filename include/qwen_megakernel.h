@@ -416,8 +416,8 @@ int qmk_gemm_packed_tn(const void *a, const void *b, const void *b2, void *c, in
  * their total, logprobs[row] (DEVICE fp32, may be null) the logarithm of w / total for it.  A temperature that is not above 0 takes the
  * largest value (the lowest index of ties), one above 2^100 counts as 2^100.  A row without a largest value (all NaN or -inf) gives 2^31 - 1
  * and NaN, as a greedy step.  temperatures, top_ks, top_ps, min_ps: DEVICE arrays with a value per row, or null: the scalar behind it for all
- * rows (a scalar that is negative, or no number, and a top_p of 0 are refused; in an array a top_p that is not above 0 keeps the first token, and a top_p
- * or min_p that is no number is off).  A row_stride of 0 draws from one row `rows` times.  rows in [0, 65536], vocab in [1, 262144].  Picks do
+ * rows (a scalar that is negative, or no number, and a top_p of 0 are refused; in an array a top_p that is not above 0 or a min_p above 1 keeps the
+ * first token alone, and a top_p or min_p that is no number is off).  A row_stride of 0 draws from one row `rows` times.  rows in [0, 65536], vocab in [1, 262144].  Picks do
  * not depend on the other rows or on the run: masses are summed as whole multiples of 2^-45.  Does not block, allocates nothing, may be
  * captured behind a first call on the device. */
 int qmk_sample_tokens(const void *logits, int logits_type, long long row_stride, int rows, int vocab, const float *uniforms,

@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(THREADS, AN_SM) sample_rows(const Params p) {
     });
   };
   const bool empty = top == -INFINITY;
-  if (empty || !(asked > 0.0f) || top_k == 1) {
+  if (empty || !(asked > 0.0f) || top_k == 1 || min_p > 1.0f) {      // (no mass is above that of the largest value: the first of the order stays alone)
     uint32_t at = 0xffffffffu;
     if (!empty) each_from(top, [&](float v, int i) { if (v == top) at = min(at, static_cast<uint32_t>(i)); });
     at = __reduce_min_sync(0xffffffffu, at);

@@ -326,3 +326,61 @@ def test_top_p_of_rows_with_masked_tokens(gpu, masked, stay):
     for p in (0.5, 0.95):
         check(gpu, x, u, temperature=0.8, top_p=p, skipped=0.1)
     check(gpu, x, u, temperature=0.8, top_p=0.9, min_p=0.02, skipped=0.1)
+
+
+def _garbage_outputs(rows):
+    """What the next outputs of this size are made of: neither tokens nor logarithms."""
+    for _ in range(4):
+        torch.full((rows,), -77, dtype=torch.int32, device="cuda")
+        torch.full((rows,), 77.0, device="cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("vocab", [1, 300, 40000])
+def test_a_min_p_above_one_keeps_the_first_token(gpu, vocab, dtype):
+    """In an array, where it is not refused: no token's mass is above the largest one's, and one token always stays - the first of equal ones."""
+    ways = [(0, 1.0), (0, 0.9), (0, 0.99999), (50, 1.0), (50, 0.9), (20000, 1.0), (20000, 0.9), (20000, 0.99999)]
+    rows = len(ways)
+    x, u, _ = rows_of_logits(rows, vocab, 41)
+    x = (x - x.amax(1, keepdim=True)).to(DTYPES[dtype])          # (bounds around the largest value are closest to it at 0)
+    ties = x.clone()
+    at = [vocab // 3, vocab // 2, vocab - 1]
+    ties[:, at] = 0.0
+    flat = torch.zeros_like(x)
+    for case in (x, x + 5.0, ties, flat, -40.0 + ties):
+        for least in (1.0000001, 1.5, 1e30, float("inf")):
+            options = dict(top_k=torch.tensor([k for k, _ in ways], dtype=torch.int32), top_p=torch.tensor([p for _, p in ways]),
+                           min_p=torch.full((rows,), least))
+            _garbage_outputs(rows)
+            got = check(gpu, case, u, temperature=torch.tensor([0.05, 0.7, 1.0, 2.5] * (rows // 4)), skipped=1.0, **options)
+            assert got.tolist() == case.float().argmax(1).tolist()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [50, 20000])
+def test_what_arrays_of_options_may_hold(gpu, vocab):
+    """Values that a scalar may not have: a row's meaning is that of the valid value beside it, and the rows around it are as they were."""
+    nan, inf = float("nan"), float("inf")
+    means = [  # (temperature, top_k, top_p, min_p), and the same in valid values
+        ((0.8, 0, 1.0, 0.0), None), ((-1.0, 0, 0.9, 0.0), (0.0, 0, 1.0, 0.0)), ((nan, 5, 1.0, 0.1), (0.0, 0, 1.0, 0.0)), ((-inf, 0, 1.0, 0.0), (0.0, 0, 1.0, 0.0)),
+        ((-0.0, 0, 1.0, 0.0), (0.0, 0, 1.0, 0.0)), ((inf, 0, 1.0, 0.0), (2.0 ** 100, 0, 1.0, 0.0)), ((1e38, 7, 1.0, 0.0), (2.0 ** 100, 7, 1.0, 0.0)),
+        ((0.8, -3, 1.0, 0.0), (0.8, 0, 1.0, 0.0)), ((0.8, -2 ** 31, 0.9, 0.0), (0.8, 0, 0.9, 0.0)), ((0.8, 2 ** 31 - 1, 0.9, 0.0), (0.8, 0, 0.9, 0.0)),
+        ((0.8, 0, 0.0, 0.0), (0.8, 1, 1.0, 0.0)), ((0.8, 40, -0.5, 0.0), (0.8, 1, 1.0, 0.0)), ((0.8, 0, -inf, 0.3), (0.8, 1, 1.0, 0.0)), ((0.8, 0, 1e-45, 0.0), (0.8, 1, 1.0, 0.0)),
+        ((0.8, 0, nan, 0.0), (0.8, 0, 1.0, 0.0)), ((0.8, 30, nan, 0.05), (0.8, 30, 1.0, 0.05)), ((0.8, 0, 2.0, 0.0), (0.8, 0, 1.0, 0.0)), ((0.8, 0, inf, 0.0), (0.8, 0, 1.0, 0.0)),
+        ((0.8, 0, 1.0, nan), (0.8, 0, 1.0, 0.0)), ((0.8, 30, 0.9, nan), (0.8, 30, 0.9, 0.0)), ((0.8, 0, 1.0, -1.0), (0.8, 0, 1.0, 0.0)), ((0.8, 0, 0.95, -inf), (0.8, 0, 0.95, 0.0)),
+        ((0.8, 0, 1.0, 1.0), None), ((0.8, 0, 0.9, 1.0), None), ((0.8, 0, 0.9, 0.2), None)]
+    rows = len(means)
+    x, u, _ = rows_of_logits(rows, vocab, 43)
+    given = list(zip(*(g for g, _ in means)))
+    got, logp = gpu.sample_tokens(x.cuda(), u.cuda(), torch.tensor(given[0]).cuda(), torch.tensor(given[1], dtype=torch.int32).cuda(),
+                                  torch.tensor(given[2]).cuda(), torch.tensor(given[3]).cuda())
+    got, logp, borders = got.cpu(), logp.cpu(), 0
+    for i, (g, same) in enumerate(means):
+        t, k, p, mp = same or g
+        token, lp, near = definition(x[i].double().numpy(), float(u[i]), float(np.float32(t)), k, p, mp)
+        borders += near
+        if not near:
+            assert int(got[i]) == token, (i, g)
+            assert abs(float(logp[i]) - lp) <= abs(lp) * 2.0 ** -24 + 2.0 ** -28, (i, g)
+    assert borders <= 1
