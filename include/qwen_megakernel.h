@@ -430,7 +430,8 @@ int qmk_sample_tokens(const void *logits, int logits_type, long long row_stride,
  * logarithm of the sum of exp(scale * q . k).  Nothing visible: zeros and -inf.  Rows behind the last are not looked at.  Strides in
  * elements, multiples of 8; the head dimension is contiguous; pointers 16-byte aligned (the workspace 32).  Limits: 1 to 128 sequences, 1 to
  * 16 query heads per kv head, head_dim 64 or 128, 2^24 rows.  Does not block, allocates nothing, may be captured behind a first call with its types
- * and sizes on the device; the workspace (DEVICE, size from qmk_attention_shared_prefix_workspace) belongs to the call until it is done. */
+ * and sizes on the device; the workspace (DEVICE, size from qmk_attention_shared_prefix_workspace) belongs to the call until it is done.  Waits on
+ * the device are bounded: where one runs out, the rows concerned are NaN and `status` says so. */
 typedef struct qmk_shared_prefix_args {
   int type;                          /* 0 fp16, 1 bf16: q, caches and out */
   int num_sequences, q_heads, kv_heads, head_dim;
@@ -452,6 +453,8 @@ typedef struct qmk_shared_prefix_args {
   float *lse;                        /* [num_sequences][q_heads], may be null */
   void *workspace;
   long long workspace_bytes;
+  unsigned int *status;              /* DEVICE, may be null: where a bounded wait runs out, QMK_ERR_WAIT_TIMEOUT goes into it if it holds 0 */
+  int timeout_ms;                    /* budget of those waits; 0: 2000 */
 } qmk_shared_prefix_args;
 int qmk_attention_shared_prefix(const qmk_shared_prefix_args *args, cudaStream_t stream);
 long long qmk_attention_shared_prefix_workspace(int num_sequences, int q_heads, int kv_heads, int head_dim, int prefix_len, int own_rows);
@@ -500,6 +503,9 @@ int qmk_selftest_attention_wait_timeout(int budget_us);
 /* The same for the attention of a step of qmk_decode_batched.  what = 1: nothing is loaded; 2: one chunk of cache rows never comes while
  * others are in flight. */
 int qmk_selftest_decode_attention_wait_timeout(int budget_us, int what);
+/* The same for qmk_attention_shared_prefix on tcgen05: score products that stop behind the second tile, keys and values in flight; returns
+ * QMK_ERR_WAIT_TIMEOUT when that happened as designed and the outputs of all rows are NaN. */
+int qmk_selftest_shared_prefix_wait_timeout(int budget_us);
 
 /* The same for the pairs of CTAs that multiply more than 512 rows.  what = 1: no loads; 2: the issuing thread gives up behind its
  * first tile, with a ring of copies in flight; 3: the second CTA of the pair loads nothing. */

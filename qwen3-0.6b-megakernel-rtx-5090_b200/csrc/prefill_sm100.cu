@@ -1513,6 +1513,8 @@ static int decode_batched(const char *who, const Sampling *sampling, int num_seq
         a.out = w.attn;
         a.workspace = w.shared_ws;
         a.workspace_bytes = static_cast<long long>(w.shared_ws_bytes);
+        a.status = w.status;
+        a.timeout_ms = env.timeout_ms;
         if ((r2 = qmk_attention_shared_prefix(&a, s)) != QMK_OK) { err = qmk_last_error(); return r2; }
       } else if (env.attn_mma)
         PF_CUDA(qmk_tc::launch_kernel(decode_attention_mma<>, dim3(attn_ctas), dim3((DAM_WARPS + 1) * 32), DAM_SMEM_BYTES, s,
@@ -1634,8 +1636,8 @@ static int decode_batched(const char *who, const Sampling *sampling, int num_seq
   PF_CUDA(cudaStreamSynchronize(stream));
   if (host_status[0] != 0)
     return qmk_internal::report(static_cast<int>(host_status[0]),
-                                host_status[0] == QMK_ERR_BAD_TOKEN ? "decode_batched: a pick outside [0, vocab) (logits without a largest value)"
-                                                                    : "decode_batched: a bounded device wait ran out");
+                                std::string(who) + (host_status[0] == QMK_ERR_BAD_TOKEN ? ": a pick outside [0, vocab) (logits without a largest value)"
+                                                                                        : ": a bounded device wait ran out"));
   return QMK_OK;
 }
 

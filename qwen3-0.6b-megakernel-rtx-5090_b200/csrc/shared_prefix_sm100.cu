@@ -59,7 +59,7 @@ bool make_maps(CUtensorMap *maps, const Params &p, const Split &s, int head_dim,
 }
 
 template <typename T, int D, int NT>
-cudaError_t launch(Params &p, const Split &s, const CUtensorMap *maps, unsigned int *status, cudaStream_t stream) {
+cudaError_t launch(Params &p, const Split &s, const CUtensorMap *maps, unsigned int *status, unsigned long long budget_ns, cudaStream_t stream) {
   using Own = OwnRows<T, D, NT, own_warps(D)>;
   using Beside = OwnRows<T, D, NT, WARPS>;
   constexpr int own_smem = OWN_STAGES * 2 * Own::TILE, beside_smem = OWN_STAGES * 2 * Beside::TILE, smem = STAGES * 2 * KEYS * D * 2;
@@ -75,7 +75,7 @@ cudaError_t launch(Params &p, const Split &s, const CUtensorMap *maps, unsigned 
     if (e == cudaSuccess) e = cudaFuncSetAttribute(own_parts<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, own_smem);
     if (e == cudaSuccess)
       e = qmk_tc::launch_kernel(prefix_parts_tc<T, D>, dim3(prefix_items), dim3(TC_THREADS), tc_smem_bytes<D>(), stream, maps[0], maps[1], maps[2], p,
-                                s.seqs_per_tile, status);
+                                s.seqs_per_tile, status, budget_ns);
     dependent = true;                            // (of the launch before, inside this call)
     const qmk_tc::PdlScope scope(true);
     if (e == cudaSuccess && own_items > 0) e = qmk_tc::launch_kernel(own_parts<T, D, NT>, dim3(own_items), dim3(32 * own_warps(D)), own_smem, stream, p);
@@ -91,9 +91,9 @@ cudaError_t launch(Params &p, const Split &s, const CUtensorMap *maps, unsigned 
   return qmk_tc::launch_kernel(join_parts<T, D>, dim3(p.seqs * p.q_heads), dim3(128), 0, stream, p);
 }
 template <typename T>
-cudaError_t launch(Params &p, const Split &s, int head_dim, const CUtensorMap *maps, unsigned int *status, cudaStream_t stream) {
-  if (p.group > 8) return head_dim == 64 ? launch<T, 64, 2>(p, s, maps, status, stream) : launch<T, 128, 2>(p, s, maps, status, stream);
-  return head_dim == 64 ? launch<T, 64, 1>(p, s, maps, status, stream) : launch<T, 128, 1>(p, s, maps, status, stream);
+cudaError_t launch(Params &p, const Split &s, int head_dim, const CUtensorMap *maps, unsigned int *status, unsigned long long budget_ns, cudaStream_t stream) {
+  if (p.group > 8) return head_dim == 64 ? launch<T, 64, 2>(p, s, maps, status, budget_ns, stream) : launch<T, 128, 2>(p, s, maps, status, budget_ns, stream);
+  return head_dim == 64 ? launch<T, 64, 1>(p, s, maps, status, budget_ns, stream) : launch<T, 128, 1>(p, s, maps, status, budget_ns, stream);
 }
 
 }  // namespace
@@ -118,6 +118,7 @@ extern "C" int qmk_attention_shared_prefix(const qmk_shared_prefix_args *a, cuda
   if (!a->q || !a->out || (a->prefix_len > 0 && (!a->k_prefix || !a->v_prefix)) || (a->own_rows > 0 && (a->k_own ? !a->v_own : !a->k_own_base || !a->v_own_base)) || (a->own_rows > 0 && !a->own_lens))
     return refuse("null pointer argument");
   if (!(a->scale > -2.0e38f && a->scale < 2.0e38f)) return refuse("the scale must be finite, and below 2e38");   // (times log2 e too)
+  if (a->timeout_ms < 0) return refuse("timeout_ms is negative");
   auto aligned = [](const void *ptr) { return (reinterpret_cast<unsigned long long>(ptr) & 15u) == 0; };
   bool ok = aligned(a->q) && aligned(a->k_prefix) && aligned(a->v_prefix) && aligned(a->out) && (reinterpret_cast<unsigned long long>(a->workspace) & 31u) == 0;
   Params p;
@@ -165,14 +166,75 @@ extern "C" int qmk_attention_shared_prefix(const qmk_shared_prefix_args *a, cuda
   const long long states = static_cast<long long>(s.prefix_parts + s.own_parts) * p.seqs * p.q_heads;
   p.part_out = static_cast<float *>(a->workspace);
   p.part_ml = reinterpret_cast<float2 *>(p.part_out + states * a->head_dim);
-  unsigned int *const status = reinterpret_cast<unsigned int *>(p.part_ml + states);
+  unsigned int *const status = a->status ? a->status : reinterpret_cast<unsigned int *>(p.part_ml + states);      // (in the workspace for nobody)
+  const unsigned long long budget_ns = (a->timeout_ms ? a->timeout_ms : 2000) * 1000000ull;
   p.out = a->out;
   p.lse = a->lse;
-  const cudaError_t e = a->type == 0 ? launch<__half>(p, s, a->head_dim, maps, status, stream) : launch<__nv_bfloat16>(p, s, a->head_dim, maps, status, stream);
+  const cudaError_t e = a->type == 0 ? launch<__half>(p, s, a->head_dim, maps, status, budget_ns, stream)
+                                     : launch<__nv_bfloat16>(p, s, a->head_dim, maps, status, budget_ns, stream);
   if (e != cudaSuccess) {
     cudaGetLastError();
     qmk_internal::note_error(std::string("qmk_attention_shared_prefix: ") + cudaGetErrorString(e));
     return QMK_ERR_CUDA;
   }
   return QMK_OK;
+}
+
+extern "C" int qmk_selftest_shared_prefix_wait_timeout(int budget_us) {
+  qmk_internal::begin_call();
+  if (budget_us < 1 || budget_us > 1000000) return refuse("budget_us must be in [1, 1e6]");
+  // 64 sequences of two heads on each of two kv heads (a tile of 128 query rows), 1024 prefix rows in one range
+  constexpr int SEQS = 64, GROUP = 2, KV = 2, HEADS = GROUP * KV, D = 128, ROWS = 1024, STATES = SEQS * HEADS;
+  constexpr size_t q_bytes = 2ull * STATES * D, kv_bytes = 2ull * KV * ROWS * D, at_k = q_bytes, at_v = at_k + kv_bytes, at_out = at_v + kv_bytes,
+                   at_lse = at_out + q_bytes, at_parts = at_lse + 4ull * STATES, at_ml = at_parts + 4ull * STATES * D, at_status = at_ml + 8ull * STATES,
+                   total = at_status + 16;
+  unsigned char *buf = nullptr;
+  cudaError_t e = cudaMalloc(&buf, total);
+  if (e == cudaSuccess) e = cudaMemset(buf, 0, total);
+  Params p = {};
+  p.q = buf;
+  p.q_seq = HEADS * D;
+  p.q_head = D;
+  p.seqs = SEQS;
+  p.group = GROUP;
+  p.q_heads = HEADS;
+  p.kv_heads = KV;
+  p.k_prefix = buf + at_k;
+  p.v_prefix = buf + at_v;
+  p.prefix_row = D;
+  p.prefix_head = ROWS * D;
+  p.prefix_len = p.prefix_range = ROWS;
+  p.prefix_parts = p.row_tiles = 1;
+  p.scale_log2 = 1.0f;
+  p.part_out = reinterpret_cast<float *>(buf + at_parts);
+  p.part_ml = reinterpret_cast<float2 *>(buf + at_ml);
+  p.out = buf + at_out;
+  p.lse = reinterpret_cast<float *>(buf + at_lse);
+  unsigned int *const status = reinterpret_cast<unsigned int *>(buf + at_status);
+  Split s = {};
+  s.seqs_per_tile = SEQS;
+  CUtensorMap maps[3];
+  unsigned int word = 0;
+  float lse[STATES];
+  __half out[STATES];                       // one dimension of every row
+  if (e == cudaSuccess && !make_maps(maps, p, s, D, false)) e = cudaErrorInvalidValue;
+  auto *const kernel = prefix_parts_tc<__half, D, true>;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(tc_smem_bytes<D>()));
+  if (e == cudaSuccess) {
+    kernel<<<KV, TC_THREADS, tc_smem_bytes<D>()>>>(maps[0], maps[1], maps[2], p, SEQS, status, budget_us * 1000ull);
+    join_parts<__half, D><<<STATES, 128>>>(p);
+    e = cudaGetLastError();
+  }
+  if (e == cudaSuccess) e = cudaMemcpy(&word, status, 4, cudaMemcpyDeviceToHost);
+  if (e == cudaSuccess) e = cudaMemcpy(lse, p.lse, sizeof(lse), cudaMemcpyDeviceToHost);
+  if (e == cudaSuccess) e = cudaMemcpy2D(out, 2, p.out, 2 * D, 2, STATES, cudaMemcpyDeviceToHost);
+  cudaFree(buf);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    qmk_internal::note_error(std::string("self test of the attention over a shared prefix: ") + cudaGetErrorString(e));
+    return QMK_ERR_CUDA;
+  }
+  for (int i = 0; i < STATES; ++i)
+    if (lse[i] == lse[i] || !__hisnan(out[i])) return QMK_OK;
+  return static_cast<int>(word);
 }

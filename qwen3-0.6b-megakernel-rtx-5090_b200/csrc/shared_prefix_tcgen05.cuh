@@ -13,7 +13,7 @@
 //
 // The running maximum is raised when it grew by more than 2^3; weights are stored times 2^P_SHIFT (fp16: 2^12, so at most 2^15), which keeps ten
 // more bits of the small ones than storing them as they are.
-// Waits are bounded by 2 s.  A CTA whose wait ran out leaves NaN as the state of its rows, so that the result is NaN.
+// Waits are bounded.  On a time-out the CTA sets *status = 4 and leaves NaN as the state of its rows, so that the result is NaN.
 #ifndef QMK_SHARED_PREFIX_TCGEN05_CUH_
 #define QMK_SHARED_PREFIX_TCGEN05_CUH_
 
@@ -24,7 +24,6 @@
 
 namespace qmk_spa {
 
-constexpr unsigned long long WAIT_NS = 2000000000ull;
 constexpr int TC_THREADS = qmk_attn::THREADS;
 constexpr int TC_ROWS = 128;                                       // prefix rows per tile
 constexpr uint32_t BOX_BYTES = 64 * 128, BLOCK_BYTES = 128 * 128;  // [64 rows x 64 dims], [128 rows x 64 dims or keys], swizzled
@@ -39,11 +38,11 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
 }
 
 // map_q: {dims, heads of a kv head, kv heads, sequences}, boxes of {64, group, 1, seqs_per_tile}; map_k / map_v: {dims, prefix rows, kv heads}, boxes of
-// {64, 64, 1}; 128-byte swizzle, zeros outside.
-template <typename T, int D>
+// {64, 64, 1}; 128-byte swizzle, zeros outside.  TEST: the self test's score issuer that stops behind its second tile.
+template <typename T, int D, bool TEST = false>
 __global__ void __launch_bounds__(TC_THREADS, 1)
 prefix_parts_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                const __grid_constant__ Params p, int seqs_per_tile, unsigned int *status) {
+                const __grid_constant__ Params p, int seqs_per_tile, unsigned int *status, unsigned long long budget_ns) {
   using namespace qmk_gemm;
   using qmk_attn::tma_load_3d;
   using qmk_attn::fast_exp2;
@@ -124,25 +123,26 @@ prefix_parts_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       const bool is_v = warp != 0;
       int issued = is_v ? 0 : k_prefilled;
       for (int j = issued; j < ntiles; ++j) {
-        if (j >= 2 && !bar_wait(is_v ? v_empty(j & 1) : k_empty(j & 1), ((j >> 1) - 1) & 1, abort_flag, status, WAIT_NS)) break;
+        if (j >= 2 && !bar_wait(is_v ? v_empty(j & 1) : k_empty(j & 1), ((j >> 1) - 1) & 1, abort_flag, status, budget_ns)) break;
         if (*abort_flag) break;
         load_tile(is_v, j);
         issued = j + 1;
       }
       if (*abort_flag)
-        for (int j = (issued > 2 ? issued - 2 : 0); j < issued; ++j) bar_drain(is_v ? v_full(j & 1) : k_full(j & 1), (j >> 1) & 1, WAIT_NS);
+        for (int j = (issued > 2 ? issued - 2 : 0); j < issued; ++j) bar_drain(is_v ? v_full(j & 1) : k_full(j & 1), (j >> 1) & 1, budget_ns);
     }
   } else if (warp == 1) {
     if (elect_one()) {                     // ---- scores
       for (int j = 0; j < ntiles; ++j) {
         const int c = j & 1, n = j >> 1;
-        const bool ok = (j > 0 || bar_wait(q_full, 0, abort_flag, status, WAIT_NS)) && bar_wait(k_full(c), n & 1, abort_flag, status, WAIT_NS) &&
-                        (n == 0 || bar_wait(s_free(c), (n - 1) & 1, abort_flag, status, WAIT_NS));
+        bool ok = (j > 0 || bar_wait(q_full, 0, abort_flag, status, budget_ns)) && bar_wait(k_full(c), n & 1, abort_flag, status, budget_ns) &&
+                  (n == 0 || bar_wait(s_free(c), (n - 1) & 1, abort_flag, status, budget_ns));
+        if (TEST && j == 2) ok = bar_wait(s_stopped, 0, abort_flag, status, budget_ns);      // (nothing arrives)
         if (!ok) {                         // the products issued end, and so do the copies that the loader may have asked for
-          bar_drain(q_full, 0, WAIT_NS);
+          bar_drain(q_full, 0, budget_ns);
           mma_commit(s_stopped);
-          bar_drain(s_stopped, 0, WAIT_NS);
-          for (int i = j; i < ntiles && i < j + 2; ++i) bar_drain(k_full(i & 1), (i >> 1) & 1, WAIT_NS);
+          bar_drain(s_stopped, 0, budget_ns);
+          for (int i = j; i < ntiles && i < j + 2; ++i) bar_drain(k_full(i & 1), (i >> 1) & 1, budget_ns);
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -160,10 +160,10 @@ prefix_parts_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     if (elect_one()) {                     // ---- P . V
       for (int j = 0; j < ntiles; ++j) {
         const int c = j & 1, n = j >> 1;
-        if (!bar_wait(v_full(c), n & 1, abort_flag, status, WAIT_NS) || !bar_wait(p_ready(c), n & 1, abort_flag, status, WAIT_NS)) {
+        if (!bar_wait(v_full(c), n & 1, abort_flag, status, budget_ns) || !bar_wait(p_ready(c), n & 1, abort_flag, status, budget_ns)) {
           mma_commit(pv_stopped);
-          bar_drain(pv_stopped, 0, WAIT_NS);
-          for (int i = j; i < ntiles && i < j + 2; ++i) bar_drain(v_full(i & 1), (i >> 1) & 1, WAIT_NS);
+          bar_drain(pv_stopped, 0, budget_ns);
+          for (int i = j; i < ntiles && i < j + 2; ++i) bar_drain(v_full(i & 1), (i >> 1) & 1, budget_ns);
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -190,7 +190,7 @@ prefix_parts_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     bool ok = true;
     for (int j = chain; j < ntiles && ok; j += CHAINS) {
       const int n = j >> 1;
-      ok = __all_sync(0xffffffffu, bar_wait(s_full(chain), n & 1, abort_flag, status, WAIT_NS));
+      ok = __all_sync(0xffffffffu, bar_wait(s_full(chain), n & 1, abort_flag, status, budget_ns));
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       uint32_t s[4][32];
@@ -225,7 +225,7 @@ prefix_parts_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       const bool raise = mx > m_used + RAISE;                        // always from -inf, but for scores of -inf
       const float m_new = raise ? mx : m_used, alpha = raise ? exp2f(m_used - m_new) : 1.0f;
       if (n > 0) {
-        ok = __all_sync(0xffffffffu, bar_wait(pv_done(chain), (n - 1) & 1, abort_flag, status, WAIT_NS));
+        ok = __all_sync(0xffffffffu, bar_wait(pv_done(chain), (n - 1) & 1, abort_flag, status, budget_ns));
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (__any_sync(0xffffffffu, raise)) {
@@ -250,7 +250,7 @@ prefix_parts_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       // The chains take turns at the exponentials, so that one's products run under the other's: side by side in step, both wait for products
       // and then share the units.
       if (chain == 1 || n > 0) {
-        ok = __all_sync(0xffffffffu, bar_wait(turn(chain), (chain == 1 ? n : n - 1) & 1, abort_flag, status, WAIT_NS));
+        ok = __all_sync(0xffffffffu, bar_wait(turn(chain), (chain == 1 ? n : n - 1) & 1, abort_flag, status, budget_ns));
         if (!ok) break;
       }
       const float sub = Half<T>::P_SHIFT - (m_used == -INFINITY ? 0.f : m_used);
@@ -277,8 +277,8 @@ prefix_parts_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(p_ready(chain)) : "memory");
     }
     const int my_tiles = (ntiles - chain + 1) / CHAINS;
-    if (ok && my_tiles > 0) ok = __all_sync(0xffffffffu, bar_wait(pv_done(chain), (my_tiles - 1) & 1, abort_flag, status, WAIT_NS));
-    if (!ok) bar_drain(pv_done(chain), (my_tiles - 1) & 1, WAIT_NS);
+    if (ok && my_tiles > 0) ok = __all_sync(0xffffffffu, bar_wait(pv_done(chain), (my_tiles - 1) & 1, abort_flag, status, budget_ns));
+    if (!ok) bar_drain(pv_done(chain), (my_tiles - 1) & 1, budget_ns);
     // ---- the two chains' states, joined per row; (maximum, sum) go through the chain's own P tile
     asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(p_tile + static_cast<uint32_t>(row) * 8u), "f"(m_used), "f"(l) : "memory");
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

@@ -104,13 +104,13 @@ class _SharedPrefixArgs(ctypes.Structure):
                 ("k_prefix", _P), ("v_prefix", _P), ("prefix_len", _I), ("prefix_row_stride", _LL), ("prefix_head_stride", _LL),
                 ("k_own", _P), ("v_own", _P), ("k_own_base", _P), ("v_own_base", _P), ("own_seq_stride", _LL), ("own_rows", _I), ("own_row_stride", _LL), ("own_head_stride", _LL),
                 ("own_lens", _P), ("own_lens_add", _I), ("scale", _F), ("out", _P), ("lse", _P), ("workspace", _P),
-                ("workspace_bytes", _LL)]
+                ("workspace_bytes", _LL), ("status", _P), ("timeout_ms", _I)]
 
 
 _lib.qmk_attention_shared_prefix.argtypes = [ctypes.POINTER(_SharedPrefixArgs), _P]
 _lib.qmk_attention_shared_prefix.restype = _I
 # The same as bytes, which take a fifth of the time to fill (1.3 us)
-_pack_shared_prefix_args = struct.Struct("@5i P2q 2Pi2q 4Pqi2q P if 3Pq")
+_pack_shared_prefix_args = struct.Struct("@5i P2q 2Pi2q 4Pqi2q P if 3Pq Pi0q")
 assert _pack_shared_prefix_args.size == ctypes.sizeof(_SharedPrefixArgs)
 _pack_shared_prefix_args = _pack_shared_prefix_args.pack
 _attention_shared_prefix = ctypes.CFUNCTYPE(_I, ctypes.c_char_p, _P)(("qmk_attention_shared_prefix", _lib))
@@ -151,6 +151,8 @@ _lib.qmk_selftest_attention_wait_timeout.argtypes = [_I]
 _lib.qmk_selftest_attention_wait_timeout.restype = _I
 _lib.qmk_selftest_decode_attention_wait_timeout.argtypes = [_I, _I]
 _lib.qmk_selftest_decode_attention_wait_timeout.restype = _I
+_lib.qmk_selftest_shared_prefix_wait_timeout.argtypes = [_I]
+_lib.qmk_selftest_shared_prefix_wait_timeout.restype = _I
 _lib.qmk_selftest_gemm_pair_wait_timeout.argtypes = [_I, _I]
 _lib.qmk_selftest_gemm_pair_wait_timeout.restype = _I
 
@@ -158,7 +160,7 @@ EXPORTED_SYMBOLS = (
     "launch_ldg_decode_direct", "launch_ldg_decode_persistent", "launch_ldg_generate_nosync",
     "launch_ldg_prefill", "qmk_abi_version", "qmk_configure", "qmk_set_inv_freq", "qmk_set_logits_dump",
     "qmk_set_weight_format", "qmk_set_tuning", "qmk_set_tuning2", "qmk_set_profile_buffer", "qmk_set_fused", "qmk_set_step_overlap", "qmk_set_prefill_attention", "qmk_set_decode_attention", "qmk_invalidate_weights", "qmk_release_weights", "qmk_decode", "qmk_generate", "qmk_generate_static", "qmk_generate_batch", "qmk_gemm_f16_tn", "qmk_gemm_packed_tn", "qmk_sample_tokens", "qmk_attention_shared_prefix", "qmk_attention_shared_prefix_workspace", "qmk_sample_batched", "qmk_decode_batched", "qmk_prefill_chunked", "qmk_prefill_packed", "qmk_prefill_packed_passes", "qmk_prefill", "qmk_engine_create", "qmk_engine_destroy", "qmk_engine_apply", "qmk_engine_decode", "qmk_engine_generate", "qmk_engine_prefill", "qmk_sync_status", "qmk_last_error", "qmk_num_ctas",
-    "qmk_scratch_bytes", "qmk_selftest_decode_ring", "qmk_selftest_wait_timeout", "qmk_selftest_gemm_wait_timeout", "qmk_selftest_attention_wait_timeout", "qmk_selftest_gemm_pair_wait_timeout", "qmk_selftest_decode_attention_wait_timeout",
+    "qmk_scratch_bytes", "qmk_selftest_decode_ring", "qmk_selftest_wait_timeout", "qmk_selftest_gemm_wait_timeout", "qmk_selftest_attention_wait_timeout", "qmk_selftest_gemm_pair_wait_timeout", "qmk_selftest_decode_attention_wait_timeout", "qmk_selftest_shared_prefix_wait_timeout",
 )
 
 
@@ -789,7 +791,7 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     args = _pack_shared_prefix_args(code, n, q_heads, kv_heads, dim, q.data_ptr(), q_seq, q_head, k_prefix.data_ptr(), v_prefix.data_ptr(), prefix,
                                     prefix_strides[1], prefix_strides[0], k_ptrs, v_ptrs, k_base, v_base, own_seq, rows, own_row, own_head,
                                     own_lens.data_ptr(), 0, dim ** -0.5 if scale is None else scale, out.data_ptr(), lse.data_ptr(), workspace.data_ptr(),
-                                    need)
+                                    need, 0, 0)
     rc = _on_device(index, _attention_shared_prefix, args)
     if rc != 0:
         raise RuntimeError(f"{who}: {_lib.qmk_last_error().decode()} (status {rc})")
@@ -847,6 +849,12 @@ def selftest_decode_attention_wait_timeout(budget_us: int = 300, what: int = 1) 
     """The bounded waits of a decode step's attention: nothing loaded (1), or one chunk of cache rows that never comes (2); 4 is the
     designed answer."""
     return int(_lib.qmk_selftest_decode_attention_wait_timeout(int(budget_us), int(what)))
+
+
+def selftest_shared_prefix_wait_timeout(budget_us: int = 300) -> int:
+    """The same for the attention over a shared prefix on tcgen05."""
+    _require_cuda()
+    return int(_lib.qmk_selftest_shared_prefix_wait_timeout(int(budget_us)))
 
 
 def selftest_gemm_pair_wait_timeout(budget_us: int = 300, what: int = 1) -> int:

@@ -345,3 +345,43 @@ def test_many_queries_two_calls_at_once_and_in_graphs(gpu):
         torch.cuda.synchronize()
         for (o, l), w in zip((*results, got), (*want, want[0])):
             assert torch.equal(o, w[0]) and torch.equal(l, w[1])
+
+
+# ------------------------------------------------------------------------------------------------------------- waits that run out
+def test_a_negative_budget_of_the_waits_is_refused(C):
+    assert C._lib.qmk_attention_shared_prefix(ctypes.byref(args(C, timeout_ms=-1)), None) == 2 and b"timeout_ms" in C._lib.qmk_last_error()
+    for budget in (0, -5, 1000001):
+        assert C._lib.qmk_selftest_shared_prefix_wait_timeout(budget) == 2 and b"budget_us" in C._lib.qmk_last_error()
+
+
+@pytest.mark.gpu
+def test_waits_run_out_and_leave_the_device_usable(gpu):
+    """Score products that stop behind the second tile, with keys and values in flight: status 4 after the budget, NaN for the rows concerned,
+    copies landed and TMEM freed (the calls behind it allocate all of it), their results as before."""
+    case = inputs(90, 16, 8, 128, 2000, 99, [(31 * i) % 100 for i in range(90)], "fp16", seed=5)
+    want = gpu.attention_shared_prefix(*case)
+    check(want, *case)
+    for _ in range(3):
+        assert gpu.selftest_shared_prefix_wait_timeout(300) == 4
+        got = gpu.attention_shared_prefix(*case)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs,prefix", [(3, 200), (90, 2000)])
+def test_the_callers_status_word(gpu, seqs, prefix):
+    """A call whose waits end leaves the word as it is, on both ways through."""
+    case = inputs(seqs, 16, 8, 128, prefix, 40, [(7 * i) % 41 for i in range(seqs)], "fp16", seed=9)
+    q, kp, vp, ko, vo, lens = case
+    want = gpu.attention_shared_prefix(*case)
+    out, lse, word = torch.empty_like(q), torch.empty(seqs, 16, device="cuda"), torch.tensor([0, 7], dtype=torch.int32, device="cuda")
+    need = gpu._lib.qmk_attention_shared_prefix_workspace(seqs, 16, 8, 128, prefix, 40)
+    workspace = torch.empty(need, dtype=torch.uint8, device="cuda")
+    for i, budget in ((0, 0), (1, 500)):
+        a = gpu._SharedPrefixArgs(type=0, num_sequences=seqs, q_heads=16, kv_heads=8, head_dim=128, q=q.data_ptr(), q_seq_stride=2048, q_head_stride=128,
+                                  k_prefix=kp.data_ptr(), v_prefix=vp.data_ptr(), prefix_len=prefix, prefix_row_stride=128, prefix_head_stride=128 * prefix,
+                                  k_own_base=ko.data_ptr(), v_own_base=vo.data_ptr(), own_seq_stride=8 * 40 * 128, own_rows=40, own_row_stride=128,
+                                  own_head_stride=40 * 128, own_lens=lens.data_ptr(), scale=128 ** -0.5, out=out.data_ptr(), lse=lse.data_ptr(),
+                                  workspace=workspace.data_ptr(), workspace_bytes=need, status=word.data_ptr() + 4 * i, timeout_ms=budget)
+        assert gpu._lib.qmk_attention_shared_prefix(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1]) and word.tolist() == [0, 7]
