@@ -180,3 +180,45 @@ def test_null_pointers_are_refused(C):
         assert lib.qmk_sample_batched(1, None, None, 1, *[None] * 8, 0, *[None] * 9, 1, 64, 1.0, None) != 0 and b"null" in lib.qmk_last_error()
     else:
         assert lib.qmk_sample_batched(1, None, None, 1, *[None] * 8, 0, *[None] * 9, 1, 64, 1.0, None) != 0 and lib.qmk_last_error() == b"no CUDA device"
+
+
+def _past_the_borders(gpu, n, prefix, tails, L, steps, check):
+    """``n`` prompts of ``prefix`` tokens in common and ``tails[i]`` of their own: picks, logarithms and logits of the sequences ``check`` against the oracle;
+    captured steps, their replay and kernels one after the other give the same bits."""
+    w = S.make_weights(seed=39, num_layers=2, vocab_size=VOCAB, norm_std=0.1, max_seq_len=16)
+    system = S.make_prompt(prefix, seed=6, vocab_size=VOCAB)
+    prompts = [system + S.make_prompt(tails[i], seed=200 + i, vocab_size=VOCAB) if tails[i] else list(system) for i in range(n)]
+    uniforms = torch.rand(steps, n, generator=torch.Generator().manual_seed(prefix))
+    options = [[0.8] * n, [(0, 40)[i % 2] for i in range(n)], [0.95] * n, [0.0] * n]
+    eng = _engine(w, n, L, engine="gemm", prefill_mode="tensor")
+    kw = dict(uniforms=uniforms.cuda(), temperature=options[0], top_k=options[1], top_p=options[2], min_p=options[3])
+    tokens, logprobs, dump = _run(gpu, eng, prompts, steps, **kw)
+    _check(w, eng, prompts, steps, tokens, logprobs, dump, uniforms, options, L, which=check)
+    try:
+        for overlap in (True, True, False, True):
+            gpu.set_step_overlap(overlap)
+            again, again_lp = eng.sample_ids(prompts, steps, **kw)
+            assert again == tokens and again_lp == logprobs, overlap
+            assert torch.equal(_run(gpu, eng, prompts, steps, **kw)[2], dump), overlap
+    finally:
+        gpu.set_step_overlap(True)
+
+
+@pytest.mark.gpu
+def test_a_full_batch_of_answers_whose_prefix_is_on_tcgen05(gpu):
+    """256 query rows a kv head against 410 prefix rows: 107 M products, from 96 M on on tcgen05."""
+    assert 128 * 16 * 128 * 410 >= 96 << 20
+    _past_the_borders(gpu, 128, 411, [0] * 128, 512, 3, [0, 63, 64, 127])
+
+
+@pytest.mark.gpu
+def test_long_tails_behind_a_long_prefix(gpu):
+    """48 query rows a kv head against 2100 prefix rows on tcgen05, and up to three ranges of 256 rows of their own."""
+    assert 24 * 16 * 128 * 2100 >= 96 << 20
+    _past_the_borders(gpu, 24, 2100, [1 + (173 * i) % 700 for i in range(24)], 2816, 3, [0, 4, 11, 23])
+
+
+@pytest.mark.gpu
+def test_long_tails_behind_a_short_prefix(gpu):
+    """Prefix and several ranges of own rows in one grid (mma.sync): sequences start up to 600 rows behind the prefix."""
+    _past_the_borders(gpu, 9, 50, [1 + (307 * i) % 600 for i in range(9)], 768, 3, [0, 1, 7])
