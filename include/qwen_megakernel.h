@@ -205,7 +205,7 @@ int qmk_set_decode_attention(int tensor_core);
 /* Batched decode (qmk_decode_batched): 1 (default) launches the ~200 kernels of a decode step as programmatic
  * dependents of one another - each kernel is scheduled while its predecessor still runs, sets itself up, streams the
  * operands no kernel of the step writes (weight tiles, cache rows of earlier steps) and only then waits for the
- * predecessor to complete; 0 launches them strictly one after the other.  The same switch covers every
+ * predecessor to complete; 0 launches them strictly one after the other.  The same switch covers the steps of qmk_sample_batched and every
  * kernel behind the first of a chunk of qmk_prefill_chunked / qmk_prefill_packed and of qmk_prefill's chunked pass.  Same results either way; negative keeps. */
 int qmk_set_step_overlap(int enabled);
 
@@ -455,6 +455,7 @@ typedef struct qmk_shared_prefix_args {
   long long workspace_bytes;
   unsigned int *status;              /* DEVICE, may be null: where a bounded wait runs out, QMK_ERR_WAIT_TIMEOUT goes into it if it holds 0 */
   int timeout_ms;                    /* budget of those waits; 0: 2000 */
+  int no_overlap;                    /* 1: the call's kernels strictly one after the other, as qmk_set_step_overlap(0) has those of a step */
 } qmk_shared_prefix_args;
 int qmk_attention_shared_prefix(const qmk_shared_prefix_args *args, cudaStream_t stream);
 long long qmk_attention_shared_prefix_workspace(int num_sequences, int q_heads, int kv_heads, int head_dim, int prefix_len, int own_rows);

@@ -1515,6 +1515,7 @@ static int decode_batched(const char *who, const Sampling *sampling, int num_seq
         a.workspace_bytes = static_cast<long long>(w.shared_ws_bytes);
         a.status = w.status;
         a.timeout_ms = env.timeout_ms;
+        a.no_overlap = env.pdl == 0;
         if ((r2 = qmk_attention_shared_prefix(&a, s)) != QMK_OK) { err = qmk_last_error(); return r2; }
       } else if (env.attn_mma)
         PF_CUDA(qmk_tc::launch_kernel(decode_attention_mma<>, dim3(attn_ctas), dim3((DAM_WARPS + 1) * 32), DAM_SMEM_BYTES, s,

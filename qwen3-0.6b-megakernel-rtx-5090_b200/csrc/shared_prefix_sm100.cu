@@ -58,8 +58,14 @@ bool make_maps(CUtensorMap *maps, const Params &p, const Split &s, int head_dim,
          qmk_tc::make_map_tiled(maps + 2, bf16, 3, p.v_prefix, kv_dims, kv_strides, kv_box);
 }
 
+// The waits of prefix_parts_tc, and whether a kernel of the call may start early behind the one before it.
+struct Waits {
+  unsigned int *status;
+  unsigned long long budget_ns;
+  bool overlap;
+};
 template <typename T, int D, int NT>
-cudaError_t launch(Params &p, const Split &s, const CUtensorMap *maps, unsigned int *status, unsigned long long budget_ns, cudaStream_t stream) {
+cudaError_t launch(Params &p, const Split &s, const CUtensorMap *maps, const Waits &waits, cudaStream_t stream) {
   using Own = OwnRows<T, D, NT, own_warps(D)>;
   using Beside = OwnRows<T, D, NT, WARPS>;
   constexpr int own_smem = OWN_STAGES * 2 * Own::TILE, beside_smem = OWN_STAGES * 2 * Beside::TILE, smem = STAGES * 2 * KEYS * D * 2;
@@ -75,9 +81,9 @@ cudaError_t launch(Params &p, const Split &s, const CUtensorMap *maps, unsigned 
     if (e == cudaSuccess) e = cudaFuncSetAttribute(own_parts<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, own_smem);
     if (e == cudaSuccess)
       e = qmk_tc::launch_kernel(prefix_parts_tc<T, D>, dim3(prefix_items), dim3(TC_THREADS), tc_smem_bytes<D>(), stream, maps[0], maps[1], maps[2], p,
-                                s.seqs_per_tile, status, budget_ns);
-    dependent = true;                            // (of the launch before, inside this call)
-    const qmk_tc::PdlScope scope(true);
+                                s.seqs_per_tile, waits.status, waits.budget_ns);
+    dependent = waits.overlap;                   // (of the launch before, inside this call)
+    const qmk_tc::PdlScope scope(dependent);
     if (e == cudaSuccess && own_items > 0) e = qmk_tc::launch_kernel(own_parts<T, D, NT>, dim3(own_items), dim3(32 * own_warps(D)), own_smem, stream, p);
     if (e != cudaSuccess) return e;
   } else if (prefix_items + own_items > 0) {
@@ -85,15 +91,15 @@ cudaError_t launch(Params &p, const Split &s, const CUtensorMap *maps, unsigned 
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess) e = qmk_tc::launch_kernel(kernel, dim3(prefix_items + own_items), dim3(THREADS), prefix_items > 0 ? smem : beside_smem, stream, p);
     if (e != cudaSuccess) return e;
-    dependent = true;
+    dependent = waits.overlap;
   }
   const qmk_tc::PdlScope scope(dependent);
   return qmk_tc::launch_kernel(join_parts<T, D>, dim3(p.seqs * p.q_heads), dim3(128), 0, stream, p);
 }
 template <typename T>
-cudaError_t launch(Params &p, const Split &s, int head_dim, const CUtensorMap *maps, unsigned int *status, unsigned long long budget_ns, cudaStream_t stream) {
-  if (p.group > 8) return head_dim == 64 ? launch<T, 64, 2>(p, s, maps, status, budget_ns, stream) : launch<T, 128, 2>(p, s, maps, status, budget_ns, stream);
-  return head_dim == 64 ? launch<T, 64, 1>(p, s, maps, status, budget_ns, stream) : launch<T, 128, 1>(p, s, maps, status, budget_ns, stream);
+cudaError_t launch(Params &p, const Split &s, int head_dim, const CUtensorMap *maps, const Waits &waits, cudaStream_t stream) {
+  if (p.group > 8) return head_dim == 64 ? launch<T, 64, 2>(p, s, maps, waits, stream) : launch<T, 128, 2>(p, s, maps, waits, stream);
+  return head_dim == 64 ? launch<T, 64, 1>(p, s, maps, waits, stream) : launch<T, 128, 1>(p, s, maps, waits, stream);
 }
 
 }  // namespace
@@ -166,12 +172,11 @@ extern "C" int qmk_attention_shared_prefix(const qmk_shared_prefix_args *a, cuda
   const long long states = static_cast<long long>(s.prefix_parts + s.own_parts) * p.seqs * p.q_heads;
   p.part_out = static_cast<float *>(a->workspace);
   p.part_ml = reinterpret_cast<float2 *>(p.part_out + states * a->head_dim);
-  unsigned int *const status = a->status ? a->status : reinterpret_cast<unsigned int *>(p.part_ml + states);      // (in the workspace for nobody)
-  const unsigned long long budget_ns = (a->timeout_ms ? a->timeout_ms : 2000) * 1000000ull;
+  const Waits waits = {a->status ? a->status : reinterpret_cast<unsigned int *>(p.part_ml + states),      // (in the workspace: for nobody)
+                       (a->timeout_ms ? a->timeout_ms : 2000) * 1000000ull, a->no_overlap == 0};
   p.out = a->out;
   p.lse = a->lse;
-  const cudaError_t e = a->type == 0 ? launch<__half>(p, s, a->head_dim, maps, status, budget_ns, stream)
-                                     : launch<__nv_bfloat16>(p, s, a->head_dim, maps, status, budget_ns, stream);
+  const cudaError_t e = a->type == 0 ? launch<__half>(p, s, a->head_dim, maps, waits, stream) : launch<__nv_bfloat16>(p, s, a->head_dim, maps, waits, stream);
   if (e != cudaSuccess) {
     cudaGetLastError();
     qmk_internal::note_error(std::string("qmk_attention_shared_prefix: ") + cudaGetErrorString(e));

@@ -104,13 +104,13 @@ class _SharedPrefixArgs(ctypes.Structure):
                 ("k_prefix", _P), ("v_prefix", _P), ("prefix_len", _I), ("prefix_row_stride", _LL), ("prefix_head_stride", _LL),
                 ("k_own", _P), ("v_own", _P), ("k_own_base", _P), ("v_own_base", _P), ("own_seq_stride", _LL), ("own_rows", _I), ("own_row_stride", _LL), ("own_head_stride", _LL),
                 ("own_lens", _P), ("own_lens_add", _I), ("scale", _F), ("out", _P), ("lse", _P), ("workspace", _P),
-                ("workspace_bytes", _LL), ("status", _P), ("timeout_ms", _I)]
+                ("workspace_bytes", _LL), ("status", _P), ("timeout_ms", _I), ("no_overlap", _I)]
 
 
 _lib.qmk_attention_shared_prefix.argtypes = [ctypes.POINTER(_SharedPrefixArgs), _P]
 _lib.qmk_attention_shared_prefix.restype = _I
 # The same as bytes, which take a fifth of the time to fill (1.3 us)
-_pack_shared_prefix_args = struct.Struct("@5i P2q 2Pi2q 4Pqi2q P if 3Pq Pi0q")
+_pack_shared_prefix_args = struct.Struct("@5i P2q 2Pi2q 4Pqi2q P if 3Pq P2i")
 assert _pack_shared_prefix_args.size == ctypes.sizeof(_SharedPrefixArgs)
 _pack_shared_prefix_args = _pack_shared_prefix_args.pack
 _attention_shared_prefix = ctypes.CFUNCTYPE(_I, ctypes.c_char_p, _P)(("qmk_attention_shared_prefix", _lib))
@@ -791,7 +791,7 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     args = _pack_shared_prefix_args(code, n, q_heads, kv_heads, dim, q.data_ptr(), q_seq, q_head, k_prefix.data_ptr(), v_prefix.data_ptr(), prefix,
                                     prefix_strides[1], prefix_strides[0], k_ptrs, v_ptrs, k_base, v_base, own_seq, rows, own_row, own_head,
                                     own_lens.data_ptr(), 0, dim ** -0.5 if scale is None else scale, out.data_ptr(), lse.data_ptr(), workspace.data_ptr(),
-                                    need, 0, 0)
+                                    need, 0, 0, 0)
     rc = _on_device(index, _attention_shared_prefix, args)
     if rc != 0:
         raise RuntimeError(f"{who}: {_lib.qmk_last_error().decode()} (status {rc})")

@@ -385,3 +385,34 @@ def test_the_callers_status_word(gpu, seqs, prefix):
                                   workspace=workspace.data_ptr(), workspace_bytes=need, status=word.data_ptr() + 4 * i, timeout_ms=budget)
         assert gpu._lib.qmk_attention_shared_prefix(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == 0
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1]) and word.tolist() == [0, 7]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs,prefix,kernels", [(3, 200, 2), (90, 2000, 3)])
+def test_kernels_of_a_call_one_after_the_other(gpu, seqs, prefix, kernels):
+    """``no_overlap``: no edge between the call's kernels is a programmatic one, which all of them are without it; the same bits."""
+    class Edge(ctypes.Structure):                                # cudaGraphEdgeData; type 1: programmatic
+        _fields_ = [("from_port", ctypes.c_ubyte), ("to_port", ctypes.c_ubyte), ("type", ctypes.c_ubyte), ("reserved", ctypes.c_ubyte * 5)]
+    runtime = ctypes.CDLL("libcudart.so.12")
+    q, kp, vp, ko, vo, lens = case = inputs(seqs, 16, 8, 128, prefix, 40, [(7 * i) % 41 for i in range(seqs)], "fp16", seed=9)
+    want = gpu.attention_shared_prefix(*case)
+    out, lse = torch.empty_like(q), torch.empty(seqs, 16, device="cuda")
+    need = gpu._lib.qmk_attention_shared_prefix_workspace(seqs, 16, 8, 128, prefix, 40)
+    workspace = torch.empty(need, dtype=torch.uint8, device="cuda")
+    a = gpu._SharedPrefixArgs(type=0, num_sequences=seqs, q_heads=16, kv_heads=8, head_dim=128, q=q.data_ptr(), q_seq_stride=2048, q_head_stride=128,
+                              k_prefix=kp.data_ptr(), v_prefix=vp.data_ptr(), prefix_len=prefix, prefix_row_stride=128, prefix_head_stride=128 * prefix,
+                              k_own_base=ko.data_ptr(), v_own_base=vo.data_ptr(), own_seq_stride=8 * 40 * 128, own_rows=40, own_row_stride=128,
+                              own_head_stride=40 * 128, own_lens=lens.data_ptr(), scale=128 ** -0.5, out=out.data_ptr(), lse=lse.data_ptr(),
+                              workspace=workspace.data_ptr(), workspace_bytes=need)
+    for serial in (0, 1):
+        a.no_overlap = serial
+        graph = torch.cuda.CUDAGraph(keep_graph=True)
+        with torch.cuda.graph(graph):
+            assert gpu._lib.qmk_attention_shared_prefix(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+        nodes, edges, count = ((ctypes.c_void_p * 8)() for _ in range(2)), (Edge * 8)(), ctypes.c_size_t(8)
+        assert runtime.cudaGraphGetEdges_v2(ctypes.c_void_p(graph.raw_cuda_graph()), *nodes, edges, ctypes.byref(count)) == 0
+        assert [e.type for e in edges[:count.value]] == [0 if serial else 1] * (kernels - 1)
+        graph.instantiate()
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
