@@ -416,3 +416,59 @@ def test_kernels_of_a_call_one_after_the_other(gpu, seqs, prefix, kernels):
         out.zero_()
         graph.replay()
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+# ------------------------------------------------------------------------------------------------------------- visible rows whose scores are no numbers
+def _hidden_by_scores(seqs, prefix, own, dtype, seed):
+    """Inputs some of whose rows have scores of -inf with every query, and the same without these rows."""
+    q, kp, vp, ko, vo, lens = inputs(seqs, 16, 8, 128, prefix, own, [(11 * i) % (own + 1) for i in range(seqs)], dtype, seed=seed)
+    q[..., 5] = q[..., 5].abs() + 0.5
+    g = torch.Generator().manual_seed(seed)
+    out_prefix = torch.rand(prefix, generator=g) < 0.3
+    out_prefix[:min(prefix, 300)] = True                         # whole tiles at the beginning
+    out_own = torch.rand(seqs, own, generator=g) < 0.3
+    out_own[0] = True
+    out_own[1::3, :16] = True
+    kp[:, out_prefix.cuda(), 5] = -math.inf
+    ko.transpose(1, 2)[out_own.cuda()] = ko.transpose(1, 2)[out_own.cuda()].index_fill(2, torch.tensor([5], device="cuda"), -math.inf)
+    keep = (~out_prefix).cuda()
+    rows = [[j for j in range(int(lens[b])) if not out_own[b, j]] for b in range(seqs)]
+    fewer = (q, kp[:, keep], vp[:, keep], [ko[b][:, r] for b, r in enumerate(rows)], [vo[b][:, r] for b, r in enumerate(rows)], [len(r) for r in rows])
+    return (q, kp, vp, ko, vo, lens), fewer
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("seqs,prefix,own", [(3, 0, 40), (3, 130, 40), (5, 700, 300), (20, 700, 40), (100, 600, 40), (100, 300, 300), (100, 620, 20)])
+def test_rows_whose_scores_are_minus_infinity_weigh_nothing(gpu, dtype, seqs, prefix, own):
+    """As a mask inside the keys has it: single rows, whole tiles and ranges, all rows of a sequence (zeros and -inf, as without rows)."""
+    case, fewer = _hidden_by_scores(seqs, prefix, own, dtype, seqs + prefix + own)
+    got = gpu.attention_shared_prefix(*case)
+    check(got, *fewer)
+    if prefix <= 300:
+        assert bool((got[0][0] == 0).all()) and bool((got[1][0] == -math.inf).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("seqs,prefix", [(3, 130), (20, 700), (100, 600)])
+def test_a_score_that_is_no_number_makes_its_head_none(gpu, bad, seqs, prefix):
+    """A NaN or +inf score of a visible row: NaN for the heads and sequences that see it, the bits of the others as without it."""
+    q, kp, vp, ko, vo, lens = inputs(seqs, 16, 8, 128, prefix, 40, [40] * seqs, "fp16", seed=3)
+    q[..., 5] = q[..., 5].abs() + 0.5
+    want = gpu.attention_shared_prefix(q, kp, vp, ko, vo, lens)
+    own = ko.clone()
+    own[1, 3, 17, 5] = bad                                       # kv head 3 of sequence 1 alone: query heads 6 and 7
+    out, lse = gpu.attention_shared_prefix(q, kp, vp, own, vo, lens)
+    assert bool(out[1, 6:8].isnan().all()) and not bool(lse[1, 6:8].isfinite().any())
+    rest = torch.ones(seqs, 16, dtype=torch.bool, device="cuda")
+    rest[1, 6:8] = False
+    assert torch.equal(out[rest], want[0][rest]) and torch.equal(lse[rest], want[1][rest])
+    for rows in ([prefix // 2], list(range(prefix))):            # one shared row of kv head 2, and all of them
+        k = kp.clone()
+        k[2, rows, 5] = bad
+        out, lse = gpu.attention_shared_prefix(q, k, vp, ko, vo, lens)
+        assert bool(out[:, 4:6].isnan().all()) and not bool(lse[:, 4:6].isfinite().any())
+        rest = torch.ones(16, dtype=torch.bool, device="cuda")
+        rest[4:6] = False
+        assert torch.equal(out[:, rest], want[0][:, rest]) and torch.equal(lse[:, rest], want[1][:, rest])
