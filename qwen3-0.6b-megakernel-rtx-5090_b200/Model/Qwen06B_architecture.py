@@ -630,6 +630,10 @@ class BatchDecoder:
             uniforms = torch.rand(steps, n, device=dev, generator=generator)
         elif tuple(uniforms.shape) != (steps, n):
             raise ValueError(f"uniforms must be [{steps}, {n}]")
+        elif uniforms.device != dev:
+            raise RuntimeError(f"uniforms must be on {dev}")
+        uniforms = uniforms.contiguous()
+        options = _require_megakernel_op("check_sampling")(n, steps, uniforms, *options)       # (before any slot changes)
         self.prefill_many([0] if once else list(range(n)), heads[:1] if once else heads)
         if once:
             self.positions[1:n] = [0] * (n - 1)
@@ -641,7 +645,7 @@ class BatchDecoder:
         _require_megakernel_op("sample_batched")(
             [ids[-1] for ids in prompts], [len(ids) for ids in heads], steps, base._embed_weight, base._layer_weights_packed, base._final_norm_weight,
             base._lm_head_weight, base._cos_table, base._sin_table, self._k_caches[0], self._v_caches[0], shared, self._k_caches[:n], self._v_caches[:n],
-            uniforms.contiguous(), *options, [self._logs[b][:steps] for b in range(n)], list(logprobs.unbind(0)), base.num_layers, self.max_seq_len,
+            uniforms, *options, [self._logs[b][:steps] for b in range(n)], list(logprobs.unbind(0)), base.num_layers, self.max_seq_len,
             base._attn_scale)
         eos = base._eos()
         outs, scores = [], []

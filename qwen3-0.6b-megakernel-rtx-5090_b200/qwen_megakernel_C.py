@@ -531,6 +531,17 @@ def decode_batched(first_token_ids, start_positions, num_steps, embed_weight, la
     return output_logs
 
 
+def check_sampling(n, num_steps, uniforms, temperatures, top_ks, top_ps, min_ps):
+    """Raises ``RuntimeError`` where ``sample_batched`` would refuse these options of ``n`` sequences; they as numbers of its types."""
+    _check(all(len(v) == n for v in (temperatures, top_ks, top_ps, min_ps)), "sample_batched: per-sequence lists differ in length")
+    _check(uniforms.dtype == torch.float32 and uniforms.is_cuda and uniforms.is_contiguous() and tuple(uniforms.shape) == (num_steps, n),
+           f"sample_batched: uniforms must be a contiguous fp32 CUDA tensor [{num_steps}, {n}]")
+    temperatures, top_ps, min_ps = ([ctypes.c_float(float(v)).value for v in values] for values in (temperatures, top_ps, min_ps))
+    _check(all(t >= 0 for t in temperatures) and all(p > 0 for p in top_ps) and all(0 <= m <= 1 for m in min_ps),
+           "sample_batched: temperature below 0, top_p not above 0 or min_p outside [0, 1]")
+    return temperatures, [min(max(int(v), 0), _INT_MAX) for v in top_ks], top_ps, min_ps
+
+
 def sample_batched(first_token_ids, start_positions, num_steps, embed_weight, layer_weights_packed, final_norm_weight, lm_head_weight, cos_table,
                    sin_table, k_prefix, v_prefix, prefix_len, k_caches, v_caches, uniforms, temperatures, top_ks, top_ps, min_ps, output_logs,
                    logprob_logs, num_layers, max_seq_len, attn_scale):
@@ -541,22 +552,19 @@ def sample_batched(first_token_ids, start_positions, num_steps, embed_weight, la
     _require_cuda()
     n, num_steps = len(first_token_ids), int(num_steps)
     _check(1 <= n <= MAX_GEMM_BATCH_SEQUENCES, "sample_batched: 1 to 128 sequences per call")
-    _check(all(len(v) == n for v in (start_positions, k_caches, v_caches, temperatures, top_ks, top_ps, min_ps, output_logs, logprob_logs)),
-           "sample_batched: per-sequence lists differ in length")
+    _check(all(len(v) == n for v in (start_positions, k_caches, v_caches, output_logs, logprob_logs)), "sample_batched: per-sequence lists differ in length")
     for logs, dtype in ((output_logs, torch.int32), (logprob_logs, torch.float32)):
         for log in logs:
             _check(log.dtype == dtype and log.is_cuda and log.is_contiguous() and log.numel() >= num_steps,
                    f"sample_batched: each log must be a contiguous {dtype} CUDA tensor of >= num_steps entries")
-    _check(uniforms.dtype == torch.float32 and uniforms.is_cuda and uniforms.is_contiguous() and tuple(uniforms.shape) == (num_steps, n),
-           f"sample_batched: uniforms must be a contiguous fp32 CUDA tensor [{num_steps}, {n}]")
+    temperatures, top_ks, top_ps, min_ps = check_sampling(n, num_steps, uniforms, temperatures, top_ks, top_ps, min_ps)
     _check_table(layer_weights_packed, "sample_batched")
     ints, floats, ptrs = ctypes.c_int * n, ctypes.c_float * n, ctypes.c_void_p * n
     rc = _lib.qmk_sample_batched(
         n, ints(*[int(t) for t in first_token_ids]), ints(*[int(p) for p in start_positions]), num_steps,
         _ptr(embed_weight), _ptr(layer_weights_packed), _ptr(final_norm_weight), _ptr(lm_head_weight), _ptr(cos_table), _ptr(sin_table),
         _ptr(k_prefix), _ptr(v_prefix), int(prefix_len), ptrs(*[_ptr(t) for t in k_caches]), ptrs(*[_ptr(t) for t in v_caches]),
-        _ptr(uniforms), floats(*[float(v) for v in temperatures]), ints(*[min(max(int(v), 0), _INT_MAX) for v in top_ks]), floats(*[float(v) for v in top_ps]),
-        floats(*[float(v) for v in min_ps]), ptrs(*[_ptr(t) for t in output_logs]), ptrs(*[_ptr(t) for t in logprob_logs]),
+        _ptr(uniforms), floats(*temperatures), ints(*top_ks), floats(*top_ps), floats(*min_ps), ptrs(*[_ptr(t) for t in output_logs]), ptrs(*[_ptr(t) for t in logprob_logs]),
         int(num_layers), int(max_seq_len), float(attn_scale), _stream())
     if rc != 0:
         raise RuntimeError(f"sample_batched: {_lib.qmk_last_error().decode()} (status {rc})")

@@ -222,3 +222,26 @@ def test_long_tails_behind_a_long_prefix(gpu):
 def test_long_tails_behind_a_short_prefix(gpu):
     """Prefix and several ranges of own rows in one grid (mma.sync): sequences start up to 600 rows behind the prefix."""
     _past_the_borders(gpu, 9, 50, [1 + (307 * i) % 600 for i in range(9)], 768, 3, [0, 1, 7])
+
+
+@pytest.mark.gpu
+def test_refused_options_leave_the_slots_as_they_were(gpu):
+    """What ``sample_ids`` refuses it refuses before it fills a slot: positions and caches go on as if the call had not been made."""
+    w = S.make_weights(seed=37, num_layers=2, vocab_size=VOCAB, norm_std=0.1, max_seq_len=16)
+    prompts = [S.make_prompt(20 + 9 * i, seed=90 + i, vocab_size=VOCAB) for i in range(3)]
+    eng = _engine(w, 3, 128, engine="gemm", prefill_mode="tensor")
+    first = [ids[-1] for ids in eng.generate_ids(prompts, 4)]
+    positions, rows = list(eng.positions), [(k.clone(), v.clone()) for k, v in zip(eng._k_caches, eng._v_caches)]
+    other = [S.make_prompt(33, seed=99, vocab_size=VOCAB)]
+    good = torch.rand(4, 2, device="cuda")
+    for bad in (dict(temperature=-1.0), dict(temperature=float("nan")), dict(top_p=0.0), dict(top_p=1e-60), dict(top_p=[1.0, float("nan")]), dict(min_p=2.0),
+                dict(min_p=-0.1), dict(uniforms=good.cpu()), dict(uniforms=good.double()), dict(uniforms=good.half()), dict(uniforms=good[:3]), dict(top_k=[1]),
+                dict(temperature="warm"), dict(top_k=float("nan"))):
+        for prompts_ in (other * 2, [other[0], other[0][:-3]]):
+            with pytest.raises((RuntimeError, ValueError)):
+                eng.sample_ids(prompts_, 4, **bad)
+        assert eng.positions == positions
+        assert all(torch.equal(k, a) and torch.equal(v, b) for k, v, (a, b) in zip(eng._k_caches, eng._v_caches, rows)), bad
+    more = eng.decode_slots([0, 1, 2], first, 3)
+    again = _engine(w, 3, 128, engine="gemm", prefill_mode="tensor")
+    assert [ids[4:] for ids in again.generate_ids(prompts, 7)] == more
