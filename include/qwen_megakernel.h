@@ -458,6 +458,7 @@ typedef struct qmk_shared_prefix_args {
   int no_overlap;                    /* 1: the call's kernels strictly one after the other, as qmk_set_step_overlap(0) has those of a step */
 } qmk_shared_prefix_args;
 int qmk_attention_shared_prefix(const qmk_shared_prefix_args *args, cudaStream_t stream);
+/* Bytes; 0 for sizes that the call refuses. */
 long long qmk_attention_shared_prefix_workspace(int num_sequences, int q_heads, int kv_heads, int head_dim, int prefix_len, int own_rows);
 
 /* qmk_decode_batched with sampled picks and a shared prefix: many answers to one prompt, or many prompts behind one system prompt.  Every

@@ -13,9 +13,21 @@ namespace {
 
 using namespace qmk_spa;
 
+constexpr int MAX_ROWS = 1 << 24;                // of a prefix or an own cache
+
 int refuse(const std::string &why) {
   qmk_internal::note_error("qmk_attention_shared_prefix: " + why);
   return QMK_ERR_BAD_ARGUMENT;
+}
+
+// What is wrong with sizes; null: nothing
+const char *refused_heads(int q_heads, int kv_heads, int head_dim) {
+  if (head_dim != 64 && head_dim != 128) return "head_dim must be 64 or 128";
+  if (kv_heads < 1 || q_heads < 1 || q_heads % kv_heads || q_heads / kv_heads > MAX_GROUP || q_heads > 1024) return "q_heads must be 1 to 16 times kv_heads, and at most 1024";
+  return nullptr;
+}
+const char *refused_lengths(int prefix_len, int own_rows) {
+  return prefix_len < 0 || own_rows < 0 || prefix_len > MAX_ROWS || own_rows > MAX_ROWS ? "a length is negative or above 2^24" : nullptr;
 }
 
 // How a call is cut into items.  More than 32 rows of queries against a kv head and 96 M products (rows x prefix rows x kv heads x dims) go through
@@ -26,7 +38,7 @@ struct Split {
   bool tc;
   int row_warps, row_tiles, seqs_per_tile, prefix_parts, prefix_range, own_parts, own_range;
 };
-constexpr int SMS = 148, MAX_ROWS = 1 << 24;
+constexpr int SMS = 148;
 constexpr long long TC_PRODUCTS = 96 << 20;
 Split split_of(int seqs, int q_heads, int kv_heads, int head_dim, int prefix_len, int own_rows, bool tc) {
   Split s;
@@ -106,8 +118,7 @@ cudaError_t launch(Params &p, const Split &s, int head_dim, const CUtensorMap *m
 
 extern "C" long long qmk_attention_shared_prefix_workspace(int num_sequences, int q_heads, int kv_heads, int head_dim, int prefix_len,
                                                            int own_rows) {
-  if (num_sequences < 1 || num_sequences > MAX_SEQS || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || prefix_len < 0 || own_rows < 0)
-    return 0;
+  if (num_sequences < 1 || num_sequences > MAX_SEQS || refused_heads(q_heads, kv_heads, head_dim) || refused_lengths(prefix_len, own_rows)) return 0;
   return std::max(workspace_bytes(split_of(num_sequences, q_heads, kv_heads, head_dim, prefix_len, own_rows, true), num_sequences, q_heads, head_dim),
                   workspace_bytes(split_of(num_sequences, q_heads, kv_heads, head_dim, prefix_len, own_rows, false), num_sequences, q_heads, head_dim));
 }
@@ -117,10 +128,8 @@ extern "C" int qmk_attention_shared_prefix(const qmk_shared_prefix_args *a, cuda
   if (!a) return refuse("null pointer argument");
   if (a->num_sequences < 1 || a->num_sequences > MAX_SEQS) return refuse("num_sequences must be in [1, 128]");
   if (a->type < 0 || a->type > 1) return refuse("the type is fp16 (0) or bf16 (1)");
-  if (a->head_dim != 64 && a->head_dim != 128) return refuse("head_dim must be 64 or 128");
-  if (a->kv_heads < 1 || a->q_heads < 1 || a->q_heads % a->kv_heads || a->q_heads / a->kv_heads > MAX_GROUP || a->q_heads > 1024)
-    return refuse("q_heads must be 1 to 16 times kv_heads, and at most 1024");
-  if (a->prefix_len < 0 || a->own_rows < 0 || a->prefix_len > MAX_ROWS || a->own_rows > MAX_ROWS) return refuse("a length is negative or above 2^24");
+  if (const char *why = refused_heads(a->q_heads, a->kv_heads, a->head_dim)) return refuse(why);
+  if (const char *why = refused_lengths(a->prefix_len, a->own_rows)) return refuse(why);
   if (!a->q || !a->out || (a->prefix_len > 0 && (!a->k_prefix || !a->v_prefix)) || (a->own_rows > 0 && (a->k_own ? !a->v_own : !a->k_own_base || !a->v_own_base)) || (a->own_rows > 0 && !a->own_lens))
     return refuse("null pointer argument");
   if (!(a->scale > -2.0e38f && a->scale < 2.0e38f)) return refuse("the scale must be finite, and below 2e38");   // (times log2 e too)

@@ -472,3 +472,31 @@ def test_a_score_that_is_no_number_makes_its_head_none(gpu, bad, seqs, prefix):
         rest = torch.ones(16, dtype=torch.bool, device="cuda")
         rest[4:6] = False
         assert torch.equal(out[:, rest], want[0][:, rest]) and torch.equal(lse[:, rest], want[1][:, rest])
+
+
+# ------------------------------------------------------------------------------------------------------------- more refusals
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", range(1, 6))
+@pytest.mark.parametrize("lists", [False, True])
+def test_a_tensor_of_the_host_is_refused(gpu, which, lists):
+    """Each of the caches and lengths in turn, own caches as one tensor or a list: no address of the host's memory reaches a kernel."""
+    case = list(inputs(2, 4, 2, 64, 8, 8, [1, 2], "fp16"))
+    case[which] = case[which].cpu()
+    if lists:
+        case[3], case[4] = list(case[3]), list(case[4])
+    with pytest.raises(RuntimeError):
+        gpu.attention_shared_prefix(*case)
+
+
+@pytest.mark.parametrize("sizes", [(128, 1 << 30, 1 << 30, 128, 100, 10), (128, 2 ** 31 - 1, 1, 128, 100, 10), (1, 16, 8, 128, 2 ** 31 - 1, 10), (1, 16, 8, 128, 10, 2 ** 31 - 1),
+                                   (1, 16, 8, 128, (1 << 24) + 1, 0), (1, 16, 8, 96, 10, 10), (1, 16, 8, 0, 10, 10), (0, 16, 8, 128, 10, 10), (129, 16, 8, 128, 10, 10),
+                                   (1, 17, 1, 128, 10, 10), (1, 12, 8, 128, 10, 10), (1, 0, 0, 128, 10, 10), (1, 16, 8, 128, -1, 10)])
+def test_no_workspace_for_sizes_that_are_refused(C, sizes):
+    """... nor sums that leave 32 bits on the way to it."""
+    assert C._lib.qmk_attention_shared_prefix_workspace(*sizes) == 0
+
+
+def test_workspace_of_the_largest_sizes(C):
+    """128 sequences of 1024 query heads of 128 dims, prefix and own caches of 2^24 rows: a state of 130 floats for each, in at most 17 parts a head."""
+    need = C._lib.qmk_attention_shared_prefix_workspace(128, 1024, 64, 128, 1 << 24, 1 << 24)
+    assert 17 * 128 * 1024 * 130 * 4 <= need <= 17 * 128 * 1024 * 130 * 4 + 16
