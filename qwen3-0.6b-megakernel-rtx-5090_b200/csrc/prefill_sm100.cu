@@ -1351,6 +1351,9 @@ static int decode_batched(const char *who, const Sampling *sampling, int num_seq
       if (start_positions[b] < sampling->prefix_len)
         return qmk_internal::report(QMK_ERR_POSITION, std::string(who) + ": a sequence starts inside the shared prefix");
       if (!sampling->logprob_logs[b]) return qmk_internal::report(QMK_ERR_BAD_ARGUMENT, std::string(who) + ": null cache or log pointer");
+      for (int a = 0; a < b; ++a)
+        if (sampling->logprob_logs[a] == sampling->logprob_logs[b])
+          return qmk_internal::report(QMK_ERR_BAD_ARGUMENT, std::string(who) + ": two sequences share a log of logarithms");
       if (!(sampling->temperatures[b] >= 0.f) || !(sampling->top_ps[b] > 0.f) || !(sampling->min_ps[b] >= 0.f && sampling->min_ps[b] <= 1.f))
         return qmk_internal::report(QMK_ERR_BAD_ARGUMENT, std::string(who) + ": temperature below 0, top_p not above 0 or min_p outside [0, 1]");
     }

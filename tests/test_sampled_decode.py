@@ -245,3 +245,19 @@ def test_refused_options_leave_the_slots_as_they_were(gpu):
     more = eng.decode_slots([0, 1, 2], first, 3)
     again = _engine(w, 3, 128, engine="gemm", prefill_mode="tensor")
     assert [ids[4:] for ids in again.generate_ids(prompts, 7)] == more
+
+
+@pytest.mark.gpu
+def test_two_sequences_with_one_log_of_logarithms_are_refused(gpu):
+    eng = _engine(S.make_weights(seed=37, num_layers=2, vocab_size=VOCAB, norm_std=0.1, max_seq_len=16), 2, 64)
+    base = eng._base
+    base.apply_options()
+    logs, scores = [torch.zeros(4, dtype=torch.int32, device="cuda") for _ in range(2)], [torch.zeros(4, device="cuda") for _ in range(2)]
+
+    def call(scores):
+        gpu.sample_batched([1, 2], [8, 9], 4, base._embed_weight, base._layer_weights_packed, base._final_norm_weight, base._lm_head_weight, base._cos_table,
+                           base._sin_table, None, None, 0, eng._k_caches, eng._v_caches, torch.rand(4, 2, device="cuda"), [1.0, 1.0], [0, 0], [1.0, 1.0],
+                           [0.0, 0.0], logs, scores, base.num_layers, 64, base._attn_scale)
+    with pytest.raises(RuntimeError, match="share"):
+        call([scores[0]] * 2)
+    call(scores)
