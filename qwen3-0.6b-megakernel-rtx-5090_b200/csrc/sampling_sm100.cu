@@ -26,6 +26,7 @@ extern "C" int qmk_sample_tokens(const void *logits, int logits_type, long long 
   if (vocab < 1 || vocab > MAX_VOCAB) return refuse("the vocabulary must be in [1, 262144]");
   if (logits_type < 0 || logits_type > 2) return refuse("logits are fp32 (0), fp16 (1) or bf16 (2)");
   if (!logits || !uniforms || !tokens) return refuse("null pointer argument");
+  if (reinterpret_cast<unsigned long long>(logits) % (logits_type == 0 ? 4 : 2)) return refuse("the logits' address must be aligned to their size");
   if (rows > 1 && row_stride < vocab && row_stride != 0) return refuse("rows overlap: the row stride is below the vocabulary");
   if (!temperatures && !(temperature >= 0.0f)) return refuse("the temperature must not be negative");
   if (!top_ps && !(top_p > 0.0f)) return refuse("top_p must be above 0");

@@ -384,3 +384,10 @@ def test_what_arrays_of_options_may_hold(gpu, vocab):
             assert int(got[i]) == token, (i, g)
             assert abs(float(logp[i]) - lp) <= abs(lp) * 2.0 ** -24 + 2.0 ** -28, (i, g)
     assert borders <= 1
+
+
+@pytest.mark.parametrize("address,kind,refused", [(4097, 0, True), (4098, 0, True), (4099, 1, True), (4097, 2, True), (4098, 1, False), (4098, 2, False), (4100, 0, False)])
+def test_logits_between_addresses_of_their_type_are_refused(C, address, kind, refused):
+    """(A stride below the vocabulary is refused behind it, so that nothing runs.)"""
+    rc = C._lib.qmk_sample_tokens(address, kind, 99, 2, 100, 4096, None, 1.0, None, 0, None, 1.0, None, 0.0, 4096, None, None)
+    assert rc == 2 and (b"aligned" if refused else b"overlap") in C._lib.qmk_last_error()
