@@ -633,7 +633,12 @@ class BatchDecoder:
         elif uniforms.device != dev:
             raise RuntimeError(f"uniforms must be on {dev}")
         uniforms = uniforms.contiguous()
-        options = _require_megakernel_op("check_sampling")(n, steps, uniforms, *options)       # (before any slot changes)
+        if steps:                                                # (what the steps would refuse, before any slot changes)
+            options = _require_megakernel_op("check_sampling")(n, steps, uniforms, *options)
+            if base.vocab_size % 128:
+                raise RuntimeError("sample_ids needs a vocabulary that is a multiple of 128")
+            if any(not 0 <= ids[-1] < base.vocab_size for ids in prompts):
+                raise RuntimeError("first token outside [0, vocab)")
         self.prefill_many([0] if once else list(range(n)), heads[:1] if once else heads)
         if once:
             self.positions[1:n] = [0] * (n - 1)

@@ -261,3 +261,20 @@ def test_two_sequences_with_one_log_of_logarithms_are_refused(gpu):
     with pytest.raises(RuntimeError, match="share"):
         call([scores[0]] * 2)
     call(scores)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("engine,vocab,last", [("gemm", VOCAB, VOCAB), ("gemm", VOCAB, -1), ("persistent", VOCAB, VOCAB + 5), ("persistent", 1000, 3)])
+def test_refused_tokens_and_vocabularies_leave_the_slots_as_they_were(gpu, engine, vocab, last):
+    """A last token outside the vocabulary, and an engine whose vocabulary the sampled steps do not read."""
+    from Model.Qwen06B_architecture import BatchDecoder
+    w = S.make_weights(seed=37, num_layers=2, vocab_size=vocab, norm_std=0.1, max_seq_len=16)
+    eng = BatchDecoder(weights=S.weights_to(w, "cuda"), tokenizer=S.StubTokenizer(-1, vocab), num_sequences=2, max_seq_len=128, engine=engine)
+    prompts = [S.make_prompt(20 + 9 * i, seed=90 + i, vocab_size=vocab) for i in range(2)]
+    eng.generate_ids(prompts, 4)
+    positions, rows = list(eng.positions), [(k.clone(), v.clone()) for k, v in zip(eng._k_caches, eng._v_caches)]
+    with pytest.raises(RuntimeError):
+        eng.sample_ids([[5, 6, 7, 8], [5, 6, 7, last]], 4)
+    assert eng.positions == positions
+    assert all(torch.equal(k, a) and torch.equal(v, b) for k, v, (a, b) in zip(eng._k_caches, eng._v_caches, rows))
+    assert eng.sample_ids([[5, 6, 7, 8]], 0, temperature=-1.0) == ([[]], [[]])
