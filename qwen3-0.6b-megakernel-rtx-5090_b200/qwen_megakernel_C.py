@@ -503,6 +503,7 @@ def generate_batch(first_token_ids, start_positions, num_steps, embed_weight, la
 
 
 MAX_GEMM_BATCH_SEQUENCES = 128
+_CACHE_ROW_BYTES = 8 * 128 * 2       # a position's keys (or values) of a layer: kv heads x head_dim, fp16
 
 
 def decode_batched(first_token_ids, start_positions, num_steps, embed_weight, layer_weights_packed,
@@ -557,6 +558,10 @@ def sample_batched(first_token_ids, start_positions, num_steps, embed_weight, la
         for log in logs:
             _check(log.dtype == dtype and log.is_cuda and log.is_contiguous() and log.numel() >= num_steps,
                    f"sample_batched: each log must be a contiguous {dtype} CUDA tensor of >= num_steps entries")
+    cache_bytes = _CACHE_ROW_BYTES * int(num_layers) * int(max_seq_len)
+    for cache in (*((k_prefix, v_prefix) if int(prefix_len) > 0 else ()), *k_caches, *v_caches):
+        _check(cache is not None and cache.is_cuda and cache.is_contiguous() and cache.nbytes >= cache_bytes,
+               "sample_batched: each cache, the prefix's too, must be a contiguous CUDA tensor [num_layers, kv_heads, max_seq_len, head_dim] of fp16")
     temperatures, top_ks, top_ps, min_ps = check_sampling(n, num_steps, uniforms, temperatures, top_ks, top_ps, min_ps)
     _check_table(layer_weights_packed, "sample_batched")
     ints, floats, ptrs = ctypes.c_int * n, ctypes.c_float * n, ctypes.c_void_p * n

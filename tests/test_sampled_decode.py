@@ -278,3 +278,27 @@ def test_refused_tokens_and_vocabularies_leave_the_slots_as_they_were(gpu, engin
     assert eng.positions == positions
     assert all(torch.equal(k, a) and torch.equal(v, b) for k, v, (a, b) in zip(eng._k_caches, eng._v_caches, rows))
     assert eng.sample_ids([[5, 6, 7, 8]], 0, temperature=-1.0) == ([[]], [[]])
+
+
+@pytest.mark.gpu
+def test_caches_that_the_steps_could_not_read_are_refused(gpu):
+    """Of the host's memory, of fewer rows than the call says, not contiguous, or none: the prefix's caches and the sequences' own."""
+    eng = _engine(S.make_weights(seed=37, num_layers=2, vocab_size=VOCAB, norm_std=0.1, max_seq_len=16), 2, 64)
+    base = eng._base
+    base.apply_options()
+    logs, scores = [torch.zeros(4, dtype=torch.int32, device="cuda") for _ in range(2)], [torch.zeros(4, device="cuda") for _ in range(2)]
+
+    def call(k_prefix, v_prefix, k, v, max_seq_len=64):
+        gpu.sample_batched([1, 2], [8, 9], 4, base._embed_weight, base._layer_weights_packed, base._final_norm_weight, base._lm_head_weight, base._cos_table,
+                           base._sin_table, k_prefix, v_prefix, 8, k, v, torch.rand(4, 2, device="cuda"), [1.0, 1.0], [0, 0], [1.0, 1.0],
+                           [0.0, 0.0], logs, scores, base.num_layers, max_seq_len, base._attn_scale)
+    good = [eng._k_caches[0], eng._v_caches[0], eng._k_caches, eng._v_caches]
+    for which in range(4):
+        for bad in (lambda t: t.cpu(), lambda t: t[:, :, :60].contiguous(), lambda t: t[:1], lambda t: torch.cat((t, t), 3)[..., :128], lambda t: None):
+            case = list(good)
+            case[which] = bad(good[which]) if which < 2 else [good[which][0], bad(good[which][1])]
+            with pytest.raises(RuntimeError, match="cache"):
+                call(*case)
+    with pytest.raises(RuntimeError, match="cache"):
+        call(*good, max_seq_len=65)
+    call(*good)
