@@ -1092,8 +1092,8 @@ __global__ void __launch_bounds__(256) argmax_pairs(const float *val, const int 
   }
 }
 
-// What the steps of a qmk_sample_batched call read beside the weights: options and addresses of the call, and what next_sampled_step leaves
-// for the step at hand.
+// What the steps of a qmk_sample_batched call read beside the weights: options of the call and addresses (those that the attention reads are in its
+// launches), and what next_sampled_step leaves for the step at hand.
 struct SampleState {
   unsigned long long kv_ptrs[2 * 128];           // K and V cache of every sequence
   float *logprob_logs[128];

@@ -1431,7 +1431,8 @@ static int decode_batched(const char *who, const Sampling *sampling, int num_seq
   const int M = qmk_gemm::BM;   // one tile of rows; rows >= B are computed and ignored
   // One decode step for all sequences, enqueued on `s`.  Everything that changes from step to step (tokens,
   // positions) or from call to call (cache and log pointers) lives in device arrays at fixed addresses, so the
-  // same sequence of launches - and a graph captured from it - serves every step.
+  // same sequence of launches - and a graph captured from it - serves every step.  (Sampled steps are an exception: their attention's
+  // launches hold the caches' addresses, the prefix's length and the rows of an own cache in steps of 256; see the key of their graph.)
   // The O (K = 2048) and down (K = 3072) projections have only 1024 output columns: K is split four ways and the
   // following RMSNorm adds the partial matrices.
   // N tiles of 32 columns: 128 (q/k/v), 96 (gate/up) and, with K split four ways, 128 CTAs (O, down) per GEMM
@@ -1596,7 +1597,8 @@ static int decode_batched(const char *who, const Sampling *sampling, int num_seq
         reinterpret_cast<unsigned long long>(rope), reinterpret_cast<unsigned long long>(cos_table),
         reinterpret_cast<unsigned long long>(sin_table) ^ (static_cast<unsigned long long>(env.timeout_ms) << 48) ^
             (static_cast<unsigned long long>(env.pdl != 0) << 63) ^ (static_cast<unsigned long long>(env.attn_mma != 0) << 62)};
-    // (a sampled step's attention has the caches' addresses in its launches)
+    // (A sampled step's attention has the caches' addresses and the prefix's length in its launches: a call with others captures the step again, 0.9 to
+    // 1.3 ms with 28 layers, once a call.)
     std::vector<unsigned long long> sample_key;
     if (sampling) {
       sample_key.assign(key, key + 12);

@@ -10,18 +10,23 @@
 // moves a border of the cumulative distribution by 2^-46 a token, where 32-bit floating sums would move it by up to 2^-24 of the total,
 // more than a token in the tail of a large vocabulary has.
 //
-// A cluster of CTAs takes a row, as many as leave every row's CTAs resident together.  A row is read from one to three times; it crosses
-// HBM the first time, and is in L1 or L2 then.  (Rows kept in shared memory as fp32 needed clusters of eight for 151,936 tokens, so 128
+// A cluster of CTAs takes a row, as many as leave every row's CTAs resident together.  A row crosses HBM once, and is in L1 or L2 when it
+// is read again: twice in all for the plain draw, min-p, top-k up to 1280 (768 with one CTA a row; with top-p or not) and top-p alone; three to six times for larger k, for top-p
+// behind them, at temperatures below 0.16 or where its window misses; and six times more for each threshold that search finds.  (Rows kept in shared memory as fp32 needed clusters of eight for 151,936 tokens, so 128
 // rows four waves of CTAs in lockstep: 76 us for the plain draw and 88 with top-k, where two CTAs a row without it take 52 and 38.)
 // A threshold (of top-k, of top-p) is found by narrowing down: a histogram of counts over the distance to the maximum, then, where
 // the tokens up to the border's bin are few, a list of them that one CTA sorts and finishes; else a list of the border's bins alone.  Rows
 // whose border lies among more (nearly) equal values than a list holds go through eight-bit histograms of the keys (search).  Top-p alone, the
 // common case, has its histogram from the first pass, while the row crosses HBM: its bins lie on a ring and need no maximum.
 //
-// Measured, us a call in a graph with fp32 rows of 151,936 tokens, one / 32 / 128 of them (12 us of HBM): plain draw 13 / 20 / 52, min-p 10 / 13 / 29, top-k 50 with
-// top-p 17 / 22 / 38, top-p alone 29 / 43 / 86.  Few rows: the chain of reductions across the cluster, 1 to 2 us each.  Many: instruction issue, a
-// mass (a power of two in 64 bits, rounded to a whole number) of every token within SPAN of the maximum in each pass - the plain draw and top-p have one such
-// pass; min-p and top-k compare in 32 bits and leave few tokens to weigh.
+// Measured, us a call in a graph with fp32 rows of 151,936 tokens out of HBM, one / 32 / 128 of them (12 us of HBM): plain draw 14 / 21 / 53, min-p 12 / 16 / 34, top-k
+// 50 with top-p 19 / 25 / 41, top-p alone 31 / 43 / 88.  Few rows: the chain of reductions across the cluster, 1 to 2 us each.  Many: no unit is full (issue
+// slots 49 to 60 %, fp64 12 to 21 %); it is 32 instructions for a token's mass (a power of two in 64 bits, rounded to a whole number) of every token within
+// SPAN of the maximum - the plain draw and top-p have one such pass; min-p and top-k compare in 32 bits and leave few tokens to weigh - and their
+// latency at two CTAs an SM, whose 64 registers a thread spill (some 850 bytes of loads in the whole kernel; 110 to 130 with one CTA an SM).
+// The other ways, one / 128 rows: top-k 5000 34 / 105, with top-p 51 / 175; top-p at temperature 0.1 71 / 246; normal logits of deviation 0.05, top-p 119 / 485, top-k
+// 5000 with top-p 236 / 1233; all logits equal, top-p 2300 / 13,100, top-k 5000 with top-p 3300 / 14,200: search adds 64-bit numbers to one bin of a histogram, one behind the
+// other (a sort of 128 such rows takes 6000).
 #ifndef QMK_SAMPLING_CUH_
 #define QMK_SAMPLING_CUH_
 

@@ -9,7 +9,8 @@
 //
 // An item is a block of query rows against a range of cache rows of one kv head: (row tile, kv head, prefix range) or (sequence, kv
 // head, range of own rows).  Three or two launches: the items' states (up to 32 query rows of a kv head here, more in shared_prefix_tcgen05.cuh with the
-// own rows' kernel beside it), then the join, which starts early and waits (programmatic dependent launch).
+// own rows' kernel behind it), then the join.  Each starts early, behind the last CTAs of the one before, and waits where it has to (programmatic dependent
+// launch).
 //
 // Measured, caches cold, 16 query heads on 8 kv heads of 128 dims: attend_parts with 8 sequences and 32,768 shared rows 25.5 us, 5.3 TB/s, bound by
 // HBM and the ramp of the CTAs' first tiles; own_parts with 64 sequences of 512 own rows 16.5 us, 4.1 TB/s; join_parts 6 to 10 us, the latency of two
@@ -78,7 +79,10 @@ template <> struct Half<__half> {
     return *reinterpret_cast<const uint32_t *>(&h);
   }
   static __device__ __forceinline__ __half from(float a) { return __float2half_rn(a); }
-  // Weights are at most 2^P_SHIFT: rounding 2^-11 of the value down to 2^-14, and so for weights of 2^-26 of the row's largest on.
+  // Weights are rounded to the operand type, once, because the tensor cores multiply 16-bit operands by values of 16 bits only; the sum of the weights, the
+  // outputs and the joined states stay fp32.  Each weight is off by at most 2^-11 of itself in fp16 (2^-8 in bf16), as much as the output's own rounding, so the
+  // error against 64 bits grows by 1.4 at most where many weights count (16,384 equal-sized ones: 2.8e-4 of the outputs' size, with fp32 weights 2.1e-4).
+  // They are at most 2^P_SHIFT: rounding 2^-11 of the value down to 2^-14, and so for weights of 2^-26 of the row's largest on.
   static constexpr float P_SHIFT = 12.0f;
   static constexpr bool BF16 = false;
 };
@@ -437,8 +441,9 @@ __global__ void __launch_bounds__(THREADS) attend_parts(const __grid_constant__ 
   const size_t off = static_cast<size_t>(kv) * p.prefix_head + static_cast<size_t>(first) * p.prefix_row;
   item_mma<T, D, MT>(p, smem, part, kv, row0, live, static_cast<const T *>(p.k_prefix) + off, static_cast<const T *>(p.v_prefix) + off, p.prefix_row, n);
 }
-// Many: the own rows alone, launched behind prefix_parts_tc, which has waited for what is read here: they run beside it and end behind it.  Small CTAs, six
-// an SM: what one waits for (its length, the queries, the first rows, its warps at the end) passes under the others.
+// Many: the own rows alone, launched behind prefix_parts_tc, which has waited for what is read here: they start on the SMs that it does not use or has
+// left - no CTA of this kernel fits beside one of it, which has 168 x 384 registers and with 128 dims 229,632 bytes of shared memory - and end behind
+// it.  Small CTAs, six an SM: what one waits for (its length, the queries, the first rows, its warps at the end) passes under the others.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32 * own_warps(D), D == 64 ? 4 : 6) own_parts(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) unsigned char smem[];
