@@ -630,10 +630,10 @@ class BatchDecoder:
             uniforms = torch.rand(steps, n, device=dev, generator=generator)
         elif tuple(uniforms.shape) != (steps, n):
             raise ValueError(f"uniforms must be [{steps}, {n}]")
-        elif uniforms.device != dev:
-            raise RuntimeError(f"uniforms must be on {dev}")
         uniforms = uniforms.contiguous()
         if steps:                                                # (what the steps would refuse, before any slot changes)
+            if uniforms.device != dev:
+                raise RuntimeError(f"uniforms must be on {dev}")
             options = _require_megakernel_op("check_sampling")(n, steps, uniforms, *options)
             if base.vocab_size % 128:
                 raise RuntimeError("sample_ids needs a vocabulary that is a multiple of 128")

@@ -749,7 +749,8 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     ``[n, kv_heads, rows, dim]``, or lists of ``n`` tensors ``[kv_heads, rows, dim]`` with the same strides (views of cache tensors), of which
     sequence ``b`` sees the first ``own_lens[b]`` (int32 on the device, taken into ``[0, rows]``).  fp16 or bf16; at most 128 sequences,
     16 query heads per kv head, ``dim`` 64 or 128.  ``scale`` defaults to ``dim ** -0.5``.  ``out`` is like ``q`` (contiguous), ``lse``
-    the fp32 ``[n, q_heads]`` logarithms of the softmax sums; a sequence that sees no row gets zeros and -inf.  Runs on the current
+    the fp32 ``[n, q_heads]`` logarithms of the softmax sums; a sequence that sees no row gets zeros and -inf (and NaN what a wait of the kernel's that ran out
+    behind 2 s concerns).  Runs on the current
     stream of the tensors' device, does not synchronise, may be captured in a graph (behind a call with these types and sizes on the device)."""
     who = "attention_shared_prefix"
     dtype = q.dtype
