@@ -479,6 +479,55 @@ int qmk_sample_batched(
     int *const *output_logs, float *const *logprob_logs,
     int num_layers, int max_seq_len, float attn_scale, cudaStream_t stream);
 
+/* Caches kept in 4 or 8 bits (no counterpart in the reference, whose cache is fp16).  A packed row - what a kv head keeps of a position - is
+ * head_dim * bits / 8 bytes of codes and a 16-byte trailer: four fp16 scales s and four fp16 centres z, a pair for each quarter b of the
+ * dimensions.  With M = 2^(bits - 1) a code n stands for z + s (n - M); s = fp16((hi - lo) / (2^bits - 1)), z = fp16(lo + M s), n the whole number
+ * nearest to (x - z) / s (ties to even; 0 where s is 0) + M, taken into [0, 2^bits - 1], lo and hi the quarter's least and largest value.  A quarter that holds
+ * a value that is no number, infinite or above 65504 in size reads back as NaN.  Dimension head_dim/4 b + head_dim/32 g + j (b < 4, g < 8) has its code at
+ * index head_dim/8 g + head_dim/32 b + j, 4-bit codes in the low half of a byte first.  A row takes 80 bytes (128 dimensions, 4 bits), 144 (128, 8), 48 (64, 4)
+ * or 80 (64, 8).  Addresses and strides are multiples of 16 bytes. */
+typedef struct qmk_packed_cache {
+  int bits, head_dim, num_sequences, kv_heads, rows;   /* 4 or 8; 64 or 128; 1 to 128; 1 to 1024; rows a cache has room for, up to 2^24 */
+  void *const *k, *const *v;         /* HOST arrays of DEVICE pointers, one per sequence: [kv_heads][rows][row bytes], the same strides for all */
+  void *k_base, *v_base;             /* used where k is null: the caches of sequence 0, seq_stride bytes between sequences */
+  long long seq_stride, head_stride, row_stride;       /* bytes */
+} qmk_packed_cache;
+/* Rows of a call: [num_sequences][kv_heads][rows][head_dim], the head dimension contiguous, strides in elements (multiples of 8), 16-byte aligned.
+ * Row t of sequence b belongs to row starts[b] + t of its cache; there are lens[b] of them.  DEVICE arrays, or null: `start` and `rows` for all. */
+typedef struct qmk_packed_rows {
+  int type;                          /* 0 fp16, 1 bf16 */
+  int rows;                          /* of a sequence in this call, 0 to 2^24; below 2^31 over all sequences and heads */
+  void *k, *v;                       /* DEVICE, the same strides for both */
+  long long seq_stride, head_stride, row_stride;
+  const int *starts, *lens;
+  int start;
+} qmk_packed_rows;
+/* Quantises the rows into the caches; those that fall outside a cache or behind lens[b] are left out, all other rows of the caches stay as they are.  Two
+ * rows of one call must not fall on the same row of a cache.  Does not block, allocates nothing, may be captured. */
+int qmk_write_cache_packed(const qmk_packed_cache *cache, const qmk_packed_rows *rows, cudaStream_t stream);
+/* The values of the caches' rows, each rounded once to the type (one past the largest fp16 number to that); zeros in rows that are outside a cache or behind lens[b].  Does not block,
+ * allocates nothing, may be captured. */
+int qmk_read_cache_packed(const qmk_packed_cache *cache, const qmk_packed_rows *rows, cudaStream_t stream);
+/* Attention of one new token per sequence over packed caches.  Per sequence b and query head h (kv head h / (q_heads / kv_heads)): out = softmax(scale * q . k) v
+ * over the values of rows [0, lens[b]) (lens taken into [0, rows]), lse the natural logarithm of the sum of exp(scale * q . k).  Nothing visible: zeros and -inf.
+ * Rows behind the last are not looked at.  1 to 16 query heads per kv head.  Does not block, allocates nothing, may be captured behind a first call
+ * with its types and sizes on the device; the workspace (DEVICE, 16-byte aligned, size from qmk_attention_packed_cache_workspace) belongs to the call until it is done. */
+typedef struct qmk_packed_attention {
+  int type;                          /* 0 fp16, 1 bf16: q and out */
+  int q_heads;
+  const void *q;                     /* [num_sequences][q_heads][head_dim], strides in elements (multiples of 8), 16-byte aligned */
+  long long q_seq_stride, q_head_stride;
+  const int *lens;                   /* DEVICE, one per sequence */
+  float scale;
+  void *out;                         /* [num_sequences][q_heads][head_dim], contiguous */
+  float *lse;                        /* [num_sequences][q_heads], may be null */
+  void *workspace;
+  long long workspace_bytes;
+} qmk_packed_attention;
+int qmk_attention_packed_cache(const qmk_packed_cache *cache, const qmk_packed_attention *args, cudaStream_t stream);
+/* Bytes; 0 for sizes that the call refuses. */
+long long qmk_attention_packed_cache_workspace(int num_sequences, int q_heads, int kv_heads, int head_dim, int bits, int rows);
+
 /* Synchronises the device and returns the status word of the last launch
  * (QMK_OK, or the first error a CTA recorded). */
 int qmk_sync_status(void);

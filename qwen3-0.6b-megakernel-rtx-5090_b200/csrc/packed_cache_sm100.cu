@@ -1,0 +1,148 @@
+// C entries of the packed caches (packed_cache.cuh) and of the attention over them (packed_attention.cuh).
+#include "../../include/qwen_megakernel.h"
+
+#include <algorithm>
+#include <string>
+
+#include "engine_internal.h"
+#include "packed_attention.cuh"
+#include "packed_cache.cuh"
+
+namespace {
+
+using namespace qmk_packed;
+
+constexpr int MAX_ROWS = 1 << 24;                // of a cache
+constexpr int MAX_HEADS = 1024;
+
+int refuse(const char *who, const std::string &why) {
+  qmk_internal::note_error(std::string(who) + ": " + why);
+  return QMK_ERR_BAD_ARGUMENT;
+}
+int answer(const char *who, cudaError_t e) {
+  if (e == cudaSuccess) return QMK_OK;
+  cudaGetLastError();
+  qmk_internal::note_error(std::string(who) + ": " + cudaGetErrorString(e));
+  return QMK_ERR_CUDA;
+}
+bool odd(const void *ptr) { return (reinterpret_cast<unsigned long long>(ptr) & 15u) != 0; }
+bool odd(long long stride, int size, int of) { return size > 1 && stride % of; }
+
+// What is wrong with a cache; null: nothing, and `c` says where it is
+const char *read_cache(const qmk_packed_cache *a, Caches *c) {
+  if (!a) return "null pointer argument";
+  if (a->bits != 4 && a->bits != 8) return "bits must be 4 or 8";
+  if (a->head_dim != 64 && a->head_dim != 128) return "head_dim must be 64 or 128";
+  if (a->num_sequences < 1 || a->num_sequences > MAX_SEQS) return "num_sequences must be in [1, 128]";
+  if (a->kv_heads < 1 || a->kv_heads > MAX_HEADS) return "kv_heads must be in [1, 1024]";
+  if (a->rows < 0 || a->rows > MAX_ROWS) return "rows must be in [0, 2^24]";
+  if (a->rows > 0 && (a->k ? !a->v : !a->k_base || !a->v_base)) return "null pointer argument";
+  if (odd(a->seq_stride, a->num_sequences, 16) || odd(a->head_stride, a->kv_heads, 16) || odd(a->row_stride, a->rows, 16)) return "a cache's strides must be multiples of 16 bytes";
+  if (a->rows > 1 && a->row_stride < a->head_dim * a->bits / 8 + TRAILER) return "rows of a cache overlap: the row stride is below a row's bytes";
+  c->seqs = a->num_sequences;
+  c->kv_heads = a->kv_heads;
+  c->rows = a->rows;
+  c->head = a->head_stride;
+  c->row = a->row_stride;
+  for (int b = 0; b < a->num_sequences; ++b) {
+    c->k[b] = static_cast<const unsigned char *>(a->k ? a->k[b] : static_cast<const char *>(a->k_base) + b * a->seq_stride);
+    c->v[b] = static_cast<const unsigned char *>(a->k ? a->v[b] : static_cast<const char *>(a->v_base) + b * a->seq_stride);
+    if (a->rows > 0 && (!c->k[b] || !c->v[b])) return "null pointer argument";
+    if (odd(c->k[b]) || odd(c->v[b])) return "a cache's address must be a multiple of 16";
+  }
+  return nullptr;
+}
+
+// What is wrong with the rows of a call; null: nothing
+const char *read_rows_of(const qmk_packed_rows *a, RowParams *p) {
+  if (!a) return "null pointer argument";
+  if (a->type < 0 || a->type > 1) return "the type is fp16 (0) or bf16 (1)";
+  if (a->rows < 0 || a->rows > MAX_ROWS) return "rows must be in [0, 2^24]";
+  if (static_cast<long long>(p->caches.seqs) * p->caches.kv_heads * a->rows > 0x7fffffffll) return "2^31 rows of all heads or more";
+  if (a->rows > 0 && (!a->k || !a->v)) return "null pointer argument";
+  if (odd(a->k) || odd(a->v)) return "the rows' addresses must be multiples of 16";
+  if (odd(a->seq_stride, p->caches.seqs, 8) || odd(a->head_stride, p->caches.kv_heads, 8) || odd(a->row_stride, a->rows, 8)) return "the rows' strides must be multiples of 8 elements";
+  p->k = a->k;
+  p->v = a->v;
+  p->seq = a->seq_stride;
+  p->head = a->head_stride;
+  p->row = a->row_stride;
+  p->rows = a->rows;
+  p->starts = a->starts;
+  p->start = a->start;
+  p->lens = a->lens;
+  return nullptr;
+}
+
+template <typename T, int DIM, int BITS>
+void (*row_kernel(bool write))(RowParams, unsigned int) { return write ? write_rows<T, DIM, BITS> : read_rows<T, DIM, BITS>; }
+template <typename T>
+void (*row_kernel(bool write, int dim, int bits))(RowParams, unsigned int) {
+  if (bits == 4) return dim == 64 ? row_kernel<T, 64, 4>(write) : row_kernel<T, 128, 4>(write);
+  return dim == 64 ? row_kernel<T, 64, 8>(write) : row_kernel<T, 128, 8>(write);
+}
+
+int rows_call(const char *who, const qmk_packed_cache *cache, const qmk_packed_rows *rows, bool write, cudaStream_t stream) {
+  qmk_internal::begin_call();
+  RowParams p;
+  if (const char *why = read_cache(cache, &p.caches)) return refuse(who, why);
+  if (const char *why = read_rows_of(rows, &p)) return refuse(who, why);
+  const unsigned int count = static_cast<unsigned int>(p.caches.seqs) * p.caches.kv_heads * p.rows;
+  if (count == 0) return QMK_OK;
+  const unsigned int blocks = std::min((count + THREADS / 8 - 1) / (THREADS / 8), 148u * 16);
+  void (*const kernel)(RowParams, unsigned int) = rows->type == 0 ? row_kernel<__half>(write, cache->head_dim, cache->bits) : row_kernel<__nv_bfloat16>(write, cache->head_dim, cache->bits);
+  kernel<<<blocks, THREADS, 0, stream>>>(p, count);
+  return answer(who, cudaGetLastError());
+}
+
+template <typename T, int DIM, int BITS>
+cudaError_t attend(const AttendParams &p, cudaStream_t stream) {
+  attend_rows<T, DIM, BITS><<<p.caches.seqs * p.q_heads, 128, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+template <typename T>
+cudaError_t attend(const AttendParams &p, int dim, int bits, cudaStream_t stream) {
+  if (bits == 4) return dim == 64 ? attend<T, 64, 4>(p, stream) : attend<T, 128, 4>(p, stream);
+  return dim == 64 ? attend<T, 64, 8>(p, stream) : attend<T, 128, 8>(p, stream);
+}
+
+}  // namespace
+
+extern "C" int qmk_write_cache_packed(const qmk_packed_cache *cache, const qmk_packed_rows *rows, cudaStream_t stream) {
+  return rows_call("qmk_write_cache_packed", cache, rows, true, stream);
+}
+extern "C" int qmk_read_cache_packed(const qmk_packed_cache *cache, const qmk_packed_rows *rows, cudaStream_t stream) {
+  return rows_call("qmk_read_cache_packed", cache, rows, false, stream);
+}
+
+extern "C" long long qmk_attention_packed_cache_workspace(int num_sequences, int q_heads, int kv_heads, int head_dim, int bits, int rows) {
+  if (num_sequences < 1 || num_sequences > MAX_SEQS || kv_heads < 1 || kv_heads > MAX_HEADS || q_heads < 1 || q_heads % kv_heads || q_heads / kv_heads > MAX_GROUP ||
+      (head_dim != 64 && head_dim != 128) || (bits != 4 && bits != 8) || rows < 0 || rows > MAX_ROWS)
+    return 0;
+  return 16;
+}
+
+extern "C" int qmk_attention_packed_cache(const qmk_packed_cache *cache, const qmk_packed_attention *a, cudaStream_t stream) {
+  const char *const who = "qmk_attention_packed_cache";
+  qmk_internal::begin_call();
+  AttendParams p;
+  if (const char *why = read_cache(cache, &p.caches)) return refuse(who, why);
+  if (!a || !a->q || !a->out || !a->lens || !a->workspace) return refuse(who, "null pointer argument");
+  if (a->type < 0 || a->type > 1) return refuse(who, "the type is fp16 (0) or bf16 (1)");
+  if (a->q_heads < 1 || a->q_heads % cache->kv_heads || a->q_heads / cache->kv_heads > MAX_GROUP) return refuse(who, "q_heads must be 1 to 16 times kv_heads");
+  if (!(a->scale > -2.0e38f && a->scale < 2.0e38f)) return refuse(who, "the scale must be finite, and below 2e38");   // (times log2 e too)
+  if (odd(a->q) || odd(a->out) || odd(a->workspace)) return refuse(who, "pointers must be 16-byte aligned");
+  if (odd(a->q_seq_stride, cache->num_sequences, 8) || odd(a->q_head_stride, a->q_heads, 8)) return refuse(who, "the queries' strides must be multiples of 8 elements");
+  if (a->workspace_bytes < qmk_attention_packed_cache_workspace(cache->num_sequences, a->q_heads, cache->kv_heads, cache->head_dim, cache->bits, cache->rows))
+    return refuse(who, "workspace too small");
+  p.q = a->q;
+  p.q_seq = a->q_seq_stride;
+  p.q_head = a->q_head_stride;
+  p.q_heads = a->q_heads;
+  p.group = a->q_heads / cache->kv_heads;
+  p.lens = a->lens;
+  p.scale_log2 = a->scale * LOG2E;
+  p.out = a->out;
+  p.lse = a->lse;
+  return answer(who, a->type == 0 ? attend<__half>(p, cache->head_dim, cache->bits, stream) : attend<__nv_bfloat16>(p, cache->head_dim, cache->bits, stream));
+}

@@ -120,6 +120,32 @@ _lib.qmk_sample_batched.argtypes = [_I, _P, _P, _I, *([_P] * 6), _P, _P, _I, _P,
 _lib.qmk_sample_batched.restype = _I
 
 
+class _PackedCache(ctypes.Structure):
+    _fields_ = [("bits", _I), ("head_dim", _I), ("num_sequences", _I), ("kv_heads", _I), ("rows", _I), ("k", _P), ("v", _P), ("k_base", _P), ("v_base", _P),
+                ("seq_stride", _LL), ("head_stride", _LL), ("row_stride", _LL)]
+
+
+class _PackedRows(ctypes.Structure):
+    _fields_ = [("type", _I), ("rows", _I), ("k", _P), ("v", _P), ("seq_stride", _LL), ("head_stride", _LL), ("row_stride", _LL), ("starts", _P), ("lens", _P),
+                ("start", _I)]
+
+
+class _PackedAttention(ctypes.Structure):
+    _fields_ = [("type", _I), ("q_heads", _I), ("q", _P), ("q_seq_stride", _LL), ("q_head_stride", _LL), ("lens", _P), ("scale", _F), ("out", _P), ("lse", _P),
+                ("workspace", _P), ("workspace_bytes", _LL)]
+
+
+_pack_packed_cache, _pack_packed_rows, _pack_packed_attention = (struct.Struct(f) for f in ("@5i 4P3q", "@2i 2P3q 2Pi0q", "@2i P2q P f 3Pq"))
+for _made, _fields in ((_pack_packed_cache, _PackedCache), (_pack_packed_rows, _PackedRows), (_pack_packed_attention, _PackedAttention)):
+    assert _made.size == ctypes.sizeof(_fields)
+_pack_packed_cache, _pack_packed_rows, _pack_packed_attention = _pack_packed_cache.pack, _pack_packed_rows.pack, _pack_packed_attention.pack
+for _name in ("qmk_write_cache_packed", "qmk_read_cache_packed", "qmk_attention_packed_cache"):
+    getattr(_lib, _name).argtypes = [ctypes.c_char_p, ctypes.c_char_p, _P]
+    getattr(_lib, _name).restype = _I
+_lib.qmk_attention_packed_cache_workspace.argtypes = [_I] * 6
+_lib.qmk_attention_packed_cache_workspace.restype = _LL
+
+
 class _EngineConfig(ctypes.Structure):
     _fields_ = [("device", _I), ("vocab_size", _I), ("weight_format", _I), ("rope_from_table", _I),
                 ("split_len", _I), ("max_ctas", _I), ("timeout_ms", _I), ("fused", _I), ("inv_freq64", _P)]
@@ -159,7 +185,7 @@ _lib.qmk_selftest_gemm_pair_wait_timeout.restype = _I
 EXPORTED_SYMBOLS = (
     "launch_ldg_decode_direct", "launch_ldg_decode_persistent", "launch_ldg_generate_nosync",
     "launch_ldg_prefill", "qmk_abi_version", "qmk_configure", "qmk_set_inv_freq", "qmk_set_logits_dump",
-    "qmk_set_weight_format", "qmk_set_tuning", "qmk_set_tuning2", "qmk_set_profile_buffer", "qmk_set_fused", "qmk_set_step_overlap", "qmk_set_prefill_attention", "qmk_set_decode_attention", "qmk_invalidate_weights", "qmk_release_weights", "qmk_decode", "qmk_generate", "qmk_generate_static", "qmk_generate_batch", "qmk_gemm_f16_tn", "qmk_gemm_packed_tn", "qmk_sample_tokens", "qmk_attention_shared_prefix", "qmk_attention_shared_prefix_workspace", "qmk_sample_batched", "qmk_decode_batched", "qmk_prefill_chunked", "qmk_prefill_packed", "qmk_prefill_packed_passes", "qmk_prefill", "qmk_engine_create", "qmk_engine_destroy", "qmk_engine_apply", "qmk_engine_decode", "qmk_engine_generate", "qmk_engine_prefill", "qmk_sync_status", "qmk_last_error", "qmk_num_ctas",
+    "qmk_set_weight_format", "qmk_set_tuning", "qmk_set_tuning2", "qmk_set_profile_buffer", "qmk_set_fused", "qmk_set_step_overlap", "qmk_set_prefill_attention", "qmk_set_decode_attention", "qmk_invalidate_weights", "qmk_release_weights", "qmk_decode", "qmk_generate", "qmk_generate_static", "qmk_generate_batch", "qmk_gemm_f16_tn", "qmk_gemm_packed_tn", "qmk_sample_tokens", "qmk_attention_shared_prefix", "qmk_attention_shared_prefix_workspace", "qmk_write_cache_packed", "qmk_read_cache_packed", "qmk_attention_packed_cache", "qmk_attention_packed_cache_workspace", "qmk_sample_batched", "qmk_decode_batched", "qmk_prefill_chunked", "qmk_prefill_packed", "qmk_prefill_packed_passes", "qmk_prefill", "qmk_engine_create", "qmk_engine_destroy", "qmk_engine_apply", "qmk_engine_decode", "qmk_engine_generate", "qmk_engine_prefill", "qmk_sync_status", "qmk_last_error", "qmk_num_ctas",
     "qmk_scratch_bytes", "qmk_selftest_decode_ring", "qmk_selftest_wait_timeout", "qmk_selftest_gemm_wait_timeout", "qmk_selftest_attention_wait_timeout", "qmk_selftest_gemm_pair_wait_timeout", "qmk_selftest_decode_attention_wait_timeout", "qmk_selftest_shared_prefix_wait_timeout",
 )
 
@@ -684,11 +710,12 @@ def gemm_packed_tn(a: torch.Tensor, b: torch.Tensor, weight_format, b2: torch.Te
     return out
 
 
-# The two operators below are called once per layer or step: their checks are plain expressions, and the stream is asked for without an
+# The operators below are called once per layer or step: their checks are plain expressions, and the stream is asked for without an
 # object around it (a call's host time 25 -> 12 us for a row of logits, of which the launch is 5).
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 _LOGIT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_FP32, _INT32 = torch.float32, torch.int32
+_FP32, _INT32, _UINT8 = torch.float32, torch.int32, torch.uint8
+_ROW_TYPES = {torch.float16: 0, torch.bfloat16: 1}
 
 
 def _on_device(index: int, call, *args):
@@ -816,6 +843,168 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
 def _shared_prefix_workspace(*sizes):
     """Bytes of workspace for these sizes (``qmk_attention_shared_prefix_workspace``, at least a few)."""
     return (max(int(_lib.qmk_attention_shared_prefix_workspace(*sizes)), 256) + 3) // 4 * 4
+
+
+MAX_PACKED_SEQUENCES = 128
+PACKED_TRAILER_BYTES = 16
+
+
+def packed_row_bytes(dim: int, bits: int) -> int:
+    """Bytes of a packed cache row of ``dim`` (64 or 128) values in ``bits`` (4 or 8): codes and scales; the format: ``qmk_packed_cache`` in include/qwen_megakernel.h."""
+    _check(dim in (64, 128) and bits in (4, 8), "packed_row_bytes: dim must be 64 or 128 and bits 4 or 8")
+    return dim * bits // 8 + PACKED_TRAILER_BYTES
+
+
+def _packed_cache(who, k_cache, v_cache, n, dim, index):
+    """(``qmk_packed_cache`` as bytes, sequences, kv heads, rows, bits, what has to outlive the call) of a cache pair for ``n`` sequences (None: as many as there are)."""
+    if isinstance(k_cache, torch.Tensor) and isinstance(v_cache, torch.Tensor):
+        shape, strides = k_cache.shape, k_cache.stride()
+        if not (len(shape) == 4 and shape == v_cache.shape and strides == v_cache.stride() and (n is None or shape[0] == n)):
+            raise RuntimeError(f"{who}: k_cache and v_cache must be [n, kv_heads, rows, row bytes] with the same strides")
+        n, heads, rows, row_bytes = shape
+        seq, head, row, last = strides
+        like = k_cache.dtype is _UINT8 and v_cache.dtype is _UINT8 and k_cache.get_device() == index and v_cache.get_device() == index
+        k_ptrs, v_ptrs, k_base, v_base, keep = 0, 0, k_cache.data_ptr(), v_cache.data_ptr(), None
+    else:
+        k_cache, v_cache = list(k_cache), list(v_cache)
+        if n is None:
+            n = len(k_cache)
+        if not (len(k_cache) == n and len(v_cache) == n and n >= 1 and all(t.dim() == 3 for t in (*k_cache, *v_cache))):
+            raise RuntimeError(f"{who}: one cache pair [kv_heads, rows, row bytes] per sequence")
+        shape, strides = k_cache[0].shape, k_cache[0].stride()
+        heads, rows, row_bytes = shape
+        seq, (head, row, last) = 0, strides
+        like = all(t.shape == shape and t.stride() == strides and t.dtype is _UINT8 and t.get_device() == index for t in (*k_cache, *v_cache))
+        pointers = ctypes.c_void_p * n
+        keep = pointers(*[t.data_ptr() for t in k_cache]), pointers(*[t.data_ptr() for t in v_cache])
+        k_ptrs, v_ptrs, k_base, v_base = ctypes.addressof(keep[0]), ctypes.addressof(keep[1]), 0, 0
+    if not (like and last == 1 and index >= 0):
+        raise RuntimeError(f"{who}: packed caches must be uint8 CUDA tensors on the same device, contiguous within a row, and of the same shape and strides")
+    bits = (row_bytes - PACKED_TRAILER_BYTES) * 8 // dim
+    if dim not in (64, 128) or bits not in (4, 8) or row_bytes != dim * bits // 8 + PACKED_TRAILER_BYTES:
+        raise RuntimeError(f"{who}: no packed row of {dim} values has {row_bytes} bytes (packed_row_bytes)")
+    if not 1 <= n <= MAX_PACKED_SEQUENCES:
+        raise RuntimeError(f"{who}: 1 to {MAX_PACKED_SEQUENCES} sequences per call")
+    return _pack_packed_cache(bits, dim, n, heads, rows, k_ptrs, v_ptrs, k_base, v_base, seq, head, row), n, heads, rows, bits, keep
+
+
+def _per_sequence(who, value, n, index, name):
+    """Device pointer of an int32 tensor with a value per sequence; 0 for None."""
+    if value is None:
+        return 0
+    if not (isinstance(value, torch.Tensor) and value.dtype is _INT32 and value.is_cuda and value.get_device() == index and value.dim() == 1 and value.shape[0] == n
+            and value.is_contiguous()):
+        raise RuntimeError(f"{who}: {name} must be a contiguous int32 tensor with one value per sequence on the caches' device")
+    return value.data_ptr()
+
+
+def _starts(who, starts, n, index):
+    if starts is None or isinstance(starts, int):
+        start = starts or 0
+        if not -_INT_MAX <= start <= _INT_MAX:
+            raise RuntimeError(f"{who}: starts is no 32-bit number")
+        return 0, start
+    return _per_sequence(who, starts, n, index, "starts"), 0
+
+
+def write_cache_packed(k: torch.Tensor, v: torch.Tensor, k_cache, v_cache, starts=0, lens=None) -> None:
+    """Quantises rows into packed caches: ``k`` / ``v [n, kv_heads, rows, dim]`` (fp16 or bf16, the same strides for both; views such as a projection's output
+    with its heads moved to the front) go to rows ``starts[b] + t`` of ``k_cache`` / ``v_cache [n, kv_heads, cache rows, packed_row_bytes(dim, bits)]`` (uint8; or
+    lists of ``n`` tensors ``[kv_heads, cache rows, row bytes]`` with the same strides).  ``starts``: a number, or an int32 CUDA tensor with one per
+    sequence; ``lens`` (int32 tensor, optional): only the first ``lens[b]`` rows of sequence ``b`` are there.  Rows that fall outside a cache are left out, all
+    others of the caches stay as they are; two rows of a call must not fall on one.  The format and its rounding: ``qmk_packed_cache`` in include/qwen_megakernel.h.  Runs
+    on the current stream of the tensors' device, does not synchronise, may be captured in a graph."""
+    who = "write_cache_packed"
+    code = _ROW_TYPES.get(k.dtype, -1)
+    if code < 0 or not k.is_cuda or k.dim() != 4 or k.stride(3) != 1:
+        _require_cuda()
+        raise RuntimeError(f"{who}: k must be a CUDA tensor [n, kv_heads, rows, dim] of fp16 or bf16, contiguous along dim")
+    index, strides = k.get_device(), k.stride()
+    n, heads, rows, dim = k.shape
+    if not (v.shape == k.shape and v.dtype is k.dtype and v.get_device() == index and v.stride() == strides):
+        raise RuntimeError(f"{who}: v must be like k, with the same strides")
+    cache, n, cache_heads, _, _, keep = _packed_cache(who, k_cache, v_cache, n, dim, index)
+    if heads != cache_heads:
+        raise RuntimeError(f"{who}: the caches have {cache_heads} kv heads, the rows {heads}")
+    at, start = _starts(who, starts, n, index)
+    args = _pack_packed_rows(code, rows, k.data_ptr(), v.data_ptr(), strides[0], strides[1], strides[2], at, _per_sequence(who, lens, n, index, "lens"), start)
+    rc = _on_device(index, _lib.qmk_write_cache_packed, cache, args)
+    if rc != 0:
+        raise RuntimeError(f"{who}: {_lib.qmk_last_error().decode()} (status {rc})")
+
+
+def read_cache_packed(k_cache, v_cache, rows: int, dim: int = 128, dtype: torch.dtype = torch.float16, starts=0, lens=None, k_out: torch.Tensor = None,
+                      v_out: torch.Tensor = None):
+    """Values of packed caches (``write_cache_packed``): ``(k, v) [n, kv_heads, rows, dim]`` of ``dtype`` (fp16 or bf16), row ``t`` of sequence ``b`` from row ``starts[b] + t``
+    of its cache; zeros behind ``lens[b]`` (optional) and where a cache has no such row.  ``k_out`` / ``v_out``: where they go, of that shape and with the same
+    strides (views of fp16 caches, say).  Runs on the current stream of the caches' device, does not synchronise, may be captured in a graph."""
+    who = "read_cache_packed"
+    code = _ROW_TYPES.get(dtype, -1)
+    if code < 0:
+        raise RuntimeError(f"{who}: the type must be fp16 or bf16")
+    first = k_cache if isinstance(k_cache, torch.Tensor) else k_cache[0]
+    if not first.is_cuda:
+        _require_cuda()
+        raise RuntimeError(f"{who}: packed caches must be CUDA tensors")
+    index = first.get_device()
+    cache, n, heads, _, _, keep = _packed_cache(who, k_cache, v_cache, None, dim, index)
+    rows = int(rows)
+    if rows < 0:
+        raise RuntimeError(f"{who}: rows is negative")
+    shape = (n, heads, rows, dim)
+    if k_out is None and v_out is None:
+        k_out, v_out = torch.empty(shape, dtype=dtype, device=first.device), torch.empty(shape, dtype=dtype, device=first.device)
+    if k_out is None or v_out is None or not all(tuple(t.shape) == shape and t.dtype is dtype and t.get_device() == index for t in (k_out, v_out)):
+        raise RuntimeError(f"{who}: k_out and v_out must both be {list(shape)} of {dtype} on the caches' device")
+    strides = k_out.stride()
+    if strides != v_out.stride() or strides[3] != 1:
+        raise RuntimeError(f"{who}: k_out and v_out must have the same strides, contiguous along dim")
+    at, start = _starts(who, starts, n, index)
+    args = _pack_packed_rows(code, rows, k_out.data_ptr(), v_out.data_ptr(), strides[0], strides[1], strides[2], at, _per_sequence(who, lens, n, index, "lens"), start)
+    rc = _on_device(index, _lib.qmk_read_cache_packed, cache, args)
+    if rc != 0:
+        raise RuntimeError(f"{who}: {_lib.qmk_last_error().decode()} (status {rc})")
+    return k_out, v_out
+
+
+def attention_packed_cache(q: torch.Tensor, k_cache, v_cache, lens: torch.Tensor, scale: float = None):
+    """Attention of one new token per sequence over packed caches (``write_cache_packed``): ``(out, lse)``.
+
+    ``q [n, q_heads, dim]`` of fp16 or bf16; ``k_cache`` / ``v_cache [n, kv_heads, rows, row bytes]`` (uint8; or lists of ``n`` tensors ``[kv_heads, rows, row bytes]`` with
+    the same strides), of which sequence ``b`` sees the first ``lens[b]`` rows (int32 on the device, taken into ``[0, rows]``).  At most 128
+    sequences, 16 query heads per kv head, ``dim`` 64 or 128.  ``scale`` defaults to ``dim ** -0.5``.  ``out`` is like ``q`` (contiguous), ``lse`` the fp32
+    ``[n, q_heads]`` logarithms of the softmax sums; a sequence that sees no row gets zeros and -inf.  Runs on the current stream of the tensors' device, does not
+    synchronise, may be captured in a graph (behind a call with these types and sizes on the device)."""
+    who = "attention_packed_cache"
+    dtype = q.dtype
+    code = _ROW_TYPES.get(dtype, -1)
+    if code < 0 or not q.is_cuda or q.dim() != 3 or q.stride(2) != 1:
+        _require_cuda()
+        raise RuntimeError(f"{who}: q must be a CUDA tensor [n, q_heads, dim] of fp16 or bf16, contiguous along dim")
+    n, q_heads, dim = q.shape
+    index = q.get_device()
+    cache, n, heads, rows, bits, keep = _packed_cache(who, k_cache, v_cache, n, dim, index)
+    seen = _per_sequence(who, lens, n, index, "lens")
+    if not seen:
+        raise RuntimeError(f"{who}: lens must be a contiguous int32 tensor with one value per sequence on the caches' device")
+    device = q.device
+    out = torch.empty_like(q) if q.is_contiguous() else torch.empty(n, q_heads, dim, dtype=dtype, device=device)
+    lse = torch.empty(n, q_heads, dtype=_FP32, device=device)
+    need = _packed_attention_workspace(n, q_heads, heads, dim, bits, rows)
+    workspace = lens.new_empty(need >> 2)
+    q_seq, q_head, _ = q.stride()
+    args = _pack_packed_attention(code, q_heads, q.data_ptr(), q_seq, q_head, seen, dim ** -0.5 if scale is None else scale, out.data_ptr(), lse.data_ptr(),
+                                  workspace.data_ptr(), need)
+    rc = _on_device(index, _lib.qmk_attention_packed_cache, cache, args)
+    if rc != 0:
+        raise RuntimeError(f"{who}: {_lib.qmk_last_error().decode()} (status {rc})")
+    return out, lse
+
+
+@functools.lru_cache(maxsize=256)
+def _packed_attention_workspace(*sizes):
+    """Bytes of workspace for these sizes (``qmk_attention_packed_cache_workspace``, at least a few)."""
+    return (max(int(_lib.qmk_attention_packed_cache_workspace(*sizes)), 256) + 3) // 4 * 4
 
 
 def sync_status() -> int:

@@ -1,0 +1,521 @@
+"""``write_cache_packed``, ``read_cache_packed`` and ``attention_packed_cache`` against their definitions in 64 bits.
+
+Codes and scales are compared bit by bit.  A value that is read back is off by its own rounding, half a step of the type, and by the fp32 sum before
+it (2^-24).  Tolerance of an output element of the attention, with w the weights, z and s the centre and scale of a row's quarter, n - M its code, A the sum of
+w (|z| + |s (n - M)|), U the sum of w (|z| + s 2^bits): its own rounding, eps / 2 of it; weights and weights times scale rounded to fp16 before they
+multiply, 2^-11 of A; the scores' fp32 sums over dim products, dim 2^-24 of the largest sum of |q| (|z| + s 2^bits) times scale as an absolute error of the
+exponent, so the same relative error of a weight, twice (numerator and denominator), of U; the fp32 sums of the output, whose accumulator may truncate,
+2^-23 for each of the n / 16 steps of U, and as much for the sum of weights.  exp2 in hardware adds 2^-21.  Weights below 2^-21 of the largest lose bits in fp16, at most 2^-32 of
+the largest each, times codes of up to 2^bits of the largest scale.  The logarithm has the scores' error, 2^-22 of itself, and that of the sum."""
+
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def C(built_library):
+    import qwen_megakernel_C
+    return qwen_megakernel_C
+
+
+@pytest.fixture(scope="module")
+def gpu(C):
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return C
+
+
+# ------------------------------------------------------------------------------------------------------------- the definition
+def order(dim):
+    """Index of each dimension's code."""
+    d = np.arange(dim)
+    return dim // 8 * (d % (dim // 4) // (dim // 32)) + dim // 32 * (d // (dim // 4)) + d % (dim // 32)
+
+
+def packed(x, bits):
+    """Packed rows (uint8) of values ``[..., dim]``, by the definition."""
+    x = x.detach().cpu().double().numpy()
+    dim, middle = x.shape[-1], 2 ** (bits - 1)
+    quarters = x.reshape(*x.shape[:-1], 4, dim // 4)
+    low, high = quarters.min(-1, keepdims=True), quarters.max(-1, keepdims=True)      # (NaN where one is)
+    good = (low >= -65504) & (high <= 65504)
+    low, high, quarters = (np.where(good, a, 0.0) for a in (low, high, quarters))
+    s = np.where(good, (high - low) / (2 ** bits - 1), np.nan).astype(np.float16)
+    z = (low + middle * s.astype(np.float64)).astype(np.float16)
+    step = np.where(s > 0, s, 1).astype(np.float64)
+    n = np.where(s > 0, np.rint((quarters - np.where(good, z, 0).astype(np.float64)) / step), 0) + middle
+    n = np.clip(n, 0, 2 ** bits - 1).astype(np.uint8).reshape(x.shape)
+    codes = np.empty_like(n)
+    codes[..., order(dim)] = n
+    if bits == 4:
+        codes = codes[..., 0::2] | codes[..., 1::2] << 4
+    trailer = np.concatenate((s[..., 0], z[..., 0]), -1)
+    trailer[np.isnan(trailer)] = np.uint16(0x7fff).view(np.float16)
+    return torch.from_numpy(np.concatenate((codes, np.ascontiguousarray(trailer).view(np.uint8)), -1))
+
+
+def parts(rows, dim):
+    """(z, s, n - M) of each dimension of packed rows, in 64 bits."""
+    bits = (rows.shape[-1] - 16) * 8 // dim
+    rows = rows.cpu().numpy()
+    n = rows[..., :-16]
+    if bits == 4:
+        n = np.stack((n & 15, n >> 4), -1).reshape(*n.shape[:-1], dim)
+    trailer = np.ascontiguousarray(rows[..., -16:]).view(np.float16).astype(np.float64)
+    quarter = np.arange(dim) // (dim // 4)
+    return tuple(torch.from_numpy(a) for a in (trailer[..., 4 + quarter], trailer[..., quarter], n[..., order(dim)].astype(np.float64) - 2 ** (bits - 1)))
+
+
+def values(rows, dim):
+    z, s, n = parts(rows, dim)
+    return z + s * n
+
+
+def made(*shape, dtype="fp16", seed=0, gain=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * gain).to(DTYPES[dtype]).cuda()
+
+
+def rounded_off(want, dtype):
+    """How far a value of 64 bits may be from what is read back."""
+    return want.abs() * (torch.finfo(dtype).eps / 2 + 2.0 ** -23) + torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2
+
+
+def check_attention(got, q, kc, vc, lens, scale=None):
+    out, lse = got
+    seqs, q_heads, dim = q.shape
+    group = q_heads // kc[0].shape[0]
+    bits = (kc[0].shape[-1] - 16) * 8 // dim
+    scale = dim ** -0.5 if scale is None else scale
+    assert out.dtype == q.dtype and out.shape == q.shape and out.is_contiguous() and lse.dtype == torch.float32 and lse.shape == (seqs, q_heads)
+    out, lse, eps = out.double().cpu(), lse.double().cpu(), torch.finfo(q.dtype).eps
+    for b in range(seqs):
+        n = min(max(int(lens[b]), 0), kc[b].shape[1])
+        if n == 0:
+            assert bool((out[b] == 0).all()) and bool((lse[b] == -math.inf).all())
+            continue
+        (kz, ks, kn), (vz, vs, vn) = (tuple(x.repeat_interleave(group, 0) for x in parts(c[b][:, :n], dim)) for c in (kc, vc))
+        qb = q[b].double().cpu()
+        s = torch.einsum("hd,hnd->hn", qb, kz + ks * kn) * scale
+        w = torch.softmax(s, 1)
+        want = torch.einsum("hn,hnd->hd", w, vz + vs * vn)
+        a = torch.einsum("hn,hnd->hd", w, vz.abs() + (vs * vn).abs())
+        u = torch.einsum("hn,hnd->hd", w, vz.abs() + vs * 2 ** bits)
+        ds = dim * 2.0 ** -24 * torch.einsum("hd,hnd->hn", qb.abs(), kz.abs() + ks * 2 ** bits).amax(1, keepdim=True) * abs(scale) + s.abs().amax(1, keepdim=True) * 2.0 ** -23
+        steps = (n / 16 + 2) * 2.0 ** -23
+        tol = eps / 2 * want.abs() + 2.0 ** -11 * 1.001 * a + u * (2 * ds + 2 * steps + 2.0 ** -21) + n * 2.0 ** -32 * (vz.abs() + vs * 2 ** bits).amax()
+        err = (out[b] - want).abs()
+        assert bool((err <= tol).all()), (b, float((err / tol).max()))
+        want_lse = torch.logsumexp(s, 1)
+        err = (lse[b] - want_lse).abs()
+        assert bool((err <= ds[:, 0] + 2.0 ** -22 * (1 + want_lse.abs()) + steps).all()), (b, float(err.max()))
+
+
+def attention_inputs(seqs, q_heads, kv_heads, dim, bits, rows, dtype="fp16", seed=0, gain=1.0):
+    k, v, q = made(seqs, kv_heads, rows, dim, seed=seed), made(seqs, kv_heads, rows, dim, seed=seed + 1, gain=0.5), made(seqs, q_heads, dim, dtype=dtype, seed=seed + 2, gain=gain)
+    return q, packed(k, bits).cuda(), packed(v, bits).cuda()
+
+
+# ------------------------------------------------------------------------------------------------------------- refusals (no device)
+def cache_args(C, **change):
+    n = change.get("num_sequences", 2)
+    one = (ctypes.c_void_p * max(n, 1))(*[4096] * max(n, 1))
+    a = dict(bits=4, head_dim=128, num_sequences=2, kv_heads=8, rows=16, k=ctypes.addressof(one), v=ctypes.addressof(one), seq_stride=0, head_stride=1280, row_stride=80)
+    a.update(change)
+    cache = C._PackedCache(**a)
+    cache.keep = one
+    return cache
+
+
+def row_args(C, **change):
+    a = dict(type=0, rows=4, k=4096, v=4096, seq_stride=4096, head_stride=512, row_stride=128, start=0)
+    a.update(change)
+    return C._PackedRows(**a)
+
+
+def attention_args(C, **change):
+    a = dict(type=0, q_heads=16, q=4096, q_seq_stride=2048, q_head_stride=128, lens=4096, scale=1.0, out=4096, workspace=4096, workspace_bytes=1 << 30)
+    a.update(change)
+    return C._PackedAttention(**a)
+
+
+def call(C, name, *args):
+    return getattr(C._lib, name)(*[None if a is None else bytes(a) for a in args], None), C._lib.qmk_last_error()
+
+
+CACHE_FAULTS = [(dict(bits=5), b"bits"), (dict(head_dim=96), b"head_dim"), (dict(num_sequences=0), b"num_sequences"), (dict(num_sequences=129), b"num_sequences"),
+                (dict(kv_heads=0), b"kv_heads"), (dict(kv_heads=1025), b"kv_heads"), (dict(rows=-1), b"rows"), (dict(rows=(1 << 24) + 1), b"rows"),
+                (dict(k=None), b"null"), (dict(v=None), b"null"), (dict(k=None, k_base=4096), b"null"), (dict(head_stride=1288), b"strides"), (dict(row_stride=84), b"strides"),
+                (dict(row_stride=64), b"overlap"), (dict(row_stride=0), b"overlap"), (dict(k=None, k_base=4104, v_base=4096), b"multiple of 16"),
+                (dict(k=None, k_base=4096, v_base=4096, seq_stride=8), b"strides")]
+
+
+@pytest.mark.parametrize("change,text", CACHE_FAULTS)
+def test_caches_are_refused_before_anything_runs(C, change, text):
+    cache = cache_args(C, **change)
+    for name, args in (("qmk_write_cache_packed", row_args(C)), ("qmk_read_cache_packed", row_args(C)), ("qmk_attention_packed_cache", attention_args(C))):
+        rc, why = call(C, name, cache, args)
+        assert rc == 2 and text in why and name.encode() in why, (name, why)
+
+
+@pytest.mark.parametrize("change,text", [(dict(type=2), b"type"), (dict(rows=-1), b"rows"), (dict(rows=(1 << 24) + 1), b"rows"), (dict(k=None), b"null"), (dict(v=None), b"null"),
+                                         (dict(k=4104), b"16"), (dict(seq_stride=4), b"strides"), (dict(head_stride=12), b"strides"), (dict(row_stride=130), b"strides")])
+@pytest.mark.parametrize("name", ["qmk_write_cache_packed", "qmk_read_cache_packed"])
+def test_rows_are_refused_before_anything_runs(C, name, change, text):
+    rc, why = call(C, name, cache_args(C), row_args(C, **change))
+    assert rc == 2 and text in why, why
+
+
+def test_more_rows_than_an_index_holds_are_refused(C):
+    rc, why = call(C, "qmk_write_cache_packed", cache_args(C, num_sequences=128), row_args(C, rows=1 << 21))
+    assert rc == 2 and b"2^31" in why
+
+
+@pytest.mark.parametrize("change,text", [(dict(type=2), b"type"), (dict(q_heads=12), b"q_heads"), (dict(q_heads=0), b"q_heads"), (dict(q_heads=136), b"q_heads"), (dict(q=None), b"null"),
+                                         (dict(out=None), b"null"), (dict(lens=None), b"null"), (dict(workspace=None), b"null"), (dict(workspace_bytes=4), b"workspace"),
+                                         (dict(scale=float("inf")), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(scale=3e38), b"scale"), (dict(q=4104), b"aligned"),
+                                         (dict(out=4104), b"aligned"), (dict(workspace=4104), b"aligned"), (dict(q_seq_stride=2052), b"strides"), (dict(q_head_stride=4), b"strides")])
+def test_attention_is_refused_before_anything_runs(C, change, text):
+    rc, why = call(C, "qmk_attention_packed_cache", cache_args(C), attention_args(C, **change))
+    assert rc == 2 and text in why, why
+
+
+def test_null_arguments_are_refused(C):
+    for name, args in (("qmk_write_cache_packed", row_args(C)), ("qmk_read_cache_packed", row_args(C)), ("qmk_attention_packed_cache", attention_args(C))):
+        assert call(C, name, None, args)[0] == 2 and call(C, name, cache_args(C), None)[0] == 2
+        holes = (ctypes.c_void_p * 2)(4096, None)
+        rc, why = call(C, name, cache_args(C, v=ctypes.addressof(holes)), args)
+        assert rc == 2 and b"null" in why
+
+
+def test_workspace_is_0_for_sizes_that_are_refused(C):
+    size = C._lib.qmk_attention_packed_cache_workspace
+    assert size(1, 16, 8, 128, 4, 100) > 0
+    for bad in ((0, 16, 8, 128, 4, 100), (129, 16, 8, 128, 4, 100), (1, 12, 8, 128, 4, 100), (1, 136, 8, 128, 4, 100), (1, 16, 0, 128, 4, 100), (1, 16, 8, 96, 4, 100),
+                (1, 16, 8, 128, 5, 100), (1, 16, 8, 128, 4, -1), (1, 16, 8, 128, 4, (1 << 24) + 1)):
+        assert size(*bad) == 0
+
+
+def test_packed_row_bytes(C):
+    assert [C.packed_row_bytes(d, b) for d, b in ((128, 4), (128, 8), (64, 4), (64, 8))] == [80, 144, 48, 80]
+    for bad in ((96, 4), (128, 5)):
+        with pytest.raises(RuntimeError):
+            C.packed_row_bytes(*bad)
+
+
+@pytest.mark.gpu
+def test_wrong_tensors_are_refused(gpu):
+    q, kc, vc = attention_inputs(2, 4, 2, 64, 4, 8)
+    k, v, lens = made(2, 2, 3, 64), made(2, 2, 3, 64), torch.tensor([1, 2], dtype=torch.int32).cuda()
+    for bad in ((q.float(), kc, vc, lens), (q[0], kc, vc, lens), (q.cpu(), kc, vc, lens), (q, kc[:1], vc, lens), (q, kc.cpu(), vc.cpu(), lens), (q, kc.view(torch.int8), vc.view(torch.int8), lens),
+                (q, kc[..., :40], vc[..., :40], lens), (q, kc, vc[:, :, :4], lens), (q, kc, vc, lens.long()), (q, kc, vc, lens[:1]), (q, kc, vc, lens.cpu()), (q, kc, vc, None),
+                (q, list(kc)[:1], list(vc), lens), (q[:, :3], kc, vc, lens), (q, [kc[0], kc[1].transpose(0, 1)], list(vc), lens), (made(2, 4, 96), kc, vc, lens),
+                (q, kc[:, :, :1].expand(-1, -1, 8, -1), vc[:, :, :1].expand(-1, -1, 8, -1), lens)):
+        with pytest.raises(RuntimeError):
+            gpu.attention_packed_cache(*bad)
+    for bad in ((k.float(), v.float(), kc, vc), (k[0], v[0], kc, vc), (k.cpu(), v.cpu(), kc, vc), (k, v.bfloat16(), kc, vc), (k, v[:1], kc, vc), (k[:, :1], v[:, :1], kc, vc),
+                (k, v.transpose(1, 2).contiguous().transpose(1, 2), kc, vc), (k[..., ::2], v[..., ::2], kc, vc), (k, v, kc.cpu(), vc.cpu()), (k, v, kc, vc, lens.long()),
+                (k, v, kc, vc, 2 ** 31), (k, v, kc, vc, 0, lens.cpu()), (k, v, kc, vc, 1.5), (k[:1], v[:1], kc, vc)):
+        with pytest.raises(RuntimeError):
+            gpu.write_cache_packed(*bad)
+    for bad, named in (((kc, vc, 3, 96), {}), ((kc, vc, -1, 64), {}), ((kc, vc, 3, 64, torch.float32), {}), ((kc, vc, 3, 128), {}), ((kc.cpu(), vc.cpu(), 3, 64), {}),
+                       ((kc, vc, 3, 64), dict(k_out=k)), ((kc, vc, 3, 64), dict(k_out=k, v_out=v.bfloat16())), ((kc, vc, 4, 64), dict(k_out=k, v_out=v)),
+                       ((kc, vc, 3, 64), dict(k_out=k, v_out=v.transpose(1, 2).contiguous().transpose(1, 2)))):
+        with pytest.raises(RuntimeError):
+            gpu.read_cache_packed(*bad, **named)
+
+
+# ------------------------------------------------------------------------------------------------------------- rows in and out
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("dim,bits", [(64, 4), (64, 8), (128, 4), (128, 8)])
+@pytest.mark.parametrize("seqs,heads,rows,cache", [(1, 1, 1, 1), (1, 8, 1, 40), (3, 2, 33, 50), (128, 8, 1, 5), (2, 5, 257, 300), (7, 3, 31, 31)])
+def test_rows_become_their_codes_and_read_back(gpu, dtype, dim, bits, seqs, heads, rows, cache):
+    """Rows of a projection's output (heads behind rows), at a start for each sequence, some sequences with fewer; everything else stays."""
+    k, v = (made(seqs, rows, heads, dim, dtype=dtype, seed=seqs + i, gain=3.0).transpose(1, 2) for i in (0, 1))
+    starts = torch.tensor([(5 * b) % (cache - rows + 1) for b in range(seqs)], dtype=torch.int32)
+    lens = torch.tensor([rows if b % 3 != 1 else rows // 2 for b in range(seqs)], dtype=torch.int32)
+    size = gpu.packed_row_bytes(dim, bits)
+    kc, vc = (torch.randint(0, 256, (seqs, heads, cache, size), dtype=torch.uint8, generator=torch.Generator().manual_seed(9 + i)).cuda() for i in (0, 1))
+    want = [c.cpu().clone() for c in (kc, vc)]
+    for c, x in zip(want, (k, v)):
+        new = packed(x, bits)
+        for b in range(seqs):
+            n, at = int(lens[b]), int(starts[b])
+            c[b, :, at:at + n] = new[b, :, :n]
+    gpu.write_cache_packed(k, v, kc, vc, starts.cuda(), lens.cuda())
+    assert torch.equal(kc.cpu(), want[0]) and torch.equal(vc.cpu(), want[1])
+    back = gpu.read_cache_packed(kc, vc, rows, dim, DTYPES[dtype], starts.cuda(), lens.cuda())
+    for x, c in zip(back, want):
+        assert x.dtype == DTYPES[dtype] and tuple(x.shape) == (seqs, heads, rows, dim)
+        for b in range(seqs):
+            n, at = int(lens[b]), int(starts[b])
+            exact = values(c[b, :, at:at + n], dim)
+            assert bool(((x[b, :, :n].double().cpu() - exact).abs() <= rounded_off(exact, DTYPES[dtype])).all())
+            assert bool((x[b, :, n:] == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_values_that_quantise_badly(gpu, dtype, bits):
+    """Constant quarters, values on the border of two codes, one far value, the smallest and largest ones, offsets, values that are no numbers."""
+    x = torch.zeros(1, 1, 40, 128)
+    x[0, 0, 1] = 7.25
+    x[0, 0, 2] = torch.arange(128) % 32 * 0.5                                  # many quotients end in a half
+    x[0, 0, 3, ::32] = 60000.0
+    x[0, 0, 4] = torch.linspace(-65504, 65504, 128)
+    x[0, 0, 5] = torch.arange(128) * 2.0 ** -24
+    x[0, 0, 6] = 1000 + torch.arange(128) % 3
+    x[0, 0, 7, 5], x[0, 0, 8, 40], x[0, 0, 9, 127] = math.nan, math.inf, -math.inf
+    x[0, 0, 10] = 1e5                                                          # (infinite in fp16, too large for a scale in bf16)
+    x[0, 0, 11] = -(2.0 ** -20) * (torch.arange(128) + 1)
+    x[0, 0, 12:] = torch.randint(-8, 9, (28, 128), generator=torch.Generator().manual_seed(1)) / 8
+    x[0, 0, 20:] += torch.randint(0, 2, (20, 128), generator=torch.Generator().manual_seed(2)) * 2.0 ** -12
+    x[0, 0, 30:] *= 1024
+    x = x.to(DTYPES[dtype]).cuda()
+    kc, vc = (torch.zeros(1, 1, 40, gpu.packed_row_bytes(128, bits), dtype=torch.uint8, device="cuda") for _ in range(2))
+    gpu.write_cache_packed(x, -x, kc, vc)
+    for got, rows in ((kc, x), (vc, -x)):
+        want, got = packed(rows, bits), got.cpu()
+        bad = torch.isnan(values(want, 128))
+        assert bool((got[..., -16:] == want[..., -16:]).all())
+        # rows 7 to 9 a quarter each, row 10 all four; in bf16 the ends of row 4 are 65536 (65504 lies between 65280 and that): two quarters more
+        assert bool(((values(got, 128) == values(want, 128)) | bad).all()) and int(bad.sum()) == 3 * 32 + 128 + (64 if dtype == "bf16" else 0)
+    k, _ = gpu.read_cache_packed(kc, vc, 40, 128, DTYPES[dtype])
+    assert torch.equal(torch.isnan(k.cpu()), torch.isnan(values(packed(x, bits), 128)))
+    exact = values(packed(x, bits), 128)
+    assert bool(((k.double().cpu() - exact).abs() <= rounded_off(exact, DTYPES[dtype])).nan_to_num(0).logical_or(torch.isnan(exact)).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+def test_rows_outside_the_caches(gpu, bits):
+    """Starts in front of a cache and behind it, lengths below 0 and above the rows that are there."""
+    heads, rows, cache = 2, 9, 12
+    starts = torch.tensor([-4, 8, 100, -100, 2 ** 31 - 1, -2 ** 31, 0], dtype=torch.int32)
+    lens = torch.tensor([9, 9, 9, 9, 9, 9, -3], dtype=torch.int32)
+    k, v = made(7, heads, rows, 64, seed=1), made(7, heads, rows, 64, seed=2)
+    kc, vc = (torch.full((7, heads, cache, gpu.packed_row_bytes(64, bits)), 170, dtype=torch.uint8, device="cuda") for _ in range(2))
+    gpu.write_cache_packed(k, v, kc, vc, starts.cuda(), lens.cuda())
+    want = torch.full(kc.shape, 170, dtype=torch.uint8)
+    want[0, :, :5] = packed(k[0, :, 4:], bits)
+    want[1, :, 8:] = packed(k[1, :, :4], bits)
+    assert torch.equal(kc.cpu(), want)
+    k2, v2 = gpu.read_cache_packed(kc, vc, rows, 64, starts=starts.cuda(), lens=lens.cuda())
+    assert bool((k2[0, :, :4] == 0).all()) and bool((k2[1, :, 4:] == 0).all()) and bool((k2[2:] == 0).all()) and bool((v2[2:] == 0).all())
+    assert bool((k2[0, :, 4:] != 0).any()) and bool((k2[1, :, :4] != 0).any())
+    gpu.write_cache_packed(k, v, kc, vc, 3, torch.full((7,), 100, dtype=torch.int32).cuda())
+    assert torch.equal(kc[:, :, 3:].cpu(), packed(k, bits)) and torch.equal(vc[:, :, 3:].cpu(), packed(v, bits)) and torch.equal(kc[:, :, :3].cpu(), want[:, :, :3])
+
+
+@pytest.mark.gpu
+def test_lists_of_caches_strides_and_no_rows(gpu):
+    """Layers of caches that belong to different sequences, rows and outputs that are views; nothing to do is nothing done."""
+    big = torch.zeros(3, 4, 2, 20, 2, 80, dtype=torch.uint8, device="cuda")               # [sequence, layer, head, row, k / v, bytes]
+    kc, vc = [big[b, 1, :, :, 0] for b in (2, 0, 1)], [big[b, 1, :, :, 1] for b in (2, 0, 1)]
+    k, v = made(3, 6, 4, 128, seed=3)[:, :5, 1:3].transpose(1, 2), made(3, 6, 4, 128, seed=4)[:, :5, 1:3].transpose(1, 2)
+    gpu.write_cache_packed(k, v, kc, vc, 7)
+    for i, b in enumerate((2, 0, 1)):
+        assert torch.equal(big[b, 1, :, 7:12, 0].cpu(), packed(k[i], 4)) and torch.equal(big[b, 1, :, 7:12, 1].cpu(), packed(v[i], 4))
+    assert int((big != 0).sum()) == int((big[:, 1, :, 7:12] != 0).sum())
+    outs = [torch.full((2, 3, 9, 128), 5.0, dtype=torch.float16, device="cuda").transpose(0, 1) for _ in range(2)]
+    got = gpu.read_cache_packed(kc, vc, 5, 128, starts=7, k_out=outs[0][:, :, 2:7], v_out=outs[1][:, :, 2:7])
+    want = gpu.read_cache_packed(kc, vc, 5, 128, starts=7)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and bool((outs[0][:, :, :2] == 5).all()) and bool((outs[0][:, :, 7:] == 5).all())
+    before = big.clone()
+    gpu.write_cache_packed(k[:, :, :0], v[:, :, :0], kc, vc, 7)
+    assert torch.equal(before, big) and gpu.read_cache_packed(kc, vc, 0, 128)[0].shape == (3, 2, 0, 128)
+
+
+# ------------------------------------------------------------------------------------------------------------- attention
+HEADS = [(16, 8), (4, 4), (6, 2), (8, 1), (16, 1), (9, 1), (32, 4)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("dim,bits", [(64, 4), (64, 8), (128, 4), (128, 8)])
+@pytest.mark.parametrize("q_heads,kv_heads", HEADS)
+@pytest.mark.parametrize("seqs,rows", [(1, 1), (1, 17), (2, 64), (3, 333), (19, 65)])
+def test_attention_matches_the_definition(gpu, dtype, dim, bits, q_heads, kv_heads, seqs, rows):
+    q, kc, vc = attention_inputs(seqs, q_heads, kv_heads, dim, bits, rows, dtype, seed=seqs + rows)
+    lens = torch.tensor([rows * (i + 1) // seqs if i % 5 != 1 else 0 for i in range(seqs)], dtype=torch.int32)
+    check_attention(gpu.attention_packed_cache(q, kc, vc, lens.cuda()), q, kc, vc, lens)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("seqs,q_heads,kv_heads,rows", [(1, 16, 8, 20000), (128, 16, 8, 300), (40, 32, 2, 1500), (3, 8, 8, 5001)])
+def test_long_caches_and_full_batches(gpu, bits, seqs, q_heads, kv_heads, rows):
+    q, kc, vc = attention_inputs(seqs, q_heads, kv_heads, 128, bits, rows, seed=rows, gain=1.5)
+    lens = torch.tensor([rows if seqs == 1 else (7919 * (i + 1)) % (rows + 1) for i in range(seqs)], dtype=torch.int32)
+    check_attention(gpu.attention_packed_cache(q, kc, vc, lens.cuda()), q, kc, vc, lens)
+
+
+@pytest.mark.gpu
+def test_no_rows_and_lengths_outside_the_cache(gpu):
+    q, kc, vc = attention_inputs(4, 4, 2, 64, 4, 30)
+    for lens in ([0, 0, 0, 0], [-5, 1000, 2 ** 31 - 1, -2 ** 31]):
+        check_attention(gpu.attention_packed_cache(q, kc, vc, torch.tensor(lens, dtype=torch.int32).cuda()), q, kc, vc, lens)
+    out, lse = gpu.attention_packed_cache(q, kc[:, :, :0], vc[:, :, :0], torch.tensor([3, 0, 0, 1], dtype=torch.int32).cuda())
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_rows_behind_the_last_are_not_looked_at(gpu, dim, bits):
+    """Whatever bytes they hold, NaN in their trailers among them."""
+    q, kc, vc = attention_inputs(3, 8, 2, dim, bits, 200)
+    lens = torch.tensor([1, 77, 130], dtype=torch.int32)
+    want = gpu.attention_packed_cache(q, kc, vc, lens.cuda())
+    for c in (kc, vc):
+        for b in range(3):
+            c[b, :, int(lens[b]):] = 255
+    got = gpu.attention_packed_cache(q, kc, vc, lens.cuda())
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+def test_visible_rows_that_are_no_numbers(gpu, bits):
+    """A key without numbers leaves none in its head's outputs, a value in its quarter's; the other heads and sequences keep theirs."""
+    q, kc, vc = attention_inputs(2, 8, 4, 128, bits, 100)
+    lens = torch.tensor([100, 90], dtype=torch.int32).cuda()
+    want = gpu.attention_packed_cache(q, kc, vc, lens)
+    k, v = gpu.read_cache_packed(kc, vc, 100, 128)
+    k[0, 1, 50, 3] = math.nan
+    v[1, 2, 7, 40] = math.inf
+    v[1, 3, 95, 0] = math.nan                                                  # (behind the last row)
+    kc2, vc2 = kc.clone(), vc.clone()
+    gpu.write_cache_packed(k[:1, :, 50:51], v[:1, :, 50:51], kc2[:1], vc2[:1], 50)
+    gpu.write_cache_packed(k[1:, :, 7:8], v[1:, :, 7:8], kc2[1:], vc2[1:], 7)
+    gpu.write_cache_packed(k[1:, :, 95:96], v[1:, :, 95:96], kc2[1:], vc2[1:], 95)
+    kc2[0, 0], kc2[0, 2:], vc2[0] = kc[0, 0], kc[0, 2:], vc[0]                # (read back and written again: not always the same codes)
+    kc2[1], vc2[1, :2], vc2[1, 3, :95] = kc[1], vc[1, :2], vc[1, 3, :95]
+    out, lse = gpu.attention_packed_cache(q, kc2, vc2, lens)
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[0, 2:4] = True
+    bad[1, 4:6, 32:64] = True
+    assert torch.equal(torch.isnan(out), bad) and torch.equal(torch.isnan(lse), bad.all(2))
+    other = ~bad
+    other[1, 4:6] = False
+    assert torch.equal(out[other], want[0][other]) and torch.equal(lse[~bad.all(2)], want[1][~bad.all(2)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_sizes_of_values_and_scores(gpu, dtype, bits):
+    """Values from 2^-12 to 2^12 in quarters side by side and in rows behind one another, scores that rise and fall by hundreds, negative and zero scales."""
+    seqs, rows = 3, 300
+    k, q = made(seqs, 2, rows, 128, seed=5), made(seqs, 4, 128, dtype=dtype, seed=6, gain=8.0)
+    v = made(seqs, 2, rows, 128, seed=7).float()
+    v *= 2.0 ** torch.linspace(-12, 12, 4).repeat_interleave(32).cuda()
+    v[1] *= 2.0 ** torch.linspace(0, -12, rows).cuda()[:, None]
+    v[2] = v[2].flip(1) * 2.0 ** torch.linspace(-3, 0, rows).cuda()[:, None]
+    kc, vc = packed(k, bits).cuda(), packed(v.half(), bits).cuda()
+    lens = torch.tensor([300, 299, 170], dtype=torch.int32)
+    for scale in (None, 3.0, -0.5, 0.0, 1e-30):
+        check_attention(gpu.attention_packed_cache(q, kc, vc, lens.cuda(), scale=scale), q, kc, vc, lens, scale)
+
+
+@pytest.mark.gpu
+def test_queries_of_any_size(gpu):
+    """Queries at both ends of their types, and tiny ones beside them."""
+    _, kc, vc = attention_inputs(1, 4, 2, 128, 4, 50)
+    lens = torch.tensor([50], dtype=torch.int32)
+    for dtype, sizes in ((torch.float16, (6e4, 2.0 ** -14, 2.0 ** -24)), (torch.bfloat16, (1e30, 6e4, 1e-30, 2.0 ** -133))):
+        for size in sizes:
+            q = (made(1, 4, 128, seed=3).float().clamp(-1, 1) * size).to(dtype)
+            q[0, 0, 0], q[0, 1, 5] = 0.0, size / 2 ** 12
+            scale = 0.1 / max(size, 1e-30) if size > 1e-4 else 1e10
+            check_attention(gpu.attention_packed_cache(q, kc, vc, lens.cuda(), scale=scale), q, kc, vc, lens, scale)
+    zero = torch.zeros(1, 4, 128, dtype=torch.float16, device="cuda")
+    check_attention(gpu.attention_packed_cache(zero, kc, vc, lens.cuda()), zero, kc, vc, lens)
+
+
+@pytest.mark.gpu
+def test_lists_views_and_strides(gpu):
+    q, kc, vc = attention_inputs(5, 8, 2, 128, 8, 70)
+    lens = torch.tensor([70, 1, 0, 33, 64], dtype=torch.int32)
+    want = gpu.attention_packed_cache(q, kc, vc, lens.cuda())
+    again = gpu.attention_packed_cache(q, list(kc), list(vc), lens.cuda())
+    assert torch.equal(want[0], again[0]) and torch.equal(want[1], again[1])
+    both = torch.stack((kc, vc), 3).transpose(1, 2).contiguous().transpose(1, 2)           # [sequence, row, head, k / v, bytes] in memory
+    qv = torch.cat((q, q), 2).view(5, 8, 256)[:, :, 128:]
+    again = gpu.attention_packed_cache(qv, both[:, :, :, 0], both[:, :, :, 1], lens.cuda())
+    assert torch.equal(want[0], again[0]) and torch.equal(want[1], again[1])
+    same = gpu.attention_packed_cache(q, kc[:1].expand(5, -1, -1, -1), vc[:1].expand(5, -1, -1, -1), lens.cuda())      # one cache for all
+    check_attention(same, q, [kc[0]] * 5, [vc[0]] * 5, lens)
+
+
+@pytest.mark.gpu
+def test_results_do_not_depend_on_the_run_or_the_other_sequences(gpu):
+    q, kc, vc = attention_inputs(33, 16, 8, 128, 4, 700)
+    lens = torch.tensor([(131 * i) % 701 for i in range(33)], dtype=torch.int32).cuda()
+    first = gpu.attention_packed_cache(q, kc, vc, lens)
+    for _ in range(5):
+        again = gpu.attention_packed_cache(q, kc, vc, lens)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+# ------------------------------------------------------------------------------------------------------------- together
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+def test_prompt_then_steps_in_a_captured_graph(gpu, bits):
+    """A prompt's rows written, then decode steps - the new rows written, the attention over everything so far - replayed from one graph, on a stream of
+    their own, with positions that move on the device."""
+    seqs, q_heads, kv_heads, dim, room, prompt = 3, 16, 8, 128, 64, 30
+    kc, vc = (torch.zeros(seqs, kv_heads, room, gpu.packed_row_bytes(dim, bits), dtype=torch.uint8, device="cuda") for _ in range(2))
+    k, v = made(seqs, kv_heads, room, dim, seed=1), made(seqs, kv_heads, room, dim, seed=2)
+    lens = torch.tensor([30, 7, 0], dtype=torch.int32)
+    gpu.write_cache_packed(k[:, :, :prompt], v[:, :, :prompt], kc, vc, 0, lens.cuda())
+    at = lens.cuda()
+    qs = made(10, seqs, q_heads, dim, seed=3)
+    q, kn, vn = torch.empty_like(qs[0]), torch.empty(seqs, kv_heads, 1, dim, dtype=torch.float16, device="cuda"), torch.empty(seqs, kv_heads, 1, dim, dtype=torch.float16, device="cuda")
+    gpu.attention_packed_cache(qs[0], kc, vc, at)
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=stream):
+        gpu.write_cache_packed(kn, vn, kc, vc, at)
+        after = at + 1
+        out, lse = gpu.attention_packed_cache(q, kc, vc, after)
+        at.copy_(after)
+    for step in range(10):
+        rows = [int(lens[b]) + step for b in range(seqs)]
+        q.copy_(qs[step])
+        for b in range(seqs):
+            kn[b, :, 0].copy_(k[b, :, rows[b]])
+            vn[b, :, 0].copy_(v[b, :, rows[b]])
+        graph.replay()
+        torch.cuda.synchronize()
+        check_attention((out, lse), q, packed(k, bits), packed(v, bits), [r + 1 for r in rows])
+    back, _ = gpu.read_cache_packed(kc, vc, room, dim)
+    for b in range(seqs):
+        n = int(lens[b]) + 10
+        exact = values(packed(k[b, :, :n], bits), dim)
+        assert bool(((back[b, :, :n].double().cpu() - exact).abs() <= rounded_off(exact, torch.float16)).all())
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(gpu):
+    cases = [attention_inputs(9, 16, 8, 128, 4, 500, seed=s) for s in (1, 2)]
+    lens = torch.tensor([500 - 50 * i for i in range(9)], dtype=torch.int32).cuda()
+    want = [gpu.attention_packed_cache(*c, lens) for c in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(gpu.attention_packed_cache(*cases[i], lens))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert all(torch.equal(o, want[i][0]) and torch.equal(e, want[i][1]) for o, e in got[i])
