@@ -7,6 +7,7 @@
 #include "engine_internal.h"
 #include "packed_attention.cuh"
 #include "packed_cache.cuh"
+#include "prefill_sm100.h"
 
 namespace {
 
@@ -95,11 +96,29 @@ int rows_call(const char *who, const qmk_packed_cache *cache, const qmk_packed_r
   return answer(who, cudaGetLastError());
 }
 
-template <typename T, int DIM, int BITS>
-cudaError_t attend(const AttendParams &p, cudaStream_t stream) {
-  attend_rows<T, DIM, BITS><<<p.caches.seqs * p.q_heads, 128, 0, stream>>>(p);
-  return cudaGetLastError();
+// Stretches of a call: a warp each, all resident together, not more than there can be tiles.
+long long most_tiles(int seqs, int kv_heads, int rows) { return static_cast<long long>(seqs) * kv_heads * ((rows + TILE - 1) / TILE); }
+int blocks_of(int group) { return group > 8 ? 2 : 1; }                    // of eight query heads
+int warps_of(int seqs, int kv_heads, int group, int rows) {
+  return static_cast<int>(std::min<long long>(std::max(most_tiles(seqs, kv_heads, rows), 1ll), SMS * ctas_per_sm(blocks_of(group)) * WARPS));
 }
+long long workspace_bytes(int warps, int group, int dim) { return 2ll * warps * group * (dim * 4ll + 8); }
+
+template <typename T, int DIM, int BITS, int NT>
+cudaError_t attend(const AttendParams &p, cudaStream_t stream) {
+  using A = Attend<T, DIM, BITS, NT>;
+  cudaError_t e = cudaSuccess;
+  if (p.caches.rows > 0) {
+    e = cudaFuncSetAttribute(attend_tiles<T, DIM, BITS, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, A::SMEM);
+    const int ctas = std::min(p.warps, SMS * ctas_per_sm(NT));           // (a warp of each where there are few)
+    if (e == cudaSuccess) e = qmk_tc::launch_kernel(attend_tiles<T, DIM, BITS, NT>, dim3(ctas), dim3(WARPS * 32), A::SMEM, stream, p);
+  }
+  if (e != cudaSuccess) return e;
+  const qmk_tc::PdlScope scope(true);
+  return qmk_tc::launch_kernel(join_stretches<T, DIM>, dim3(p.caches.seqs * p.q_heads), dim3(JOIN_WARPS * 32), 0, stream, p);
+}
+template <typename T, int DIM, int BITS>
+cudaError_t attend(const AttendParams &p, cudaStream_t stream) { return blocks_of(p.group) == 2 ? attend<T, DIM, BITS, 2>(p, stream) : attend<T, DIM, BITS, 1>(p, stream); }
 template <typename T>
 cudaError_t attend(const AttendParams &p, int dim, int bits, cudaStream_t stream) {
   if (bits == 4) return dim == 64 ? attend<T, 64, 4>(p, stream) : attend<T, 128, 4>(p, stream);
@@ -119,7 +138,8 @@ extern "C" long long qmk_attention_packed_cache_workspace(int num_sequences, int
   if (num_sequences < 1 || num_sequences > MAX_SEQS || kv_heads < 1 || kv_heads > MAX_HEADS || q_heads < 1 || q_heads % kv_heads || q_heads / kv_heads > MAX_GROUP ||
       (head_dim != 64 && head_dim != 128) || (bits != 4 && bits != 8) || rows < 0 || rows > MAX_ROWS)
     return 0;
-  return 16;
+  if (most_tiles(num_sequences, kv_heads, rows) > 0x7fffffffll) return 0;
+  return workspace_bytes(warps_of(num_sequences, kv_heads, q_heads / kv_heads, rows), q_heads / kv_heads, head_dim);
 }
 
 extern "C" int qmk_attention_packed_cache(const qmk_packed_cache *cache, const qmk_packed_attention *a, cudaStream_t stream) {
@@ -130,6 +150,7 @@ extern "C" int qmk_attention_packed_cache(const qmk_packed_cache *cache, const q
   if (!a || !a->q || !a->out || !a->lens || !a->workspace) return refuse(who, "null pointer argument");
   if (a->type < 0 || a->type > 1) return refuse(who, "the type is fp16 (0) or bf16 (1)");
   if (a->q_heads < 1 || a->q_heads % cache->kv_heads || a->q_heads / cache->kv_heads > MAX_GROUP) return refuse(who, "q_heads must be 1 to 16 times kv_heads");
+  if (most_tiles(cache->num_sequences, cache->kv_heads, cache->rows) > 0x7fffffffll) return refuse(who, "2^36 rows of all heads or more");
   if (!(a->scale > -2.0e38f && a->scale < 2.0e38f)) return refuse(who, "the scale must be finite, and below 2e38");   // (times log2 e too)
   if (odd(a->q) || odd(a->out) || odd(a->workspace)) return refuse(who, "pointers must be 16-byte aligned");
   if (odd(a->q_seq_stride, cache->num_sequences, 8) || odd(a->q_head_stride, a->q_heads, 8)) return refuse(who, "the queries' strides must be multiples of 8 elements");
@@ -142,6 +163,9 @@ extern "C" int qmk_attention_packed_cache(const qmk_packed_cache *cache, const q
   p.group = a->q_heads / cache->kv_heads;
   p.lens = a->lens;
   p.scale_log2 = a->scale * LOG2E;
+  p.warps = warps_of(cache->num_sequences, cache->kv_heads, p.group, cache->rows);
+  p.part_out = static_cast<float *>(a->workspace);
+  p.part_ml = reinterpret_cast<float2 *>(p.part_out + 2ll * p.warps * p.group * cache->head_dim);
   p.out = a->out;
   p.lse = a->lse;
   return answer(who, a->type == 0 ? attend<__half>(p, cache->head_dim, cache->bits, stream) : attend<__nv_bfloat16>(p, cache->head_dim, cache->bits, stream));
