@@ -31,6 +31,7 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // Weights are 2^SHIFT at the row's maximum, up to 2^(SHIFT + SLACK) where that has risen since it was last looked at: fp16 has 11 bits of them down to 2^-21 of
 // the largest.
 constexpr float SHIFT = 7.0f, SLACK = 8.0f;
+constexpr float NOTHING = 3.0e38f;               // in the exponent while no score has been seen: the first one rises, -inf stays that
 
 struct AttendParams {
   Caches caches;
@@ -51,6 +52,7 @@ __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;"
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there) {         // zeros where there is no row
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -59,10 +61,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
-}
-__device__ __forceinline__ void mma_k8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
-  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%7, %7, %7, %7};"
-               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(b0), "f"(0.0f));
 }
 __device__ __forceinline__ uint32_t pack2(float a, float b) { return bits_of(__floats2half2_rn(a, b)); }
 __device__ __forceinline__ __half2 h2(uint32_t x) { return from_bits<__half2>(x); }
@@ -78,11 +76,18 @@ template <int N> __device__ __forceinline__ void lds(uint32_t at, uint32_t (&w)[
   else if constexpr (N == 2) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
   else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(at) : "memory");
 }
-__device__ __forceinline__ uint32_t lds16(uint32_t at) {
-  unsigned short h;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(at) : "memory");
-  return h;
+// The trailers of 16 rows as 8 x 8 tiles that make an operand of a product: row g's entries 2 t and 2 t + 1 and row g + 8's, twice; transposed: entry g of rows
+// 2 t and 2 t + 1, twice, and of rows 2 t + 8 and 2 t + 9, twice.
+template <bool TRANSPOSED, int ROW> __device__ __forceinline__ void trailers(uint32_t first, int lane, uint32_t (&w)[4]) {
+  if constexpr (TRANSPOSED) {
+    const uint32_t at = first + ((lane & 7) + (lane >> 4) * 8) * ROW;
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+  } else {
+    const uint32_t at = first + (lane & 15) * ROW;
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+  }
 }
+constexpr uint32_t ONES = 0x3c003c00u;           // (1, 1)
 
 // Codes of quarter b of two chunks (DIM/8 codes each), the first in the lower halves: x[j] = (a_j, b_j) as fp16 numbers of 2^-24, of 4-bit codes every second of
 // 2^-20.
@@ -168,35 +173,43 @@ struct Place {
   }
 };
 
-template <typename T, int DIM, int BITS, int NT>
-struct Attend {
+// DIM/32 values of a row side by side
+template <int DIM> __device__ __forceinline__ void store_part(float *to, const float (&v)[DIM / 32]) {
+  if constexpr (DIM == 128) *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[DIM / 32 - 2], v[DIM / 32 - 1]);
+  else *reinterpret_cast<float2 *>(to) = make_float2(v[0], v[1]);
+}
+template <typename T, int DIM> __device__ __forceinline__ void store_out(T *to, const float (&v)[DIM / 32], float by) {
+  T o[DIM / 32];
+#pragma unroll
+  for (int j = 0; j < DIM / 32; ++j) o[j] = static_cast<T>(v[j] * by);
+  if constexpr (DIM == 128) *reinterpret_cast<uint2 *>(to) = make_uint2(*reinterpret_cast<const uint32_t *>(o), *reinterpret_cast<const uint32_t *>(o + DIM / 32 - 2));
+  else *reinterpret_cast<uint32_t *>(to) = *reinterpret_cast<const uint32_t *>(o);
+}
+
+// What both ways to take a tile below have in common.
+template <int DIM, int BITS, int BLOCKS>
+struct Tiles {
   static constexpr int ROW = ROW_BYTES<DIM, BITS>, CODES = ROW - TRAILER, PIECES = ROW / 16;
   static constexpr int CHUNK = CODES / 8, N = CHUNK / 4, J = DIM / 32, STEPS = J / 2;       // bytes and words of a chunk; codes of a quarter in it; k steps of a quarter
   static constexpr int STAGE = 2 * TILE * ROW;                                              // keys, then values
-  static constexpr int STAGES = stages(NT, ROW), SMEM = WARPS * STAGES * STAGE;
+  static constexpr int STAGES = stages(BLOCKS, ROW), SMEM = WARPS * STAGES * STAGE;
   static constexpr float M = 1 << (BITS - 1), UNIT = 0x1p-24f;
   static constexpr bool SPREAD = BITS == 8 && DIM == 128;                                   // a lane's two chunks of keys: four apart, or one behind the other
-
-  uint32_t qb[NT][4][STEPS][2], qz[NT];          // queries; sums over quarters, as upper and lower fp16 parts
-  float start[NT][4][2], factor[NT][2];          // -M Q_b, and scale * log2 e over the queries' power of two, of heads 2 t and 2 t + 1
-  float acc[NT][4][STEPS][4], zacc[NT][4], m[NT][2], l[NT][2];
-  __half2 f01, f23;                              // powers of two that take the quarters' scales of values to 1 or below
+  static __device__ __forceinline__ int chunk_of(int t, int c) { return SPREAD ? t + 4 * c : 2 * t + c; }
 
   static __device__ __forceinline__ void load(const AttendParams &p, const Place &at, uint32_t dst, int lane) {
     const long long base = static_cast<long long>(at.head) * p.caches.head + static_cast<long long>(at.tile) * TILE * p.caches.row;
     const unsigned char *const k = p.caches.k[at.b] + base, *const v = p.caches.v[at.b] + base;
     const int pieces = min(at.rows - at.tile * TILE, TILE) * PIECES;
-    if (p.caches.row == ROW) {                   // rows right behind one another
+    if (p.caches.row == ROW && pieces == TILE * PIECES) {                   // rows right behind one another, all there
+      const unsigned char *const ks = k + lane * 16, *const vs = v + lane * 16;
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
-        const int piece = lane + 32 * i;
-        const bool there = piece < pieces;
-        const int off = there ? piece * 16 : 0;
-        copy16(dst + piece * 16, k + off, there);
-        copy16(dst + TILE * ROW + piece * 16, v + off, there);
+        copy16(dst + lane * 16 + 512 * i, ks + 512 * i);
+        copy16(dst + lane * 16 + TILE * ROW + 512 * i, vs + 512 * i);
       }
     } else {
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < PIECES; ++i) {
         const int piece = lane + 32 * i;
         const bool there = piece < pieces;
@@ -206,6 +219,291 @@ struct Attend {
       }
     }
   }
+  // The lane's two chunks of keys of row g
+  static __device__ __forceinline__ void keys(uint32_t row, int t, uint32_t (&w)[2][N]) {
+    if constexpr (SPREAD) {
+      lds<N>(row + t * CHUNK, w[0]);
+      lds<N>(row + (t + 4) * CHUNK, w[1]);
+    } else {
+      uint32_t both[2 * N];
+      lds<2 * N>(row + 2 * t * CHUNK, both);
+#pragma unroll
+      for (int i = 0; i < N; ++i) { w[0][i] = both[i]; w[1][i] = both[N + i]; }
+    }
+  }
+  // The power of two that queries of which the largest is `top` are multiplied with: to at most 2^TOP, so that M times the sum over a quarter stays in fp16; entries lose
+  // bits from 2^-26 of the largest on.
+  static constexpr int TOP = BITS == 4 ? 5 : 1;
+  static __device__ __forceinline__ int lift(float top) {
+    const int e = static_cast<int>(__float_as_uint(top) >> 23) - 126;      // top < 2^e
+    return top == 0.0f || top == INFINITY ? 0 : min(max(TOP - e, -126), 126);
+  }
+  // What a score is multiplied by (a factor of 0 would make no number of the scores of rows that are not there, -inf)
+  static __device__ __forceinline__ float factor_of(const AttendParams &p, int lifted) { return fmaxf(fabsf(p.scale_log2) * power2(-lifted) / UNIT, 0x1p-120f); }
+  // The power of two that takes a scale into (1/2, 1], at most `old`
+  static __device__ __forceinline__ float taken(float most, float old) {
+    const int e = static_cast<int>((__float_as_uint(fmaxf(most, 0.0f)) + 0x7fffffu) >> 23) - 127;
+    return fminf(old, power2(min(max(-e, -14), 15)));
+  }
+};
+
+// One or two query heads: each takes four of the eight columns, one for each quarter of the dimensions.  Keys: queries are zero outside their column's
+// quarter, so one product over all codes has the quarters' sums side by side, each is scaled once, and pairs of codes need not be of one quarter; values: the weights'
+// scales are the columns', one operand for all dimensions, of whose columns each quarter of the output keeps its own.
+template <typename T, int DIM, int BITS>
+struct AttendPair : Tiles<DIM, BITS, 1> {
+  using Base = Tiles<DIM, BITS, 1>;
+  using Base::ROW; using Base::CODES; using Base::N; using Base::J; using Base::STEPS; using Base::M; using Base::UNIT; using Base::CHUNK;
+  static constexpr bool LOWER = !Type<T>::BF16;            // whether weights have a lower part
+  static constexpr int PAIRS = 16 / BITS, KSTEPS = N * PAIRS;               // operand words of a word of codes; k steps of a row of keys
+  static constexpr int HEADS = 1;                          // of a thread's columns
+
+  uint32_t qb[KSTEPS][2], qz[2];                 // queries; sums over quarters, as upper and lower fp16 parts
+  float factor, m, off, l;                       // what a score is multiplied by, the largest score, what is added in the exponent, the sum of weights
+  float acc[4][STEPS][4], sums[4], zacc[4];      // out^T, quarter by quarter; sums of weights times scales; of weights times centres (lanes g >= 4: of quarter g - 4)
+  __half2 f;                                     // power of two that takes quarter g & 3's scales of values to 1 or below
+  uint32_t ones;
+
+  __device__ __forceinline__ void begin(const AttendParams &p, int b, int kv_head, int lane) {
+    const int t = lane & 3, g = lane >> 2, h = g >> 2, quarter = g & 3;
+    const bool live = h < p.group;
+    const T *const q = static_cast<const T *>(p.q) + b * p.q_seq + (kv_head * p.group + (live ? h : 0)) * p.q_head + DIM / 4 * quarter;
+    float x[2][J], top = 0.0f;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        x[c][j] = live ? static_cast<float>(q[DIM / 32 * Base::chunk_of(t, c) + j]) : 0.0f;
+        top = fmaxf(top, fabsf(x[c][j]));
+      }
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const int up = Base::lift(top);
+    const float by = copysignf(power2(up), p.scale_log2);
+    float sum = 0.0f;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int j = 0; j < J; ++j) { x[c][j] *= by; sum += x[c][j]; }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    // operand word i of the row: codes PAIRS / 2 ... of a word, the lower and the upper half's
+#pragma unroll
+    for (int i = 0; i < 2 * KSTEPS; ++i) {
+      const int c = i / KSTEPS, low = i % KSTEPS / PAIRS * (2 * PAIRS) + i % PAIRS, high = low + PAIRS;
+      const float unit = BITS == 4 && i % 2 ? 0.0625f : 1.0f;
+      qb[i / 2][i % 2] = pack2(quarter == low / J ? x[c][low % J] * unit : 0.0f, quarter == high / J ? x[c][high % J] * unit : 0.0f);
+    }
+    const float coefficient = t < 2 ? -M * sum : sum;
+    const bool even = quarter == (2 * t & 3), odd = quarter == (2 * t & 3) + 1;
+    const __half upper = __float2half_rn(coefficient);
+    const float rest = coefficient - __half2float(upper);
+    qz[0] = pack2(even ? __half2float(upper) : 0.0f, odd ? __half2float(upper) : 0.0f);
+    qz[1] = pack2(even ? rest : 0.0f, odd ? rest : 0.0f);
+    factor = __shfl_sync(0xffffffffu, Base::factor_of(p, up), t < 2 ? 0 : 16);
+    m = -INFINITY;
+    off = NOTHING;
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sums[i] = zacc[i] = 0.0f;
+#pragma unroll
+      for (int u = 0; u < STEPS; ++u) { acc[i][u][0] = 0.0f; acc[i][u][1] = 0.0f; acc[i][u][2] = 0.0f; acc[i][u][3] = 0.0f; }
+    }
+    f = __float2half2_rn(0x1p15f);
+    ones = ONES;
+  }
+
+  // Scores of rows g and g + 8 of 16, times the power of two, head t / 2
+  __device__ __forceinline__ void scores(uint32_t kt, int lane, float (&y)[2]) const {
+    const int t = lane & 3, g = lane >> 2;
+    uint32_t w[2][2][N], pair[4];
+    trailers<false, ROW>(kt + CODES, lane, pair);
+    Base::keys(kt + g * ROW, t, w[0]);
+    Base::keys(kt + (g + 8) * ROW, t, w[1]);
+    float c[4], z[4];
+    mma(z, pair[0], pair[1], pair[2], pair[3], qz[0], qz[1], 0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) {
+      uint32_t x[2][PAIRS];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t word = w[r][i / N][i % N];
+        if constexpr (BITS == 4) {
+          x[r][0] = word & 0x000f000fu;
+          x[r][1] = word & 0x00f000f0u;
+          x[r][PAIRS - 2] = word >> 8 & 0x000f000fu;
+          x[r][PAIRS - 1] = word >> 8 & 0x00f000f0u;
+        } else {
+          x[r][0] = word & 0x00ff00ffu;
+          x[r][1] = word >> 8 & 0x00ff00ffu;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < PAIRS / 2; ++u) {
+        const uint32_t (&b)[2] = qb[i * (PAIRS / 2) + u];
+        if (i == 0 && u == 0) mma(c, x[0][0], x[1][0], x[0][1], x[1][1], b[0], b[1], 0.0f, 0.0f, 0.0f, 0.0f);
+        else mma(c, x[0][2 * u], x[1][2 * u], x[0][2 * u + 1], x[1][2 * u + 1], b[0], b[1], c[0], c[1], c[2], c[3]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float2 s = __half22float2(h2(__shfl_sync(0xffffffffu, pair[r], lane & ~2)));
+      const float v = fmaf(c[2 * r], s.x, z[2 * r] * UNIT) + fmaf(c[2 * r + 1], s.y, z[2 * r + 1] * UNIT);
+      y[r] = v + __shfl_xor_sync(0xffffffffu, v, 1);
+    }
+  }
+
+  // A scale exceeds 1: the powers of two follow
+  __device__ __forceinline__ void rescale(int lane, const uint32_t (&raw)[4]) {
+    const __half2 top = __hmax2(h2(raw[0]), h2(raw[2]));
+    float most = fmaxf(__low2float(top), __high2float(top));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    most = __shfl_sync(0xffffffffu, most, lane & 15);                       // (of quarter g & 3)
+    const float old = __low2float(f), now = Base::taken(most, old), by = now / old;
+    f = __float2half2_rn(now);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float r = __shfl_sync(0xffffffffu, by, 4 * i);
+#pragma unroll
+      for (int u = 0; u < STEPS; ++u) { acc[i][u][0] *= r; acc[i][u][1] *= r; acc[i][u][2] *= r; acc[i][u][3] *= r; }
+    }
+    // (columns 2 t and 2 t + 1: quarters 2 t & 3 and the next)
+    const float r0 = __shfl_sync(0xffffffffu, by, 8 * (lane & 1)), r1 = __shfl_sync(0xffffffffu, by, 8 * (lane & 1) + 4);
+    sums[0] *= r0; sums[1] *= r1; sums[2] *= r0; sums[3] *= r1;
+  }
+
+  // Weights of 16 rows (upper and lower parts, rows 2 t, 2 t + 1 and those + 8 of column g) times their values
+  __device__ __forceinline__ void weigh(uint32_t vt, int lane, const uint32_t (&hi)[2], const uint32_t (&lo)[2]) {
+    const int t = lane & 3, g = lane >> 2;
+    uint32_t raw[4], w[4][N], pb[2];
+    trailers<true, ROW>(vt + CODES, lane, raw);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) lds<N>(vt + (2 * t + (r & 1) + 8 * (r >> 1)) * ROW + g * CHUNK, w[r]);
+    const uint32_t r0 = __shfl_sync(0xffffffffu, raw[0], lane & 15), r1 = __shfl_sync(0xffffffffu, raw[2], lane & 15);
+    __half2 s0 = __hmul2(h2(r0), f), s1 = __hmul2(h2(r1), f);
+    if (__any_sync(0xffffffffu, !__hble2(__hmax2(s0, s1), __float2half2_rn(1.0f)))) {
+      rescale(lane, raw);
+      s0 = __hmul2(h2(r0), f);
+      s1 = __hmul2(h2(r1), f);
+    }
+    if constexpr (LOWER) {
+      pb[0] = bits_of(__hfma2(h2(hi[0]), s0, __hmul2(h2(lo[0]), s0)));
+      pb[1] = bits_of(__hfma2(h2(hi[1]), s1, __hmul2(h2(lo[1]), s1)));
+    } else {
+      pb[0] = bits_of(__hmul2(h2(hi[0]), s0));
+      pb[1] = bits_of(__hmul2(h2(hi[1]), s1));
+    }
+    mma(sums, ones, ones, ones, ones, pb[0], pb[1], sums[0], sums[1], sums[2], sums[3]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t first[J], second[J];
+      expand<DIM, BITS>(w[0], w[1], i, first);
+      expand<DIM, BITS>(w[2], w[3], i, second);
+#pragma unroll
+      for (int u = 0; u < STEPS; ++u) {
+        float (&c)[4] = acc[i][u];
+        mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pb[0], pb[1], c[0], c[1], c[2], c[3]);
+      }
+    }
+    mma(zacc, raw[0], raw[1], raw[2], raw[3], hi[0], hi[1], zacc[0], zacc[1], zacc[2], zacc[3]);
+    if constexpr (LOWER) mma(zacc, raw[0], raw[1], raw[2], raw[3], lo[0], lo[1], zacc[0], zacc[1], zacc[2], zacc[3]);
+  }
+
+  // A tile, of which `rows` rows (32 or fewer) are there
+  __device__ __forceinline__ void tile(uint32_t kt, int rows, int lane) {
+    const int g = lane >> 2;
+    const uint32_t vt = kt + TILE * ROW;
+    float x[2][2];
+    scores(kt, lane, x[0]);
+    scores(kt + 16 * ROW, lane, x[1]);
+    if (rows < TILE) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (8 * e + g >= rows) x[e / 2][e % 2] = -INFINITY;
+    }
+    // the maximum moves when a score is SLACK above it
+    float v = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
+    if (__any_sync(0xffffffffu, fmaf(v, factor, off) > SHIFT + SLACK)) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+      v = fmaxf(v, m);
+      if (v != -INFINITY) {
+        const float by = exp2_fast((m - v) * factor);
+        m = v;
+        off = fmaf(-v, factor, SHIFT);
+        l *= by;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sums[i] *= by;
+          zacc[i] *= by;
+#pragma unroll
+          for (int u = 0; u < STEPS; ++u) { acc[i][u][0] *= by; acc[i][u][1] *= by; acc[i][u][2] *= by; acc[i][u][3] *= by; }
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t hi[2], lo[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float w = exp2_fast(fmaf(x[h][r], factor, off));
+        l += w;
+        const uint32_t upper = pack2(w, w);
+        hi[r] = transposed(upper);
+        lo[r] = 0u;
+        if constexpr (LOWER) {
+          const float rest = w - __low2float(h2(upper));
+          lo[r] = transposed(pack2(rest, rest));
+        }
+      }
+      weigh(vt + 16 * h * ROW, lane, hi, lo);
+    }
+  }
+
+  // The state of a part to the workspace (slot >= 0), or the output of a whole item
+  __device__ __forceinline__ void end(const AttendParams &p, int b, int kv_head, int slot, int lane) {
+    const int t = lane & 3, g = lane >> 2, h = t >> 1;
+    float total = l;
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const float by = total == 0.0f ? 0.0f : 1.0f / total;
+    const size_t part = static_cast<size_t>(slot) * p.group + h, row = static_cast<size_t>(b) * p.q_heads + kv_head * p.group + h;
+    const bool live = h < p.group;
+    // this lane's columns: quarters 2 t & 3 and the next
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = (2 * t & 3) + e;
+      const float z = __shfl_sync(0xffffffffu, zacc[e], 4 * i + 16 + t), inverse = 1.0f / __shfl_sync(0xffffffffu, __low2float(f), 4 * i);
+      float v[J];
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const float c = t & 1 ? acc[2 + e][j / 2][e + 2 * (j % 2)] : acc[e][j / 2][e + 2 * (j % 2)];
+        v[j] = fmaf(fmaf(c, (BITS == 4 && j % 2 ? 0.0625f : 1.0f) / UNIT, -M * sums[e]), inverse, z);
+      }
+      if (!live) continue;
+      if (slot >= 0) store_part<DIM>(p.part_out + part * DIM + DIM / 4 * i + J * g, v);
+      else store_out<T, DIM>(static_cast<T *>(p.out) + row * DIM + DIM / 4 * i + J * g, v, by);
+    }
+    if (!live || (t & 1) || g) return;
+    if (slot >= 0) p.part_ml[part] = make_float2(total == 0.0f ? -INFINITY : -off, total);
+    else if (p.lse) p.lse[row] = total == 0.0f ? -INFINITY : logf(total) - off * LN2;
+  }
+};
+
+// Up to sixteen query heads, in NT blocks of eight columns.
+template <typename T, int DIM, int BITS, int NT>
+struct Attend : Tiles<DIM, BITS, NT> {
+  using Base = Tiles<DIM, BITS, NT>;
+  using Base::ROW; using Base::CODES; using Base::N; using Base::J; using Base::STEPS; using Base::M; using Base::UNIT; using Base::CHUNK;
+  static constexpr bool LOWER = !Type<T>::BF16;            // whether weights have a lower part
+
+  uint32_t qb[NT][4][STEPS][2], qz[NT][2];       // queries; sums over quarters, as upper and lower fp16 parts
+  float factor[NT][2], m[NT][2], off[NT][2], l[NT][2];     // of heads 2 t and 2 t + 1: what a score is multiplied by, the largest score, what is added in the exponent, the sum of weights
+  float acc[NT][4][STEPS][4], sums[NT][4][4], zacc[NT][4]; // out^T, quarter by quarter; sums of weights times scales; of weights times centres (lanes g >= 4: of quarter g - 4)
+  __half2 f;                                     // power of two that takes quarter g & 3's scales of values to 1 or below
+  uint32_t ones;
 
   // The queries of an item, and nothing seen yet
   __device__ __forceinline__ void begin(const AttendParams &p, int b, int kv_head, int lane) {
@@ -221,17 +519,13 @@ struct Attend {
         for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int j = 0; j < J; ++j) {
-            const int chunk = SPREAD ? t + 4 * c : 2 * t + c;
-            x[i][c * J + j] = live ? static_cast<float>(q[DIM / 4 * i + DIM / 32 * chunk + j]) : 0.0f;
+            x[i][c * J + j] = live ? static_cast<float>(q[DIM / 4 * i + DIM / 32 * Base::chunk_of(t, c) + j]) : 0.0f;
             top = fmaxf(top, fabsf(x[i][c * J + j]));
           }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // taken to at most 2^9, so that sums over a quarter stay in fp16 and entries lose bits from 2^-29 of the largest on
-      int e = static_cast<int>(__float_as_uint(top) >> 23) - 126;        // top < 2^e
-      e = top == 0.0f || top == INFINITY ? 9 : e;
-      const int up = min(max(9 - e, -126), 126);
-      const float by = power2(up);
+      const int up = Base::lift(top);
+      const float by = copysignf(power2(up), p.scale_log2);
       float sum[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -246,57 +540,51 @@ struct Attend {
           qb[nt][i][u][1] = pack2(x[i][2 * u + 1] * (BITS == 4 ? 0.0625f : 1.0f), x[i][J + 2 * u + 1] * (BITS == 4 ? 0.0625f : 1.0f));
         }
       }
-      // columns 2 t and 2 t + 1 of the sums: lanes 8 t and 8 t + 4
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        start[nt][i][0] = -M * UNIT * __shfl_sync(0xffffffffu, sum[i], 8 * t);
-        start[nt][i][1] = -M * UNIT * __shfl_sync(0xffffffffu, sum[i], 8 * t + 4);
-      }
-      const float down = p.scale_log2 * power2(-up);
+      // heads 2 t and 2 t + 1: lanes 8 t and 8 t + 4
+      const float down = Base::factor_of(p, up);
       factor[nt][0] = __shfl_sync(0xffffffffu, down, 8 * t);
       factor[nt][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
-      const float s0 = t & 1 ? sum[2] : sum[0], s1 = t & 1 ? sum[3] : sum[1];
+      const float by0 = t < 2 ? -M : 1.0f, s0 = by0 * (t & 1 ? sum[2] : sum[0]), s1 = by0 * (t & 1 ? sum[3] : sum[1]);
       const uint32_t upper = pack2(s0, s1);
       const float2 back = __half22float2(h2(upper));
-      qz[nt] = t < 2 ? upper : pack2(s0 - back.x, s1 - back.y);
+      qz[nt][0] = upper;
+      qz[nt][1] = pack2(s0 - back.x, s1 - back.y);
       m[nt][0] = m[nt][1] = -INFINITY;
+      off[nt][0] = off[nt][1] = NOTHING;
       l[nt][0] = l[nt][1] = 0.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         zacc[nt][i] = 0.0f;
+        sums[nt][i][0] = 0.0f; sums[nt][i][1] = 0.0f; sums[nt][i][2] = 0.0f; sums[nt][i][3] = 0.0f;
 #pragma unroll
         for (int u = 0; u < STEPS; ++u) { acc[nt][i][u][0] = 0.0f; acc[nt][i][u][1] = 0.0f; acc[nt][i][u][2] = 0.0f; acc[nt][i][u][3] = 0.0f; }
       }
     }
-    f01 = f23 = __float2half2_rn(0x1p15f);
+    f = __float2half2_rn(0x1p15f);
+    ones = ONES;
   }
 
-  // Scores of 16 rows, in powers of two: rows g and g + 8, heads 2 t and 2 t + 1
+  // Scores of 16 rows, times the power of two: rows g and g + 8, heads 2 t and 2 t + 1
   __device__ __forceinline__ void scores(uint32_t kt, int lane, float (&x)[NT][4]) const {
     const int t = lane & 3, g = lane >> 2;
-    uint32_t w[2][2][N];                         // row, chunk
+    uint32_t w[2][2][N], pair[4];                // row, chunk
     float s[2][4];
-    uint32_t z[2];
+    trailers<false, ROW>(kt + CODES, lane, pair);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const uint32_t at = kt + (g + 8 * r) * ROW;
-      if constexpr (SPREAD) {
-        lds<N>(at + t * CHUNK, w[r][0]);
-        lds<N>(at + (t + 4) * CHUNK, w[r][1]);
-      } else {
-        uint32_t both[2 * N];
-        lds<2 * N>(at + 2 * t * CHUNK, both);
-#pragma unroll
-        for (int i = 0; i < N; ++i) { w[r][0][i] = both[i]; w[r][1][i] = both[N + i]; }
-      }
-      uint32_t sw[2], zw[1];
+      Base::keys(at, t, w[r]);
+      uint32_t sw[2];
       lds<2>(at + CODES, sw);
-      lds<1>(at + CODES + 8 + 4 * (t & 1), zw);
       const float2 s01 = __half22float2(h2(sw[0])), s23 = __half22float2(h2(sw[1]));
       s[r][0] = s01.x; s[r][1] = s01.y; s[r][2] = s23.x; s[r][3] = s23.y;
-      z[r] = zw[0];
     }
-    float y[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      mma(x[nt], pair[0], pair[1], pair[2], pair[3], qz[nt][0], qz[nt][1], 0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[nt][e] *= UNIT;
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t top[J], low[J];
@@ -305,53 +593,66 @@ struct Attend {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float c[4];
-        mma(c, top[0], low[0], top[1], low[1], qb[nt][i][0][0], qb[nt][i][0][1], start[nt][i][0], start[nt][i][1], start[nt][i][0], start[nt][i][1]);
+        mma(c, top[0], low[0], top[1], low[1], qb[nt][i][0][0], qb[nt][i][0][1], 0.0f, 0.0f, 0.0f, 0.0f);
         if constexpr (STEPS == 2) mma(c, top[J - 2], low[J - 2], top[J - 1], low[J - 1], qb[nt][i][STEPS - 1][0], qb[nt][i][STEPS - 1][1], c[0], c[1], c[2], c[3]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[nt][e] = i == 0 ? c[e] * s[e / 2][0] : fmaf(c[e], s[e / 2][i], y[nt][e]);
+        for (int e = 0; e < 4; ++e) x[nt][e] = fmaf(c[e], s[e / 2][i], x[nt][e]);
       }
     }
+  }
+
+  // A scale exceeds 1: the powers of two follow
+  __device__ __forceinline__ void rescale(int lane, const uint32_t (&raw)[4]) {
+    const __half2 top = __hmax2(h2(raw[0]), h2(raw[2]));
+    float most = fmaxf(__low2float(top), __high2float(top));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    most = __shfl_sync(0xffffffffu, most, lane & 15);                       // (of quarter g & 3)
+    const float old = __low2float(f), now = Base::taken(most, old), by = now / old;
+    f = __float2half2_rn(now);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float c[4];
-      mma_k8(c, z[0], z[1], qz[nt]);
+    for (int i = 0; i < 4; ++i) {
+      const float r = __shfl_sync(0xffffffffu, by, 4 * i);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[nt][e] = fmaf(y[nt][e], factor[nt][e % 2] * 0x1p24f, c[e] * factor[nt][e % 2]);
+      for (int nt = 0; nt < NT; ++nt) {
+        sums[nt][i][0] *= r; sums[nt][i][1] *= r; sums[nt][i][2] *= r; sums[nt][i][3] *= r;
+#pragma unroll
+        for (int u = 0; u < STEPS; ++u) { acc[nt][i][u][0] *= r; acc[nt][i][u][1] *= r; acc[nt][i][u][2] *= r; acc[nt][i][u][3] *= r; }
+      }
     }
   }
 
   // Weights of 16 rows (upper and lower parts, rows 2 t, 2 t + 1 and those + 8 of head g) times their values
   __device__ __forceinline__ void weigh(uint32_t vt, int lane, const uint32_t (&hi)[NT][2], const uint32_t (&lo)[NT][2]) {
     const int t = lane & 3, g = lane >> 2;
-    uint32_t w[4][N], s[4][2], z[2];
+    uint32_t raw[4], w[4][N];
+    trailers<true, ROW>(vt + CODES, lane, raw);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const uint32_t at = vt + (2 * t + (r & 1) + 8 * (r >> 1)) * ROW;
-      lds<N>(at + g * CHUNK, w[r]);
-      lds<2>(at + CODES, s[r]);
-      s[r][0] = bits_of(__hmul2(h2(s[r][0]), f01));
-      s[r][1] = bits_of(__hmul2(h2(s[r][1]), f23));
-      const uint32_t one = lds16(at + CODES + 8 + 2 * (g & 3));
-      z[r >> 1] = r & 1 ? z[r >> 1] | one << 16 : one;
+    for (int r = 0; r < 4; ++r) lds<N>(vt + (2 * t + (r & 1) + 8 * (r >> 1)) * ROW + g * CHUNK, w[r]);
+    __half2 s0 = __hmul2(h2(raw[0]), f), s1 = __hmul2(h2(raw[2]), f);
+    if (__any_sync(0xffffffffu, g < 4 && !__hble2(__hmax2(s0, s1), __float2half2_rn(1.0f)))) {
+      rescale(lane, raw);
+      s0 = __hmul2(h2(raw[0]), f);
+      s1 = __hmul2(h2(raw[2]), f);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t first[J], second[J], pb[NT][2];
-      const uint32_t sel = i % 2 ? 0x7632 : 0x5410;
-      const __half2 s0 = h2(__byte_perm(s[0][i / 2], s[1][i / 2], sel)), s1 = h2(__byte_perm(s[2][i / 2], s[3][i / 2], sel));
+      const __half2 a0 = h2(__shfl_sync(0xffffffffu, bits_of(s0), 4 * i + t)), a1 = h2(__shfl_sync(0xffffffffu, bits_of(s1), 4 * i + t));
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        pb[nt][0] = bits_of(__hfma2(h2(hi[nt][0]), s0, __hmul2(h2(lo[nt][0]), s0)));
-        pb[nt][1] = bits_of(__hfma2(h2(hi[nt][1]), s1, __hmul2(h2(lo[nt][1]), s1)));
+        if constexpr (LOWER) {
+          pb[nt][0] = bits_of(__hfma2(h2(hi[nt][0]), a0, __hmul2(h2(lo[nt][0]), a0)));
+          pb[nt][1] = bits_of(__hfma2(h2(hi[nt][1]), a1, __hmul2(h2(lo[nt][1]), a1)));
+        } else {
+          pb[nt][0] = bits_of(__hmul2(h2(hi[nt][0]), a0));
+          pb[nt][1] = bits_of(__hmul2(h2(hi[nt][1]), a1));
+        }
+        float (&c)[4] = sums[nt][i];
+        mma(c, ones, ones, ones, ones, pb[nt][0], pb[nt][1], c[0], c[1], c[2], c[3]);
       }
       expand<DIM, BITS>(w[0], w[1], i, first);
       expand<DIM, BITS>(w[2], w[3], i, second);
-#pragma unroll
-      for (int j = 0; j < J; ++j) {              // (exact: whole multiples of 2^-24)
-        const __half2 middle = __float2half2_rn(-M * UNIT * (BITS == 4 && j % 2 ? 16.0f : 1.0f));
-        first[j] = bits_of(__hadd2(h2(first[j]), middle));
-        second[j] = bits_of(__hadd2(h2(second[j]), middle));
-      }
 #pragma unroll
       for (int u = 0; u < STEPS; ++u)
 #pragma unroll
@@ -363,8 +664,8 @@ struct Attend {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float (&c)[4] = zacc[nt];
-      mma(c, z[0], z[0], z[1], z[1], hi[nt][0], hi[nt][1], c[0], c[1], c[2], c[3]);
-      mma(c, z[0], z[0], z[1], z[1], lo[nt][0], lo[nt][1], c[0], c[1], c[2], c[3]);
+      mma(c, raw[0], raw[1], raw[2], raw[3], hi[nt][0], hi[nt][1], c[0], c[1], c[2], c[3]);
+      if constexpr (LOWER) mma(c, raw[0], raw[1], raw[2], raw[3], lo[nt][0], lo[nt][1], c[0], c[1], c[2], c[3]);
     }
   }
 
@@ -392,7 +693,7 @@ struct Attend {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         top[nt][e] = fmaxf(fmaxf(x[0][nt][e], x[0][nt][e + 2]), fmaxf(x[1][nt][e], x[1][nt][e + 2]));
-        rises |= top[nt][e] > m[nt][e] + SLACK;
+        rises |= fmaf(top[nt][e], factor[nt][e], off[nt][e]) > SHIFT + SLACK;
       }
     if (__any_sync(0xffffffffu, rises)) {
 #pragma unroll
@@ -403,46 +704,22 @@ struct Attend {
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
           v = fmaxf(v, m[nt][e]);
-          const float f = v == -INFINITY ? 1.0f : exp2_fast(m[nt][e] - v);
-          m[nt][e] = v;
-          l[nt][e] *= f;
-          zacc[nt][e] *= f;
-          zacc[nt][e + 2] *= f;
+          if (v != -INFINITY) {
+            const float by = exp2_fast((m[nt][e] - v) * factor[nt][e]);
+            m[nt][e] = v;
+            off[nt][e] = fmaf(-v, factor[nt][e], SHIFT);
+            l[nt][e] *= by;
+            zacc[nt][e] *= by;
+            zacc[nt][e + 2] *= by;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i) {
+              sums[nt][i][e] *= by;
+              sums[nt][i][e + 2] *= by;
 #pragma unroll
-            for (int u = 0; u < STEPS; ++u) { acc[nt][i][u][e] *= f; acc[nt][i][u][e + 2] *= f; }
+              for (int u = 0; u < STEPS; ++u) { acc[nt][i][u][e] *= by; acc[nt][i][u][e + 2] *= by; }
+            }
+          }
         }
-    }
-    // the scales of values: a row to a lane
-    {
-      uint32_t s[2];
-      lds<2>(vt + lane * ROW + CODES, s);
-      const __half2 over = __hmax2(__hmul2(h2(s[0]), f01), __hmul2(h2(s[1]), f23));
-      if (__any_sync(0xffffffffu, __low2float(over) > 1.0f || __high2float(over) > 1.0f)) {
-        __half2 a = h2(s[0]), c = h2(s[1]);
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          a = __hmax2(a, h2(__shfl_xor_sync(0xffffffffu, bits_of(a), o)));
-          c = __hmax2(c, h2(__shfl_xor_sync(0xffffffffu, bits_of(c), o)));
-        }
-        const float2 a2 = __half22float2(a), c2 = __half22float2(c), f2 = __half22float2(f01), g2 = __half22float2(f23);
-        const float most[4] = {a2.x, a2.y, c2.x, c2.y}, old[4] = {f2.x, f2.y, g2.x, g2.y};
-        float now[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // the power of two that takes `most` into (1/2, 1]
-          const int e = static_cast<int>((__float_as_uint(most[i]) + 0x7fffffu) >> 23) - 127;
-          now[i] = fminf(old[i], power2(min(max(-e, -14), 15)));
-          const float f = now[i] / old[i];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int u = 0; u < STEPS; ++u) { acc[nt][i][u][0] *= f; acc[nt][i][u][1] *= f; acc[nt][i][u][2] *= f; acc[nt][i][u][3] *= f; }
-        }
-        f01 = __floats2half2_rn(now[0], now[1]);
-        f23 = __floats2half2_rn(now[2], now[3]);
-      }
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -452,16 +729,18 @@ struct Attend {
         float w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float at = m[nt][e % 2];
-          w[e] = exp2_fast(x[h][nt][e] - ((at == -INFINITY ? 0.0f : at) - SHIFT));
+          w[e] = exp2_fast(fmaf(x[h][nt][e], factor[nt][e % 2], off[nt][e % 2]));
           l[nt][e % 2] += w[e];
         }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const uint32_t upper = pack2(w[2 * r], w[2 * r + 1]);
-          const float2 back = __half22float2(h2(upper));
           hi[nt][r] = transposed(upper);
-          lo[nt][r] = transposed(pack2(w[2 * r] - back.x, w[2 * r + 1] - back.y));
+          lo[nt][r] = 0u;
+          if constexpr (LOWER) {
+            const float2 back = __half22float2(h2(upper));
+            lo[nt][r] = transposed(pack2(w[2 * r] - back.x, w[2 * r + 1] - back.y));
+          }
         }
       }
       weigh(vt + 16 * h * ROW, lane, hi, lo);
@@ -471,8 +750,9 @@ struct Attend {
   // The state of a part to the workspace (slot >= 0), or the output of a whole item
   __device__ __forceinline__ void end(const AttendParams &p, int b, int kv_head, int slot, int lane) {
     const int t = lane & 3, g = lane >> 2;
-    const float2 f2 = __half22float2(f01), g2 = __half22float2(f23);
-    const float inverse[4] = {1.0f / f2.x / UNIT, 1.0f / f2.y / UNIT, 1.0f / g2.x / UNIT, 1.0f / g2.y / UNIT};
+    float inverse[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) inverse[i] = 1.0f / __shfl_sync(0xffffffffu, __low2float(f), 4 * i);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -480,45 +760,29 @@ struct Attend {
         float total = l[nt][e];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        float v[4][J];
+        const int h = nt * 8 + 2 * t + e;
+        const float by = total == 0.0f ? 0.0f : 1.0f / total;
+        const size_t part = static_cast<size_t>(slot) * p.group + h, row = static_cast<size_t>(b) * p.q_heads + kv_head * p.group + h;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float z = __shfl_sync(0xffffffffu, zacc[nt][e], 4 * i + t);
+          const float z = __shfl_sync(0xffffffffu, zacc[nt][e], 4 * i + 16 + t);
+          float v[J];
 #pragma unroll
-          for (int j = 0; j < J; ++j) v[i][j] = fmaf(acc[nt][i][j / 2][e + 2 * (j % 2)], inverse[i] * (BITS == 4 && j % 2 ? 0.0625f : 1.0f), z);
+          for (int j = 0; j < J; ++j)
+            v[j] = fmaf(fmaf(acc[nt][i][j / 2][e + 2 * (j % 2)], (BITS == 4 && j % 2 ? 0.0625f : 1.0f) / UNIT, -M * sums[nt][i][e]), inverse[i], z);
+          if (h >= p.group) continue;
+          if (slot >= 0) store_part<DIM>(p.part_out + part * DIM + DIM / 4 * i + J * g, v);
+          else store_out<T, DIM>(static_cast<T *>(p.out) + row * DIM + DIM / 4 * i + J * g, v, by);
         }
-        const int h = nt * 8 + 2 * t + e;
-        if (h >= p.group) continue;
-        if (slot >= 0) {
-          const size_t at = static_cast<size_t>(slot) * p.group + h;
-          if (g == 0) p.part_ml[at] = make_float2(m[nt][e], total);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float *const to = p.part_out + at * DIM + DIM / 4 * i + J * g;
-            if constexpr (J == 4) *reinterpret_cast<float4 *>(to) = make_float4(v[i][0], v[i][1], v[i][J - 2], v[i][J - 1]);
-            else *reinterpret_cast<float2 *>(to) = make_float2(v[i][0], v[i][1]);
-          }
-        } else {
-          const size_t at = static_cast<size_t>(b) * p.q_heads + kv_head * p.group + h;
-          if (g == 0 && p.lse) p.lse[at] = total == 0.0f ? -INFINITY : (m[nt][e] - SHIFT) * LN2 + logf(total);
-          const float by = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            T *const to = static_cast<T *>(p.out) + at * DIM + DIM / 4 * i + J * g;
-            T o[J];
-#pragma unroll
-            for (int j = 0; j < J; ++j) o[j] = static_cast<T>(v[i][j] * by);
-            if constexpr (J == 4) *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<const uint2 *>(o);
-            else *reinterpret_cast<uint32_t *>(to) = *reinterpret_cast<const uint32_t *>(o);
-          }
-        }
+        if (h >= p.group || g) continue;
+        if (slot >= 0) p.part_ml[part] = make_float2(total == 0.0f ? -INFINITY : -off[nt][e], total);
+        else if (p.lse) p.lse[row] = total == 0.0f ? -INFINITY : logf(total) - off[nt][e] * LN2;
       }
   }
 };
 
-template <typename T, int DIM, int BITS, int NT>
-__global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(NT)) attend_tiles(const __grid_constant__ AttendParams p) {
-  using A = Attend<T, DIM, BITS, NT>;
+template <typename A, int BLOCKS>
+__global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(BLOCKS)) attend_tiles(const __grid_constant__ AttendParams p) {
   constexpr int STAGES = A::STAGES;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Line line;
@@ -648,7 +912,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_stretches(const __grid_c
     out = fmaf(sa[w][threadIdx.x], f, out);
   }
   static_cast<T *>(p.out)[row * DIM + threadIdx.x] = static_cast<T>(total == 0.0f ? 0.0f : out / total);
-  if (p.lse && threadIdx.x == 0) p.lse[row] = total == 0.0f ? -INFINITY : (top - SHIFT) * LN2 + logf(total);
+  if (p.lse && threadIdx.x == 0) p.lse[row] = total == 0.0f ? -INFINITY : top * LN2 + logf(total);
 }
 
 }  // namespace qmk_packed

@@ -104,21 +104,23 @@ int warps_of(int seqs, int kv_heads, int group, int rows) {
 }
 long long workspace_bytes(int warps, int group, int dim) { return 2ll * warps * group * (dim * 4ll + 8); }
 
-template <typename T, int DIM, int BITS, int NT>
+template <typename A, int BLOCKS>
+cudaError_t launch_tiles(const AttendParams &p, cudaStream_t stream) {
+  const cudaError_t e = cudaFuncSetAttribute(attend_tiles<A, BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, A::SMEM);
+  if (e != cudaSuccess) return e;
+  const int ctas = std::min(p.warps, SMS * ctas_per_sm(BLOCKS));         // (a warp of each where there are few)
+  return qmk_tc::launch_kernel(attend_tiles<A, BLOCKS>, dim3(ctas), dim3(WARPS * 32), A::SMEM, stream, p);
+}
+template <typename T, int DIM, int BITS>
 cudaError_t attend(const AttendParams &p, cudaStream_t stream) {
-  using A = Attend<T, DIM, BITS, NT>;
-  cudaError_t e = cudaSuccess;
-  if (p.caches.rows > 0) {
-    e = cudaFuncSetAttribute(attend_tiles<T, DIM, BITS, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, A::SMEM);
-    const int ctas = std::min(p.warps, SMS * ctas_per_sm(NT));           // (a warp of each where there are few)
-    if (e == cudaSuccess) e = qmk_tc::launch_kernel(attend_tiles<T, DIM, BITS, NT>, dim3(ctas), dim3(WARPS * 32), A::SMEM, stream, p);
-  }
+  const cudaError_t e = p.caches.rows == 0 ? cudaSuccess
+                        : p.group <= 2     ? launch_tiles<AttendPair<T, DIM, BITS>, 1>(p, stream)
+                        : p.group <= 8     ? launch_tiles<Attend<T, DIM, BITS, 1>, 1>(p, stream)
+                                           : launch_tiles<Attend<T, DIM, BITS, 2>, 2>(p, stream);
   if (e != cudaSuccess) return e;
   const qmk_tc::PdlScope scope(true);
   return qmk_tc::launch_kernel(join_stretches<T, DIM>, dim3(p.caches.seqs * p.q_heads), dim3(JOIN_WARPS * 32), 0, stream, p);
 }
-template <typename T, int DIM, int BITS>
-cudaError_t attend(const AttendParams &p, cudaStream_t stream) { return blocks_of(p.group) == 2 ? attend<T, DIM, BITS, 2>(p, stream) : attend<T, DIM, BITS, 1>(p, stream); }
 template <typename T>
 cudaError_t attend(const AttendParams &p, int dim, int bits, cudaStream_t stream) {
   if (bits == 4) return dim == 64 ? attend<T, 64, 4>(p, stream) : attend<T, 128, 4>(p, stream);
