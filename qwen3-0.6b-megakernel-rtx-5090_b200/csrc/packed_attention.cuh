@@ -23,8 +23,10 @@ constexpr int TILE = 32;                         // rows
 constexpr int WARPS = 4, SMS = 148;
 // CTAs on an SM: what registers allow (168 a thread, 255 with two blocks of heads); tiles of a warp's ring: what their shared memory does
 constexpr int ctas_per_sm(int blocks) { return blocks == 1 ? 3 : 2; }
+// (228 KB an SM; of a CTA 1 KB is the system's, 1.25 KB the line's)
+constexpr int warp_bytes(int blocks) { return (228 * 1024 - ctas_per_sm(blocks) * 2304) / (ctas_per_sm(blocks) * WARPS); }
 constexpr int stages(int blocks, int row_bytes) {
-  const int fit = 225 * 1024 / (ctas_per_sm(blocks) * WARPS * 2 * TILE * row_bytes);
+  const int fit = warp_bytes(blocks) / (2 * TILE * row_bytes);
   return fit < 4 ? fit : 4;
 }
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -119,15 +121,15 @@ __device__ __forceinline__ void expand(const uint32_t (&a)[DIM * BITS / 256], co
 // The line of tiles: sequence by sequence, kv head by kv head.
 struct Line {
   int total;                                     // tiles
-  int before[MAX_SEQS];                          // tiles in front of a sequence
+  int before[MAX_SEQS], rows[MAX_SEQS];          // tiles in front of a sequence, rows that it sees
 };
 __device__ __forceinline__ int seen_rows(const AttendParams &p, int b) { return min(max(p.lens[b], 0), p.caches.rows); }
 __device__ __forceinline__ int tiles_of(int rows) { return (rows + TILE - 1) / TILE; }
 // (a sequence to each of the first threads; in front of a barrier of the caller's)
 __device__ __forceinline__ void make_line(const AttendParams &p, Line &line, int (&sums)[MAX_SEQS / 32]) {
   const int i = threadIdx.x, lane = i & 31;
-  int n = i < p.caches.seqs ? tiles_of(seen_rows(p, i)) * p.caches.kv_heads : 0;
-  const int own = n;
+  const int rows = i < p.caches.seqs ? seen_rows(p, i) : 0, own = tiles_of(rows) * p.caches.kv_heads;
+  int n = own;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int up = __shfl_up_sync(0xffffffffu, n, o);
@@ -138,7 +140,7 @@ __device__ __forceinline__ void make_line(const AttendParams &p, Line &line, int
 #pragma unroll
   for (int w = 0; w < MAX_SEQS / 32; ++w)
     if (w < (i >> 5)) n += sums[w];
-  if (i < MAX_SEQS) line.before[i] = n - own;
+  if (i < MAX_SEQS) { line.before[i] = n - own; line.rows[i] = rows; }
   if (i == MAX_SEQS - 1) line.total = n;
 }
 // Stretch r of `parts` equal ones begins at tile total * r / parts; the stretch that holds tile t
@@ -148,9 +150,9 @@ __device__ __forceinline__ int part_of(int total, int parts, int t) { return sta
 // A place in the line
 struct Place {
   int b, head, tile, tiles, rows;
-  __device__ __forceinline__ void sequence(const AttendParams &p, int at) {
+  __device__ __forceinline__ void sequence(const Line &line, int at) {
     b = at;
-    rows = b < p.caches.seqs ? seen_rows(p, b) : 0;
+    rows = b < MAX_SEQS ? line.rows[b] : 0;
     tiles = tiles_of(rows);
   }
   __device__ __forceinline__ void start(const AttendParams &p, const Line &line, int t) {
@@ -159,17 +161,17 @@ struct Place {
       const int mid = (low + high + 1) / 2;
       if (line.before[mid] <= t) low = mid; else high = mid - 1;
     }
-    sequence(p, low);
+    sequence(line, low);
     const int i = t - line.before[low];
     head = i / tiles;
     tile = i - head * tiles;
   }
-  __device__ __forceinline__ void next(const AttendParams &p) {
+  __device__ __forceinline__ void next(const AttendParams &p, const Line &line) {
     if (++tile < tiles) return;
     tile = 0;
     if (++head < p.caches.kv_heads) return;
     head = 0;
-    do sequence(p, b + 1); while (tiles == 0 && b < p.caches.seqs);
+    do sequence(line, b + 1); while (tiles == 0 && b < p.caches.seqs);
   }
 };
 
@@ -187,12 +189,15 @@ template <typename T, int DIM> __device__ __forceinline__ void store_out(T *to, 
 }
 
 // What both ways to take a tile below have in common.
-template <int DIM, int BITS, int BLOCKS>
+template <int DIM, int BITS, int BLOCKS, int HEADS>
 struct Tiles {
   static constexpr int ROW = ROW_BYTES<DIM, BITS>, CODES = ROW - TRAILER, PIECES = ROW / 16;
   static constexpr int CHUNK = CODES / 8, N = CHUNK / 4, J = DIM / 32, STEPS = J / 2;       // bytes and words of a chunk; codes of a quarter in it; k steps of a quarter
   static constexpr int STAGE = 2 * TILE * ROW;                                              // keys, then values
-  static constexpr int STAGES = stages(BLOCKS, ROW), SMEM = WARPS * STAGES * STAGE;
+  static constexpr int STAGES = stages(BLOCKS, ROW);
+  // Queries of the next item, copied with its first rows; where a warp's shared memory has room
+  static constexpr int QUERIES = STAGES * STAGE + HEADS * DIM * 2 <= warp_bytes(BLOCKS) ? HEADS * DIM * 2 : 0;
+  static constexpr int QUERY_STRIDE = DIM, WARP_SMEM = STAGES * STAGE + QUERIES, SMEM = WARPS * WARP_SMEM;
   static constexpr float M = 1 << (BITS - 1), UNIT = 0x1p-24f;
   static constexpr bool SPREAD = BITS == 8 && DIM == 128;                                   // a lane's two chunks of keys: four apart, or one behind the other
   static __device__ __forceinline__ int chunk_of(int t, int c) { return SPREAD ? t + 4 * c : 2 * t + c; }
@@ -218,6 +223,12 @@ struct Tiles {
         copy16(dst + TILE * ROW + piece * 16, v + off, there);
       }
     }
+  }
+  // The queries of an item, one head behind the other
+  template <typename T>
+  static __device__ __forceinline__ void load_queries(const AttendParams &p, const Place &at, uint32_t dst, int lane) {
+    const T *const q = static_cast<const T *>(p.q) + at.b * p.q_seq + static_cast<long long>(at.head) * p.group * p.q_head;
+    for (int i = lane; i < p.group * (DIM / 8); i += 32) copy16(dst + i * 16, q + i / (DIM / 8) * p.q_head + i % (DIM / 8) * 8);
   }
   // The lane's two chunks of keys of row g
   static __device__ __forceinline__ void keys(uint32_t row, int t, uint32_t (&w)[2][N]) {
@@ -251,12 +262,12 @@ struct Tiles {
 // quarter, so one product over all codes has the quarters' sums side by side, each is scaled once, and pairs of codes need not be of one quarter; values: the weights'
 // scales are the columns', one operand for all dimensions, of whose columns each quarter of the output keeps its own.
 template <typename T, int DIM, int BITS>
-struct AttendPair : Tiles<DIM, BITS, 1> {
-  using Base = Tiles<DIM, BITS, 1>;
+struct AttendPair : Tiles<DIM, BITS, 1, 2> {
+  using Value = T;
+  using Base = Tiles<DIM, BITS, 1, 2>;
   using Base::ROW; using Base::CODES; using Base::N; using Base::J; using Base::STEPS; using Base::M; using Base::UNIT; using Base::CHUNK;
   static constexpr bool LOWER = !Type<T>::BF16;            // whether weights have a lower part
   static constexpr int PAIRS = 16 / BITS, KSTEPS = N * PAIRS;               // operand words of a word of codes; k steps of a row of keys
-  static constexpr int HEADS = 1;                          // of a thread's columns
 
   uint32_t qb[KSTEPS][2], qz[2];                 // queries; sums over quarters, as upper and lower fp16 parts
   float factor, m, off, l;                       // what a score is multiplied by, the largest score, what is added in the exponent, the sum of weights
@@ -264,10 +275,10 @@ struct AttendPair : Tiles<DIM, BITS, 1> {
   __half2 f;                                     // power of two that takes quarter g & 3's scales of values to 1 or below
   uint32_t ones;
 
-  __device__ __forceinline__ void begin(const AttendParams &p, int b, int kv_head, int lane) {
+  __device__ __forceinline__ void begin(const AttendParams &p, const T *queries, long long stride, int lane) {
     const int t = lane & 3, g = lane >> 2, h = g >> 2, quarter = g & 3;
     const bool live = h < p.group;
-    const T *const q = static_cast<const T *>(p.q) + b * p.q_seq + (kv_head * p.group + (live ? h : 0)) * p.q_head + DIM / 4 * quarter;
+    const T *const q = queries + (live ? h : 0) * stride + DIM / 4 * quarter;
     float x[2][J], top = 0.0f;
 #pragma unroll
     for (int c = 0; c < 2; ++c)
@@ -494,8 +505,9 @@ struct AttendPair : Tiles<DIM, BITS, 1> {
 
 // Up to sixteen query heads, in NT blocks of eight columns.
 template <typename T, int DIM, int BITS, int NT>
-struct Attend : Tiles<DIM, BITS, NT> {
-  using Base = Tiles<DIM, BITS, NT>;
+struct Attend : Tiles<DIM, BITS, NT, 8 * NT> {
+  using Value = T;
+  using Base = Tiles<DIM, BITS, NT, 8 * NT>;
   using Base::ROW; using Base::CODES; using Base::N; using Base::J; using Base::STEPS; using Base::M; using Base::UNIT; using Base::CHUNK;
   static constexpr bool LOWER = !Type<T>::BF16;            // whether weights have a lower part
 
@@ -505,13 +517,13 @@ struct Attend : Tiles<DIM, BITS, NT> {
   __half2 f;                                     // power of two that takes quarter g & 3's scales of values to 1 or below
   uint32_t ones;
 
-  // The queries of an item, and nothing seen yet
-  __device__ __forceinline__ void begin(const AttendParams &p, int b, int kv_head, int lane) {
+  // An item's queries, `stride` apart (global or shared memory), and nothing seen yet
+  __device__ __forceinline__ void begin(const AttendParams &p, const T *queries, long long stride, int lane) {
     const int t = lane & 3, g = lane >> 2;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const bool live = nt * 8 + g < p.group;
-      const T *const q = static_cast<const T *>(p.q) + b * p.q_seq + (kv_head * p.group + (live ? nt * 8 + g : 0)) * p.q_head;
+      const T *const q = queries + (live ? nt * 8 + g : 0) * stride;
       float x[4][2 * J], top = 0.0f;             // of the lane's two chunks
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -791,19 +803,25 @@ __global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(BLOCKS)) attend_tiles(
   pdl_trigger();
   make_line(p, line, sums);
   __syncthreads();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (a warp's number that the compiler knows to be one for the warp)
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int r = warp * gridDim.x + blockIdx.x, parts = min(p.warps, line.total);          // (few stretches: on as many SMs)
   if (r >= parts) return;
   const int first = begin_of(line.total, parts, r), last = begin_of(line.total, parts, r + 1);
-  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * (STAGES * A::STAGE);
+  unsigned char *const own = smem + warp * A::WARP_SMEM;
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(own));
   Place ahead, now;
   now.start(p, line, first);
   ahead = now;
-  int fetched = first;
+  int fetched = first, queries_of = -1;          // the first tile of the item whose queries wait in shared memory
   auto fetch = [&]() {
     if (fetched < last) {
       A::load(p, ahead, ring + (fetched - first) % STAGES * A::STAGE, lane);
-      ahead.next(p);
+      if (A::QUERIES && queries_of < 0 && (ahead.tile == 0 || fetched == first)) {
+        A::template load_queries<typename A::Value>(p, ahead, ring + STAGES * A::STAGE, lane);
+        queries_of = fetched;
+      }
+      ahead.next(p, line);
     }
     ++fetched;
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -811,11 +829,22 @@ __global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(BLOCKS)) attend_tiles(
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) fetch();
   A a;
-  a.begin(p, now.b, now.head, lane);
   int began = now.tile;
   for (int i = first; i < last; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     __syncwarp();                                // every lane's copies of tile i are there, and tile i - 1 has been read
+    if (now.tile == 0 || i == first) {
+      const typename A::Value *q = static_cast<const typename A::Value *>(p.q) + now.b * p.q_seq + static_cast<long long>(now.head) * p.group * p.q_head;
+      long long stride = p.q_head;
+      if (A::QUERIES && queries_of == i) {
+        q = reinterpret_cast<const typename A::Value *>(own + STAGES * A::STAGE);
+        stride = A::QUERY_STRIDE;
+      }
+      a.begin(p, q, stride, lane);
+      __syncwarp();                              // (read by all lanes before the next are copied)
+      if (queries_of == i) queries_of = -1;
+      began = now.tile;
+    }
     fetch();
     a.tile(ring + (i - first) % STAGES * A::STAGE, min(now.rows - now.tile * TILE, TILE), lane);
     const bool done = now.tile == now.tiles - 1;
@@ -823,95 +852,133 @@ __global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(BLOCKS)) attend_tiles(
       const bool whole = done && began == 0;
       a.end(p, now.b, now.head, whole ? -1 : 2 * r + (began == 0 && i - first > now.tile), lane);
     }
-    if (i == last - 1) break;
-    now.next(p);
-    if (done) {
-      a.begin(p, now.b, now.head, lane);
-      began = 0;
-    }
+    if (i < last - 1) now.next(p, line);
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// A CTA joins the parts of a (sequence, query head): a warp takes every JOIN_WARPS-th, eight at a time.
-constexpr int JOIN_WARPS = 8;
+// The join: outputs of items whose parts lie in several stretches, and of sequences without rows.
+// (a maximum of -inf: nothing seen, or a sum that is no number and stays one)
+__device__ __forceinline__ float part_weight(float m, float l, float top) { return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2f(m - top); }
+template <int DIM, int AHEAD>
+struct Joined {
+  static constexpr int E = DIM / 32;
+  float M, L, A[E];                              // dimensions lane * E ... of the warp's parts
+  // parts of stretches r0 + from, r0 + from + step, ... up to r1, AHEAD at a time; `inside`: the first is not the first item of its stretch
+  __device__ __forceinline__ void take(const AttendParams &p, int r0, int r1, int from, int step, bool inside, int head, int lane) {
+    M = -INFINITY;
+    L = 0.0f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) A[i] = 0.0f;
+    for (int first = r0 + from; first <= r1; first += step * AHEAD) {
+      float v[AHEAD][E];
+      float2 ml[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const int r = first + i * step;
+        ml[i] = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+        for (int k = 0; k < E; ++k) v[i][k] = 0.0f;
+        if (r <= r1) {
+          const size_t at = static_cast<size_t>(2 * r + (r == r0 && inside)) * p.group + head;
+          ml[i] = p.part_ml[at];
+          const float *const src = p.part_out + at * DIM + lane * E;
+          if constexpr (E == 4) { const float4 a = *reinterpret_cast<const float4 *>(src); v[i][0] = a.x; v[i][1] = a.y; v[i][E - 2] = a.z; v[i][E - 1] = a.w; }
+          else { const float2 a = *reinterpret_cast<const float2 *>(src); v[i][0] = a.x; v[i][1] = a.y; }
+        }
+      }
+      float top = M;
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) top = fmaxf(top, ml[i].x);
+      const float f0 = part_weight(M, L, top);
+      M = top;
+      L *= f0;
+#pragma unroll
+      for (int k = 0; k < E; ++k) A[k] *= f0;
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const float f = part_weight(ml[i].x, ml[i].y, top);
+        L = fmaf(ml[i].y, f, L);
+#pragma unroll
+        for (int k = 0; k < E; ++k) A[k] = fmaf(v[i][k], f, A[k]);
+      }
+    }
+  }
+};
+template <typename T>
+__device__ __forceinline__ void zero_empty(const AttendParams &p, const Line &line, int dim, int first, int step, int lane) {
+  for (int b = first; b < p.caches.seqs; b += step) {
+    if (line.rows[b] > 0) continue;
+    const size_t row = static_cast<size_t>(b) * p.q_heads;
+    for (int i = lane; i < p.q_heads * (dim / 8); i += 32) *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + row * dim + i * 8) = make_uint4(0, 0, 0, 0);
+    for (int i = lane; p.lse && i < p.q_heads; i += 32) p.lse[row + i] = -INFINITY;
+  }
+}
+// A warp takes a query head of an item: for items of few parts.
+constexpr int FEW = 4;                           // parts asked for together
 template <typename T, int DIM>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) join_stretches(const __grid_constant__ AttendParams p) {
-  constexpr int E = DIM / 32, AHEAD = 8;
+__global__ void __launch_bounds__(256) join_few(const __grid_constant__ AttendParams p) {
   __shared__ Line line;
   __shared__ int sums[MAX_SEQS / 32];
-  __shared__ float sm[JOIN_WARPS], sl[JOIN_WARPS];
-  __shared__ __align__(16) float sa[JOIN_WARPS][DIM];
-  const int b = static_cast<int>(blockIdx.x) / p.q_heads, head = static_cast<int>(blockIdx.x) % p.q_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, w = static_cast<int>(blockIdx.x) * 8 + warp, warps = static_cast<int>(gridDim.x) * 8;
   // (the lengths were there before the kernel that this one follows)
   make_line(p, line, sums);
   __syncthreads();
-  const int tiles = tiles_of(seen_rows(p, b));
-  const size_t row = blockIdx.x;
+  const int parts = min(p.warps, line.total);
+  pdl_wait();
+  zero_empty<T>(p, line, DIM, w, warps, lane);
+  // unit: a stretch that begins inside an item, as the first to do so, and a query head
+  for (int u = w; u < (parts - 1) * p.group; u += warps) {
+    const int r = u / p.group + 1, head = u - (r - 1) * p.group, t = begin_of(line.total, parts, r), before = begin_of(line.total, parts, r - 1);
+    Place at;
+    at.start(p, line, t);
+    const int t0 = t - at.tile;
+    if (at.tile == 0 || before > t0) continue;
+    Joined<DIM, FEW> j;
+    j.take(p, r - 1, part_of(line.total, parts, t0 + at.tiles - 1), 0, 1, before < t0, head, lane);
+    const size_t row = static_cast<size_t>(at.b) * p.q_heads + at.head * p.group + head;
+    store_out<T, DIM>(static_cast<T *>(p.out) + row * DIM + lane * (DIM / 32), j.A, j.L == 0.0f ? 0.0f : 1.0f / j.L);
+    if (lane == 0 && p.lse) p.lse[row] = j.L == 0.0f ? -INFINITY : j.M * LN2 + logf(j.L);
+  }
+}
+// A CTA takes a query head of an item, its W warps every W-th part: for items of many.
+template <typename T, int DIM, int W>
+__global__ void __launch_bounds__(32 * W) join_many(const __grid_constant__ AttendParams p) {
+  constexpr int E = DIM / 32;
+  __shared__ Line line;
+  __shared__ int sums[MAX_SEQS / 32];
+  __shared__ float sm[W], sl[W];
+  __shared__ __align__(16) float sa[W][DIM];
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, row = blockIdx.x, b = row / p.q_heads, head = row - b * p.q_heads;
+  make_line(p, line, sums);
+  __syncthreads();
+  const int parts = min(p.warps, line.total), tiles = tiles_of(line.rows[b]);
   if (tiles == 0) {
     pdl_wait();
-    if (threadIdx.x < DIM) static_cast<T *>(p.out)[row * DIM + threadIdx.x] = static_cast<T>(0.0f);
-    if (threadIdx.x == 0 && p.lse) p.lse[row] = -INFINITY;
+    if (head == 0 && warp == 0) zero_empty<T>(p, line, DIM, b, MAX_SEQS, lane);
     return;
   }
-  const int parts = min(p.warps, line.total), t0 = line.before[b] + head / p.group * tiles;
-  const int r0 = part_of(line.total, parts, t0), r1 = part_of(line.total, parts, t0 + tiles - 1);
+  const int t0 = line.before[b] + head / p.group * tiles, r0 = part_of(line.total, parts, t0), r1 = part_of(line.total, parts, t0 + tiles - 1);
+  const bool inside = begin_of(line.total, parts, r0) < t0;
   pdl_wait();
   if (r0 == r1) return;                          // (written there)
-  const bool inside = begin_of(line.total, parts, r0) < t0;
-  float M = -INFINITY, L = 0.0f, A[E];
+  Joined<DIM, 8> j;
+  j.take(p, r0, r1, warp, W, inside, head % p.group, lane);
+  if (lane == 0) { sm[warp] = j.M; sl[warp] = j.L; }
 #pragma unroll
-  for (int i = 0; i < E; ++i) A[i] = 0.0f;
-  // (a maximum of -inf: nothing seen, or a sum that is no number and stays one)
-  auto weight = [](float m, float l, float top) { return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2f(m - top); };
-  for (int first = r0 + warp; first <= r1; first += JOIN_WARPS * AHEAD) {
-    float v[AHEAD][E];
-    float2 ml[AHEAD];
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      const int r = first + i * JOIN_WARPS;
-      ml[i] = make_float2(-INFINITY, 0.0f);
-#pragma unroll
-      for (int k = 0; k < E; ++k) v[i][k] = 0.0f;
-      if (r <= r1) {
-        const size_t at = static_cast<size_t>(2 * r + (r == r0 && inside)) * p.group + head % p.group;
-        ml[i] = p.part_ml[at];
-        const float *const src = p.part_out + at * DIM + lane * E;
-        if constexpr (E == 4) { const float4 a = *reinterpret_cast<const float4 *>(src); v[i][0] = a.x; v[i][1] = a.y; v[i][E - 2] = a.z; v[i][E - 1] = a.w; }
-        else { const float2 a = *reinterpret_cast<const float2 *>(src); v[i][0] = a.x; v[i][1] = a.y; }
-      }
-    }
-    float top = M;
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) top = fmaxf(top, ml[i].x);
-    const float f0 = weight(M, L, top);
-    M = top;
-    L *= f0;
-#pragma unroll
-    for (int k = 0; k < E; ++k) A[k] *= f0;
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      const float f = weight(ml[i].x, ml[i].y, top);
-      L = fmaf(ml[i].y, f, L);
-#pragma unroll
-      for (int k = 0; k < E; ++k) A[k] = fmaf(v[i][k], f, A[k]);
-    }
-  }
-  if (lane == 0) { sm[warp] = M; sl[warp] = L; }
-#pragma unroll
-  for (int i = 0; i < E; ++i) sa[warp][lane * E + i] = A[i];
+  for (int i = 0; i < E; ++i) sa[warp][lane * E + i] = j.A[i];
   __syncthreads();
   if (threadIdx.x >= DIM) return;
-  float top = -INFINITY, total = 0.0f, out = 0.0f;
+  float top = -INFINITY, total = 0.0f, sum = 0.0f;
 #pragma unroll
-  for (int w = 0; w < JOIN_WARPS; ++w) top = fmaxf(top, sm[w]);
+  for (int i = 0; i < W; ++i) top = fmaxf(top, sm[i]);
 #pragma unroll
-  for (int w = 0; w < JOIN_WARPS; ++w) {
-    const float f = weight(sm[w], sl[w], top);
-    total = fmaf(sl[w], f, total);
-    out = fmaf(sa[w][threadIdx.x], f, out);
+  for (int i = 0; i < W; ++i) {
+    const float f = part_weight(sm[i], sl[i], top);
+    total = fmaf(sl[i], f, total);
+    sum = fmaf(sa[i][threadIdx.x], f, sum);
   }
-  static_cast<T *>(p.out)[row * DIM + threadIdx.x] = static_cast<T>(total == 0.0f ? 0.0f : out / total);
+  static_cast<T *>(p.out)[static_cast<size_t>(row) * DIM + threadIdx.x] = static_cast<T>(total == 0.0f ? 0.0f : sum / total);
   if (p.lse && threadIdx.x == 0) p.lse[row] = total == 0.0f ? -INFINITY : top * LN2 + logf(total);
 }
 

@@ -104,6 +104,19 @@ int warps_of(int seqs, int kv_heads, int group, int rows) {
 }
 long long workspace_bytes(int warps, int group, int dim) { return 2ll * warps * group * (dim * 4ll + 8); }
 
+// How the parts are joined goes by how many an item has where all stretches are used: warps, or CTAs of eight or 32 warps.
+template <typename T, int DIM>
+cudaError_t launch_join(const AttendParams &p, cudaStream_t stream) {
+  const qmk_tc::PdlScope scope(true);
+  const int rows = p.caches.seqs * p.q_heads, each = p.warps / (p.caches.seqs * p.caches.kv_heads);
+  if (each <= FEW) {
+    const int units = std::max(p.warps * p.group, p.caches.seqs);
+    return qmk_tc::launch_kernel(join_few<T, DIM>, dim3(std::min((units + 7) / 8, 8 * SMS)), dim3(256), 0, stream, p);
+  }
+  if (each <= 64) return qmk_tc::launch_kernel(join_many<T, DIM, 8>, dim3(rows), dim3(256), 0, stream, p);
+  return qmk_tc::launch_kernel(join_many<T, DIM, 32>, dim3(rows), dim3(1024), 0, stream, p);
+}
+
 template <typename A, int BLOCKS>
 cudaError_t launch_tiles(const AttendParams &p, cudaStream_t stream) {
   const cudaError_t e = cudaFuncSetAttribute(attend_tiles<A, BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, A::SMEM);
@@ -118,8 +131,7 @@ cudaError_t attend(const AttendParams &p, cudaStream_t stream) {
                         : p.group <= 8     ? launch_tiles<Attend<T, DIM, BITS, 1>, 1>(p, stream)
                                            : launch_tiles<Attend<T, DIM, BITS, 2>, 2>(p, stream);
   if (e != cudaSuccess) return e;
-  const qmk_tc::PdlScope scope(true);
-  return qmk_tc::launch_kernel(join_stretches<T, DIM>, dim3(p.caches.seqs * p.q_heads), dim3(JOIN_WARPS * 32), 0, stream, p);
+  return launch_join<T, DIM>(p, stream);
 }
 template <typename T>
 cudaError_t attend(const AttendParams &p, int dim, int bits, cudaStream_t stream) {
