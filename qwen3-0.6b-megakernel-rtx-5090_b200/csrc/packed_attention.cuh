@@ -942,7 +942,7 @@ __global__ void __launch_bounds__(256) join_few(const __grid_constant__ AttendPa
   }
 }
 // A CTA takes a query head of an item, its W warps every W-th part: for items of many.
-template <typename T, int DIM, int W>
+template <typename T, int DIM, int W, int AHEAD>
 __global__ void __launch_bounds__(32 * W) join_many(const __grid_constant__ AttendParams p) {
   constexpr int E = DIM / 32;
   __shared__ Line line;
@@ -962,7 +962,7 @@ __global__ void __launch_bounds__(32 * W) join_many(const __grid_constant__ Atte
   const bool inside = begin_of(line.total, parts, r0) < t0;
   pdl_wait();
   if (r0 == r1) return;                          // (written there)
-  Joined<DIM, 8> j;
+  Joined<DIM, AHEAD> j;
   j.take(p, r0, r1, warp, W, inside, head % p.group, lane);
   if (lane == 0) { sm[warp] = j.M; sl[warp] = j.L; }
 #pragma unroll

@@ -64,8 +64,7 @@ template <> struct Type<__nv_bfloat16> {
 template <typename V> __device__ __forceinline__ uint32_t bits_of(V x) { return *reinterpret_cast<const uint32_t *>(&x); }
 template <typename V> __device__ __forceinline__ V from_bits(uint32_t x) { return *reinterpret_cast<const V *>(&x); }
 
-// Eight lanes share a row; lane g of them has the codes of dimensions DIM/4 b + DIM/32 g + j.  A row of the call: (sequence, head, row), rows first, so that
-// the four rows of a warp lie together in the cache.
+// A row of the call: (sequence, head, row), rows first, so that the rows of a warp lie together in the cache.
 struct RowOfCall {
   int b, head, t, at;                            // at: row of the cache
   bool there;
@@ -82,104 +81,143 @@ __device__ __forceinline__ RowOfCall row_of(const RowParams &p, unsigned int i) 
   return r;
 }
 
-// The code of x.  The quotient in fp32 is off by 2^-20 (4 bits; 8: 2^-16) at most; where that may cross a border the exact one decides: difference and
-// product of fp16 numbers are exact in 64 bits, and a quotient of them is not within 2^-53 of a border that it is not on.
-template <int BITS>
-__device__ __forceinline__ uint32_t code_of(float x, float z, float s, float inverse) {
-  constexpr float M = 1 << (BITS - 1), NEAR = BITS == 4 ? 0x1p-18f : 0x1p-14f;
-  const float t = (x - z) * inverse;
-  float n = rintf(t);
-  if (fabsf(t - n) > 0.5f - NEAR) n = static_cast<float>(rint((static_cast<double>(x) - static_cast<double>(z)) / static_cast<double>(s)));
-  return static_cast<uint32_t>(fminf(fmaxf(n + M, 0.0f), 2.0f * M - 1.0f));
+template <typename Two> __device__ __forceinline__ Two shuffled(Two x, int o) { return from_bits<Two>(__shfl_xor_sync(0xffffffffu, bits_of(x), o)); }
+// (a.low, b.low), (a.high, b.high), (a.low, b.high)
+template <typename Two> __device__ __forceinline__ Two lows(Two a, Two b) { return from_bits<Two>(__byte_perm(bits_of(a), bits_of(b), 0x5410)); }
+template <typename Two> __device__ __forceinline__ Two highs(Two a, Two b) { return from_bits<Two>(__byte_perm(bits_of(a), bits_of(b), 0x7632)); }
+template <typename Two> __device__ __forceinline__ Two low_high(Two a, Two b) { return from_bits<Two>(__byte_perm(bits_of(a), bits_of(b), 0x7610)); }
+// Two fp32 operations in one
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{.reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%6, %7}; fma.rn.f32x2 x, x, y, z; mov.b64 {%0, %1}, x;}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x;}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 
-// One row of values (at `src`, this lane's DIM/8) to a packed one.
+// A row of values to a packed one at `dst` (where `there`): four lanes, x[b] lane t's DIM/16 of quarter b, those of chunks 2 t and 2 t + 1.
+//
+// The quarters' least and largest values are reduced and scattered: each lane ends up with one quarter's, makes its scale and centre and hands out what the codes are computed
+// with, so a division is done once a lane.  A code: t = x / s + (M - z / s), one multiply-add; t + 1.5 2^23 is it rounded, in the low bits of a word, and a
+// shift and an addition put it into its place, the 1.5 2^23 of all taken off at once.  All but those for two values at a time.  What t is off by may cross a border: exact
+// halves are common (x, z and s have eleven bits each), so quarters with a t that near one are looked at again, value by value, in 64 bits, where difference and
+// products are exact; and those whose rounded scale and centre lead codes out of range, which are clamped there.
 template <typename T, int DIM, int BITS>
-__device__ __forceinline__ void pack_row(const uint32_t (&x)[4][DIM / 64], unsigned char *dst, int g, bool there) {
+__device__ __forceinline__ void pack_row(const uint32_t (&x)[4][DIM / 32], unsigned char *dst, int lane, bool there) {
   using Two = typename Type<T>::Two;
-  constexpr int W = DIM / 64, CODES = DIM / 8;   // 32-bit words of values in a quarter; codes of the lane
-  constexpr float M = 1 << (BITS - 1), LEVELS = (1 << BITS) - 1;
-  // least and largest value of the quarters, two in a register, over the eight lanes
-  Two lo[2], hi[2];
+  constexpr int W = DIM / 32, J = DIM / 32, CODES = DIM / 4, PER_WORD = 32 / BITS;         // words of values in a quarter; codes of a quarter in a chunk, of the lane, of a word
+  constexpr float M = 1 << (BITS - 1), LEVELS = (1 << BITS) - 1, MAGIC = 12582912.0f;
+  const int t = lane & 3;
+  Two lo[2], hi[2];                              // least and largest of quarters (0, 1) and (2, 3) in the lane
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     Two l[2], h[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       l[b] = h[b] = from_bits<Two>(x[2 * i + b][0]);
-      if (W == 2) { l[b] = __hmin2_nan(l[b], from_bits<Two>(x[2 * i + b][W - 1])); h[b] = __hmax2_nan(h[b], from_bits<Two>(x[2 * i + b][W - 1])); }
-    }
-    lo[i] = __hmin2_nan(from_bits<Two>(__byte_perm(bits_of(l[0]), bits_of(l[1]), 0x5410)), from_bits<Two>(__byte_perm(bits_of(l[0]), bits_of(l[1]), 0x7632)));
-    hi[i] = __hmax2_nan(from_bits<Two>(__byte_perm(bits_of(h[0]), bits_of(h[1]), 0x5410)), from_bits<Two>(__byte_perm(bits_of(h[0]), bits_of(h[1]), 0x7632)));
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-      lo[i] = __hmin2_nan(lo[i], from_bits<Two>(__shfl_xor_sync(0xffffffffu, bits_of(lo[i]), o)));
-      hi[i] = __hmax2_nan(hi[i], from_bits<Two>(__shfl_xor_sync(0xffffffffu, bits_of(hi[i]), o)));
+      for (int w = 1; w < W; ++w) { l[b] = __hmin2_nan(l[b], from_bits<Two>(x[2 * i + b][w])); h[b] = __hmax2_nan(h[b], from_bits<Two>(x[2 * i + b][w])); }
     }
+    lo[i] = __hmin2_nan(lows(l[0], l[1]), highs(l[0], l[1]));
+    hi[i] = __hmax2_nan(lows(h[0], h[1]), highs(h[0], h[1]));
   }
-  uint32_t words[CODES * BITS / 32];
-  uint32_t mine = 0;                             // this lane's 16 bits of the trailer
+  // the upper two lanes go on with quarters 2 and 3, the odd ones with the second of those
+  const bool upper = t & 2, second = t & 1;
+  const Two l = __hmin2_nan(upper ? lo[1] : lo[0], shuffled(upper ? lo[0] : lo[1], 2)), h = __hmax2_nan(upper ? hi[1] : hi[0], shuffled(upper ? hi[0] : hi[1], 2));
+  const Two first = lows(l, h), other = highs(l, h), mine = second ? other : first, come = shuffled(second ? first : other, 1);
+  const float2 range = Type<T>::floats(low_high(__hmin2_nan(mine, come), __hmax2_nan(mine, come)));
+  const bool good = range.x >= -65504.0f && range.y <= 65504.0f;
+  const __half sh = good ? __float2half_rn((range.y - range.x) / LEVELS) : __ushort_as_half(0x7fff);
+  const float s = __half2float(sh);
+  const __half zh = good ? __float2half_rn(fmaf(M, s, range.x)) : __ushort_as_half(0x7fff);
+  const float z = __half2float(zh);
+  // t = x k + c; k, c and the sum are rounded once each, k's error counts for x - z: off by (2 LEVELS + 2 + |c|) 2^-24 at most
+  const float k0 = s > 0.0f ? __frcp_rn(s) : 0.0f, c0 = good ? fmaf(-z, k0, M) : M, off = (2.0f * LEVELS + 2.0f + fabsf(c0)) * 0x1p-24f;
+  const bool inside = fmaf(range.x, k0, c0) > -0.5f + off && fmaf(range.y, k0, c0) < LEVELS + 0.5f - off;
+  const float limit0 = s > 0.0f ? inside ? 0.5f - off : -1.0f : 1.0f;
+  const uint32_t pair = __half_as_ushort(sh) | static_cast<uint32_t>(__half_as_ushort(zh)) << 16;
+  uint32_t words[CODES / PER_WORD];
 #pragma unroll
-  for (int i = 0; i < CODES * BITS / 32; ++i) words[i] = 0;
+  for (int i = 0; i < CODES / PER_WORD; ++i) words[i] = 0u - 0x4b400000u * (BITS == 4 ? 0x11111111u : 0x01010101u);
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
-    const float2 l2 = Type<T>::floats(lo[b / 2]), h2 = Type<T>::floats(hi[b / 2]);
-    const float low = b % 2 ? l2.y : l2.x, high = b % 2 ? h2.y : h2.x;
-    const bool good = low >= -65504.0f && high <= 65504.0f;
-    const __half sh = good ? __float2half_rn((high - low) / LEVELS) : __ushort_as_half(0x7fff);
-    const float s = __half2float(sh);
-    const __half zh = good ? __float2half_rn(fmaf(M, s, low)) : __ushort_as_half(0x7fff);
-    const float z = __half2float(zh), inverse = s > 0.0f ? 1.0f / s : 0.0f;
-    if (g == b) mine = __half_as_ushort(sh);
-    if (g == 4 + b) mine = __half_as_ushort(zh);
+    const float k = __shfl_sync(0xffffffffu, k0, b, 4), c = __shfl_sync(0xffffffffu, c0, b, 4), limit = __shfl_sync(0xffffffffu, limit0, b, 4);
+    float worst = 0.0f;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const float2 v = Type<T>::floats(from_bits<Two>(x[b][w]));
+      const float2 u = fma2(Type<T>::floats(from_bits<Two>(x[b][w])), make_float2(k, k), make_float2(c, c)), y = add2(u, make_float2(MAGIC, MAGIC)),
+                   n = add2(y, make_float2(-MAGIC, -MAGIC)), r = add2(u, make_float2(-n.x, -n.y));
+      worst = fmaxf(worst, fmaxf(fabsf(r.x), fabsf(r.y)));
+      // values 2 w and 2 w + 1: of chunk w / (W / 2), the codes (2 w) % J and the next of the quarter
+      const int index = CODES / 2 * (2 * w / J) + J * b + 2 * w % J, word = index / PER_WORD, place = index % PER_WORD;
+      words[word] += __float_as_uint(y.x) << (BITS * place);
+      words[word] += __float_as_uint(y.y) << (BITS * (place + 1));
+    }
+    if (__any_sync(0xffffffffu, worst > limit)) {
+      const uint32_t both = __shfl_sync(0xffffffffu, pair, b, 4);
+      const double sd = __half2float(__ushort_as_half(both & 0xffffu)), zd = __half2float(__ushort_as_half(both >> 16));
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int index = 2 * W * b + 2 * w + j;
-        const uint32_t n = inverse > 0.0f ? code_of<BITS>(j ? v.y : v.x, z, s, inverse) : 1u << (BITS - 1);
-        words[index * BITS / 32] |= n << (index * BITS % 32);
+      for (int w = 0; w < W; ++w) {
+        const float2 v = Type<T>::floats(from_bits<Two>(x[b][w])), u = fma2(v, make_float2(k, k), make_float2(c, c));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float y = (j ? u.y : u.x) + MAGIC, n = y - MAGIC, r = (j ? u.y : u.x) - n;
+          if (fabsf(r) > limit) {
+            const float m = r < 0.0f ? n - 1.0f : n;       // between codes m and m + 1
+            const double above = (static_cast<double>(j ? v.y : v.x) - zd) - (static_cast<double>(m - M) + 0.5) * sd;
+            const float code = fminf(fmaxf(above > 0.0 || (above == 0.0 && (static_cast<int>(m) & 1)) ? m + 1.0f : m, 0.0f), LEVELS);
+            const int index = CODES / 2 * (2 * w / J) + J * b + 2 * w % J + j;
+            words[index / PER_WORD] += static_cast<uint32_t>(static_cast<int>(code - n)) << (BITS * (index % PER_WORD));
+          }
+        }
       }
     }
   }
   if (!there) return;
-  unsigned char *const to = dst + g * (CODES * BITS / 8);
-  if constexpr (CODES * BITS == 128) *reinterpret_cast<uint4 *>(to) = make_uint4(words[0], words[1], words[2], words[3]);
-  else if constexpr (CODES * BITS == 64) *reinterpret_cast<uint2 *>(to) = make_uint2(words[0], words[1]);
-  else *reinterpret_cast<uint32_t *>(to) = words[0];
-  *reinterpret_cast<unsigned short *>(dst + DIM * BITS / 8 + 2 * g) = static_cast<unsigned short>(mine);
+  uint4 *const to = reinterpret_cast<uint4 *>(dst + t * (CODES * BITS / 8));
+  if constexpr (CODES * BITS == 64) *reinterpret_cast<uint2 *>(to) = make_uint2(words[0], words[1]);
+  else {
+#pragma unroll
+    for (int i = 0; i < CODES * BITS / 128; ++i) to[i] = make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
+  }
+  unsigned short *const trailer = reinterpret_cast<unsigned short *>(dst + DIM * BITS / 8);
+  trailer[t] = static_cast<unsigned short>(pair);
+  trailer[4 + t] = static_cast<unsigned short>(pair >> 16);
 }
 
-// This lane's words of a row of values: two or four at a time of each quarter
+// Lane t's words of a row of values: DIM/16 of each quarter, side by side
 template <int DIM>
-__device__ __forceinline__ void load_values(const void *src, int g, bool there, uint32_t (&x)[4][DIM / 64]) {
+__device__ __forceinline__ void load_values(const void *src, int t, bool there, uint32_t (&x)[4][DIM / 32]) {
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
-    const char *const at = static_cast<const char *>(src) + (DIM / 4 * b + DIM / 32 * g) * 2;
+    const char *const at = static_cast<const char *>(src) + (DIM / 4 * b + DIM / 16 * t) * 2;
     if constexpr (DIM == 128) {
-      const uint2 w = there ? __ldg(reinterpret_cast<const uint2 *>(at)) : make_uint2(0, 0);
-      x[b][0] = w.x;
-      x[b][DIM / 64 - 1] = w.y;
+      const uint4 w = there ? __ldg(reinterpret_cast<const uint4 *>(at)) : make_uint4(0, 0, 0, 0);
+      x[b][0] = w.x; x[b][1] = w.y; x[b][DIM / 32 - 2] = w.z; x[b][DIM / 32 - 1] = w.w;
     } else {
-      x[b][0] = there ? __ldg(reinterpret_cast<const uint32_t *>(at)) : 0u;
+      const uint2 w = there ? __ldg(reinterpret_cast<const uint2 *>(at)) : make_uint2(0, 0);
+      x[b][0] = w.x; x[b][1] = w.y;
     }
   }
 }
 
 template <typename T, int DIM, int BITS>
 __global__ void __launch_bounds__(THREADS) write_rows(const __grid_constant__ RowParams p, unsigned int count) {
-  const int g = threadIdx.x & 7;
-  for (unsigned int first = blockIdx.x * (THREADS / 8); first < count; first += gridDim.x * (THREADS / 8)) {
-    const unsigned int i = first + (threadIdx.x >> 3);
+  const int lane = threadIdx.x & 31, t = lane & 3;
+  for (unsigned int first = blockIdx.x * (THREADS / 4); first < count; first += gridDim.x * (THREADS / 4)) {
+    const unsigned int i = first + (threadIdx.x >> 2);
     const RowOfCall r = row_of(p, i < count ? i : count - 1);
     const bool there = r.there && i < count;
     const long long from = r.b * p.seq + r.head * p.head + r.t * p.row, to = r.head * p.caches.head + r.at * p.caches.row;
-    uint32_t k[4][DIM / 64], v[4][DIM / 64];
-    load_values<DIM>(static_cast<const T *>(p.k) + from, g, there, k);
-    load_values<DIM>(static_cast<const T *>(p.v) + from, g, there, v);
-    pack_row<T, DIM, BITS>(k, const_cast<unsigned char *>(p.caches.k[r.b]) + to, g, there);
-    pack_row<T, DIM, BITS>(v, const_cast<unsigned char *>(p.caches.v[r.b]) + to, g, there);
+    uint32_t k[4][DIM / 32], v[4][DIM / 32];
+    load_values<DIM>(static_cast<const T *>(p.k) + from, t, there, k);
+    load_values<DIM>(static_cast<const T *>(p.v) + from, t, there, v);
+    pack_row<T, DIM, BITS>(k, const_cast<unsigned char *>(p.caches.k[r.b]) + to, lane, there);
+    pack_row<T, DIM, BITS>(v, const_cast<unsigned char *>(p.caches.v[r.b]) + to, lane, there);
   }
 }
 

@@ -90,7 +90,7 @@ int rows_call(const char *who, const qmk_packed_cache *cache, const qmk_packed_r
   if (const char *why = read_rows_of(rows, &p)) return refuse(who, why);
   const unsigned int count = static_cast<unsigned int>(p.caches.seqs) * p.caches.kv_heads * p.rows;
   if (count == 0) return QMK_OK;
-  const unsigned int blocks = std::min((count + THREADS / 8 - 1) / (THREADS / 8), 148u * 16);
+  const unsigned int rows_of_block = THREADS / (write ? 4 : 8), blocks = std::min((count + rows_of_block - 1) / rows_of_block, 148u * 16);
   void (*const kernel)(RowParams, unsigned int) = rows->type == 0 ? row_kernel<__half>(write, cache->head_dim, cache->bits) : row_kernel<__nv_bfloat16>(write, cache->head_dim, cache->bits);
   kernel<<<blocks, THREADS, 0, stream>>>(p, count);
   return answer(who, cudaGetLastError());
@@ -104,7 +104,7 @@ int warps_of(int seqs, int kv_heads, int group, int rows) {
 }
 long long workspace_bytes(int warps, int group, int dim) { return 2ll * warps * group * (dim * 4ll + 8); }
 
-// How the parts are joined goes by how many an item has where all stretches are used: warps, or CTAs of eight or 32 warps.
+// How the parts are joined goes by how many an item has where all stretches are used: warps, or CTAs of four, eight or 32 warps.
 template <typename T, int DIM>
 cudaError_t launch_join(const AttendParams &p, cudaStream_t stream) {
   const qmk_tc::PdlScope scope(true);
@@ -113,8 +113,9 @@ cudaError_t launch_join(const AttendParams &p, cudaStream_t stream) {
     const int units = std::max(p.warps * p.group, p.caches.seqs);
     return qmk_tc::launch_kernel(join_few<T, DIM>, dim3(std::min((units + 7) / 8, 8 * SMS)), dim3(256), 0, stream, p);
   }
-  if (each <= 64) return qmk_tc::launch_kernel(join_many<T, DIM, 8>, dim3(rows), dim3(256), 0, stream, p);
-  return qmk_tc::launch_kernel(join_many<T, DIM, 32>, dim3(rows), dim3(1024), 0, stream, p);
+  if (each <= 16) return qmk_tc::launch_kernel(join_many<T, DIM, 4, 4>, dim3(rows), dim3(128), 0, stream, p);
+  if (each <= 64) return qmk_tc::launch_kernel(join_many<T, DIM, 8, 8>, dim3(rows), dim3(256), 0, stream, p);
+  return qmk_tc::launch_kernel(join_many<T, DIM, 32, 8>, dim3(rows), dim3(1024), 0, stream, p);
 }
 
 template <typename A, int BLOCKS>
