@@ -22,11 +22,11 @@ constexpr int MAX_GROUP = 16;                    // query heads per kv head
 constexpr int TILE = 32;                         // rows
 constexpr int WARPS = 4, SMS = 148;
 // CTAs on an SM: what registers allow (168 a thread, 255 with two blocks of heads); tiles of a warp's ring: what their shared memory does
-constexpr int ctas_per_sm(int blocks) { return blocks == 1 ? 3 : 2; }
+constexpr int ctas_per_sm(int blocks, int row_bytes) { return blocks == 2 ? 2 : row_bytes <= 80 ? 4 : 3; }
 // (228 KB an SM; of a CTA 1 KB is the system's, 1.25 KB the line's)
-constexpr int warp_bytes(int blocks) { return (228 * 1024 - ctas_per_sm(blocks) * 2304) / (ctas_per_sm(blocks) * WARPS); }
+constexpr int warp_bytes(int blocks, int row_bytes) { return (228 * 1024 - ctas_per_sm(blocks, row_bytes) * 2304) / (ctas_per_sm(blocks, row_bytes) * WARPS); }
 constexpr int stages(int blocks, int row_bytes) {
-  const int fit = warp_bytes(blocks) / (2 * TILE * row_bytes);
+  const int fit = warp_bytes(blocks, row_bytes) / (2 * TILE * row_bytes);
   return fit < 4 ? fit : 4;
 }
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -196,7 +196,7 @@ struct Tiles {
   static constexpr int STAGE = 2 * TILE * ROW;                                              // keys, then values
   static constexpr int STAGES = stages(BLOCKS, ROW);
   // Queries of the next item, copied with its first rows; where a warp's shared memory has room
-  static constexpr int QUERIES = STAGES * STAGE + HEADS * DIM * 2 <= warp_bytes(BLOCKS) ? HEADS * DIM * 2 : 0;
+  static constexpr int QUERIES = STAGES * STAGE + HEADS * DIM * 2 <= warp_bytes(BLOCKS, ROW) ? HEADS * DIM * 2 : 0;
   static constexpr int QUERY_STRIDE = DIM, WARP_SMEM = STAGES * STAGE + QUERIES, SMEM = WARPS * WARP_SMEM;
   static constexpr float M = 1 << (BITS - 1), UNIT = 0x1p-24f;
   static constexpr bool SPREAD = BITS == 8 && DIM == 128;                                   // a lane's two chunks of keys: four apart, or one behind the other
@@ -794,7 +794,7 @@ struct Attend : Tiles<DIM, BITS, NT, 8 * NT> {
 };
 
 template <typename A, int BLOCKS>
-__global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(BLOCKS)) attend_tiles(const __grid_constant__ AttendParams p) {
+__global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(BLOCKS, A::ROW)) attend_tiles(const __grid_constant__ AttendParams p) {
   constexpr int STAGES = A::STAGES;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Line line;
@@ -925,7 +925,6 @@ __global__ void __launch_bounds__(256) join_few(const __grid_constant__ AttendPa
   make_line(p, line, sums);
   __syncthreads();
   const int parts = min(p.warps, line.total);
-  pdl_wait();
   zero_empty<T>(p, line, DIM, w, warps, lane);
   // unit: a stretch that begins inside an item, as the first to do so, and a query head
   for (int u = w; u < (parts - 1) * p.group; u += warps) {
@@ -934,12 +933,15 @@ __global__ void __launch_bounds__(256) join_few(const __grid_constant__ AttendPa
     at.start(p, line, t);
     const int t0 = t - at.tile;
     if (at.tile == 0 || before > t0) continue;
-    Joined<DIM, FEW> j;
-    j.take(p, r - 1, part_of(line.total, parts, t0 + at.tiles - 1), 0, 1, before < t0, head, lane);
+    const int r1 = part_of(line.total, parts, t0 + at.tiles - 1);
     const size_t row = static_cast<size_t>(at.b) * p.q_heads + at.head * p.group + head;
+    pdl_wait();                                  // (all the above passes under the other kernel's end)
+    Joined<DIM, FEW> j;
+    j.take(p, r - 1, r1, 0, 1, before < t0, head, lane);
     store_out<T, DIM>(static_cast<T *>(p.out) + row * DIM + lane * (DIM / 32), j.A, j.L == 0.0f ? 0.0f : 1.0f / j.L);
     if (lane == 0 && p.lse) p.lse[row] = j.L == 0.0f ? -INFINITY : j.M * LN2 + logf(j.L);
   }
+  pdl_wait();
 }
 // A CTA takes a query head of an item, its W warps every W-th part: for items of many.
 template <typename T, int DIM, int W, int AHEAD>

@@ -191,15 +191,15 @@ __device__ __forceinline__ void pack_row(const uint32_t (&x)[4][DIM / 32], unsig
 
 // Lane t's words of a row of values: DIM/16 of each quarter, side by side
 template <int DIM>
-__device__ __forceinline__ void load_values(const void *src, int t, bool there, uint32_t (&x)[4][DIM / 32]) {
+__device__ __forceinline__ void load_values(const void *src, int t, uint32_t (&x)[4][DIM / 32]) {
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
     const char *const at = static_cast<const char *>(src) + (DIM / 4 * b + DIM / 16 * t) * 2;
     if constexpr (DIM == 128) {
-      const uint4 w = there ? __ldg(reinterpret_cast<const uint4 *>(at)) : make_uint4(0, 0, 0, 0);
+      const uint4 w = __ldg(reinterpret_cast<const uint4 *>(at));
       x[b][0] = w.x; x[b][1] = w.y; x[b][DIM / 32 - 2] = w.z; x[b][DIM / 32 - 1] = w.w;
     } else {
-      const uint2 w = there ? __ldg(reinterpret_cast<const uint2 *>(at)) : make_uint2(0, 0);
+      const uint2 w = __ldg(reinterpret_cast<const uint2 *>(at));
       x[b][0] = w.x; x[b][1] = w.y;
     }
   }
@@ -214,8 +214,9 @@ __global__ void __launch_bounds__(THREADS) write_rows(const __grid_constant__ Ro
     const bool there = r.there && i < count;
     const long long from = r.b * p.seq + r.head * p.head + r.t * p.row, to = r.head * p.caches.head + r.at * p.caches.row;
     uint32_t k[4][DIM / 32], v[4][DIM / 32];
-    load_values<DIM>(static_cast<const T *>(p.k) + from, t, there, k);
-    load_values<DIM>(static_cast<const T *>(p.v) + from, t, there, v);
+    // (rows that go nowhere too: they are there, and starts and lengths need not be waited for)
+    load_values<DIM>(static_cast<const T *>(p.k) + from, t, k);
+    load_values<DIM>(static_cast<const T *>(p.v) + from, t, v);
     pack_row<T, DIM, BITS>(k, const_cast<unsigned char *>(p.caches.k[r.b]) + to, lane, there);
     pack_row<T, DIM, BITS>(v, const_cast<unsigned char *>(p.caches.v[r.b]) + to, lane, there);
   }

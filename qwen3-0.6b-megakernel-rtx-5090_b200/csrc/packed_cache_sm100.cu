@@ -2,6 +2,7 @@
 #include "../../include/qwen_megakernel.h"
 
 #include <algorithm>
+#include <atomic>
 #include <string>
 
 #include "engine_internal.h"
@@ -99,8 +100,8 @@ int rows_call(const char *who, const qmk_packed_cache *cache, const qmk_packed_r
 // Stretches of a call: a warp each, all resident together, not more than there can be tiles.
 long long most_tiles(int seqs, int kv_heads, int rows) { return static_cast<long long>(seqs) * kv_heads * ((rows + TILE - 1) / TILE); }
 int blocks_of(int group) { return group > 8 ? 2 : 1; }                    // of eight query heads
-int warps_of(int seqs, int kv_heads, int group, int rows) {
-  return static_cast<int>(std::min<long long>(std::max(most_tiles(seqs, kv_heads, rows), 1ll), SMS * ctas_per_sm(blocks_of(group)) * WARPS));
+int warps_of(int seqs, int kv_heads, int group, int dim, int bits, int rows) {
+  return static_cast<int>(std::min<long long>(std::max(most_tiles(seqs, kv_heads, rows), 1ll), SMS * ctas_per_sm(blocks_of(group), dim * bits / 8 + TRAILER) * WARPS));
 }
 long long workspace_bytes(int warps, int group, int dim) { return 2ll * warps * group * (dim * 4ll + 8); }
 
@@ -120,9 +121,17 @@ cudaError_t launch_join(const AttendParams &p, cudaStream_t stream) {
 
 template <typename A, int BLOCKS>
 cudaError_t launch_tiles(const AttendParams &p, cudaStream_t stream) {
-  const cudaError_t e = cudaFuncSetAttribute(attend_tiles<A, BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, A::SMEM);
+  // (once a device; the call takes half a microsecond)
+  static std::atomic<unsigned long long> known{0};
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  const unsigned long long bit = device < 64 ? 1ull << device : 0;
+  if (e == cudaSuccess && !(known.load() & bit)) {
+    e = cudaFuncSetAttribute(attend_tiles<A, BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, A::SMEM);
+    if (e == cudaSuccess) known |= bit;
+  }
   if (e != cudaSuccess) return e;
-  const int ctas = std::min(p.warps, SMS * ctas_per_sm(BLOCKS));         // (a warp of each where there are few)
+  const int ctas = std::min(p.warps, SMS * ctas_per_sm(BLOCKS, A::ROW));                    // (a warp of each where there are few)
   return qmk_tc::launch_kernel(attend_tiles<A, BLOCKS>, dim3(ctas), dim3(WARPS * 32), A::SMEM, stream, p);
 }
 template <typename T, int DIM, int BITS>
@@ -154,7 +163,7 @@ extern "C" long long qmk_attention_packed_cache_workspace(int num_sequences, int
       (head_dim != 64 && head_dim != 128) || (bits != 4 && bits != 8) || rows < 0 || rows > MAX_ROWS)
     return 0;
   if (most_tiles(num_sequences, kv_heads, rows) > 0x7fffffffll) return 0;
-  return workspace_bytes(warps_of(num_sequences, kv_heads, q_heads / kv_heads, rows), q_heads / kv_heads, head_dim);
+  return workspace_bytes(warps_of(num_sequences, kv_heads, q_heads / kv_heads, head_dim, bits, rows), q_heads / kv_heads, head_dim);
 }
 
 extern "C" int qmk_attention_packed_cache(const qmk_packed_cache *cache, const qmk_packed_attention *a, cudaStream_t stream) {
@@ -178,7 +187,7 @@ extern "C" int qmk_attention_packed_cache(const qmk_packed_cache *cache, const q
   p.group = a->q_heads / cache->kv_heads;
   p.lens = a->lens;
   p.scale_log2 = a->scale * LOG2E;
-  p.warps = warps_of(cache->num_sequences, cache->kv_heads, p.group, cache->rows);
+  p.warps = warps_of(cache->num_sequences, cache->kv_heads, p.group, cache->head_dim, cache->bits, cache->rows);
   p.part_out = static_cast<float *>(a->workspace);
   p.part_ml = reinterpret_cast<float2 *>(p.part_out + 2ll * p.warps * p.group * cache->head_dim);
   p.out = a->out;
