@@ -953,12 +953,15 @@ def read_cache_packed(k_cache, v_cache, rows: int, dim: int = 128, dtype: torch.
         raise RuntimeError(f"{who}: rows is negative")
     shape = (n, heads, rows, dim)
     if k_out is None and v_out is None:
-        k_out, v_out = torch.empty(shape, dtype=dtype, device=first.device), torch.empty(shape, dtype=dtype, device=first.device)
-    if k_out is None or v_out is None or not all(tuple(t.shape) == shape and t.dtype is dtype and t.get_device() == index for t in (k_out, v_out)):
-        raise RuntimeError(f"{who}: k_out and v_out must both be {list(shape)} of {dtype} on the caches' device")
-    strides = k_out.stride()
-    if strides != v_out.stride() or strides[3] != 1:
-        raise RuntimeError(f"{who}: k_out and v_out must have the same strides, contiguous along dim")
+        k_out = torch.empty(shape, dtype=dtype, device=first.device)
+        v_out = torch.empty_like(k_out)
+        strides = k_out.stride()
+    else:
+        if k_out is None or v_out is None or not all(tuple(t.shape) == shape and t.dtype is dtype and t.get_device() == index for t in (k_out, v_out)):
+            raise RuntimeError(f"{who}: k_out and v_out must both be {list(shape)} of {dtype} on the caches' device")
+        strides = k_out.stride()
+        if strides != v_out.stride() or strides[3] != 1:
+            raise RuntimeError(f"{who}: k_out and v_out must have the same strides, contiguous along dim")
     at, start = _starts(who, starts, n, index)
     args = _pack_packed_rows(code, rows, k_out.data_ptr(), v_out.data_ptr(), strides[0], strides[1], strides[2], at, _per_sequence(who, lens, n, index, "lens"), start)
     rc = _on_device(index, _lib.qmk_read_cache_packed, cache, args)
@@ -977,8 +980,8 @@ def attention_packed_cache(q: torch.Tensor, k_cache, v_cache, lens: torch.Tensor
     synchronise, may be captured in a graph (behind a call with these types and sizes on the device)."""
     who = "attention_packed_cache"
     dtype = q.dtype
-    code = _ROW_TYPES.get(dtype, -1)
-    if code < 0 or not q.is_cuda or q.dim() != 3 or q.stride(2) != 1:
+    code, strides = _ROW_TYPES.get(dtype, -1), q.stride()
+    if code < 0 or not q.is_cuda or len(strides) != 3 or strides[2] != 1:
         _require_cuda()
         raise RuntimeError(f"{who}: q must be a CUDA tensor [n, q_heads, dim] of fp16 or bf16, contiguous along dim")
     n, q_heads, dim = q.shape
@@ -987,13 +990,11 @@ def attention_packed_cache(q: torch.Tensor, k_cache, v_cache, lens: torch.Tensor
     seen = _per_sequence(who, lens, n, index, "lens")
     if not seen:
         raise RuntimeError(f"{who}: lens must be a contiguous int32 tensor with one value per sequence on the caches' device")
-    device = q.device
-    out = torch.empty_like(q) if q.is_contiguous() else torch.empty(n, q_heads, dim, dtype=dtype, device=device)
-    lse = torch.empty(n, q_heads, dtype=_FP32, device=device)
+    out = torch.empty_like(q) if q.is_contiguous() else torch.empty(n, q_heads, dim, dtype=dtype, device=q.device)
+    lse = torch.empty(n, q_heads, dtype=_FP32, device=q.device)
     need = _packed_attention_workspace(n, q_heads, heads, dim, bits, rows)
     workspace = lens.new_empty(need >> 2)
-    q_seq, q_head, _ = q.stride()
-    args = _pack_packed_attention(code, q_heads, q.data_ptr(), q_seq, q_head, seen, dim ** -0.5 if scale is None else scale, out.data_ptr(), lse.data_ptr(),
+    args = _pack_packed_attention(code, q_heads, q.data_ptr(), strides[0], strides[1], seen, dim ** -0.5 if scale is None else scale, out.data_ptr(), lse.data_ptr(),
                                   workspace.data_ptr(), need)
     rc = _on_device(index, _lib.qmk_attention_packed_cache, cache, args)
     if rc != 0:
