@@ -22,7 +22,7 @@ from __future__ import annotations
 import contextlib
 import math
 import os
-from typing import List, Optional, Sequence, Tuple
+from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -337,6 +337,14 @@ class Decoder:
         return self.tokenizer.decode(out, skip_special_tokens=True), len(ids), len(out)
 
 
+class ParkedSequence(NamedTuple):
+    """Cache rows that ``BatchDecoder.park_slot`` took out of a slot: packed, ``[num_layers, kv_heads, length, row bytes]``."""
+    k: torch.Tensor
+    v: torch.Tensor
+    length: int
+    bits: int
+
+
 class BatchDecoder:
     """Greedy decode of several independent sequences: up to four per persistent launch, up to 128 on the GEMM path.
 
@@ -517,6 +525,38 @@ class BatchDecoder:
         for group in passes:
             for b, ids in group:
                 self.positions[b] = len(ids)
+
+    def park_slot(self, b: int, bits: int = 8) -> "ParkedSequence":
+        """Slot ``b``'s cache rows in 8 or 4 bits (``write_cache_packed``): 0.56 or 0.31 of their fp16 bytes, for a conversation that waits for its
+        next turn.  The slot stays as it is and may be filled with another prompt; ``resume_slot`` brings the rows back.  Blocks."""
+        if not 0 <= b < self.num_sequences:
+            raise ValueError("slot out of range")
+        row_bytes = _require_megakernel_op("packed_row_bytes")(HEAD_DIM, bits)
+        length, layers = self.positions[b], self._base.num_layers
+        k, v = (torch.empty(layers, NUM_KV_HEADS, length, row_bytes, dtype=torch.uint8, device=self._base._embed_weight.device) for _ in range(2))
+        write = _require_megakernel_op("write_cache_packed")
+        for first in range(0, layers if length else 0, 128):           # (a call takes 128 caches)
+            part = slice(first, first + 128)
+            write(self._k_caches[b][part, :, :length], self._v_caches[b][part, :, :length], k[part], v[part])
+        torch.cuda.current_stream(k.device).synchronize()
+        return ParkedSequence(k, v, length, int(bits))
+
+    def resume_slot(self, b: int, parked: "ParkedSequence") -> None:
+        """Rows of a parked sequence back into slot ``b``, which goes on from its position (``read_cache_packed``: each value is the fp16 number
+        nearest to what its code stands for).  ``parked`` may be used again, in other slots and decoders of the same layers too.  Blocks."""
+        if not 0 <= b < self.num_sequences:
+            raise ValueError("slot out of range")
+        layers, length = self._base.num_layers, parked.length
+        if length > self.max_seq_len:
+            raise ValueError("parked sequence exceeds max_seq_len")
+        if parked.k.shape[0] != layers:
+            raise ValueError(f"parked sequence of {parked.k.shape[0]} layers, the decoder has {layers}")
+        read = _require_megakernel_op("read_cache_packed")
+        for first in range(0, layers if length else 0, 128):
+            part = slice(first, first + 128)
+            read(parked.k[part], parked.v[part], length, HEAD_DIM, k_out=self._k_caches[b][part, :, :length], v_out=self._v_caches[b][part, :, :length])
+        torch.cuda.current_stream(parked.k.device).synchronize()
+        self.positions[b] = length
 
     def decode_slots(self, slots: Sequence[int], first_tokens: Sequence[int], steps: int) -> List[List[int]]:
         """One launch: ``steps`` greedy tokens for every slot in ``slots`` (any subset, each from its own

@@ -519,3 +519,65 @@ def test_two_streams_at_once(gpu):
     torch.cuda.synchronize()
     for i in (0, 1):
         assert all(torch.equal(o, want[i][0]) and torch.equal(e, want[i][1]) for o, e in got[i])
+
+
+# ------------------------------------------------------------------------------------------------------------- sequences set aside
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+def test_a_parked_sequence_comes_back(gpu, bits):
+    """A slot's rows packed, the slot used for something else, the rows back in another slot: they are what the codes stand for, and decoding goes on exactly as from
+    a cache that holds those values."""
+    import synthetic as S
+    from Model.Qwen06B_architecture import BatchDecoder
+    w = S.make_weights(seed=31, num_layers=3, vocab_size=2048, norm_std=0.1, max_seq_len=16)
+    eng = BatchDecoder(weights=S.weights_to(w, "cuda"), tokenizer=S.StubTokenizer(-1, 2048), num_sequences=3, max_seq_len=96, engine="gemm", prefill_mode="tensor")
+    prompt = S.make_prompt(50, seed=3, vocab_size=2048)
+    eng.prefill_slot(0, prompt[:-1])
+    k, v = eng._k_caches[0][:, :, :49].clone(), eng._v_caches[0][:, :, :49].clone()
+    parked = eng.park_slot(0, bits)
+    assert parked.length == 49 and parked.bits == bits and parked.k.shape == (3, 8, 49, gpu.packed_row_bytes(128, bits))
+    assert torch.equal(parked.k.cpu(), packed(k, bits)) and torch.equal(parked.v.cpu(), packed(v, bits)) and torch.equal(eng._k_caches[0][:, :, :49], k)
+    eng.prefill_slot(0, S.make_prompt(20, seed=4, vocab_size=2048))
+    eng.prefill_slot(2, S.make_prompt(30, seed=5, vocab_size=2048))
+    behind = eng._k_caches[2][:, :, 49:].clone()
+    eng.resume_slot(2, parked)
+    assert eng.positions == [20, 0, 49]
+    for cache, x in ((eng._k_caches[2], k), (eng._v_caches[2], v)):
+        exact = values(packed(x, bits), 128)
+        assert bool(((cache[:, :, :49].double().cpu() - exact).abs() <= rounded_off(exact, torch.float16)).all())
+    assert torch.equal(eng._k_caches[2][:, :, 49:], behind)
+    eng._k_caches[1][:, :, :49], eng._v_caches[1][:, :, :49] = eng._k_caches[2][:, :, :49], eng._v_caches[2][:, :, :49]
+    torch.cuda.synchronize()
+    eng.positions[1] = 49
+    one, other = eng.decode_slots([1, 2], [prompt[-1]] * 2, 6)
+    assert one == other and eng.positions == [20, 55, 55]
+    for bad in (lambda: eng.park_slot(3), lambda: eng.resume_slot(-1, parked), lambda: eng.resume_slot(0, parked._replace(length=97)),
+                lambda: eng.resume_slot(0, parked._replace(k=parked.k[:2]))):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError):
+        eng.park_slot(0, 5)
+    assert eng.positions == [20, 55, 55]
+    eng.positions[0] = 0
+    empty = eng.park_slot(0)
+    eng.resume_slot(1, empty)
+    assert empty.length == 0 and eng.positions[1] == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+def test_caches_further_apart_than_32_bits(gpu, bits):
+    """Sequences and heads more than 4 GiB apart."""
+    size = gpu.packed_row_bytes(128, bits)
+    apart = (1 << 32) + 4096
+    memory = torch.empty(3 * apart + 20 * size, dtype=torch.uint8, device="cuda")
+    k, v, q = made(2, 2, 9, 128, seed=1), made(2, 2, 9, 128, seed=2), made(2, 4, 128, seed=3)
+    kc, vc = (memory[first:].as_strided((2, 2, 10, size), (2 * apart, apart, size, 1)) for first in (0, 10 * size))
+    gpu.write_cache_packed(k, v, kc, vc, 1)
+    assert torch.equal(kc[:, :, 1:].cpu(), packed(k, bits)) and torch.equal(vc[:, :, 1:].cpu(), packed(v, bits))
+    kc[:, :, 0], vc[:, :, 0] = kc[:, :, 1], vc[:, :, 1]
+    back = gpu.read_cache_packed(kc, vc, 10, 128)
+    exact = values(kc.cpu(), 128)
+    assert bool(((back[0].double().cpu() - exact).abs() <= rounded_off(exact, torch.float16)).all())
+    lens = torch.tensor([10, 7], dtype=torch.int32)
+    check_attention(gpu.attention_packed_cache(q, kc, vc, lens.cuda()), q, kc, vc, lens)
