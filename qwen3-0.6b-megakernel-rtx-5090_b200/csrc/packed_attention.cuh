@@ -22,13 +22,12 @@ constexpr int MAX_GROUP = 16;                    // query heads per kv head
 constexpr int TILE = 32;                         // rows
 constexpr int WARPS = 4, SMS = 148;
 // CTAs on an SM: what registers allow (168 a thread, 255 with two blocks of heads); tiles of a warp's ring: what their shared memory does
-constexpr int ctas_per_sm(int blocks, int row_bytes) { return blocks == 2 ? 2 : row_bytes <= 80 ? 4 : 3; }
+// How a tile is taken: by one or two query heads (PAIR), three or four (QUAD), blocks of up to eight (ONE, TWO)
+enum Way { PAIR, QUAD, ONE, TWO };
+__host__ __device__ constexpr Way way_of(int group) { return group <= 2 ? PAIR : group <= 4 ? QUAD : group <= 8 ? ONE : TWO; }
+__host__ __device__ constexpr int ctas_per_sm(Way way, int dim, int bits) { return way == TWO ? 2 : bits * dim <= 512 && (way != ONE || dim == 64) ? 4 : 3; }
 // (228 KB an SM; of a CTA 1 KB is the system's, 1.25 KB the line's)
-constexpr int warp_bytes(int blocks, int row_bytes) { return (228 * 1024 - ctas_per_sm(blocks, row_bytes) * 2304) / (ctas_per_sm(blocks, row_bytes) * WARPS); }
-constexpr int stages(int blocks, int row_bytes) {
-  const int fit = warp_bytes(blocks, row_bytes) / (2 * TILE * row_bytes);
-  return fit < 4 ? fit : 4;
-}
+constexpr int warp_bytes(int ctas) { return (228 * 1024 - ctas * 2304) / (ctas * WARPS); }
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // Weights are 2^SHIFT at the row's maximum, up to 2^(SHIFT + SLACK) where that has risen since it was last looked at: fp16 has 11 bits of them down to 2^-21 of
 // the largest.
@@ -189,14 +188,15 @@ template <typename T, int DIM> __device__ __forceinline__ void store_out(T *to, 
 }
 
 // What both ways to take a tile below have in common.
-template <int DIM, int BITS, int BLOCKS, int HEADS>
+template <int DIM, int BITS, Way WAY, int HEADS>
 struct Tiles {
+  static constexpr int CTAS = ctas_per_sm(WAY, DIM, BITS);
   static constexpr int ROW = ROW_BYTES<DIM, BITS>, CODES = ROW - TRAILER, PIECES = ROW / 16;
   static constexpr int CHUNK = CODES / 8, N = CHUNK / 4, J = DIM / 32, STEPS = J / 2;       // bytes and words of a chunk; codes of a quarter in it; k steps of a quarter
   static constexpr int STAGE = 2 * TILE * ROW;                                              // keys, then values
-  static constexpr int STAGES = stages(BLOCKS, ROW);
+  static constexpr int FIT = warp_bytes(CTAS) / STAGE, STAGES = FIT < 4 ? FIT : 4;
   // Queries of the next item, copied with its first rows; where a warp's shared memory has room
-  static constexpr int QUERIES = STAGES * STAGE + HEADS * DIM * 2 <= warp_bytes(BLOCKS, ROW) ? HEADS * DIM * 2 : 0;
+  static constexpr int QUERIES = STAGES * STAGE + HEADS * DIM * 2 <= warp_bytes(CTAS) ? HEADS * DIM * 2 : 0;
   static constexpr int QUERY_STRIDE = DIM, WARP_SMEM = STAGES * STAGE + QUERIES, SMEM = WARPS * WARP_SMEM;
   static constexpr float M = 1 << (BITS - 1), UNIT = 0x1p-24f;
   static constexpr bool SPREAD = BITS == 8 && DIM == 128;                                   // a lane's two chunks of keys: four apart, or one behind the other
@@ -258,13 +258,57 @@ struct Tiles {
   }
 };
 
+// A tile where all of a thread's columns are of one query head; `rows` rows of it (32 or fewer) are there.
+template <int ROW, typename A>
+__device__ __forceinline__ void take_tile(A &a, uint32_t kt, int rows, int lane) {
+  const int g = lane >> 2;
+  const uint32_t vt = kt + TILE * ROW;
+  float x[2][2];
+  a.scores(kt, lane, x[0]);
+  a.scores(kt + 16 * ROW, lane, x[1]);
+  if (rows < TILE) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (8 * e + g >= rows) x[e / 2][e % 2] = -INFINITY;
+  }
+  // the maximum moves when a score is SLACK above it
+  float v = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
+  if (__any_sync(0xffffffffu, fmaf(v, a.factor, a.off) > SHIFT + SLACK)) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    v = fmaxf(v, a.m);
+    if (v != -INFINITY) {
+      a.scale(exp2_fast((a.m - v) * a.factor));
+      a.m = v;
+      a.off = fmaf(-v, a.factor, SHIFT);
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t hi[2], lo[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float w = exp2_fast(fmaf(x[h][r], a.factor, a.off));
+      a.l += w;
+      const uint32_t upper = pack2(w, w);
+      hi[r] = transposed(upper);
+      lo[r] = 0u;
+      if constexpr (A::LOWER) {
+        const float rest = w - __low2float(h2(upper));
+        lo[r] = transposed(pack2(rest, rest));
+      }
+    }
+    a.weigh(vt + 16 * h * ROW, lane, hi, lo);
+  }
+}
+
 // One or two query heads: each takes four of the eight columns, one for each quarter of the dimensions.  Keys: queries are zero outside their column's
 // quarter, so one product over all codes has the quarters' sums side by side, each is scaled once, and pairs of codes need not be of one quarter; values: the weights'
 // scales are the columns', one operand for all dimensions, of whose columns each quarter of the output keeps its own.
 template <typename T, int DIM, int BITS>
-struct AttendPair : Tiles<DIM, BITS, 1, 2> {
+struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
   using Value = T;
-  using Base = Tiles<DIM, BITS, 1, 2>;
+  using Base = Tiles<DIM, BITS, PAIR, 2>;
   using Base::ROW; using Base::CODES; using Base::N; using Base::J; using Base::STEPS; using Base::M; using Base::UNIT; using Base::CHUNK;
   static constexpr bool LOWER = !Type<T>::BF16;            // whether weights have a lower part
   static constexpr int PAIRS = 16 / BITS, KSTEPS = N * PAIRS;               // operand words of a word of codes; k steps of a row of keys
@@ -422,56 +466,18 @@ struct AttendPair : Tiles<DIM, BITS, 1, 2> {
     if constexpr (LOWER) mma(zacc, raw[0], raw[1], raw[2], raw[3], lo[0], lo[1], zacc[0], zacc[1], zacc[2], zacc[3]);
   }
 
-  // A tile, of which `rows` rows (32 or fewer) are there
-  __device__ __forceinline__ void tile(uint32_t kt, int rows, int lane) {
-    const int g = lane >> 2;
-    const uint32_t vt = kt + TILE * ROW;
-    float x[2][2];
-    scores(kt, lane, x[0]);
-    scores(kt + 16 * ROW, lane, x[1]);
-    if (rows < TILE) {
+  // All there is of the head scaled: its maximum has moved
+  __device__ __forceinline__ void scale(float by) {
+    l *= by;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (8 * e + g >= rows) x[e / 2][e % 2] = -INFINITY;
-    }
-    // the maximum moves when a score is SLACK above it
-    float v = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
-    if (__any_sync(0xffffffffu, fmaf(v, factor, off) > SHIFT + SLACK)) {
+    for (int i = 0; i < 4; ++i) {
+      sums[i] *= by;
+      zacc[i] *= by;
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-      v = fmaxf(v, m);
-      if (v != -INFINITY) {
-        const float by = exp2_fast((m - v) * factor);
-        m = v;
-        off = fmaf(-v, factor, SHIFT);
-        l *= by;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          sums[i] *= by;
-          zacc[i] *= by;
-#pragma unroll
-          for (int u = 0; u < STEPS; ++u) { acc[i][u][0] *= by; acc[i][u][1] *= by; acc[i][u][2] *= by; acc[i][u][3] *= by; }
-        }
-      }
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t hi[2], lo[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float w = exp2_fast(fmaf(x[h][r], factor, off));
-        l += w;
-        const uint32_t upper = pack2(w, w);
-        hi[r] = transposed(upper);
-        lo[r] = 0u;
-        if constexpr (LOWER) {
-          const float rest = w - __low2float(h2(upper));
-          lo[r] = transposed(pack2(rest, rest));
-        }
-      }
-      weigh(vt + 16 * h * ROW, lane, hi, lo);
+      for (int u = 0; u < STEPS; ++u) { acc[i][u][0] *= by; acc[i][u][1] *= by; acc[i][u][2] *= by; acc[i][u][3] *= by; }
     }
   }
+  __device__ __forceinline__ void tile(uint32_t kt, int rows, int lane) { take_tile<ROW>(*this, kt, rows, lane); }
 
   // The state of a part to the workspace (slot >= 0), or the output of a whole item
   __device__ __forceinline__ void end(const AttendParams &p, int b, int kv_head, int slot, int lane) {
@@ -503,11 +509,213 @@ struct AttendPair : Tiles<DIM, BITS, 1, 2> {
   }
 };
 
+// Three or four query heads: each takes two of the eight columns, one for each half of the dimensions.  A quarter's products have it in the columns of its half, which
+// alone are looked at; two operands of weights times scales, for the even and the odd quarters.
+template <typename T, int DIM, int BITS>
+struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
+  using Value = T;
+  using Base = Tiles<DIM, BITS, QUAD, 4>;
+  using Base::ROW; using Base::CODES; using Base::N; using Base::J; using Base::STEPS; using Base::M; using Base::UNIT; using Base::CHUNK;
+  static constexpr bool LOWER = !Type<T>::BF16;            // whether weights have a lower part
+
+  uint32_t qb[2][STEPS][2], qz[2];               // queries of the column's even and odd quarter; sums over quarters, as upper and lower fp16 parts
+  float factor, m, off, l;                       // what a score is multiplied by, the largest score, what is added in the exponent, the sum of weights; of head t
+  float acc[4][STEPS][4], sums[2][4], zacc[4];   // out^T, quarter by quarter; sums of weights times scales; of weights times centres (lanes g >= 4: of quarter g - 4)
+  __half2 f;                                     // power of two that takes quarter g & 3's scales of values to 1 or below
+  uint32_t ones;
+
+  __device__ __forceinline__ void begin(const AttendParams &p, const T *queries, long long stride, int lane) {
+    const int t = lane & 3, g = lane >> 2, h = g >> 1, half = g & 1;
+    const bool live = h < p.group;
+    const T *const q = queries + (live ? h : 0) * stride + DIM / 2 * half;
+    float x[2][2][J], top = 0.0f;                // of the column's quarters, of the lane's two chunks
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          x[i][c][j] = live ? static_cast<float>(q[DIM / 4 * i + DIM / 32 * Base::chunk_of(t, c) + j]) : 0.0f;
+          top = fmaxf(top, fabsf(x[i][c][j]));
+        }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const int up = Base::lift(top);
+    const float by = copysignf(power2(up), p.scale_log2);
+    float sum[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      sum[i] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int j = 0; j < J; ++j) { x[i][c][j] *= by; sum[i] += x[i][c][j]; }
+      sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+      sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+#pragma unroll
+      for (int u = 0; u < STEPS; ++u) {
+        constexpr float ODD = BITS == 4 ? 0.0625f : 1.0f;
+        qb[i][u][0] = pack2(x[i][0][2 * u], x[i][1][2 * u]);
+        qb[i][u][1] = pack2(x[i][0][2 * u + 1] * ODD, x[i][1][2 * u + 1] * ODD);
+      }
+    }
+    // a trailer's entries 2 t and 2 t + 1: scales (t < 2) or centres of half t & 1
+    const float unit = half == (t & 1) ? t < 2 ? -M : 1.0f : 0.0f;
+    qz[0] = pack2(unit * sum[0], unit * sum[1]);
+    const float2 back = __half22float2(h2(qz[0]));
+    qz[1] = pack2(unit * sum[0] - back.x, unit * sum[1] - back.y);
+    factor = __shfl_sync(0xffffffffu, Base::factor_of(p, up), 8 * t);
+    m = -INFINITY;
+    off = NOTHING;
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sums[0][i] = sums[1][i] = zacc[i] = 0.0f;
+#pragma unroll
+      for (int u = 0; u < STEPS; ++u) { acc[i][u][0] = 0.0f; acc[i][u][1] = 0.0f; acc[i][u][2] = 0.0f; acc[i][u][3] = 0.0f; }
+    }
+    f = __float2half2_rn(0x1p15f);
+    ones = ONES;
+  }
+
+  // Scores of rows g and g + 8 of 16, times the power of two, head t
+  __device__ __forceinline__ void scores(uint32_t kt, int lane, float (&y)[2]) const {
+    const int t = lane & 3, g = lane >> 2;
+    uint32_t w[2][2][N], pair[4];
+    float s[2][4], z[4];
+    trailers<false, ROW>(kt + CODES, lane, pair);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const uint32_t at = kt + (g + 8 * r) * ROW;
+      Base::keys(at, t, w[r]);
+      uint32_t sw[2];
+      lds<2>(at + CODES, sw);
+      const float2 s01 = __half22float2(h2(sw[0])), s23 = __half22float2(h2(sw[1]));
+      s[r][0] = s01.x; s[r][1] = s01.y; s[r][2] = s23.x; s[r][3] = s23.y;
+    }
+    mma(z, pair[0], pair[1], pair[2], pair[3], qz[0], qz[1], 0.0f, 0.0f, 0.0f, 0.0f);
+    y[0] = (z[0] + z[1]) * UNIT;
+    y[1] = (z[2] + z[3]) * UNIT;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t top[J], low[J];
+      expand<DIM, BITS>(w[0][0], w[0][1], i, top);
+      expand<DIM, BITS>(w[1][0], w[1][1], i, low);
+      const uint32_t (&b)[STEPS][2] = qb[i % 2];
+      float c[4];
+      mma(c, top[0], low[0], top[1], low[1], b[0][0], b[0][1], 0.0f, 0.0f, 0.0f, 0.0f);
+      if constexpr (STEPS == 2) mma(c, top[J - 2], low[J - 2], top[J - 1], low[J - 1], b[STEPS - 1][0], b[STEPS - 1][1], c[0], c[1], c[2], c[3]);
+      y[0] = fmaf(c[i / 2], s[0][i], y[0]);
+      y[1] = fmaf(c[2 + i / 2], s[1][i], y[1]);
+    }
+  }
+
+  // A scale exceeds 1: the powers of two follow
+  __device__ __forceinline__ void rescale(int lane, const uint32_t (&raw)[4]) {
+    const __half2 top = __hmax2(h2(raw[0]), h2(raw[2]));
+    float most = fmaxf(__low2float(top), __high2float(top));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    most = __shfl_sync(0xffffffffu, most, lane & 15);                       // (of quarter g & 3)
+    const float old = __low2float(f), now = Base::taken(most, old), by = now / old;
+    f = __float2half2_rn(now);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float r = __shfl_sync(0xffffffffu, by, 4 * i);
+      sums[i % 2][i / 2] *= r;
+      sums[i % 2][2 + i / 2] *= r;
+#pragma unroll
+      for (int u = 0; u < STEPS; ++u) { acc[i][u][0] *= r; acc[i][u][1] *= r; acc[i][u][2] *= r; acc[i][u][3] *= r; }
+    }
+  }
+
+  // Weights of 16 rows (upper and lower parts, rows 2 t, 2 t + 1 and those + 8 of column g) times their values
+  __device__ __forceinline__ void weigh(uint32_t vt, int lane, const uint32_t (&hi)[2], const uint32_t (&lo)[2]) {
+    const int t = lane & 3, g = lane >> 2;
+    uint32_t raw[4], w[4][N], pb[2][2];
+    trailers<true, ROW>(vt + CODES, lane, raw);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) lds<N>(vt + (2 * t + (r & 1) + 8 * (r >> 1)) * ROW + g * CHUNK, w[r]);
+    __half2 s0 = __hmul2(h2(raw[0]), f), s1 = __hmul2(h2(raw[2]), f);
+    if (__any_sync(0xffffffffu, g < 4 && !__hble2(__hmax2(s0, s1), __float2half2_rn(1.0f)))) {
+      rescale(lane, raw);
+      s0 = __hmul2(h2(raw[0]), f);
+      s1 = __hmul2(h2(raw[2]), f);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {                // quarter 2 (g & 1) + i
+      const int from = 8 * (g & 1) + 4 * i + t;
+      const __half2 a0 = h2(__shfl_sync(0xffffffffu, bits_of(s0), from)), a1 = h2(__shfl_sync(0xffffffffu, bits_of(s1), from));
+      if constexpr (LOWER) {
+        pb[i][0] = bits_of(__hfma2(h2(hi[0]), a0, __hmul2(h2(lo[0]), a0)));
+        pb[i][1] = bits_of(__hfma2(h2(hi[1]), a1, __hmul2(h2(lo[1]), a1)));
+      } else {
+        pb[i][0] = bits_of(__hmul2(h2(hi[0]), a0));
+        pb[i][1] = bits_of(__hmul2(h2(hi[1]), a1));
+      }
+      float (&c)[4] = sums[i];
+      mma(c, ones, ones, ones, ones, pb[i][0], pb[i][1], c[0], c[1], c[2], c[3]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t first[J], second[J];
+      expand<DIM, BITS>(w[0], w[1], i, first);
+      expand<DIM, BITS>(w[2], w[3], i, second);
+#pragma unroll
+      for (int u = 0; u < STEPS; ++u) {
+        float (&c)[4] = acc[i][u];
+        mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pb[i % 2][0], pb[i % 2][1], c[0], c[1], c[2], c[3]);
+      }
+    }
+    mma(zacc, raw[0], raw[1], raw[2], raw[3], hi[0], hi[1], zacc[0], zacc[1], zacc[2], zacc[3]);
+    if constexpr (LOWER) mma(zacc, raw[0], raw[1], raw[2], raw[3], lo[0], lo[1], zacc[0], zacc[1], zacc[2], zacc[3]);
+  }
+
+  // All there is of head t scaled: its maximum has moved
+  __device__ __forceinline__ void scale(float by) {
+    l *= by;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sums[0][i] *= by;
+      sums[1][i] *= by;
+      zacc[i] *= by;
+#pragma unroll
+      for (int u = 0; u < STEPS; ++u) { acc[i][u][0] *= by; acc[i][u][1] *= by; acc[i][u][2] *= by; acc[i][u][3] *= by; }
+    }
+  }
+  __device__ __forceinline__ void tile(uint32_t kt, int rows, int lane) { take_tile<ROW>(*this, kt, rows, lane); }
+
+  // The state of a part to the workspace (slot >= 0), or the output of a whole item
+  __device__ __forceinline__ void end(const AttendParams &p, int b, int kv_head, int slot, int lane) {
+    const int t = lane & 3, g = lane >> 2, h = t;
+    float total = l;
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const float by = total == 0.0f ? 0.0f : 1.0f / total;
+    const size_t part = static_cast<size_t>(slot) * p.group + h, row = static_cast<size_t>(b) * p.q_heads + kv_head * p.group + h;
+    const bool live = h < p.group;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float z = __shfl_sync(0xffffffffu, zacc[0], 4 * i + 16 + t), inverse = 1.0f / __shfl_sync(0xffffffffu, __low2float(f), 4 * i);
+      float v[J];
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        v[j] = fmaf(fmaf(acc[i][j / 2][i / 2 + 2 * (j % 2)], (BITS == 4 && j % 2 ? 0.0625f : 1.0f) / UNIT, -M * sums[i % 2][i / 2]), inverse, z);
+      if (!live) continue;
+      if (slot >= 0) store_part<DIM>(p.part_out + part * DIM + DIM / 4 * i + J * g, v);
+      else store_out<T, DIM>(static_cast<T *>(p.out) + row * DIM + DIM / 4 * i + J * g, v, by);
+    }
+    if (!live || g) return;
+    if (slot >= 0) p.part_ml[part] = make_float2(total == 0.0f ? -INFINITY : -off, total);
+    else if (p.lse) p.lse[row] = total == 0.0f ? -INFINITY : logf(total) - off * LN2;
+  }
+};
+
 // Up to sixteen query heads, in NT blocks of eight columns.
 template <typename T, int DIM, int BITS, int NT>
-struct Attend : Tiles<DIM, BITS, NT, 8 * NT> {
+struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
   using Value = T;
-  using Base = Tiles<DIM, BITS, NT, 8 * NT>;
+  using Base = Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT>;
   using Base::ROW; using Base::CODES; using Base::N; using Base::J; using Base::STEPS; using Base::M; using Base::UNIT; using Base::CHUNK;
   static constexpr bool LOWER = !Type<T>::BF16;            // whether weights have a lower part
 
@@ -793,8 +1001,8 @@ struct Attend : Tiles<DIM, BITS, NT, 8 * NT> {
   }
 };
 
-template <typename A, int BLOCKS>
-__global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(BLOCKS, A::ROW)) attend_tiles(const __grid_constant__ AttendParams p) {
+template <typename A>
+__global__ void __launch_bounds__(WARPS * 32, A::CTAS) attend_tiles(const __grid_constant__ AttendParams p) {
   constexpr int STAGES = A::STAGES;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Line line;

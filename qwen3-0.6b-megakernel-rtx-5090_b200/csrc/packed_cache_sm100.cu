@@ -99,9 +99,8 @@ int rows_call(const char *who, const qmk_packed_cache *cache, const qmk_packed_r
 
 // Stretches of a call: a warp each, all resident together, not more than there can be tiles.
 long long most_tiles(int seqs, int kv_heads, int rows) { return static_cast<long long>(seqs) * kv_heads * ((rows + TILE - 1) / TILE); }
-int blocks_of(int group) { return group > 8 ? 2 : 1; }                    // of eight query heads
 int warps_of(int seqs, int kv_heads, int group, int dim, int bits, int rows) {
-  return static_cast<int>(std::min<long long>(std::max(most_tiles(seqs, kv_heads, rows), 1ll), SMS * ctas_per_sm(blocks_of(group), dim * bits / 8 + TRAILER) * WARPS));
+  return static_cast<int>(std::min<long long>(std::max(most_tiles(seqs, kv_heads, rows), 1ll), SMS * ctas_per_sm(way_of(group), dim, bits) * WARPS));
 }
 long long workspace_bytes(int warps, int group, int dim) { return 2ll * warps * group * (dim * 4ll + 8); }
 
@@ -119,7 +118,7 @@ cudaError_t launch_join(const AttendParams &p, cudaStream_t stream) {
   return qmk_tc::launch_kernel(join_many<T, DIM, 32, 8>, dim3(rows), dim3(1024), 0, stream, p);
 }
 
-template <typename A, int BLOCKS>
+template <typename A>
 cudaError_t launch_tiles(const AttendParams &p, cudaStream_t stream) {
   // (once a device; the call takes half a microsecond)
   static std::atomic<unsigned long long> known{0};
@@ -127,19 +126,24 @@ cudaError_t launch_tiles(const AttendParams &p, cudaStream_t stream) {
   cudaError_t e = cudaGetDevice(&device);
   const unsigned long long bit = device < 64 ? 1ull << device : 0;
   if (e == cudaSuccess && !(known.load() & bit)) {
-    e = cudaFuncSetAttribute(attend_tiles<A, BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, A::SMEM);
+    e = cudaFuncSetAttribute(attend_tiles<A>, cudaFuncAttributeMaxDynamicSharedMemorySize, A::SMEM);
     if (e == cudaSuccess) known |= bit;
   }
   if (e != cudaSuccess) return e;
-  const int ctas = std::min(p.warps, SMS * ctas_per_sm(BLOCKS, A::ROW));                    // (a warp of each where there are few)
-  return qmk_tc::launch_kernel(attend_tiles<A, BLOCKS>, dim3(ctas), dim3(WARPS * 32), A::SMEM, stream, p);
+  const int ctas = std::min(p.warps, SMS * A::CTAS);                    // (a warp of each where there are few)
+  return qmk_tc::launch_kernel(attend_tiles<A>, dim3(ctas), dim3(WARPS * 32), A::SMEM, stream, p);
 }
 template <typename T, int DIM, int BITS>
 cudaError_t attend(const AttendParams &p, cudaStream_t stream) {
-  const cudaError_t e = p.caches.rows == 0 ? cudaSuccess
-                        : p.group <= 2     ? launch_tiles<AttendPair<T, DIM, BITS>, 1>(p, stream)
-                        : p.group <= 8     ? launch_tiles<Attend<T, DIM, BITS, 1>, 1>(p, stream)
-                                           : launch_tiles<Attend<T, DIM, BITS, 2>, 2>(p, stream);
+  cudaError_t e = cudaSuccess;
+  if (p.caches.rows > 0) {
+    switch (way_of(p.group)) {
+      case PAIR: e = launch_tiles<AttendPair<T, DIM, BITS>>(p, stream); break;
+      case QUAD: e = launch_tiles<AttendQuad<T, DIM, BITS>>(p, stream); break;
+      case ONE: e = launch_tiles<Attend<T, DIM, BITS, 1>>(p, stream); break;
+      case TWO: e = launch_tiles<Attend<T, DIM, BITS, 2>>(p, stream); break;
+    }
+  }
   if (e != cudaSuccess) return e;
   return launch_join<T, DIM>(p, stream);
 }

@@ -335,7 +335,7 @@ def test_lists_of_caches_strides_and_no_rows(gpu):
 
 
 # ------------------------------------------------------------------------------------------------------------- attention
-HEADS = [(16, 8), (4, 4), (6, 2), (8, 1), (16, 1), (9, 1), (32, 4)]
+HEADS = [(16, 8), (4, 4), (6, 2), (8, 2), (10, 2), (8, 1), (16, 1), (9, 1), (32, 4)]
 
 
 @pytest.mark.gpu
