@@ -41,6 +41,7 @@ struct AttendParams {
   int q_heads, group;
   const int *lens;
   float scale_log2;                              // scale * log2 e
+  int ranks;                                     // where items have clusters of their own: log2 of the CTAs that share one, + 1; else 0
   int warps;                                     // of the launch
   float *part_out;                               // [2 warps][group][DIM]
   float2 *part_ml;                               // [2 warps][group]
@@ -190,7 +191,7 @@ template <typename T, int DIM> __device__ __forceinline__ void store_out(T *to, 
 // What both ways to take a tile below have in common.
 template <int DIM, int BITS, Way WAY, int HEADS>
 struct Tiles {
-  static constexpr int CTAS = ctas_per_sm(WAY, DIM, BITS);
+  static constexpr int CTAS = ctas_per_sm(WAY, DIM, BITS), HEAD_DIM = DIM;
   static constexpr int ROW = ROW_BYTES<DIM, BITS>, CODES = ROW - TRAILER, PIECES = ROW / 16;
   static constexpr int CHUNK = CODES / 8, N = CHUNK / 4, J = DIM / 32, STEPS = J / 2;       // bytes and words of a chunk; codes of a quarter in it; k steps of a quarter
   static constexpr int STAGE = 2 * TILE * ROW;                                              // keys, then values
@@ -198,6 +199,7 @@ struct Tiles {
   // Queries of the next item, copied with its first rows; where a warp's shared memory has room
   static constexpr int QUERIES = STAGES * STAGE + HEADS * DIM * 2 <= warp_bytes(CTAS) ? HEADS * DIM * 2 : 0;
   static constexpr int QUERY_STRIDE = DIM, WARP_SMEM = STAGES * STAGE + QUERIES, SMEM = WARPS * WARP_SMEM;
+  static_assert(STAGES * STAGE >= HEADS * (DIM * 4 + 8), "a warp's state fits its ring");
   static constexpr float M = 1 << (BITS - 1), UNIT = 0x1p-24f;
   static constexpr bool SPREAD = BITS == 8 && DIM == 128;                                   // a lane's two chunks of keys: four apart, or one behind the other
   static __device__ __forceinline__ int chunk_of(int t, int c) { return SPREAD ? t + 4 * c : 2 * t + c; }
@@ -479,14 +481,14 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
   }
   __device__ __forceinline__ void tile(uint32_t kt, int rows, int lane) { take_tile<ROW>(*this, kt, rows, lane); }
 
-  // The state of a part to the workspace (slot >= 0), or the output of a whole item
-  __device__ __forceinline__ void end(const AttendParams &p, int b, int kv_head, int slot, int lane) {
+  // The state of a part to `state` and `ml`, one head behind the other, or (null) the output of a whole item
+  __device__ __forceinline__ void end(const AttendParams &p, int b, int kv_head, float *state, float2 *ml, int lane) {
     const int t = lane & 3, g = lane >> 2, h = t >> 1;
     float total = l;
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     const float by = total == 0.0f ? 0.0f : 1.0f / total;
-    const size_t part = static_cast<size_t>(slot) * p.group + h, row = static_cast<size_t>(b) * p.q_heads + kv_head * p.group + h;
+    const size_t row = static_cast<size_t>(b) * p.q_heads + kv_head * p.group + h;
     const bool live = h < p.group;
     // this lane's columns: quarters 2 t & 3 and the next
 #pragma unroll
@@ -500,11 +502,11 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
         v[j] = fmaf(fmaf(c, (BITS == 4 && j % 2 ? 0.0625f : 1.0f) / UNIT, -M * sums[e]), inverse, z);
       }
       if (!live) continue;
-      if (slot >= 0) store_part<DIM>(p.part_out + part * DIM + DIM / 4 * i + J * g, v);
+      if (state) store_part<DIM>(state + h * DIM + DIM / 4 * i + J * g, v);
       else store_out<T, DIM>(static_cast<T *>(p.out) + row * DIM + DIM / 4 * i + J * g, v, by);
     }
     if (!live || (t & 1) || g) return;
-    if (slot >= 0) p.part_ml[part] = make_float2(total == 0.0f ? -INFINITY : -off, total);
+    if (state) ml[h] = make_float2(total == 0.0f ? -INFINITY : -off, total);
     else if (p.lse) p.lse[row] = total == 0.0f ? -INFINITY : logf(total) - off * LN2;
   }
 };
@@ -685,14 +687,14 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
   }
   __device__ __forceinline__ void tile(uint32_t kt, int rows, int lane) { take_tile<ROW>(*this, kt, rows, lane); }
 
-  // The state of a part to the workspace (slot >= 0), or the output of a whole item
-  __device__ __forceinline__ void end(const AttendParams &p, int b, int kv_head, int slot, int lane) {
+  // The state of a part to `state` and `ml`, one head behind the other, or (null) the output of a whole item
+  __device__ __forceinline__ void end(const AttendParams &p, int b, int kv_head, float *state, float2 *ml, int lane) {
     const int t = lane & 3, g = lane >> 2, h = t;
     float total = l;
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     const float by = total == 0.0f ? 0.0f : 1.0f / total;
-    const size_t part = static_cast<size_t>(slot) * p.group + h, row = static_cast<size_t>(b) * p.q_heads + kv_head * p.group + h;
+    const size_t row = static_cast<size_t>(b) * p.q_heads + kv_head * p.group + h;
     const bool live = h < p.group;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -702,11 +704,11 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
       for (int j = 0; j < J; ++j)
         v[j] = fmaf(fmaf(acc[i][j / 2][i / 2 + 2 * (j % 2)], (BITS == 4 && j % 2 ? 0.0625f : 1.0f) / UNIT, -M * sums[i % 2][i / 2]), inverse, z);
       if (!live) continue;
-      if (slot >= 0) store_part<DIM>(p.part_out + part * DIM + DIM / 4 * i + J * g, v);
+      if (state) store_part<DIM>(state + h * DIM + DIM / 4 * i + J * g, v);
       else store_out<T, DIM>(static_cast<T *>(p.out) + row * DIM + DIM / 4 * i + J * g, v, by);
     }
     if (!live || g) return;
-    if (slot >= 0) p.part_ml[part] = make_float2(total == 0.0f ? -INFINITY : -off, total);
+    if (state) ml[h] = make_float2(total == 0.0f ? -INFINITY : -off, total);
     else if (p.lse) p.lse[row] = total == 0.0f ? -INFINITY : logf(total) - off * LN2;
   }
 };
@@ -967,8 +969,8 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
     }
   }
 
-  // The state of a part to the workspace (slot >= 0), or the output of a whole item
-  __device__ __forceinline__ void end(const AttendParams &p, int b, int kv_head, int slot, int lane) {
+  // The state of a part to `state` and `ml`, one head behind the other, or (null) the output of a whole item
+  __device__ __forceinline__ void end(const AttendParams &p, int b, int kv_head, float *state, float2 *ml, int lane) {
     const int t = lane & 3, g = lane >> 2;
     float inverse[4];
 #pragma unroll
@@ -982,7 +984,7 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
         for (int o = 4; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
         const int h = nt * 8 + 2 * t + e;
         const float by = total == 0.0f ? 0.0f : 1.0f / total;
-        const size_t part = static_cast<size_t>(slot) * p.group + h, row = static_cast<size_t>(b) * p.q_heads + kv_head * p.group + h;
+        const size_t row = static_cast<size_t>(b) * p.q_heads + kv_head * p.group + h;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float z = __shfl_sync(0xffffffffu, zacc[nt][e], 4 * i + 16 + t);
@@ -991,11 +993,11 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
           for (int j = 0; j < J; ++j)
             v[j] = fmaf(fmaf(acc[nt][i][j / 2][e + 2 * (j % 2)], (BITS == 4 && j % 2 ? 0.0625f : 1.0f) / UNIT, -M * sums[nt][i][e]), inverse[i], z);
           if (h >= p.group) continue;
-          if (slot >= 0) store_part<DIM>(p.part_out + part * DIM + DIM / 4 * i + J * g, v);
+          if (state) store_part<DIM>(state + h * DIM + DIM / 4 * i + J * g, v);
           else store_out<T, DIM>(static_cast<T *>(p.out) + row * DIM + DIM / 4 * i + J * g, v, by);
         }
         if (h >= p.group || g) continue;
-        if (slot >= 0) p.part_ml[part] = make_float2(total == 0.0f ? -INFINITY : -off[nt][e], total);
+        if (state) ml[h] = make_float2(total == 0.0f ? -INFINITY : -off[nt][e], total);
         else if (p.lse) p.lse[row] = total == 0.0f ? -INFINITY : logf(total) - off[nt][e] * LN2;
       }
   }
@@ -1057,17 +1059,152 @@ __global__ void __launch_bounds__(WARPS * 32, A::CTAS) attend_tiles(const __grid
     a.tile(ring + (i - first) % STAGES * A::STAGE, min(now.rows - now.tile * TILE, TILE), lane);
     const bool done = now.tile == now.tiles - 1;
     if (done || i == last - 1) {
+      const size_t slot = static_cast<size_t>(2 * r + (began == 0 && i - first > now.tile)) * p.group;
       const bool whole = done && began == 0;
-      a.end(p, now.b, now.head, whole ? -1 : 2 * r + (began == 0 && i - first > now.tile), lane);
+      a.end(p, now.b, now.head, whole ? nullptr : p.part_out + slot * A::HEAD_DIM, whole ? nullptr : p.part_ml + slot, lane);
     }
     if (i < last - 1) now.next(p, line);
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// The join: outputs of items whose parts lie in several stretches, and of sequences without rows.
 // (a maximum of -inf: nothing seen, or a sum that is no number and stays one)
 __device__ __forceinline__ float part_weight(float m, float l, float top) { return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2f(m - top); }
+// Zeros for a sequence's query heads [first, first + n), which see no row
+template <typename T>
+__device__ __forceinline__ void zero_heads(const AttendParams &p, int dim, int b, int first, int n, int lane) {
+  const size_t row = static_cast<size_t>(b) * p.q_heads + first;
+  for (int i = lane; i < n * (dim / 8); i += 32) *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + row * dim + i * 8) = make_uint4(0, 0, 0, 0);
+  for (int i = lane; p.lse && i < n; i += 32) p.lse[row + i] = -INFINITY;
+}
+// Short items, one launch: a cluster of CTAs takes an item, each warp an equal part of its tiles; the states stay in shared memory, where all of the cluster
+// can read them, and its warps join them, 16 dimensions of a query head each.
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of `at` in the shared memory of the cluster's CTA `rank`
+__device__ __forceinline__ uint32_t of_rank(uint32_t at, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+  return r;
+}
+template <int E> __device__ __forceinline__ void ld_cluster(uint32_t at, float (&v)[E]) {
+  if constexpr (E == 4) asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(at) : "memory");
+  else asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(at) : "memory");
+}
+// An item's parts: a warp each of 2^shift CTAs, part w warp w >> shift of CTA w & 2^shift - 1 (few tiles: in different CTAs), its first tile.  (Items have few tiles.)
+__device__ __forceinline__ int begin_of_part(int tiles, int shift, int w) { return tiles * w >> (shift + 2); }
+static_assert(WARPS == 4, "a CTA has four of an item's parts");
+// The states of an item's parts, at most 32, joined by warps `mine` and so on.  Unit: DIM / GROUPS dimensions of a query head; groups of lanes take every
+// GROUPS-th part, eight or four at a time.
+template <typename A, int GROUPS>
+__device__ __forceinline__ void join_cluster(const AttendParams &p, const Place &item, int shift, unsigned char *smem, int mine, int lane) {
+  using T = typename A::Value;
+  constexpr int DIM = A::HEAD_DIM, UNIT_DIMS = DIM / GROUPS, LANES = 32 / GROUPS, E = UNIT_DIMS / LANES, EACH = GROUPS == 1 ? 8 : 4;      // dimensions of a lane
+  const int parts = WARPS << shift, group = lane / LANES;
+  const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+  auto part_at = [&](int w) { return of_rank(base + (w >> shift) * A::WARP_SMEM, w & ((1 << shift) - 1)); };
+  const bool there = lane < parts && begin_of_part(item.tiles, shift, lane) < begin_of_part(item.tiles, shift, lane + 1);
+  const unsigned int any = __ballot_sync(0xffffffffu, there);
+  for (int u = mine; u < p.group * GROUPS; u += parts) {
+    const int h = u / GROUPS, d = u % GROUPS * UNIT_DIMS + lane % LANES * E;
+    float ml[2] = {-INFINITY, 0.0f}, out[E];                                // a part's maximum and sum to a lane
+    if (there) ld_cluster<2>(part_at(lane) + p.group * DIM * 4 + h * 8, ml);
+    float top = 0.0f, f = 0.0f, total = 0.0f;
+#pragma unroll
+    for (int k = 0; k < E; ++k) out[k] = 0.0f;
+    for (int first = 0; first < parts; first += EACH * GROUPS) {
+      float v[EACH][E];
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const int w = first + group + GROUPS * i;
+#pragma unroll
+        for (int k = 0; k < E; ++k) v[i][k] = 0.0f;
+        if (any >> w & 1u) ld_cluster<E>(part_at(w) + (h * DIM + d) * 4, v[i]);
+      }
+      if (first == 0) {                          // (beside the states)
+        top = ml[0];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        f = part_weight(ml[0], ml[1], top);
+        total = ml[1] * f;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      }
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const float by = __shfl_sync(0xffffffffu, f, first + group + GROUPS * i);
+#pragma unroll
+        for (int k = 0; k < E; ++k) out[k] = fmaf(v[i][k], by, out[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < E; ++k)
+#pragma unroll
+      for (int o = LANES; o < 32; o <<= 1) out[k] += __shfl_xor_sync(0xffffffffu, out[k], o);
+    const size_t row = static_cast<size_t>(item.b) * p.q_heads + item.head * p.group + h;
+    if (lane < LANES) store_out<T, 32 * E>(static_cast<T *>(p.out) + row * DIM + d, out, total == 0.0f ? 0.0f : 1.0f / total);
+    if (lane == 0 && u % GROUPS == 0 && p.lse) p.lse[row] = total == 0.0f ? -INFINITY : top * LN2 + logf(total);
+  }
+}
+template <typename A>
+__global__ void __launch_bounds__(WARPS * 32, A::CTAS) attend_items(const __grid_constant__ AttendParams p) {
+  using T = typename A::Value;
+  constexpr int STAGES = A::STAGES, DIM = A::HEAD_DIM;
+  extern __shared__ __align__(128) unsigned char smem[];
+  pdl_wait();
+  pdl_trigger();
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, rank = cluster_rank();
+  const int shift = p.ranks - 1, item = static_cast<int>(blockIdx.x) >> shift;
+  Place now;
+  now.b = item / p.caches.kv_heads;
+  now.head = item - now.b * p.caches.kv_heads;
+  now.rows = seen_rows(p, now.b);
+  now.tiles = tiles_of(now.rows);
+  if (now.tiles == 0) {                          // (all of the cluster)
+    if (rank == 0 && warp == 0) zero_heads<T>(p, DIM, now.b, now.head * p.group, p.group, lane);
+    return;
+  }
+  const int mine = (warp << shift) + rank, first = begin_of_part(now.tiles, shift, mine), last = begin_of_part(now.tiles, shift, mine + 1);
+  unsigned char *const own = smem + warp * A::WARP_SMEM;
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(own));
+  if (first < last) {
+    Place ahead = now;
+    ahead.tile = first;
+    auto fetch = [&]() {
+      if (ahead.tile < last) A::load(p, ahead, ring + (ahead.tile - first) % STAGES * A::STAGE, lane);
+      ++ahead.tile;
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) fetch();
+    A a;
+    a.begin(p, static_cast<const T *>(p.q) + now.b * p.q_seq + static_cast<long long>(now.head) * p.group * p.q_head, p.q_head, lane);
+    for (int i = first; i < last; ++i) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+      __syncwarp();                              // every lane's copies of tile i are there, and tile i - 1 has been read
+      fetch();
+      a.tile(ring + (i - first) % STAGES * A::STAGE, min(now.rows - i * TILE, TILE), lane);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
+    float *const state = reinterpret_cast<float *>(own);
+    a.end(p, now.b, now.head, state, reinterpret_cast<float2 *>(state + p.group * DIM), lane);
+  }
+  cluster_sync();
+  // whole heads where there are few parts, or heads enough for the warps; else eighths.  (One CTA, two heads: 128 rows 5.6 us, with eighths 8.7; four CTAs, eight heads:
+  // 12.8 and 13.0; eight CTAs, two heads, 1024 rows: 10.8 and 7.2.)
+  if (shift < 2 || 2 * p.group >= (WARPS << shift)) join_cluster<A, 1>(p, now, shift, smem, mine, lane);
+  else join_cluster<A, 8>(p, now, shift, smem, mine, lane);
+  cluster_sync();                                // (nobody leaves while its states are read)
+}
+
+// The join: outputs of items whose parts lie in several stretches, and of sequences without rows.
 template <int DIM, int AHEAD>
 struct Joined {
   static constexpr int E = DIM / 32;
@@ -1115,12 +1252,8 @@ struct Joined {
 };
 template <typename T>
 __device__ __forceinline__ void zero_empty(const AttendParams &p, const Line &line, int dim, int first, int step, int lane) {
-  for (int b = first; b < p.caches.seqs; b += step) {
-    if (line.rows[b] > 0) continue;
-    const size_t row = static_cast<size_t>(b) * p.q_heads;
-    for (int i = lane; i < p.q_heads * (dim / 8); i += 32) *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + row * dim + i * 8) = make_uint4(0, 0, 0, 0);
-    for (int i = lane; p.lse && i < p.q_heads; i += 32) p.lse[row + i] = -INFINITY;
-  }
+  for (int b = first; b < p.caches.seqs; b += step)
+    if (line.rows[b] == 0) zero_heads<T>(p, dim, b, 0, p.q_heads, lane);
 }
 // A warp takes a query head of an item: for items of few parts.
 constexpr int FEW = 4;                           // parts asked for together

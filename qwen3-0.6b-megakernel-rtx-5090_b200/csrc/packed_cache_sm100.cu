@@ -16,6 +16,7 @@ using namespace qmk_packed;
 
 constexpr int MAX_ROWS = 1 << 24;                // of a cache
 constexpr int MAX_HEADS = 1024;
+constexpr int MAX_RANKS = 4;                     // clusters of 2^(4 - 1) CTAs
 
 int refuse(const char *who, const std::string &why) {
   qmk_internal::note_error(std::string(who) + ": " + why);
@@ -97,12 +98,25 @@ int rows_call(const char *who, const qmk_packed_cache *cache, const qmk_packed_r
   return answer(who, cudaGetLastError());
 }
 
-// Stretches of a call: a warp each, all resident together, not more than there can be tiles.
+// How a call is cut.  Where no warp gets more than ITEM_TILES tiles of caches that are full, a cluster of CTAs takes an item, one launch; up to ITEM_WAVES times as many items
+// as are resident together.  Else a warp takes a stretch of the line of tiles, all resident together, not more of them than there can be tiles, and a
+// second launch joins.  Stretches against clusters, us a call in a graph, 128 dims, 4 bits, 16 query heads on 8, lengths from 0 up: one sequence of 128 rows 6.0 and 4.7; 16 of
+// up to 2048 (4 tiles a warp) 14.0 and 12.1; 128 of up to 1024 (8 tiles, seven CTAs an SM one after the other) 30.4 and 27.3; 16 of up to 4096 (8) 18.2 and 17.4, of up to 8192 (16) 25.4
+// and 27.5 (a cluster has a longest item to wait for, a stretch has not); one of 8192 (8) 12.0 and 9.7, of 32,768 (32) 19.8 and 27.2.  On the host 16 and 13.
+// Clusters of 16 CTAs start late: one sequence of 2048 rows 15.5, of eight 5.7.
+constexpr int ITEM_TILES = 8, ITEM_WAVES = 4;
+struct Cut {
+  int ranks, warps;
+};
 long long most_tiles(int seqs, int kv_heads, int rows) { return static_cast<long long>(seqs) * kv_heads * ((rows + TILE - 1) / TILE); }
-int warps_of(int seqs, int kv_heads, int group, int dim, int bits, int rows) {
-  return static_cast<int>(std::min<long long>(std::max(most_tiles(seqs, kv_heads, rows), 1ll), SMS * ctas_per_sm(way_of(group), dim, bits) * WARPS));
+Cut cut_of(int seqs, int kv_heads, int group, int dim, int bits, int rows) {
+  const int ctas = SMS * ctas_per_sm(way_of(group), dim, bits), tiles = (rows + TILE - 1) / TILE, items = seqs * kv_heads;
+  int ranks = 1;                                 // log2 of a cluster's CTAs, + 1
+  while (ranks < MAX_RANKS && (items << ranks) <= ctas && (WARPS << (ranks - 1)) < tiles) ++ranks;
+  if (items <= ITEM_WAVES * ctas && tiles <= ITEM_TILES * (WARPS << (ranks - 1))) return Cut{ranks, 0};
+  return Cut{0, static_cast<int>(std::min<long long>(std::max(most_tiles(seqs, kv_heads, rows), 1ll), ctas * WARPS))};
 }
-long long workspace_bytes(int warps, int group, int dim) { return 2ll * warps * group * (dim * 4ll + 8); }
+long long workspace_bytes(const Cut &cut, int group, int dim) { return std::max(2ll * cut.warps * group * (dim * 4ll + 8), 16ll); }
 
 // How the parts are joined goes by how many an item has where all stretches are used: warps, or CTAs of four, eight or 32 warps.
 template <typename T, int DIM>
@@ -118,25 +132,46 @@ cudaError_t launch_join(const AttendParams &p, cudaStream_t stream) {
   return qmk_tc::launch_kernel(join_many<T, DIM, 32, 8>, dim3(rows), dim3(1024), 0, stream, p);
 }
 
-template <typename A>
-cudaError_t launch_tiles(const AttendParams &p, cudaStream_t stream) {
-  // (once a device; the call takes half a microsecond)
-  static std::atomic<unsigned long long> known{0};
+// A kernel's shared memory, once a device (the call takes half a microsecond)
+template <typename K>
+cudaError_t allow(std::atomic<unsigned long long> &known, K kernel, int bytes) {
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
   const unsigned long long bit = device < 64 ? 1ull << device : 0;
-  if (e == cudaSuccess && !(known.load() & bit)) {
-    e = cudaFuncSetAttribute(attend_tiles<A>, cudaFuncAttributeMaxDynamicSharedMemorySize, A::SMEM);
-    if (e == cudaSuccess) known |= bit;
+  if (e != cudaSuccess || (known.load() & bit)) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) known |= bit;
+  return e;
+}
+template <typename A>
+cudaError_t launch_tiles(const AttendParams &p, cudaStream_t stream) {
+  static std::atomic<unsigned long long> tiles_known{0}, items_known{0};
+  if (p.ranks == 0) {
+    const cudaError_t e = allow(tiles_known, attend_tiles<A>, A::SMEM);
+    if (e != cudaSuccess) return e;
+    return qmk_tc::launch_kernel(attend_tiles<A>, dim3(std::min(p.warps, SMS * A::CTAS)), dim3(WARPS * 32), A::SMEM, stream, p);         // (a warp of each where there are few)
   }
+  const cudaError_t e = allow(items_known, attend_items<A>, A::SMEM);
   if (e != cudaSuccess) return e;
-  const int ctas = std::min(p.warps, SMS * A::CTAS);                    // (a warp of each where there are few)
-  return qmk_tc::launch_kernel(attend_tiles<A>, dim3(ctas), dim3(WARPS * 32), A::SMEM, stream, p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((p.caches.seqs * p.caches.kv_heads) << (p.ranks - 1));
+  cfg.blockDim = dim3(WARPS * 32);
+  cfg.dynamicSmemBytes = A::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1 << (p.ranks - 1);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = qmk_tc::pdl_active() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, attend_items<A>, p);
 }
 template <typename T, int DIM, int BITS>
 cudaError_t attend(const AttendParams &p, cudaStream_t stream) {
   cudaError_t e = cudaSuccess;
-  if (p.caches.rows > 0) {
+  if (p.caches.rows > 0 || p.ranks > 0) {
     switch (way_of(p.group)) {
       case PAIR: e = launch_tiles<AttendPair<T, DIM, BITS>>(p, stream); break;
       case QUAD: e = launch_tiles<AttendQuad<T, DIM, BITS>>(p, stream); break;
@@ -144,8 +179,7 @@ cudaError_t attend(const AttendParams &p, cudaStream_t stream) {
       case TWO: e = launch_tiles<Attend<T, DIM, BITS, 2>>(p, stream); break;
     }
   }
-  if (e != cudaSuccess) return e;
-  return launch_join<T, DIM>(p, stream);
+  return e != cudaSuccess || p.ranks > 0 ? e : launch_join<T, DIM>(p, stream);
 }
 template <typename T>
 cudaError_t attend(const AttendParams &p, int dim, int bits, cudaStream_t stream) {
@@ -167,7 +201,7 @@ extern "C" long long qmk_attention_packed_cache_workspace(int num_sequences, int
       (head_dim != 64 && head_dim != 128) || (bits != 4 && bits != 8) || rows < 0 || rows > MAX_ROWS)
     return 0;
   if (most_tiles(num_sequences, kv_heads, rows) > 0x7fffffffll) return 0;
-  return workspace_bytes(warps_of(num_sequences, kv_heads, q_heads / kv_heads, head_dim, bits, rows), q_heads / kv_heads, head_dim);
+  return workspace_bytes(cut_of(num_sequences, kv_heads, q_heads / kv_heads, head_dim, bits, rows), q_heads / kv_heads, head_dim);
 }
 
 extern "C" int qmk_attention_packed_cache(const qmk_packed_cache *cache, const qmk_packed_attention *a, cudaStream_t stream) {
@@ -191,7 +225,9 @@ extern "C" int qmk_attention_packed_cache(const qmk_packed_cache *cache, const q
   p.group = a->q_heads / cache->kv_heads;
   p.lens = a->lens;
   p.scale_log2 = a->scale * LOG2E;
-  p.warps = warps_of(cache->num_sequences, cache->kv_heads, p.group, cache->head_dim, cache->bits, cache->rows);
+  const Cut cut = cut_of(cache->num_sequences, cache->kv_heads, p.group, cache->head_dim, cache->bits, cache->rows);
+  p.ranks = cut.ranks;
+  p.warps = cut.warps;
   p.part_out = static_cast<float *>(a->workspace);
   p.part_ml = reinterpret_cast<float2 *>(p.part_out + 2ll * p.warps * p.group * cache->head_dim);
   p.out = a->out;

@@ -359,6 +359,31 @@ def test_long_caches_and_full_batches(gpu, bits, seqs, q_heads, kv_heads, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("dim,bits", [(64, 4), (64, 8), (128, 4), (128, 8)])
+@pytest.mark.parametrize("q_heads,kv_heads", HEADS)
+@pytest.mark.parametrize("seqs,room,rows", [(1, 40000, 700), (5, 33000, 333), (37, 17000, 70)])
+def test_caches_with_room_to_spare(gpu, dtype, dim, bits, q_heads, kv_heads, seqs, room, rows):
+    """Caches made for more rows than the sequences have: the call is cut for long ones."""
+    q, k, v = attention_inputs(seqs, q_heads, kv_heads, dim, bits, rows, dtype, seed=seqs + dim)
+    kc, vc = (torch.full((seqs, kv_heads, room, x.shape[3]), 255, dtype=torch.uint8, device="cuda") for x in (k, v))
+    lens = torch.tensor([rows * (i + 1) // seqs if i % 5 != 1 else 0 for i in range(seqs)], dtype=torch.int32)
+    kc[:, :, :rows], vc[:, :, :rows] = k, v
+    check_attention(gpu.attention_packed_cache(q, kc, vc, lens.cuda()), q, kc, vc, lens)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_heads,kv_heads,dim,bits", [(16, 8, 64, 4), (32, 8, 64, 8), (64, 8, 64, 4), (16, 1, 128, 4)])
+def test_full_batches_with_room_to_spare(gpu, q_heads, kv_heads, dim, bits):
+    q, k, v = attention_inputs(128, q_heads, kv_heads, dim, bits, 90, seed=dim)
+    kc, vc = (torch.full((128, kv_heads, 9000, x.shape[3]), 255, dtype=torch.uint8, device="cuda") for x in (k, v))
+    kc[:, :, :90], vc[:, :, :90] = k, v
+    for lens in ([(37 * i) % 91 for i in range(128)], [0] * 127 + [90], [1] * 128):
+        lens = torch.tensor(lens, dtype=torch.int32)
+        check_attention(gpu.attention_packed_cache(q, kc, vc, lens.cuda()), q, kc, vc, lens)
+
+
+@pytest.mark.gpu
 def test_no_rows_and_lengths_outside_the_cache(gpu):
     q, kc, vc = attention_inputs(4, 4, 2, 64, 4, 30)
     for lens in ([0, 0, 0, 0], [-5, 1000, 2 ** 31 - 1, -2 ** 31]):
@@ -384,9 +409,13 @@ def test_rows_behind_the_last_are_not_looked_at(gpu, dim, bits):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("bits", [4, 8])
-def test_visible_rows_that_are_no_numbers(gpu, bits):
+@pytest.mark.parametrize("room", [100, 40000])
+@pytest.mark.parametrize("q_heads", [8, 16, 32, 64])
+def test_visible_rows_that_are_no_numbers(gpu, bits, room, q_heads):
     """A key without numbers leaves none in its head's outputs, a value in its quarter's; the other heads and sequences keep theirs."""
-    q, kc, vc = attention_inputs(2, 8, 4, 128, bits, 100)
+    group = q_heads // 4
+    q, kc, vc = attention_inputs(2, q_heads, 4, 128, bits, 100)
+    kc, vc = (torch.cat((c, torch.full((2, 4, room - 100, c.shape[3]), 255, dtype=torch.uint8, device="cuda")), 2) for c in (kc, vc))
     lens = torch.tensor([100, 90], dtype=torch.int32).cuda()
     want = gpu.attention_packed_cache(q, kc, vc, lens)
     k, v = gpu.read_cache_packed(kc, vc, 100, 128)
@@ -401,21 +430,22 @@ def test_visible_rows_that_are_no_numbers(gpu, bits):
     kc2[1], vc2[1, :2], vc2[1, 3, :95] = kc[1], vc[1, :2], vc[1, 3, :95]
     out, lse = gpu.attention_packed_cache(q, kc2, vc2, lens)
     bad = torch.zeros_like(out, dtype=torch.bool)
-    bad[0, 2:4] = True
-    bad[1, 4:6, 32:64] = True
+    bad[0, group:2 * group] = True
+    bad[1, 2 * group:3 * group, 32:64] = True
     assert torch.equal(torch.isnan(out), bad) and torch.equal(torch.isnan(lse), bad.all(2))
     other = ~bad
-    other[1, 4:6] = False
+    other[1, 2 * group:3 * group] = False
     assert torch.equal(out[other], want[0][other]) and torch.equal(lse[~bad.all(2)], want[1][~bad.all(2)])
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 @pytest.mark.parametrize("bits", [4, 8])
-def test_sizes_of_values_and_scores(gpu, dtype, bits):
+@pytest.mark.parametrize("q_heads", [4, 8, 16, 32])
+def test_sizes_of_values_and_scores(gpu, dtype, bits, q_heads):
     """Values from 2^-12 to 2^12 in quarters side by side and in rows behind one another, scores that rise and fall by hundreds, negative and zero scales."""
     seqs, rows = 3, 300
-    k, q = made(seqs, 2, rows, 128, seed=5), made(seqs, 4, 128, dtype=dtype, seed=6, gain=8.0)
+    k, q = made(seqs, 2, rows, 128, seed=5), made(seqs, q_heads, 128, dtype=dtype, seed=6, gain=8.0)
     v = made(seqs, 2, rows, 128, seed=7).float()
     v *= 2.0 ** torch.linspace(-12, 12, 4).repeat_interleave(32).cuda()
     v[1] *= 2.0 ** torch.linspace(0, -12, rows).cuda()[:, None]
@@ -427,17 +457,19 @@ def test_sizes_of_values_and_scores(gpu, dtype, bits):
 
 
 @pytest.mark.gpu
-def test_queries_of_any_size(gpu):
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("heads", [4, 8, 16, 32])
+def test_queries_of_any_size(gpu, bits, heads):
     """Queries at both ends of their types, and tiny ones beside them."""
-    _, kc, vc = attention_inputs(1, 4, 2, 128, 4, 50)
+    _, kc, vc = attention_inputs(1, 4, 2, 128, bits, 50)
     lens = torch.tensor([50], dtype=torch.int32)
     for dtype, sizes in ((torch.float16, (6e4, 2.0 ** -14, 2.0 ** -24)), (torch.bfloat16, (1e30, 6e4, 1e-30, 2.0 ** -133))):
         for size in sizes:
-            q = (made(1, 4, 128, seed=3).float().clamp(-1, 1) * size).to(dtype)
+            q = (made(1, heads, 128, seed=3).float().clamp(-1, 1) * size).to(dtype)
             q[0, 0, 0], q[0, 1, 5] = 0.0, size / 2 ** 12
             scale = 0.1 / max(size, 1e-30) if size > 1e-4 else 1e10
             check_attention(gpu.attention_packed_cache(q, kc, vc, lens.cuda(), scale=scale), q, kc, vc, lens, scale)
-    zero = torch.zeros(1, 4, 128, dtype=torch.float16, device="cuda")
+    zero = torch.zeros(1, heads, 128, dtype=torch.float16, device="cuda")
     check_attention(gpu.attention_packed_cache(zero, kc, vc, lens.cuda()), zero, kc, vc, lens)
 
 
