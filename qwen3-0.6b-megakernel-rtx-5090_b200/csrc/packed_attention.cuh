@@ -1,16 +1,25 @@
 // Attention of one new token per sequence over a packed cache (packed_cache.cuh): out = softmax(scale * q . k) v, k and v the rows' values.
 //
-// With c(d) = n - M the codes around their middle, b(d) the quarter of dimension d, s and z a row's scales and centres:
+// With n the codes, M = 2^(BITS - 1), b(d) the quarter of dimension d, s and z a row's scales and centres:
 //   q . k = sum_b s_b (sum_{d in b} q_d n_d - M Q_b) + sum_b z_b Q_b,   Q_b = sum_{d in b} q_d,
-//   out_d = sum_r p_r z_{r,b(d)} + sum_r (p_r s_{r,b(d)}) c_{r,d},
-// so codes enter the products as they are: n as the fp16 number n 2^-24 is its own bit pattern, and masking four bits of each half of a word makes two
-// operands at once.  Rows of the cache are the 16 rows of an mma.sync tile and query heads its eight columns (NT blocks of them).  Scores: codes times queries, one
-// sum for each quarter, which starts at -M Q_b; out^T: codes times weights times scales.  Weights are carried as two fp16 numbers and the product with a
-// scale is rounded once, to fp16: as much as the rounding of an fp16 output; sums, softmax statistics and outputs are fp32.
+//   out_d = sum_r p_r z_{r,b(d)} + sum_r (p_r s_{r,b(d)}) n_{r,d} - M sum_r (p_r s_{r,b(d)}),
+// so codes enter the products as they are: the number n 2^-24 is the fp16 pattern n, and masking some bits of both halves of a word makes two operands.  Rows
+// of the cache are the 16 rows of an mma.sync tile, query heads its eight columns (tcgen05's 128 rows of queries are not there: a kv head has one to sixteen); a row's trailer, 16 bytes,
+// is a row of an 8 x 8 tile, so ldmatrix makes the operands of the sums over centres.
 //
-// Work: tiles of 32 rows of a (sequence, kv head), all in one line; each warp takes an equal stretch of it, whatever the sequences' lengths, with a ring of copies
-// of its own.  A stretch that holds a whole item writes its output; parts of an item leave their states - the maximum, the sum and the unnormalised output -
-// in the workspace, and a second launch joins them.
+// Roundings: queries are taken to fp16 times a power of two, which leaves them as they are but for entries below 2^-26 of the largest.  Weights are carried
+// as two fp16 numbers (one where the output is bf16), and the product with a scale is rounded once, to fp16, because the tensor cores multiply 16-bit numbers: as much
+// as the output's own rounding, so the error against 64 bits is 1.4 times an exact softmax's (1.0 in bf16).  The third sum above takes the rounded products, so M does
+// not add to that.  Sums, softmax statistics and outputs are fp32.
+//
+// Work: tiles of 32 rows, a tile to a warp, each with a ring of copies of its own (cp.async: no waits but for its own copies).  attend_items: a cluster of CTAs has a (sequence, kv
+// head) and joins its states - the maximum, the sum and the unnormalised output - in shared memory.  attend_tiles: the tiles of all items in one line, of which
+// each warp takes an equal stretch, whatever the sequences' lengths; a stretch that holds a whole item writes its output, parts of items leave their states in the workspace,
+// and a second launch joins them.
+//
+// Measured, caches cold: 96 sequences of 8192 rows, two heads on each of eight kv heads, 4 bits: 160 to 164 us in all, 6.2 TB/s, 0.95 of the copy rate; bound by HBM, with 250 warp
+// instructions for 16 rows.  32 of 8192 rows (336 MB), us of attend_tiles alone with 2 / 4 / 8 / 16 query heads a kv head: 63 / 69 / 76 / 114: bound by the issue of
+// instructions from 4 on (55 %, four or three warps a scheduler, waits for the ALU and fixed latencies), by 255 registers and two warps a scheduler with 16.  The joins: 4 to 6 us.
 #ifndef QMK_PACKED_ATTENTION_CUH_
 #define QMK_PACKED_ATTENTION_CUH_
 
@@ -21,10 +30,11 @@ namespace qmk_packed {
 constexpr int MAX_GROUP = 16;                    // query heads per kv head
 constexpr int TILE = 32;                         // rows
 constexpr int WARPS = 4, SMS = 148;
-// CTAs on an SM: what registers allow (168 a thread, 255 with two blocks of heads); tiles of a warp's ring: what their shared memory does
 // How a tile is taken: by one or two query heads (PAIR), three or four (QUAD), blocks of up to eight (ONE, TWO)
 enum Way { PAIR, QUAD, ONE, TWO };
 __host__ __device__ constexpr Way way_of(int group) { return group <= 2 ? PAIR : group <= 4 ? QUAD : group <= 8 ? ONE : TWO; }
+// CTAs on an SM: four where 128 registers do and a tile has at most 5 KB, three of 168, or two of 255.  Four against three, us: 96 sequences of 8192 rows 160 and 164 (PAIR), 128 of up
+// to 256 14.7 and 17.7; ONE with 128 dims spills in 128 registers: 64 sequences of up to 4096 rows, eight heads a kv head, 35.0 and 32.5.
 __host__ __device__ constexpr int ctas_per_sm(Way way, int dim, int bits) { return way == TWO ? 2 : bits * dim <= 512 && (way != ONE || dim == 64) ? 4 : 3; }
 // (228 KB an SM; of a CTA 1 KB is the system's, 1.25 KB the line's)
 constexpr int warp_bytes(int ctas) { return (228 * 1024 - ctas * 2304) / (ctas * WARPS); }
@@ -188,7 +198,7 @@ template <typename T, int DIM> __device__ __forceinline__ void store_out(T *to, 
   else *reinterpret_cast<uint32_t *>(to) = *reinterpret_cast<const uint32_t *>(o);
 }
 
-// What both ways to take a tile below have in common.
+// What the ways to take a tile have in common.
 template <int DIM, int BITS, Way WAY, int HEADS>
 struct Tiles {
   static constexpr int CTAS = ctas_per_sm(WAY, DIM, BITS), HEAD_DIM = DIM;
@@ -1078,7 +1088,7 @@ __device__ __forceinline__ void zero_heads(const AttendParams &p, int dim, int b
   for (int i = lane; p.lse && i < n; i += 32) p.lse[row + i] = -INFINITY;
 }
 // Short items, one launch: a cluster of CTAs takes an item, each warp an equal part of its tiles; the states stay in shared memory, where all of the cluster
-// can read them, and its warps join them, 16 dimensions of a query head each.
+// can read them, and its warps join them.
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));

@@ -942,8 +942,10 @@ def read_cache_packed(k_cache, v_cache, rows: int, dim: int = 128, dtype: torch.
     code = _ROW_TYPES.get(dtype, -1)
     if code < 0:
         raise RuntimeError(f"{who}: the type must be fp16 or bf16")
-    first = k_cache if isinstance(k_cache, torch.Tensor) else k_cache[0]
-    if not first.is_cuda:
+    if not isinstance(k_cache, torch.Tensor):
+        k_cache = list(k_cache)
+    first = k_cache if isinstance(k_cache, torch.Tensor) else k_cache[0] if k_cache else None
+    if first is None or not first.is_cuda:
         _require_cuda()
         raise RuntimeError(f"{who}: packed caches must be CUDA tensors")
     index = first.get_device()

@@ -122,6 +122,12 @@ def attention_inputs(seqs, q_heads, kv_heads, dim, bits, rows, dtype="fp16", see
     return q, packed(k, bits).cuda(), packed(v, bits).cuda()
 
 
+def with_room(cache, rows):
+    """The cache with room for ``rows`` rows, nothing sensible in those behind its own."""
+    n, heads, have, size = cache.shape
+    return torch.cat((cache, torch.full((n, heads, rows - have, size), 255, dtype=torch.uint8, device="cuda")), 2) if rows > have else cache
+
+
 # ------------------------------------------------------------------------------------------------------------- refusals (no device)
 def cache_args(C, **change):
     n = change.get("num_sequences", 2)
@@ -224,7 +230,7 @@ def test_wrong_tensors_are_refused(gpu):
                 (k, v, kc, vc, 2 ** 31), (k, v, kc, vc, 0, lens.cpu()), (k, v, kc, vc, 1.5), (k[:1], v[:1], kc, vc)):
         with pytest.raises(RuntimeError):
             gpu.write_cache_packed(*bad)
-    for bad, named in (((kc, vc, 3, 96), {}), ((kc, vc, -1, 64), {}), ((kc, vc, 3, 64, torch.float32), {}), ((kc, vc, 3, 128), {}), ((kc.cpu(), vc.cpu(), 3, 64), {}),
+    for bad, named in (((kc, vc, 3, 96), {}), ((kc, vc, -1, 64), {}), ((kc, vc, 3, 64, torch.float32), {}), ((kc, vc, 3, 128), {}), ((kc.cpu(), vc.cpu(), 3, 64), {}), (([], [], 3, 64), {}), ((list(kc), list(vc)[:1], 3, 64), {}),
                        ((kc, vc, 3, 64), dict(k_out=k)), ((kc, vc, 3, 64), dict(k_out=k, v_out=v.bfloat16())), ((kc, vc, 4, 64), dict(k_out=k, v_out=v)),
                        ((kc, vc, 3, 64), dict(k_out=k, v_out=v.transpose(1, 2).contiguous().transpose(1, 2)))):
         with pytest.raises(RuntimeError):
@@ -415,7 +421,7 @@ def test_visible_rows_that_are_no_numbers(gpu, bits, room, q_heads):
     """A key without numbers leaves none in its head's outputs, a value in its quarter's; the other heads and sequences keep theirs."""
     group = q_heads // 4
     q, kc, vc = attention_inputs(2, q_heads, 4, 128, bits, 100)
-    kc, vc = (torch.cat((c, torch.full((2, 4, room - 100, c.shape[3]), 255, dtype=torch.uint8, device="cuda")), 2) for c in (kc, vc))
+    kc, vc = with_room(kc, room), with_room(vc, room)
     lens = torch.tensor([100, 90], dtype=torch.int32).cuda()
     want = gpu.attention_packed_cache(q, kc, vc, lens)
     k, v = gpu.read_cache_packed(kc, vc, 100, 128)
@@ -474,14 +480,17 @@ def test_queries_of_any_size(gpu, bits, heads):
 
 
 @pytest.mark.gpu
-def test_lists_views_and_strides(gpu):
-    q, kc, vc = attention_inputs(5, 8, 2, 128, 8, 70)
+@pytest.mark.parametrize("room", [70, 30000])
+@pytest.mark.parametrize("q_heads,bits", [(4, 4), (8, 8), (16, 4), (32, 8)])
+def test_lists_views_and_strides(gpu, room, q_heads, bits):
+    q, kc, vc = attention_inputs(5, q_heads, 2, 128, bits, 70)
+    kc, vc = with_room(kc, room), with_room(vc, room)
     lens = torch.tensor([70, 1, 0, 33, 64], dtype=torch.int32)
     want = gpu.attention_packed_cache(q, kc, vc, lens.cuda())
     again = gpu.attention_packed_cache(q, list(kc), list(vc), lens.cuda())
     assert torch.equal(want[0], again[0]) and torch.equal(want[1], again[1])
     both = torch.stack((kc, vc), 3).transpose(1, 2).contiguous().transpose(1, 2)           # [sequence, row, head, k / v, bytes] in memory
-    qv = torch.cat((q, q), 2).view(5, 8, 256)[:, :, 128:]
+    qv = torch.cat((q, q), 2).view(5, q_heads, 256)[:, :, 128:]
     again = gpu.attention_packed_cache(qv, both[:, :, :, 0], both[:, :, :, 1], lens.cuda())
     assert torch.equal(want[0], again[0]) and torch.equal(want[1], again[1])
     same = gpu.attention_packed_cache(q, kc[:1].expand(5, -1, -1, -1), vc[:1].expand(5, -1, -1, -1), lens.cuda())      # one cache for all
@@ -489,8 +498,10 @@ def test_lists_views_and_strides(gpu):
 
 
 @pytest.mark.gpu
-def test_results_do_not_depend_on_the_run_or_the_other_sequences(gpu):
+@pytest.mark.parametrize("room", [700, 9000])
+def test_results_do_not_depend_on_the_run(gpu, room):
     q, kc, vc = attention_inputs(33, 16, 8, 128, 4, 700)
+    kc, vc = with_room(kc, room), with_room(vc, room)
     lens = torch.tensor([(131 * i) % 701 for i in range(33)], dtype=torch.int32).cuda()
     first = gpu.attention_packed_cache(q, kc, vc, lens)
     for _ in range(5):
@@ -501,11 +512,12 @@ def test_results_do_not_depend_on_the_run_or_the_other_sequences(gpu):
 # ------------------------------------------------------------------------------------------------------------- together
 @pytest.mark.gpu
 @pytest.mark.parametrize("bits", [4, 8])
-def test_prompt_then_steps_in_a_captured_graph(gpu, bits):
+@pytest.mark.parametrize("cache", [64, 20000])
+def test_prompt_then_steps_in_a_captured_graph(gpu, bits, cache):
     """A prompt's rows written, then decode steps - the new rows written, the attention over everything so far - replayed from one graph, on a stream of
     their own, with positions that move on the device."""
     seqs, q_heads, kv_heads, dim, room, prompt = 3, 16, 8, 128, 64, 30
-    kc, vc = (torch.zeros(seqs, kv_heads, room, gpu.packed_row_bytes(dim, bits), dtype=torch.uint8, device="cuda") for _ in range(2))
+    kc, vc = (torch.zeros(seqs, kv_heads, cache, gpu.packed_row_bytes(dim, bits), dtype=torch.uint8, device="cuda") for _ in range(2))
     k, v = made(seqs, kv_heads, room, dim, seed=1), made(seqs, kv_heads, room, dim, seed=2)
     lens = torch.tensor([30, 7, 0], dtype=torch.int32)
     gpu.write_cache_packed(k[:, :, :prompt], v[:, :, :prompt], kc, vc, 0, lens.cuda())
@@ -537,8 +549,10 @@ def test_prompt_then_steps_in_a_captured_graph(gpu, bits):
 
 
 @pytest.mark.gpu
-def test_two_streams_at_once(gpu):
+@pytest.mark.parametrize("room", [500, 20000])
+def test_two_streams_at_once(gpu, room):
     cases = [attention_inputs(9, 16, 8, 128, 4, 500, seed=s) for s in (1, 2)]
+    cases = [(q, with_room(kc, room), with_room(vc, room)) for q, kc, vc in cases]
     lens = torch.tensor([500 - 50 * i for i in range(9)], dtype=torch.int32).cuda()
     want = [gpu.attention_packed_cache(*c, lens) for c in cases]
     streams = [torch.cuda.Stream(), torch.cuda.Stream()]
@@ -597,12 +611,35 @@ def test_a_parked_sequence_comes_back(gpu, bits):
 
 
 @pytest.mark.gpu
+def test_a_graph_beside_another_and_other_sizes_in_between(gpu):
+    """Two graphs of the two ways a call is cut, replayed in turn and with calls of their own between: each keeps its workspace."""
+    cases = [attention_inputs(3, 16, 8, 128, 4, 300, seed=s) for s in (1, 2)]
+    cases[1] = (cases[1][0], with_room(cases[1][1], 20000), with_room(cases[1][2], 20000))
+    lens = torch.tensor([300, 0, 117], dtype=torch.int32).cuda()
+    want = [gpu.attention_packed_cache(*c, lens) for c in cases]
+    graphs, got = [], []
+    for c in cases * 2:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got.append(gpu.attention_packed_cache(*c, lens))
+        graphs.append(graph)
+    for _ in range(3):
+        for graph in graphs:
+            graph.replay()
+        again = gpu.attention_packed_cache(*cases[1], lens)
+    torch.cuda.synchronize()
+    for i, (out, lse) in enumerate(got):
+        assert torch.equal(out, want[i % 2][0]) and torch.equal(lse, want[i % 2][1])
+    assert torch.equal(again[0], want[1][0])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bits", [4, 8])
 def test_caches_further_apart_than_32_bits(gpu, bits):
     """Sequences and heads more than 4 GiB apart."""
     size = gpu.packed_row_bytes(128, bits)
     apart = (1 << 32) + 4096
-    memory = torch.empty(3 * apart + 20 * size, dtype=torch.uint8, device="cuda")
+    memory = torch.empty(3 * apart + 20000 * size, dtype=torch.uint8, device="cuda")
     k, v, q = made(2, 2, 9, 128, seed=1), made(2, 2, 9, 128, seed=2), made(2, 4, 128, seed=3)
     kc, vc = (memory[first:].as_strided((2, 2, 10, size), (2 * apart, apart, size, 1)) for first in (0, 10 * size))
     gpu.write_cache_packed(k, v, kc, vc, 1)
@@ -613,3 +650,8 @@ def test_caches_further_apart_than_32_bits(gpu, bits):
     assert bool(((back[0].double().cpu() - exact).abs() <= rounded_off(exact, torch.float16)).all())
     lens = torch.tensor([10, 7], dtype=torch.int32)
     check_attention(gpu.attention_packed_cache(q, kc, vc, lens.cuda()), q, kc, vc, lens)
+    # the same with room for many rows: the line of tiles
+    long = memory.as_strided((1, 2, 20000, size), (0, apart, size, 1))
+    long[:, :, :9] = packed(k[:1], bits).cuda()
+    lens = torch.tensor([9], dtype=torch.int32)
+    check_attention(gpu.attention_packed_cache(q[:1], long, long, lens.cuda()), q[:1], long, long, lens)
