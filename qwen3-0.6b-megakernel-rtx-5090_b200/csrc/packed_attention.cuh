@@ -9,8 +9,9 @@
 //
 // Roundings: queries are taken to fp16 times a power of two, which leaves them as they are but for entries below 2^-26 of the largest.  Weights are carried
 // as two fp16 numbers (one where the output is bf16), and the product with a scale is rounded once, to fp16, because the tensor cores multiply 16-bit numbers: as much
-// as the output's own rounding, so the error against 64 bits is 1.4 times an exact softmax's (1.0 in bf16).  The third sum above takes the rounded products, so M does
-// not add to that.  Sums, softmax statistics and outputs are fp32.
+// as the output's own rounding, so the error against 64 bits is 1.2 to 1.4 times an exact softmax's (1.0 in bf16).  The third sum above takes the rounded products, so M does
+// not add to that.  Sums, softmax statistics and outputs are fp32.  Every second 16 rows go in as 2^BITS - 1 - n with the weights' sign turned (the same instructions): the running
+// sums stay around zero, whose size the accumulator's truncation goes by (with n throughout one sequence of 32,768 rows was 1.8 times off).
 //
 // Work: tiles of 32 rows, a tile to a warp, each with a ring of copies of its own (cp.async: no waits but for its own copies).  attend_items: a cluster of CTAs has a (sequence, kv
 // head) and joins its states - the maximum, the sum and the unnormalised output - in shared memory.  attend_tiles: the tiles of all items in one line, of which
@@ -99,32 +100,32 @@ template <bool TRANSPOSED, int ROW> __device__ __forceinline__ void trailers(uin
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
   }
 }
-constexpr uint32_t ONES = 0x3c003c00u;           // (1, 1)
 
 // Codes of quarter b of two chunks (DIM/8 codes each), the first in the lower halves: x[j] = (a_j, b_j) as fp16 numbers of 2^-24, of 4-bit codes every second of
-// 2^-20.
-template <int DIM, int BITS>
+// 2^-20; FLIP: 2^BITS - 1 less the code.
+template <int DIM, int BITS, bool FLIP = false>
 __device__ __forceinline__ void expand(const uint32_t (&a)[DIM * BITS / 256], const uint32_t (&c)[DIM * BITS / 256], int b, uint32_t (&x)[DIM / 32]) {
+  constexpr uint32_t ALL = FLIP ? 0xffffffffu : 0u;
   if constexpr (BITS == 4 && DIM == 64) {
     const uint32_t w = __byte_perm(a[0], c[0], b | b << 4 | (4 + b) << 8 | (4 + b) << 12);
-    x[0] = w & 0x000f000fu;
-    x[1] = w & 0x00f000f0u;
+    x[0] = (w ^ ALL) & 0x000f000fu;
+    x[1] = (w ^ ALL) & 0x00f000f0u;
   } else if constexpr (BITS == 4) {
     const uint32_t w = __byte_perm(a[b / 2], c[b / 2], b % 2 ? 0x7632 : 0x5410), u = w >> 8;
-    x[0] = w & 0x000f000fu;
-    x[1] = w & 0x00f000f0u;
-    x[2] = u & 0x000f000fu;
-    x[3] = u & 0x00f000f0u;
+    x[0] = (w ^ ALL) & 0x000f000fu;
+    x[1] = (w ^ ALL) & 0x00f000f0u;
+    x[2] = (u ^ ALL) & 0x000f000fu;
+    x[3] = (u ^ ALL) & 0x00f000f0u;
   } else if constexpr (DIM == 64) {
-    const uint32_t w = __byte_perm(a[b / 2], c[b / 2], b % 2 ? 0x7632 : 0x5410);
-    x[0] = w & 0x00ff00ffu;
-    x[1] = w >> 8 & 0x00ff00ffu;
+    const uint32_t w = __byte_perm(a[b / 2], c[b / 2], b % 2 ? 0x7632 : 0x5410), u = w >> 8;
+    x[0] = (w ^ ALL) & 0x00ff00ffu;
+    x[1] = (u ^ ALL) & 0x00ff00ffu;
   } else {
-    const uint32_t w = __byte_perm(a[b], c[b], 0x5410), u = __byte_perm(a[b], c[b], 0x7632);
-    x[0] = w & 0x00ff00ffu;
-    x[1] = w >> 8 & 0x00ff00ffu;
-    x[2] = u & 0x00ff00ffu;
-    x[3] = u >> 8 & 0x00ff00ffu;
+    const uint32_t w = __byte_perm(a[b], c[b], 0x5410), u = __byte_perm(a[b], c[b], 0x7632), w8 = w >> 8, u8 = u >> 8;
+    x[0] = (w ^ ALL) & 0x00ff00ffu;
+    x[1] = (w8 ^ ALL) & 0x00ff00ffu;
+    x[2] = (u ^ ALL) & 0x00ff00ffu;
+    x[3] = (u8 ^ ALL) & 0x00ff00ffu;
   }
 }
 
@@ -211,6 +212,8 @@ struct Tiles {
   static constexpr int QUERY_STRIDE = DIM, WARP_SMEM = STAGES * STAGE + QUERIES, SMEM = WARPS * WARP_SMEM;
   static_assert(STAGES * STAGE >= HEADS * (DIM * 4 + 8), "a warp's state fits its ring");
   static constexpr float M = 1 << (BITS - 1), UNIT = 0x1p-24f;
+  // What the codes (the flipped ones) are above the numbers they stand for, negative, as pairs of fp16 numbers
+  static constexpr uint32_t MIDDLE = BITS == 4 ? 0xc800c800u : 0xd800d800u, MIDDLE_FLIPPED = BITS == 4 ? 0xc700c700u : 0xd7f0d7f0u;         // -8, -128; -7, -127
   static constexpr bool SPREAD = BITS == 8 && DIM == 128;                                   // a lane's two chunks of keys: four apart, or one behind the other
   static __device__ __forceinline__ int chunk_of(int t, int c) { return SPREAD ? t + 4 * c : 2 * t + c; }
 
@@ -310,7 +313,8 @@ __device__ __forceinline__ void take_tile(A &a, uint32_t kt, int rows, int lane)
         lo[r] = transposed(pack2(rest, rest));
       }
     }
-    a.weigh(vt + 16 * h * ROW, lane, hi, lo);
+    if (h == 0) a.template weigh<false>(vt, lane, hi, lo);
+    else a.template weigh<true>(vt + 16 * ROW, lane, hi, lo);
   }
 }
 
@@ -327,9 +331,8 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
 
   uint32_t qb[KSTEPS][2], qz[2];                 // queries; sums over quarters, as upper and lower fp16 parts
   float factor, m, off, l;                       // what a score is multiplied by, the largest score, what is added in the exponent, the sum of weights
-  float acc[4][STEPS][4], sums[4], zacc[4];      // out^T, quarter by quarter; sums of weights times scales; of weights times centres (lanes g >= 4: of quarter g - 4)
+  float acc[4][STEPS][4], sums[4], zacc[4];      // out^T, quarter by quarter; what is to be taken off; sums of weights times centres (lanes g >= 4: of quarter g - 4)
   __half2 f;                                     // power of two that takes quarter g & 3's scales of values to 1 or below
-  uint32_t ones;
 
   __device__ __forceinline__ void begin(const AttendParams &p, const T *queries, long long stride, int lane) {
     const int t = lane & 3, g = lane >> 2, h = g >> 2, quarter = g & 3;
@@ -378,7 +381,6 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
       for (int u = 0; u < STEPS; ++u) { acc[i][u][0] = 0.0f; acc[i][u][1] = 0.0f; acc[i][u][2] = 0.0f; acc[i][u][3] = 0.0f; }
     }
     f = __float2half2_rn(0x1p15f);
-    ones = ONES;
   }
 
   // Scores of rows g and g + 8 of 16, times the power of two, head t / 2
@@ -442,7 +444,9 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
   }
 
   // Weights of 16 rows (upper and lower parts, rows 2 t, 2 t + 1 and those + 8 of column g) times their values
+  template <bool FLIP>
   __device__ __forceinline__ void weigh(uint32_t vt, int lane, const uint32_t (&hi)[2], const uint32_t (&lo)[2]) {
+    constexpr uint32_t MIDDLE = FLIP ? Base::MIDDLE_FLIPPED : Base::MIDDLE;
     const int t = lane & 3, g = lane >> 2;
     uint32_t raw[4], w[4][N], pb[2];
     trailers<true, ROW>(vt + CODES, lane, raw);
@@ -455,6 +459,7 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
       s0 = __hmul2(h2(r0), f);
       s1 = __hmul2(h2(r1), f);
     }
+    if (FLIP) { s0 = __hneg2(s0); s1 = __hneg2(s1); }
     if constexpr (LOWER) {
       pb[0] = bits_of(__hfma2(h2(hi[0]), s0, __hmul2(h2(lo[0]), s0)));
       pb[1] = bits_of(__hfma2(h2(hi[1]), s1, __hmul2(h2(lo[1]), s1)));
@@ -462,12 +467,12 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
       pb[0] = bits_of(__hmul2(h2(hi[0]), s0));
       pb[1] = bits_of(__hmul2(h2(hi[1]), s1));
     }
-    mma(sums, ones, ones, ones, ones, pb[0], pb[1], sums[0], sums[1], sums[2], sums[3]);
+    mma(sums, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pb[0], pb[1], sums[0], sums[1], sums[2], sums[3]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t first[J], second[J];
-      expand<DIM, BITS>(w[0], w[1], i, first);
-      expand<DIM, BITS>(w[2], w[3], i, second);
+      expand<DIM, BITS, FLIP>(w[0], w[1], i, first);
+      expand<DIM, BITS, FLIP>(w[2], w[3], i, second);
 #pragma unroll
       for (int u = 0; u < STEPS; ++u) {
         float (&c)[4] = acc[i][u];
@@ -509,7 +514,7 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         const float c = t & 1 ? acc[2 + e][j / 2][e + 2 * (j % 2)] : acc[e][j / 2][e + 2 * (j % 2)];
-        v[j] = fmaf(fmaf(c, (BITS == 4 && j % 2 ? 0.0625f : 1.0f) / UNIT, -M * sums[e]), inverse, z);
+        v[j] = fmaf(fmaf(c, (BITS == 4 && j % 2 ? 0.0625f : 1.0f) / UNIT, sums[e]), inverse, z);
       }
       if (!live) continue;
       if (state) store_part<DIM>(state + h * DIM + DIM / 4 * i + J * g, v);
@@ -532,9 +537,8 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
 
   uint32_t qb[2][STEPS][2], qz[2];               // queries of the column's even and odd quarter; sums over quarters, as upper and lower fp16 parts
   float factor, m, off, l;                       // what a score is multiplied by, the largest score, what is added in the exponent, the sum of weights; of head t
-  float acc[4][STEPS][4], sums[2][4], zacc[4];   // out^T, quarter by quarter; sums of weights times scales; of weights times centres (lanes g >= 4: of quarter g - 4)
+  float acc[4][STEPS][4], sums[2][4], zacc[4];   // out^T, quarter by quarter; what is to be taken off; sums of weights times centres (lanes g >= 4: of quarter g - 4)
   __half2 f;                                     // power of two that takes quarter g & 3's scales of values to 1 or below
-  uint32_t ones;
 
   __device__ __forceinline__ void begin(const AttendParams &p, const T *queries, long long stride, int lane) {
     const int t = lane & 3, g = lane >> 2, h = g >> 1, half = g & 1;
@@ -587,7 +591,6 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
       for (int u = 0; u < STEPS; ++u) { acc[i][u][0] = 0.0f; acc[i][u][1] = 0.0f; acc[i][u][2] = 0.0f; acc[i][u][3] = 0.0f; }
     }
     f = __float2half2_rn(0x1p15f);
-    ones = ONES;
   }
 
   // Scores of rows g and g + 8 of 16, times the power of two, head t
@@ -642,7 +645,9 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
   }
 
   // Weights of 16 rows (upper and lower parts, rows 2 t, 2 t + 1 and those + 8 of column g) times their values
+  template <bool FLIP>
   __device__ __forceinline__ void weigh(uint32_t vt, int lane, const uint32_t (&hi)[2], const uint32_t (&lo)[2]) {
+    constexpr uint32_t MIDDLE = FLIP ? Base::MIDDLE_FLIPPED : Base::MIDDLE;
     const int t = lane & 3, g = lane >> 2;
     uint32_t raw[4], w[4][N], pb[2][2];
     trailers<true, ROW>(vt + CODES, lane, raw);
@@ -657,7 +662,8 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {                // quarter 2 (g & 1) + i
       const int from = 8 * (g & 1) + 4 * i + t;
-      const __half2 a0 = h2(__shfl_sync(0xffffffffu, bits_of(s0), from)), a1 = h2(__shfl_sync(0xffffffffu, bits_of(s1), from));
+      __half2 a0 = h2(__shfl_sync(0xffffffffu, bits_of(s0), from)), a1 = h2(__shfl_sync(0xffffffffu, bits_of(s1), from));
+      if (FLIP) { a0 = __hneg2(a0); a1 = __hneg2(a1); }
       if constexpr (LOWER) {
         pb[i][0] = bits_of(__hfma2(h2(hi[0]), a0, __hmul2(h2(lo[0]), a0)));
         pb[i][1] = bits_of(__hfma2(h2(hi[1]), a1, __hmul2(h2(lo[1]), a1)));
@@ -666,13 +672,13 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
         pb[i][1] = bits_of(__hmul2(h2(hi[1]), a1));
       }
       float (&c)[4] = sums[i];
-      mma(c, ones, ones, ones, ones, pb[i][0], pb[i][1], c[0], c[1], c[2], c[3]);
+      mma(c, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pb[i][0], pb[i][1], c[0], c[1], c[2], c[3]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t first[J], second[J];
-      expand<DIM, BITS>(w[0], w[1], i, first);
-      expand<DIM, BITS>(w[2], w[3], i, second);
+      expand<DIM, BITS, FLIP>(w[0], w[1], i, first);
+      expand<DIM, BITS, FLIP>(w[2], w[3], i, second);
 #pragma unroll
       for (int u = 0; u < STEPS; ++u) {
         float (&c)[4] = acc[i][u];
@@ -712,7 +718,7 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
       float v[J];
 #pragma unroll
       for (int j = 0; j < J; ++j)
-        v[j] = fmaf(fmaf(acc[i][j / 2][i / 2 + 2 * (j % 2)], (BITS == 4 && j % 2 ? 0.0625f : 1.0f) / UNIT, -M * sums[i % 2][i / 2]), inverse, z);
+        v[j] = fmaf(fmaf(acc[i][j / 2][i / 2 + 2 * (j % 2)], (BITS == 4 && j % 2 ? 0.0625f : 1.0f) / UNIT, sums[i % 2][i / 2]), inverse, z);
       if (!live) continue;
       if (state) store_part<DIM>(state + h * DIM + DIM / 4 * i + J * g, v);
       else store_out<T, DIM>(static_cast<T *>(p.out) + row * DIM + DIM / 4 * i + J * g, v, by);
@@ -733,9 +739,8 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
 
   uint32_t qb[NT][4][STEPS][2], qz[NT][2];       // queries; sums over quarters, as upper and lower fp16 parts
   float factor[NT][2], m[NT][2], off[NT][2], l[NT][2];     // of heads 2 t and 2 t + 1: what a score is multiplied by, the largest score, what is added in the exponent, the sum of weights
-  float acc[NT][4][STEPS][4], sums[NT][4][4], zacc[NT][4]; // out^T, quarter by quarter; sums of weights times scales; of weights times centres (lanes g >= 4: of quarter g - 4)
+  float acc[NT][4][STEPS][4], sums[NT][4][4], zacc[NT][4]; // out^T, quarter by quarter; what is to be taken off; sums of weights times centres (lanes g >= 4: of quarter g - 4)
   __half2 f;                                     // power of two that takes quarter g & 3's scales of values to 1 or below
-  uint32_t ones;
 
   // An item's queries, `stride` apart (global or shared memory), and nothing seen yet
   __device__ __forceinline__ void begin(const AttendParams &p, const T *queries, long long stride, int lane) {
@@ -793,7 +798,6 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
       }
     }
     f = __float2half2_rn(0x1p15f);
-    ones = ONES;
   }
 
   // Scores of 16 rows, times the power of two: rows g and g + 8, heads 2 t and 2 t + 1
@@ -855,7 +859,9 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
   }
 
   // Weights of 16 rows (upper and lower parts, rows 2 t, 2 t + 1 and those + 8 of head g) times their values
+  template <bool FLIP>
   __device__ __forceinline__ void weigh(uint32_t vt, int lane, const uint32_t (&hi)[NT][2], const uint32_t (&lo)[NT][2]) {
+    constexpr uint32_t MIDDLE = FLIP ? Base::MIDDLE_FLIPPED : Base::MIDDLE;
     const int t = lane & 3, g = lane >> 2;
     uint32_t raw[4], w[4][N];
     trailers<true, ROW>(vt + CODES, lane, raw);
@@ -870,7 +876,8 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t first[J], second[J], pb[NT][2];
-      const __half2 a0 = h2(__shfl_sync(0xffffffffu, bits_of(s0), 4 * i + t)), a1 = h2(__shfl_sync(0xffffffffu, bits_of(s1), 4 * i + t));
+      __half2 a0 = h2(__shfl_sync(0xffffffffu, bits_of(s0), 4 * i + t)), a1 = h2(__shfl_sync(0xffffffffu, bits_of(s1), 4 * i + t));
+      if (FLIP) { a0 = __hneg2(a0); a1 = __hneg2(a1); }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         if constexpr (LOWER) {
@@ -881,10 +888,10 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
           pb[nt][1] = bits_of(__hmul2(h2(hi[nt][1]), a1));
         }
         float (&c)[4] = sums[nt][i];
-        mma(c, ones, ones, ones, ones, pb[nt][0], pb[nt][1], c[0], c[1], c[2], c[3]);
+        mma(c, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pb[nt][0], pb[nt][1], c[0], c[1], c[2], c[3]);
       }
-      expand<DIM, BITS>(w[0], w[1], i, first);
-      expand<DIM, BITS>(w[2], w[3], i, second);
+      expand<DIM, BITS, FLIP>(w[0], w[1], i, first);
+      expand<DIM, BITS, FLIP>(w[2], w[3], i, second);
 #pragma unroll
       for (int u = 0; u < STEPS; ++u)
 #pragma unroll
@@ -975,7 +982,8 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
           }
         }
       }
-      weigh(vt + 16 * h * ROW, lane, hi, lo);
+      if (h == 0) weigh<false>(vt, lane, hi, lo);
+      else weigh<true>(vt + 16 * ROW, lane, hi, lo);
     }
   }
 
@@ -1001,7 +1009,7 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
           float v[J];
 #pragma unroll
           for (int j = 0; j < J; ++j)
-            v[j] = fmaf(fmaf(acc[nt][i][j / 2][e + 2 * (j % 2)], (BITS == 4 && j % 2 ? 0.0625f : 1.0f) / UNIT, -M * sums[nt][i][e]), inverse[i], z);
+            v[j] = fmaf(fmaf(acc[nt][i][j / 2][e + 2 * (j % 2)], (BITS == 4 && j % 2 ? 0.0625f : 1.0f) / UNIT, sums[nt][i][e]), inverse[i], z);
           if (h >= p.group) continue;
           if (state) store_part<DIM>(state + h * DIM + DIM / 4 * i + J * g, v);
           else store_out<T, DIM>(static_cast<T *>(p.out) + row * DIM + DIM / 4 * i + J * g, v, by);
