@@ -177,13 +177,28 @@ struct Place {
     head = i / tiles;
     tile = i - head * tiles;
   }
+};
+
+// An item on a warp's way along the line, and how many of its rows are left
+struct Item {
+  int b, head, left;
   __device__ __forceinline__ void next(const AttendParams &p, const Line &line) {
-    if (++tile < tiles) return;
-    tile = 0;
-    if (++head < p.caches.kv_heads) return;
-    head = 0;
-    do sequence(line, b + 1); while (tiles == 0 && b < p.caches.seqs);
+    if (++head == p.caches.kv_heads) {
+      head = 0;
+      do ++b; while (b < p.caches.seqs && line.rows[b] == 0);
+    }
+    left = b < p.caches.seqs ? line.rows[b] : 0;
   }
+};
+// Where its next tile is copied from: the lane's first 16 bytes of it
+struct Source {
+  const unsigned char *k, *v;
+  __device__ __forceinline__ void at(const AttendParams &p, const Item &item, int tile, int lane) {
+    const long long base = static_cast<long long>(item.head) * p.caches.head + static_cast<long long>(tile) * TILE * p.caches.row + lane * 16;
+    k = p.caches.k[item.b] + base;
+    v = p.caches.v[item.b] + base;
+  }
+  __device__ __forceinline__ void next(const AttendParams &p) { k += TILE * p.caches.row; v += TILE * p.caches.row; }
 };
 
 // DIM/32 values of a row side by side
@@ -217,18 +232,16 @@ struct Tiles {
   static constexpr bool SPREAD = BITS == 8 && DIM == 128;                                   // a lane's two chunks of keys: four apart, or one behind the other
   static __device__ __forceinline__ int chunk_of(int t, int c) { return SPREAD ? t + 4 * c : 2 * t + c; }
 
-  static __device__ __forceinline__ void load(const AttendParams &p, const Place &at, uint32_t dst, int lane) {
-    const long long base = static_cast<long long>(at.head) * p.caches.head + static_cast<long long>(at.tile) * TILE * p.caches.row;
-    const unsigned char *const k = p.caches.k[at.b] + base, *const v = p.caches.v[at.b] + base;
-    const int pieces = min(at.rows - at.tile * TILE, TILE) * PIECES;
-    if (p.caches.row == ROW && pieces == TILE * PIECES) {                   // rows right behind one another, all there
-      const unsigned char *const ks = k + lane * 16, *const vs = v + lane * 16;
+  static __device__ __forceinline__ void load(const AttendParams &p, const Source &from, int rows, uint32_t dst, int lane) {
+    if (p.caches.row == ROW && rows >= TILE) {   // rows right behind one another, all there
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
-        copy16(dst + lane * 16 + 512 * i, ks + 512 * i);
-        copy16(dst + lane * 16 + TILE * ROW + 512 * i, vs + 512 * i);
+        copy16(dst + lane * 16 + 512 * i, from.k + 512 * i);
+        copy16(dst + lane * 16 + TILE * ROW + 512 * i, from.v + 512 * i);
       }
     } else {
+      const unsigned char *const k = from.k - lane * 16, *const v = from.v - lane * 16;
+      const int pieces = min(rows, TILE) * PIECES;
 #pragma unroll 1
       for (int i = 0; i < PIECES; ++i) {
         const int piece = lane + 32 * i;
@@ -241,7 +254,7 @@ struct Tiles {
   }
   // The queries of an item, one head behind the other
   template <typename T>
-  static __device__ __forceinline__ void load_queries(const AttendParams &p, const Place &at, uint32_t dst, int lane) {
+  static __device__ __forceinline__ void load_queries(const AttendParams &p, const Item &at, uint32_t dst, int lane) {
     const T *const q = static_cast<const T *>(p.q) + at.b * p.q_seq + static_cast<long long>(at.head) * p.group * p.q_head;
     for (int i = lane; i < p.group * (DIM / 8); i += 32) copy16(dst + i * 16, q + i / (DIM / 8) * p.q_head + i % (DIM / 8) * 8);
   }
@@ -273,7 +286,7 @@ struct Tiles {
   }
 };
 
-// A tile where all of a thread's columns are of one query head; `rows` rows of it (32 or fewer) are there.
+// A tile where all of a thread's columns are of one query head; `rows` rows of it are there (32 or more: all).
 template <int ROW, typename A>
 __device__ __forceinline__ void take_tile(A &a, uint32_t kt, int rows, int lane) {
   const int g = lane >> 2;
@@ -908,7 +921,7 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
     }
   }
 
-  // A tile, of which `rows` rows (32 or fewer) are there
+  // A tile, of which `rows` rows are there (32 or more: all)
   __device__ __forceinline__ void tile(uint32_t kt, int rows, int lane) {
     const int g = lane >> 2;
     const uint32_t vt = kt + TILE * ROW;
@@ -1038,18 +1051,30 @@ __global__ void __launch_bounds__(WARPS * 32, A::CTAS) attend_tiles(const __grid
   const int first = begin_of(line.total, parts, r), last = begin_of(line.total, parts, r + 1);
   unsigned char *const own = smem + warp * A::WARP_SMEM;
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(own));
-  Place ahead, now;
-  now.start(p, line, first);
-  ahead = now;
-  int fetched = first, queries_of = -1;          // the first tile of the item whose queries wait in shared memory
+  Place place;
+  place.start(p, line, first);
+  Item now{place.b, place.head, place.rows - place.tile * TILE}, ahead = now;
+  Source source;
+  source.at(p, ahead, place.tile, lane);
+  int fetched = first, began = first - place.tile, queries_of = -1;         // tiles asked for; the item's first tile; the one whose item's queries wait in shared memory
+  uint32_t put = ring, get = ring;
+  bool fresh = true;                             // whether the next tile to ask for is the first of its item, or of all
   auto fetch = [&]() {
     if (fetched < last) {
-      A::load(p, ahead, ring + (fetched - first) % STAGES * A::STAGE, lane);
-      if (A::QUERIES && queries_of < 0 && (ahead.tile == 0 || fetched == first)) {
+      A::load(p, source, ahead.left, put, lane);
+      if (A::QUERIES && fresh && queries_of < 0) {
         A::template load_queries<typename A::Value>(p, ahead, ring + STAGES * A::STAGE, lane);
         queries_of = fetched;
       }
-      ahead.next(p, line);
+      put = put == ring + (STAGES - 1) * A::STAGE ? ring : put + A::STAGE;
+      ahead.left -= TILE;
+      fresh = ahead.left <= 0;
+      if (fresh && fetched + 1 < last) {
+        ahead.next(p, line);
+        source.at(p, ahead, 0, lane);
+      } else {
+        source.next(p);
+      }
     }
     ++fetched;
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -1057,11 +1082,11 @@ __global__ void __launch_bounds__(WARPS * 32, A::CTAS) attend_tiles(const __grid
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) fetch();
   A a;
-  int began = now.tile;
+  bool begins = true;                            // whether tile i is the first of its item, or of all
   for (int i = first; i < last; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     __syncwarp();                                // every lane's copies of tile i are there, and tile i - 1 has been read
-    if (now.tile == 0 || i == first) {
+    if (begins) {
       const typename A::Value *q = static_cast<const typename A::Value *>(p.q) + now.b * p.q_seq + static_cast<long long>(now.head) * p.group * p.q_head;
       long long stride = p.q_head;
       if (A::QUERIES && queries_of == i) {
@@ -1071,17 +1096,21 @@ __global__ void __launch_bounds__(WARPS * 32, A::CTAS) attend_tiles(const __grid
       a.begin(p, q, stride, lane);
       __syncwarp();                              // (read by all lanes before the next are copied)
       if (queries_of == i) queries_of = -1;
-      began = now.tile;
+      begins = false;
     }
     fetch();
-    a.tile(ring + (i - first) % STAGES * A::STAGE, min(now.rows - now.tile * TILE, TILE), lane);
-    const bool done = now.tile == now.tiles - 1;
-    if (done || i == last - 1) {
-      const size_t slot = static_cast<size_t>(2 * r + (began == 0 && i - first > now.tile)) * p.group;
-      const bool whole = done && began == 0;
+    a.tile(get, now.left, lane);
+    get = get == ring + (STAGES - 1) * A::STAGE ? ring : get + A::STAGE;
+    now.left -= TILE;
+    if (now.left <= 0 || i == last - 1) {
+      const size_t slot = static_cast<size_t>(2 * r + (began > first)) * p.group;
+      const bool whole = now.left <= 0 && began >= first;
       a.end(p, now.b, now.head, whole ? nullptr : p.part_out + slot * A::HEAD_DIM, whole ? nullptr : p.part_ml + slot, lane);
+      if (i == last - 1) break;
+      now.next(p, line);
+      began = i + 1;
+      begins = true;
     }
-    if (i < last - 1) now.next(p, line);
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
@@ -1192,11 +1221,17 @@ __global__ void __launch_bounds__(WARPS * 32, A::CTAS) attend_items(const __grid
   unsigned char *const own = smem + warp * A::WARP_SMEM;
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(own));
   if (first < last) {
-    Place ahead = now;
-    ahead.tile = first;
+    Source source;
+    source.at(p, Item{now.b, now.head, 0}, first, lane);
+    int fetched = first;
+    uint32_t put = ring, get = ring;
     auto fetch = [&]() {
-      if (ahead.tile < last) A::load(p, ahead, ring + (ahead.tile - first) % STAGES * A::STAGE, lane);
-      ++ahead.tile;
+      if (fetched < last) {
+        A::load(p, source, now.rows - fetched * TILE, put, lane);
+        put = put == ring + (STAGES - 1) * A::STAGE ? ring : put + A::STAGE;
+        source.next(p);
+      }
+      ++fetched;
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
@@ -1207,7 +1242,8 @@ __global__ void __launch_bounds__(WARPS * 32, A::CTAS) attend_items(const __grid
       asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
       __syncwarp();                              // every lane's copies of tile i are there, and tile i - 1 has been read
       fetch();
-      a.tile(ring + (i - first) % STAGES * A::STAGE, min(now.rows - i * TILE, TILE), lane);
+      a.tile(get, now.rows - i * TILE, lane);
+      get = get == ring + (STAGES - 1) * A::STAGE ? ring : get + A::STAGE;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncwarp();
