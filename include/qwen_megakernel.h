@@ -525,7 +525,7 @@ typedef struct qmk_packed_attention {
   long long workspace_bytes;
 } qmk_packed_attention;
 int qmk_attention_packed_cache(const qmk_packed_cache *cache, const qmk_packed_attention *args, cudaStream_t stream);
-/* Bytes; 0 for sizes that the call refuses. */
+/* Bytes (0: the call needs none, and takes a null pointer); -1 for sizes that the call refuses. */
 long long qmk_attention_packed_cache_workspace(int num_sequences, int q_heads, int kv_heads, int head_dim, int bits, int rows);
 
 /* Synchronises the device and returns the status word of the last launch

@@ -116,7 +116,7 @@ Cut cut_of(int seqs, int kv_heads, int group, int dim, int bits, int rows) {
   if (items <= ITEM_WAVES * ctas && tiles <= ITEM_TILES * (WARPS << (ranks - 1))) return Cut{ranks, 0};
   return Cut{0, static_cast<int>(std::min<long long>(std::max(most_tiles(seqs, kv_heads, rows), 1ll), ctas * WARPS))};
 }
-long long workspace_bytes(const Cut &cut, int group, int dim) { return std::max(2ll * cut.warps * group * (dim * 4ll + 8), 16ll); }
+long long workspace_bytes(const Cut &cut, int group, int dim) { return 2ll * cut.warps * group * (dim * 4ll + 8); }
 
 // How the parts are joined goes by how many an item has where all stretches are used: warps, or CTAs of four, eight or 32 warps.
 template <typename T, int DIM>
@@ -199,8 +199,8 @@ extern "C" int qmk_read_cache_packed(const qmk_packed_cache *cache, const qmk_pa
 extern "C" long long qmk_attention_packed_cache_workspace(int num_sequences, int q_heads, int kv_heads, int head_dim, int bits, int rows) {
   if (num_sequences < 1 || num_sequences > MAX_SEQS || kv_heads < 1 || kv_heads > MAX_HEADS || q_heads < 1 || q_heads % kv_heads || q_heads / kv_heads > MAX_GROUP ||
       (head_dim != 64 && head_dim != 128) || (bits != 4 && bits != 8) || rows < 0 || rows > MAX_ROWS)
-    return 0;
-  if (most_tiles(num_sequences, kv_heads, rows) > 0x7fffffffll) return 0;
+    return -1;
+  if (most_tiles(num_sequences, kv_heads, rows) > 0x7fffffffll) return -1;
   return workspace_bytes(cut_of(num_sequences, kv_heads, q_heads / kv_heads, head_dim, bits, rows), q_heads / kv_heads, head_dim);
 }
 
@@ -209,23 +209,22 @@ extern "C" int qmk_attention_packed_cache(const qmk_packed_cache *cache, const q
   qmk_internal::begin_call();
   AttendParams p;
   if (const char *why = read_cache(cache, &p.caches)) return refuse(who, why);
-  if (!a || !a->q || !a->out || !a->lens || !a->workspace) return refuse(who, "null pointer argument");
+  if (!a || !a->q || !a->out || !a->lens) return refuse(who, "null pointer argument");
   if (a->type < 0 || a->type > 1) return refuse(who, "the type is fp16 (0) or bf16 (1)");
   if (a->q_heads < 1 || a->q_heads % cache->kv_heads || a->q_heads / cache->kv_heads > MAX_GROUP) return refuse(who, "q_heads must be 1 to 16 times kv_heads");
   if (most_tiles(cache->num_sequences, cache->kv_heads, cache->rows) > 0x7fffffffll) return refuse(who, "2^36 rows of all heads or more");
   if (!(a->scale > -2.0e38f && a->scale < 2.0e38f)) return refuse(who, "the scale must be finite, and below 2e38");   // (times log2 e too)
   if (odd(a->q) || odd(a->out) || odd(a->workspace)) return refuse(who, "pointers must be 16-byte aligned");
   if (odd(a->q_seq_stride, cache->num_sequences, 8) || odd(a->q_head_stride, a->q_heads, 8)) return refuse(who, "the queries' strides must be multiples of 8 elements");
-  if (a->workspace_bytes < qmk_attention_packed_cache_workspace(cache->num_sequences, a->q_heads, cache->kv_heads, cache->head_dim, cache->bits, cache->rows))
-    return refuse(who, "workspace too small");
+  p.group = a->q_heads / cache->kv_heads;
+  const Cut cut = cut_of(cache->num_sequences, cache->kv_heads, p.group, cache->head_dim, cache->bits, cache->rows);
+  if (cut.warps > 0 && (!a->workspace || a->workspace_bytes < workspace_bytes(cut, p.group, cache->head_dim))) return refuse(who, "workspace too small");
   p.q = a->q;
   p.q_seq = a->q_seq_stride;
   p.q_head = a->q_head_stride;
   p.q_heads = a->q_heads;
-  p.group = a->q_heads / cache->kv_heads;
   p.lens = a->lens;
   p.scale_log2 = a->scale * LOG2E;
-  const Cut cut = cut_of(cache->num_sequences, cache->kv_heads, p.group, cache->head_dim, cache->bits, cache->rows);
   p.ranks = cut.ranks;
   p.warps = cut.warps;
   p.part_out = static_cast<float *>(a->workspace);

@@ -892,8 +892,7 @@ def _per_sequence(who, value, n, index, name):
     """Device pointer of an int32 tensor with a value per sequence; 0 for None."""
     if value is None:
         return 0
-    if not (isinstance(value, torch.Tensor) and value.dtype is _INT32 and value.is_cuda and value.get_device() == index and value.dim() == 1 and value.shape[0] == n
-            and value.is_contiguous()):
+    if not (isinstance(value, torch.Tensor) and value.dtype is _INT32 and value.get_device() == index and value.shape == (n,) and value.is_contiguous()):
         raise RuntimeError(f"{who}: {name} must be a contiguous int32 tensor with one value per sequence on the caches' device")
     return value.data_ptr()
 
@@ -995,9 +994,9 @@ def attention_packed_cache(q: torch.Tensor, k_cache, v_cache, lens: torch.Tensor
     out = torch.empty_like(q) if q.is_contiguous() else torch.empty(n, q_heads, dim, dtype=dtype, device=q.device)
     lse = torch.empty(n, q_heads, dtype=_FP32, device=q.device)
     need = _packed_attention_workspace(n, q_heads, heads, dim, bits, rows)
-    workspace = lens.new_empty(need >> 2)
+    workspace = lens.new_empty(need >> 2) if need else None
     args = _pack_packed_attention(code, q_heads, q.data_ptr(), strides[0], strides[1], seen, dim ** -0.5 if scale is None else scale, out.data_ptr(), lse.data_ptr(),
-                                  workspace.data_ptr(), need)
+                                  workspace.data_ptr() if need else 0, need)
     rc = _on_device(index, _lib.qmk_attention_packed_cache, cache, args)
     if rc != 0:
         raise RuntimeError(f"{who}: {_lib.qmk_last_error().decode()} (status {rc})")
@@ -1006,8 +1005,8 @@ def attention_packed_cache(q: torch.Tensor, k_cache, v_cache, lens: torch.Tensor
 
 @functools.lru_cache(maxsize=256)
 def _packed_attention_workspace(*sizes):
-    """Bytes of workspace for these sizes (``qmk_attention_packed_cache_workspace``, at least a few)."""
-    return (max(int(_lib.qmk_attention_packed_cache_workspace(*sizes)), 256) + 3) // 4 * 4
+    """Bytes of workspace for these sizes (``qmk_attention_packed_cache_workspace``; 0 for sizes that the call refuses too)."""
+    return max(int(_lib.qmk_attention_packed_cache_workspace(*sizes)), 0)
 
 
 def sync_status() -> int:

@@ -184,12 +184,18 @@ def test_more_rows_than_an_index_holds_are_refused(C):
 
 
 @pytest.mark.parametrize("change,text", [(dict(type=2), b"type"), (dict(q_heads=12), b"q_heads"), (dict(q_heads=0), b"q_heads"), (dict(q_heads=136), b"q_heads"), (dict(q=None), b"null"),
-                                         (dict(out=None), b"null"), (dict(lens=None), b"null"), (dict(workspace=None), b"null"), (dict(workspace_bytes=4), b"workspace"),
+                                         (dict(out=None), b"null"), (dict(lens=None), b"null"),
                                          (dict(scale=float("inf")), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(scale=3e38), b"scale"), (dict(q=4104), b"aligned"),
                                          (dict(out=4104), b"aligned"), (dict(workspace=4104), b"aligned"), (dict(q_seq_stride=2052), b"strides"), (dict(q_head_stride=4), b"strides")])
 def test_attention_is_refused_before_anything_runs(C, change, text):
     rc, why = call(C, "qmk_attention_packed_cache", cache_args(C), attention_args(C, **change))
     assert rc == 2 and text in why, why
+
+
+@pytest.mark.parametrize("change", [dict(workspace=None), dict(workspace_bytes=4), dict(workspace_bytes=-1)])
+def test_a_workspace_that_is_needed_and_not_there_is_refused(C, change):
+    rc, why = call(C, "qmk_attention_packed_cache", cache_args(C, rows=100000, head_stride=8000000), attention_args(C, **change))
+    assert rc == 2 and b"workspace" in why
 
 
 def test_null_arguments_are_refused(C):
@@ -200,12 +206,12 @@ def test_null_arguments_are_refused(C):
         assert rc == 2 and b"null" in why
 
 
-def test_workspace_is_0_for_sizes_that_are_refused(C):
+def test_no_workspace_for_sizes_that_are_refused(C):
     size = C._lib.qmk_attention_packed_cache_workspace
-    assert size(1, 16, 8, 128, 4, 100) > 0
+    assert size(1, 16, 8, 128, 4, 100) == 0 and size(1, 16, 8, 128, 4, 100000) > 0
     for bad in ((0, 16, 8, 128, 4, 100), (129, 16, 8, 128, 4, 100), (1, 12, 8, 128, 4, 100), (1, 136, 8, 128, 4, 100), (1, 16, 0, 128, 4, 100), (1, 16, 8, 96, 4, 100),
                 (1, 16, 8, 128, 5, 100), (1, 16, 8, 128, 4, -1), (1, 16, 8, 128, 4, (1 << 24) + 1)):
-        assert size(*bad) == 0
+        assert size(*bad) == -1
 
 
 def test_packed_row_bytes(C):
