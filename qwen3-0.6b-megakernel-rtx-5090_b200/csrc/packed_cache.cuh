@@ -31,8 +31,23 @@ struct Caches {
   long long head, row;
   const unsigned char *k[MAX_SEQS], *v[MAX_SEQS];
 };
+// Division of numbers below 2^31 by one that the host knows: with l the bits of d - 1 and m = ceil(2^(31 + l) / d), n m >> 31 + l is n / d, since m d exceeds the power by
+// less than 2^l.
+struct Divisor {
+  unsigned int d, m;
+  int shift;
+  __host__ void set(unsigned int by) {
+    int l = 0;
+    while (l < 31 && (1u << l) < by) ++l;
+    d = by;
+    m = by > 1 ? static_cast<unsigned int>(((1ull << (31 + l)) + by - 1) / by) : 0;
+    shift = l - 1;
+  }
+  __device__ __forceinline__ unsigned int of(unsigned int n) const { return d > 1 ? __umulhi(n, m) >> shift : n; }
+};
 struct RowParams {
   Caches caches;
+  Divisor by_rows, by_heads;
   void *k, *v;                                   // the rows: strides in elements
   long long seq, head, row;
   int rows;                                      // of a sequence, in the call
@@ -71,9 +86,9 @@ struct RowOfCall {
 };
 __device__ __forceinline__ RowOfCall row_of(const RowParams &p, unsigned int i) {
   RowOfCall r;
-  const unsigned int pair = i / static_cast<unsigned int>(p.rows);
+  const unsigned int pair = p.by_rows.of(i);
   r.t = static_cast<int>(i - pair * p.rows);
-  r.b = static_cast<int>(pair / static_cast<unsigned int>(p.caches.kv_heads));
+  r.b = static_cast<int>(p.by_heads.of(pair));
   r.head = static_cast<int>(pair - r.b * static_cast<unsigned int>(p.caches.kv_heads));
   const long long at = static_cast<long long>(p.starts ? p.starts[r.b] : p.start) + r.t;
   r.there = r.t < (p.lens ? p.lens[r.b] : p.rows) && at >= 0 && at < p.caches.rows;
@@ -205,20 +220,19 @@ __device__ __forceinline__ void load_values(const void *src, int t, uint32_t (&x
   }
 }
 
+// Keys by the blocks of blockIdx.y 0, values by the others.
 template <typename T, int DIM, int BITS>
-__global__ void __launch_bounds__(THREADS) write_rows(const __grid_constant__ RowParams p, unsigned int count) {
+__global__ void __launch_bounds__(THREADS, 4) write_rows(const __grid_constant__ RowParams p, unsigned int count) {
   const int lane = threadIdx.x & 31, t = lane & 3;
+  const T *const values = static_cast<const T *>(blockIdx.y ? p.v : p.k);
   for (unsigned int first = blockIdx.x * (THREADS / 4); first < count; first += gridDim.x * (THREADS / 4)) {
     const unsigned int i = first + (threadIdx.x >> 2);
     const RowOfCall r = row_of(p, i < count ? i : count - 1);
-    const bool there = r.there && i < count;
-    const long long from = r.b * p.seq + r.head * p.head + r.t * p.row, to = r.head * p.caches.head + r.at * p.caches.row;
-    uint32_t k[4][DIM / 32], v[4][DIM / 32];
+    uint32_t x[4][DIM / 32];
     // (rows that go nowhere too: they are there, and starts and lengths need not be waited for)
-    load_values<DIM>(static_cast<const T *>(p.k) + from, t, k);
-    load_values<DIM>(static_cast<const T *>(p.v) + from, t, v);
-    pack_row<T, DIM, BITS>(k, const_cast<unsigned char *>(p.caches.k[r.b]) + to, lane, there);
-    pack_row<T, DIM, BITS>(v, const_cast<unsigned char *>(p.caches.v[r.b]) + to, lane, there);
+    load_values<DIM>(values + r.b * p.seq + r.head * p.head + r.t * p.row, t, x);
+    unsigned char *const cache = const_cast<unsigned char *>(blockIdx.y ? p.caches.v[r.b] : p.caches.k[r.b]);
+    pack_row<T, DIM, BITS>(x, cache + (r.head * p.caches.head + r.at * p.caches.row), lane, r.there && i < count);
   }
 }
 

@@ -92,9 +92,11 @@ int rows_call(const char *who, const qmk_packed_cache *cache, const qmk_packed_r
   if (const char *why = read_rows_of(rows, &p)) return refuse(who, why);
   const unsigned int count = static_cast<unsigned int>(p.caches.seqs) * p.caches.kv_heads * p.rows;
   if (count == 0) return QMK_OK;
+  p.by_rows.set(p.rows);
+  p.by_heads.set(p.caches.kv_heads);
   const unsigned int rows_of_block = THREADS / (write ? 4 : 8), blocks = std::min((count + rows_of_block - 1) / rows_of_block, 148u * 16);
   void (*const kernel)(RowParams, unsigned int) = rows->type == 0 ? row_kernel<__half>(write, cache->head_dim, cache->bits) : row_kernel<__nv_bfloat16>(write, cache->head_dim, cache->bits);
-  kernel<<<blocks, THREADS, 0, stream>>>(p, count);
+  kernel<<<dim3(blocks, write ? 2 : 1), THREADS, 0, stream>>>(p, count);
   return answer(who, cudaGetLastError());
 }
 
