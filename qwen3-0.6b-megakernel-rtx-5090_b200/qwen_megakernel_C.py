@@ -713,6 +713,7 @@ def gemm_packed_tn(a: torch.Tensor, b: torch.Tensor, weight_format, b2: torch.Te
 # The operators below are called once per layer or step: their checks are plain expressions, and the stream is asked for without an
 # object around it (a call's host time 25 -> 12 us for a row of logits, of which the launch is 5).
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device      # (where there are tensors on a device, it is set up)
 _LOGIT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _FP32, _INT32, _UINT8 = torch.float32, torch.int32, torch.uint8
 _ROW_TYPES = {torch.float16: 0, torch.bfloat16: 1}
@@ -720,7 +721,7 @@ _ROW_TYPES = {torch.float16: 0, torch.bfloat16: 1}
 
 def _on_device(index: int, call, *args):
     """``call(*args, stream)`` with the device current and its current stream."""
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         return call(*args, _raw_stream(index))
     with torch.cuda.device(index):
         return call(*args, _raw_stream(index))
@@ -914,13 +915,14 @@ def write_cache_packed(k: torch.Tensor, v: torch.Tensor, k_cache, v_cache, start
     others of the caches stay as they are; two rows of a call must not fall on one.  The format and its rounding: ``qmk_packed_cache`` in include/qwen_megakernel.h.  Runs
     on the current stream of the tensors' device, does not synchronise, may be captured in a graph."""
     who = "write_cache_packed"
-    code = _ROW_TYPES.get(k.dtype, -1)
-    if code < 0 or not k.is_cuda or k.dim() != 4 or k.stride(3) != 1:
+    dtype, shape, strides = k.dtype, k.shape, k.stride()
+    code = _ROW_TYPES.get(dtype, -1)
+    if code < 0 or not k.is_cuda or len(strides) != 4 or strides[3] != 1:
         _require_cuda()
         raise RuntimeError(f"{who}: k must be a CUDA tensor [n, kv_heads, rows, dim] of fp16 or bf16, contiguous along dim")
-    index, strides = k.get_device(), k.stride()
-    n, heads, rows, dim = k.shape
-    if not (v.shape == k.shape and v.dtype is k.dtype and v.get_device() == index and v.stride() == strides):
+    index = k.get_device()
+    n, heads, rows, dim = shape
+    if not (v.shape == shape and v.dtype is dtype and v.get_device() == index and v.stride() == strides):
         raise RuntimeError(f"{who}: v must be like k, with the same strides")
     cache, n, cache_heads, _, _, keep = _packed_cache(who, k_cache, v_cache, n, dim, index)
     if heads != cache_heads:
