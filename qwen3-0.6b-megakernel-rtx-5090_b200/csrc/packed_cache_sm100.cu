@@ -94,7 +94,8 @@ int rows_call(const char *who, const qmk_packed_cache *cache, const qmk_packed_r
   if (count == 0) return QMK_OK;
   p.by_rows.set(p.rows);
   p.by_heads.set(p.caches.kv_heads);
-  const unsigned int rows_of_block = THREADS / (write ? 4 : 8), blocks = std::min((count + rows_of_block - 1) / rows_of_block, 148u * 16);
+  // (CTAs: 4 x 4096 rows of 8 heads written by four an SM for keys and four for values 20.6 us, by eight 20.8, by sixteen 21.9; 28 x 4096 read by 64 an SM 104, by sixteen 109, by eight 124)
+  const unsigned int rows_of_block = THREADS / (write ? 4 : 8), blocks = std::min((count + rows_of_block - 1) / rows_of_block, 148u * (write ? 4 : 64));
   void (*const kernel)(RowParams, unsigned int) = rows->type == 0 ? row_kernel<__half>(write, cache->head_dim, cache->bits) : row_kernel<__nv_bfloat16>(write, cache->head_dim, cache->bits);
   kernel<<<dim3(blocks, write ? 2 : 1), THREADS, 0, stream>>>(p, count);
   return answer(who, cudaGetLastError());
