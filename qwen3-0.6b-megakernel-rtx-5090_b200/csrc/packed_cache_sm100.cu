@@ -105,7 +105,7 @@ int rows_call(const char *who, const qmk_packed_cache *cache, const qmk_packed_r
 // as are resident together.  Else a warp takes a stretch of the line of tiles, all resident together, not more of them than there can be tiles, and a
 // second launch joins.  Stretches against clusters, us a call in a graph, 128 dims, 4 bits, 16 query heads on 8, lengths from 0 up: one sequence of 128 rows 6.0 and 4.7; 16 of
 // up to 2048 (4 tiles a warp) 14.0 and 12.1; 128 of up to 1024 (8 tiles, seven CTAs an SM one after the other) 30.4 and 27.3; 16 of up to 4096 (8) 18.2 and 17.4, of up to 8192 (16) 25.4
-// and 27.5 (a cluster has a longest item to wait for, a stretch has not); one of 8192 (8) 12.0 and 9.7, of 32,768 (32) 19.8 and 27.2.  On the host 16 and 13.
+// and 27.5 (a cluster has a longest item to wait for, a stretch has not); one of 8192 (8) 12.0 and 9.7, of 32,768 (32) 19.8 and 27.2.  On the host 16 and 11.
 // Clusters of 16 CTAs start late: one sequence of 2048 rows 15.5, of eight 5.7.
 constexpr int ITEM_TILES = 8, ITEM_WAVES = 4;
 struct Cut {
