@@ -4,7 +4,8 @@
 //   q . k = sum_b s_b (sum_{d in b} q_d n_d - M Q_b) + sum_b z_b Q_b,   Q_b = sum_{d in b} q_d,
 //   out_d = sum_r p_r z_{r,b(d)} + sum_r (p_r s_{r,b(d)}) n_{r,d} - M sum_r (p_r s_{r,b(d)}),
 // so codes enter the products as they are: the number n 2^-24 is the fp16 pattern n, and masking some bits of both halves of a word makes two operands.  Rows
-// of the cache are the 16 rows of an mma.sync tile, query heads its eight columns (tcgen05's 128 rows of queries are not there: a kv head has one to sixteen); a row's trailer, 16 bytes,
+// of the cache are the 16 rows of an mma.sync tile, query heads its eight columns (tcgen05's 128 rows of queries are not there: a kv head has one to sixteen); a row's
+// trailer, 16 bytes,
 // is a row of an 8 x 8 tile, so ldmatrix makes the operands of the sums over centres.
 //
 // Roundings: queries are taken to fp16 times a power of two, which leaves them as they are but for entries below 2^-26 of the largest.  Weights are carried
@@ -16,7 +17,7 @@
 // Work: tiles of 32 rows, a tile to a warp, each with a ring of copies of its own (cp.async: no waits but for its own copies).  attend_items: a cluster of CTAs has a (sequence, kv
 // head) and joins its states - the maximum, the sum and the unnormalised output - in shared memory.  attend_tiles: the tiles of all items in one line, of which
 // each warp takes an equal stretch, whatever the sequences' lengths; a stretch that holds a whole item writes its output, parts of items leave their states in the workspace,
-// and a second launch joins them.
+// and a second launch joins them.  Of few long items each is shared by many clusters of attend_items, which leave a state each.
 //
 // Measured, caches cold: 96 sequences of 8192 rows, two heads on each of eight kv heads, 4 bits: 160 to 164 us in all, 6.2 TB/s, 0.95 of the copy rate; bound by HBM, with 250 warp
 // instructions for 16 rows.  32 of 8192 rows (336 MB), us of attend_tiles alone with 2 / 4 / 8 / 16 query heads a kv head: 63 / 69 / 76 / 114: bound by the issue of
@@ -53,8 +54,9 @@ struct AttendParams {
   const int *lens;
   float scale_log2;                              // scale * log2 e
   int ranks;                                     // where items have clusters of their own: log2 of the CTAs that share one, + 1; else 0
-  int warps;                                     // of the launch
-  float *part_out;                               // [2 warps][group][DIM]
+  int splits;                                    // the clusters of an item, at most
+  int warps;                                     // parts that are left for a second launch, at most: of warps, or of clusters (0: none)
+  float *part_out;                               // [2 warps][group][DIM], every second one unused where clusters make them
   float2 *part_ml;                               // [2 warps][group]
   void *out;                                     // [seq][q_head][DIM]
   float *lse;
@@ -1125,7 +1127,7 @@ __device__ __forceinline__ void zero_heads(const AttendParams &p, int dim, int b
   for (int i = lane; p.lse && i < n; i += 32) p.lse[row + i] = -INFINITY;
 }
 // Short items, one launch: a cluster of CTAs takes an item, each warp an equal part of its tiles; the states stay in shared memory, where all of the cluster
-// can read them, and its warps join them.
+// can read them, and its warps join them.  Long items, few: `splits` clusters each have an equal part of one (as many as it has tiles, if that is fewer).
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -1144,13 +1146,14 @@ template <int E> __device__ __forceinline__ void ld_cluster(uint32_t at, float (
   if constexpr (E == 4) asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(at) : "memory");
   else asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(at) : "memory");
 }
-// An item's parts: a warp each of 2^shift CTAs, part w warp w >> shift of CTA w & 2^shift - 1 (few tiles: in different CTAs), its first tile.  (Items have few tiles.)
+// A cluster's parts: a warp each of 2^shift CTAs, part w warp w >> shift of CTA w & 2^shift - 1 (few tiles: in different CTAs), its first tile.  (A cluster has at most 2^19 / 8.)
 __device__ __forceinline__ int begin_of_part(int tiles, int shift, int w) { return tiles * w >> (shift + 2); }
-static_assert(WARPS == 4, "a CTA has four of an item's parts");
-// The states of an item's parts, at most 32, joined by warps `mine` and so on.  Unit: DIM / GROUPS dimensions of a query head; groups of lanes take every
+static_assert(WARPS == 4, "a CTA has four of a cluster's parts");
+// The states of a cluster's parts, at most 32, joined by warps `mine` and so on; `part`: where the joined state goes, -1 for the output of a whole item.  Unit: DIM /
+// GROUPS dimensions of a query head; groups of lanes take every
 // GROUPS-th part, eight or four at a time.
 template <typename A, int GROUPS>
-__device__ __forceinline__ void join_cluster(const AttendParams &p, const Place &item, int shift, unsigned char *smem, int mine, int lane) {
+__device__ __forceinline__ void join_cluster(const AttendParams &p, const Place &item, int part, int shift, unsigned char *smem, int mine, int lane) {
   using T = typename A::Value;
   constexpr int DIM = A::HEAD_DIM, UNIT_DIMS = DIM / GROUPS, LANES = 32 / GROUPS, E = UNIT_DIMS / LANES, EACH = GROUPS == 1 ? 8 : 4;      // dimensions of a lane
   const int parts = WARPS << shift, group = lane / LANES;
@@ -1194,6 +1197,12 @@ __device__ __forceinline__ void join_cluster(const AttendParams &p, const Place 
     for (int k = 0; k < E; ++k)
 #pragma unroll
       for (int o = LANES; o < 32; o <<= 1) out[k] += __shfl_xor_sync(0xffffffffu, out[k], o);
+    if (part >= 0) {
+      const size_t at = 2ull * part * p.group + h;
+      if (lane < LANES) store_part<32 * E>(p.part_out + at * DIM + d, out);
+      if (lane == 0 && u % GROUPS == 0) p.part_ml[at] = make_float2(top, total);
+      continue;
+    }
     const size_t row = static_cast<size_t>(item.b) * p.q_heads + item.head * p.group + h;
     if (lane < LANES) store_out<T, 32 * E>(static_cast<T *>(p.out) + row * DIM + d, out, total == 0.0f ? 0.0f : 1.0f / total);
     if (lane == 0 && u % GROUPS == 0 && p.lse) p.lse[row] = total == 0.0f ? -INFINITY : top * LN2 + logf(total);
@@ -1207,17 +1216,20 @@ __global__ void __launch_bounds__(WARPS * 32, A::CTAS) attend_items(const __grid
   pdl_wait();
   pdl_trigger();
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, rank = cluster_rank();
-  const int shift = p.ranks - 1, item = static_cast<int>(blockIdx.x) >> shift;
+  const int shift = p.ranks - 1, cluster = static_cast<int>(blockIdx.x) >> shift, item = cluster / p.splits, split = cluster - item * p.splits;
   Place now;
   now.b = item / p.caches.kv_heads;
   now.head = item - now.b * p.caches.kv_heads;
   now.rows = seen_rows(p, now.b);
   now.tiles = tiles_of(now.rows);
   if (now.tiles == 0) {                          // (all of the cluster)
-    if (rank == 0 && warp == 0) zero_heads<T>(p, DIM, now.b, now.head * p.group, p.group, lane);
+    if (split == 0 && rank == 0 && warp == 0) zero_heads<T>(p, DIM, now.b, now.head * p.group, p.group, lane);
     return;
   }
-  const int mine = (warp << shift) + rank, first = begin_of_part(now.tiles, shift, mine), last = begin_of_part(now.tiles, shift, mine + 1);
+  const int splits = min(p.splits, now.tiles), begin = begin_of(now.tiles, splits, split);
+  if (split >= splits) return;                   // (all of the cluster)
+  now.tiles = begin_of(now.tiles, splits, split + 1) - begin;               // the cluster's
+  const int mine = (warp << shift) + rank, first = begin + begin_of_part(now.tiles, shift, mine), last = begin + begin_of_part(now.tiles, shift, mine + 1);
   unsigned char *const own = smem + warp * A::WARP_SMEM;
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(own));
   if (first < last) {
@@ -1251,10 +1263,11 @@ __global__ void __launch_bounds__(WARPS * 32, A::CTAS) attend_items(const __grid
     a.end(p, now.b, now.head, state, reinterpret_cast<float2 *>(state + p.group * DIM), lane);
   }
   cluster_sync();
+  const int part = splits > 1 ? cluster : -1;    // (one: the whole item)
   // whole heads where there are few parts, or heads enough for the warps; else eighths.  (One CTA, two heads: 128 rows 5.6 us, with eighths 8.7; four CTAs, eight heads:
   // 12.8 and 13.0; eight CTAs, two heads, 1024 rows: 10.8 and 7.2.)
-  if (shift < 2 || 2 * p.group >= (WARPS << shift)) join_cluster<A, 1>(p, now, shift, smem, mine, lane);
-  else join_cluster<A, 8>(p, now, shift, smem, mine, lane);
+  if (shift < 2 || 2 * p.group >= (WARPS << shift)) join_cluster<A, 1>(p, now, part, shift, smem, mine, lane);
+  else join_cluster<A, 8>(p, now, part, shift, smem, mine, lane);
   cluster_sync();                                // (nobody leaves while its states are read)
 }
 
@@ -1347,16 +1360,25 @@ __global__ void __launch_bounds__(32 * W) join_many(const __grid_constant__ Atte
   __shared__ float sm[W], sl[W];
   __shared__ __align__(16) float sa[W][DIM];
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, row = blockIdx.x, b = row / p.q_heads, head = row - b * p.q_heads;
-  make_line(p, line, sums);
-  __syncthreads();
-  const int parts = min(p.warps, line.total), tiles = tiles_of(line.rows[b]);
-  if (tiles == 0) {
-    pdl_wait();
-    if (head == 0 && warp == 0) zero_empty<T>(p, line, DIM, b, MAX_SEQS, lane);
-    return;
+  int r0, r1;
+  bool inside = false;
+  if (p.ranks > 0) {                             // (clusters' parts)
+    const int item = b * p.caches.kv_heads + head / p.group, splits = min(p.splits, tiles_of(seen_rows(p, b)));
+    r0 = item * p.splits;
+    r1 = r0 + max(splits, 1) - 1;
+  } else {
+    make_line(p, line, sums);
+    __syncthreads();
+    const int parts = min(p.warps, line.total), tiles = tiles_of(line.rows[b]);
+    if (tiles == 0) {
+      pdl_wait();
+      if (head == 0 && warp == 0) zero_empty<T>(p, line, DIM, b, MAX_SEQS, lane);
+      return;
+    }
+    const int t0 = line.before[b] + head / p.group * tiles;
+    r0 = part_of(line.total, parts, t0), r1 = part_of(line.total, parts, t0 + tiles - 1);
+    inside = begin_of(line.total, parts, r0) < t0;
   }
-  const int t0 = line.before[b] + head / p.group * tiles, r0 = part_of(line.total, parts, t0), r1 = part_of(line.total, parts, t0 + tiles - 1);
-  const bool inside = begin_of(line.total, parts, r0) < t0;
   pdl_wait();
   if (r0 == r1) return;                          // (written there)
   Joined<DIM, AHEAD> j;

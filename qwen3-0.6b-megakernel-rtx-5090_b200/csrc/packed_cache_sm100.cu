@@ -102,31 +102,40 @@ int rows_call(const char *who, const qmk_packed_cache *cache, const qmk_packed_r
 }
 
 // How a call is cut.  Where no warp gets more than ITEM_TILES tiles of caches that are full, a cluster of CTAs takes an item, one launch; up to ITEM_WAVES times as many items
-// as are resident together.  Else a warp takes a stretch of the line of tiles, all resident together, not more of them than there can be tiles, and a
-// second launch joins.  Stretches against clusters, us a call in a graph, 128 dims, 4 bits, 16 query heads on 8, lengths from 0 up: one sequence of 128 rows 6.0 and 4.7; 16 of
-// up to 2048 (4 tiles a warp) 14.0 and 12.1; 128 of up to 1024 (8 tiles, seven CTAs an SM one after the other) 30.4 and 27.3; 16 of up to 4096 (8) 18.2 and 17.4, of up to 8192 (16) 25.4
+// as are resident together.  Else, of few sequences, as many clusters of two CTAs as are resident together share an item, and a second launch joins what theirs have joined; of more
+// sequences a warp takes a stretch of the line of tiles, all resident together, not more of them than there can be tiles, and a second launch joins.  Stretches against
+// clusters, us a call in a graph, 128 dims, 4 bits, 16 query heads on 8, lengths from 0 up: one sequence of 128 rows 6.0 and 4.7; 16 of
+// up to 2048 (4 tiles a warp) 14.0 and 12.1; 128 of up to 1024 (8 tiles, seven CTAs an SM one after the other) 30.4 and 27.3; 16 of up to 4096 (8) 18.2 and 17.4, of up
+// to 8192 (16) 25.4
 // and 27.5 (a cluster has a longest item to wait for, a stretch has not); one of 8192 (8) 12.0 and 9.7, of 32,768 (32) 19.8 and 27.2.  On the host 16 and 11.
 // Clusters of 16 CTAs start late: one sequence of 2048 rows 15.5, of eight 5.7.
+// Stretches against pairs that share: one sequence of 16,384 rows 15.5 and 12.8, of 32,768 19.0 and 16.1 (16 query heads on 2 21.6 and 18.8), of 131,072 38.0 and 34.8;
+// four of up to 16,384 18.5 and
+// 16.7, all full 23.5 and 22.0; eight of up to 32,768 38 and 44.  Sharing by single CTAs 17.6 where pairs take 16.4, by four or eight 19.5; one of 8192 by pairs 11.2, by
+// one cluster of eight 10.6.
 constexpr int ITEM_TILES = 8, ITEM_WAVES = 4;
+constexpr int SHARING_SEQS = 4, SHARING_PAIRS = 8;                          // sequences at most, pairs of an item at least (fewer leave many places of the device empty)
 struct Cut {
-  int ranks, warps;
+  int ranks, splits, warps;
 };
 long long most_tiles(int seqs, int kv_heads, int rows) { return static_cast<long long>(seqs) * kv_heads * ((rows + TILE - 1) / TILE); }
 Cut cut_of(int seqs, int kv_heads, int group, int dim, int bits, int rows) {
   const int ctas = SMS * ctas_per_sm(way_of(group), dim, bits), tiles = (rows + TILE - 1) / TILE, items = seqs * kv_heads;
   int ranks = 1;                                 // log2 of a cluster's CTAs, + 1
   while (ranks < MAX_RANKS && (items << ranks) <= ctas && (WARPS << (ranks - 1)) < tiles) ++ranks;
-  if (items <= ITEM_WAVES * ctas && tiles <= ITEM_TILES * (WARPS << (ranks - 1))) return Cut{ranks, 0};
-  return Cut{0, static_cast<int>(std::min<long long>(std::max(most_tiles(seqs, kv_heads, rows), 1ll), ctas * WARPS))};
+  if (items <= ITEM_WAVES * ctas && tiles <= ITEM_TILES * (WARPS << (ranks - 1))) return Cut{ranks, 1, 0};
+  const int pairs = ctas / 2 / items;
+  if (seqs <= SHARING_SEQS && pairs >= SHARING_PAIRS) return Cut{2, pairs, items * pairs};
+  return Cut{0, 1, static_cast<int>(std::min<long long>(std::max(most_tiles(seqs, kv_heads, rows), 1ll), ctas * WARPS))};
 }
 long long workspace_bytes(const Cut &cut, int group, int dim) { return 2ll * cut.warps * group * (dim * 4ll + 8); }
 
-// How the parts are joined goes by how many an item has where all stretches are used: warps, or CTAs of four, eight or 32 warps.
+// How the parts are joined goes by how many an item has where all stretches or pairs are used: warps (of stretches), or CTAs of four, eight or 32 warps.
 template <typename T, int DIM>
 cudaError_t launch_join(const AttendParams &p, cudaStream_t stream) {
   const qmk_tc::PdlScope scope(true);
   const int rows = p.caches.seqs * p.q_heads, each = p.warps / (p.caches.seqs * p.caches.kv_heads);
-  if (each <= FEW) {
+  if (each <= FEW && p.ranks == 0) {
     const int units = std::max(p.warps * p.group, p.caches.seqs);
     return qmk_tc::launch_kernel(join_few<T, DIM>, dim3(std::min((units + 7) / 8, 8 * SMS)), dim3(256), 0, stream, p);
   }
@@ -157,7 +166,7 @@ cudaError_t launch_tiles(const AttendParams &p, cudaStream_t stream) {
   const cudaError_t e = allow(items_known, attend_items<A>, A::SMEM);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((p.caches.seqs * p.caches.kv_heads) << (p.ranks - 1));
+  cfg.gridDim = dim3((p.caches.seqs * p.caches.kv_heads * p.splits) << (p.ranks - 1));
   cfg.blockDim = dim3(WARPS * 32);
   cfg.dynamicSmemBytes = A::SMEM;
   cfg.stream = stream;
@@ -182,7 +191,7 @@ cudaError_t attend(const AttendParams &p, cudaStream_t stream) {
       case TWO: e = launch_tiles<Attend<T, DIM, BITS, 2>>(p, stream); break;
     }
   }
-  return e != cudaSuccess || p.ranks > 0 ? e : launch_join<T, DIM>(p, stream);
+  return e != cudaSuccess || p.warps == 0 ? e : launch_join<T, DIM>(p, stream);
 }
 template <typename T>
 cudaError_t attend(const AttendParams &p, int dim, int bits, cudaStream_t stream) {
@@ -229,6 +238,7 @@ extern "C" int qmk_attention_packed_cache(const qmk_packed_cache *cache, const q
   p.lens = a->lens;
   p.scale_log2 = a->scale * LOG2E;
   p.ranks = cut.ranks;
+  p.splits = cut.splits;
   p.warps = cut.warps;
   p.part_out = static_cast<float *>(a->workspace);
   p.part_ml = reinterpret_cast<float2 *>(p.part_out + 2ll * p.warps * p.group * cache->head_dim);

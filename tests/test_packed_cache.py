@@ -396,6 +396,51 @@ def test_full_batches_with_room_to_spare(gpu, q_heads, kv_heads, dim, bits):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("q_heads,kv_heads,dim,bits,dtype", [(2, 2, 128, 4, "fp16"), (4, 2, 128, 8, "bf16"), (16, 2, 64, 4, "fp16"), (16, 4, 128, 4, "bf16"), (5, 1, 128, 8, "fp16"), (16, 1, 64, 8, "fp16"), (4, 4, 64, 8, "fp16")])
+def test_few_long_sequences(gpu, q_heads, kv_heads, dim, bits, dtype):
+    """Clusters take parts of a sequence: lengths of no row, of fewer tiles than there are clusters, of one more than all tiles alike, of the whole cache."""
+    q, kc, vc = attention_inputs(4, q_heads, kv_heads, dim, bits, 19000, dtype, seed=dim + q_heads)
+    for lens in ([19000, 1, 0, 9001], [33, 32, 700, 0], [2369, 8 * 37 * 32 + 1, 18999, 64]):
+        check_attention(gpu.attention_packed_cache(q, kc, vc, torch.tensor(lens, dtype=torch.int32).cuda()), q, kc, vc, lens)
+    for b, n in ((0, 19000), (2, 18977)):
+        check_attention(gpu.attention_packed_cache(q[b:b + 1], kc[b:b + 1], vc[b:b + 1], torch.tensor([n], dtype=torch.int32).cuda()), q[b:b + 1], kc[b:b + 1], vc[b:b + 1], [n])
+    room = (with_room(kc, 40000), with_room(vc, 40000))
+    lens = torch.zeros(4, dtype=torch.int32)
+    check_attention(gpu.attention_packed_cache(q, *room, lens.cuda()), q, *room, lens)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_heads,kv_heads,dim,bits", [(16, 8, 128, 4), (4, 2, 64, 8), (8, 2, 128, 8), (16, 2, 128, 4), (32, 2, 128, 8), (3, 1, 64, 4)])
+def test_each_way_a_call_is_cut(gpu, q_heads, kv_heads, dim, bits):
+    """The same rows in caches of their size, in long ones and in long ones of more sequences, then with a key and a value that are no numbers."""
+    q, kc, vc = attention_inputs(4, q_heads, kv_heads, dim, bits, 700)
+    lens = torch.tensor([0, 20, 700, 333], dtype=torch.int32)
+    which = torch.tensor([0, 1, 2, 3, 2, 3, 1])
+
+    def ways(kc, vc):
+        at = which.cuda()
+        long = with_room(kc, 20000), with_room(vc, 20000)
+        lists = [long[0][i] for i in which], [long[1][i] for i in which]
+        return [gpu.attention_packed_cache(q, kc, vc, lens.cuda()), gpu.attention_packed_cache(q, *long, lens.cuda()), gpu.attention_packed_cache(q[at], *lists, lens.cuda()[at])]
+
+    want = ways(kc, vc)
+    for got in want[:2]:
+        check_attention(got, q, kc, vc, lens)
+    check_attention(want[2], q[which.cuda()], [kc[i] for i in which], [vc[i] for i in which], lens[which])
+    none = torch.full((1, kv_heads, 1, dim), math.nan, dtype=torch.float16, device="cuda")
+    one = torch.ones_like(none)
+    kn, vn = kc.clone(), vc.clone()
+    gpu.write_cache_packed(none, one, kn[2:3], vn[2:3], 650)
+    gpu.write_cache_packed(one, none, kn[3:], vn[3:], 332)
+    gpu.write_cache_packed(none, none, kn[1:2], vn[1:2], 20)                   # (behind the last row)
+    for i, (out, lse) in enumerate(ways(kn, vn)):
+        seq = which if i == 2 else torch.arange(4)
+        bad_key, bad = (seq == 2).cuda(), ((seq == 2) | (seq == 3)).cuda()
+        assert torch.equal(lse.isnan(), bad_key[:, None].expand_as(lse)) and torch.equal(out.isnan(), bad[:, None, None].expand_as(out))
+        assert torch.equal(out[~bad], want[i][0][~bad]) and torch.equal(lse[~bad], want[i][1][~bad])
+
+
+@pytest.mark.gpu
 def test_no_rows_and_lengths_outside_the_cache(gpu):
     q, kc, vc = attention_inputs(4, 4, 2, 64, 4, 30)
     for lens in ([0, 0, 0, 0], [-5, 1000, 2 ** 31 - 1, -2 ** 31]):
@@ -656,8 +701,10 @@ def test_caches_further_apart_than_32_bits(gpu, bits):
     assert bool(((back[0].double().cpu() - exact).abs() <= rounded_off(exact, torch.float16)).all())
     lens = torch.tensor([10, 7], dtype=torch.int32)
     check_attention(gpu.attention_packed_cache(q, kc, vc, lens.cuda()), q, kc, vc, lens)
-    # the same with room for many rows: the line of tiles
+    # the same with room for many rows: clusters of a sequence, the line of tiles
     long = memory.as_strided((1, 2, 20000, size), (0, apart, size, 1))
     long[:, :, :9] = packed(k[:1], bits).cuda()
     lens = torch.tensor([9], dtype=torch.int32)
     check_attention(gpu.attention_packed_cache(q[:1], long, long, lens.cuda()), q[:1], long, long, lens)
+    long, lens = long.expand(40, -1, -1, -1), torch.tensor([9 - b % 4 for b in range(40)], dtype=torch.int32)
+    check_attention(gpu.attention_packed_cache(q[:1].expand(40, -1, -1), long, long, lens.cuda()), q[:1].expand(40, -1, -1), long, long, lens)
