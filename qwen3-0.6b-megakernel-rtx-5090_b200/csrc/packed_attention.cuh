@@ -1150,8 +1150,7 @@ template <int E> __device__ __forceinline__ void ld_cluster(uint32_t at, float (
 __device__ __forceinline__ int begin_of_part(int tiles, int shift, int w) { return tiles * w >> (shift + 2); }
 static_assert(WARPS == 4, "a CTA has four of a cluster's parts");
 // The states of a cluster's parts, at most 32, joined by warps `mine` and so on; `part`: where the joined state goes, -1 for the output of a whole item.  Unit: DIM /
-// GROUPS dimensions of a query head; groups of lanes take every
-// GROUPS-th part, eight or four at a time.
+// GROUPS dimensions of a query head; groups of lanes take every GROUPS-th part, eight or four at a time.
 template <typename A, int GROUPS>
 __device__ __forceinline__ void join_cluster(const AttendParams &p, const Place &item, int part, int shift, unsigned char *smem, int mine, int lane) {
   using T = typename A::Value;

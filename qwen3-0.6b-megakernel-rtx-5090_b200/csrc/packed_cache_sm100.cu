@@ -102,17 +102,14 @@ int rows_call(const char *who, const qmk_packed_cache *cache, const qmk_packed_r
 }
 
 // How a call is cut.  Where no warp gets more than ITEM_TILES tiles of caches that are full, a cluster of CTAs takes an item, one launch; up to ITEM_WAVES times as many items
-// as are resident together.  Else, of few sequences, as many clusters of two CTAs as are resident together share an item, and a second launch joins what theirs have joined; of more
-// sequences a warp takes a stretch of the line of tiles, all resident together, not more of them than there can be tiles, and a second launch joins.  Stretches against
-// clusters, us a call in a graph, 128 dims, 4 bits, 16 query heads on 8, lengths from 0 up: one sequence of 128 rows 6.0 and 4.7; 16 of
-// up to 2048 (4 tiles a warp) 14.0 and 12.1; 128 of up to 1024 (8 tiles, seven CTAs an SM one after the other) 30.4 and 27.3; 16 of up to 4096 (8) 18.2 and 17.4, of up
-// to 8192 (16) 25.4
-// and 27.5 (a cluster has a longest item to wait for, a stretch has not); one of 8192 (8) 12.0 and 9.7, of 32,768 (32) 19.8 and 27.2.  On the host 16 and 11.
-// Clusters of 16 CTAs start late: one sequence of 2048 rows 15.5, of eight 5.7.
-// Stretches against pairs that share: one sequence of 16,384 rows 15.5 and 12.8, of 32,768 19.0 and 16.1 (16 query heads on 2 21.6 and 18.8), of 131,072 38.0 and 34.8;
-// four of up to 16,384 18.5 and
-// 16.7, all full 23.5 and 22.0; eight of up to 32,768 38 and 44.  Sharing by single CTAs 17.6 where pairs take 16.4, by four or eight 19.5; one of 8192 by pairs 11.2, by
-// one cluster of eight 10.6.
+// as are resident together.  Else, of few sequences, as many clusters of two CTAs as are resident together share the items, and a second launch joins what they have
+// joined; of more sequences a warp takes a stretch of the line of tiles, all resident together, not more of them than there can be tiles, and a second launch joins.
+// Measured in a graph, us, 128 dims, 4 bits, 16 query heads on 8, lengths from 0 up (tiles a warp in brackets).  Stretches against a cluster an item: one sequence of 128 rows
+// 6.0 and 4.7; 16 of up to 2048 (4) 14.0 and 12.1; 128 of up to 1024 (8, seven CTAs an SM one after the other) 30.4 and 27.3; 16 of up to 4096 (8) 18.2 and 17.4, of up to 8192
+// (16) 25.4 and 27.5 (a cluster has a longest item to wait for, a stretch has not); one of 8192 (8) 12.0 and 9.7, of 32,768 (32) 19.8 and 27.2.  On the host 16 and 11.
+// Clusters of 16 CTAs start late: one sequence of 2048 rows 15.5, of eight 5.7.  Stretches against pairs that share: one sequence of 16,384 rows 15.5 and 12.8, of 32,768 19.0
+// and 16.1 (16 query heads on 2 21.6 and 18.8), of 131,072 38.0 and 34.8; four of up to 16,384 18.5 and 16.7, all full 23.5 and 22.0; eight of up to 32,768 38 and 44.
+// Sharing by single CTAs 17.6 where pairs take 16.4, by four or eight 19.5; one of 8192 by pairs 11.2, by one cluster of eight 10.6.
 constexpr int ITEM_TILES = 8, ITEM_WAVES = 4;
 constexpr int SHARING_SEQS = 4, SHARING_PAIRS = 8;                          // sequences at most, pairs of an item at least (fewer leave many places of the device empty)
 struct Cut {
