@@ -122,7 +122,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 // halves are common (x, z and s have eleven bits each), so quarters with a t that near one are looked at again, value by value, in 64 bits, where difference and
 // products are exact; and those whose rounded scale and centre lead codes out of range, which are clamped there.
 template <typename T, int DIM, int BITS>
-__device__ __forceinline__ void pack_row(const uint32_t (&x)[4][DIM / 32], unsigned char *dst, int lane, bool there) {
+__device__ __forceinline__ void pack_row(uint32_t (&x)[4][DIM / 32], unsigned char *dst, int lane, bool there) {
   using Two = typename Type<T>::Two;
   constexpr int W = DIM / 32, J = DIM / 32, CODES = DIM / 4, PER_WORD = 32 / BITS;         // words of values in a quarter; codes of a quarter in a chunk, of the lane, of a word
   constexpr float M = 1 << (BITS - 1), LEVELS = (1 << BITS) - 1, MAGIC = 12582912.0f;
@@ -150,6 +150,15 @@ __device__ __forceinline__ void pack_row(const uint32_t (&x)[4][DIM / 32], unsig
   const float s = __half2float(sh);
   const __half zh = good ? __float2half_rn(fmaf(M, s, range.x)) : __ushort_as_half(0x7fff);
   const float z = __half2float(zh);
+  // A quarter without numbers has codes of M: a product with its values would be none either, and its bits, added into a word, would run over into other quarters' codes
+  if (__any_sync(0xffffffffu, !good)) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const bool keep = __shfl_sync(0xffffffffu, static_cast<int>(good), b, 4) != 0;
+#pragma unroll
+      for (int w = 0; w < W; ++w) x[b][w] = keep ? x[b][w] : 0u;
+    }
+  }
   // t = x k + c; k, c and the sum are rounded once each, k's error counts for x - z: off by (2 LEVELS + 2 + |c|) 2^-24 at most
   const float k0 = s > 0.0f ? __frcp_rn(s) : 0.0f, c0 = good ? fmaf(-z, k0, M) : M, off = (2.0f * LEVELS + 2.0f + fabsf(c0)) * 0x1p-24f;
   const bool inside = fmaf(range.x, k0, c0) > -0.5f + off && fmaf(range.y, k0, c0) < LEVELS + 0.5f - off;

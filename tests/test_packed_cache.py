@@ -708,3 +708,58 @@ def test_caches_further_apart_than_32_bits(gpu, bits):
     check_attention(gpu.attention_packed_cache(q[:1], long, long, lens.cuda()), q[:1], long, long, lens)
     long, lens = long.expand(40, -1, -1, -1), torch.tensor([9 - b % 4 for b in range(40)], dtype=torch.int32)
     check_attention(gpu.attention_packed_cache(q[:1].expand(40, -1, -1), long, long, lens.cuda()), q[:1].expand(40, -1, -1), long, long, lens)
+
+
+# ------------------------------------------------------------------------------------------------------------- quarters that are no numbers beside others
+def with_bad_quarters(dim, dtype, seed=0):
+    """Rows of random values, each with a NaN or an infinity at one place of a quarter, at several, or in several quarters; rows without one between them."""
+    x = torch.randn(1, 3, 4 * 3 * (dim // 4) + 9, dim, generator=torch.Generator().manual_seed(seed)).to(DTYPES[dtype])
+    n = 0
+    for quarter in range(4):
+        for bad in (math.nan, math.inf, -math.inf):
+            for d in range(dim // 4):
+                x[0, n % 3, n, dim // 4 * quarter + d] = bad
+                if n % 5 == 0:
+                    x[0, n % 3, n, (dim // 4 * (quarter + 1) + d) % dim] = -bad
+                if n % 7 == 0:
+                    x[0, n % 3, n, dim // 4 * quarter:dim // 4 * (quarter + 1)] = bad
+                n += 1
+    x[0, 0, n] = math.nan
+    x[0, 1, n + 1, 3], x[0, 1, n + 1, 4] = math.inf, -math.inf
+    return x
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("dim,bits", [(64, 4), (64, 8), (128, 4), (128, 8)])
+def test_quarters_beside_one_without_numbers_keep_their_codes(gpu, dim, bits, dtype):
+    """Every byte of such rows: the other quarters' codes, the middle code in the bad ones, the trailers."""
+    x = with_bad_quarters(dim, dtype)
+    want = packed(x, bits), packed(-x, bits)
+    got = [torch.zeros(want[0].shape, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    gpu.write_cache_packed(x.cuda(), -x.cuda(), *got)
+    for w, g in zip(want, got):
+        assert torch.equal(g.cpu(), w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,bits", [(64, 4), (64, 8), (128, 4), (128, 8)])
+@pytest.mark.parametrize("q_heads", [2, 4, 8, 16])
+def test_outputs_beside_a_value_without_numbers(gpu, dim, bits, q_heads):
+    """A value that is no number leaves the other three quarters of its head's outputs what the rows' values give, written by the operator itself."""
+    rows = 40
+    q, kc, vc = attention_inputs(4, q_heads, 1, dim, bits, rows)
+    v = made(4, 1, rows, dim, seed=1, gain=0.5)
+    for b in range(4):
+        v[b, 0, 7 + b, dim // 4 * b + 1] = (math.nan, math.inf, -math.inf, math.nan)[b]
+    gpu.write_cache_packed(made(4, 1, rows, dim, seed=0), v, kc, vc)
+    lens = torch.full((4,), rows, dtype=torch.int32)
+    out, lse = gpu.attention_packed_cache(q, kc, vc, lens.cuda())
+    quarter = torch.arange(dim) // (dim // 4)
+    bad = (quarter == torch.arange(4)[:, None])[:, None].expand(4, q_heads, dim).cuda()
+    assert torch.equal(out.isnan(), bad)
+    # a row's bad quarter made 0: what the others' outputs go by
+    good = v.clone()
+    for b in range(4):
+        good[b, 0, 7 + b, dim // 4 * b:dim // 4 * (b + 1)] = 0.0
+    check_attention((torch.where(bad, gpu.attention_packed_cache(q, kc, packed(good, bits).cuda(), lens.cuda())[0], out), lse), q, kc, packed(good, bits), lens)
