@@ -114,6 +114,14 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
+// hi - lo, rounded to odd: where 24 bits do not hold it, the one of the two numbers around it whose last bit is set.  LEVELS times a tie of the fp16 scale has at most 20
+// bits, so it is none of these, and the division keeps a quotient on its side of a tie (it is off it by more than a half of its last place).
+__device__ __forceinline__ float difference(float hi, float lo) {
+  const float d = __fsub_rn(hi, lo), b = __fsub_rn(d, hi), rest = __fsub_rn(__fsub_rn(hi, __fsub_rn(d, b)), __fadd_rn(lo, b));      // d + rest is exact
+  const int bits = __float_as_int(d);            // (hi >= lo)
+  return rest == 0.0f || (bits & 1) ? d : __int_as_float(rest > 0.0f ? bits + 1 : bits - 1);
+}
+
 // A row of values to a packed one at `dst` (where `there`): four lanes, x[b] lane t's DIM/16 of quarter b, those of chunks 2 t and 2 t + 1.
 //
 // The quarters' least and largest values are reduced and scattered: each lane ends up with one quarter's, makes its scale and centre and hands out what the codes are computed
@@ -146,7 +154,7 @@ __device__ __forceinline__ void pack_row(uint32_t (&x)[4][DIM / 32], unsigned ch
   const Two first = lows(l, h), other = highs(l, h), mine = second ? other : first, come = shuffled(second ? first : other, 1);
   const float2 range = Type<T>::floats(low_high(__hmin2_nan(mine, come), __hmax2_nan(mine, come)));
   const bool good = range.x >= -65504.0f && range.y <= 65504.0f;
-  const __half sh = good ? __float2half_rn((range.y - range.x) / LEVELS) : __ushort_as_half(0x7fff);
+  const __half sh = good ? __float2half_rn(difference(range.y, range.x) / LEVELS) : __ushort_as_half(0x7fff);
   const float s = __half2float(sh);
   const __half zh = good ? __float2half_rn(fmaf(M, s, range.x)) : __ushort_as_half(0x7fff);
   const float z = __half2float(zh);

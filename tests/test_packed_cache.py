@@ -763,3 +763,26 @@ def test_outputs_beside_a_value_without_numbers(gpu, dim, bits, q_heads):
     for b in range(4):
         good[b, 0, 7 + b, dim // 4 * b:dim // 4 * (b + 1)] = 0.0
     check_attention((torch.where(bad, gpu.attention_packed_cache(q, kc, packed(good, bits).cuda(), lens.cuda())[0], out), lse), q, kc, packed(good, bits), lens)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,bits", [(64, 4), (64, 8), (128, 4), (128, 8)])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_ranges_that_32_bits_do_not_hold(gpu, dtype, dim, bits):
+    """Ranges beside a tie of the scale, where a difference rounded to 32 bits would lie on it: the scales and codes of exact arithmetic.  fp16: 316 pairs of lowest and
+    highest value with 4 bits, 576 with 8; bf16: 12 with 8 and the smallest scales."""
+    mantissa, levels, pairs = {"fp16": 10, "bf16": 7}[dtype], 2 ** bits - 1, [(15 * 2.0 ** -25, -2.0 ** -60), (45 * 2.0 ** -25, 2.0 ** -60)]
+    high = np.arange(2 ** mantissa, 2 ** (mantissa + 1)) * 2.0 ** (14 - mantissa)
+    for below in range(8, 24):
+        low = -high * 2.0 ** -below
+        exact = ((high[:, None] - low) / levels).astype(np.float16)
+        rounded = ((high.astype(np.float32)[:, None] - low.astype(np.float32)) / np.float32(levels)).astype(np.float16)
+        pairs += [(high[i], low[j]) for i, j in zip(*np.nonzero(exact != rounded))]
+    pairs = np.array(pairs)
+    assert len(pairs) == 2 + {("fp16", 4): 316, ("fp16", 8): 576, ("bf16", 4): 0, ("bf16", 8): 12}[dtype, bits]
+    share = np.random.default_rng(1).random((1, 1, len(pairs), dim))
+    share[..., ::dim // 4], share[..., 1::dim // 4] = 0.0, 1.0
+    x = torch.from_numpy(pairs[:, 1:] + (pairs[:, :1] - pairs[:, 1:]) * share).to(DTYPES[dtype])
+    got = [torch.zeros(1, 1, len(pairs), gpu.packed_row_bytes(dim, bits), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    gpu.write_cache_packed(x.cuda(), -x.cuda(), *got)
+    assert torch.equal(got[0].cpu(), packed(x, bits)) and torch.equal(got[1].cpu(), packed(-x, bits))
