@@ -127,8 +127,8 @@ __device__ __forceinline__ float difference(float hi, float lo) {
 // The quarters' least and largest values are reduced and scattered: each lane ends up with one quarter's, makes its scale and centre and hands out what the codes are computed
 // with, so a division is done once a lane.  A code: t = x / s + (M - z / s), one multiply-add; t + 1.5 2^23 is it rounded, in the low bits of a word, and a
 // shift and an addition put it into its place, the 1.5 2^23 of all taken off at once.  All but those for two values at a time.  What t is off by may cross a border: exact
-// halves are common (x, z and s have eleven bits each), so quarters with a t that near one are looked at again, value by value, in 64 bits, where difference and
-// products are exact; and those whose rounded scale and centre lead codes out of range, which are clamped there.
+// halves are common (x, z and s have eleven bits each), so quarters with a t that near one are looked at again, value by value, in 64 bits, where the border
+// is exact (z and s are multiples of 2^-24) and the difference has the right sign; and those whose rounded scale and centre lead codes out of range, which are clamped there.
 template <typename T, int DIM, int BITS>
 __device__ __forceinline__ void pack_row(uint32_t (&x)[4][DIM / 32], unsigned char *dst, int lane, bool there) {
   using Two = typename Type<T>::Two;
@@ -200,7 +200,7 @@ __device__ __forceinline__ void pack_row(uint32_t (&x)[4][DIM / 32], unsigned ch
           const float y = (j ? u.y : u.x) + MAGIC, n = y - MAGIC, r = (j ? u.y : u.x) - n;
           if (fabsf(r) > limit) {
             const float m = r < 0.0f ? n - 1.0f : n;       // between codes m and m + 1
-            const double above = (static_cast<double>(j ? v.y : v.x) - zd) - (static_cast<double>(m - M) + 0.5) * sd;
+            const double border = zd + (static_cast<double>(m - M) + 0.5) * sd, above = static_cast<double>(j ? v.y : v.x) - border;
             const float code = fminf(fmaxf(above > 0.0 || (above == 0.0 && (static_cast<int>(m) & 1)) ? m + 1.0f : m, 0.0f), LEVELS);
             const int index = CODES / 2 * (2 * w / J) + J * b + 2 * w % J + j;
             words[index / PER_WORD] += static_cast<uint32_t>(static_cast<int>(code - n)) << (BITS * (index % PER_WORD));

@@ -786,3 +786,25 @@ def test_ranges_that_32_bits_do_not_hold(gpu, dtype, dim, bits):
     got = [torch.zeros(1, 1, len(pairs), gpu.packed_row_bytes(dim, bits), dtype=torch.uint8, device="cuda") for _ in range(2)]
     gpu.write_cache_packed(x.cuda(), -x.cuda(), *got)
     assert torch.equal(got[0].cpu(), packed(x, bits)) and torch.equal(got[1].cpu(), packed(-x, bits))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,bits", [(64, 4), (64, 8), (128, 4), (128, 8)])
+def test_values_beside_a_border_by_less_than_64_bits_hold(gpu, dim, bits):
+    """Quarters from -L to L (L half the levels: scale 1, centre 1/2), so 0 lies between the codes M - 1 and M: bf16 values above it become M, those below it M - 1, 0 itself
+    the even one, M."""
+    levels, middle = 2 ** bits - 1, 2 ** (bits - 1)
+    n = dim // 4 - 2
+    sizes = 2.0 ** -torch.arange(20, 20 + 4 * n * 2, 2).double().clamp(max=133).view(4, 1, n).expand(4, 3, n)
+    x = torch.zeros(4, 3, 4, n + 2, dtype=torch.float64)
+    x[..., 0], x[..., 1] = -levels / 2, levels / 2
+    x[..., 2:] = (sizes * torch.tensor([1.0, -1.0, 0.0]).double()[:, None])[:, :, None]
+    x = x.view(1, 4, 3, dim).bfloat16()
+    assert bool((x.double().view(4, 3, 4, n + 2)[:, :2, :, 2:].abs() == sizes[:, :2, None]).all())
+    got = [torch.zeros(1, 4, 3, gpu.packed_row_bytes(dim, bits), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    gpu.write_cache_packed(x.cuda(), (-x).cuda(), *got)
+    for sign, cache in zip((1.0, -1.0), got):
+        z, s, n = parts(cache, dim)
+        at = x.double() * sign
+        want = torch.where(at.abs() == levels / 2, at - 0.5, torch.where(at < 0, -1.0, 0.0))
+        assert bool((z == 0.5).all()) and bool((s == 1).all()) and torch.equal(n, want)
