@@ -44,7 +44,10 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // Weights are 2^SHIFT at the row's maximum, up to 2^(SHIFT + SLACK) where that has risen since it was last looked at: fp16 has 11 bits of them down to 2^-21 of
 // the largest.
 constexpr float SHIFT = 7.0f, SLACK = 8.0f;
-constexpr float NOTHING = 3.0e38f;               // in the exponent while no score has been seen: the first one rises, -inf stays that
+constexpr float NOTHING = -3.0e38f;              // the maximum while no score has been seen: the first one rises (times 2^-120 it is -256 below), -inf stays that
+// The largest factor (scores are below 2^7 in their units, so products stay finite).  One that is cut to it makes the same weights: scores that differ do so by 2^-72 at least, and
+// that times 2^120 leaves the largest alone.
+constexpr float MOST = 0x1p120f;
 
 struct AttendParams {
   Caches caches;
@@ -280,7 +283,17 @@ struct Tiles {
     return top == 0.0f || top == INFINITY ? 0 : min(max(TOP - e, -126), 126);
   }
   // What a score is multiplied by (a factor of 0 would make no number of the scores of rows that are not there, -inf)
-  static __device__ __forceinline__ float factor_of(const AttendParams &p, int lifted) { return fmaxf(fabsf(p.scale_log2) * power2(-lifted) / UNIT, 0x1p-120f); }
+  static __device__ __forceinline__ float factor_of(const AttendParams &p, int lifted) { return fminf(fmaxf(fabsf(p.scale_log2) * power2(-lifted) / UNIT, 0x1p-120f), MOST); }
+  // The score, times log2 e, whose weight is 1 where that of the maximum is 2^SHIFT; at most the largest number.  Of a head whose factor was cut to MOST by what that would have been
+  template <typename T>
+  static __device__ __forceinline__ float level_of(const AttendParams &p, float m, float factor, int b, int q_head) {
+    if (factor < MOST || isinf(m)) return fmaf(m, factor, -SHIFT);
+    const T *const q = static_cast<const T *>(p.q) + b * p.q_seq + q_head * p.q_head;
+    float top = 0.0f;
+    for (int d = 0; d < DIM; ++d) top = fmaxf(top, fabsf(static_cast<float>(q[d])));
+    const double x = static_cast<double>(m) * fabsf(p.scale_log2) * power2(-lift(top)) / UNIT;
+    return static_cast<float>(fmin(fmax(x, -3.4e38), 3.4e38));
+  }
   // The power of two that takes a scale into (1/2, 1], at most `old`
   static __device__ __forceinline__ float taken(float most, float old) {
     const int e = static_cast<int>((__float_as_uint(fmaxf(most, 0.0f)) + 0x7fffffu) >> 23) - 127;
@@ -303,22 +316,19 @@ __device__ __forceinline__ void take_tile(A &a, uint32_t kt, int rows, int lane)
   }
   // the maximum moves when a score is SLACK above it
   float v = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
-  if (__any_sync(0xffffffffu, fmaf(v, a.factor, a.off) > SHIFT + SLACK)) {
+  if (__any_sync(0xffffffffu, (v - a.m) * a.factor > SLACK)) {
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     v = fmaxf(v, a.m);
-    if (v != -INFINITY) {
-      a.scale(exp2_fast((a.m - v) * a.factor));
-      a.m = v;
-      a.off = fmaf(-v, a.factor, SHIFT);
-    }
+    a.scale(exp2_fast((a.m - v) * a.factor));
+    a.m = v;
   }
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     uint32_t hi[2], lo[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const float w = exp2_fast(fmaf(x[h][r], a.factor, a.off));
+      const float w = exp2_fast(fmaf(x[h][r] - a.m, a.factor, SHIFT));
       a.l += w;
       const uint32_t upper = pack2(w, w);
       hi[r] = transposed(upper);
@@ -345,7 +355,7 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
   static constexpr int PAIRS = 16 / BITS, KSTEPS = N * PAIRS;               // operand words of a word of codes; k steps of a row of keys
 
   uint32_t qb[KSTEPS][2], qz[2];                 // queries; sums over quarters, as upper and lower fp16 parts
-  float factor, m, off, l;                       // what a score is multiplied by, the largest score, what is added in the exponent, the sum of weights
+  float factor, m, l;                            // what a score is multiplied by, the largest score, the sum of weights
   float acc[4][STEPS][4], sums[4], zacc[4];      // out^T, quarter by quarter; what is to be taken off; sums of weights times centres (lanes g >= 4: of quarter g - 4)
   __half2 f;                                     // power of two that takes quarter g & 3's scales of values to 1 or below
 
@@ -386,8 +396,7 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
     qz[0] = pack2(even ? __half2float(upper) : 0.0f, odd ? __half2float(upper) : 0.0f);
     qz[1] = pack2(even ? rest : 0.0f, odd ? rest : 0.0f);
     factor = __shfl_sync(0xffffffffu, Base::factor_of(p, up), t < 2 ? 0 : 16);
-    m = -INFINITY;
-    off = NOTHING;
+    m = NOTHING;
     l = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -536,8 +545,9 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
       else store_out<T, DIM>(static_cast<T *>(p.out) + row * DIM + DIM / 4 * i + J * g, v, by);
     }
     if (!live || (t & 1) || g) return;
-    if (state) ml[h] = make_float2(total == 0.0f ? -INFINITY : -off, total);
-    else if (p.lse) p.lse[row] = total == 0.0f ? -INFINITY : logf(total) - off * LN2;
+    const float most = total == 0.0f ? -INFINITY : Base::template level_of<T>(p, m, factor, b, kv_head * p.group + h);
+    if (state) ml[h] = make_float2(most, total);
+    else if (p.lse) p.lse[row] = logf(total) + most * LN2;
   }
 };
 
@@ -551,7 +561,7 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
   static constexpr bool LOWER = !Type<T>::BF16;            // whether weights have a lower part
 
   uint32_t qb[2][STEPS][2], qz[2];               // queries of the column's even and odd quarter; sums over quarters, as upper and lower fp16 parts
-  float factor, m, off, l;                       // what a score is multiplied by, the largest score, what is added in the exponent, the sum of weights; of head t
+  float factor, m, l;                            // what a score is multiplied by, the largest score, the sum of weights; of head t
   float acc[4][STEPS][4], sums[2][4], zacc[4];   // out^T, quarter by quarter; what is to be taken off; sums of weights times centres (lanes g >= 4: of quarter g - 4)
   __half2 f;                                     // power of two that takes quarter g & 3's scales of values to 1 or below
 
@@ -596,8 +606,7 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
     const float2 back = __half22float2(h2(qz[0]));
     qz[1] = pack2(unit * sum[0] - back.x, unit * sum[1] - back.y);
     factor = __shfl_sync(0xffffffffu, Base::factor_of(p, up), 8 * t);
-    m = -INFINITY;
-    off = NOTHING;
+    m = NOTHING;
     l = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -739,8 +748,9 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
       else store_out<T, DIM>(static_cast<T *>(p.out) + row * DIM + DIM / 4 * i + J * g, v, by);
     }
     if (!live || g) return;
-    if (state) ml[h] = make_float2(total == 0.0f ? -INFINITY : -off, total);
-    else if (p.lse) p.lse[row] = total == 0.0f ? -INFINITY : logf(total) - off * LN2;
+    const float most = total == 0.0f ? -INFINITY : Base::template level_of<T>(p, m, factor, b, kv_head * p.group + h);
+    if (state) ml[h] = make_float2(most, total);
+    else if (p.lse) p.lse[row] = logf(total) + most * LN2;
   }
 };
 
@@ -753,7 +763,7 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
   static constexpr bool LOWER = !Type<T>::BF16;            // whether weights have a lower part
 
   uint32_t qb[NT][4][STEPS][2], qz[NT][2];       // queries; sums over quarters, as upper and lower fp16 parts
-  float factor[NT][2], m[NT][2], off[NT][2], l[NT][2];     // of heads 2 t and 2 t + 1: what a score is multiplied by, the largest score, what is added in the exponent, the sum of weights
+  float factor[NT][2], m[NT][2], l[NT][2];       // of heads 2 t and 2 t + 1: what a score is multiplied by, the largest score, the sum of weights
   float acc[NT][4][STEPS][4], sums[NT][4][4], zacc[NT][4]; // out^T, quarter by quarter; what is to be taken off; sums of weights times centres (lanes g >= 4: of quarter g - 4)
   __half2 f;                                     // power of two that takes quarter g & 3's scales of values to 1 or below
 
@@ -801,8 +811,7 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
       const float2 back = __half22float2(h2(upper));
       qz[nt][0] = upper;
       qz[nt][1] = pack2(s0 - back.x, s1 - back.y);
-      m[nt][0] = m[nt][1] = -INFINITY;
-      off[nt][0] = off[nt][1] = NOTHING;
+      m[nt][0] = m[nt][1] = NOTHING;
       l[nt][0] = l[nt][1] = 0.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -947,7 +956,7 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         top[nt][e] = fmaxf(fmaxf(x[0][nt][e], x[0][nt][e + 2]), fmaxf(x[1][nt][e], x[1][nt][e + 2]));
-        rises |= fmaf(top[nt][e], factor[nt][e], off[nt][e]) > SHIFT + SLACK;
+        rises |= (top[nt][e] - m[nt][e]) * factor[nt][e] > SLACK;
       }
     if (__any_sync(0xffffffffu, rises)) {
 #pragma unroll
@@ -958,20 +967,17 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
           v = fmaxf(v, m[nt][e]);
-          if (v != -INFINITY) {
-            const float by = exp2_fast((m[nt][e] - v) * factor[nt][e]);
-            m[nt][e] = v;
-            off[nt][e] = fmaf(-v, factor[nt][e], SHIFT);
-            l[nt][e] *= by;
-            zacc[nt][e] *= by;
-            zacc[nt][e + 2] *= by;
+          const float by = exp2_fast((m[nt][e] - v) * factor[nt][e]);
+          m[nt][e] = v;
+          l[nt][e] *= by;
+          zacc[nt][e] *= by;
+          zacc[nt][e + 2] *= by;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              sums[nt][i][e] *= by;
-              sums[nt][i][e + 2] *= by;
+          for (int i = 0; i < 4; ++i) {
+            sums[nt][i][e] *= by;
+            sums[nt][i][e + 2] *= by;
 #pragma unroll
-              for (int u = 0; u < STEPS; ++u) { acc[nt][i][u][e] *= by; acc[nt][i][u][e + 2] *= by; }
-            }
+            for (int u = 0; u < STEPS; ++u) { acc[nt][i][u][e] *= by; acc[nt][i][u][e + 2] *= by; }
           }
         }
     }
@@ -983,7 +989,7 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
         float w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          w[e] = exp2_fast(fmaf(x[h][nt][e], factor[nt][e % 2], off[nt][e % 2]));
+          w[e] = exp2_fast(fmaf(x[h][nt][e] - m[nt][e % 2], factor[nt][e % 2], SHIFT));
           l[nt][e % 2] += w[e];
         }
 #pragma unroll
@@ -1030,8 +1036,9 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
           else store_out<T, DIM>(static_cast<T *>(p.out) + row * DIM + DIM / 4 * i + J * g, v, by);
         }
         if (h >= p.group || g) continue;
-        if (state) ml[h] = make_float2(total == 0.0f ? -INFINITY : -off[nt][e], total);
-        else if (p.lse) p.lse[row] = total == 0.0f ? -INFINITY : logf(total) - off[nt][e] * LN2;
+        const float most = total == 0.0f ? -INFINITY : Base::template level_of<T>(p, m[nt][e], factor[nt][e], b, kv_head * p.group + h);
+        if (state) ml[h] = make_float2(most, total);
+        else if (p.lse) p.lse[row] = logf(total) + most * LN2;
       }
   }
 };

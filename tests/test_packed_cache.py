@@ -808,3 +808,41 @@ def test_values_beside_a_border_by_less_than_64_bits_hold(gpu, dim, bits):
         at = x.double() * sign
         want = torch.where(at.abs() == levels / 2, at - 0.5, torch.where(at < 0, -1.0, 0.0))
         assert bool((z == 0.5).all()) and bool((s == 1).all()) and torch.equal(n, want)
+
+
+def check_hardest(got, q, kc, vc, lens, scale):
+    """``check_attention`` where scores lie so far apart that the largest takes all: the output is its row, off by its rounding and by that of the scale to 11 bits; the
+    logarithm is its score, which has the error of a fp32 sum.  Heads whose two largest scores are closer than that are left out of the first."""
+    out, lse, sure_heads = *(x.double().cpu() for x in got), []
+    dim, group, bits = q.shape[2], q.shape[1] // kc.shape[1], (kc.shape[3] - 16) * 8 // q.shape[2]
+    for b in range(q.shape[0]):
+        (kz, ks, kn), (vz, vs, vn) = (tuple(x.repeat_interleave(group, 0) for x in parts(c[b][:, :int(lens[b])], dim)) for c in (kc, vc))
+        qb = q[b].double().cpu()
+        s = torch.einsum("hd,hnd->hn", qb, kz + ks * kn) * scale
+        error = (dim + 8) * 2.0 ** -24 * torch.einsum("hd,hnd->hn", qb.abs(), kz.abs() + ks * 2 ** bits).amax(1) * abs(scale)
+        first, second = s.topk(2, 1).values.unbind(1)
+        sure = first - second > 2 * error + 1e3
+        sure_heads.append(sure)
+        at = s.argmax(1)[:, None, None].expand(-1, 1, dim)
+        z, move = vz.gather(1, at)[:, 0], (vs * vn).gather(1, at)[:, 0]
+        tol = torch.finfo(q.dtype).eps / 2 * (z + move).abs() + 2.0 ** -11 * 1.001 * (z.abs() + move.abs()) + 2.0 ** -20 * (z.abs() + vs.gather(1, at)[:, 0] * 2 ** bits)
+        assert bool(((out[b] - z - move).abs() <= tol)[sure].all()) and bool(out.isfinite().all()), (b, float(((out[b] - z - move).abs() / tol)[sure].max()))
+        assert bool(((lse[b] - first).abs() <= error + 2.0 ** -22 * first.abs()).all()), (b, lse[b], first)
+    assert float(torch.cat(sure_heads).double().mean()) >= 0.8                 # (of the inputs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,bits", [(64, 4), (64, 8), (128, 4), (128, 8)])
+@pytest.mark.parametrize("q_heads", [4, 8, 16, 32])
+@pytest.mark.parametrize("room", [300, 20000])
+def test_scores_far_apart(gpu, dim, bits, q_heads, room):
+    """Scores of 1e9 to 1e37: large scales, bf16 queries of up to 2^118, and keys so small that the scale alone has no place in 32 bits."""
+    seqs, rows = 3, 300
+    lens = torch.tensor([300, 41, 230], dtype=torch.int32)
+    for dtype, size, keys, scale in (("fp16", 1.0, 1.0, 1e9), ("fp16", 1.0, 1.0, -1e20), ("fp16", 2.0 ** -10, 1.0, 1e30), ("fp16", 1.0, 2.0 ** -8, 1e37), ("fp16", 1.0, 2.0 ** -12, -1.9e38),
+                                     ("bf16", 1.0, 1.0, 1e36), ("bf16", 2.0 ** 107, 1.0, None), ("bf16", 2.0 ** 116, 1.0, None), ("bf16", 2.0 ** 118, 2.0 ** -9, -2.0),
+                                     ("bf16", 2.0 ** 100, 2.0 ** -12, 2.0 ** 20), ("bf16", 2.0 ** -100, 1.0, 1e37)):
+        q = (made(seqs, q_heads, dim, seed=6).float().clamp(-4, 4) * size).to(DTYPES[dtype])
+        k, v = made(seqs, 2, rows, dim, seed=7, gain=keys), made(seqs, 2, rows, dim, seed=8)
+        kc, vc = (with_room(packed(x, bits).cuda(), room) for x in (k, v))
+        check_hardest(gpu.attention_packed_cache(q, kc, vc, lens.cuda(), scale=scale), q, kc, vc, lens, dim ** -0.5 if scale is None else scale)
