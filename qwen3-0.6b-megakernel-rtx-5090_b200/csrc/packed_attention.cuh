@@ -8,11 +8,11 @@
 // trailer, 16 bytes,
 // is a row of an 8 x 8 tile, so ldmatrix makes the operands of the sums over centres.
 //
-// Roundings: queries are taken to fp16 times a power of two, which leaves them as they are but for entries below 2^-26 of the largest.  Weights are carried
-// as two fp16 numbers (one where the output is bf16), and the product with a scale is rounded once, to fp16, because the tensor cores multiply 16-bit numbers: as much
-// as the output's own rounding, so the error against 64 bits is 1.2 to 1.4 times an exact softmax's (1.0 in bf16).  The third sum above takes the rounded products, so M does
-// not add to that.  Sums, softmax statistics and outputs are fp32.  Every second 16 rows go in as 2^BITS - 1 - n with the weights' sign turned (the same instructions): the running
-// sums stay around zero, whose size the accumulator's truncation goes by (with n throughout one sequence of 32,768 rows was 1.8 times off).
+// Roundings: queries are taken to fp16 times a power of two (Tiles::lift).  Weights and their products with scales are carried as two fp16 numbers each, because the tensor cores multiply
+// 16-bit numbers: over many outputs the error against 64 bits is 1.00 to 1.01 times that of rounding the exact result (1.06 to 1.36 times with one number a product, which took 16 of up to 2048
+// rows 12.8 us, 128 of up to 8192 122, 96 of 8192 160 and 32 of up to 4096 with sixteen heads a kv head 23.5, where two take 13.6, 125, 175 and 27.9).  One each where the output is
+// bf16, whose own rounding is eight times theirs: 1.00 to 1.01 times too.  Sums, softmax statistics and outputs are fp32.  Every second 16 rows go in as 2^BITS - 1 - n with the
+// weights' sign turned (the same instructions): the running sums stay around zero, whose size the accumulator's truncation goes by.
 //
 // Work: tiles of 32 rows, a tile to a warp, each with a ring of copies of its own (cp.async: no waits but for its own copies).  attend_items: a cluster of CTAs has a (sequence, kv
 // head) and joins its states - the maximum, the sum and the unnormalised output - in shared memory.  attend_tiles: the tiles of all items in one line, of which
@@ -299,6 +299,13 @@ struct Tiles {
     const int e = static_cast<int>((__float_as_uint(fmaxf(most, 0.0f)) + 0x7fffffu) >> 23) - 127;
     return fminf(old, power2(min(max(-e, -14), 15)));
   }
+  // Two rows' weights (upper and lower parts) times scales, as upper and, of an output in fp16, lower parts
+  template <bool LOWER, bool FLIP>
+  static __device__ __forceinline__ void times(uint32_t hi, uint32_t lo, __half2 scales, uint32_t &upper, uint32_t &lower) {
+    const __half2 s = FLIP ? __hneg2(scales) : scales, first = __hmul2(h2(hi), s);
+    upper = bits_of(first);
+    if constexpr (LOWER) lower = bits_of(__hfma2(h2(lo), s, __hfma2(h2(hi), s, __hneg2(first))));
+  }
 };
 
 // A tile where all of a thread's columns are of one query head; `rows` rows of it are there (32 or more: all).
@@ -472,7 +479,7 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
   __device__ __forceinline__ void weigh(uint32_t vt, int lane, const uint32_t (&hi)[2], const uint32_t (&lo)[2]) {
     constexpr uint32_t MIDDLE = FLIP ? Base::MIDDLE_FLIPPED : Base::MIDDLE;
     const int t = lane & 3, g = lane >> 2;
-    uint32_t raw[4], w[4][N], pb[2];
+    uint32_t raw[4], w[4][N], pb[2], pl[2];
     trailers<true, ROW>(vt + CODES, lane, raw);
 #pragma unroll
     for (int r = 0; r < 4; ++r) lds<N>(vt + (2 * t + (r & 1) + 8 * (r >> 1)) * ROW + g * CHUNK, w[r]);
@@ -483,15 +490,10 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
       s0 = __hmul2(h2(r0), f);
       s1 = __hmul2(h2(r1), f);
     }
-    if (FLIP) { s0 = __hneg2(s0); s1 = __hneg2(s1); }
-    if constexpr (LOWER) {
-      pb[0] = bits_of(__hfma2(h2(hi[0]), s0, __hmul2(h2(lo[0]), s0)));
-      pb[1] = bits_of(__hfma2(h2(hi[1]), s1, __hmul2(h2(lo[1]), s1)));
-    } else {
-      pb[0] = bits_of(__hmul2(h2(hi[0]), s0));
-      pb[1] = bits_of(__hmul2(h2(hi[1]), s1));
-    }
+    Base::template times<LOWER, FLIP>(hi[0], lo[0], s0, pb[0], pl[0]);
+    Base::template times<LOWER, FLIP>(hi[1], lo[1], s1, pb[1], pl[1]);
     mma(sums, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pb[0], pb[1], sums[0], sums[1], sums[2], sums[3]);
+    if constexpr (LOWER) mma(sums, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pl[0], pl[1], sums[0], sums[1], sums[2], sums[3]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t first[J], second[J];
@@ -501,6 +503,7 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
       for (int u = 0; u < STEPS; ++u) {
         float (&c)[4] = acc[i][u];
         mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pb[0], pb[1], c[0], c[1], c[2], c[3]);
+        if constexpr (LOWER) mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pl[0], pl[1], c[0], c[1], c[2], c[3]);
       }
     }
     mma(zacc, raw[0], raw[1], raw[2], raw[3], hi[0], hi[1], zacc[0], zacc[1], zacc[2], zacc[3]);
@@ -673,7 +676,7 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
   __device__ __forceinline__ void weigh(uint32_t vt, int lane, const uint32_t (&hi)[2], const uint32_t (&lo)[2]) {
     constexpr uint32_t MIDDLE = FLIP ? Base::MIDDLE_FLIPPED : Base::MIDDLE;
     const int t = lane & 3, g = lane >> 2;
-    uint32_t raw[4], w[4][N], pb[2][2];
+    uint32_t raw[4], w[4][N], pb[2][2], pl[2][2];
     trailers<true, ROW>(vt + CODES, lane, raw);
 #pragma unroll
     for (int r = 0; r < 4; ++r) lds<N>(vt + (2 * t + (r & 1) + 8 * (r >> 1)) * ROW + g * CHUNK, w[r]);
@@ -686,17 +689,12 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {                // quarter 2 (g & 1) + i
       const int from = 8 * (g & 1) + 4 * i + t;
-      __half2 a0 = h2(__shfl_sync(0xffffffffu, bits_of(s0), from)), a1 = h2(__shfl_sync(0xffffffffu, bits_of(s1), from));
-      if (FLIP) { a0 = __hneg2(a0); a1 = __hneg2(a1); }
-      if constexpr (LOWER) {
-        pb[i][0] = bits_of(__hfma2(h2(hi[0]), a0, __hmul2(h2(lo[0]), a0)));
-        pb[i][1] = bits_of(__hfma2(h2(hi[1]), a1, __hmul2(h2(lo[1]), a1)));
-      } else {
-        pb[i][0] = bits_of(__hmul2(h2(hi[0]), a0));
-        pb[i][1] = bits_of(__hmul2(h2(hi[1]), a1));
-      }
+      const __half2 a0 = h2(__shfl_sync(0xffffffffu, bits_of(s0), from)), a1 = h2(__shfl_sync(0xffffffffu, bits_of(s1), from));
+      Base::template times<LOWER, FLIP>(hi[0], lo[0], a0, pb[i][0], pl[i][0]);
+      Base::template times<LOWER, FLIP>(hi[1], lo[1], a1, pb[i][1], pl[i][1]);
       float (&c)[4] = sums[i];
       mma(c, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pb[i][0], pb[i][1], c[0], c[1], c[2], c[3]);
+      if constexpr (LOWER) mma(c, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pl[i][0], pl[i][1], c[0], c[1], c[2], c[3]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -707,6 +705,7 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
       for (int u = 0; u < STEPS; ++u) {
         float (&c)[4] = acc[i][u];
         mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pb[i % 2][0], pb[i % 2][1], c[0], c[1], c[2], c[3]);
+        if constexpr (LOWER) mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pl[i % 2][0], pl[i % 2][1], c[0], c[1], c[2], c[3]);
       }
     }
     mma(zacc, raw[0], raw[1], raw[2], raw[3], hi[0], hi[1], zacc[0], zacc[1], zacc[2], zacc[3]);
@@ -899,20 +898,15 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      uint32_t first[J], second[J], pb[NT][2];
-      __half2 a0 = h2(__shfl_sync(0xffffffffu, bits_of(s0), 4 * i + t)), a1 = h2(__shfl_sync(0xffffffffu, bits_of(s1), 4 * i + t));
-      if (FLIP) { a0 = __hneg2(a0); a1 = __hneg2(a1); }
+      uint32_t first[J], second[J], pb[NT][2], pl[NT][2];
+      const __half2 a0 = h2(__shfl_sync(0xffffffffu, bits_of(s0), 4 * i + t)), a1 = h2(__shfl_sync(0xffffffffu, bits_of(s1), 4 * i + t));
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        if constexpr (LOWER) {
-          pb[nt][0] = bits_of(__hfma2(h2(hi[nt][0]), a0, __hmul2(h2(lo[nt][0]), a0)));
-          pb[nt][1] = bits_of(__hfma2(h2(hi[nt][1]), a1, __hmul2(h2(lo[nt][1]), a1)));
-        } else {
-          pb[nt][0] = bits_of(__hmul2(h2(hi[nt][0]), a0));
-          pb[nt][1] = bits_of(__hmul2(h2(hi[nt][1]), a1));
-        }
+        Base::template times<LOWER, FLIP>(hi[nt][0], lo[nt][0], a0, pb[nt][0], pl[nt][0]);
+        Base::template times<LOWER, FLIP>(hi[nt][1], lo[nt][1], a1, pb[nt][1], pl[nt][1]);
         float (&c)[4] = sums[nt][i];
         mma(c, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pb[nt][0], pb[nt][1], c[0], c[1], c[2], c[3]);
+        if constexpr (LOWER) mma(c, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pl[nt][0], pl[nt][1], c[0], c[1], c[2], c[3]);
       }
       expand<DIM, BITS, FLIP>(w[0], w[1], i, first);
       expand<DIM, BITS, FLIP>(w[2], w[3], i, second);
@@ -922,6 +916,7 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
         for (int nt = 0; nt < NT; ++nt) {
           float (&c)[4] = acc[nt][i][u];
           mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pb[nt][0], pb[nt][1], c[0], c[1], c[2], c[3]);
+          if constexpr (LOWER) mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pl[nt][0], pl[nt][1], c[0], c[1], c[2], c[3]);
         }
     }
 #pragma unroll

@@ -846,3 +846,18 @@ def test_scores_far_apart(gpu, dim, bits, q_heads, room):
         k, v = made(seqs, 2, rows, dim, seed=7, gain=keys), made(seqs, 2, rows, dim, seed=8)
         kc, vc = (with_room(packed(x, bits).cuda(), room) for x in (k, v))
         check_hardest(gpu.attention_packed_cache(q, kc, vc, lens.cuda(), scale=scale), q, kc, vc, lens, dim ** -0.5 if scale is None else scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,bits", [(64, 4), (64, 8), (128, 4), (128, 8)])
+@pytest.mark.parametrize("q_heads", [4, 8, 16, 32])
+@pytest.mark.parametrize("room", [300, 20000])
+def test_fp16_outputs_are_as_near_as_their_rounding(gpu, dim, bits, q_heads, room):
+    """Weights and their products with scales keep 22 bits or more: over all outputs the error is that of rounding the results in 64 bits to fp16, about 2^-12.2 of them.  A
+    twentieth more leaves 2^-16.5 for the fp32 sums, whose steps of 2^-24 add up to some 2^-20."""
+    rows = 300
+    q, kc, vc = attention_inputs(4, q_heads, 2, dim, bits, rows, seed=q_heads)
+    out, _ = gpu.attention_packed_cache(q, with_room(kc, room), with_room(vc, room), torch.full((4,), rows, dtype=torch.int32).cuda())
+    k, v = (values(c, dim).repeat_interleave(q_heads // 2, 1) for c in (kc, vc))
+    want = torch.einsum("bhn,bhnd->bhd", torch.softmax(torch.einsum("bhd,bhnd->bhn", q.double().cpu(), k) * dim ** -0.5, 2), v)
+    assert float((out.double().cpu() - want).norm()) <= 1.05 * float((want.half().double() - want).norm())
