@@ -306,6 +306,17 @@ struct Tiles {
     upper = bits_of(first);
     if constexpr (LOWER) lower = bits_of(__hfma2(h2(lo), s, __hfma2(h2(hi), s, __hneg2(first))));
   }
+  // The same where one of the powers of two is below 1, a scale above 1 having been seen: fp16 might not hold small scales times it, so they come as they are and it apart
+  template <bool LOWER, bool FLIP>
+  static __device__ __forceinline__ void times(uint32_t hi, uint32_t lo, __half2 scales, float power, uint32_t &upper, uint32_t &lower) {
+    const float2 a = __half22float2(h2(hi)), b = __half22float2(h2(lo)), s = __half22float2(scales);
+    const float by = FLIP ? -power : power, x = (a.x + b.x) * s.x * by, y = (a.y + b.y) * s.y * by;
+    upper = pack2(x, y);
+    if constexpr (LOWER) {
+      const float2 back = __half22float2(h2(upper));
+      lower = pack2(x - back.x, y - back.y);
+    }
+  }
 };
 
 // A tile where all of a thread's columns are of one query head; `rows` rows of it are there (32 or more: all).
@@ -365,6 +376,7 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
   float factor, m, l;                            // what a score is multiplied by, the largest score, the sum of weights
   float acc[4][STEPS][4], sums[4], zacc[4];      // out^T, quarter by quarter; what is to be taken off; sums of weights times centres (lanes g >= 4: of quarter g - 4)
   __half2 f;                                     // power of two that takes quarter g & 3's scales of values to 1 or below
+  bool wide;                                     // whether one of these is below 1
 
   __device__ __forceinline__ void begin(const AttendParams &p, const T *queries, long long stride, int lane) {
     const int t = lane & 3, g = lane >> 2, h = g >> 2, quarter = g & 3;
@@ -412,6 +424,7 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
       for (int u = 0; u < STEPS; ++u) { acc[i][u][0] = 0.0f; acc[i][u][1] = 0.0f; acc[i][u][2] = 0.0f; acc[i][u][3] = 0.0f; }
     }
     f = __float2half2_rn(0x1p15f);
+    wide = false;
   }
 
   // Scores of rows g and g + 8 of 16, times the power of two, head t / 2
@@ -463,6 +476,7 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
     most = __shfl_sync(0xffffffffu, most, lane & 15);                       // (of quarter g & 3)
     const float old = __low2float(f), now = Base::taken(most, old), by = now / old;
     f = __float2half2_rn(now);
+    wide = __any_sync(0xffffffffu, now < 1.0f);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float r = __shfl_sync(0xffffffffu, by, 4 * i);
@@ -492,6 +506,10 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
     }
     Base::template times<LOWER, FLIP>(hi[0], lo[0], s0, pb[0], pl[0]);
     Base::template times<LOWER, FLIP>(hi[1], lo[1], s1, pb[1], pl[1]);
+    if (wide) {
+      Base::template times<LOWER, FLIP>(hi[0], lo[0], h2(r0), __low2float(f), pb[0], pl[0]);
+      Base::template times<LOWER, FLIP>(hi[1], lo[1], h2(r1), __low2float(f), pb[1], pl[1]);
+    }
     mma(sums, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pb[0], pb[1], sums[0], sums[1], sums[2], sums[3]);
     if constexpr (LOWER) mma(sums, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pl[0], pl[1], sums[0], sums[1], sums[2], sums[3]);
 #pragma unroll
@@ -567,6 +585,7 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
   float factor, m, l;                            // what a score is multiplied by, the largest score, the sum of weights; of head t
   float acc[4][STEPS][4], sums[2][4], zacc[4];   // out^T, quarter by quarter; what is to be taken off; sums of weights times centres (lanes g >= 4: of quarter g - 4)
   __half2 f;                                     // power of two that takes quarter g & 3's scales of values to 1 or below
+  bool wide;                                     // whether one of these is below 1
 
   __device__ __forceinline__ void begin(const AttendParams &p, const T *queries, long long stride, int lane) {
     const int t = lane & 3, g = lane >> 2, h = g >> 1, half = g & 1;
@@ -618,6 +637,7 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
       for (int u = 0; u < STEPS; ++u) { acc[i][u][0] = 0.0f; acc[i][u][1] = 0.0f; acc[i][u][2] = 0.0f; acc[i][u][3] = 0.0f; }
     }
     f = __float2half2_rn(0x1p15f);
+    wide = false;
   }
 
   // Scores of rows g and g + 8 of 16, times the power of two, head t
@@ -661,6 +681,7 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
     most = __shfl_sync(0xffffffffu, most, lane & 15);                       // (of quarter g & 3)
     const float old = __low2float(f), now = Base::taken(most, old), by = now / old;
     f = __float2half2_rn(now);
+    wide = __any_sync(0xffffffffu, now < 1.0f);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float r = __shfl_sync(0xffffffffu, by, 4 * i);
@@ -692,6 +713,18 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
       const __half2 a0 = h2(__shfl_sync(0xffffffffu, bits_of(s0), from)), a1 = h2(__shfl_sync(0xffffffffu, bits_of(s1), from));
       Base::template times<LOWER, FLIP>(hi[0], lo[0], a0, pb[i][0], pl[i][0]);
       Base::template times<LOWER, FLIP>(hi[1], lo[1], a1, pb[i][1], pl[i][1]);
+    }
+    if (wide) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int from = 8 * (g & 1) + 4 * i + t;
+        const float power = __shfl_sync(0xffffffffu, __low2float(f), from);
+        Base::template times<LOWER, FLIP>(hi[0], lo[0], h2(__shfl_sync(0xffffffffu, raw[0], from)), power, pb[i][0], pl[i][0]);
+        Base::template times<LOWER, FLIP>(hi[1], lo[1], h2(__shfl_sync(0xffffffffu, raw[2], from)), power, pb[i][1], pl[i][1]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
       float (&c)[4] = sums[i];
       mma(c, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pb[i][0], pb[i][1], c[0], c[1], c[2], c[3]);
       if constexpr (LOWER) mma(c, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pl[i][0], pl[i][1], c[0], c[1], c[2], c[3]);
@@ -765,6 +798,7 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
   float factor[NT][2], m[NT][2], l[NT][2];       // of heads 2 t and 2 t + 1: what a score is multiplied by, the largest score, the sum of weights
   float acc[NT][4][STEPS][4], sums[NT][4][4], zacc[NT][4]; // out^T, quarter by quarter; what is to be taken off; sums of weights times centres (lanes g >= 4: of quarter g - 4)
   __half2 f;                                     // power of two that takes quarter g & 3's scales of values to 1 or below
+  bool wide;                                     // whether one of these is below 1
 
   // An item's queries, `stride` apart (global or shared memory), and nothing seen yet
   __device__ __forceinline__ void begin(const AttendParams &p, const T *queries, long long stride, int lane) {
@@ -821,6 +855,7 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
       }
     }
     f = __float2half2_rn(0x1p15f);
+    wide = false;
   }
 
   // Scores of 16 rows, times the power of two: rows g and g + 8, heads 2 t and 2 t + 1
@@ -869,6 +904,7 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
     most = __shfl_sync(0xffffffffu, most, lane & 15);                       // (of quarter g & 3)
     const float old = __low2float(f), now = Base::taken(most, old), by = now / old;
     f = __float2half2_rn(now);
+    wide = __any_sync(0xffffffffu, now < 1.0f);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float r = __shfl_sync(0xffffffffu, by, 4 * i);
@@ -896,28 +932,54 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
       s0 = __hmul2(h2(raw[0]), f);
       s1 = __hmul2(h2(raw[2]), f);
     }
+    constexpr int SPAN = NT == 1 ? 4 : 1;        // quarters whose operands are made together, with one look at `wide` (of two blocks of heads one: registers)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t first[J], second[J], pb[NT][2], pl[NT][2];
-      const __half2 a0 = h2(__shfl_sync(0xffffffffu, bits_of(s0), 4 * i + t)), a1 = h2(__shfl_sync(0xffffffffu, bits_of(s1), 4 * i + t));
+    for (int first_of = 0; first_of < 4; first_of += SPAN) {
+      uint32_t pb[SPAN][NT][2], pl[SPAN][NT][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        Base::template times<LOWER, FLIP>(hi[nt][0], lo[nt][0], a0, pb[nt][0], pl[nt][0]);
-        Base::template times<LOWER, FLIP>(hi[nt][1], lo[nt][1], a1, pb[nt][1], pl[nt][1]);
-        float (&c)[4] = sums[nt][i];
-        mma(c, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pb[nt][0], pb[nt][1], c[0], c[1], c[2], c[3]);
-        if constexpr (LOWER) mma(c, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pl[nt][0], pl[nt][1], c[0], c[1], c[2], c[3]);
-      }
-      expand<DIM, BITS, FLIP>(w[0], w[1], i, first);
-      expand<DIM, BITS, FLIP>(w[2], w[3], i, second);
-#pragma unroll
-      for (int u = 0; u < STEPS; ++u)
+      for (int k = 0; k < SPAN; ++k) {
+        const int from = 4 * (first_of + k) + t;
+        const __half2 a0 = h2(__shfl_sync(0xffffffffu, bits_of(s0), from)), a1 = h2(__shfl_sync(0xffffffffu, bits_of(s1), from));
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float (&c)[4] = acc[nt][i][u];
-          mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pb[nt][0], pb[nt][1], c[0], c[1], c[2], c[3]);
-          if constexpr (LOWER) mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pl[nt][0], pl[nt][1], c[0], c[1], c[2], c[3]);
+          Base::template times<LOWER, FLIP>(hi[nt][0], lo[nt][0], a0, pb[k][nt][0], pl[k][nt][0]);
+          Base::template times<LOWER, FLIP>(hi[nt][1], lo[nt][1], a1, pb[k][nt][1], pl[k][nt][1]);
         }
+      }
+      if (wide) {
+#pragma unroll
+        for (int k = 0; k < SPAN; ++k) {
+          const int from = 4 * (first_of + k) + t;
+          const float power = __shfl_sync(0xffffffffu, __low2float(f), from);
+          const __half2 r0 = h2(__shfl_sync(0xffffffffu, raw[0], from)), r1 = h2(__shfl_sync(0xffffffffu, raw[2], from));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            Base::template times<LOWER, FLIP>(hi[nt][0], lo[nt][0], r0, power, pb[k][nt][0], pl[k][nt][0]);
+            Base::template times<LOWER, FLIP>(hi[nt][1], lo[nt][1], r1, power, pb[k][nt][1], pl[k][nt][1]);
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < SPAN; ++k) {
+        const int i = first_of + k;
+        uint32_t first[J], second[J];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float (&c)[4] = sums[nt][i];
+          mma(c, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pb[k][nt][0], pb[k][nt][1], c[0], c[1], c[2], c[3]);
+          if constexpr (LOWER) mma(c, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pl[k][nt][0], pl[k][nt][1], c[0], c[1], c[2], c[3]);
+        }
+        expand<DIM, BITS, FLIP>(w[0], w[1], i, first);
+        expand<DIM, BITS, FLIP>(w[2], w[3], i, second);
+#pragma unroll
+        for (int u = 0; u < STEPS; ++u)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float (&c)[4] = acc[nt][i][u];
+            mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pb[k][nt][0], pb[k][nt][1], c[0], c[1], c[2], c[3]);
+            if constexpr (LOWER) mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pl[k][nt][0], pl[k][nt][1], c[0], c[1], c[2], c[3]);
+          }
+      }
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {

@@ -861,3 +861,25 @@ def test_fp16_outputs_are_as_near_as_their_rounding(gpu, dim, bits, q_heads, roo
     k, v = (values(c, dim).repeat_interleave(q_heads // 2, 1) for c in (kc, vc))
     want = torch.einsum("bhn,bhnd->bhd", torch.softmax(torch.einsum("bhd,bhnd->bhn", q.double().cpu(), k) * dim ** -0.5, 2), v)
     assert float((out.double().cpu() - want).norm()) <= 1.05 * float((want.half().double() - want).norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("dim,bits", [(64, 4), (64, 8), (128, 4), (128, 8)])
+@pytest.mark.parametrize("q_heads", [4, 8, 16, 32])
+@pytest.mark.parametrize("far", [2.0 ** 10, 2.0 ** 14])
+def test_rows_beside_much_larger_ones(gpu, dim, bits, q_heads, far, dtype):
+    """A row whose values are up to 2^16 times the others', and whose weight is next to nothing: the output is as near to that of 64 bits as its rounding.  A product of
+    weight and scale is a number of 22 bits (11 for bf16), its last at 2^-25 of 2^7 times the largest scale: 2^-32 2^16 of a row's own values, and sums of 300 rows' errors are less than a row's."""
+    rows = 300
+    q, k = made(4, q_heads, dim, dtype=dtype, seed=1), made(4, 2, rows, dim, seed=2)
+    v = made(4, 2, rows, dim, seed=3, gain=0.25)
+    q[..., 0], k[:, :, ::97, 0] = 16.0, -40.0 * (dim / 64) ** 0.5
+    v[:, :, ::97] = (made(4, 2, rows, dim, seed=4)[:, :, ::97].float().clamp(-3.5, 3.5) * far).half()
+    kc, vc = packed(k, bits).cuda(), packed(v, bits).cuda()
+    out, _ = gpu.attention_packed_cache(q, kc, vc, torch.full((4,), rows, dtype=torch.int32).cuda())
+    kd, vd = (values(c, dim).repeat_interleave(q_heads // 2, 1) for c in (kc, vc))
+    w = torch.softmax(torch.einsum("bhd,bhnd->bhn", q.double().cpu(), kd) * dim ** -0.5, 2)
+    assert float(w[:, :, ::97].sum(2).max()) * far < 2.0 ** -40
+    want = torch.einsum("bhn,bhnd->bhd", w, vd)
+    assert float((out.double().cpu() - want).norm()) <= 1.05 * float((want.to(DTYPES[dtype]).double() - want).norm())
