@@ -519,6 +519,7 @@ typedef struct qmk_packed_attention {
   long long q_seq_stride, q_head_stride;
   const int *lens;                   /* DEVICE, one per sequence */
   float scale;
+  int no_overlap;                    /* 1: the call's kernels strictly one after the other, as qmk_set_step_overlap(0) has those of a step */
   void *out;                         /* [num_sequences][q_heads][head_dim], contiguous */
   float *lse;                        /* [num_sequences][q_heads], may be null */
   void *workspace;

@@ -129,8 +129,8 @@ long long workspace_bytes(const Cut &cut, int group, int dim) { return 2ll * cut
 
 // How the parts are joined goes by how many an item has where all stretches or pairs are used: warps (of stretches), or CTAs of four, eight or 32 warps.
 template <typename T, int DIM>
-cudaError_t launch_join(const AttendParams &p, cudaStream_t stream) {
-  const qmk_tc::PdlScope scope(true);
+cudaError_t launch_join(const AttendParams &p, bool overlap, cudaStream_t stream) {
+  const qmk_tc::PdlScope scope(overlap);
   const int rows = p.caches.seqs * p.q_heads, each = p.warps / (p.caches.seqs * p.caches.kv_heads);
   if (each <= FEW && p.ranks == 0) {
     const int units = std::max(p.warps * p.group, p.caches.seqs);
@@ -178,7 +178,7 @@ cudaError_t launch_tiles(const AttendParams &p, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, attend_items<A>, p);
 }
 template <typename T, int DIM, int BITS>
-cudaError_t attend(const AttendParams &p, cudaStream_t stream) {
+cudaError_t attend(const AttendParams &p, bool overlap, cudaStream_t stream) {
   cudaError_t e = cudaSuccess;
   if (p.caches.rows > 0 || p.ranks > 0) {
     switch (way_of(p.group)) {
@@ -188,12 +188,12 @@ cudaError_t attend(const AttendParams &p, cudaStream_t stream) {
       case TWO: e = launch_tiles<Attend<T, DIM, BITS, 2>>(p, stream); break;
     }
   }
-  return e != cudaSuccess || p.warps == 0 ? e : launch_join<T, DIM>(p, stream);
+  return e != cudaSuccess || p.warps == 0 ? e : launch_join<T, DIM>(p, overlap, stream);
 }
 template <typename T>
-cudaError_t attend(const AttendParams &p, int dim, int bits, cudaStream_t stream) {
-  if (bits == 4) return dim == 64 ? attend<T, 64, 4>(p, stream) : attend<T, 128, 4>(p, stream);
-  return dim == 64 ? attend<T, 64, 8>(p, stream) : attend<T, 128, 8>(p, stream);
+cudaError_t attend(const AttendParams &p, int dim, int bits, bool overlap, cudaStream_t stream) {
+  if (bits == 4) return dim == 64 ? attend<T, 64, 4>(p, overlap, stream) : attend<T, 128, 4>(p, overlap, stream);
+  return dim == 64 ? attend<T, 64, 8>(p, overlap, stream) : attend<T, 128, 8>(p, overlap, stream);
 }
 
 }  // namespace
@@ -241,5 +241,6 @@ extern "C" int qmk_attention_packed_cache(const qmk_packed_cache *cache, const q
   p.part_ml = reinterpret_cast<float2 *>(p.part_out + 2ll * p.warps * p.group * cache->head_dim);
   p.out = a->out;
   p.lse = a->lse;
-  return answer(who, a->type == 0 ? attend<__half>(p, cache->head_dim, cache->bits, stream) : attend<__nv_bfloat16>(p, cache->head_dim, cache->bits, stream));
+  return answer(who, a->type == 0 ? attend<__half>(p, cache->head_dim, cache->bits, a->no_overlap == 0, stream)
+                                  : attend<__nv_bfloat16>(p, cache->head_dim, cache->bits, a->no_overlap == 0, stream));
 }

@@ -131,11 +131,11 @@ class _PackedRows(ctypes.Structure):
 
 
 class _PackedAttention(ctypes.Structure):
-    _fields_ = [("type", _I), ("q_heads", _I), ("q", _P), ("q_seq_stride", _LL), ("q_head_stride", _LL), ("lens", _P), ("scale", _F), ("out", _P), ("lse", _P),
-                ("workspace", _P), ("workspace_bytes", _LL)]
+    _fields_ = [("type", _I), ("q_heads", _I), ("q", _P), ("q_seq_stride", _LL), ("q_head_stride", _LL), ("lens", _P), ("scale", _F), ("no_overlap", _I), ("out", _P),
+                ("lse", _P), ("workspace", _P), ("workspace_bytes", _LL)]
 
 
-_pack_packed_cache, _pack_packed_rows, _pack_packed_attention = (struct.Struct(f) for f in ("@5i 4P3q", "@2i 2P3q 2Pi0q", "@2i P2q P f 3Pq"))
+_pack_packed_cache, _pack_packed_rows, _pack_packed_attention = (struct.Struct(f) for f in ("@5i 4P3q", "@2i 2P3q 2Pi0q", "@2i P2q P fi 3Pq"))
 for _made, _fields in ((_pack_packed_cache, _PackedCache), (_pack_packed_rows, _PackedRows), (_pack_packed_attention, _PackedAttention)):
     assert _made.size == ctypes.sizeof(_fields)
 _pack_packed_cache, _pack_packed_rows, _pack_packed_attention = _pack_packed_cache.pack, _pack_packed_rows.pack, _pack_packed_attention.pack
@@ -997,7 +997,7 @@ def attention_packed_cache(q: torch.Tensor, k_cache, v_cache, lens: torch.Tensor
     lse = torch.empty(n, q_heads, dtype=_FP32, device=q.device)
     need = _packed_attention_workspace(n, q_heads, heads, dim, bits, rows)
     workspace = lens.new_empty(need >> 2) if need else None
-    args = _pack_packed_attention(code, q_heads, q.data_ptr(), strides[0], strides[1], seen, dim ** -0.5 if scale is None else scale, out.data_ptr(), lse.data_ptr(),
+    args = _pack_packed_attention(code, q_heads, q.data_ptr(), strides[0], strides[1], seen, dim ** -0.5 if scale is None else scale, 0, out.data_ptr(), lse.data_ptr(),
                                   workspace.data_ptr() if need else 0, need)
     rc = _on_device(index, _lib.qmk_attention_packed_cache, cache, args)
     if rc != 0:

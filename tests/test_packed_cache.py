@@ -883,3 +883,37 @@ def test_rows_beside_much_larger_ones(gpu, dim, bits, q_heads, far, dtype):
     assert float(w[:, :, ::97].sum(2).max()) * far < 2.0 ** -40
     want = torch.einsum("bhn,bhnd->bhd", w, vd)
     assert float((out.double().cpu() - want).norm()) <= 1.05 * float((want.to(DTYPES[dtype]).double() - want).norm())
+
+
+# ------------------------------------------------------------------------------------------------------------- the kernels of a call
+def edges_of(graph):
+    """Types of a captured graph's edges (cudaGraphEdgeData; 1: programmatic)."""
+    class Edge(ctypes.Structure):
+        _fields_ = [("from_port", ctypes.c_ubyte), ("to_port", ctypes.c_ubyte), ("type", ctypes.c_ubyte), ("reserved", ctypes.c_ubyte * 5)]
+    nodes, edges, count = ((ctypes.c_void_p * 8)() for _ in range(2)), (Edge * 8)(), ctypes.c_size_t(8)
+    assert ctypes.CDLL("libcudart.so.12").cudaGraphGetEdges_v2(ctypes.c_void_p(graph.raw_cuda_graph()), *nodes, edges, ctypes.byref(count)) == 0
+    return [e.type for e in edges[:count.value]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs,room,kernels", [(3, 100, 1), (2, 20000, 2), (40, 20000, 2)])
+def test_kernels_of_a_call_one_after_the_other(gpu, seqs, room, kernels):
+    """``no_overlap``: no edge between the call's kernels is a programmatic one, which it is without it; the same bits."""
+    q, kc, vc = attention_inputs(seqs, 16, 8, 128, 4, 100)
+    kc, vc = with_room(kc, room), with_room(vc, room)
+    lens = torch.tensor([(37 * i) % 101 for i in range(seqs)], dtype=torch.int32).cuda()
+    want = gpu.attention_packed_cache(q, kc, vc, lens)
+    out, lse = torch.empty_like(q), torch.empty(seqs, 16, device="cuda")
+    need = gpu._lib.qmk_attention_packed_cache_workspace(seqs, 16, 8, 128, 4, room)
+    workspace = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+    cache = cache_args(gpu, num_sequences=seqs, rows=room, k=None, v=None, k_base=kc.data_ptr(), v_base=vc.data_ptr(), seq_stride=8 * room * 80, head_stride=room * 80)
+    for serial in (0, 1):
+        a = attention_args(gpu, q=q.data_ptr(), lens=lens.data_ptr(), scale=128 ** -0.5, no_overlap=serial, out=out.data_ptr(), lse=lse.data_ptr(), workspace=workspace.data_ptr(), workspace_bytes=need)
+        graph = torch.cuda.CUDAGraph(keep_graph=True)
+        with torch.cuda.graph(graph):
+            assert gpu._lib.qmk_attention_packed_cache(bytes(cache), bytes(a), torch.cuda.current_stream().cuda_stream) == 0
+        assert edges_of(graph) == [0 if serial else 1] * (kernels - 1)
+        graph.instantiate()
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
