@@ -180,7 +180,8 @@ cudaError_t launch_tiles(const AttendParams &p, cudaStream_t stream) {
 template <typename T, int DIM, int BITS>
 cudaError_t attend(const AttendParams &p, bool overlap, cudaStream_t stream) {
   cudaError_t e = cudaSuccess;
-  if (p.caches.rows > 0 || p.ranks > 0) {
+  const bool tiles = p.caches.rows > 0 || p.ranks > 0;
+  if (tiles) {
     switch (way_of(p.group)) {
       case PAIR: e = launch_tiles<AttendPair<T, DIM, BITS>>(p, stream); break;
       case QUAD: e = launch_tiles<AttendQuad<T, DIM, BITS>>(p, stream); break;
@@ -188,7 +189,7 @@ cudaError_t attend(const AttendParams &p, bool overlap, cudaStream_t stream) {
       case TWO: e = launch_tiles<Attend<T, DIM, BITS, 2>>(p, stream); break;
     }
   }
-  return e != cudaSuccess || p.warps == 0 ? e : launch_join<T, DIM>(p, overlap, stream);
+  return e != cudaSuccess || p.warps == 0 ? e : launch_join<T, DIM>(p, overlap && tiles, stream);    // (alone, it would not wait for the kernel of another call in front of it)
 }
 template <typename T>
 cudaError_t attend(const AttendParams &p, int dim, int bits, bool overlap, cudaStream_t stream) {

@@ -917,3 +917,21 @@ def test_kernels_of_a_call_one_after_the_other(gpu, seqs, room, kernels):
         out.zero_()
         graph.replay()
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+@pytest.mark.gpu
+def test_a_call_without_rows_waits_for_the_kernel_before_it(gpu):
+    """More items than clusters take and caches of no rows: one kernel, which writes zeros, no programmatic dependent of what runs before the call."""
+    q = made(128, 40, 64)
+    kc = torch.empty(128, 20, 0, 48, dtype=torch.uint8, device="cuda")
+    lens = torch.full((128,), 5, dtype=torch.int32, device="cuda")
+    gpu.attention_packed_cache(q, kc, kc, lens)
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        lens.add_(1)
+        out, lse = gpu.attention_packed_cache(q, kc, kc, lens)
+    assert edges_of(graph) == [0]
+    graph.instantiate()
+    out.fill_(1.0)
+    graph.replay()
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
