@@ -48,9 +48,11 @@ const char *read_cache(const qmk_packed_cache *a, Caches *c) {
   c->head = a->head_stride;
   c->row = a->row_stride;
   for (int b = 0; b < a->num_sequences; ++b) {
+    c->k[b] = c->v[b] = nullptr;
+    if (a->rows == 0) continue;                  // (no address is looked at)
     c->k[b] = static_cast<const unsigned char *>(a->k ? a->k[b] : static_cast<const char *>(a->k_base) + b * a->seq_stride);
     c->v[b] = static_cast<const unsigned char *>(a->k ? a->v[b] : static_cast<const char *>(a->v_base) + b * a->seq_stride);
-    if (a->rows > 0 && (!c->k[b] || !c->v[b])) return "null pointer argument";
+    if (!c->k[b] || !c->v[b]) return "null pointer argument";
     if (odd(c->k[b]) || odd(c->v[b])) return "a cache's address must be a multiple of 16";
   }
   return nullptr;

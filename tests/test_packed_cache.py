@@ -935,3 +935,13 @@ def test_a_call_without_rows_waits_for_the_kernel_before_it(gpu):
     out.fill_(1.0)
     graph.replay()
     assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+
+
+def test_no_address_of_a_cache_without_rows_is_looked_at(C):
+    """Host arrays or bases that are not there: the calls go on to their next check, or have nothing to do."""
+    for where in (dict(v=None), dict(k=None), dict(k=None, v=None), dict(k=None, v=None, k_base=None, v_base=None)):
+        cache = cache_args(C, rows=0, **where)
+        for name in ("qmk_write_cache_packed", "qmk_read_cache_packed"):
+            assert call(C, name, cache, row_args(C, rows=0))[0] == 0
+        rc, why = call(C, "qmk_attention_packed_cache", cache, attention_args(C, scale=math.inf))
+        assert rc == 2 and b"scale" in why
