@@ -16,6 +16,7 @@ using namespace qmk_packed;
 
 constexpr int MAX_ROWS = 1 << 24;                // of a cache
 constexpr int MAX_HEADS = 1024;
+constexpr long long MAX_TILES = 0x7ffffff0;       // of all sequences and heads: a warp counts up to three past its last one
 constexpr int MAX_RANKS = 4;                     // clusters of 2^(4 - 1) CTAs
 
 int refuse(const char *who, const std::string &why) {
@@ -212,7 +213,7 @@ extern "C" long long qmk_attention_packed_cache_workspace(int num_sequences, int
   if (num_sequences < 1 || num_sequences > MAX_SEQS || kv_heads < 1 || kv_heads > MAX_HEADS || q_heads < 1 || q_heads % kv_heads || q_heads / kv_heads > MAX_GROUP ||
       (head_dim != 64 && head_dim != 128) || (bits != 4 && bits != 8) || rows < 0 || rows > MAX_ROWS)
     return -1;
-  if (most_tiles(num_sequences, kv_heads, rows) > 0x7fffffffll) return -1;
+  if (most_tiles(num_sequences, kv_heads, rows) > MAX_TILES) return -1;
   return workspace_bytes(cut_of(num_sequences, kv_heads, q_heads / kv_heads, head_dim, bits, rows), q_heads / kv_heads, head_dim);
 }
 
@@ -224,7 +225,7 @@ extern "C" int qmk_attention_packed_cache(const qmk_packed_cache *cache, const q
   if (!a || !a->q || !a->out || !a->lens) return refuse(who, "null pointer argument");
   if (a->type < 0 || a->type > 1) return refuse(who, "the type is fp16 (0) or bf16 (1)");
   if (a->q_heads < 1 || a->q_heads % cache->kv_heads || a->q_heads / cache->kv_heads > MAX_GROUP) return refuse(who, "q_heads must be 1 to 16 times kv_heads");
-  if (most_tiles(cache->num_sequences, cache->kv_heads, cache->rows) > 0x7fffffffll) return refuse(who, "2^36 rows of all heads or more");
+  if (most_tiles(cache->num_sequences, cache->kv_heads, cache->rows) > MAX_TILES) return refuse(who, "2^36 rows of all heads (512 less), or more");
   if (!(a->scale > -2.0e38f && a->scale < 2.0e38f)) return refuse(who, "the scale must be finite, and below 2e38");   // (times log2 e too)
   if (odd(a->q) || odd(a->out) || odd(a->workspace)) return refuse(who, "pointers must be 16-byte aligned");
   if (odd(a->q_seq_stride, cache->num_sequences, 8) || odd(a->q_head_stride, a->q_heads, 8)) return refuse(who, "the queries' strides must be multiples of 8 elements");

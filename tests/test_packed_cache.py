@@ -945,3 +945,13 @@ def test_no_address_of_a_cache_without_rows_is_looked_at(C):
             assert call(C, name, cache, row_args(C, rows=0))[0] == 0
         rc, why = call(C, "qmk_attention_packed_cache", cache, attention_args(C, scale=math.inf))
         assert rc == 2 and b"scale" in why
+
+
+@pytest.mark.parametrize("seqs,heads,tiles", [(42, 341, 149943), (1, 1, 1), (127, 129, 131081)])
+def test_the_most_rows_of_all_heads(C, seqs, heads, tiles):
+    """Caches shared by sequences and heads (strides of 0) may have this many rows: 2^31 - 2 tiles of 32 rows, which a warp's count would pass, are refused; fewer go on to the next check."""
+    many = seqs * heads * tiles > 2 ** 31 - 16
+    cache = cache_args(C, num_sequences=seqs, kv_heads=heads, rows=32 * tiles, head_stride=0)
+    rc, why = call(C, "qmk_attention_packed_cache", cache, attention_args(C, q_heads=heads, scale=math.inf))
+    assert rc == 2 and (b"2^36" if many else b"scale") in why
+    assert (C._lib.qmk_attention_packed_cache_workspace(seqs, heads, heads, 128, 4, 32 * tiles) < 0) == many
