@@ -503,9 +503,10 @@ typedef struct qmk_packed_rows {
   int start;
 } qmk_packed_rows;
 /* Quantises the rows into the caches; those that fall outside a cache or behind lens[b] are left out, all other rows of the caches stay as they are.  Two
- * rows of one call must not fall on the same row of a cache.  Does not block, allocates nothing, may be captured. */
+ * rows of one call must not fall on the same row of a cache (refused where strides or addresses alone say that they do).  Does not block, allocates nothing, may be captured. */
 int qmk_write_cache_packed(const qmk_packed_cache *cache, const qmk_packed_rows *rows, cudaStream_t stream);
-/* The values of the caches' rows, each rounded once to the type (one past the largest fp16 number to that); zeros in rows that are outside a cache or behind lens[b].  Does not block,
+/* The values of the caches' rows, each rounded once to the type (one past the largest fp16 number to that); zeros in rows that are outside a cache or behind lens[b].  The outputs' rows
+ * must not share memory (refused where a stride is 0 or keys and values have one address).  Does not block,
  * allocates nothing, may be captured. */
 int qmk_read_cache_packed(const qmk_packed_cache *cache, const qmk_packed_rows *rows, cudaStream_t stream);
 /* Attention of one new token per sequence over packed caches.  Per sequence b and query head h (kv head h / (q_heads / kv_heads)): out = softmax(scale * q . k) v

@@ -80,6 +80,20 @@ const char *read_rows_of(const qmk_packed_rows *a, RowParams *p) {
   return nullptr;
 }
 
+// Rows that a call would write twice whatever its starts and lengths; null: none
+const char *shared_rows(const Caches &c) {
+  if (c.rows == 0) return nullptr;
+  if (c.kv_heads > 1 && c.head == 0) return "heads share a cache's rows: the head stride is 0";
+  for (int b = 0; b < c.seqs; ++b)
+    if (c.k[b] == c.v[b]) return "keys and values share a cache";
+  return nullptr;
+}
+const char *shared_rows(const RowParams &p) {
+  if (p.k == p.v) return "keys and values share rows";
+  if ((p.caches.seqs > 1 && p.seq == 0) || (p.caches.kv_heads > 1 && p.head == 0) || (p.rows > 1 && p.row == 0)) return "rows share memory: a stride is 0";
+  return nullptr;
+}
+
 template <typename T, int DIM, int BITS>
 void (*row_kernel(bool write))(RowParams, unsigned int) { return write ? write_rows<T, DIM, BITS> : read_rows<T, DIM, BITS>; }
 template <typename T>
@@ -95,6 +109,7 @@ int rows_call(const char *who, const qmk_packed_cache *cache, const qmk_packed_r
   if (const char *why = read_rows_of(rows, &p)) return refuse(who, why);
   const unsigned int count = static_cast<unsigned int>(p.caches.seqs) * p.caches.kv_heads * p.rows;
   if (count == 0) return QMK_OK;
+  if (const char *why = write ? shared_rows(p.caches) : shared_rows(p)) return refuse(who, why);
   p.by_rows.set(p.rows);
   p.by_heads.set(p.caches.kv_heads);
   // (CTAs: 4 x 4096 rows of 8 heads written by four an SM for keys and four for values 20.6 us, by eight 20.8, by sixteen 21.9; 28 x 4096 read by 64 an SM 104, by sixteen 109, by eight 124)

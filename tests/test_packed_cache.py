@@ -955,3 +955,40 @@ def test_the_most_rows_of_all_heads(C, seqs, heads, tiles):
     rc, why = call(C, "qmk_attention_packed_cache", cache, attention_args(C, q_heads=heads, scale=math.inf))
     assert rc == 2 and (b"2^36" if many else b"scale") in why
     assert (C._lib.qmk_attention_packed_cache_workspace(seqs, heads, heads, 128, 4, 32 * tiles) < 0) == many
+
+
+def two_places(C, **change):
+    return cache_args(C, **{**dict(k=None, v=None, k_base=1 << 20, v_base=1 << 21, seq_stride=1 << 16), **change})
+
+
+@pytest.mark.parametrize("change", [dict(head_stride=0), dict(v_base=1 << 20)])
+def test_caches_whose_rows_would_be_written_twice_are_refused(C, change):
+    rc, why = call(C, "qmk_write_cache_packed", two_places(C, **change), row_args(C))
+    assert rc == 2 and b"share" in why
+    assert call(C, "qmk_write_cache_packed", two_places(C, **change), row_args(C, rows=0))[0] == 0
+    one = (ctypes.c_void_p * 2)(1 << 20, 1 << 21), (ctypes.c_void_p * 2)(1 << 22, 1 << 21)
+    rc, why = call(C, "qmk_write_cache_packed", cache_args(C, k=ctypes.addressof(one[0]), v=ctypes.addressof(one[1])), row_args(C))
+    assert rc == 2 and b"share" in why
+
+
+@pytest.mark.parametrize("change", [dict(v=4096), dict(seq_stride=0), dict(head_stride=0), dict(row_stride=0)])
+def test_outputs_whose_rows_share_memory_are_refused(C, change):
+    rc, why = call(C, "qmk_read_cache_packed", two_places(C), row_args(C, **{**dict(v=1 << 20), **change}))
+    assert rc == 2 and b"share" in why
+
+
+@pytest.mark.gpu
+def test_rows_and_caches_that_may_be_shared(gpu):
+    """One row for all heads, sequences and positions written, one cache read for all sequences and by keys and values alike, rows of sequences side by side in one cache."""
+    size = gpu.packed_row_bytes(64, 4)
+    row, kc, vc = made(1, 1, 1, 64), *(torch.zeros(3, 2, 12, size, dtype=torch.uint8, device="cuda") for _ in range(2))
+    same = row.expand(3, 2, 4, 64)
+    gpu.write_cache_packed(same, same, kc, vc, 5)
+    assert torch.equal(kc[:, :, 5:9].cpu(), packed(row, 4).expand(3, 2, 4, size)) and torch.equal(kc, vc)
+    k, v = gpu.read_cache_packed(kc[:1].expand(3, -1, -1, -1), kc[:1].expand(3, -1, -1, -1), 4, 64, starts=5)
+    want = values(packed(row, 4), 64).expand(3, 2, 4, 64)
+    assert torch.equal(k, v) and bool(((k.double().cpu() - want).abs() <= rounded_off(want, torch.float16)).all())
+    rows = made(3, 2, 4, 64, seed=2)
+    gpu.write_cache_packed(rows, rows, kc[:1].expand(3, -1, -1, -1), vc[:1].expand(3, -1, -1, -1), torch.tensor([8, 0, 4], dtype=torch.int32).cuda())
+    for b, at in enumerate((8, 0, 4)):
+        assert torch.equal(kc[0, :, at:at + 4].cpu(), packed(rows[b], 4)) and torch.equal(vc[0], kc[0])
