@@ -881,11 +881,13 @@ def _packed_cache(who, k_cache, v_cache, n, dim, index):
         k_ptrs, v_ptrs, k_base, v_base = ctypes.addressof(keep[0]), ctypes.addressof(keep[1]), 0, 0
     if not (like and last == 1 and index >= 0):
         raise RuntimeError(f"{who}: packed caches must be uint8 CUDA tensors on the same device, contiguous within a row, and of the same shape and strides")
-    bits = (row_bytes - PACKED_TRAILER_BYTES) * 8 // dim
-    if dim not in (64, 128) or bits not in (4, 8) or row_bytes != dim * bits // 8 + PACKED_TRAILER_BYTES:
+    bits = (row_bytes - PACKED_TRAILER_BYTES) * 8 // dim if dim in (64, 128) else 0
+    if bits not in (4, 8) or row_bytes != dim * bits // 8 + PACKED_TRAILER_BYTES:
         raise RuntimeError(f"{who}: no packed row of {dim} values has {row_bytes} bytes (packed_row_bytes)")
     if not 1 <= n <= MAX_PACKED_SEQUENCES:
         raise RuntimeError(f"{who}: 1 to {MAX_PACKED_SEQUENCES} sequences per call")
+    if max(heads, rows) > _INT_MAX:
+        raise RuntimeError(f"{who}: more heads or rows than 32 bits hold")
     return _pack_packed_cache(bits, dim, n, heads, rows, k_ptrs, v_ptrs, k_base, v_base, seq, head, row), n, heads, rows, bits, keep
 
 
@@ -993,6 +995,8 @@ def attention_packed_cache(q: torch.Tensor, k_cache, v_cache, lens: torch.Tensor
     seen = _per_sequence(who, lens, n, index, "lens")
     if not seen:
         raise RuntimeError(f"{who}: lens must be a contiguous int32 tensor with one value per sequence on the caches' device")
+    if scale is not None and not -2e38 < scale < 2e38:
+        raise RuntimeError(f"{who}: the scale must be finite, and below 2e38")
     out = torch.empty_like(q) if q.is_contiguous() else torch.empty(n, q_heads, dim, dtype=dtype, device=q.device)
     lse = torch.empty(n, q_heads, dtype=_FP32, device=q.device)
     need = _packed_attention_workspace(n, q_heads, heads, dim, bits, rows)

@@ -992,3 +992,18 @@ def test_rows_and_caches_that_may_be_shared(gpu):
     gpu.write_cache_packed(rows, rows, kc[:1].expand(3, -1, -1, -1), vc[:1].expand(3, -1, -1, -1), torch.tensor([8, 0, 4], dtype=torch.int32).cuda())
     for b, at in enumerate((8, 0, 4)):
         assert torch.equal(kc[0, :, at:at + 4].cpu(), packed(rows[b], 4)) and torch.equal(vc[0], kc[0])
+
+
+@pytest.mark.gpu
+def test_sizes_and_scales_that_no_structure_holds_are_refused(gpu):
+    q, kc, vc = attention_inputs(2, 4, 2, 64, 4, 8)
+    lens = torch.tensor([1, 2], dtype=torch.int32).cuda()
+    many = kc[:1, :1, :1].expand(1, 1, 2 ** 31, -1), vc[:1, :1, :1].expand(1, 1, 2 ** 31, -1)
+    for scale in (1e39, -1e300, math.inf, math.nan, 3e38):
+        with pytest.raises(RuntimeError, match="scale"):
+            gpu.attention_packed_cache(q, kc, vc, lens, scale=scale)
+    none = torch.empty(2, 4, 0, dtype=torch.float16, device="cuda")
+    for call in (lambda: gpu.attention_packed_cache(none, kc, vc, lens), lambda: gpu.write_cache_packed(none[:, :2, None], none[:, :2, None], kc, vc), lambda: gpu.read_cache_packed(kc, vc, 3, 0),
+                 lambda: gpu.attention_packed_cache(q[:1, :1], *many, lens[:1]), lambda: gpu.read_cache_packed(*many, 3, 64), lambda: gpu.write_cache_packed(made(1, 1, 2, 64), made(1, 1, 2, 64), *many)):
+        with pytest.raises(RuntimeError):
+            call()
