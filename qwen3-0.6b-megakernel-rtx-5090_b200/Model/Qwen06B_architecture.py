@@ -551,6 +551,8 @@ class BatchDecoder:
             raise ValueError("parked sequence exceeds max_seq_len")
         if parked.k.shape[0] != layers:
             raise ValueError(f"parked sequence of {parked.k.shape[0]} layers, the decoder has {layers}")
+        if not 0 <= length <= parked.k.shape[2]:
+            raise ValueError(f"parked sequence of length {length} has {parked.k.shape[2]} rows")
         read = _require_megakernel_op("read_cache_packed")
         for first in range(0, layers if length else 0, 128):
             part = slice(first, first + 128)

@@ -1007,3 +1007,21 @@ def test_sizes_and_scales_that_no_structure_holds_are_refused(gpu):
                  lambda: gpu.attention_packed_cache(q[:1, :1], *many, lens[:1]), lambda: gpu.read_cache_packed(*many, 3, 64), lambda: gpu.write_cache_packed(made(1, 1, 2, 64), made(1, 1, 2, 64), *many)):
         with pytest.raises(RuntimeError):
             call()
+
+
+@pytest.mark.gpu
+def test_a_parked_sequence_is_resumed_up_to_its_rows(gpu):
+    """Fewer rows than were parked come back if asked for; more than there are, which would read as zeros, are refused and change nothing."""
+    import synthetic as S
+    from Model.Qwen06B_architecture import BatchDecoder
+    w = S.make_weights(seed=31, num_layers=2, vocab_size=2048, norm_std=0.1, max_seq_len=16)
+    eng = BatchDecoder(weights=S.weights_to(w, "cuda"), tokenizer=S.StubTokenizer(-1, 2048), num_sequences=2, max_seq_len=96, engine="gemm", prefill_mode="tensor")
+    eng.prefill_slot(0, S.make_prompt(30, seed=3, vocab_size=2048))
+    parked = eng.park_slot(0)
+    before = eng._k_caches[1].clone()
+    for length in (31, 96, -1):
+        with pytest.raises(ValueError):
+            eng.resume_slot(1, parked._replace(length=length))
+    assert eng.positions == [30, 0] and torch.equal(eng._k_caches[1], before)
+    eng.resume_slot(1, parked._replace(length=20))
+    assert eng.positions == [30, 20] and torch.equal(eng._k_caches[1][:, :, 20:], before[:, :, 20:]) and not torch.equal(eng._k_caches[1][:, :, :20], before[:, :, :20])
