@@ -10,8 +10,8 @@
 //
 // Roundings: queries are taken to fp16 times a power of two (Tiles::lift).  Weights and their products with scales are carried as two fp16 numbers each, because the tensor cores multiply
 // 16-bit numbers: over many outputs the error against 64 bits is 1.00 to 1.01 times that of rounding the exact result (1.06 to 1.36 times with one number a product, which took 16 of up to 2048
-// rows 12.8 us, 128 of up to 8192 122, 96 of 8192 160 and 32 of up to 4096 with sixteen heads a kv head 23.5, where two take 13.6, 125, 175 and 27.9).  One each where the output is
-// bf16, whose own rounding is eight times theirs: 1.00 to 1.01 times too.  Sums, softmax statistics and outputs are fp32.  Every second 16 rows go in as 2^BITS - 1 - n with the
+// rows 12.8 us, 128 of up to 8192 122, 96 of 8192 160 and 32 of up to 4096 with sixteen heads a kv head 23.5, where two take 13.6, 125, 175 and 27.9).  So for bf16 outputs: with one number each
+// an output whose terms cancel is off by up to 2^-10 of these.  Sums, softmax statistics and outputs are fp32.  Every second 16 rows go in as 2^BITS - 1 - n with the
 // weights' sign turned (the same instructions): the running sums stay around zero, whose size the accumulator's truncation goes by.
 //
 // Work: tiles of 32 rows, a tile to a warp, each with a ring of copies of its own (cp.async: no waits but for its own copies).  attend_items: a cluster of CTAs has a (sequence, kv
@@ -299,23 +299,21 @@ struct Tiles {
     const int e = static_cast<int>((__float_as_uint(fmaxf(most, 0.0f)) + 0x7fffffu) >> 23) - 127;
     return fminf(old, power2(min(max(-e, -14), 15)));
   }
-  // Two rows' weights (upper and lower parts) times scales, as upper and, of an output in fp16, lower parts
-  template <bool LOWER, bool FLIP>
+  // Two rows' weights times scales, all as upper and lower fp16 parts
+  template <bool FLIP>
   static __device__ __forceinline__ void times(uint32_t hi, uint32_t lo, __half2 scales, uint32_t &upper, uint32_t &lower) {
     const __half2 s = FLIP ? __hneg2(scales) : scales, first = __hmul2(h2(hi), s);
     upper = bits_of(first);
-    if constexpr (LOWER) lower = bits_of(__hfma2(h2(lo), s, __hfma2(h2(hi), s, __hneg2(first))));
+    lower = bits_of(__hfma2(h2(lo), s, __hfma2(h2(hi), s, __hneg2(first))));
   }
   // The same where one of the powers of two is below 1, a scale above 1 having been seen: fp16 might not hold small scales times it, so they come as they are and it apart
-  template <bool LOWER, bool FLIP>
+  template <bool FLIP>
   static __device__ __forceinline__ void times(uint32_t hi, uint32_t lo, __half2 scales, float power, uint32_t &upper, uint32_t &lower) {
     const float2 a = __half22float2(h2(hi)), b = __half22float2(h2(lo)), s = __half22float2(scales);
     const float by = FLIP ? -power : power, x = (a.x + b.x) * s.x * by, y = (a.y + b.y) * s.y * by;
     upper = pack2(x, y);
-    if constexpr (LOWER) {
-      const float2 back = __half22float2(h2(upper));
-      lower = pack2(x - back.x, y - back.y);
-    }
+    const float2 back = __half22float2(h2(upper));
+    lower = pack2(x - back.x, y - back.y);
   }
 };
 
@@ -349,12 +347,9 @@ __device__ __forceinline__ void take_tile(A &a, uint32_t kt, int rows, int lane)
       const float w = exp2_fast(fmaf(x[h][r] - a.m, a.factor, SHIFT));
       a.l += w;
       const uint32_t upper = pack2(w, w);
+      const float rest = w - __low2float(h2(upper));
       hi[r] = transposed(upper);
-      lo[r] = 0u;
-      if constexpr (A::LOWER) {
-        const float rest = w - __low2float(h2(upper));
-        lo[r] = transposed(pack2(rest, rest));
-      }
+      lo[r] = transposed(pack2(rest, rest));
     }
     if (h == 0) a.template weigh<false>(vt, lane, hi, lo);
     else a.template weigh<true>(vt + 16 * ROW, lane, hi, lo);
@@ -369,7 +364,6 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
   using Value = T;
   using Base = Tiles<DIM, BITS, PAIR, 2>;
   using Base::ROW; using Base::CODES; using Base::N; using Base::J; using Base::STEPS; using Base::M; using Base::UNIT; using Base::CHUNK;
-  static constexpr bool LOWER = !Type<T>::BF16;            // whether weights have a lower part
   static constexpr int PAIRS = 16 / BITS, KSTEPS = N * PAIRS;               // operand words of a word of codes; k steps of a row of keys
 
   uint32_t qb[KSTEPS][2], qz[2];                 // queries; sums over quarters, as upper and lower fp16 parts
@@ -504,14 +498,14 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
       s0 = __hmul2(h2(r0), f);
       s1 = __hmul2(h2(r1), f);
     }
-    Base::template times<LOWER, FLIP>(hi[0], lo[0], s0, pb[0], pl[0]);
-    Base::template times<LOWER, FLIP>(hi[1], lo[1], s1, pb[1], pl[1]);
+    Base::template times<FLIP>(hi[0], lo[0], s0, pb[0], pl[0]);
+    Base::template times<FLIP>(hi[1], lo[1], s1, pb[1], pl[1]);
     if (wide) {
-      Base::template times<LOWER, FLIP>(hi[0], lo[0], h2(r0), __low2float(f), pb[0], pl[0]);
-      Base::template times<LOWER, FLIP>(hi[1], lo[1], h2(r1), __low2float(f), pb[1], pl[1]);
+      Base::template times<FLIP>(hi[0], lo[0], h2(r0), __low2float(f), pb[0], pl[0]);
+      Base::template times<FLIP>(hi[1], lo[1], h2(r1), __low2float(f), pb[1], pl[1]);
     }
     mma(sums, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pb[0], pb[1], sums[0], sums[1], sums[2], sums[3]);
-    if constexpr (LOWER) mma(sums, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pl[0], pl[1], sums[0], sums[1], sums[2], sums[3]);
+    mma(sums, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pl[0], pl[1], sums[0], sums[1], sums[2], sums[3]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t first[J], second[J];
@@ -521,11 +515,11 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
       for (int u = 0; u < STEPS; ++u) {
         float (&c)[4] = acc[i][u];
         mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pb[0], pb[1], c[0], c[1], c[2], c[3]);
-        if constexpr (LOWER) mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pl[0], pl[1], c[0], c[1], c[2], c[3]);
+        mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pl[0], pl[1], c[0], c[1], c[2], c[3]);
       }
     }
     mma(zacc, raw[0], raw[1], raw[2], raw[3], hi[0], hi[1], zacc[0], zacc[1], zacc[2], zacc[3]);
-    if constexpr (LOWER) mma(zacc, raw[0], raw[1], raw[2], raw[3], lo[0], lo[1], zacc[0], zacc[1], zacc[2], zacc[3]);
+    mma(zacc, raw[0], raw[1], raw[2], raw[3], lo[0], lo[1], zacc[0], zacc[1], zacc[2], zacc[3]);
   }
 
   // All there is of the head scaled: its maximum has moved
@@ -579,7 +573,6 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
   using Value = T;
   using Base = Tiles<DIM, BITS, QUAD, 4>;
   using Base::ROW; using Base::CODES; using Base::N; using Base::J; using Base::STEPS; using Base::M; using Base::UNIT; using Base::CHUNK;
-  static constexpr bool LOWER = !Type<T>::BF16;            // whether weights have a lower part
 
   uint32_t qb[2][STEPS][2], qz[2];               // queries of the column's even and odd quarter; sums over quarters, as upper and lower fp16 parts
   float factor, m, l;                            // what a score is multiplied by, the largest score, the sum of weights; of head t
@@ -711,23 +704,23 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
     for (int i = 0; i < 2; ++i) {                // quarter 2 (g & 1) + i
       const int from = 8 * (g & 1) + 4 * i + t;
       const __half2 a0 = h2(__shfl_sync(0xffffffffu, bits_of(s0), from)), a1 = h2(__shfl_sync(0xffffffffu, bits_of(s1), from));
-      Base::template times<LOWER, FLIP>(hi[0], lo[0], a0, pb[i][0], pl[i][0]);
-      Base::template times<LOWER, FLIP>(hi[1], lo[1], a1, pb[i][1], pl[i][1]);
+      Base::template times<FLIP>(hi[0], lo[0], a0, pb[i][0], pl[i][0]);
+      Base::template times<FLIP>(hi[1], lo[1], a1, pb[i][1], pl[i][1]);
     }
     if (wide) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int from = 8 * (g & 1) + 4 * i + t;
         const float power = __shfl_sync(0xffffffffu, __low2float(f), from);
-        Base::template times<LOWER, FLIP>(hi[0], lo[0], h2(__shfl_sync(0xffffffffu, raw[0], from)), power, pb[i][0], pl[i][0]);
-        Base::template times<LOWER, FLIP>(hi[1], lo[1], h2(__shfl_sync(0xffffffffu, raw[2], from)), power, pb[i][1], pl[i][1]);
+        Base::template times<FLIP>(hi[0], lo[0], h2(__shfl_sync(0xffffffffu, raw[0], from)), power, pb[i][0], pl[i][0]);
+        Base::template times<FLIP>(hi[1], lo[1], h2(__shfl_sync(0xffffffffu, raw[2], from)), power, pb[i][1], pl[i][1]);
       }
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       float (&c)[4] = sums[i];
       mma(c, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pb[i][0], pb[i][1], c[0], c[1], c[2], c[3]);
-      if constexpr (LOWER) mma(c, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pl[i][0], pl[i][1], c[0], c[1], c[2], c[3]);
+      mma(c, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pl[i][0], pl[i][1], c[0], c[1], c[2], c[3]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -738,11 +731,11 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
       for (int u = 0; u < STEPS; ++u) {
         float (&c)[4] = acc[i][u];
         mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pb[i % 2][0], pb[i % 2][1], c[0], c[1], c[2], c[3]);
-        if constexpr (LOWER) mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pl[i % 2][0], pl[i % 2][1], c[0], c[1], c[2], c[3]);
+        mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pl[i % 2][0], pl[i % 2][1], c[0], c[1], c[2], c[3]);
       }
     }
     mma(zacc, raw[0], raw[1], raw[2], raw[3], hi[0], hi[1], zacc[0], zacc[1], zacc[2], zacc[3]);
-    if constexpr (LOWER) mma(zacc, raw[0], raw[1], raw[2], raw[3], lo[0], lo[1], zacc[0], zacc[1], zacc[2], zacc[3]);
+    mma(zacc, raw[0], raw[1], raw[2], raw[3], lo[0], lo[1], zacc[0], zacc[1], zacc[2], zacc[3]);
   }
 
   // All there is of head t scaled: its maximum has moved
@@ -792,7 +785,6 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
   using Value = T;
   using Base = Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT>;
   using Base::ROW; using Base::CODES; using Base::N; using Base::J; using Base::STEPS; using Base::M; using Base::UNIT; using Base::CHUNK;
-  static constexpr bool LOWER = !Type<T>::BF16;            // whether weights have a lower part
 
   uint32_t qb[NT][4][STEPS][2], qz[NT][2];       // queries; sums over quarters, as upper and lower fp16 parts
   float factor[NT][2], m[NT][2], l[NT][2];       // of heads 2 t and 2 t + 1: what a score is multiplied by, the largest score, the sum of weights
@@ -942,8 +934,8 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
         const __half2 a0 = h2(__shfl_sync(0xffffffffu, bits_of(s0), from)), a1 = h2(__shfl_sync(0xffffffffu, bits_of(s1), from));
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          Base::template times<LOWER, FLIP>(hi[nt][0], lo[nt][0], a0, pb[k][nt][0], pl[k][nt][0]);
-          Base::template times<LOWER, FLIP>(hi[nt][1], lo[nt][1], a1, pb[k][nt][1], pl[k][nt][1]);
+          Base::template times<FLIP>(hi[nt][0], lo[nt][0], a0, pb[k][nt][0], pl[k][nt][0]);
+          Base::template times<FLIP>(hi[nt][1], lo[nt][1], a1, pb[k][nt][1], pl[k][nt][1]);
         }
       }
       if (wide) {
@@ -954,8 +946,8 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
           const __half2 r0 = h2(__shfl_sync(0xffffffffu, raw[0], from)), r1 = h2(__shfl_sync(0xffffffffu, raw[2], from));
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            Base::template times<LOWER, FLIP>(hi[nt][0], lo[nt][0], r0, power, pb[k][nt][0], pl[k][nt][0]);
-            Base::template times<LOWER, FLIP>(hi[nt][1], lo[nt][1], r1, power, pb[k][nt][1], pl[k][nt][1]);
+            Base::template times<FLIP>(hi[nt][0], lo[nt][0], r0, power, pb[k][nt][0], pl[k][nt][0]);
+            Base::template times<FLIP>(hi[nt][1], lo[nt][1], r1, power, pb[k][nt][1], pl[k][nt][1]);
           }
         }
       }
@@ -967,7 +959,7 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
         for (int nt = 0; nt < NT; ++nt) {
           float (&c)[4] = sums[nt][i];
           mma(c, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pb[k][nt][0], pb[k][nt][1], c[0], c[1], c[2], c[3]);
-          if constexpr (LOWER) mma(c, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pl[k][nt][0], pl[k][nt][1], c[0], c[1], c[2], c[3]);
+          mma(c, MIDDLE, MIDDLE, MIDDLE, MIDDLE, pl[k][nt][0], pl[k][nt][1], c[0], c[1], c[2], c[3]);
         }
         expand<DIM, BITS, FLIP>(w[0], w[1], i, first);
         expand<DIM, BITS, FLIP>(w[2], w[3], i, second);
@@ -977,7 +969,7 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
           for (int nt = 0; nt < NT; ++nt) {
             float (&c)[4] = acc[nt][i][u];
             mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pb[k][nt][0], pb[k][nt][1], c[0], c[1], c[2], c[3]);
-            if constexpr (LOWER) mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pl[k][nt][0], pl[k][nt][1], c[0], c[1], c[2], c[3]);
+            mma(c, first[2 * u], first[2 * u + 1], second[2 * u], second[2 * u + 1], pl[k][nt][0], pl[k][nt][1], c[0], c[1], c[2], c[3]);
           }
       }
     }
@@ -985,7 +977,7 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
     for (int nt = 0; nt < NT; ++nt) {
       float (&c)[4] = zacc[nt];
       mma(c, raw[0], raw[1], raw[2], raw[3], hi[nt][0], hi[nt][1], c[0], c[1], c[2], c[3]);
-      if constexpr (LOWER) mma(c, raw[0], raw[1], raw[2], raw[3], lo[nt][0], lo[nt][1], c[0], c[1], c[2], c[3]);
+      mma(c, raw[0], raw[1], raw[2], raw[3], lo[nt][0], lo[nt][1], c[0], c[1], c[2], c[3]);
     }
   }
 
@@ -1052,12 +1044,9 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const uint32_t upper = pack2(w[2 * r], w[2 * r + 1]);
+          const float2 back = __half22float2(h2(upper));
           hi[nt][r] = transposed(upper);
-          lo[nt][r] = 0u;
-          if constexpr (LOWER) {
-            const float2 back = __half22float2(h2(upper));
-            lo[nt][r] = transposed(pack2(w[2 * r] - back.x, w[2 * r + 1] - back.y));
-          }
+          lo[nt][r] = transposed(pack2(w[2 * r] - back.x, w[2 * r + 1] - back.y));
         }
       }
       if (h == 0) weigh<false>(vt, lane, hi, lo);

@@ -57,7 +57,6 @@ struct RowParams {
 
 template <typename T> struct Type;
 template <> struct Type<__half> {
-  static constexpr bool BF16 = false;
   using Two = __half2;
   static __device__ __forceinline__ float2 floats(Two x) { return __half22float2(x); }
   // (a scale that was rounded up may lead a code past the largest fp16 number: that one then, and not infinity)
@@ -68,7 +67,6 @@ template <> struct Type<__half> {
   }
 };
 template <> struct Type<__nv_bfloat16> {
-  static constexpr bool BF16 = true;
   using Two = __nv_bfloat162;
   static __device__ __forceinline__ float2 floats(Two x) { return __bfloat1622float2(x); }
   static __device__ __forceinline__ uint32_t two(float a, float b) {

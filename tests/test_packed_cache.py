@@ -1025,3 +1025,24 @@ def test_a_parked_sequence_is_resumed_up_to_its_rows(gpu):
     assert eng.positions == [30, 0] and torch.equal(eng._k_caches[1], before)
     eng.resume_slot(1, parked._replace(length=20))
     assert eng.positions == [30, 20] and torch.equal(eng._k_caches[1][:, :, 20:], before[:, :, 20:]) and not torch.equal(eng._k_caches[1][:, :, :20], before[:, :, :20])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("dim,bits", [(64, 4), (64, 8), (128, 4), (128, 8)])
+@pytest.mark.parametrize("q_heads", [4, 8, 16, 32])
+@pytest.mark.parametrize("room", [300, 20000])
+def test_outputs_whose_terms_cancel(gpu, dim, bits, q_heads, room, dtype):
+    """Element by element, behind nearly equal weights, whose scores have next to no error: an output that is small beside the sum A of its terms' sizes is as near.  Weights and
+    products of weights and scales are two fp16 numbers: off by 2^-22 each of the largest weight's size, and of a scale 2^-4 times the largest 2^-18 of its product; the sums as above."""
+    rows, scale = 300, 1e-4
+    q, kc, vc = attention_inputs(3, q_heads, 2, dim, bits, rows, dtype, seed=q_heads + dim)
+    out, _ = gpu.attention_packed_cache(q, with_room(kc, room), with_room(vc, room), torch.full((3,), rows, dtype=torch.int32).cuda(), scale=scale)
+    (kz, ks, kn), (vz, vs, vn) = (tuple(x.repeat_interleave(q_heads // 2, 1) for x in parts(c, dim)) for c in (kc, vc))
+    qd = q.double().cpu()
+    w = torch.softmax(torch.einsum("bhd,bhnd->bhn", qd, kz + ks * kn) * scale, 2)
+    want, a, u = (torch.einsum("bhn,bhnd->bhd", w, x) for x in (vz + vs * vn, vz.abs() + (vs * vn).abs(), vz.abs() + vs * 2 ** bits))
+    ds = dim * 2.0 ** -24 * torch.einsum("bhd,bhnd->bhn", qd.abs(), kz.abs() + ks * 2 ** bits).amax(2, keepdim=True) * scale
+    tol = torch.finfo(q.dtype).eps / 2 * want.abs() + 2.0 ** -18 * a + u * (2 * ds + 2 * (rows / 16 + 2) * 2.0 ** -23 + 2.0 ** -21)
+    err = (out.double().cpu() - want).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
