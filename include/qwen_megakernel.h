@@ -505,7 +505,7 @@ typedef struct qmk_packed_rows {
 /* Quantises the rows into the caches; those that fall outside a cache or behind lens[b] are left out, all other rows of the caches stay as they are.  Two
  * rows of one call must not fall on the same row of a cache (refused where strides or addresses alone say that they do).  Does not block, allocates nothing, may be captured. */
 int qmk_write_cache_packed(const qmk_packed_cache *cache, const qmk_packed_rows *rows, cudaStream_t stream);
-/* The values of the caches' rows, each rounded once to the type (one past the largest fp16 number to that); zeros in rows that are outside a cache or behind lens[b].  The outputs' rows
+/* The values of the caches' rows, computed in fp32 and rounded to the type (one past the largest fp16 number to that); zeros in rows that are outside a cache or behind lens[b].  The outputs' rows
  * must not share memory (refused where a stride is 0 or keys and values have one address).  Does not block,
  * allocates nothing, may be captured. */
 int qmk_read_cache_packed(const qmk_packed_cache *cache, const qmk_packed_rows *rows, cudaStream_t stream);

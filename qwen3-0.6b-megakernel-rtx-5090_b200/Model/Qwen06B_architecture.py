@@ -542,8 +542,8 @@ class BatchDecoder:
         return ParkedSequence(k, v, length, int(bits))
 
     def resume_slot(self, b: int, parked: "ParkedSequence") -> None:
-        """Rows of a parked sequence back into slot ``b``, which goes on from its position (``read_cache_packed``: each value is the fp16 number
-        nearest to what its code stands for).  ``parked`` may be used again, in other slots and decoders of the same layers too.  Blocks."""
+        """Rows of a parked sequence back into slot ``b``, which goes on from its position (``read_cache_packed``: each value is what its code
+        stands for, rounded to fp16).  ``parked`` may be used again, in other slots and decoders of the same layers too.  Blocks."""
         if not 0 <= b < self.num_sequences:
             raise ValueError("slot out of range")
         layers, length = self._base.num_layers, parked.length

@@ -4,9 +4,10 @@
 //   q . k = sum_b s_b (sum_{d in b} q_d n_d - M Q_b) + sum_b z_b Q_b,   Q_b = sum_{d in b} q_d,
 //   out_d = sum_r p_r z_{r,b(d)} + sum_r (p_r s_{r,b(d)}) n_{r,d} - M sum_r (p_r s_{r,b(d)}),
 // so codes enter the products as they are: the number n 2^-24 is the fp16 pattern n, and masking some bits of both halves of a word makes two operands.  Rows
-// of the cache are the 16 rows of an mma.sync tile, query heads its eight columns (tcgen05's 128 rows of queries are not there: a kv head has one to sixteen); a row's
-// trailer, 16 bytes,
-// is a row of an 8 x 8 tile, so ldmatrix makes the operands of the sums over centres.
+// of the cache are the 16 rows of an mma.sync tile, query heads its eight columns; a row's trailer, 16 bytes, is a row of an 8 x 8 tile, so ldmatrix makes the operands of the sums over
+// centres.  tcgen05 could have rows of the cache, or dimensions, as its M too, but takes that operand from shared or tensor memory: codes would be expanded into it, 512 bytes a row of keys
+// and values of 128 dims, by estimate 4 cycles of an SM's shared memory a row or 90 us of 96 sequences of 8192 rows, besides reading it; mma.sync takes them from the
+// registers in which they are expanded.
 //
 // Roundings: queries are taken to fp16 times a power of two (Tiles::lift).  Weights and their products with scales are carried as two fp16 numbers each, because the tensor cores multiply
 // 16-bit numbers: over many outputs the error against 64 bits is 1.00 to 1.01 times that of rounding the exact result (1.06 to 1.36 times with one number a product, which took 16 of up to 2048
@@ -19,9 +20,10 @@
 // each warp takes an equal stretch, whatever the sequences' lengths; a stretch that holds a whole item writes its output, parts of items leave their states in the workspace,
 // and a second launch joins them.  Of few long items each is shared by many clusters of attend_items, which leave a state each.
 //
-// Measured, caches cold: 96 sequences of 8192 rows, two heads on each of eight kv heads, 4 bits: 160 to 164 us in all, 6.2 TB/s, 0.95 of the copy rate; bound by HBM, with 250 warp
-// instructions for 16 rows.  32 of 8192 rows (336 MB), us of attend_tiles alone with 2 / 4 / 8 / 16 query heads a kv head: 63 / 69 / 76 / 114: bound by the issue of
-// instructions from 4 on (55 %, four or three warps a scheduler, waits for the ALU and fixed latencies), by 255 registers and two warps a scheduler with 16.  The joins: 4 to 6 us.
+// Measured in a graph, caches cold: 96 sequences of 8192 rows, two heads on each of eight kv heads, 4 bits: 175 us, 5.75 TB/s, 0.88 of the copy rate, with 263 warp
+// instructions for 16 rows: HBM and the issue of instructions.  32 of 8192 rows (336 MB) with 2 / 4 / 8 / 16 query heads a kv head: 66 / 75 / 88 / 153, attend_tiles alone under the
+// profiler 67 / 77 / 87 / 151: instructions from 4 on (263 / 292 / 328 / 475 for 16 rows, issued in 54 / 52 / 52 / 43 % of the cycles; four or three warps a scheduler, waits for the ALU
+// and fixed latencies), with 16 also 255 registers and two warps a scheduler.  The joins: 4 to 6 us.
 #ifndef QMK_PACKED_ATTENTION_CUH_
 #define QMK_PACKED_ATTENTION_CUH_
 
@@ -35,8 +37,9 @@ constexpr int WARPS = 4, SMS = 148;
 // How a tile is taken: by one or two query heads (PAIR), three or four (QUAD), blocks of up to eight (ONE, TWO)
 enum Way { PAIR, QUAD, ONE, TWO };
 __host__ __device__ constexpr Way way_of(int group) { return group <= 2 ? PAIR : group <= 4 ? QUAD : group <= 8 ? ONE : TWO; }
-// CTAs on an SM: four where 128 registers do and a tile has at most 5 KB, three of 168, or two of 255.  Four against three, us: 96 sequences of 8192 rows 160 and 164 (PAIR), 128 of up
-// to 256 14.7 and 17.7; ONE with 128 dims spills in 128 registers: 64 sequences of up to 4096 rows, eight heads a kv head, 35.0 and 32.5.
+// CTAs on an SM: four where 128 registers do and a tile has at most 5 KB, three of 168, or two of 255.  Four against three, us: 96 sequences of 8192 rows 173 and 178 (PAIR), 128 of up
+// to 256 16.5 and 19.9; four heads a kv head (QUAD), 64 of up to 512 rows 14.5 and 17.7, one of 32,768 18.5 and 19.3, 64 of up to 4096 49.2 and 46.7; ONE with 128 dims spills in 128
+// registers: 64 of up to 4096, eight heads a kv head, 42.0 and 36.2.
 __host__ __device__ constexpr int ctas_per_sm(Way way, int dim, int bits) { return way == TWO ? 2 : bits * dim <= 512 && (way != ONE || dim == 64) ? 4 : 3; }
 // (228 KB an SM; of a CTA 1 KB is the system's, 1.25 KB the line's)
 constexpr int warp_bytes(int ctas) { return (228 * 1024 - ctas * 2304) / (ctas * WARPS); }
@@ -275,8 +278,8 @@ struct Tiles {
       for (int i = 0; i < N; ++i) { w[0][i] = both[i]; w[1][i] = both[N + i]; }
     }
   }
-  // The power of two that queries of which the largest is `top` are multiplied with: to at most 2^TOP, so that M times the sum over a quarter stays in fp16; entries lose
-  // bits from 2^-26 of the largest on.
+  // The power of two that queries of which the largest is `top` are multiplied with: to at most 2^TOP, so that M times the sum over a quarter stays in fp16.  An entry
+  // is off by 2^-25 of the largest at most: those below about 2^-14 of it may lose bits.
   static constexpr int TOP = BITS == 4 ? 5 : 1;
   static __device__ __forceinline__ int lift(float top) {
     const int e = static_cast<int>(__float_as_uint(top) >> 23) - 126;      // top < 2^e

@@ -235,8 +235,8 @@ __device__ __forceinline__ void load_values(const void *src, int t, uint32_t (&x
   }
 }
 
-// Keys by the blocks of blockIdx.y 0, values by the others.  4 x 4096 rows of 8 heads of 128, 4 bits: 20.6 us, 88 MB, 4.3 TB/s; bound by the instructions of the codes (215 of a warp for 8
-// rows, 67 % of the issue rate) and the loads in front of them; the next rows asked for before these are packed (80 registers, three CTAs an SM): 24.2.
+// Keys by the blocks of blockIdx.y 0, values by the others.  4 x 4096 rows of 8 heads of 128, 4 bits: 21.3 us, 88 MB, 4.1 TB/s (8 bits 22.1, bf16 22.6; 8 x 4096 of 64 dims 30.4); bound by the instructions of
+// the codes (445 of a warp for 8 rows, 68 % of the issue rate) and the loads in front of them; the next rows asked for before these are packed (80 registers, three CTAs an SM): 3.6 us more.
 template <typename T, int DIM, int BITS>
 __global__ void __launch_bounds__(THREADS, 4) write_rows(const __grid_constant__ RowParams p, unsigned int count) {
   const int lane = threadIdx.x & 31, t = lane & 3;

@@ -112,7 +112,7 @@ int rows_call(const char *who, const qmk_packed_cache *cache, const qmk_packed_r
   if (const char *why = write ? shared_rows(p.caches) : shared_rows(p)) return refuse(who, why);
   p.by_rows.set(p.rows);
   p.by_heads.set(p.caches.kv_heads);
-  // (CTAs: 4 x 4096 rows of 8 heads written by four an SM for keys and four for values 20.6 us, by eight 20.8, by sixteen 21.9; 28 x 4096 read by 64 an SM 104, by sixteen 109, by eight 124)
+  // (CTAs: 4 x 4096 rows of 8 heads written by four an SM for keys and four for values 20.9 us, by eight 21.1, by sixteen 22.2; 28 x 4096 read by 64 an SM 104, by sixteen 108, by eight 123)
   const unsigned int rows_of_block = THREADS / (write ? 4 : 8), blocks = std::min((count + rows_of_block - 1) / rows_of_block, 148u * (write ? 4 : 64));
   void (*const kernel)(RowParams, unsigned int) = rows->type == 0 ? row_kernel<__half>(write, cache->head_dim, cache->bits) : row_kernel<__nv_bfloat16>(write, cache->head_dim, cache->bits);
   kernel<<<dim3(blocks, write ? 2 : 1), THREADS, 0, stream>>>(p, count);
@@ -123,11 +123,13 @@ int rows_call(const char *who, const qmk_packed_cache *cache, const qmk_packed_r
 // as are resident together.  Else, of few sequences, as many clusters of two CTAs as are resident together share the items, and a second launch joins what they have
 // joined; of more sequences a warp takes a stretch of the line of tiles, all resident together, not more of them than there can be tiles, and a second launch joins.
 // Measured in a graph, us, 128 dims, 4 bits, 16 query heads on 8, lengths from 0 up (tiles a warp in brackets).  Stretches against a cluster an item: one sequence of 128 rows
-// 6.0 and 4.7; 16 of up to 2048 (4) 14.0 and 12.1; 128 of up to 1024 (8, seven CTAs an SM one after the other) 30.4 and 27.3; 16 of up to 4096 (8) 18.2 and 17.4, of up to 8192
-// (16) 25.4 and 27.5 (a cluster has a longest item to wait for, a stretch has not); one of 8192 (8) 12.0 and 9.7, of 32,768 (32) 19.8 and 27.2.  On the host 16 and 11.
-// Clusters of 16 CTAs start late: one sequence of 2048 rows 15.5, of eight 5.7.  Stretches against pairs that share: one sequence of 16,384 rows 15.5 and 12.8, of 32,768 19.0
-// and 16.1 (16 query heads on 2 21.6 and 18.8), of 131,072 38.0 and 34.8; four of up to 16,384 18.5 and 16.7, all full 23.5 and 22.0; eight of up to 32,768 38 and 44.
-// Sharing by single CTAs 17.6 where pairs take 16.4, by four or eight 19.5; one of 8192 by pairs 11.2, by one cluster of eight 10.6.
+// 6.2 and 5.1; 16 of up to 2048 (4) 15.1 and 13.7; 128 of up to 1024 (8, seven CTAs an SM one after the other) 32.0 and 30.2; 16 of up to 4096 (8) 19.0 and 19.5, of up to 8192
+// (16) 26.3 and 30.1 (a cluster has a longest item to wait for, a stretch has not); one of 8192 (8) 13.3 and 11.7, of 32,768 (32) 20.4 and 29.5.  On the host 16 and 11.
+// Clusters of 16 CTAs start late: one sequence of 2048 rows 15.5, of eight 6.2.  Stretches against pairs that share: one sequence of 16,384 rows 16.5 and 13.7, of 32,768 20.4
+// and 17.4 (16 query heads on 2 21.3 and 16.5), of 131,072 40.4 and 36.0; four of up to 16,384 19.7 and 18.0, all full 25.3 and 24.0; eight of up to 32,768 42 and 50.
+// Sharing by single CTAs 18.4 where pairs take 17.4, by four or eight 21.0; one of 8192 by pairs or by one cluster of eight 11.7.
+// The rule sees how long the caches may be, and so does that of the join; lengths are on the device.  Of 128 caches of 8192 rows one full and the others empty takes 77 us, most of
+// them join_few's (one warp a head for some 256 parts), where that sequence in a call of its own takes 11.7; one of 32,768 beside 127 of 200 68.
 constexpr int ITEM_TILES = 8, ITEM_WAVES = 4;
 constexpr int SHARING_SEQS = 4, SHARING_PAIRS = 8;                          // sequences at most, pairs of an item at least (fewer leave many places of the device empty)
 struct Cut {
