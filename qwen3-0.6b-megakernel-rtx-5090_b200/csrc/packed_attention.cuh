@@ -3,14 +3,14 @@
 // With n the codes, M = 2^(BITS - 1), b(d) the quarter of dimension d, s and z a row's scales and centres:
 //   q . k = sum_b s_b (sum_{d in b} q_d n_d - M Q_b) + sum_b z_b Q_b,   Q_b = sum_{d in b} q_d,
 //   out_d = sum_r p_r z_{r,b(d)} + sum_r (p_r s_{r,b(d)}) n_{r,d} - M sum_r (p_r s_{r,b(d)}),
-// so codes enter the products as they are: the number n 2^-24 is the fp16 pattern n, and masking some bits of both halves of a word makes two operands.  Rows
+// so codes enter the products as they are: the number n 2^-24 is the fp16 pattern n (of 4 bits 16 n, 2^-20 each), and masking some bits of both halves of a word makes two operands.  Rows
 // of the cache are the 16 rows of an mma.sync tile, query heads its eight columns; a row's trailer, 16 bytes, is a row of an 8 x 8 tile, so ldmatrix makes the operands of the sums over
 // centres.  tcgen05 could have rows of the cache, or dimensions, as its M too, but takes that operand from shared or tensor memory: codes would be expanded into it, 512 bytes a row of keys
 // and values of 128 dims, by estimate 4 cycles of an SM's shared memory a row or 90 us of 96 sequences of 8192 rows, besides reading it; mma.sync takes them from the
 // registers in which they are expanded.
 //
 // Roundings: queries are taken to fp16 times a power of two (Tiles::lift).  Weights and their products with scales are carried as two fp16 numbers each, because the tensor cores multiply
-// 16-bit numbers: over many outputs the error against 64 bits is 1.00 to 1.01 times that of rounding the exact result (1.06 to 1.36 times with one number a product, which took 16 of up to 2048
+// 16-bit numbers: over many outputs the error against 64 bits is that of rounding the exact result (1.06 to 1.36 times with one number a product, which took 16 of up to 2048
 // rows 12.8 us, 128 of up to 8192 122, 96 of 8192 160 and 32 of up to 4096 with sixteen heads a kv head 23.5, where two take 13.6, 125, 175 and 27.9).  So for bf16 outputs: with one number each
 // an output whose terms cancel is off by up to 2^-10 of these.  Sums, softmax statistics and outputs are fp32.  Every second 16 rows go in as 2^BITS - 1 - n with the
 // weights' sign turned (the same instructions): the running sums stay around zero, whose size the accumulator's truncation goes by.
@@ -48,9 +48,9 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // the largest.
 constexpr float SHIFT = 7.0f, SLACK = 8.0f;
 constexpr float NOTHING = -3.0e38f;              // the maximum while no score has been seen: the first one rises (times 2^-120 it is -256 below), -inf stays that
-// The largest factor (scores are below 2^7 in their units, so products stay finite).  One that is cut to it makes the same weights: scores that differ do so by 2^-72 at least, and
-// that times 2^120 leaves the largest alone.
-constexpr float MOST = 0x1p120f;
+// The largest factor (scores are below 2^12 in their units, so products stay finite).  One that is cut to it makes the same weights: scores that differ do so by 2^-72 at least, and
+// that times 2^112 leaves the largest alone.
+constexpr float MOST = 0x1p112f;
 
 struct AttendParams {
   Caches caches;
@@ -109,20 +109,27 @@ template <bool TRANSPOSED, int ROW> __device__ __forceinline__ void trailers(uin
   }
 }
 
-// Codes of quarter b of two chunks (DIM/8 codes each), the first in the lower halves: x[j] = (a_j, b_j) as fp16 numbers of 2^-24, of 4-bit codes every second of
-// 2^-20; FLIP: 2^BITS - 1 less the code.
+// (as a multiplication, whose pipe has room where that of shifts and masks has not: 128 sequences of up to 8192 rows 133.2 us, by a shift 135.0)
+__device__ __forceinline__ uint32_t times16(uint32_t x) {
+  uint32_t y;
+  asm("mad.lo.u32 %0, %1, %2, 0;" : "=r"(y) : "r"(x), "r"(16u));
+  return y;
+}
+// Codes of quarter b of two chunks (DIM/8 codes each), the first in the lower halves: x[j] = (a_j, b_j) as fp16 numbers of UNIT (2^-24; 4-bit codes of 2^-20); FLIP:
+// 2^BITS - 1 less the code.  These numbers have fp16's smallest exponent, by which the tensor cores line products up: codes of 4 bits in the lowest places would keep four bits less
+// of them, so that sums of a few rows were off by up to 2^-17 of their terms, scores by 2^-20.
 template <int DIM, int BITS, bool FLIP = false>
 __device__ __forceinline__ void expand(const uint32_t (&a)[DIM * BITS / 256], const uint32_t (&c)[DIM * BITS / 256], int b, uint32_t (&x)[DIM / 32]) {
   constexpr uint32_t ALL = FLIP ? 0xffffffffu : 0u;
   if constexpr (BITS == 4 && DIM == 64) {
     const uint32_t w = __byte_perm(a[0], c[0], b | b << 4 | (4 + b) << 8 | (4 + b) << 12);
-    x[0] = (w ^ ALL) & 0x000f000fu;
+    x[0] = (times16(w) ^ ALL) & 0x00f000f0u;
     x[1] = (w ^ ALL) & 0x00f000f0u;
   } else if constexpr (BITS == 4) {
     const uint32_t w = __byte_perm(a[b / 2], c[b / 2], b % 2 ? 0x7632 : 0x5410), u = w >> 8;
-    x[0] = (w ^ ALL) & 0x000f000fu;
+    x[0] = (times16(w) ^ ALL) & 0x00f000f0u;
     x[1] = (w ^ ALL) & 0x00f000f0u;
-    x[2] = (u ^ ALL) & 0x000f000fu;
+    x[2] = (times16(u) ^ ALL) & 0x00f000f0u;
     x[3] = (u ^ ALL) & 0x00f000f0u;
   } else if constexpr (DIM == 64) {
     const uint32_t w = __byte_perm(a[b / 2], c[b / 2], b % 2 ? 0x7632 : 0x5410), u = w >> 8;
@@ -234,7 +241,7 @@ struct Tiles {
   static constexpr int QUERIES = STAGES * STAGE + HEADS * DIM * 2 <= warp_bytes(CTAS) ? HEADS * DIM * 2 : 0;
   static constexpr int QUERY_STRIDE = DIM, WARP_SMEM = STAGES * STAGE + QUERIES, SMEM = WARPS * WARP_SMEM;
   static_assert(STAGES * STAGE >= HEADS * (DIM * 4 + 8), "a warp's state fits its ring");
-  static constexpr float M = 1 << (BITS - 1), UNIT = 0x1p-24f;
+  static constexpr float M = 1 << (BITS - 1), UNIT = BITS == 4 ? 0x1p-20f : 0x1p-24f;
   // What the codes (the flipped ones) are above the numbers they stand for, negative, as pairs of fp16 numbers
   static constexpr uint32_t MIDDLE = BITS == 4 ? 0xc800c800u : 0xd800d800u, MIDDLE_FLIPPED = BITS == 4 ? 0xc700c700u : 0xd7f0d7f0u;         // -8, -128; -7, -127
   static constexpr bool SPREAD = BITS == 8 && DIM == 128;                                   // a lane's two chunks of keys: four apart, or one behind the other
@@ -402,8 +409,7 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
 #pragma unroll
     for (int i = 0; i < 2 * KSTEPS; ++i) {
       const int c = i / KSTEPS, low = i % KSTEPS / PAIRS * (2 * PAIRS) + i % PAIRS, high = low + PAIRS;
-      const float unit = BITS == 4 && i % 2 ? 0.0625f : 1.0f;
-      qb[i / 2][i % 2] = pack2(quarter == low / J ? x[c][low % J] * unit : 0.0f, quarter == high / J ? x[c][high % J] * unit : 0.0f);
+      qb[i / 2][i % 2] = pack2(quarter == low / J ? x[c][low % J] : 0.0f, quarter == high / J ? x[c][high % J] : 0.0f);
     }
     const float coefficient = t < 2 ? -M * sum : sum;
     const bool even = quarter == (2 * t & 3), odd = quarter == (2 * t & 3) + 1;
@@ -440,9 +446,9 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
       for (int r = 0; r < 2; ++r) {
         const uint32_t word = w[r][i / N][i % N];
         if constexpr (BITS == 4) {
-          x[r][0] = word & 0x000f000fu;
+          x[r][0] = times16(word) & 0x00f000f0u;
           x[r][1] = word & 0x00f000f0u;
-          x[r][PAIRS - 2] = word >> 8 & 0x000f000fu;
+          x[r][PAIRS - 2] = times16(word >> 8) & 0x00f000f0u;
           x[r][PAIRS - 1] = word >> 8 & 0x00f000f0u;
         } else {
           x[r][0] = word & 0x00ff00ffu;
@@ -556,7 +562,7 @@ struct AttendPair : Tiles<DIM, BITS, PAIR, 2> {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         const float c = t & 1 ? acc[2 + e][j / 2][e + 2 * (j % 2)] : acc[e][j / 2][e + 2 * (j % 2)];
-        v[j] = fmaf(fmaf(c, (BITS == 4 && j % 2 ? 0.0625f : 1.0f) / UNIT, sums[e]), inverse, z);
+        v[j] = fmaf(fmaf(c, 1.0f / UNIT, sums[e]), inverse, z);
       }
       if (!live) continue;
       if (state) store_part<DIM>(state + h * DIM + DIM / 4 * i + J * g, v);
@@ -613,9 +619,8 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
       sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
 #pragma unroll
       for (int u = 0; u < STEPS; ++u) {
-        constexpr float ODD = BITS == 4 ? 0.0625f : 1.0f;
         qb[i][u][0] = pack2(x[i][0][2 * u], x[i][1][2 * u]);
-        qb[i][u][1] = pack2(x[i][0][2 * u + 1] * ODD, x[i][1][2 * u + 1] * ODD);
+        qb[i][u][1] = pack2(x[i][0][2 * u + 1], x[i][1][2 * u + 1]);
       }
     }
     // a trailer's entries 2 t and 2 t + 1: scales (t < 2) or centres of half t & 1
@@ -770,7 +775,7 @@ struct AttendQuad : Tiles<DIM, BITS, QUAD, 4> {
       float v[J];
 #pragma unroll
       for (int j = 0; j < J; ++j)
-        v[j] = fmaf(fmaf(acc[i][j / 2][i / 2 + 2 * (j % 2)], (BITS == 4 && j % 2 ? 0.0625f : 1.0f) / UNIT, sums[i % 2][i / 2]), inverse, z);
+        v[j] = fmaf(fmaf(acc[i][j / 2][i / 2 + 2 * (j % 2)], 1.0f / UNIT, sums[i % 2][i / 2]), inverse, z);
       if (!live) continue;
       if (state) store_part<DIM>(state + h * DIM + DIM / 4 * i + J * g, v);
       else store_out<T, DIM>(static_cast<T *>(p.out) + row * DIM + DIM / 4 * i + J * g, v, by);
@@ -827,7 +832,7 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
 #pragma unroll
         for (int u = 0; u < STEPS; ++u) {
           qb[nt][i][u][0] = pack2(x[i][2 * u], x[i][J + 2 * u]);
-          qb[nt][i][u][1] = pack2(x[i][2 * u + 1] * (BITS == 4 ? 0.0625f : 1.0f), x[i][J + 2 * u + 1] * (BITS == 4 ? 0.0625f : 1.0f));
+          qb[nt][i][u][1] = pack2(x[i][2 * u + 1], x[i][J + 2 * u + 1]);
         }
       }
       // heads 2 t and 2 t + 1: lanes 8 t and 8 t + 4
@@ -1079,7 +1084,7 @@ struct Attend : Tiles<DIM, BITS, NT == 1 ? ONE : TWO, 8 * NT> {
           float v[J];
 #pragma unroll
           for (int j = 0; j < J; ++j)
-            v[j] = fmaf(fmaf(acc[nt][i][j / 2][e + 2 * (j % 2)], (BITS == 4 && j % 2 ? 0.0625f : 1.0f) / UNIT, sums[nt][i][e]), inverse[i], z);
+            v[j] = fmaf(fmaf(acc[nt][i][j / 2][e + 2 * (j % 2)], 1.0f / UNIT, sums[nt][i][e]), inverse[i], z);
           if (h >= p.group) continue;
           if (state) store_part<DIM>(state + h * DIM + DIM / 4 * i + J * g, v);
           else store_out<T, DIM>(static_cast<T *>(p.out) + row * DIM + DIM / 4 * i + J * g, v, by);

@@ -1046,3 +1046,19 @@ def test_outputs_whose_terms_cancel(gpu, dim, bits, q_heads, room, dtype):
     tol = torch.finfo(q.dtype).eps / 2 * want.abs() + 2.0 ** -18 * a + u * (2 * ds + 2 * (rows / 16 + 2) * 2.0 ** -23 + 2.0 ** -21)
     err = (out.double().cpu() - want).abs()
     assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("dim,bits", [(64, 4), (64, 8), (128, 4), (128, 8)])
+@pytest.mark.parametrize("q_heads", [4, 8, 16, 32])
+def test_scores_are_sums_of_32_bits(gpu, dim, bits, q_heads, dtype):
+    """One row: the logarithm is its score.  S the sum of |q| (|z| + s 2^bits) times scale, of which the running sums are less than half: four groups of products and the sum over centres,
+    each cut off at 2^-24 of its running sum or rounded, come to no more than the 2^-24 S that a rounding of S would."""
+    q, kc, vc = attention_inputs(60, q_heads, 2, dim, bits, 1, dtype, seed=q_heads)
+    _, lse = gpu.attention_packed_cache(q, kc, vc, torch.ones(60, dtype=torch.int32).cuda())
+    z, s, n = (x.repeat_interleave(q_heads // 2, 1)[:, :, 0] for x in parts(kc, dim))
+    qd = q.double().cpu()
+    want, size = (torch.einsum("bhd,bhd->bh", a, b) * dim ** -0.5 for a, b in ((qd, z + s * n), (qd.abs(), z.abs() + s * 2 ** bits)))
+    err = (lse.double().cpu() - want).abs() / size
+    assert float(err.max()) <= 2.0 ** -24, math.log2(float(err.max()))
