@@ -6,12 +6,12 @@
 // so codes enter the products as they are: the number n 2^-24 is the fp16 pattern n (of 4 bits 16 n, 2^-20 each), and masking some bits of both halves of a word makes two operands.  Rows
 // of the cache are the 16 rows of an mma.sync tile, query heads its eight columns; a row's trailer, 16 bytes, is a row of an 8 x 8 tile, so ldmatrix makes the operands of the sums over
 // centres.  tcgen05 could have rows of the cache, or dimensions, as its M too, but takes that operand from shared or tensor memory: codes would be expanded into it, 512 bytes a row of keys
-// and values of 128 dims, by estimate 4 cycles of an SM's shared memory a row or 90 us of 96 sequences of 8192 rows, besides reading it; mma.sync takes them from the
+// and values of 128 dims, by estimate 4 cycles of an SM's shared memory a row or 90 us of the 187 of 96 sequences of 8192 rows, besides reading it; mma.sync takes them from the
 // registers in which they are expanded.
 //
 // Roundings: queries are taken to fp16 times a power of two (Tiles::lift).  Weights and their products with scales are carried as two fp16 numbers each, because the tensor cores multiply
 // 16-bit numbers: over many outputs the error against 64 bits is that of rounding the exact result (1.06 to 1.36 times with one number a product, which took 16 of up to 2048
-// rows 12.8 us, 128 of up to 8192 122, 96 of 8192 160 and 32 of up to 4096 with sixteen heads a kv head 23.5, where two take 13.6, 125, 175 and 27.9).  So for bf16 outputs: with one number each
+// rows 12.8 us, 128 of up to 8192 122, 96 of 8192 160 and 32 of up to 4096 with sixteen heads a kv head 23.5, where two took 13.6, 125, 175 and 27.9).  So for bf16 outputs: with one number each
 // an output whose terms cancel is off by up to 2^-10 of these.  Sums, softmax statistics and outputs are fp32.  Every second 16 rows go in as 2^BITS - 1 - n with the
 // weights' sign turned (the same instructions): the running sums stay around zero, whose size the accumulator's truncation goes by.
 //
@@ -20,10 +20,10 @@
 // each warp takes an equal stretch, whatever the sequences' lengths; a stretch that holds a whole item writes its output, parts of items leave their states in the workspace,
 // and a second launch joins them.  Of few long items each is shared by many clusters of attend_items, which leave a state each.
 //
-// Measured in a graph, caches cold: 96 sequences of 8192 rows, two heads on each of eight kv heads, 4 bits: 175 us, 5.75 TB/s, 0.88 of the copy rate, with 263 warp
-// instructions for 16 rows: HBM and the issue of instructions.  32 of 8192 rows (336 MB) with 2 / 4 / 8 / 16 query heads a kv head: 66 / 75 / 88 / 153, attend_tiles alone under the
-// profiler 67 / 77 / 87 / 151: instructions from 4 on (263 / 292 / 328 / 475 for 16 rows, issued in 54 / 52 / 52 / 43 % of the cycles; four or three warps a scheduler, waits for the ALU
-// and fixed latencies), with 16 also 255 registers and two warps a scheduler.  The joins: 4 to 6 us.
+// Measured in a graph, caches cold: 96 sequences of 8192 rows, two heads on each of eight kv heads, 4 bits: 187 us, 5.4 TB/s, 0.82 of the copy rate, with 291 warp
+// instructions for 16 rows: HBM and the issue of instructions; 64 of up to 4096 in 8 bits 57, 0.82.  32 of 8192 rows (336 MB) with 2 / 4 / 8 / 16 query heads a kv head: 70 / 78 / 93 / 161,
+// attend_tiles alone under the profiler 72 / 81 / 93 / 160: instructions (291 / 321 / 359 / 509 for 16 rows, issued in 56 / 54 / 53 / 44 % of the cycles; four or three warps a scheduler,
+// waits for the ALU and fixed latencies), with 16 also 255 registers and two warps a scheduler.  The joins: 4 to 6 us.
 #ifndef QMK_PACKED_ATTENTION_CUH_
 #define QMK_PACKED_ATTENTION_CUH_
 
@@ -37,9 +37,9 @@ constexpr int WARPS = 4, SMS = 148;
 // How a tile is taken: by one or two query heads (PAIR), three or four (QUAD), blocks of up to eight (ONE, TWO)
 enum Way { PAIR, QUAD, ONE, TWO };
 __host__ __device__ constexpr Way way_of(int group) { return group <= 2 ? PAIR : group <= 4 ? QUAD : group <= 8 ? ONE : TWO; }
-// CTAs on an SM: four where 128 registers do and a tile has at most 5 KB, three of 168, or two of 255.  Four against three, us: 96 sequences of 8192 rows 173 and 178 (PAIR), 128 of up
-// to 256 16.5 and 19.9; four heads a kv head (QUAD), 64 of up to 512 rows 14.5 and 17.7, one of 32,768 18.5 and 19.3, 64 of up to 4096 49.2 and 46.7; ONE with 128 dims spills in 128
-// registers: 64 of up to 4096, eight heads a kv head, 42.0 and 36.2.
+// CTAs on an SM: four where 128 registers do and a tile has at most 5 KB, three of 168, or two of 255.  Four against three, us: 96 sequences of 8192 rows 187 and 188 (PAIR), 128 of up
+// to 256 17.4 and 20.8; four heads a kv head (QUAD), 64 of up to 512 rows 15.1 and 18.5, one of 32,768 19.3 and 19.9, 64 of up to 4096 51.2 and 48.4; ONE with 128 dims spills in 128
+// registers: 64 of up to 4096, eight heads a kv head, 43.4 and 37.6.
 __host__ __device__ constexpr int ctas_per_sm(Way way, int dim, int bits) { return way == TWO ? 2 : bits * dim <= 512 && (way != ONE || dim == 64) ? 4 : 3; }
 // (228 KB an SM; of a CTA 1 KB is the system's, 1.25 KB the line's)
 constexpr int warp_bytes(int ctas) { return (228 * 1024 - ctas * 2304) / (ctas * WARPS); }

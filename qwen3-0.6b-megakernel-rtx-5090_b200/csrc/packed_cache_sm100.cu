@@ -123,13 +123,13 @@ int rows_call(const char *who, const qmk_packed_cache *cache, const qmk_packed_r
 // as are resident together.  Else, of few sequences, as many clusters of two CTAs as are resident together share the items, and a second launch joins what they have
 // joined; of more sequences a warp takes a stretch of the line of tiles, all resident together, not more of them than there can be tiles, and a second launch joins.
 // Measured in a graph, us, 128 dims, 4 bits, 16 query heads on 8, lengths from 0 up (tiles a warp in brackets).  Stretches against a cluster an item: one sequence of 128 rows
-// 6.2 and 5.1; 16 of up to 2048 (4) 15.1 and 13.7; 128 of up to 1024 (8, seven CTAs an SM one after the other) 32.0 and 30.2; 16 of up to 4096 (8) 19.0 and 19.5, of up to 8192
-// (16) 26.3 and 30.1 (a cluster has a longest item to wait for, a stretch has not); one of 8192 (8) 13.3 and 11.7, of 32,768 (32) 20.4 and 29.5.  On the host 16 and 11.
-// Clusters of 16 CTAs start late: one sequence of 2048 rows 15.5, of eight 6.2.  Stretches against pairs that share: one sequence of 16,384 rows 16.5 and 13.7, of 32,768 20.4
-// and 17.4 (16 query heads on 2 21.3 and 16.5), of 131,072 40.4 and 36.0; four of up to 16,384 19.7 and 18.0, all full 25.3 and 24.0; eight of up to 32,768 42 and 50.
-// Sharing by single CTAs 18.4 where pairs take 17.4, by four or eight 21.0; one of 8192 by pairs or by one cluster of eight 11.7.
+// 6.3 and 5.3; 16 of up to 2048 (4) 15.4 and 14.0; 128 of up to 1024 (8, seven CTAs an SM one after the other) 32.7 and 31.8; 16 of up to 4096 (8) 19.6 and 20.1, of up to 8192
+// (16) 27.4 and 31.4 (a cluster has a longest item to wait for, a stretch has not); one of 8192 (8) 13.5 and 12.0, of 32,768 (32) 21.0 and 30.8.  On the host 16 and 11.
+// Clusters of 16 CTAs start late: one sequence of 2048 rows 15.5, of eight 6.5.  Stretches against pairs that share: one sequence of 16,384 rows 16.7 and 14.0, of 32,768 21.0
+// and 17.9 (16 query heads on 2 21.5 and 16.7), of 131,072 42.5 and 37.5; four of up to 16,384 20.2 and 18.7, all full 26.2 and 24.8; eight of up to 32,768 44 and 54.
+// Sharing by single CTAs 19.0 where pairs take 17.9, by four or eight 22; one of 8192 by pairs or by one cluster of eight 12.0.
 // The rule sees how long the caches may be, and so does that of the join; lengths are on the device.  Of 128 caches of 8192 rows one full and the others empty takes 77 us, most of
-// them join_few's (one warp a head for some 256 parts), where that sequence in a call of its own takes 11.7; one of 32,768 beside 127 of 200 68.
+// them join_few's (one warp a head for some 256 parts), where that sequence in a call of its own takes 12; one of 32,768 beside 127 of 200 68.
 constexpr int ITEM_TILES = 8, ITEM_WAVES = 4;
 constexpr int SHARING_SEQS = 4, SHARING_PAIRS = 8;                          // sequences at most, pairs of an item at least (fewer leave many places of the device empty)
 struct Cut {
